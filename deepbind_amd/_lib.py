@@ -18,7 +18,7 @@ class DeepbindError(RuntimeError):
     """Raised when a library call reports a failure (counterpart of the reference's SmatException)."""
 
 
-DBK_F32, DBK_F64 = 0, 1
+DBK_F32, DBK_F64, DBK_BF16 = 0, 1, 2
 PT_MAX, PT_AVG, PT_SUM, PT_ALL = 0, 1, 2, 3
 str2pooltype = {"max": PT_MAX, "avg": PT_AVG, "sum": PT_SUM, "all": PT_ALL}
 # loss_kind of dbk_head_train / dbk_train_step*: output non-linearity + loss (reference: deepity/std/loss.py:131-174)
@@ -98,6 +98,18 @@ _SIGNATURES = {
     "dbk_gradient_map_takes": [_Z, _Z, _Z, _Z, _I, _Z],
     "dbk_gradient_map": [_P, _P, _P, _Z, _Z, _P, _P, _Z, _Z, _Z, _I, _Z, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P],
     "dbk_gather_maps": [_P, _I, _P, _Z, _Z, _I, _P, _P, _P],
+    "dbk_layernorm": [_P, _I, _P, _Z, _P, _P, _Z, _Z, _Z, _D, _P, _Z, _P],
+    "dbk_layernorm_bprop_workspace": [_I, _Z, _Z, _Z, _P],
+    "dbk_layernorm_bprop": [_P, _I, _P, _Z, _P, _P, _P, _Z, _Z, _Z, _Z, _P, _Z, _P, _P, _P, _Z],
+    "dbk_causalconv_workspace": [_I, _Z, _Z, _Z, _Z, _I, _P],
+    "dbk_causalconv": [_P, _I, _P, _Z, _P, _P, _Z, _Z, _Z, _P, _Z, _I, _P, _P, _Z, _P, _P, _Z],
+    "dbk_causalconv_bprop": [_P, _I, _P, _Z, _P, _P, _Z, _Z, _Z, _P, _Z, _I, _P, _Z, _P, _Z, _P, _P, _P, _Z],
+    "dbk_causalconv_step": [_P, _I, _P, _Z, _P, _P, _Z, _Z, _Z, _I, _P, _P, _P, _Z],
+    "dbk_statescan_args_size": [],
+    "dbk_statescan_workspace": [_P, _I, _P],
+    "dbk_statescan": [_P, _P, _P, _Z],
+    "dbk_statescan_bprop": [_P, _P, _P, _Z],
+    "dbk_statescan_step": [_P, _P],
     "dbk_train_step": [_P, _P],
     "dbk_train_steps": [_P, _Z, _P],
     "dbk_train_step_single_workspace": [_P, _P],
@@ -125,6 +137,18 @@ class TrainStepArgs(ctypes.Structure):
         ("nfeat", _Z), ("feats", _P),
         ("ycol", _P), ("ldY", _Z),
     ]
+
+
+class StateScanArgs(ctypes.Structure):
+    """dbk_statescan_args of the public header, field for field."""
+    _fields_ = [
+        ("dtype", _I), ("softplus", _I), ("N", _Z), ("D", _Z), ("S", _Z), ("G", _Z), ("regions", _P), ("nregion", _Z),
+        ("X", _P), ("ldx", _Z), ("dt", _P), ("lddt", _Z), ("A", _P), ("B", _P), ("ldb", _Z), ("C", _P), ("ldc", _Z),
+        ("skip", _P), ("dt_bias", _P), ("gate", _P), ("ldgate", _Z), ("state", _P), ("Y", _P), ("ldy", _Z), ("last", _P), ("keep", _P),
+        ("dY", _P), ("lddy", _Z), ("dX", _P), ("lddx", _Z), ("ddt", _P), ("ldddt", _Z), ("dgate", _P), ("lddgate", _Z),
+        ("dB", _P), ("lddb", _Z), ("dC", _P), ("lddc", _Z), ("dA", _P), ("dskip", _P), ("ddt_bias", _P),
+    ]
+
 
 _dll = None
 
@@ -186,6 +210,92 @@ def dtype_code(t):
     if t.dtype == torch.float64:
         return DBK_F64
     raise DeepbindError("TypeError: expected a float32 or float64 tensor, got %s" % t.dtype)
+
+
+ROW_DTYPES = {torch.float32: DBK_F32, torch.float64: DBK_F64, torch.bfloat16: DBK_BF16}
+
+
+def row_dtype_code(t):
+    """Type code of a matrix of rows of the row operators."""
+    if t.dtype not in ROW_DTYPES:
+        raise DeepbindError("TypeError: expected float32, float64 or bfloat16 rows, got %s" % t.dtype)
+    return ROW_DTYPES[t.dtype]
+
+
+def wide_dtype(t):
+    """The type of the weights, statistics and states that go with rows of t's type."""
+    return torch.float64 if t.dtype == torch.float64 else torch.float32
+
+
+def check_rows(name, t, shape, dtype):
+    """A matrix of rows: its own row stride, elements of a row next to each other."""
+    require(isinstance(t, torch.Tensor) and tuple(t.shape) == tuple(shape), "ValueError: %s must be a %s matrix, got %s" %
+            (name, tuple(shape), tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__))
+    require(t.dtype == dtype, "TypeError: %s must be %s, got %s" % (name, dtype, t.dtype))
+    rows, cols = t.shape
+    require(cols <= 1 or t.stride(1) == 1, "ValueError: the elements of a row of %s must lie next to each other" % name)
+    require(rows <= 1 or t.stride(0) >= cols, "ValueError: the rows of %s must not overlap" % name)
+
+
+def check_dense(name, t, shape, dtype):
+    """A contiguous array of weights or states; None passes."""
+    if t is None:
+        return
+    require(isinstance(t, torch.Tensor) and tuple(t.shape) == tuple(shape), "ValueError: %s must be %s, got %s" %
+            (name, tuple(shape), tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__))
+    require(t.dtype == dtype, "TypeError: %s must be %s, got %s" % (name, dtype, t.dtype))
+    require(t.is_contiguous(), "ValueError: %s must be contiguous" % name)
+
+
+def row_stride(t):
+    return t.stride(0) if t is not None and t.shape[0] > 1 else (0 if t is None else t.shape[1])
+
+
+def same_device(*tensors):
+    """Refuses tensors that are not on the current device, whose stream the call would run on."""
+    for t in tensors:
+        if t is not None:
+            require(t.is_cuda, "TypeError: expected a device tensor, got a host tensor")
+            require(t.get_device() == torch.cuda.current_device(), "ValueError: a tensor lies on device %d, the current device is %d" %
+                    (t.get_device(), torch.cuda.current_device()))
+
+
+def not_shared(outs, ins):
+    """Refuses outputs that overlap an input's memory or each other's."""
+    spans = []
+    for group, tensors in ((0, ins), (1, outs)):
+        for t in tensors:
+            if t is None or t.numel() == 0:
+                continue
+            lo = t.data_ptr()
+            hi = lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+            spans.append((lo, hi, group, t))
+    spans.sort(key=lambda s: s[0])
+    for i, (lo, hi, group, t) in enumerate(spans):
+        for lo2, hi2, group2, t2 in spans[i + 1:]:
+            if lo2 >= hi:
+                break
+            # blocks of columns of one wider matrix: their spans overlap, their elements need not
+            if (group or group2) and not _column_blocks(t, t2):
+                raise DeepbindError("ValueError: an output shares memory with another argument")
+
+
+def _column_blocks(a, b):
+    if a.dim() != 2 or b.dim() != 2 or a.stride(0) != b.stride(0) or a.element_size() != b.element_size():
+        return False
+    off = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    ld = a.stride(0)
+    return off % ld >= a.shape[1] and off % ld + b.shape[1] <= ld
+
+
+def raw(t):
+    """Device pointer of a tensor that has been checked (None -> NULL)."""
+    return None if t is None else t.data_ptr()
+
+
+def workspace(nbytes, like):
+    """Scratch of one call, from torch's allocator: its own under capture, returned to the stream's pool afterwards."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
 
 
 def require(cond, msg):

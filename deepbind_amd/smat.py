@@ -3,8 +3,11 @@ Names follow the reference's array module (reference: code/libs/smat/py/smat/sma
 operations on the motif-scan path exist here, each backed by a kernel in libdeepbind_hip.so.
 torch supplies device memory and the stream; it does no arithmetic on this path.
 """
+import ctypes
+
 import torch
 
+from . import _lib
 from ._lib import call, dtype_code, ptr, require, stream
 from . import deepity_smat as _ds
 
@@ -106,6 +109,64 @@ def softmax(X, nchunk=1):
     Z = torch.empty_like(X)
     call("dbk_softmax", stream(), dtype_code(X), ptr(X), ptr(Z), X.numel(), X.shape[1] // nchunk)
     return Z
+
+
+def _norm_args(X, gamma, beta, nchunk):
+    require(isinstance(X, torch.Tensor) and X.dim() == 2, "ValueError: X must be a matrix")
+    code, wide, (n, m) = _lib.row_dtype_code(X), _lib.wide_dtype(X), X.shape
+    require(nchunk >= 1 and m % nchunk == 0 and m >= nchunk, "ValueError: the number of columns must be divisible by nchunk")
+    _lib.check_rows("X", X, (n, m), X.dtype)
+    _lib.check_dense("gamma", gamma, (1, m), wide)
+    _lib.check_dense("beta", beta, (1, m), wide)
+    return code, wide, n, m
+
+
+def layernorm(X, gamma=None, beta=None, nchunk=1, eps=1e-5, want_stats=False, out=None):
+    """(X - mean) / sqrt(mean((X - mean)^2) + eps) * gamma + beta of every row of X (n x m), or with nchunk > 1 of every
+    one of a row's nchunk equal chunks (the models' blocks of columns, as softmax takes them). gamma, beta: (1 x m) or None.
+    X: float32, float64 or bfloat16 with a row stride of its own; weights and statistics float32 (float64 beside float64).
+    Returns (Z, stats|None); stats (2 x n*nchunk): the chunks' means and reciprocal deviations, which layernorm_bprop takes.
+    out (optional): the matrix to write into."""
+    code, wide, n, m = _norm_args(X, gamma, beta, nchunk)
+    Z = torch.empty((n, m), dtype=X.dtype, device=X.device) if out is None else out
+    _lib.check_rows("out", Z, (n, m), X.dtype)
+    _lib.same_device(X, gamma, beta, out)
+    if out is not None:
+        _lib.not_shared((out,), (X, gamma, beta))
+    stats = torch.empty((2, n * nchunk), dtype=wide, device=X.device) if want_stats else None
+    call("dbk_layernorm", stream(), code, _lib.raw(X), _lib.row_stride(X), _lib.raw(gamma), _lib.raw(beta), n, m, m // nchunk, float(eps),
+         _lib.raw(Z), _lib.row_stride(Z), _lib.raw(stats))
+    return Z, stats
+
+
+def layernorm_bprop(X, gamma, stats, dZ, nchunk=1, out=None):
+    """Gradients (dX, dgamma, dbeta) of layernorm at X with the stats of its forward call; without gamma (None) the last two are None
+    (pass ones to get them). out (optional): a tuple like the returned one of tensors to write into, None where one is to be made."""
+    code, wide, n, m = _norm_args(X, gamma, None, nchunk)
+    _lib.check_dense("stats", stats, (2, n * nchunk), wide)
+    require(stats is not None, "ValueError: the statistics of the forward call are needed")
+    _lib.check_rows("dZ", dZ, (n, m), X.dtype)
+    dX, dgamma, dbeta = (None, None, None) if out is None else out
+    _lib.same_device(X, gamma, stats, dZ, dX, dgamma, dbeta)
+    if out is not None:
+        _lib.not_shared((dX, dgamma, dbeta), (X, gamma, stats, dZ))
+    if dX is None:
+        dX = torch.empty((n, m), dtype=X.dtype, device=X.device)
+    _lib.check_rows("dX", dX, (n, m), X.dtype)
+    if gamma is None:
+        require(dgamma is None and dbeta is None, "ValueError: no weights, no gradient of them")
+    else:
+        dgamma = torch.empty_like(gamma) if dgamma is None else dgamma
+        dbeta = torch.empty_like(gamma) if dbeta is None else dbeta
+        _lib.check_dense("dgamma", dgamma, (1, m), wide)
+        _lib.check_dense("dbeta", dbeta, (1, m), wide)
+    need = ctypes.c_size_t(0)
+    if gamma is not None:
+        call("dbk_layernorm_bprop_workspace", code, n, m, m // nchunk, ctypes.addressof(need))
+    work = _lib.workspace(need.value, X)
+    call("dbk_layernorm_bprop", stream(), code, _lib.raw(X), _lib.row_stride(X), _lib.raw(gamma), _lib.raw(stats), _lib.raw(dZ), _lib.row_stride(dZ),
+         n, m, m // nchunk, _lib.raw(dX), _lib.row_stride(dX), _lib.raw(dgamma), _lib.raw(dbeta), _lib.raw(work), need.value)
+    return dX, dgamma, dbeta
 
 
 def loss_terms(Z, Y, kind):

@@ -29,6 +29,9 @@ typedef void* dbk_stream_t;                 /* hipStream_t */
 
 /* reference: smat/src/smat/dtypes.h (dtype_t); only the two float types reach these ops */
 enum { DBK_F32 = 0, DBK_F64 = 1 };
+/* a third row type of the row operators (layer norm, causal convolution, state scan): bfloat16 maps with float32 weights,
+ * statistics and states. No counterpart in the reference. */
+enum { DBK_BF16 = 2 };
 
 /* reference: kangaroo/kangaroo_smat/kangaroo_smat.h:42-47 (pooltype_t) */
 enum { DBK_PT_MAX = 0, DBK_PT_AVG = 1, DBK_PT_SUM = 2, DBK_PT_ALL = 3 };
@@ -467,6 +470,71 @@ int dbk_gradient_map(dbk_stream_t stream, const float* W, const float* bias, siz
  * the pair whose prediction Z (nregion) is larger. reference: kangaroo/kangaroo/predict.py:188-199. */
 int dbk_gather_maps(dbk_stream_t stream, int dtype, const uint32_t* regions, size_t nregion, size_t padding, int strands, const void* Z,
                     const void* dX, void* map);
+
+/* ------------------------------------------------------------------ operators on the rows of a map
+ * Layers between the motif scan and the pooling (no counterpart in the reference). A map is (N, D): rows are positions, the fastest
+ * dimension is the channel (models side by side, as everywhere). dtype names the type the rows are kept in: DBK_F32, DBK_F64 or
+ * DBK_BF16; weights, statistics and states are float (double for DBK_F64), and so is all arithmetic. Matrices of rows have a row
+ * stride of their own (ld, in elements, >= columns), so that a block of columns of a wider matrix can be passed; weights and states
+ * are contiguous. regions: (nregion, 2) row ranges in any order, which must not overlap; bounds are cut at N, and a range that
+ * ends before it starts is empty. Rows in no region are not read, and left as they are in outputs. Outputs must not share memory
+ * with inputs. Results do not depend on the order in which workgroups run. `work`: caller-owned device memory of at least the bytes that the call's
+ * _workspace function names, 16-byte aligned, in any state; calls that overlap must not share it. */
+
+/* Z = c * gamma / sqrt(mean(c^2) + eps) + beta with c = X - mean(X), means over every chunk of `group` consecutive columns of each of the n
+ * rows (m columns; group divides m, as in dbk_softmax). gamma, beta: (m), may be NULL (ones, zeros). stats (may be NULL): (2, n * m / group),
+ * the chunks' means and reciprocal deviations, for the backward pass. */
+int dbk_layernorm(dbk_stream_t stream, int dtype, const void* X, size_t ldx, const void* gamma, const void* beta, size_t n, size_t m, size_t group,
+                  double eps, void* Z, size_t ldz, void* stats);
+/* dX, dgamma (m) and dbeta (m) (each weight's gradient may be NULL; written, not accumulated) from dZ, the forward's inputs and its stats. */
+int dbk_layernorm_bprop_workspace(int dtype, size_t n, size_t m, size_t group, size_t* work_bytes);
+int dbk_layernorm_bprop(dbk_stream_t stream, int dtype, const void* X, size_t ldx, const void* gamma, const void* stats, const void* dZ, size_t lddz,
+                        size_t n, size_t m, size_t group, void* dX, size_t lddx, void* dgamma, void* dbeta, void* work, size_t work_bytes);
+
+/* Causal convolution along every region's rows, a filter of 1 to 4 taps per channel: Z[t] = act(bias + sum_j W[j] * X[t - taps + 1 + j]), W (taps, D),
+ * bias (D, may be NULL), act(p) = p * sigmoid(p) with silu, p without. Rows before a region's first come from state (nregion, taps - 1, D; kept
+ * as the rows are, oldest first) or are zeros (NULL). last (nregion, taps - 1, D, may be NULL): the rows that the next piece of each sequence needs as its state. */
+int dbk_causalconv_workspace(int dtype, size_t taps, size_t N, size_t D, size_t nregion, int backward, size_t* work_bytes);
+int dbk_causalconv(dbk_stream_t stream, int dtype, const void* X, size_t ldx, const void* W, const void* bias, size_t taps, size_t N, size_t D,
+                   const uint32_t* regions, size_t nregion, int silu, const void* state, void* Z, size_t ldz, void* last, void* work, size_t work_bytes);
+/* Its backward for sequences that start from zeros: dX (regions' rows), dW (taps, D) and dbias (D, may be NULL), written, not accumulated. */
+int dbk_causalconv_bprop(dbk_stream_t stream, int dtype, const void* X, size_t ldx, const void* W, const void* bias, size_t taps, size_t N, size_t D,
+                         const uint32_t* regions, size_t nregion, int silu, const void* dZ, size_t lddz, void* dX, size_t lddx, void* dW, void* dbias,
+                         void* work, size_t work_bytes);
+/* One new row for each of n sequences: Z (n, D) from X (n, D) and state (n, taps - 1, D), whose successor goes to `into` (may be `state` itself). */
+int dbk_causalconv_step(dbk_stream_t stream, int dtype, const void* X, size_t ldx, const void* W, const void* bias, size_t taps, size_t n, size_t D, int silu,
+                        const void* state, void* into, void* Z, size_t ldz);
+
+/* Selective state space scan along every region's rows: d = softplus(dt + dt_bias) (dt + dt_bias without softplus), h = exp(d * A) * h + d * X * B,
+ * Y = sum over states of C * h + skip * X, times gate * sigmoid(gate) where there is a gate. S <= 64 states per channel; the D channels
+ * form G equal groups, each with its own S columns of B and C. */
+typedef struct dbk_statescan_args {
+    int dtype, softplus;
+    size_t N, D, S, G;                          /* rows, channels, states, groups */
+    const uint32_t* regions; size_t nregion;
+    const void* X; size_t ldx;                  /* (N, D) rows */
+    const void* dt; size_t lddt;                /* (N, D) rows */
+    const void* A;                              /* (S, D) weights */
+    const void* B; size_t ldb;                  /* (N, G * S), kept as the weights are */
+    const void* C; size_t ldc;
+    const void *skip, *dt_bias;                 /* (D) weights, may be NULL (zeros) */
+    const void* gate; size_t ldgate;            /* (N, D) rows, may be NULL */
+    const void* state;                          /* (nregion, S, D): the states before the regions' first rows, may be NULL (zeros) */
+    void* Y; size_t ldy;                        /* (N, D) rows */
+    void* last;                                 /* (nregion, S, D): the states behind the last rows, may be NULL */
+    void* keep;                                 /* forward: may be NULL; ceil(N / 16) blocks of (S, D): states that the backward pass starts from */
+    const void* dY; size_t lddy;                /* from here on: backward only */
+    void* dX; size_t lddx; void* ddt; size_t ldddt; void* dgate; size_t lddgate;
+    void* dB; size_t lddb; void* dC; size_t lddc;
+    void *dA, *dskip, *ddt_bias;                /* written, not accumulated; dskip and ddt_bias may be NULL */
+} dbk_statescan_args;
+int dbk_statescan_args_size(void);              /* sizeof(dbk_statescan_args) as the library was built */
+int dbk_statescan_workspace(const dbk_statescan_args* args, int backward, size_t* work_bytes);
+int dbk_statescan(dbk_stream_t stream, const dbk_statescan_args* args, void* work, size_t work_bytes);
+/* Backward for sequences that start from zero states; keep: as the forward call with the same inputs filled it. */
+int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* args, void* work, size_t work_bytes);
+/* One new row for each of N sequences (regions are not looked at): state (N, S, D), its successor goes to `last` (may be `state` itself). */
+int dbk_statescan_step(dbk_stream_t stream, const dbk_statescan_args* args);
 
 /* ------------------------------------------------------------------ one whole optimiser step */
 
