@@ -1,0 +1,155 @@
+// Selective state space scan along the rows of every region of a map: S states per channel that decay and take in the rows,
+//
+//   d = softplus(dt + bias) (or dt),  h[t] = exp(d A) h[t-1] + d x B[t],  y = C[t] . h[t] + D x,  y *= g sigmoid(g)
+//
+// with A (S, channels) per channel, B and C per row and group of channels. Backward, with e = dy g sigmoid(g) and the gradient g[t] of h[t]
+// running from the last row to the first:
+//
+//   g[t] = C e + a[t+1] g[t+1],  dx = d (B . g) + D e,  dd = x (B . g) + sum_s g a h[t-1] A,  dA = sum_t g a h[t-1] d,
+//   dB = sum over the group's channels of g d x,  dC = the same of e h,  dD = sum_t e x,  ddt = dd sigmoid(dt + bias),  dbias = sum_t ddt
+//
+// A lane is a channel and a workgroup one wave: B and C are then the same for a whole wave whose channels are of one group, and come as scalar
+// operands. States are float32 (double for double rows).
+#pragma once
+#include <type_traits>
+#include "rows_common.h"
+
+namespace dbk {
+
+constexpr unsigned SCAN_CHUNK = 16;              // rows between two kept states
+
+struct scan_shape {
+    unsigned N, D, S, G, gs, nregion;            // rows, channels, states, groups, channels per group, regions
+    unsigned tpg, softplus;                      // waves' tiles per group (64 lanes per group), or 0: several groups per wave
+    size_t ldx, lddt, ldb, ldc, ldg, ldy;
+};
+
+// The channel of a lane: LG = 64 lanes for the channels of one group (tpg tiles of 64), or LG lanes for each of 64 / LG groups.
+struct scan_lane { unsigned group, ch; bool active; };
+template <int LG> __device__ __forceinline__ scan_lane lane_channel(const scan_shape& p, unsigned tile, unsigned lane)
+{
+    scan_lane l;
+    unsigned in;
+    if (LG == 64) {
+        l.group = tile / p.tpg;
+        in = (tile - l.group * p.tpg) * 64u + lane;
+        l.active = in < p.gs;
+    } else {
+        l.group = tile * (64u / LG) + lane / LG;
+        in = lane % LG;
+        l.active = l.group < p.G && in < p.gs;
+        l.group = min(l.group, p.G - 1u);
+    }
+    l.ch = l.group * p.gs + min(in, p.gs - 1u);  // (a lane without a channel follows its group's last one and stores nothing)
+    return l;
+}
+
+__device__ __forceinline__ float fma_a(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ double fma_a(double a, double b, double c) { return fma(a, b, c); }
+
+template <typename A> __device__ __forceinline__ A step_of(const scan_shape& p, A raw, A& slope)
+{
+    if (p.softplus) return softplus_of(raw, slope);
+    slope = A(1);
+    return raw;
+}
+
+template <typename A> __device__ __forceinline__ A* kept_at(const scan_shape& p, A* keep, unsigned start, unsigned chunk)
+{
+    return keep + ((size_t)start / SCAN_CHUNK + chunk) * p.S * p.D;
+}
+
+constexpr unsigned SCAN_STATES = 64;             // the most states per channel
+
+// Lanes per group and tiles of channels; rows per segment of a long region and segment slots (0: no region can be long).
+struct scan_plan { int lanes; unsigned tpg, tiles, seg, slots; };
+
+// A region of up to two segments is one wave's work, a longer one is cut: its segments' states are first found from zeros (which costs
+// a second pass over its rows), carried over from segment to segment, and the rows then written with the right states in
+// front. The segment is an even share of all rows for `waves` waves: where regions and tiles alone are that many, none is cut.
+
+inline scan_plan plan_scan(size_t N, size_t D, size_t G, size_t waves, size_t least)
+{
+    scan_plan p;
+    const size_t gs = D / G;
+    p.lanes = gs <= 16 ? 16 : gs <= 32 ? 32 : 64;
+    p.tpg = p.lanes == 64 ? divup(gs, 64) : 0u;
+    p.tiles = p.lanes == 64 ? (unsigned)(G * p.tpg) : divup(G, 64 / p.lanes);
+    const size_t share = (N * p.tiles / waves + SCAN_CHUNK - 1) / SCAN_CHUNK * SCAN_CHUNK;
+    const size_t seg = share > least ? share : least, most = size_t(1) << 30;
+    p.seg = (unsigned)(seg < most ? seg : most);
+    p.slots = N > 2 * (size_t)p.seg ? (unsigned)segment_slots(N, p.seg) : 0u;
+    return p;
+}
+
+inline scan_shape shape_of(const dbk_statescan_args& a)
+{
+    scan_shape s;
+    s.N = (unsigned)a.N; s.D = (unsigned)a.D; s.S = (unsigned)a.S; s.G = (unsigned)a.G; s.gs = (unsigned)(a.D / a.G); s.nregion = (unsigned)a.nregion;
+    s.tpg = 0; s.softplus = a.softplus != 0;
+    s.ldx = a.ldx; s.lddt = a.lddt; s.ldb = a.ldb; s.ldc = a.ldc; s.ldg = a.ldgate; s.ldy = a.ldy;
+    return s;
+}
+
+template <typename F> void with_lanes(int lanes, F f)
+{
+    if (lanes == 16) f(std::integral_constant<int, 16>());
+    else if (lanes == 32) f(std::integral_constant<int, 32>());
+    else f(std::integral_constant<int, 64>());
+}
+
+// Registers for the states, and whether all of them hold one: 16 states have a form of their own without padding.
+template <typename F> void with_states(size_t S, F f)
+{
+    if (S == 16) f(std::integral_constant<int, 16>(), std::true_type());
+    else if (S <= 4) f(std::integral_constant<int, 4>(), std::false_type());
+    else if (S <= 8) f(std::integral_constant<int, 8>(), std::false_type());
+    else if (S <= 16) f(std::integral_constant<int, 16>(), std::false_type());
+    else if (S <= 32) f(std::integral_constant<int, 32>(), std::false_type());
+    else f(std::integral_constant<int, 64>(), std::false_type());
+}
+
+inline int check_scan(const dbk_statescan_args* a)
+{
+    DBK_CHECK(a, "ValueError: null argument block");
+    DBK_ROW_DTYPE_OK(a->dtype);
+    DBK_CHECK(a->S >= 1 && a->S <= SCAN_STATES, "NotImplementedError: 1 to %u states per channel, got %zu", SCAN_STATES, a->S);
+    DBK_CHECK(a->G >= 1 && a->D % a->G == 0, "ValueError: the number of channels must be divisible by the number of groups");
+    DBK_CHECK(a->N < (size_t(1) << 32) - 64 && a->D < (size_t(1) << 21) && a->nregion < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu channels, %zu regions)",
+              a->N, a->D, a->nregion);
+    DBK_CHECK(!a->D || a->A, "ValueError: null weights");
+    DBK_CHECK(!a->N || !a->D || (a->X && a->dt && a->B && a->C), "ValueError: null matrix");
+    DBK_CHECK(a->N <= 1 || (a->ldx >= a->D && a->lddt >= a->D && a->ldb >= a->G * a->S && a->ldc >= a->G * a->S && (!a->gate || a->ldgate >= a->D)),
+              "ValueError: row strides must be at least the number of columns");
+    DBK_CHECK(plan_scan(0, a->D, a->G, 1, 1).tiles <= 65535u, "ValueError: too many groups (%zu of %zu channels)", a->G, a->G ? a->D / a->G : 0);
+    return 0;
+}
+
+// The segments of a call's long regions, in its workspace: marks (one per slot), what the segments leave from zeros, the sums of
+// their steps, and the states in front of them.
+struct scan_segments { uint32_t* marks; void *local, *steps, *carry; size_t bytes; };
+inline scan_segments segments_in(void* work, const dbk_statescan_args& a, const scan_plan& p)
+{
+    scan_segments s;
+    const size_t e = acc_size(a.dtype), states = (p.slots * a.S * a.D * e + 15) / 16 * 16;
+    size_t at = ((size_t)p.slots * 4 + 15) / 16 * 16;
+    s.marks = (uint32_t*)work;
+    s.local = (char*)work + at;
+    s.carry = (char*)work + (at += states);
+    s.steps = (char*)work + (at += states);
+    s.bytes = at + (p.slots * a.D * e + 15) / 16 * 16;
+    if (!p.slots) { s.marks = nullptr; s.bytes = 0; }
+    return s;
+}
+
+// Marks the segments behind the first of every region that is cut: a wave per region.
+__device__ __forceinline__ bool is_cut(row_range g, unsigned seg) { return g.end - g.start > 2u * seg; }
+__device__ __forceinline__ bool cut_segment(const scan_shape& p, const uint32_t* regions, const uint32_t* marks, unsigned slot, unsigned seg,
+                                            unsigned& r, row_range& g, unsigned& k)
+{
+    return slot_segment(regions, p.nregion, p.N, marks, slot, seg, r, g, k) && is_cut(g, seg);
+}
+size_t bprop_work_bytes(const dbk_statescan_args& a);            // statescan_bprop.hip
+int mark_cut_regions(hipStream_t st, const uint32_t* regions, size_t nregion, size_t N, unsigned seg, uint32_t* marks);
+
+}  // namespace dbk
