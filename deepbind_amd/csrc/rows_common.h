@@ -102,13 +102,15 @@ __device__ __forceinline__ double softplus_of(double x, double& slope)
     return fmax(x, 0.0) + log1p(e);
 }
 
-// Region r's rows, bounded by the map: [start, end), empty where the table says so or lies outside.
+// Region r's rows, bounded by the map: [start, end), empty where the table says so or lies outside. r is the same in all lanes of a wave, and
+// the compiler is told that what it reads is too: addresses and branches that depend on it are then scalar.
 struct row_range { unsigned start, end; };
+__device__ __forceinline__ unsigned uniform(unsigned x) { return (unsigned)__builtin_amdgcn_readfirstlane((int)x); }
 __device__ __forceinline__ row_range region_rows(const uint32_t* regions, size_t r, unsigned N)
 {
     row_range g;
-    g.start = min(regions[2 * r], N);
-    g.end = max(min(regions[2 * r + 1], N), g.start);
+    g.start = min(uniform(regions[2 * r]), N);
+    g.end = max(min(uniform(regions[2 * r + 1]), N), g.start);
     return g;
 }
 
@@ -124,7 +126,7 @@ __device__ __forceinline__ void mark_segments(uint32_t* marks, unsigned r, row_r
 __device__ __forceinline__ bool slot_segment(const uint32_t* regions, unsigned nregion, unsigned N, const uint32_t* marks, unsigned slot, unsigned L,
                                              unsigned& r, row_range& g, unsigned& k)
 {
-    r = marks[slot];
+    r = uniform(marks[slot]);
     if (r >= nregion) return false;
     g = region_rows(regions, r, N);
     const unsigned q = g.start / L;

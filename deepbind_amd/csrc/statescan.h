@@ -44,6 +44,13 @@ template <int LG> __device__ __forceinline__ scan_lane lane_channel(const scan_s
     return l;
 }
 
+// A lane's element of a row: the row's address is the same in all lanes and stays in scalar registers, the lane's place is one 32-bit offset in
+// bytes (D * 8 < 2^32). The compiler is told nothing about the offset (opaque): it would add it to every matrix' address beforehand, in two
+// vector registers each, for as long as the kernel runs.
+template <typename V> __device__ __forceinline__ V opaque(V v) { asm volatile("" : "+v"(v)); return v; }
+template <typename T> __device__ __forceinline__ T lane_load(const T* row, unsigned bytes) { return *(const T*)((const char*)row + bytes); }
+template <typename T> __device__ __forceinline__ void lane_store(T* row, unsigned bytes, T v) { *(T*)((char*)row + bytes) = v; }
+
 __device__ __forceinline__ float fma_a(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fma_a(double a, double b, double c) { return fma(a, b, c); }
 
@@ -52,6 +59,32 @@ template <typename A> __device__ __forceinline__ A step_of(const scan_shape& p, 
     if (p.softplus) return softplus_of(raw, slope);
     slope = A(1);
     return raw;
+}
+
+// Weights of all states of one row, zero from state S on. FULL: S == NS.
+template <typename A, bool UNIFORM, int NS, bool FULL> __device__ __forceinline__ void load_row(A (&v)[NS], const A* p, unsigned S)
+{
+    typedef const __attribute__((address_space(4))) A* uniform_ptr;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+        const unsigned at = FULL ? j : min((unsigned)j, S - 1u);               // (in bounds whatever S is)
+        const A x = UNIFORM ? ((uniform_ptr)(uintptr_t)p)[at] : p[at];
+        v[j] = FULL || j < (int)S ? x : A(0);
+    }
+}
+// the states of a lane's channel between registers and (S, D) memory; null: zeros
+template <typename A, int NS> __device__ __forceinline__ void regs_from(const scan_shape& p, const scan_lane& l, A (&h)[NS], const A* from, A scale)
+{
+    const unsigned at = opaque(l.ch * (unsigned)sizeof(A));
+#pragma unroll
+    for (int j = 0; j < NS; ++j) h[j] = from && j < (int)p.S ? lane_load(from + (size_t)j * p.D, at) * scale : A(0);
+}
+template <typename A, int NS> __device__ __forceinline__ void regs_to(const scan_shape& p, const scan_lane& l, const A (&h)[NS], A* to)
+{
+    const unsigned at = opaque(l.ch * (unsigned)sizeof(A));
+    if (!l.active) return;
+#pragma unroll
+    for (int j = 0; j < NS; ++j) if (j < (int)p.S) lane_store(to + (size_t)j * p.D, at, h[j]);
 }
 
 template <typename A> __device__ __forceinline__ A* kept_at(const scan_shape& p, A* keep, unsigned start, unsigned chunk)

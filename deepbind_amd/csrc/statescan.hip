@@ -3,30 +3,6 @@
 
 namespace dbk {
 
-// Weights of all states of one row, zero from state S on. FULL: S == NS.
-template <typename A, bool UNIFORM, int NS, bool FULL> __device__ __forceinline__ void load_row(A (&v)[NS], const A* p, unsigned S)
-{
-    typedef const __attribute__((address_space(4))) A* uniform_ptr;
-#pragma unroll
-    for (int j = 0; j < NS; ++j) {
-        const unsigned at = FULL ? j : min((unsigned)j, S - 1u);               // (in bounds whatever S is)
-        const A x = UNIFORM ? ((uniform_ptr)(uintptr_t)p)[at] : p[at];
-        v[j] = FULL || j < (int)S ? x : A(0);
-    }
-}
-// the states of a lane's channel between registers and (S, D) memory; null: zeros
-template <typename A, int NS> __device__ __forceinline__ void regs_from(const scan_shape& p, const scan_lane& l, A (&h)[NS], const A* from, A scale)
-{
-#pragma unroll
-    for (int j = 0; j < NS; ++j) h[j] = from && j < (int)p.S ? from[(size_t)j * p.D + l.ch] * scale : A(0);
-}
-template <typename A, int NS> __device__ __forceinline__ void regs_to(const scan_shape& p, const scan_lane& l, const A (&h)[NS], A* to)
-{
-    if (!l.active) return;
-#pragma unroll
-    for (int j = 0; j < NS; ++j) if (j < (int)p.S) to[(size_t)j * p.D + l.ch] = h[j];
-}
-
 // n rows from `row` on, the states in registers. OUT: the rows of Y are written; otherwise only the states move on, and `steps` adds up d.
 // kept: null, or the block of states in front of the first row's chunk of 16; those in front of the next ones are written behind it.
 template <typename T, int LG, int NS, bool FULL, bool OUT>
@@ -38,14 +14,15 @@ __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& 
     typedef typename acc_of<T>::type A;
     constexpr int U = 4;                         // rows whose x, dt and gate are fetched together, a step ahead
     if (!n) return;
+    const unsigned at = opaque(l.ch * (unsigned)sizeof(T));
     T xn[U], dn[U], gn[U];
     auto fetch = [&](unsigned t) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             const size_t r = row + min(t + i, n - 1u);
-            xn[i] = X[r * p.ldx + l.ch];
-            dn[i] = dt[r * p.lddt + l.ch];
-            if (OUT && gate) gn[i] = gate[r * p.ldg + l.ch];
+            xn[i] = lane_load(X + r * p.ldx, at);
+            dn[i] = lane_load(dt + r * p.lddt, at);
+            if (OUT && gate) gn[i] = lane_load(gate + r * p.ldg, at);
         }
     };
     const A *br = B + row * p.ldb + (size_t)l.group * p.S, *cr = C + row * p.ldc + (size_t)l.group * p.S;
@@ -83,7 +60,7 @@ __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& 
                 for (int j = 0; j < NS; ++j) y[j & 3] = fma_a(c[j], h[j], y[j & 3]);
                 A out = (y[0] + y[1]) + (y[2] + y[3]);
                 if (gate) { const A gg = (A)g[i]; out *= gg * sigmoid_of(gg); }
-                if (l.active) Y[(row + t + i) * p.ldy + l.ch] = (T)out;
+                if (l.active) lane_store(Y + (row + t + i) * p.ldy, at, (T)out);
             } else
                 steps += d[i];
             __builtin_amdgcn_sched_barrier(0);

@@ -3,37 +3,26 @@
 
 namespace dbk {
 
-// four neighbouring weights of a row, those from `left` on zero; with UNIFORM the address is the same in all lanes and the loads are scalar
-template <typename A, bool UNIFORM, bool FULL> __device__ __forceinline__ void load4(A (&v)[4], const A* p, unsigned left)
-{
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (UNIFORM) {
-            typedef const __attribute__((address_space(4))) A* uniform_ptr;
-            v[i] = FULL || i < (int)left ? ((uniform_ptr)(uintptr_t)p)[i] : A(0);
-        } else
-            v[i] = FULL || i < (int)left ? p[i] : A(0);
-    }
-}
-
 template <typename A> struct quad { A v[4]; } __attribute__((aligned(16)));
 
 template <typename A> __device__ __forceinline__ void states_to(const scan_shape& p, const scan_lane& l, unsigned lane, const quad<A>* h, A* to)
 {
     if (!l.active) return;
+    const unsigned at = opaque(l.ch * (unsigned)sizeof(A));
     for (unsigned q = 0; 4u * q < p.S; ++q) {
         const quad<A> s = h[q * 64u + lane];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) if (4u * q + j < p.S) to[(size_t)(4u * q + j) * p.D + l.ch] = s.v[j];
+        for (int j = 0; j < 4; ++j) if (4u * q + j < p.S) lane_store(to + (size_t)(4u * q + j) * p.D, at, s.v[j]);
     }
 }
 // zeros where there is nothing to read
-template <typename A> __device__ __forceinline__ void states_from(const scan_shape& p, const scan_lane& l, unsigned lane, quad<A>* h, const A* from, A scale)
+template <typename A> __device__ __forceinline__ void states_from(const scan_shape& p, const scan_lane& l, unsigned lane, quad<A>* h, const A* from)
 {
+    const unsigned at = opaque(l.ch * (unsigned)sizeof(A));
     for (unsigned q = 0; 4u * q < p.S; ++q) {
         quad<A> s;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s.v[j] = from && 4u * q + j < p.S ? from[(size_t)(4u * q + j) * p.D + l.ch] * scale : A(0);
+        for (int j = 0; j < 4; ++j) s.v[j] = from && 4u * q + j < p.S ? lane_load(from + (size_t)(4u * q + j) * p.D, at) : A(0);
         h[q * 64u + lane] = s;
     }
 }
@@ -72,69 +61,175 @@ struct scan_bshape { size_t lddy, lddx, ldddt, lddg, lddb, lddc; };
 // Where a wave's sums of dB and dC go: the gradient itself where the wave holds the whole group, or its tile's share.
 template <typename A> struct scan_out { A *dB, *dC; size_t ldb, ldc; };
 
-// Backward over one chunk: the states are formed again from the one kept before it, then the rows are taken from the last to the first.
-// lds: ag = the gradient that the rows behind send to the chunk's last state, da = dA so far, both [state / 4][lane]; st: two values per
-// row and lane that are needed again at the end (the slope of the step; dY times the gate's derivative).
-template <typename T, int LG, bool WHOLE>
-__device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan_bshape& bp, const scan_lane& l, unsigned lane, unsigned nrow, size_t row0, const T* X,
-                                                 const T* dt, const T* gate, const T* dY, const typename acc_of<T>::type* B, const typename acc_of<T>::type* C,
-                                                 typename acc_of<T>::type skip, typename acc_of<T>::type bias, const typename acc_of<T>::type* before,
-                                                 const quad<typename acc_of<T>::type>* a2, quad<typename acc_of<T>::type>* ag, quad<typename acc_of<T>::type>* da,
-                                                 typename acc_of<T>::type* st, T* dX, T* ddt, T* dgate, scan_out<typename acc_of<T>::type> out,
+template <typename T> struct scan_rows_in {      // what the backward pass reads of a row
+    typedef typename acc_of<T>::type A;
+    const T *X, *dt, *gate, *dY;
+    const A *B, *C, *keep;
+    const uint32_t *regions, *marks;
+};
+template <typename T> struct scan_rows_out { T *dX, *ddt, *dgate; };
+
+// B and C of a chunk's rows in LDS, [row][B, C][group of the wave][S rounded up to fours], zeros behind the last row and state: in LDS rather than
+// in scalar registers, for which a row's work is too short to hide the loads of the next row's.
+template <typename T, int LG>
+__device__ __forceinline__ void stage_weights(const scan_shape& p, unsigned lane, unsigned nrow, size_t row0, const scan_rows_in<T>& in, typename acc_of<T>::type* bc)
+{
+    typedef typename acc_of<T>::type A;
+    constexpr unsigned GW = 64 / LG;
+    const unsigned pad = (p.S + 3u) / 4u * 4u, width = 2u * GW * pad;
+    const unsigned first = LG == 64 ? blockIdx.y / p.tpg : blockIdx.y * GW;
+    unsigned across = 64;                        // lanes for one row: several rows at a time where they are few
+    while (across / 2u >= width) across /= 2u;
+    for (unsigned i = lane % across; i < width; i += across) {
+        const unsigned g = i / pad % GW, s = i % pad;
+        const bool c = i >= GW * pad, here = s < p.S && first + g < p.G;
+        const A* from = (c ? in.C + row0 * p.ldc : in.B + row0 * p.ldb) + (size_t)(first + g) * p.S + s;
+        const size_t ld = c ? p.ldc : p.ldb;
+#pragma unroll 8
+        for (unsigned r = lane / across; r < SCAN_CHUNK; r += 64u / across) bc[r * width + i] = here && r < nrow ? from[r * ld] : A(0);
+    }
+    __builtin_amdgcn_wave_barrier();             // (one wave: LDS keeps its order)
+}
+
+// Backward over one chunk of nrow <= 16 rows: the states are formed again from the one kept before it, then the rows are taken from the last
+// to the first; four states at a time, whose values at all rows are in registers, while those of the other states wait in LDS.
+// ag: the gradient that the rows behind send to the chunk's last state, da: dA so far, both [state / 4][lane]; st: two values per
+// row and lane that are needed again at the end (the slope of the step; dY times the gate's derivative); bc: as stage_weights.
+template <typename T, int LG>
+__device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan_bshape& bp, const scan_lane& l, unsigned lane, unsigned nrow, size_t row0,
+                                                 const scan_rows_in<T>& in, const typename acc_of<T>::type* A_, typename acc_of<T>::type skip,
+                                                 typename acc_of<T>::type bias, const typename acc_of<T>::type* before,
+                                                 quad<typename acc_of<T>::type>* ag, quad<typename acc_of<T>::type>* da, typename acc_of<T>::type* st,
+                                                 typename acc_of<T>::type* bc, const scan_rows_out<T>& to, scan_out<typename acc_of<T>::type> out,
                                                  typename acc_of<T>::type& dskip, typename acc_of<T>::type& dbias)
 {
     typedef typename acc_of<T>::type A;
     constexpr int R = SCAN_CHUNK;
-    A x[R], d[R], e[R], sB[R], sA[R], y[R];
+    const bool gated = in.gate != nullptr;
+    const unsigned place = opaque(l.ch * (unsigned)sizeof(T)), place_a = opaque(l.ch * (unsigned)sizeof(A));
+    // what the next four states start from is fetched while these are worked on
+    quad<A> kn, hn;
+    auto fetch = [&](unsigned q) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        x[i] = d[i] = e[i] = sB[i] = sA[i] = y[i] = A(0);
-        if (!WHOLE && i >= (int)nrow) continue;
-        x[i] = (A)X[(row0 + i) * p.ldx + l.ch];
-        A slope;
-        d[i] = step_of(p, (A)dt[(row0 + i) * p.lddt + l.ch] + bias, slope);
-        e[i] = l.active ? (A)dY[(row0 + i) * bp.lddy + l.ch] : A(0);
-        st[i * 64u + lane] = slope;
-        if (gate) {
-            const A g = (A)gate[(row0 + i) * p.ldg + l.ch], s = sigmoid_of(g);
-            st[(R + i) * 64u + lane] = e[i] * s * fma_a(g, A(1) - s, A(1));
-            e[i] *= g * s;
+        for (int j = 0; j < 4; ++j) {
+            const unsigned s = min(4u * q + j, p.S - 1u);
+            kn.v[j] = lane_load(A_ + (size_t)s * p.D, place_a);
+            hn.v[j] = before ? lane_load(before + (size_t)s * p.D, place_a) : A(0);
         }
-    }
-    auto states = [&](auto full, unsigned q) {
-        constexpr bool FULL = decltype(full)::value;
-        const unsigned left = p.S - 4u * q;
-        const quad<A> k = a2[q * 64u + lane];
-        const A *br = B + row0 * p.ldb + (size_t)l.group * p.S + 4u * q, *cr = C + row0 * p.ldc + (size_t)l.group * p.S + 4u * q;
-        A h[R + 1][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) h[0][j] = before && (FULL || j < (int)left) ? before[(size_t)(4u * q + j) * p.D + l.ch] : A(0);
+    };
+    fetch(0);
+    A x[R], d[R], e[R], sB[R], sA[R], y[R];
+    {
+        T xr[R], dr[R], er[R], gr[R];
+        // (rows behind the chunk's last one repeat it; all loads are on their way before the first value is used)
+        const T *xp = in.X + row0 * p.ldx, *dp = in.dt + row0 * p.lddt, *ep = in.dY + row0 * bp.lddy;
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            if (!WHOLE && i >= (int)nrow) break;
-            A b[4];
-            load4<A, LG == 64, FULL>(b, br + (size_t)i * p.ldb, left);
-            const A in = d[i] * x[i];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) h[i + 1][j] = fma_a(exp2_fast(d[i] * k.v[j]), h[i][j], in * b[j]);
+            xr[i] = lane_load(xp, place);
+            dr[i] = lane_load(dp, place);
+            er[i] = lane_load(ep, place);
+            const bool more = i + 1 < (int)nrow;
+            xp += more ? p.ldx : 0;
+            dp += more ? p.lddt : 0;
+            ep += more ? bp.lddy : 0;
         }
+        if (gated) {
+            const T* gp = in.gate + row0 * p.ldg;
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                gr[i] = lane_load(gp, place);
+                gp += i + 1 < (int)nrow ? p.ldg : 0;
+            }
+        }
+        stage_weights<T, LG>(p, lane, nrow, row0, in, bc);
+        if (p.softplus) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                A slope;
+                d[i] = softplus_of((A)dr[i] + bias, slope);
+                st[i * 64u + lane] = slope;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                d[i] = (A)dr[i] + bias;
+                st[i * 64u + lane] = A(1);
+            }
+        }
+        // rows behind the last one: no step, so nothing is taken in or sent
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const bool here = i < (int)nrow;
+            x[i] = here ? (A)xr[i] : A(0);
+            d[i] = here ? d[i] : A(0);
+            e[i] = here && l.active ? (A)er[i] : A(0);
+            sB[i] = sA[i] = A(0);
+            y[i] = skip * x[i];
+        }
+        if (gated) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const A g = (A)gr[i], s = sigmoid_of(g);
+                st[(R + i) * 64u + lane] = e[i] * s * fma_a(g, A(1) - s, A(1));
+                e[i] *= g * s;
+            }
+        }
+    }
+    const unsigned pad = (p.S + 3u) / 4u * 4u, width = 2u * (64 / LG) * pad;
+    const A* weights = bc + (lane / LG) * pad;
+    for (unsigned q = 0; 4u * q < p.S; ++q) {
+        const unsigned left = p.S - 4u * q;
+        quad<A> k = kn;
+        A h[R + 1][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            k.v[j] = j < (int)left ? k.v[j] * A(1.4426950408889634) : A(0);
+            h[0][j] = j < (int)left ? hn.v[j] : A(0);
+        }
+        if (left > 4u) fetch(q + 1u);
+        const A *b = weights + 4u * q, *c = b + (64 / LG) * pad;
+        quad<A> bn = *(const quad<A>*)b;
+        // A row's work stays together, its weights being fetched a row ahead: left to itself the compiler gathers many rows' weights and
+        // spills them. Rows that do not exist are left out by fours.
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            if (i % 4 == 0 && i >= (int)nrow) break;
+            const quad<A> bi = bn;
+            if (i + 1 < R) bn = *(const quad<A>*)(b + (i + 1) * width);
+            const A dx = d[i] * x[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[i + 1][j] = fma_a(exp2_fast(d[i] * k.v[j]), h[i][j], dx * bi.v[j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        // (the decays, like the product of step and input, are formed again below: kept from the first time they would take 80 registers
+        // more, and the compiler is told nothing about their factors any more so that it does not keep them)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k.v[j] = opaque(k.v[j]);
+#pragma unroll
+        for (int i = 0; i < R; ++i) x[i] = opaque(x[i]);
         quad<A> g = ag[q * 64u + lane], sum = da[q * 64u + lane];
+        const unsigned top = (nrow + 3u) / 4u * 4u - 1u;
+        bn = *(const quad<A>*)(b + top * width);
+        quad<A> cn = *(const quad<A>*)(c + top * width);
         A rows[R];
 #pragma unroll
         for (int i = R - 1; i >= 0; --i) {
             rows[i] = A(0);
-            if (!WHOLE && i >= (int)nrow) continue;
-            A b[4], c[4], v[8];
-            load4<A, LG == 64, FULL>(b, br + (size_t)i * p.ldb, left);
-            load4<A, LG == 64, FULL>(c, cr + (size_t)i * p.ldc, left);
-            const A in = d[i] * x[i];
+            if ((i & ~3) >= (int)nrow) continue;
+            const quad<A> bi = bn, ci = cn;
+            if (i) {
+                bn = *(const quad<A>*)(b + (i - 1) * width);
+                cn = *(const quad<A>*)(c + (i - 1) * width);
+            }
+            const A dx = d[i] * x[i];
+            A v[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const A a = exp2_fast(d[i] * k.v[j]), now = fma_a(c[j], e[i], g.v[j]), w = now * (a * h[i][j]);
-                if (gate) y[i] = fma_a(c[j], h[i + 1][j], y[i]);
-                v[j] = now * in;
+                const A a = exp2_fast(d[i] * k.v[j]), now = fma_a(ci.v[j], e[i], g.v[j]), w = now * (a * h[i][j]);
+                y[i] = fma_a(ci.v[j], h[i + 1][j], y[i]);
+                v[j] = now * dx;
                 v[4 + j] = e[i] * h[i + 1][j];
-                sB[i] = fma_a(b[j], now, sB[i]);
+                sB[i] = fma_a(bi.v[j], now, sB[i]);
                 sA[i] = fma_a(w, k.v[j], sA[i]);
                 sum.v[j] = fma_a(w, d[i], sum.v[j]);
                 g.v[j] = a * now;
@@ -146,6 +241,7 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
             v[0] = join<TOP - 1>(v[0], v[2], lane);
             v[1] = join<TOP - 1>(v[1], v[3], lane);
             rows[i] = join<TOP - 2>(v[0], v[1], lane);
+            __builtin_amdgcn_sched_barrier(0);
         }
         ag[q * 64u + lane] = g;
         da[q * 64u + lane] = sum;
@@ -177,88 +273,237 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
         const unsigned base = LG == 64 ? (lane & 1u) * 2u + ((lane >> 1) & 1u) * 4u + ((lane >> 2) & 1u) * 8u
                             : LG == 32 ? (lane & 1u) * 4u + ((lane >> 1) & 1u) * 8u : (lane & 1u) * 8u;
         // (lanes of a group that does not exist carry zeros into it and their first lane says so)
-        if ((FULL || state < left) && (LG == 64 || l.active || (lane % LG >= p.gs && (lane / LG) + blockIdx.y * (64u / LG) < p.G))) {
+        if (state < left && (LG == 64 || l.active || (lane % LG >= p.gs && (lane / LG) + blockIdx.y * (64u / LG) < p.G))) {
             A* o = kind ? out.dC : out.dB;
             const size_t ld = kind ? out.ldc : out.ldb;
 #pragma unroll
             for (int i = 0; i < LEFT; ++i)
-                if (WHOLE || base + i < nrow) o[(row0 + base + i) * ld + (size_t)l.group * p.S + 4u * q + state] = rows[i];
+                if (base + i < nrow) o[(row0 + base + i) * ld + (size_t)l.group * p.S + 4u * q + state] = rows[i];
         }
-    };
-    for (unsigned q = 0; 4u * q < p.S; ++q) {
-        if (4u * q + 4u <= p.S) states(std::true_type(), q);
-        else states(std::false_type(), q);
     }
+    T *xp = to.dX + row0 * bp.lddx, *dp = to.ddt + row0 * bp.ldddt, *gp = to.dgate + row0 * bp.lddg;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        if (!WHOLE && i >= (int)nrow) continue;
+        if (i >= (int)nrow) break;
         const A dd = fma_a(x[i], sB[i], sA[i] * A(0.6931471805599453)) * st[i * 64u + lane];      // (k is A log2(e))
         dskip = fma_a(e[i], x[i], dskip);
         dbias += dd;
-        if (!l.active) continue;
-        dX[(row0 + i) * bp.lddx + l.ch] = (T)fma_a(d[i], sB[i], skip * e[i]);
-        ddt[(row0 + i) * bp.ldddt + l.ch] = (T)dd;
-        if (gate) dgate[(row0 + i) * bp.lddg + l.ch] = (T)(fma_a(skip, x[i], y[i]) * st[(R + i) * 64u + lane]);
+        if (l.active) {
+            lane_store(xp, place, (T)fma_a(d[i], sB[i], skip * e[i]));
+            lane_store(dp, place, (T)dd);
+            if (gated) lane_store(gp, place, (T)(y[i] * st[(R + i) * 64u + lane]));
+        }
+        xp += bp.lddx;
+        dp += bp.ldddt;
+        gp += bp.lddg;
     }
 }
 
-// A wave per tile of channels takes its share of the regions one after another, with dA in LDS, and leaves one block of sums:
-// part[unit][S + 2][D].
-template <typename T, int LG>
-__global__ __launch_bounds__(64) void k_scan_bprop(scan_shape p, scan_bshape bp, const uint32_t* __restrict__ regions, const T* __restrict__ X, const T* __restrict__ dt,
-                                                   const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ B,
-                                                   const typename acc_of<T>::type* __restrict__ C, const typename acc_of<T>::type* __restrict__ skip,
-                                                   const T* __restrict__ gate, const typename acc_of<T>::type* __restrict__ bias,
-                                                   const typename acc_of<T>::type* __restrict__ keep, const T* __restrict__ dY, T* __restrict__ dX,
-                                                   T* __restrict__ ddt, T* __restrict__ dgate, scan_out<typename acc_of<T>::type> out,
-                                                   size_t tile_stride, typename acc_of<T>::type* __restrict__ part)
-{
+// A wave's place in LDS and what it adds up over all its rows.
+template <typename T, int LG> struct scan_wave {
     typedef typename acc_of<T>::type A;
-    extern __shared__ char lds_raw[];
-    const unsigned lane = threadIdx.x, quads = (p.S + 3u) / 4u;
-    quad<A>*a2 = (quad<A>*)lds_raw, *ag = a2 + quads * 64u, *da = ag + quads * 64u;
-    A* st = (A*)(da + quads * 64u);
-    const scan_lane l = lane_channel<LG>(p, blockIdx.y, lane);
-    states_from(p, l, lane, a2, A_, A(1.4426950408889634));
-    states_from(p, l, lane, da, (const A*)nullptr, A(1));
-    const A sk = skip ? skip[l.ch] : A(0), bi = bias ? bias[l.ch] : A(0);
-    A dskip = 0, dbias = 0;
-    if (LG == 64) {                              // (shares of a group's tiles lie one behind another)
-        const size_t o = (size_t)(blockIdx.y - l.group * p.tpg) * tile_stride;
+    unsigned lane;
+    scan_lane l;
+    quad<A> *ag, *da;
+    A *st, *bc, sk, bi, dskip, dbias;
+    const A* A_;
+    __device__ __forceinline__ scan_wave(const scan_shape& p, char* lds, const A* decay, const A* skip, const A* bias)
+    {
+        const unsigned quads = (p.S + 3u) / 4u;
+        lane = threadIdx.x;
+        A_ = decay;
+        ag = (quad<A>*)lds;
+        da = ag + quads * 64u;
+        st = (A*)(da + quads * 64u);
+        bc = st + 2 * SCAN_CHUNK * 64;
+        l = lane_channel<LG>(p, blockIdx.y, lane);
+        states_from(p, l, lane, da, (const A*)nullptr);
+        sk = skip ? skip[l.ch] : A(0);
+        bi = bias ? bias[l.ch] : A(0);
+        dskip = dbias = A(0);
+    }
+    // rows [from, from + n) of a region that starts at `start`, from a multiple of 16 rows behind it; ag holds what the rows behind send
+    __device__ __forceinline__ void rows(const scan_shape& p, const scan_bshape& bp, unsigned start, unsigned from, unsigned n, const scan_rows_in<T>& in,
+                                         const scan_rows_out<T>& to, const scan_out<A>& out)
+    {
+        for (unsigned c = (n + SCAN_CHUNK - 1u) / SCAN_CHUNK; c-- > 0;) {
+            const unsigned at = from + c * SCAN_CHUNK, chunk = (at - start) / SCAN_CHUNK;
+            scan_chunk_bprop<T, LG>(p, bp, l, lane, min(SCAN_CHUNK, n - c * SCAN_CHUNK), at, in, A_, sk, bi, chunk ? kept_at(p, in.keep, start, chunk) : (const A*)nullptr,
+                                    ag, da, st, bc, to, out, dskip, dbias);
+        }
+    }
+    __device__ __forceinline__ void leave(const scan_shape& p, A* part)
+    {
+        states_to(p, l, lane, da, part);
+        if (!l.active) return;
+        part[(size_t)p.S * p.D + l.ch] = dskip;
+        part[(size_t)(p.S + 1u) * p.D + l.ch] = dbias;
+    }
+};
+// (shares of a group's tiles lie one behind another)
+template <int LG, typename A> __device__ __forceinline__ scan_out<A> tile_share(const scan_shape& p, scan_out<A> out, size_t tile_stride)
+{
+    if (LG == 64) {
+        const size_t o = (size_t)(blockIdx.y % p.tpg) * tile_stride;
         out.dB += o;
         out.dC += o;
     }
+    return out;
+}
+
+// A wave per tile of channels takes its share of the regions one after another, with dA in LDS, and leaves one block of sums:
+// part[unit][S + 2][D]. Of a region that is cut it takes the last segment, behind which nothing sends anything.
+template <typename T, int LG>
+__global__ __launch_bounds__(64, 2) void k_scan_bprop(scan_shape p, scan_bshape bp, unsigned seg, scan_rows_in<T> in, const typename acc_of<T>::type* __restrict__ A_,
+                                                   const typename acc_of<T>::type* __restrict__ skip, const typename acc_of<T>::type* __restrict__ bias,
+                                                   scan_rows_out<T> to, scan_out<typename acc_of<T>::type> out, size_t tile_stride,
+                                                   typename acc_of<T>::type* __restrict__ part, typename acc_of<T>::type* __restrict__ carry)
+{
+    typedef typename acc_of<T>::type A;
+    extern __shared__ char lds_raw[];
+    scan_wave<T, LG> w(p, lds_raw, A_, skip, bias);
+    out = tile_share<LG>(p, out, tile_stride);
     for (unsigned r = blockIdx.x; r < p.nregion; r += gridDim.x) {
-        const row_range g = region_rows(regions, r, p.N);
+        const row_range g = region_rows(in.regions, r, p.N);
         if (g.start == g.end) continue;
-        states_from(p, l, lane, ag, (const A*)nullptr, A(1));
-        for (unsigned chunk = (g.end - g.start - 1u) / SCAN_CHUNK + 1u; chunk-- > 0;) {
-            const size_t row = (size_t)g.start + (size_t)chunk * SCAN_CHUNK;
-            const unsigned left = g.end - (unsigned)row;
-            const A* before = chunk ? kept_at(p, keep, g.start, chunk) : (const A*)nullptr;
-            if (left >= SCAN_CHUNK)
-                scan_chunk_bprop<T, LG, true>(p, bp, l, lane, SCAN_CHUNK, row, X, dt, gate, dY, B, C, sk, bi, before, a2, ag, da, st, dX, ddt, dgate, out, dskip, dbias);
-            else
-                scan_chunk_bprop<T, LG, false>(p, bp, l, lane, left, row, X, dt, gate, dY, B, C, sk, bi, before, a2, ag, da, st, dX, ddt, dgate, out, dskip, dbias);
+        states_from(p, w.l, w.lane, w.ag, (const A*)nullptr);
+        const unsigned k = in.marks && is_cut(g, seg) ? (g.end - g.start - 1u) / seg : 0u;
+        w.rows(p, bp, g.start, g.start + k * seg, g.end - g.start - k * seg, in, to, out);
+        if (k) states_to(p, w.l, w.lane, w.ag, carry + (size_t)(g.start / seg + k) * p.S * p.D);
+    }
+    w.leave(p, part + (size_t)blockIdx.x * (p.S + 2u) * p.D);
+}
+
+// What a middle segment sends back when nothing is sent to it, and the sum of its steps: the states' gradients alone.
+template <typename T, int LG, int NS, bool FULL>
+__global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t lddy, unsigned seg, scan_rows_in<T> in, const typename acc_of<T>::type* __restrict__ A_,
+                                                         const typename acc_of<T>::type* __restrict__ bias, typename acc_of<T>::type* __restrict__ local,
+                                                         typename acc_of<T>::type* __restrict__ sums)
+{
+    typedef typename acc_of<T>::type A;
+    constexpr unsigned U = 4;
+    unsigned r, k;
+    row_range g;
+    if (!cut_segment(p, in.regions, in.marks, blockIdx.x, seg, r, g, k) || g.start + (uint64_t)(k + 1u) * seg >= g.end) return;
+    const scan_lane l = lane_channel<LG>(p, blockIdx.y, threadIdx.x);
+    const A bi = bias ? bias[l.ch] : A(0);
+    A a2[NS], ag[NS], c[NS], steps = 0;
+    regs_from(p, l, a2, A_, A(1.4426950408889634));
+    regs_from(p, l, ag, (const A*)nullptr, A(1));
+    const size_t row = (size_t)g.start + (size_t)k * seg;
+    const A* cr = in.C + row * p.ldc + (size_t)l.group * p.S;
+    const unsigned place = opaque(l.ch * (unsigned)sizeof(T));
+    T dn[U], en[U], gn[U];
+    auto fetch = [&](unsigned left) {            // the U rows in front of row + left (segments are multiples of 16 rows)
+#pragma unroll
+        for (unsigned i = 0; i < U; ++i) {
+            const size_t at = row + left - 1u - i;
+            dn[i] = lane_load(in.dt + at * p.lddt, place);
+            en[i] = lane_load(in.dY + at * lddy, place);
+            if (in.gate) gn[i] = lane_load(in.gate + at * p.ldg, place);
+        }
+    };
+    fetch(seg);
+    load_row<A, LG == 64, NS, FULL>(c, cr + (size_t)(seg - 1u) * p.ldc, p.S);
+    for (unsigned left = seg; left > 0; left -= U) {
+        A d[U], e[U];
+#pragma unroll
+        for (unsigned i = 0; i < U; ++i) {
+            A slope;
+            d[i] = step_of(p, (A)dn[i] + bi, slope);
+            e[i] = (A)en[i];
+            if (in.gate) { const A gg = (A)gn[i]; e[i] *= gg * sigmoid_of(gg); }
+        }
+        if (left > U) fetch(left - U);
+#pragma unroll
+        for (unsigned i = 0; i < U; ++i) {
+#pragma unroll
+            for (int j = 0; j < NS; ++j) ag[j] = exp2_fast(d[i] * a2[j]) * fma_a(c[j], e[i], ag[j]);
+            steps += d[i];
+            __builtin_amdgcn_sched_barrier(0);
+            const unsigned next = left - 1u - i;
+            load_row<A, LG == 64, NS, FULL>(c, cr + (size_t)(next ? next - 1u : 0u) * p.ldc, p.S);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
-    A* o = part + (size_t)blockIdx.x * (p.S + 2u) * p.D;
-    states_to(p, l, lane, da, o);
-    if (l.active) {
-        o[(size_t)p.S * p.D + l.ch] = dskip;
-        o[(size_t)(p.S + 1u) * p.D + l.ch] = dbias;
+    regs_to(p, l, ag, local + (size_t)blockIdx.x * p.S * p.D);
+    if (l.active) sums[(size_t)blockIdx.x * p.D + l.ch] = steps;
+}
+
+// carry[slot of segment k]: what segment k >= 1 of a cut region sends to the one before it; the last segment's is there.
+template <typename A>
+__global__ __launch_bounds__(256) void k_scan_carry_back(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const A* __restrict__ A_,
+                                                         const A* __restrict__ local, const A* __restrict__ sums, A* __restrict__ carry)
+{
+    constexpr unsigned U = 8;
+    const row_range g = region_rows(regions, blockIdx.x, p.N);
+    const size_t block = (size_t)p.S * p.D, at = (size_t)blockIdx.y * 256u + threadIdx.x;
+    if (!is_cut(g, seg) || at >= block) return;
+    const size_t ch = at % p.D, zero = g.start / seg;
+    const unsigned n = (g.end - g.start - 1u) / seg;             // the last segment
+    const A a2 = A_[at] * A(1.4426950408889634);
+    A s = carry[(zero + n) * block + at];
+    for (unsigned k = n - 1u; k > 0;) {
+        A add[U], sum[U];
+#pragma unroll
+        for (unsigned i = 0; i < U; ++i) {
+            const size_t slot = zero + (k > i ? k - i : 1u);
+            add[i] = local[slot * block + at];
+            sum[i] = sums[slot * p.D + ch];
+        }
+#pragma unroll
+        for (unsigned i = 0; i < U; ++i) {
+            if (!k) break;
+            s = fma_a(exp2_fast(a2 * sum[i]), s, add[i]);
+            carry[(zero + k) * block + at] = s;
+            --k;
+        }
     }
 }
 
-// dB and dC of a region's rows from the tiles' shares, in the tiles' order.
-template <typename A>
-__global__ __launch_bounds__(256) void k_scan_weights(const uint32_t* __restrict__ regions, unsigned N, unsigned tiles, size_t ncol, const A* __restrict__ share,
-                                                      size_t tile_stride, A* __restrict__ dB, size_t lddb, A* __restrict__ dC, size_t lddc)
+// The segments before the last one: the slot of segment k stands for segment k - 1, which takes in what segment k sends.
+template <typename T, int LG>
+__global__ __launch_bounds__(64, 2) void k_scan_bprop_cut(scan_shape p, scan_bshape bp, unsigned seg, unsigned nslot, unsigned unit0, scan_rows_in<T> in,
+                                                       const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ skip,
+                                                       const typename acc_of<T>::type* __restrict__ bias, scan_rows_out<T> to,
+                                                       scan_out<typename acc_of<T>::type> out, size_t tile_stride, typename acc_of<T>::type* __restrict__ part,
+                                                       const typename acc_of<T>::type* __restrict__ carry)
 {
-    const row_range g = region_rows(regions, blockIdx.x, N);
-    const size_t n = (size_t)(g.end - g.start) * 2u * ncol;
+    typedef typename acc_of<T>::type A;
+    extern __shared__ char lds_raw[];
+    scan_wave<T, LG> w(p, lds_raw, A_, skip, bias);
+    out = tile_share<LG>(p, out, tile_stride);
+    for (unsigned slot = blockIdx.x; slot < nslot; slot += gridDim.x) {
+        unsigned r, k;
+        row_range g;
+        if (!cut_segment(p, in.regions, in.marks, slot, seg, r, g, k)) continue;
+        // (a lane without a channel adds nothing to its group's sums: its e is zero, and so is what is sent to it)
+        states_from(p, w.l, w.lane, w.ag, w.l.active ? carry + (size_t)slot * p.S * p.D : (const A*)nullptr);
+        w.rows(p, bp, g.start, g.start + (k - 1u) * seg, seg, in, to, out);
+    }
+    w.leave(p, part + (size_t)(unit0 + blockIdx.x) * (p.S + 2u) * p.D);
+}
+
+// dB and dC from the tiles' shares, in the tiles' order: a region's rows (its first segment's where it is cut), or another segment's.
+template <typename A>
+__global__ __launch_bounds__(256) void k_scan_weights(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, unsigned tiles,
+                                                      size_t ncol, const A* __restrict__ share, size_t tile_stride, A* __restrict__ dB, size_t lddb, A* __restrict__ dC, size_t lddc)
+{
+    row_range g;
+    unsigned from;
+    if (blockIdx.x < p.nregion) {
+        g = region_rows(regions, blockIdx.x, p.N);
+        from = g.start;
+        if (marks && is_cut(g, seg)) g.end = g.start + seg;
+    } else {
+        unsigned r, k;
+        if (!cut_segment(p, regions, marks, blockIdx.x - p.nregion, seg, r, g, k)) return;
+        from = g.start + k * seg;
+        g.end = min(g.end, from + seg);
+    }
+    const size_t n = (size_t)(g.end - from) * 2u * ncol;
     for (size_t i = threadIdx.x; i < n; i += 256u) {
-        const size_t row = g.start + i / (2u * ncol), c = i % (2u * ncol);
+        const size_t row = from + i / (2u * ncol), c = i % (2u * ncol);
         A s = 0;
         for (unsigned t = 0; t < tiles; ++t) s += share[t * tile_stride + row * 2u * ncol + c];
         if (c < ncol) dB[row * lddb + c] = s;
@@ -268,26 +513,30 @@ __global__ __launch_bounds__(256) void k_scan_weights(const uint32_t* __restrict
 
 namespace {
 
-constexpr size_t SCAN_UNITS = 8192;              // waves that add up dA, over all tiles of channels
+constexpr size_t SCAN_UNITS = 4096;              // waves that add up dA, over all tiles of channels: four per SIMD that the chip has room for
+constexpr size_t SCAN_WAVES = 2048;              // waves that keep the vector units busy: two per SIMD, which 256 registers a lane allow
+constexpr size_t SCAN_LEAST = 32;                // rows of the shortest segment
 
-scan_plan plan_bprop(const dbk_statescan_args& a) { return plan_scan(a.N, a.D, a.G, 1, a.N + 1); }
-unsigned bprop_units(const dbk_statescan_args& a, const scan_plan& p)
+scan_plan plan_bprop(const dbk_statescan_args& a) { return plan_scan(a.N, a.D, a.G, SCAN_WAVES, SCAN_LEAST); }
+
+// Workspace: segments, tiles' shares of dB and dC (a group of several tiles), units' sums of dA, dD and dbias.
+struct bprop_layout { scan_segments seg; size_t share, part, bytes; unsigned units, slot_units; };
+bprop_layout layout_of(void* work, const dbk_statescan_args& a, const scan_plan& p)
 {
-    const size_t cap = SCAN_UNITS / p.tiles ? SCAN_UNITS / p.tiles : 1;
-    return (unsigned)(a.nregion < cap ? a.nregion : cap);
-}
-inline size_t share_bytes(const dbk_statescan_args& a, const scan_plan& p)
-{
-    return p.tpg > 1 ? (size_t)p.tpg * a.N * 2 * a.G * a.S * acc_size(a.dtype) : 0;
+    bprop_layout y;
+    const size_t e = acc_size(a.dtype), cap = SCAN_UNITS / p.tiles ? SCAN_UNITS / p.tiles : 1;
+    y.units = (unsigned)(a.nregion < cap ? a.nregion : cap);
+    y.slot_units = (unsigned)(p.slots < cap ? p.slots : cap);
+    y.seg = segments_in(work, a, p);
+    y.share = y.seg.bytes;
+    y.part = y.share + (p.tpg > 1 ? ((size_t)p.tpg * a.N * 2 * a.G * a.S * e + 15) / 16 * 16 : 0);
+    y.bytes = y.part + (size_t)(y.units + y.slot_units) * (a.S + 2) * a.D * e;
+    return y;
 }
 
 }  // namespace
 
-size_t bprop_work_bytes(const dbk_statescan_args& a)
-{
-    const scan_plan p = plan_bprop(a);
-    return share_bytes(a, p) + (size_t)bprop_units(a, p) * (a.S + 2) * a.D * acc_size(a.dtype);
-}
+size_t bprop_work_bytes(const dbk_statescan_args& a) { return layout_of(nullptr, a, plan_bprop(a)).bytes; }
 
 }  // namespace dbk
 
@@ -310,34 +559,44 @@ int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* a, void* 
         sum_partials(st, a->dtype, nullptr, 0, a->S * a->D, a->dA, a->D, a->dskip, a->D, a->ddt_bias);       // (sums of no rows: zeros)
         DBK_LAUNCH_OK();
     }
-    const size_t need = bprop_work_bytes(*a);
-    DBK_CHECK(work && work_bytes >= need, "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, need);
     const scan_plan p = plan_bprop(*a);
-    const unsigned units = bprop_units(*a, p);
+    const bprop_layout y = layout_of(work, *a, p);
+    DBK_CHECK(work && work_bytes >= y.bytes, "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, y.bytes);
+    DBK_CHECK(a->nregion + p.slots < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
     scan_shape s = shape_of(*a);
     s.tpg = p.tpg;
     const scan_bshape b = {a->lddy, a->lddx, a->ldddt, a->lddgate, a->lddb, a->lddc};
-    const size_t shares = share_bytes(*a, p), ncol = a->G * a->S;
-    void* part = (char*)work + shares;
+    const size_t ncol = a->G * a->S;
+    const bool shared = p.tpg > 1;
+    void* part = (char*)work + y.part;
+    if (p.slots) mark_cut_regions(st, a->regions, a->nregion, a->N, p.seg, y.seg.marks);
     with_row_type(a->dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
-        scan_out<A> out = {(A*)a->dB, (A*)a->dC, a->lddb, a->lddc};
-        size_t tile_stride = 0;
-        if (shares) {                            // a tile's share: (N, dB | dC)
-            out = {(A*)work, (A*)work + ncol, 2 * ncol, 2 * ncol};
-            tile_stride = a->N * 2 * ncol;
-        }
+        A* share = (A*)((char*)work + y.share);
+        const size_t tile_stride = shared ? a->N * 2 * ncol : 0;                // a tile's share: (N, dB | dC)
+        const scan_out<A> out = shared ? scan_out<A>{share, share + ncol, 2 * ncol, 2 * ncol} : scan_out<A>{(A*)a->dB, (A*)a->dC, a->lddb, a->lddc};
+        const scan_rows_in<T> in = {(const T*)a->X, (const T*)a->dt, (const T*)a->gate, (const T*)a->dY, (const A*)a->B, (const A*)a->C, (const A*)a->keep, a->regions, y.seg.marks};
+        const scan_rows_out<T> to = {(T*)a->dX, (T*)a->ddt, (T*)a->dgate};
+        const size_t quads = (a->S + 3) / 4, lds = quads * 64 * 2 * sizeof(quad<A>) + (2 * 64 + 2 * (64 / p.lanes) * quads * 4) * SCAN_CHUNK * sizeof(A);
         with_lanes(p.lanes, [&](auto lanes) {
-            const size_t lds = (a->S + 3) / 4 * 64 * 3 * sizeof(quad<A>) + 2 * SCAN_CHUNK * 64 * sizeof(A);
-            k_scan_bprop<T, lanes.value><<<dim3(units, p.tiles), 64, lds, st>>>(
-                s, b, a->regions, (const T*)a->X, (const T*)a->dt, (const A*)a->A, (const A*)a->B, (const A*)a->C, (const A*)a->skip, (const T*)a->gate, (const A*)a->dt_bias,
-                (const A*)a->keep, (const T*)a->dY, (T*)a->dX, (T*)a->ddt, (T*)a->dgate, out, tile_stride, (A*)part);
+            k_scan_bprop<T, lanes.value><<<dim3(y.units, p.tiles), 64, lds, st>>>(s, b, p.seg, in, (const A*)a->A, (const A*)a->skip, (const A*)a->dt_bias, to, out, tile_stride,
+                                                                                 (A*)part, (A*)y.seg.carry);
+            if (!p.slots) return;
+            with_states(a->S, [&](auto ns, auto full) {
+                k_scan_bprop_local<T, lanes.value, ns.value, full.value><<<dim3(p.slots, p.tiles), 64, 0, st>>>(s, b.lddy, p.seg, in, (const A*)a->A, (const A*)a->dt_bias,
+                                                                                                                (A*)y.seg.local, (A*)y.seg.steps);
+            });
+            k_scan_carry_back<A><<<dim3((unsigned)a->nregion, divup(a->S * a->D, 256)), 256, 0, st>>>(s, p.seg, a->regions, (const A*)a->A, (const A*)y.seg.local,
+                                                                                                (const A*)y.seg.steps, (A*)y.seg.carry);
+            k_scan_bprop_cut<T, lanes.value><<<dim3(y.slot_units, p.tiles), 64, lds, st>>>(s, b, p.seg, p.slots, y.units, in, (const A*)a->A, (const A*)a->skip, (const A*)a->dt_bias,
+                                                                                          to, out, tile_stride, (A*)part, (const A*)y.seg.carry);
         });
-        if (shares)
-            k_scan_weights<A><<<(unsigned)a->nregion, 256, 0, st>>>(a->regions, (unsigned)a->N, p.tpg, ncol, (const A*)work, tile_stride, (A*)a->dB, a->lddb, (A*)a->dC, a->lddc);
+        if (shared)
+            k_scan_weights<A><<<(unsigned)a->nregion + p.slots, 256, 0, st>>>(s, p.seg, a->regions, y.seg.marks, p.tpg, ncol, share, tile_stride, (A*)a->dB, a->lddb, (A*)a->dC,
+                                                                              a->lddc);
     });
-    sum_partials(st, a->dtype, part, units, a->S * a->D, a->dA, a->D, a->dskip, a->D, a->ddt_bias);
+    sum_partials(st, a->dtype, part, y.units + y.slot_units, a->S * a->D, a->dA, a->D, a->dskip, a->D, a->ddt_bias);
     DBK_LAUNCH_OK();
 }
 
