@@ -8,8 +8,8 @@
 //   g[t] = C e + a[t+1] g[t+1],  dx = d (B . g) + D e,  dd = x (B . g) + sum_s g a h[t-1] A,  dA = sum_t g a h[t-1] d,
 //   dB = sum over the group's channels of g d x,  dC = the same of e h,  dD = sum_t e x,  ddt = dd sigmoid(dt + bias),  dbias = sum_t ddt
 //
-// A lane is a channel and a workgroup one wave: B and C are then the same for a whole wave whose channels are of one group, and come as scalar
-// operands. States are float32 (double for double rows).
+// A lane is a channel and a wave a tile of 64 channels, which walks down a region's rows with the states in registers; B and C, which the lanes of a
+// group share, come through LDS. States are float32 (double for double rows).
 #pragma once
 #include <type_traits>
 #include "rows_common.h"
@@ -20,7 +20,7 @@ constexpr unsigned SCAN_CHUNK = 16;              // rows between two kept states
 
 struct scan_shape {
     unsigned N, D, S, G, gs, nregion;            // rows, channels, states, groups, channels per group, regions
-    unsigned tpg, softplus;                      // waves' tiles per group (64 lanes per group), or 0: several groups per wave
+    unsigned tpg, tiles, softplus;               // waves' tiles per group (64 lanes per group), or 0: several groups per wave; all tiles
     size_t ldx, lddt, ldb, ldc, ldg, ldy;
 };
 
@@ -61,17 +61,53 @@ template <typename A> __device__ __forceinline__ A step_of(const scan_shape& p, 
     return raw;
 }
 
-// Weights of all states of one row, zero from state S on. FULL: S == NS.
-template <typename A, bool UNIFORM, int NS, bool FULL> __device__ __forceinline__ void load_row(A (&v)[NS], const A* p, unsigned S)
-{
-    typedef const __attribute__((address_space(4))) A* uniform_ptr;
+template <typename A> struct quad { A v[4]; } __attribute__((aligned(16)));
+
+// The first of the groups that a wave's tile covers.
+template <int LG> __device__ __forceinline__ unsigned first_group(const scan_shape& p, unsigned tile) { return LG == 64 ? tile / p.tpg : tile * (64u / LG); }
+
+// Weights of SCAN_AHEAD rows for a wave: fetched from memory into registers, a few per lane, put into LDS and read from there by the lanes of
+// each group: [row][B, C][group of the wave][state], zeros from state S on. They could come as scalar operands where a wave's
+// channels are of one group, but a scalar load can not run far enough ahead of the rows: there are not the registers.
+constexpr int SCAN_AHEAD = 4;
+template <typename A, int LG, int NS, bool WITH_B, bool WITH_C> struct scan_weights {
+    static constexpr int GW = 64 / LG, PART = GW * NS, ROW = PART * (WITH_B + WITH_C), SIZE = SCAN_AHEAD * ROW, PER = (SIZE + 63) / 64;
+    const A *from[PER];
+    size_t ld[PER];
+    unsigned row[PER];
+    bool here[PER];
+    A next[PER];
+    A *lds, *mine;
+    unsigned lane;
+    __device__ __forceinline__ scan_weights(const scan_shape& p, unsigned lane_, unsigned first, const A* B, const A* C, A* lds_)
+        : lds(lds_), mine(lds_ + lane_ / LG * NS), lane(lane_)
+    {
 #pragma unroll
-    for (int j = 0; j < NS; ++j) {
-        const unsigned at = FULL ? j : min((unsigned)j, S - 1u);               // (in bounds whatever S is)
-        const A x = UNIFORM ? ((uniform_ptr)(uintptr_t)p)[at] : p[at];
-        v[j] = FULL || j < (int)S ? x : A(0);
+        for (int i = 0; i < PER; ++i) {
+            const unsigned at = lane + 64u * i, in = at % ROW, g = in % PART / NS, s = in % NS;
+            const bool c = WITH_C && in >= (WITH_B ? PART : 0);
+            row[i] = at / ROW;
+            here[i] = at < SIZE && s < p.S && first + g < p.G;
+            from[i] = (c ? C : B) + (here[i] ? (size_t)(first + g) * p.S + s : 0);
+            ld[i] = c ? p.ldc : p.ldb;
+        }
     }
-}
+    // rows t, t + 1, ... of n (the last one again behind it)
+    __device__ __forceinline__ void fetch(const scan_shape& p, unsigned t, unsigned n)
+    {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) next[i] = here[i] ? from[i][min(t + row[i], n - 1u) * ld[i]] : A(0);
+    }
+    __device__ __forceinline__ void put()
+    {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) if (SIZE % 64 == 0 || lane + 64u * i < SIZE) lds[lane + 64 * i] = next[i];
+        __builtin_amdgcn_wave_barrier();         // (one wave: LDS keeps its order)
+    }
+    __device__ __forceinline__ quad<A> b(int r, int q) const { return *(const quad<A>*)(mine + r * ROW + q); }
+    __device__ __forceinline__ quad<A> c(int r, int q) const { return *(const quad<A>*)(mine + r * ROW + (WITH_B ? PART : 0) + q); }
+};
+
 // the states of a lane's channel between registers and (S, D) memory; null: zeros
 template <typename A, int NS> __device__ __forceinline__ void regs_from(const scan_shape& p, const scan_lane& l, A (&h)[NS], const A* from, A scale)
 {
@@ -119,7 +155,7 @@ inline scan_shape shape_of(const dbk_statescan_args& a)
 {
     scan_shape s;
     s.N = (unsigned)a.N; s.D = (unsigned)a.D; s.S = (unsigned)a.S; s.G = (unsigned)a.G; s.gs = (unsigned)(a.D / a.G); s.nregion = (unsigned)a.nregion;
-    s.tpg = 0; s.softplus = a.softplus != 0;
+    s.tpg = s.tiles = 0; s.softplus = a.softplus != 0;
     s.ldx = a.ldx; s.lddt = a.lddt; s.ldb = a.ldb; s.ldc = a.ldc; s.ldg = a.ldgate; s.ldy = a.ldy;
     return s;
 }
@@ -131,15 +167,14 @@ template <typename F> void with_lanes(int lanes, F f)
     else f(std::integral_constant<int, 64>());
 }
 
-// Registers for the states, and whether all of them hold one: 16 states have a form of their own without padding.
+// Registers for the states.
 template <typename F> void with_states(size_t S, F f)
 {
-    if (S == 16) f(std::integral_constant<int, 16>(), std::true_type());
-    else if (S <= 4) f(std::integral_constant<int, 4>(), std::false_type());
-    else if (S <= 8) f(std::integral_constant<int, 8>(), std::false_type());
-    else if (S <= 16) f(std::integral_constant<int, 16>(), std::false_type());
-    else if (S <= 32) f(std::integral_constant<int, 32>(), std::false_type());
-    else f(std::integral_constant<int, 64>(), std::false_type());
+    if (S <= 4) f(std::integral_constant<int, 4>());
+    else if (S <= 8) f(std::integral_constant<int, 8>());
+    else if (S <= 16) f(std::integral_constant<int, 16>());
+    else if (S <= 32) f(std::integral_constant<int, 32>());
+    else f(std::integral_constant<int, 64>());
 }
 
 inline int check_scan(const dbk_statescan_args* a)

@@ -5,17 +5,20 @@ namespace dbk {
 
 // n rows from `row` on, the states in registers. OUT: the rows of Y are written; otherwise only the states move on, and `steps` adds up d.
 // kept: null, or the block of states in front of the first row's chunk of 16; those in front of the next ones are written behind it.
-template <typename T, int LG, int NS, bool FULL, bool OUT>
-__device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& l, size_t row, unsigned n, const T* X, const T* dt, const T* gate,
+// What four rows need comes from memory while the four before them are worked on; their weights then lie in the wave's `lds`.
+template <typename T, int LG, int NS, bool OUT>
+__device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& l, unsigned lane, unsigned first, size_t row, unsigned n, const T* X, const T* dt, const T* gate,
                                           const typename acc_of<T>::type* B, const typename acc_of<T>::type* C, typename acc_of<T>::type skip,
                                           typename acc_of<T>::type bias, typename acc_of<T>::type (&h)[NS], const typename acc_of<T>::type (&k)[NS],
-                                          T* Y, typename acc_of<T>::type* kept, typename acc_of<T>::type& steps)
+                                          T* Y, typename acc_of<T>::type* kept, typename acc_of<T>::type& steps, typename acc_of<T>::type* lds)
 {
     typedef typename acc_of<T>::type A;
-    constexpr int U = 4;                         // rows whose x, dt and gate are fetched together, a step ahead
+    constexpr int U = SCAN_AHEAD;
+    typedef scan_weights<A, LG, NS, true, OUT> weights;
     if (!n) return;
     const unsigned at = opaque(l.ch * (unsigned)sizeof(T));
     T xn[U], dn[U], gn[U];
+    weights w(p, lane, first, B + row * p.ldb, C + row * p.ldc, lds);
     auto fetch = [&](unsigned t) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
@@ -24,12 +27,8 @@ __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& 
             dn[i] = lane_load(dt + r * p.lddt, at);
             if (OUT && gate) gn[i] = lane_load(gate + r * p.ldg, at);
         }
+        w.fetch(p, t, n);
     };
-    const A *br = B + row * p.ldb + (size_t)l.group * p.S, *cr = C + row * p.ldc + (size_t)l.group * p.S;
-    // A row's C is fetched before its states are worked on and the next row's B before its y is: one of the two is on its way
-    // all the time, and 2 NS scalar registers do.
-    A b[NS], c[NS];
-    load_row<A, LG == 64, NS, FULL>(b, br, p.S);
     fetch(0);
     for (unsigned t = 0; t < n; t += U) {
         A d[U], x[U];
@@ -41,37 +40,40 @@ __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& 
             d[i] = step_of(p, (A)dn[i] + bias, slope);
             g[i] = gn[i];
         }
+        w.put();
         if (t + U < n) fetch(t + U);
         if (OUT && kept && t && t % SCAN_CHUNK == 0) regs_to(p, l, h, kept + (size_t)(t / SCAN_CHUNK) * p.S * p.D);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             if (t + i >= n) break;
-            if (OUT) load_row<A, LG == 64, NS, FULL>(c, cr + (size_t)(t + i) * p.ldc, p.S);
-            __builtin_amdgcn_sched_barrier(0);   // (or the compiler gathers many rows' weights and spills them)
             const A in = d[i] * x[i];
+            A y[4] = {skip * x[i], A(0), A(0), A(0)};
 #pragma unroll
-            for (int j = 0; j < NS; ++j) h[j] = fma_a(exp2_fast(d[i] * k[j]), h[j], in * b[j]);
-            __builtin_amdgcn_sched_barrier(0);
-            load_row<A, LG == 64, NS, FULL>(b, br + (size_t)min(t + i + 1u, n - 1u) * p.ldb, p.S);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int q = 0; q < NS; q += 4) {
+                const quad<A> b = w.b(i, q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) h[q + j] = fma_a(exp2_fast(d[i] * k[q + j]), h[q + j], in * b.v[j]);
+                if (OUT) {
+                    const quad<A> c = w.c(i, q);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[j] = fma_a(c.v[j], h[q + j], y[j]);
+                }
+            }
             if (OUT) {
-                A y[4] = {skip * x[i], A(0), A(0), A(0)};
-#pragma unroll
-                for (int j = 0; j < NS; ++j) y[j & 3] = fma_a(c[j], h[j], y[j & 3]);
                 A out = (y[0] + y[1]) + (y[2] + y[3]);
                 if (gate) { const A gg = (A)g[i]; out *= gg * sigmoid_of(gg); }
                 if (l.active) lane_store(Y + (row + t + i) * p.ldy, at, (T)out);
             } else
                 steps += d[i];
-            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);   // (a row's work stays together: its operands would fill the registers with those of others)
         }
     }
 }
 
 // Blocks below nregion: a region, all of it or its first segment (the state behind which is carried to the second one); the
 // others: what a segment makes of a zero state, where another one follows.
-template <typename T, int LG, int NS, bool FULL>
-__global__ __launch_bounds__(64) void k_scan_fprop(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
+template <typename T, int LG, int NS>
+__global__ __launch_bounds__(256) void k_scan_fprop(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
                                                    const T* __restrict__ X, const T* __restrict__ dt,
                                                    const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ B,
                                                    const typename acc_of<T>::type* __restrict__ C, const typename acc_of<T>::type* __restrict__ skip,
@@ -82,7 +84,12 @@ __global__ __launch_bounds__(64) void k_scan_fprop(scan_shape p, unsigned seg, c
                                                    typename acc_of<T>::type* __restrict__ carry)
 {
     typedef typename acc_of<T>::type A;
-    const scan_lane l = lane_channel<LG>(p, blockIdx.y, threadIdx.x);
+    const unsigned tile = blockIdx.y * blockDim.y + uniform(threadIdx.y);
+    if (tile >= p.tiles) return;
+    __shared__ A lds_all[4][scan_weights<A, LG, NS, true, true>::SIZE];
+    A* lds = lds_all[uniform(threadIdx.y)];
+    const scan_lane l = lane_channel<LG>(p, tile, threadIdx.x);
+    const unsigned first = first_group<LG>(p, tile);
     const size_t block = (size_t)p.S * p.D;
     const A sk = skip ? skip[l.ch] : A(0), bi = bias ? bias[l.ch] : A(0);
     A h[NS], a2[NS], steps = 0;
@@ -92,8 +99,8 @@ __global__ __launch_bounds__(64) void k_scan_fprop(scan_shape p, unsigned seg, c
         const bool cut = marks && is_cut(g, seg);
         regs_from(p, l, a2, A_, A(1.4426950408889634));
         regs_from(p, l, h, state ? state + (size_t)r * block : (const A*)nullptr, A(1));
-        scan_rows<T, LG, NS, FULL, true>(p, l, g.start, cut ? seg : g.end - g.start, X, dt, gate, B, C, sk, bi, h, a2, Y,
-                                         keep ? kept_at(p, keep, g.start, 0u) : (A*)nullptr, steps);
+        scan_rows<T, LG, NS, true>(p, l, threadIdx.x, first, g.start, cut ? seg : g.end - g.start, X, dt, gate, B, C, sk, bi, h, a2, Y,
+                                         keep ? kept_at(p, keep, g.start, 0u) : (A*)nullptr, steps, lds);
         if (cut) regs_to(p, l, h, carry + (size_t)(g.start / seg + 1u) * block);
         else if (last) regs_to(p, l, h, last + (size_t)r * block);
         return;
@@ -104,7 +111,7 @@ __global__ __launch_bounds__(64) void k_scan_fprop(scan_shape p, unsigned seg, c
     if (!cut_segment(p, regions, marks, slot, seg, r, g, k) || g.start + (uint64_t)(k + 1u) * seg >= g.end) return;
     regs_from(p, l, a2, A_, A(1.4426950408889634));
     regs_from(p, l, h, (const A*)nullptr, A(1));
-    scan_rows<T, LG, NS, FULL, false>(p, l, (size_t)g.start + (size_t)k * seg, seg, X, dt, gate, B, C, sk, bi, h, a2, Y, (A*)nullptr, steps);
+    scan_rows<T, LG, NS, false>(p, l, threadIdx.x, first, (size_t)g.start + (size_t)k * seg, seg, X, dt, gate, B, C, sk, bi, h, a2, Y, (A*)nullptr, steps, lds);
     regs_to(p, l, h, local + (size_t)slot * block);
     if (l.active) sums[(size_t)slot * p.D + l.ch] = steps;
 }
@@ -141,8 +148,8 @@ __global__ __launch_bounds__(256) void k_scan_carry(scan_shape p, unsigned seg, 
 }
 
 // The rows of every segment behind the first, from the state carried to it.
-template <typename T, int LG, int NS, bool FULL>
-__global__ __launch_bounds__(64) void k_scan_fprop_cut(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
+template <typename T, int LG, int NS>
+__global__ __launch_bounds__(256) void k_scan_fprop_cut(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
                                                        const T* __restrict__ X, const T* __restrict__ dt,
                                                        const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ B,
                                                        const typename acc_of<T>::type* __restrict__ C, const typename acc_of<T>::type* __restrict__ skip,
@@ -154,7 +161,12 @@ __global__ __launch_bounds__(64) void k_scan_fprop_cut(scan_shape p, unsigned se
     unsigned r, k;
     row_range g;
     if (!cut_segment(p, regions, marks, blockIdx.x, seg, r, g, k)) return;
-    const scan_lane l = lane_channel<LG>(p, blockIdx.y, threadIdx.x);
+    const unsigned tile = blockIdx.y * blockDim.y + uniform(threadIdx.y);
+    if (tile >= p.tiles) return;
+    __shared__ A lds_all[4][scan_weights<A, LG, NS, true, true>::SIZE];
+    A* lds = lds_all[uniform(threadIdx.y)];
+    const scan_lane l = lane_channel<LG>(p, tile, threadIdx.x);
+    const unsigned first = first_group<LG>(p, tile);
     const size_t block = (size_t)p.S * p.D;
     const A sk = skip ? skip[l.ch] : A(0), bi = bias ? bias[l.ch] : A(0);
     A h[NS], a2[NS], steps = 0, *kept = keep ? kept_at(p, keep, g.start, k * (seg / SCAN_CHUNK)) : (A*)nullptr;
@@ -162,7 +174,7 @@ __global__ __launch_bounds__(64) void k_scan_fprop_cut(scan_shape p, unsigned se
     regs_from(p, l, h, carry + (size_t)blockIdx.x * block, A(1));
     if (kept) regs_to(p, l, h, kept);
     const unsigned row = g.start + k * seg;
-    scan_rows<T, LG, NS, FULL, true>(p, l, row, min(seg, g.end - row), X, dt, gate, B, C, sk, bi, h, a2, Y, kept, steps);
+    scan_rows<T, LG, NS, true>(p, l, threadIdx.x, first, row, min(seg, g.end - row), X, dt, gate, B, C, sk, bi, h, a2, Y, kept, steps, lds);
     if (last && g.end - row <= seg) regs_to(p, l, h, last + (size_t)r * block);
 }
 
@@ -257,20 +269,22 @@ int dbk_statescan(dbk_stream_t stream, const dbk_statescan_args* a, void* work, 
     DBK_CHECK(a->nregion + p.slots < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
     scan_shape s = shape_of(*a);
     s.tpg = p.tpg;
+    s.tiles = p.tiles;
     hipStream_t st = as_stream(stream);
+    const unsigned waves = p.tpg < 4 ? (p.tpg ? p.tpg : 1u) : 4u;
     if (p.slots) mark_cut_regions(st, a->regions, a->nregion, a->N, p.seg, g.marks);
     with_row_type(a->dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
         with_lanes(p.lanes, [&](auto lanes) {
-            with_states(a->S, [&](auto ns, auto full) {
-                k_scan_fprop<T, lanes.value, ns.value, full.value><<<dim3((unsigned)a->nregion + p.slots, p.tiles), 64, 0, st>>>(
+            with_states(a->S, [&](auto ns) {
+                k_scan_fprop<T, lanes.value, ns.value><<<dim3((unsigned)a->nregion + p.slots, divup(p.tiles, waves)), dim3(64, waves), 0, st>>>(
                     s, p.seg, a->regions, g.marks, (const T*)a->X, (const T*)a->dt, (const A*)a->A, (const A*)a->B, (const A*)a->C, (const A*)a->skip, (const T*)a->gate,
                     (const A*)a->dt_bias, (const A*)a->state, (T*)a->Y, (A*)a->last, (A*)a->keep, (A*)g.local, (A*)g.steps, (A*)g.carry);
                 if (!p.slots) return;
                 k_scan_carry<A><<<dim3((unsigned)a->nregion, divup(a->S * a->D, 256)), 256, 0, st>>>(s, p.seg, a->regions, (const A*)a->A, (const A*)g.local, (const A*)g.steps,
                                                                                               (A*)g.carry);
-                k_scan_fprop_cut<T, lanes.value, ns.value, full.value><<<dim3(p.slots, p.tiles), 64, 0, st>>>(
+                k_scan_fprop_cut<T, lanes.value, ns.value><<<dim3(p.slots, divup(p.tiles, waves)), dim3(64, waves), 0, st>>>(
                     s, p.seg, a->regions, g.marks, (const T*)a->X, (const T*)a->dt, (const A*)a->A, (const A*)a->B, (const A*)a->C, (const A*)a->skip, (const T*)a->gate,
                     (const A*)a->dt_bias, (T*)a->Y, (A*)a->last, (A*)a->keep, (const A*)g.carry);
             });

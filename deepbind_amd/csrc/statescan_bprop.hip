@@ -3,8 +3,6 @@
 
 namespace dbk {
 
-template <typename A> struct quad { A v[4]; } __attribute__((aligned(16)));
-
 template <typename A> __device__ __forceinline__ void states_to(const scan_shape& p, const scan_lane& l, unsigned lane, const quad<A>* h, A* to)
 {
     if (!l.active) return;
@@ -375,36 +373,38 @@ __global__ __launch_bounds__(64, 2) void k_scan_bprop(scan_shape p, scan_bshape 
 }
 
 // What a middle segment sends back when nothing is sent to it, and the sum of its steps: the states' gradients alone.
-template <typename T, int LG, int NS, bool FULL>
+template <typename T, int LG, int NS>
 __global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t lddy, unsigned seg, scan_rows_in<T> in, const typename acc_of<T>::type* __restrict__ A_,
                                                          const typename acc_of<T>::type* __restrict__ bias, typename acc_of<T>::type* __restrict__ local,
                                                          typename acc_of<T>::type* __restrict__ sums)
 {
     typedef typename acc_of<T>::type A;
-    constexpr unsigned U = 4;
+    typedef scan_weights<A, LG, NS, false, true> weights;
+    constexpr unsigned U = SCAN_AHEAD;
+    __shared__ A lds[weights::SIZE];
     unsigned r, k;
     row_range g;
     if (!cut_segment(p, in.regions, in.marks, blockIdx.x, seg, r, g, k) || g.start + (uint64_t)(k + 1u) * seg >= g.end) return;
     const scan_lane l = lane_channel<LG>(p, blockIdx.y, threadIdx.x);
     const A bi = bias ? bias[l.ch] : A(0);
-    A a2[NS], ag[NS], c[NS], steps = 0;
+    A a2[NS], ag[NS], steps = 0;
     regs_from(p, l, a2, A_, A(1.4426950408889634));
     regs_from(p, l, ag, (const A*)nullptr, A(1));
     const size_t row = (size_t)g.start + (size_t)k * seg;
-    const A* cr = in.C + row * p.ldc + (size_t)l.group * p.S;
     const unsigned place = opaque(l.ch * (unsigned)sizeof(T));
+    weights w(p, threadIdx.x, first_group<LG>(p, blockIdx.y), (const A*)nullptr, in.C + row * p.ldc, lds);
     T dn[U], en[U], gn[U];
-    auto fetch = [&](unsigned left) {            // the U rows in front of row + left (segments are multiples of 16 rows)
+    auto fetch = [&](unsigned t) {               // rows t .. t + U - 1 of the segment (a multiple of 16 rows)
 #pragma unroll
         for (unsigned i = 0; i < U; ++i) {
-            const size_t at = row + left - 1u - i;
+            const size_t at = row + t + i;
             dn[i] = lane_load(in.dt + at * p.lddt, place);
             en[i] = lane_load(in.dY + at * lddy, place);
             if (in.gate) gn[i] = lane_load(in.gate + at * p.ldg, place);
         }
+        w.fetch(p, t, seg);
     };
-    fetch(seg);
-    load_row<A, LG == 64, NS, FULL>(c, cr + (size_t)(seg - 1u) * p.ldc, p.S);
+    fetch(seg - U);
     for (unsigned left = seg; left > 0; left -= U) {
         A d[U], e[U];
 #pragma unroll
@@ -414,15 +414,17 @@ __global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t ld
             e[i] = (A)en[i];
             if (in.gate) { const A gg = (A)gn[i]; e[i] *= gg * sigmoid_of(gg); }
         }
-        if (left > U) fetch(left - U);
+        w.put();
+        if (left > U) fetch(left - 2u * U);
 #pragma unroll
-        for (unsigned i = 0; i < U; ++i) {
+        for (int i = U - 1; i >= 0; --i) {
 #pragma unroll
-            for (int j = 0; j < NS; ++j) ag[j] = exp2_fast(d[i] * a2[j]) * fma_a(c[j], e[i], ag[j]);
+            for (int q = 0; q < NS; q += 4) {
+                const quad<A> c = w.c(i, q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) ag[q + j] = exp2_fast(d[i] * a2[q + j]) * fma_a(c.v[j], e[i], ag[q + j]);
+            }
             steps += d[i];
-            __builtin_amdgcn_sched_barrier(0);
-            const unsigned next = left - 1u - i;
-            load_row<A, LG == 64, NS, FULL>(c, cr + (size_t)(next ? next - 1u : 0u) * p.ldc, p.S);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -565,6 +567,7 @@ int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* a, void* 
     DBK_CHECK(a->nregion + p.slots < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
     scan_shape s = shape_of(*a);
     s.tpg = p.tpg;
+    s.tiles = p.tiles;
     const scan_bshape b = {a->lddy, a->lddx, a->ldddt, a->lddgate, a->lddb, a->lddc};
     const size_t ncol = a->G * a->S;
     const bool shared = p.tpg > 1;
@@ -583,8 +586,8 @@ int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* a, void* 
             k_scan_bprop<T, lanes.value><<<dim3(y.units, p.tiles), 64, lds, st>>>(s, b, p.seg, in, (const A*)a->A, (const A*)a->skip, (const A*)a->dt_bias, to, out, tile_stride,
                                                                                  (A*)part, (A*)y.seg.carry);
             if (!p.slots) return;
-            with_states(a->S, [&](auto ns, auto full) {
-                k_scan_bprop_local<T, lanes.value, ns.value, full.value><<<dim3(p.slots, p.tiles), 64, 0, st>>>(s, b.lddy, p.seg, in, (const A*)a->A, (const A*)a->dt_bias,
+            with_states(a->S, [&](auto ns) {
+                k_scan_bprop_local<T, lanes.value, ns.value><<<dim3(p.slots, p.tiles), 64, 0, st>>>(s, b.lddy, p.seg, in, (const A*)a->A, (const A*)a->dt_bias,
                                                                                                                 (A*)y.seg.local, (A*)y.seg.steps);
             });
             k_scan_carry_back<A><<<dim3((unsigned)a->nregion, divup(a->S * a->D, 256)), 256, 0, st>>>(s, p.seg, a->regions, (const A*)a->A, (const A*)y.seg.local,
