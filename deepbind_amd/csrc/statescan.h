@@ -66,37 +66,40 @@ template <typename A> struct quad { A v[4]; } __attribute__((aligned(16)));
 // The first of the groups that a wave's tile covers.
 template <int LG> __device__ __forceinline__ unsigned first_group(const scan_shape& p, unsigned tile) { return LG == 64 ? tile / p.tpg : tile * (64u / LG); }
 
-// Weights of SCAN_AHEAD rows for a wave: fetched from memory into registers, a few per lane, put into LDS and read from there by the lanes of
+// Weights of two rows for a wave: fetched from memory into registers, a few per lane, put into LDS and read from there by the lanes of
 // each group: [row][B, C][group of the wave][state], zeros from state S on. They could come as scalar operands where a wave's
 // channels are of one group, but a scalar load can not run far enough ahead of the rows: there are not the registers.
-constexpr int SCAN_AHEAD = 4;
+constexpr int SCAN_AHEAD = 2;
 template <typename A, int LG, int NS, bool WITH_B, bool WITH_C> struct scan_weights {
     static constexpr int GW = 64 / LG, PART = GW * NS, ROW = PART * (WITH_B + WITH_C), SIZE = SCAN_AHEAD * ROW, PER = (SIZE + 63) / 64;
     const A *from[PER];
-    size_t ld[PER];
-    unsigned row[PER];
+    size_t step[PER];
     bool here[PER];
     A next[PER];
     A *lds, *mine;
     unsigned lane;
-    __device__ __forceinline__ scan_weights(const scan_shape& p, unsigned lane_, unsigned first, const A* B, const A* C, A* lds_)
-        : lds(lds_), mine(lds_ + lane_ / LG * NS), lane(lane_)
+    // B and C at row `first_row` of the rows; back: from there towards the rows in front
+    __device__ __forceinline__ scan_weights(const scan_shape& p, unsigned lane_, unsigned first, const A* B, const A* C, A* lds_, unsigned first_row, bool back)
+        : lds(lds_), mine(lds_ + lane_ / LG * NS), lane(lane_ & 63u)
     {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const unsigned at = lane + 64u * i, in = at % ROW, g = in % PART / NS, s = in % NS;
             const bool c = WITH_C && in >= (WITH_B ? PART : 0);
-            row[i] = at / ROW;
+            const size_t ld = c ? p.ldc : p.ldb;
             here[i] = at < SIZE && s < p.S && first + g < p.G;
-            from[i] = (c ? C : B) + (here[i] ? (size_t)(first + g) * p.S + s : 0);
-            ld[i] = c ? p.ldc : p.ldb;
+            from[i] = (c ? C : B) + (here[i] ? (first_row + at / ROW) * ld + (size_t)(first + g) * p.S + s : 0);
+            step[i] = back ? 0 - SCAN_AHEAD * ld : SCAN_AHEAD * ld;
         }
     }
-    // rows t, t + 1, ... of n (the last one again behind it)
-    __device__ __forceinline__ void fetch(const scan_shape& p, unsigned t, unsigned n)
+    // the next SCAN_AHEAD rows, of which `left` exist
+    __device__ __forceinline__ void fetch(unsigned left)
     {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) next[i] = here[i] ? from[i][min(t + row[i], n - 1u) * ld[i]] : A(0);
+        for (int i = 0; i < PER; ++i) {
+            next[i] = here[i] && (lane + 64u * i) / ROW < left ? *from[i] : A(0);
+            from[i] += step[i];
+        }
     }
     __device__ __forceinline__ void put()
     {

@@ -5,7 +5,7 @@ namespace dbk {
 
 // n rows from `row` on, the states in registers. OUT: the rows of Y are written; otherwise only the states move on, and `steps` adds up d.
 // kept: null, or the block of states in front of the first row's chunk of 16; those in front of the next ones are written behind it.
-// What four rows need comes from memory while the four before them are worked on; their weights then lie in the wave's `lds`.
+// What two rows need comes from memory while the two before them are worked on; their weights then lie in the wave's `lds`.
 template <typename T, int LG, int NS, bool OUT>
 __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& l, unsigned lane, unsigned first, size_t row, unsigned n, const T* X, const T* dt, const T* gate,
                                           const typename acc_of<T>::type* B, const typename acc_of<T>::type* C, typename acc_of<T>::type skip,
@@ -18,18 +18,23 @@ __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& 
     if (!n) return;
     const unsigned at = opaque(l.ch * (unsigned)sizeof(T));
     T xn[U], dn[U], gn[U];
-    weights w(p, lane, first, B + row * p.ldb, C + row * p.ldc, lds);
-    auto fetch = [&](unsigned t) {
+    weights w(p, lane, first, B + row * p.ldb, C + row * p.ldc, lds, 0u, false);
+    const T *xp = X + row * p.ldx, *dp = dt + row * p.lddt, *gp = gate + row * p.ldg;
+    T* yp = Y + row * p.ldy;
+    auto fetch = [&](unsigned left) {            // (a row behind the last one: the last one again)
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const size_t r = row + min(t + i, n - 1u);
-            xn[i] = lane_load(X + r * p.ldx, at);
-            dn[i] = lane_load(dt + r * p.lddt, at);
-            if (OUT && gate) gn[i] = lane_load(gate + r * p.ldg, at);
+            xn[i] = lane_load(xp, at);
+            dn[i] = lane_load(dp, at);
+            if (OUT && gate) gn[i] = lane_load(gp, at);
+            const bool more = i + 1u < left;
+            xp += more ? p.ldx : 0;
+            dp += more ? p.lddt : 0;
+            gp += more ? p.ldg : 0;
         }
-        w.fetch(p, t, n);
+        w.fetch(left);
     };
-    fetch(0);
+    fetch(n);
     for (unsigned t = 0; t < n; t += U) {
         A d[U], x[U];
         T g[U];
@@ -41,7 +46,7 @@ __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& 
             g[i] = gn[i];
         }
         w.put();
-        if (t + U < n) fetch(t + U);
+        if (t + U < n) fetch(n - t - U);
         if (OUT && kept && t && t % SCAN_CHUNK == 0) regs_to(p, l, h, kept + (size_t)(t / SCAN_CHUNK) * p.S * p.D);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
@@ -62,7 +67,8 @@ __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& 
             if (OUT) {
                 A out = (y[0] + y[1]) + (y[2] + y[3]);
                 if (gate) { const A gg = (A)g[i]; out *= gg * sigmoid_of(gg); }
-                if (l.active) lane_store(Y + (row + t + i) * p.ldy, at, (T)out);
+                if (l.active) lane_store(yp, at, (T)out);
+                yp += p.ldy;
             } else
                 steps += d[i];
             __builtin_amdgcn_sched_barrier(0);   // (a row's work stays together: its operands would fill the registers with those of others)

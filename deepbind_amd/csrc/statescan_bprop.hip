@@ -392,7 +392,7 @@ __global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t ld
     regs_from(p, l, ag, (const A*)nullptr, A(1));
     const size_t row = (size_t)g.start + (size_t)k * seg;
     const unsigned place = opaque(l.ch * (unsigned)sizeof(T));
-    weights w(p, threadIdx.x, first_group<LG>(p, blockIdx.y), (const A*)nullptr, in.C + row * p.ldc, lds);
+    weights w(p, threadIdx.x, first_group<LG>(p, blockIdx.y), (const A*)nullptr, in.C + row * p.ldc, lds, seg - U, true);
     T dn[U], en[U], gn[U];
     auto fetch = [&](unsigned t) {               // rows t .. t + U - 1 of the segment (a multiple of 16 rows)
 #pragma unroll
@@ -402,7 +402,7 @@ __global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t ld
             en[i] = lane_load(in.dY + at * lddy, place);
             if (in.gate) gn[i] = lane_load(in.gate + at * p.ldg, place);
         }
-        w.fetch(p, t, seg);
+        w.fetch(U);
     };
     fetch(seg - U);
     for (unsigned left = seg; left > 0; left -= U) {
