@@ -16,7 +16,7 @@
 
 namespace dbk {
 
-constexpr unsigned SCAN_CHUNK = 16;              // rows between two kept states
+constexpr unsigned SCAN_CHUNK = 8;               // rows between two kept states
 
 struct scan_shape {
     unsigned N, D, S, G, gs, nregion;            // rows, channels, states, groups, channels per group, regions

@@ -4,7 +4,7 @@
 namespace dbk {
 
 // n rows from `row` on, the states in registers. OUT: the rows of Y are written; otherwise only the states move on, and `steps` adds up d.
-// kept: null, or the block of states in front of the first row's chunk of 16; those in front of the next ones are written behind it.
+// kept: null, or the block of states in front of the first row's chunk of 8; those in front of the next ones are written behind it.
 // What two rows need comes from memory while the two before them are worked on; their weights then lie in the wave's `lds`.
 template <typename T, int LG, int NS, bool OUT>
 __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& l, unsigned lane, unsigned first, size_t row, unsigned n, const T* X, const T* dt, const T* gate,

@@ -89,7 +89,7 @@ __device__ __forceinline__ void stage_weights(const scan_shape& p, unsigned lane
     __builtin_amdgcn_wave_barrier();             // (one wave: LDS keeps its order)
 }
 
-// Backward over one chunk of nrow <= 16 rows: the states are formed again from the one kept before it, then the rows are taken from the last
+// Backward over one chunk of nrow <= 8 rows: the states are formed again from the one kept before it, then the rows are taken from the last
 // to the first; four states at a time, whose values at all rows are in registers, while those of the other states wait in LDS.
 // ag: the gradient that the rows behind send to the chunk's last state, da: dA so far, both [state / 4][lane]; st: two values per
 // row and lane that are needed again at the end (the slope of the step; dY times the gate's derivative); bc: as stage_weights.
@@ -199,7 +199,7 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
             for (int j = 0; j < 4; ++j) h[i + 1][j] = fma_a(exp2_fast(d[i] * k.v[j]), h[i][j], dx * bi.v[j]);
             __builtin_amdgcn_sched_barrier(0);
         }
-        // (the decays, like the product of step and input, are formed again below: kept from the first time they would take 80 registers
+        // (the decays, like the product of step and input, are formed again below: kept from the first time they would take 40 registers
         // more, and the compiler is told nothing about their factors any more so that it does not keep them)
 #pragma unroll
         for (int j = 0; j < 4; ++j) k.v[j] = opaque(k.v[j]);
@@ -249,27 +249,26 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
             kind = lane >> 5;
             state = ((lane >> 4) & 1u) * 2u + ((lane >> 3) & 1u);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) rows[i] = join<2>(rows[i], rows[i + 8], lane);
+            for (int i = 0; i < 4; ++i) rows[i] = join<2>(rows[i], rows[i + 4], lane);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) rows[i] = join<1>(rows[i], rows[i + 4], lane);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) rows[i] = join<0>(rows[i], rows[i + 2], lane);
+            for (int i = 0; i < 2; ++i) rows[i] = join<1>(rows[i], rows[i + 2], lane);
+            rows[0] = join<0>(rows[0], rows[1], lane);
         } else if constexpr (LG == 32) {
             kind = (lane >> 4) & 1u;
             state = ((lane >> 3) & 1u) * 2u + ((lane >> 2) & 1u);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) rows[i] = join<1>(rows[i], rows[i + 8], lane);
+            for (int i = 0; i < 4; ++i) rows[i] = join<1>(rows[i], rows[i + 4], lane);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) rows[i] = join<0>(rows[i], rows[i + 4], lane);
+            for (int i = 0; i < 2; ++i) rows[i] = join<0>(rows[i], rows[i + 2], lane);
         } else {
             kind = (lane >> 3) & 1u;
             state = ((lane >> 2) & 1u) * 2u + ((lane >> 1) & 1u);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) rows[i] = join<0>(rows[i], rows[i + 8], lane);
+            for (int i = 0; i < 4; ++i) rows[i] = join<0>(rows[i], rows[i + 4], lane);
         }
-        constexpr int LEFT = LG == 64 ? 2 : LG == 32 ? 4 : 8;                  // rows that a lane now holds
-        const unsigned base = LG == 64 ? (lane & 1u) * 2u + ((lane >> 1) & 1u) * 4u + ((lane >> 2) & 1u) * 8u
-                            : LG == 32 ? (lane & 1u) * 4u + ((lane >> 1) & 1u) * 8u : (lane & 1u) * 8u;
+        constexpr int LEFT = LG == 64 ? 1 : LG == 32 ? 2 : 4;                  // rows that a lane now holds
+        const unsigned base = LG == 64 ? (lane & 1u) + ((lane >> 1) & 1u) * 2u + ((lane >> 2) & 1u) * 4u
+                            : LG == 32 ? (lane & 1u) * 2u + ((lane >> 1) & 1u) * 4u : (lane & 1u) * 4u;
         // (lanes of a group that does not exist carry zeros into it and their first lane says so)
         if (state < left && (LG == 64 || l.active || (lane % LG >= p.gs && (lane / LG) + blockIdx.y * (64u / LG) < p.G))) {
             A* o = kind ? out.dC : out.dB;
@@ -320,7 +319,7 @@ template <typename T, int LG> struct scan_wave {
         bi = bias ? bias[l.ch] : A(0);
         dskip = dbias = A(0);
     }
-    // rows [from, from + n) of a region that starts at `start`, from a multiple of 16 rows behind it; ag holds what the rows behind send
+    // rows [from, from + n) of a region that starts at `start`, from a multiple of 8 rows behind it; ag holds what the rows behind send
     __device__ __forceinline__ void rows(const scan_shape& p, const scan_bshape& bp, unsigned start, unsigned from, unsigned n, const scan_rows_in<T>& in,
                                          const scan_rows_out<T>& to, const scan_out<A>& out)
     {
@@ -394,7 +393,7 @@ __global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t ld
     const unsigned place = opaque(l.ch * (unsigned)sizeof(T));
     weights w(p, threadIdx.x, first_group<LG>(p, blockIdx.y), (const A*)nullptr, in.C + row * p.ldc, lds, seg - U, true);
     T dn[U], en[U], gn[U];
-    auto fetch = [&](unsigned t) {               // rows t .. t + U - 1 of the segment (a multiple of 16 rows)
+    auto fetch = [&](unsigned t) {               // rows t .. t + U - 1 of the segment (a multiple of 8 rows)
 #pragma unroll
         for (unsigned i = 0; i < U; ++i) {
             const size_t at = row + t + i;

@@ -346,8 +346,8 @@ def causalconv_step(X, W, b, state, silu=True, into=None, out=None):
 
 
 def kept_states(X, A):
-    """Empty buffer for the states that statescan keeps for statescan_bprop: one (S x D) block per 16 rows of X."""
-    return torch.empty(((X.shape[0] + 15) // 16, A.shape[0], A.shape[1]), dtype=A.dtype, device=A.device)
+    """Empty buffer for the states that statescan keeps for statescan_bprop: one (S x D) block per 8 rows of X."""
+    return torch.empty(((X.shape[0] + 7) // 8, A.shape[0], A.shape[1]), dtype=A.dtype, device=A.device)
 
 
 def _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus):
@@ -387,7 +387,7 @@ def statescan(X, dt, A, B, C, regions, D=None, gate=None, dt_bias=None, softplus
     a, wide, N, D_, S, G = _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus)
     P = _row_regions(regions).shape[0]
     _lib.check_dense("state", state, (P, S, D_), wide)
-    _lib.check_dense("keep", keep, ((N + 15) // 16, S, D_), wide)
+    _lib.check_dense("keep", keep, ((N + 7) // 8, S, D_), wide)
     require(keep is None or state is None, "ValueError: states are kept for the backward pass of whole sequences, which starts from zeros: no initial state")
     if out is not None:
         _lib.check_rows("out", out, (N, D_), X.dtype)
@@ -412,7 +412,7 @@ def statescan_bprop(X, dt, A, B, C, regions, keep, dY, D=None, gate=None, dt_bia
     a, wide, N, D_, S, G = _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus)
     P = _row_regions(regions).shape[0]
     require(keep is not None, "ValueError: the states that the forward call kept are needed")
-    _lib.check_dense("keep", keep, ((N + 15) // 16, S, D_), wide)
+    _lib.check_dense("keep", keep, ((N + 7) // 8, S, D_), wide)
     _lib.check_rows("dY", dY, (N, D_), X.dtype)
     dX, ddt, dA, dB, dC, dD, dgate, dbias = (None,) * 8 if out is None else out
     for given, grad, name in ((D, dD, "D"), (gate, dgate, "gate"), (dt_bias, dbias, "dt_bias")):

@@ -522,7 +522,7 @@ typedef struct dbk_statescan_args {
     const void* state;                          /* (nregion, S, D): the states before the regions' first rows, may be NULL (zeros) */
     void* Y; size_t ldy;                        /* (N, D) rows */
     void* last;                                 /* (nregion, S, D): the states behind the last rows, may be NULL */
-    void* keep;                                 /* forward: may be NULL; ceil(N / 16) blocks of (S, D): states that the backward pass starts from */
+    void* keep;                                 /* forward: may be NULL; ceil(N / 8) blocks of (S, D): states that the backward pass starts from */
     const void* dY; size_t lddy;                /* from here on: backward only */
     void* dX; size_t lddx; void* ddt; size_t ldddt; void* dgate; size_t lddgate;
     void* dB; size_t lddb; void* dC; size_t lddc;

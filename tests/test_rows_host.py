@@ -148,7 +148,7 @@ def test_causalconv_refusals():
 def test_statescan_refusals():
     from deepbind_amd import kangaroo_smat as ks
     X, A, B, R = torch.zeros(9, 6), torch.zeros(4, 6), torch.zeros(9, 8), torch.zeros(2, 2, dtype=torch.int32)
-    keep = torch.zeros(1, 4, 6)
+    keep = torch.zeros(2, 4, 6)
     _refused("1 to 64 states per channel, got 65", ks.statescan, X, X, torch.zeros(65, 6), torch.zeros(9, 65), torch.zeros(9, 65), R)
     _refused("B must be (rows x groups", ks.statescan, X, X, A, torch.zeros(9, 7), B, R)
     _refused("divisible by the number of groups", ks.statescan, X, X, A, torch.zeros(9, 16), torch.zeros(9, 16), R)
@@ -159,7 +159,7 @@ def test_statescan_refusals():
     _refused("D must be (1, 6)", ks.statescan, X, X, A, B, B, R, D=torch.zeros(6))
     _refused("state must be (2, 4, 6)", ks.statescan, X, X, A, B, B, R, state=torch.zeros(4, 6))
     _refused("no initial state", ks.statescan, X, X, A, B, B, R, state=torch.zeros(2, 4, 6), keep=keep)
-    _refused("keep must be (1, 4, 6)", ks.statescan, X, X, A, B, B, R, keep=torch.zeros(2, 4, 6))
+    _refused("keep must be (2, 4, 6)", ks.statescan, X, X, A, B, B, R, keep=torch.zeros(1, 4, 6))
     _refused("expected a device tensor", ks.statescan, X, X, A, B, B, R)
     _refused("kept are needed", ks.statescan_bprop, X, X, A, B, B, R, None, X)
     _refused("no gate, no gradient", ks.statescan_bprop, X, X, A, B, B, R, keep, X, out=(None,) * 6 + (X, None))
