@@ -177,7 +177,7 @@ def exported_names():
 
 def call(name, *args):
     """Calls lib.<name>(*args) and raises DeepbindError with the library's message on failure."""
-    lib = dll()
+    lib = _dll or dll()
     rc = getattr(lib, name)(*args)
     if rc != 0:
         msg = lib.dbk_last_error()
@@ -217,70 +217,91 @@ ROW_DTYPES = {torch.float32: DBK_F32, torch.float64: DBK_F64, torch.bfloat16: DB
 
 def row_dtype_code(t):
     """Type code of a matrix of rows of the row operators."""
-    if t.dtype not in ROW_DTYPES:
+    code = ROW_DTYPES.get(t.dtype)
+    if code is None:
         raise DeepbindError("TypeError: expected float32, float64 or bfloat16 rows, got %s" % t.dtype)
-    return ROW_DTYPES[t.dtype]
+    return code
 
 
 def wide_dtype(t):
     """The type of the weights, statistics and states that go with rows of t's type."""
-    return torch.float64 if t.dtype == torch.float64 else torch.float32
+    return torch.float64 if t.dtype is torch.float64 else torch.float32
+
+
+# (the checks below build their messages only where they fail: a call on a few rows costs the host no more than the device)
+def _shape_or_type(name, t, shape, dtype, what):
+    if not isinstance(t, torch.Tensor) or t.shape != shape:
+        raise DeepbindError("ValueError: %s must be %s, got %s" % (name, what % (tuple(shape),), tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__))
+    raise DeepbindError("TypeError: %s must be %s, got %s" % (name, dtype, t.dtype))
 
 
 def check_rows(name, t, shape, dtype):
     """A matrix of rows: its own row stride, elements of a row next to each other."""
-    require(isinstance(t, torch.Tensor) and tuple(t.shape) == tuple(shape), "ValueError: %s must be a %s matrix, got %s" %
-            (name, tuple(shape), tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__))
-    require(t.dtype == dtype, "TypeError: %s must be %s, got %s" % (name, dtype, t.dtype))
-    rows, cols = t.shape
-    require(cols <= 1 or t.stride(1) == 1, "ValueError: the elements of a row of %s must lie next to each other" % name)
-    require(rows <= 1 or t.stride(0) >= cols, "ValueError: the rows of %s must not overlap" % name)
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype:
+        _shape_or_type(name, t, shape, dtype, "a %s matrix")
+    if t.is_contiguous():
+        return
+    rows, cols = shape
+    if cols > 1 and t.stride(1) != 1:
+        raise DeepbindError("ValueError: the elements of a row of %s must lie next to each other" % name)
+    if rows > 1 and t.stride(0) < cols:
+        raise DeepbindError("ValueError: the rows of %s must not overlap" % name)
 
 
 def check_dense(name, t, shape, dtype):
     """A contiguous array of weights or states; None passes."""
     if t is None:
         return
-    require(isinstance(t, torch.Tensor) and tuple(t.shape) == tuple(shape), "ValueError: %s must be %s, got %s" %
-            (name, tuple(shape), tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__))
-    require(t.dtype == dtype, "TypeError: %s must be %s, got %s" % (name, dtype, t.dtype))
-    require(t.is_contiguous(), "ValueError: %s must be contiguous" % name)
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype:
+        _shape_or_type(name, t, shape, dtype, "%s")
+    if not t.is_contiguous():
+        raise DeepbindError("ValueError: %s must be contiguous" % name)
 
 
 def row_stride(t):
-    return t.stride(0) if t is not None and t.shape[0] > 1 else (0 if t is None else t.shape[1])
+    if t is None:
+        return 0
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def same_device(*tensors):
     """Refuses tensors that are not on the current device, whose stream the call would run on."""
+    current = None
     for t in tensors:
-        if t is not None:
-            require(t.is_cuda, "TypeError: expected a device tensor, got a host tensor")
-            require(t.get_device() == torch.cuda.current_device(), "ValueError: a tensor lies on device %d, the current device is %d" %
-                    (t.get_device(), torch.cuda.current_device()))
+        if t is None:
+            continue
+        at = t.get_device()
+        if at != current:
+            if at < 0:
+                raise DeepbindError("TypeError: expected a device tensor, got a host tensor")
+            current = torch.cuda.current_device()
+            if at != current:
+                raise DeepbindError("ValueError: a tensor lies on device %d, the current device is %d" % (at, current))
+
+
+def _span(t):
+    lo = t.data_ptr()
+    if t.is_contiguous():
+        return lo, lo + t.numel() * t.element_size()
+    return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
 
 
 def not_shared(outs, ins):
     """Refuses outputs that overlap an input's memory or each other's."""
-    spans = []
-    for group, tensors in ((0, ins), (1, outs)):
-        for t in tensors:
-            if t is None or t.numel() == 0:
-                continue
-            lo = t.data_ptr()
-            hi = lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-            spans.append((lo, hi, group, t))
-    spans.sort(key=lambda s: s[0])
-    for i, (lo, hi, group, t) in enumerate(spans):
-        for lo2, hi2, group2, t2 in spans[i + 1:]:
-            if lo2 >= hi:
-                break
-            # blocks of columns of one wider matrix: their spans overlap, their elements need not
-            if (group or group2) and not _column_blocks(t, t2):
+    known = [_span(t) + (t,) for t in ins if t is not None and t.numel()]
+    for t in outs:
+        if t is None or not t.numel():
+            continue
+        lo, hi = _span(t)
+        for lo2, hi2, t2 in known:
+            # (blocks of columns of one wider matrix: their spans overlap, their elements need not)
+            if lo < hi2 and lo2 < hi and not _column_blocks(*((t, t2) if lo <= lo2 else (t2, t))):
                 raise DeepbindError("ValueError: an output shares memory with another argument")
+        known.append((lo, hi, t))
 
 
 def _column_blocks(a, b):
+    """Whether b, which starts no earlier than a, is another block of columns of the same matrix."""
     if a.dim() != 2 or b.dim() != 2 or a.stride(0) != b.stride(0) or a.element_size() != b.element_size():
         return False
     off = (b.data_ptr() - a.data_ptr()) // a.element_size()

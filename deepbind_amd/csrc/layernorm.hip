@@ -33,7 +33,59 @@ template <int LANES, typename A> __device__ __forceinline__ A lanes_sum(A v, A* 
     return v;
 }
 
-template <typename T, int LANES, int NV>
+// two sums at once
+template <int LANES, typename A> __device__ __forceinline__ void lanes_sum2(A& u, A& v, A* lds)
+{
+    constexpr int W = LANES < 64 ? LANES : 64;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) {
+        u += __shfl_xor(u, o);
+        v += __shfl_xor(v, o);
+    }
+    if constexpr (LANES > 64) {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) { lds[threadIdx.x >> 6] = u; lds[4 + (threadIdx.x >> 6)] = v; }
+        __syncthreads();
+        u = (lds[0] + lds[1]) + (lds[2] + lds[3]);
+        v = (lds[4] + lds[5]) + (lds[6] + lds[7]);
+    }
+}
+
+// 16 bytes as they lie in memory, zeros where the chunk ends. EXACT: chunks are whole vectors, so a vector is there or not.
+template <typename T, bool EXACT> struct raw_vec {
+    static constexpr int N = row_vec<T>::N;
+    typedef typename acc_of<T>::type A;
+    typename row_vec<T>::raw r;
+    __device__ __forceinline__ void load(const T* p, unsigned valid)
+    {
+        if (EXACT || valid >= (unsigned)N || valid == 0) {
+            if (valid) r = *reinterpret_cast<const typename row_vec<T>::raw*>(p);
+            else
+#pragma unroll
+                for (int i = 0; i < N; ++i) r[i] = (T)A(0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = i < (int)valid ? p[i] : (T)A(0);
+        }
+    }
+    __device__ __forceinline__ A operator[](int i) const { return (A)r[i]; }
+    // (what was converted is not kept for the next time)
+    __device__ __forceinline__ void forget()
+    {
+        if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(r));
+    }
+};
+template <typename T, bool EXACT> __device__ __forceinline__ void store_vec(const row_vec<T>& v, T* p, unsigned valid)
+{
+    if (EXACT) {
+        if (valid) v.store(p, row_vec<T>::N);
+    } else
+        v.store(p, valid);
+}
+
+// A row's values come while the row before it is worked on, and stay as they lie in memory: for bfloat16 half the registers of what is
+// computed from them, which is computed twice instead.
+template <typename T, int LANES, int NV, bool EXACT>
 __global__ __launch_bounds__(256) void k_norm_fprop(norm_shape p, const T* __restrict__ X, const typename acc_of<T>::type* __restrict__ gamma,
                                                     const typename acc_of<T>::type* __restrict__ beta, typename acc_of<T>::type eps,
                                                     T* __restrict__ Z, typename acc_of<T>::type* __restrict__ stats)
@@ -43,52 +95,62 @@ __global__ __launch_bounds__(256) void k_norm_fprop(norm_shape p, const T* __res
     __shared__ A lds[4];
     const unsigned unit = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const unsigned chunk = (blockIdx.y << p.ct_log2) + (unit & ((1u << p.ct_log2) - 1u));
-    const unsigned row0 = (blockIdx.x * (256u / LANES) >> p.ct_log2) + (unit >> p.ct_log2);
+    const unsigned first = blockIdx.x * (256u / LANES) >> p.ct_log2;
     const bool own = chunk < p.nchunk;
     A g[NV][V], b[NV][V];
     unsigned valid[NV];
     const A inv = A(1) / (A)p.width;
+    const size_t column = (size_t)chunk * p.width + lane * V;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const unsigned c = (lane + i * LANES) * V;
         valid[i] = own && c < p.width ? p.width - c : 0u;
-        const size_t at = (size_t)chunk * p.width + c;
-        load_weights(g[i], gamma ? gamma + at : nullptr, valid[i], A(1));
-        load_weights(b[i], beta ? beta + at : nullptr, valid[i], A(0));
+        load_weights(g[i], gamma ? gamma + column + i * LANES * V : nullptr, valid[i], A(1));
+        load_weights(b[i], beta ? beta + column + i * LANES * V : nullptr, valid[i], A(0));
     }
+    unsigned row = first + (unit >> p.ct_log2);
+    raw_vec<T, EXACT> next[NV];
+    auto fetch = [&]() {
+        const T* x = X + (size_t)row * p.ldx + column;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) next[i].load(x + i * LANES * V, row < p.n ? valid[i] : 0u);
+    };
+    fetch();
     // (every lane of a workgroup makes the same number of steps: the sums of LANES = 256 meet at barriers)
-    for (unsigned row = row0, left = blockIdx.x * (256u / LANES) >> p.ct_log2; left < p.n; row += p.rstep, left += p.rstep) {
-        const bool here = row < p.n;
-        const T* x = X + (size_t)row * p.ldx + (size_t)chunk * p.width;
-        row_vec<T> v[NV];
+    for (unsigned left = first; left < p.n; left += p.rstep) {
+        raw_vec<T, EXACT> x[NV];
+        const unsigned now = row;
         A sum = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            v[i].load(x + (lane + i * LANES) * V, here ? valid[i] : 0u);
+            x[i] = next[i];
 #pragma unroll
-            for (int j = 0; j < V; ++j) sum += v[i].v[j];
+            for (int j = 0; j < V; ++j) sum += x[i][j];
         }
+        row += p.rstep;
+        fetch();
         const A mean = lanes_sum<LANES>(sum, lds) * inv;
         A sq = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                v[i].v[j] = j < (int)valid[i] ? v[i].v[j] - mean : A(0);
-                sq += v[i].v[j] * v[i].v[j];
+                const A c = (EXACT ? valid[i] != 0 : j < (int)valid[i]) ? x[i][j] - mean : A(0);
+                sq = fma(c, c, sq);
             }
         const A rstd = A(1) / sqrt(lanes_sum<LANES>(sq, lds) * inv + eps);
-        if (!here) continue;
-        T* z = Z + (size_t)row * p.ldz + (size_t)chunk * p.width;
+        if (now >= p.n) continue;
+        T* z = Z + (size_t)now * p.ldz + column;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (!valid[i]) continue;
+            row_vec<T> o;
+            x[i].forget();
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[i].v[j] = v[i].v[j] * rstd * g[i][j] + b[i][j];
-            v[i].store(z + (lane + i * LANES) * V, valid[i]);
+            for (int j = 0; j < V; ++j) o.v[j] = fma((x[i][j] - mean) * rstd, g[i][j], b[i][j]);
+            store_vec<T, EXACT>(o, z + i * LANES * V, valid[i]);
         }
         if (stats && own && lane == 0) {
-            const size_t at = (size_t)row * p.nchunk + chunk;
+            const size_t at = (size_t)now * p.nchunk + chunk;
             stats[at] = mean;
             stats[(size_t)p.n * p.nchunk + at] = rstd;
         }
@@ -97,14 +159,15 @@ __global__ __launch_bounds__(256) void k_norm_fprop(norm_shape p, const T* __res
 
 // The backward pass walks the rows the same way and adds dz h and dz up in registers; the workgroup's row lanes are added in
 // LDS at the end, in their order, and leave one row of partial sums per workgroup: part[blockIdx.x][2][nchunk * width].
-template <typename T, int LANES, int NV>
+// (Lanes without a column hold dz = 0, which leaves nothing in any sum.)
+template <typename T, int LANES, int NV, bool EXACT>
 __global__ __launch_bounds__(256) void k_norm_bprop(norm_shape p, size_t lddz, const T* __restrict__ X, const typename acc_of<T>::type* __restrict__ gamma,
                                                     const typename acc_of<T>::type* __restrict__ stats, const T* __restrict__ dZ,
                                                     T* __restrict__ dX, typename acc_of<T>::type* __restrict__ part)
 {
     typedef typename acc_of<T>::type A;
     constexpr int V = row_vec<T>::N;
-    __shared__ A lds[4];
+    __shared__ A lds[8];
     __shared__ A rows_lds[2][256][V];
     const unsigned unit = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const unsigned chunk = (blockIdx.y << p.ct_log2) + (unit & ((1u << p.ct_log2) - 1u));
@@ -113,48 +176,66 @@ __global__ __launch_bounds__(256) void k_norm_bprop(norm_shape p, size_t lddz, c
     A g[NV][V], dg[NV][V], db[NV][V];
     unsigned valid[NV];
     const A inv = A(1) / (A)p.width;
+    const size_t column = (size_t)chunk * p.width + lane * V;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const unsigned c = (lane + i * LANES) * V;
         valid[i] = own && c < p.width ? p.width - c : 0u;
-        load_weights(g[i], gamma ? gamma + (size_t)chunk * p.width + c : nullptr, valid[i], A(1));
+        load_weights(g[i], gamma ? gamma + column + i * LANES * V : nullptr, valid[i], A(1));
 #pragma unroll
         for (int j = 0; j < V; ++j) dg[i][j] = db[i][j] = A(0);
     }
-    for (unsigned row = first + (unit >> p.ct_log2), left = first; left < p.n; row += p.rstep, left += p.rstep) {
+    unsigned row = first + (unit >> p.ct_log2);
+    raw_vec<T, EXACT> nx[NV], nd[NV];
+    A nmean = 0, nrstd = 0;
+    auto fetch = [&]() {
         const bool here = own && row < p.n;
-        const size_t xo = (size_t)row * p.ldx + (size_t)chunk * p.width, zo = (size_t)row * lddz + (size_t)chunk * p.width;
+        const T *x = X + (size_t)row * p.ldx + column, *d = dZ + (size_t)row * lddz + column;
         const size_t at = (size_t)row * p.nchunk + chunk;
-        const A mean = here ? stats[at] : A(0), rstd = here ? stats[(size_t)p.n * p.nchunk + at] : A(0);
-        row_vec<T> h[NV], q[NV];
-        A s1 = 0, s2 = 0;
+        nmean = here ? stats[at] : A(0);
+        nrstd = here ? stats[(size_t)p.n * p.nchunk + at] : A(0);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            h[i].load(X + xo + (lane + i * LANES) * V, here ? valid[i] : 0u);
-            q[i].load(dZ + zo + (lane + i * LANES) * V, here ? valid[i] : 0u);
+            nx[i].load(x + i * LANES * V, here ? valid[i] : 0u);
+            nd[i].load(d + i * LANES * V, here ? valid[i] : 0u);
         }
+    };
+    fetch();
+    for (unsigned left = first; left < p.n; left += p.rstep) {
+        raw_vec<T, EXACT> x[NV], d[NV];
+        const A mean = nmean, rstd = nrstd;
+        const unsigned now = row;
+        A s1 = 0, s2 = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) { x[i] = nx[i]; d[i] = nd[i]; }
+        row += p.rstep;
+        fetch();
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const A d = q[i].v[j], hh = here && j < (int)valid[i] ? (h[i].v[j] - mean) * rstd : A(0);
-                dg[i][j] += d * hh;
-                db[i][j] += d;
-                h[i].v[j] = hh;
-                q[i].v[j] = d * g[i][j];
-                s1 += q[i].v[j];
-                s2 += q[i].v[j] * hh;
+                const A h = (x[i][j] - mean) * rstd, q = d[i][j] * g[i][j];
+                dg[i][j] = fma(d[i][j], h, dg[i][j]);
+                db[i][j] += d[i][j];
+                s1 += q;
+                s2 = fma(q, h, s2);
             }
-        s1 = lanes_sum<LANES>(s1, lds) * inv;
-        s2 = lanes_sum<LANES>(s2, lds) * inv;
-        if (!here) continue;
-        T* dx = dX + (size_t)row * p.ldz + (size_t)chunk * p.width;
+        lanes_sum2<LANES>(s1, s2, lds);
+        s1 *= inv;
+        s2 *= inv;
+        if (!own || now >= p.n) continue;
+        T* dx = dX + (size_t)now * p.ldz + column;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (!valid[i]) continue;
+            row_vec<T> o;
+            x[i].forget();
+            d[i].forget();
 #pragma unroll
-            for (int j = 0; j < V; ++j) q[i].v[j] = rstd * (q[i].v[j] - s1 - h[i].v[j] * s2);
-            q[i].store(dx + (lane + i * LANES) * V, valid[i]);
+            for (int j = 0; j < V; ++j) {
+                const A h = (x[i][j] - mean) * rstd;
+                o.v[j] = rstd * (fma(d[i][j], g[i][j], -s1) - h * s2);
+            }
+            store_vec<T, EXACT>(o, dx + i * LANES * V, valid[i]);
         }
     }
     if (!part) return;
@@ -369,9 +450,14 @@ norm_plan plan_norm(int dtype, size_t n, size_t m, size_t group)
 
 constexpr unsigned WIDE_ROWS = 256;              // workgroups down the rows of the wide form's weight gradient
 
-template <typename F> bool norm_layout(int lanes, int nv, F f)
+template <typename F> bool norm_layout(int lanes, int nv, bool exact, F f)
 {
-#define DBK_NORM_CASE(L, V) if (lanes == L && nv == V) { f(std::integral_constant<int, L>(), std::integral_constant<int, V>()); return true; }
+#define DBK_NORM_CASE(L, V)                                                                              \
+    if (lanes == L && nv == V) {                                                                         \
+        if (exact) f(std::integral_constant<int, L>(), std::integral_constant<int, V>(), std::true_type());      \
+        else f(std::integral_constant<int, L>(), std::integral_constant<int, V>(), std::false_type());           \
+        return true;                                                                                     \
+    }
     DBK_NORM_CASE(1, 1) DBK_NORM_CASE(2, 1) DBK_NORM_CASE(4, 1) DBK_NORM_CASE(8, 1) DBK_NORM_CASE(16, 1) DBK_NORM_CASE(32, 1)
     DBK_NORM_CASE(64, 1) DBK_NORM_CASE(64, 2) DBK_NORM_CASE(64, 3) DBK_NORM_CASE(64, 4) DBK_NORM_CASE(256, 2) DBK_NORM_CASE(256, 4)
 #undef DBK_NORM_CASE
@@ -409,8 +495,8 @@ int dbk_layernorm(dbk_stream_t stream, int dtype, const void* X, size_t ldx, con
     with_row_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
-        if (!norm_layout(p.lanes, p.nv, [&](auto lanes, auto nv) {
-                k_norm_fprop<T, lanes.value, nv.value><<<dim3(p.gx, p.gy), 256, 0, st>>>(p.shape, (const T*)X, (const A*)gamma, (const A*)beta, (A)eps, (T*)Z, (A*)stats);
+        if (!norm_layout(p.lanes, p.nv, group % row_vec<T>::N == 0, [&](auto lanes, auto nv, auto exact) {
+                k_norm_fprop<T, lanes.value, nv.value, exact.value><<<dim3(p.gx, p.gy), 256, 0, st>>>(p.shape, (const T*)X, (const A*)gamma, (const A*)beta, (A)eps, (T*)Z, (A*)stats);
             })) {
             const size_t units = n * (m / group);
             k_norm_fprop_wide<T><<<(unsigned)(units < NORM_WGS ? units : NORM_WGS), 256, 0, st>>>(p.shape, (const T*)X, (const A*)gamma, (const A*)beta, (A)eps, (T*)Z, (A*)stats);
@@ -458,8 +544,8 @@ int dbk_layernorm_bprop(dbk_stream_t stream, int dtype, const void* X, size_t ld
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
         A* part = weights ? (A*)work : nullptr;
-        if (!norm_layout(p.lanes, p.nv, [&](auto lanes, auto nv) {
-                k_norm_bprop<T, lanes.value, nv.value><<<dim3(p.gx, p.gy), 256, 0, st>>>(p.shape, lddz, (const T*)X, (const A*)gamma, (const A*)stats, (const T*)dZ, (T*)dX, part);
+        if (!norm_layout(p.lanes, p.nv, group % row_vec<T>::N == 0, [&](auto lanes, auto nv, auto exact) {
+                k_norm_bprop<T, lanes.value, nv.value, exact.value><<<dim3(p.gx, p.gy), 256, 0, st>>>(p.shape, lddz, (const T*)X, (const A*)gamma, (const A*)stats, (const T*)dZ, (T*)dX, part);
             })) {
             const size_t chunks = n * (m / group);
             k_norm_bprop_wide<T><<<(unsigned)(chunks < NORM_WGS ? chunks : NORM_WGS), 256, 0, st>>>(p.shape, lddz, (const T*)X, (const A*)gamma, (const A*)stats, (const T*)dZ, (T*)dX);

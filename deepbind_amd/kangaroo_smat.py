@@ -250,12 +250,14 @@ def scanpool_bprop(W, b, X, regions, ptype, pooled, argmax, dpooled, dW, db, ove
 # ------------------------------------------------------------------------------------------------
 def _row_regions(R):
     _regions(R)
-    require(R.shape[1] == 2 and R.is_contiguous(), "ValueError: regions must be a contiguous (P x 2) array")
+    if R.shape[1] != 2 or not R.is_contiguous():
+        raise DeepbindError("ValueError: regions must be a contiguous (P x 2) array")
     return R
 
 
 def _map(X):
-    require(isinstance(X, torch.Tensor) and X.dim() == 2, "ValueError: X must be a matrix")
+    if not isinstance(X, torch.Tensor) or X.dim() != 2:
+        raise DeepbindError("ValueError: X must be a matrix")
     _lib.check_rows("X", X, X.shape, X.dtype)
     return _lib.row_dtype_code(X), _lib.wide_dtype(X), X.shape[0], X.shape[1]
 
@@ -271,7 +273,8 @@ def _out(name, t, shape, dtype, device, dense=False):
 def _conv_args(X, W, b):
     code, wide, N, D = _map(X)
     require(isinstance(W, torch.Tensor) and W.dim() == 2 and W.shape[1] == D, "ValueError: W must be (taps x channels)")
-    require(1 <= W.shape[0] <= 4, "NotImplementedError: filters of 1 to 4 taps, got %d" % W.shape[0])
+    if not 1 <= W.shape[0] <= 4:
+        raise DeepbindError("NotImplementedError: filters of 1 to 4 taps, got %d" % W.shape[0])
     _lib.check_dense("W", W, W.shape, wide)
     _lib.check_dense("b", b, (1, D), wide)
     return code, wide, N, D, W.shape[0]
@@ -354,7 +357,8 @@ def _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus):
     code, wide, N, D_ = _map(X)
     require(isinstance(A, torch.Tensor) and A.dim() == 2 and A.shape[1] == D_ and A.shape[0] >= 1, "ValueError: A must be (states x channels)")
     S = A.shape[0]
-    require(S <= 64, "NotImplementedError: 1 to 64 states per channel, got %d" % S)
+    if S > 64:
+        raise DeepbindError("NotImplementedError: 1 to 64 states per channel, got %d" % S)
     require(isinstance(B, torch.Tensor) and B.dim() == 2 and B.shape[1] % S == 0 and B.shape[1] >= S, "ValueError: B must be (rows x groups * states)")
     G = B.shape[1] // S
     require(D_ % G == 0, "ValueError: the number of channels must be divisible by the number of groups")
@@ -367,10 +371,8 @@ def _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus):
     if gate is not None:
         _lib.check_rows("gate", gate, (N, D_), X.dtype)
     raw, ld = _lib.raw, _lib.row_stride
-    a = _lib.StateScanArgs()
-    a.dtype, a.softplus, a.N, a.D, a.S, a.G = code, int(bool(softplus)), N, D_, S, G
-    a.X, a.ldx, a.dt, a.lddt, a.A, a.B, a.ldb, a.C, a.ldc = raw(X), ld(X), raw(dt), ld(dt), raw(A), raw(B), ld(B), raw(C), ld(C)
-    a.skip, a.dt_bias, a.gate, a.ldgate = raw(D), raw(dt_bias), raw(gate), ld(gate)
+    a = _lib.StateScanArgs(code, int(bool(softplus)), N, D_, S, G, None, 0, raw(X), ld(X), raw(dt), ld(dt), raw(A), raw(B), ld(B), raw(C), ld(C),
+                           raw(D), raw(dt_bias), raw(gate), ld(gate))
     return a, wide, N, D_, S, G
 
 
