@@ -4,12 +4,16 @@
 //   dp = dz sigmoid(p) (1 + p (1 - sigmoid(p))),  dx[t] = sum_j W[j] dp[t + K - 1 - j],  dW[j] = sum_t dp[t] x[t - K + 1 + j],  db = sum_t dp[t]
 //
 // Bound by memory: x in and z out forward, x and dz in and dx out backward (p is formed again from x: reading it would cost a
-// third map, keeping it another). A lane owns 16 bytes of channels and walks down a strip of rows with the last K - 1 of
+// third map, keeping it another). A lane owns four channels (two of double) and walks down a strip of rows with the last K - 1 of
 // them in registers, so that a row is read once but for the K - 1 rows above each strip, which the caches hold.
 #include <type_traits>
 #include "rows_common.h"
 
 namespace dbk {
+
+// Four channels per lane: 16 bytes of float. (Eight bfloat16 would be 16 bytes too, but the weights, their sums and the last rows of eight
+// channels take twice the registers, and fewer waves then keep memory busy.)
+template <typename T> using conv_vec = row_vec<T, sizeof(T) == 8 ? 2 : 4>;
 
 struct conv_shape {
     unsigned N, D, nregion, seg;                 // rows, channels, regions, rows per segment of a long region
@@ -19,7 +23,7 @@ struct conv_shape {
 
 template <typename T, int K> struct conv_weights {
     typedef typename acc_of<T>::type A;
-    static constexpr int V = row_vec<T>::N;
+    static constexpr int V = conv_vec<T>::N;
     A w[K][V], b[V];
     __device__ __forceinline__ void load(const A* W, const A* bias, unsigned D, unsigned c, unsigned valid)
     {
@@ -31,7 +35,7 @@ template <typename T, int K> struct conv_weights {
 
 // row t of region r (t may lie up to K - 1 rows before its start)
 template <typename T, int K>
-__device__ __forceinline__ void conv_row(row_vec<T>& v, const T* X, size_t ldx, const T* state, unsigned D, unsigned c, unsigned valid,
+__device__ __forceinline__ void conv_row(conv_vec<T>& v, const T* X, size_t ldx, const T* state, unsigned D, unsigned c, unsigned valid,
                                          unsigned r, row_range g, int64_t t)
 {
     if (t >= (int64_t)g.start) v.load(X + (size_t)t * ldx + c, valid);
@@ -39,24 +43,47 @@ __device__ __forceinline__ void conv_row(row_vec<T>& v, const T* X, size_t ldx, 
     else v.fill(typename acc_of<T>::type(0));
 }
 
-template <typename T, int K>
+constexpr int CONV_AHEAD = 4;                    // rows that are fetched together, while the four before them are worked on
+// the next CONV_AHEAD rows from `p` on, the last of `left` rows again behind it
+template <typename T, bool EXACT> struct conv_ahead {
+    raw_vec<T, EXACT, conv_vec<T>::N> v[CONV_AHEAD];
+    __device__ __forceinline__ void fetch(const T*& p, size_t ld, unsigned valid, int64_t left)
+    {
+#pragma unroll
+        for (int i = 0; i < CONV_AHEAD; ++i) {
+            v[i].load(p, valid);
+            p += i + 1 < left ? ld : 0;
+        }
+    }
+    __device__ __forceinline__ void to(conv_vec<T>& x, int i) const
+    {
+#pragma unroll
+        for (int j = 0; j < conv_vec<T>::N; ++j) x.v[j] = v[i][j];
+    }
+};
+
+template <typename T, int K, bool EXACT>
 __device__ __forceinline__ void conv_strip(conv_shape p, const conv_weights<T, K>& w, const T* X, const T* state, T* Z, unsigned c, unsigned valid,
                                            unsigned r, row_range g, unsigned from, unsigned to)
 {
     typedef typename acc_of<T>::type A;
-    constexpr int V = row_vec<T>::N;
-    constexpr int U = 4;                         // rows whose loads are in flight together
+    constexpr int V = conv_vec<T>::N, U = CONV_AHEAD;
     if (from >= to || !valid) return;
-    row_vec<T> x[K - 1 + U];
+    conv_vec<T> x[K - 1 + U];
+    conv_ahead<T, EXACT> next;
+    const T* xp = X + (size_t)from * p.ldx + c;
+    T* zp = Z + (size_t)from * p.ldz + c;
+    next.fetch(xp, p.ldx, valid, to - from);
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) conv_row<T, K>(x[j], X, p.ldx, state, p.D, c, valid, r, g, (int64_t)from - (K - 1) + j);
     for (unsigned t = from; t < to; t += U) {
 #pragma unroll
-        for (int i = 0; i < U; ++i) if (t + i < to) x[K - 1 + i].load(X + (size_t)(t + i) * p.ldx + c, valid);
+        for (int i = 0; i < U; ++i) next.to(x[K - 1 + i], i);
+        if (to - t > (unsigned)U) next.fetch(xp, p.ldx, valid, to - t - U);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             if (t + i >= to) break;
-            row_vec<T> z;
+            conv_vec<T> z;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 A a = w.b[v];
@@ -64,7 +91,8 @@ __device__ __forceinline__ void conv_strip(conv_shape p, const conv_weights<T, K
                 for (int j = 0; j < K; ++j) a = fma(w.w[j][v], x[i + j].v[v], a);
                 z.v[v] = p.silu ? a * sigmoid_of(a) : a;
             }
-            z.store(Z + (size_t)(t + i) * p.ldz + c, valid);
+            store_vec<EXACT>(z, zp, valid);
+            zp += p.ldz;
         }
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) x[j] = x[U + j];
@@ -72,12 +100,12 @@ __device__ __forceinline__ void conv_strip(conv_shape p, const conv_weights<T, K
 }
 
 // A workgroup takes the first segment of a region (all of it, mostly), its lanes being 2^ct_log2 vectors of channels by strips of rows.
-template <typename T, int K>
+template <typename T, int K, bool EXACT>
 __global__ __launch_bounds__(256) void k_conv_fprop(conv_shape p, const T* __restrict__ X, const typename acc_of<T>::type* __restrict__ W,
                                                     const typename acc_of<T>::type* __restrict__ bias, const uint32_t* __restrict__ regions,
                                                     const T* __restrict__ state, T* __restrict__ Z, T* __restrict__ last, uint32_t* __restrict__ marks)
 {
-    constexpr int V = row_vec<T>::N;
+    constexpr int V = conv_vec<T>::N;
     const unsigned x = threadIdx.x & ((1u << p.ct_log2) - 1u), y = threadIdx.x >> p.ct_log2, strips = 256u >> p.ct_log2;
     const unsigned c = ((blockIdx.y << p.ct_log2) + x) * V, valid = c < p.D ? p.D - c : 0u;
     const unsigned r = blockIdx.x;
@@ -86,9 +114,9 @@ __global__ __launch_bounds__(256) void k_conv_fprop(conv_shape p, const T* __res
     w.load(W, bias, p.D, c, valid);
     const unsigned len = min(g.end - g.start, p.seg), strip = (len + strips - 1) / strips;
     const unsigned from = g.start + min(y * strip, len), to = g.start + min((y + 1) * strip, len);
-    conv_strip<T, K>(p, w, X, state, Z, c, valid, r, g, from, to);
+    conv_strip<T, K, EXACT>(p, w, X, state, Z, c, valid, r, g, from, to);
     if (last && y < K - 1 && valid) {            // the K - 1 rows that the next piece of this sequence needs
-        row_vec<T> v;
+        conv_vec<T> v;
         conv_row<T, K>(v, X, p.ldx, state, p.D, c, valid, r, g, (int64_t)g.end - (K - 1) + y);
         v.store(last + ((size_t)r * (K - 1) + y) * p.D + c, valid);
     }
@@ -96,12 +124,12 @@ __global__ __launch_bounds__(256) void k_conv_fprop(conv_shape p, const T* __res
 }
 
 // The other segments of long regions.
-template <typename T, int K>
+template <typename T, int K, bool EXACT>
 __global__ __launch_bounds__(256) void k_conv_fprop_long(conv_shape p, const T* __restrict__ X, const typename acc_of<T>::type* __restrict__ W,
                                                          const typename acc_of<T>::type* __restrict__ bias, const uint32_t* __restrict__ regions,
                                                          const uint32_t* __restrict__ marks, T* __restrict__ Z)
 {
-    constexpr int V = row_vec<T>::N;
+    constexpr int V = conv_vec<T>::N;
     unsigned r, k;
     row_range g;
     if (!slot_segment(regions, p.nregion, p.N, marks, blockIdx.x, p.seg, r, g, k)) return;
@@ -110,14 +138,14 @@ __global__ __launch_bounds__(256) void k_conv_fprop_long(conv_shape p, const T* 
     conv_weights<T, K> w;
     w.load(W, bias, p.D, c, valid);
     const unsigned a = g.start + k * p.seg, len = min(g.end - a, p.seg), strip = (len + strips - 1) / strips;
-    conv_strip<T, K>(p, w, X, (const T*)nullptr, Z, c, valid, r, g, a + min(y * strip, len), a + min((y + 1) * strip, len));
+    conv_strip<T, K, EXACT>(p, w, X, (const T*)nullptr, Z, c, valid, r, g, a + min(y * strip, len), a + min((y + 1) * strip, len));
 }
 
 // Backward of rows [from, to) of region g, adding to the lane's dW, db. Each row's dp is formed once, but for the K - 1 rows below
 // the strip that its own last dx need.
 template <typename T, int K> struct conv_sums {
     typedef typename acc_of<T>::type A;
-    static constexpr int V = row_vec<T>::N;
+    static constexpr int V = conv_vec<T>::N;
     A dw[K][V], db[V];
     __device__ __forceinline__ void clear()
     {
@@ -129,56 +157,77 @@ template <typename T, int K> struct conv_sums {
         }
     }
 };
-template <typename T, int K>
+template <typename T, int K, bool EXACT>
 __device__ __forceinline__ void conv_strip_bprop(conv_shape p, size_t lddz, const conv_weights<T, K>& w, conv_sums<T, K>& sums, const T* X, const T* dZ, T* dX,
                                                  unsigned c, unsigned valid, row_range g, unsigned from, unsigned to)
 {
     typedef typename acc_of<T>::type A;
-    constexpr int V = row_vec<T>::N;
+    constexpr int V = conv_vec<T>::N, U = CONV_AHEAD;
     if (from >= to || !valid) return;
-    row_vec<T> x[K], dp[K];                      // rows t - K + 1 .. t; dp[j] = dp of row t - K + 1 + j
+    conv_vec<T> x[K - 1 + U], dp[K];             // rows t - K + 1 on; dp[j] = dp of row t - K + 1 + j
+    conv_ahead<T, EXACT> nx, nd;
+    const T *xp = X + (size_t)from * p.ldx + c, *dp_ = dZ + (size_t)from * lddz + c;
+    T* op = dX + (size_t)from * p.ldz + c;
+    // rows of the region from `from` on, rows of the strip, and rows walked: K - 1 more, whose dp the strip's last rows need
+    const int64_t rows = (int64_t)g.end - from, own = to - from, stop = own + (K - 1);
+    nx.fetch(xp, p.ldx, valid, rows);
+    nd.fetch(dp_, lddz, valid, rows);
 #pragma unroll
     for (int j = 0; j < K; ++j) dp[j].fill(A(0));
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) conv_row<T, K>(x[j], X, p.ldx, (const T*)nullptr, p.D, c, valid, 0u, g, (int64_t)from - (K - 1) + j);
-    const uint64_t stop = (uint64_t)to + (K - 1);
-    for (uint64_t t = from; t < stop; ++t) {
-        if (t < g.end) {
-            x[K - 1].load(X + (size_t)t * p.ldx + c, valid);
-            row_vec<T> d;
-            d.load(dZ + (size_t)t * lddz + c, valid);
+    for (int64_t t0 = 0; t0 < stop; t0 += U) {
+        conv_vec<T> d[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            nx.to(x[K - 1 + i], i);
+            nd.to(d[i], i);
+        }
+        if (t0 + U < stop) {
+            nx.fetch(xp, p.ldx, valid, rows - t0 - U);
+            nd.fetch(dp_, lddz, valid, rows - t0 - U);
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int64_t t = t0 + i;
+            if (t >= stop) break;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                A dpre = d.v[v];
+                A dpre = d[i].v[v];
                 if (p.silu) {
                     A a = w.b[v];
 #pragma unroll
-                    for (int j = 0; j < K; ++j) a = fma(w.w[j][v], x[j].v[v], a);
+                    for (int j = 0; j < K; ++j) a = fma(w.w[j][v], x[i + j].v[v], a);
                     const A s = sigmoid_of(a);
                     dpre *= s * fma(a, A(1) - s, A(1));
                 }
-                dp[K - 1].v[v] = dpre;
-                if (t < to) {
-                    sums.db[v] += dpre;
+                dp[K - 1].v[v] = t < rows ? dpre : A(0);         // (behind the region nothing is sent back)
+            }
+            if (t < own) {
 #pragma unroll
-                    for (int j = 0; j < K; ++j) sums.dw[j][v] = fma(dpre, x[j].v[v], sums.dw[j][v]);
+                for (int v = 0; v < V; ++v) {
+                    sums.db[v] += dp[K - 1].v[v];
+#pragma unroll
+                    for (int j = 0; j < K; ++j) sums.dw[j][v] = fma(dp[K - 1].v[v], x[i + j].v[v], sums.dw[j][v]);
                 }
             }
-        } else
-            dp[K - 1].fill(A(0));
-        if (t >= (uint64_t)from + (K - 1)) {
-            row_vec<T> o;
+            if (t >= K - 1) {
+                conv_vec<T> o;
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                A a = 0;
+                for (int v = 0; v < V; ++v) {
+                    A a = 0;
 #pragma unroll
-                for (int j = 0; j < K; ++j) a = fma(w.w[j][v], dp[K - 1 - j].v[v], a);
-                o.v[v] = a;
+                    for (int j = 0; j < K; ++j) a = fma(w.w[j][v], dp[K - 1 - j].v[v], a);
+                    o.v[v] = a;
+                }
+                store_vec<EXACT>(o, op, valid);
+                op += p.ldz;
             }
-            o.store(dX + (size_t)(t - (K - 1)) * p.ldz + c, valid);
+#pragma unroll
+            for (int j = 0; j < K - 1; ++j) dp[j] = dp[j + 1];
         }
 #pragma unroll
-        for (int j = 0; j < K - 1; ++j) { x[j] = x[j + 1]; dp[j] = dp[j + 1]; }
+        for (int j = 0; j < K - 1; ++j) x[j] = x[U + j];
     }
 }
 
@@ -187,7 +236,7 @@ template <typename T, int K>
 __device__ __forceinline__ void conv_leave_sums(conv_shape p, const conv_sums<T, K>& sums, unsigned c, unsigned valid, unsigned unit, typename acc_of<T>::type* part)
 {
     typedef typename acc_of<T>::type A;
-    constexpr int V = row_vec<T>::N;
+    constexpr int V = conv_vec<T>::N;
     __shared__ A lds[256][V + 1];
     const unsigned across = 1u << p.ct_log2;
 #pragma unroll
@@ -207,13 +256,13 @@ __device__ __forceinline__ void conv_leave_sums(conv_shape p, const conv_sums<T,
     }
 }
 
-template <typename T, int K>
+template <typename T, int K, bool EXACT>
 __global__ __launch_bounds__(256) void k_conv_bprop(conv_shape p, size_t lddz, const T* __restrict__ X, const typename acc_of<T>::type* __restrict__ W,
                                                     const typename acc_of<T>::type* __restrict__ bias, const uint32_t* __restrict__ regions,
                                                     const T* __restrict__ dZ, T* __restrict__ dX, typename acc_of<T>::type* __restrict__ part,
                                                     uint32_t* __restrict__ marks)
 {
-    constexpr int V = row_vec<T>::N;
+    constexpr int V = conv_vec<T>::N;
     const unsigned x = threadIdx.x & ((1u << p.ct_log2) - 1u), y = threadIdx.x >> p.ct_log2, strips = 256u >> p.ct_log2;
     const unsigned c = ((blockIdx.y << p.ct_log2) + x) * V, valid = c < p.D ? p.D - c : 0u;
     conv_weights<T, K> w;
@@ -223,19 +272,19 @@ __global__ __launch_bounds__(256) void k_conv_bprop(conv_shape p, size_t lddz, c
     for (unsigned r = blockIdx.x; r < p.nregion; r += gridDim.x) {
         const row_range g = region_rows(regions, r, p.N);
         const unsigned len = min(g.end - g.start, p.seg), strip = (len + strips - 1) / strips;
-        conv_strip_bprop<T, K>(p, lddz, w, sums, X, dZ, dX, c, valid, g, g.start + min(y * strip, len), g.start + min((y + 1) * strip, len));
+        conv_strip_bprop<T, K, EXACT>(p, lddz, w, sums, X, dZ, dX, c, valid, g, g.start + min(y * strip, len), g.start + min((y + 1) * strip, len));
         if (marks && blockIdx.y == 0) mark_segments(marks, r, g, p.seg, threadIdx.x, 256u);
     }
     conv_leave_sums<T, K>(p, sums, c, valid, blockIdx.x, part);
 }
 
-template <typename T, int K>
+template <typename T, int K, bool EXACT>
 __global__ __launch_bounds__(256) void k_conv_bprop_long(conv_shape p, size_t lddz, unsigned nslot, unsigned unit0, const T* __restrict__ X,
                                                          const typename acc_of<T>::type* __restrict__ W, const typename acc_of<T>::type* __restrict__ bias,
                                                          const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
                                                          const T* __restrict__ dZ, T* __restrict__ dX, typename acc_of<T>::type* __restrict__ part)
 {
-    constexpr int V = row_vec<T>::N;
+    constexpr int V = conv_vec<T>::N;
     const unsigned x = threadIdx.x & ((1u << p.ct_log2) - 1u), y = threadIdx.x >> p.ct_log2, strips = 256u >> p.ct_log2;
     const unsigned c = ((blockIdx.y << p.ct_log2) + x) * V, valid = c < p.D ? p.D - c : 0u;
     conv_weights<T, K> w;
@@ -247,7 +296,7 @@ __global__ __launch_bounds__(256) void k_conv_bprop_long(conv_shape p, size_t ld
         row_range g;
         if (!slot_segment(regions, p.nregion, p.N, marks, slot, p.seg, r, g, k)) continue;
         const unsigned a = g.start + k * p.seg, len = min(g.end - a, p.seg), strip = (len + strips - 1) / strips;
-        conv_strip_bprop<T, K>(p, lddz, w, sums, X, dZ, dX, c, valid, g, a + min(y * strip, len), a + min((y + 1) * strip, len));
+        conv_strip_bprop<T, K, EXACT>(p, lddz, w, sums, X, dZ, dX, c, valid, g, a + min(y * strip, len), a + min((y + 1) * strip, len));
     }
     conv_leave_sums<T, K>(p, sums, c, valid, unit0 + blockIdx.x, part);
 }
@@ -258,13 +307,13 @@ __global__ __launch_bounds__(256) void k_conv_step(conv_shape p, const T* __rest
                                                    const typename acc_of<T>::type* __restrict__ bias, const T* state, T* into, T* __restrict__ Z)
 {
     typedef typename acc_of<T>::type A;
-    constexpr int V = row_vec<T>::N;
+    constexpr int V = conv_vec<T>::N;
     const size_t vecs = (p.D + V - 1) / V, i = (size_t)blockIdx.x * 256u + threadIdx.x;
     if (i >= vecs * p.N) return;
     const size_t r = i / vecs;
     const unsigned c = (unsigned)(i - r * vecs) * V, valid = p.D - c;
     conv_weights<T, K> w;
-    row_vec<T> x[K], z;
+    conv_vec<T> x[K], z;
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) x[j].load(state + (r * (K - 1) + j) * p.D + c, valid);
     x[K - 1].load(X + r * p.ldx + c, valid);
@@ -283,15 +332,17 @@ __global__ __launch_bounds__(256) void k_conv_step(conv_shape p, const T* __rest
 
 namespace {
 
-constexpr unsigned CONV_STRIP = 16;              // rows per lane of a full segment: the K - 1 rows read again are a fifth, from the caches
+constexpr unsigned CONV_STRIP = 32;              // rows per lane of a full segment: the K - 1 rows read again are a tenth, from the caches
 constexpr size_t CONV_UNITS = 2048;              // workgroups that add up weight gradients, per tile of channels: eight per CU
+
+size_t conv_width(int dtype) { return dtype == DBK_F64 ? 2 : 4; }
 
 struct conv_plan { unsigned ct_log2, tiles, seg, units, slots, slot_units; };
 
 conv_plan plan_conv(int dtype, size_t N, size_t D, size_t P)
 {
     conv_plan p;
-    const size_t vecs = (D + 16 / row_size(dtype) - 1) / (16 / row_size(dtype));
+    const size_t vecs = (D + conv_width(dtype) - 1) / conv_width(dtype);
     p.ct_log2 = 0;
     while (p.ct_log2 < 6 && (size_t(1) << p.ct_log2) < vecs) ++p.ct_log2;
     p.tiles = divup(vecs, size_t(1) << p.ct_log2);
@@ -303,12 +354,17 @@ conv_plan plan_conv(int dtype, size_t N, size_t D, size_t P)
     return p;
 }
 
-template <typename F> void with_taps(size_t K, F f)
+// taps, and whether rows are whole vectors
+template <typename F> void with_taps(size_t K, bool exact, F f)
 {
-    if (K == 1) f(std::integral_constant<int, 1>());
-    else if (K == 2) f(std::integral_constant<int, 2>());
-    else if (K == 3) f(std::integral_constant<int, 3>());
-    else f(std::integral_constant<int, 4>());
+    auto g = [&](auto k) {
+        if (exact) f(k, std::true_type());
+        else f(k, std::false_type());
+    };
+    if (K == 1) g(std::integral_constant<int, 1>());
+    else if (K == 2) g(std::integral_constant<int, 2>());
+    else if (K == 3) g(std::integral_constant<int, 3>());
+    else g(std::integral_constant<int, 4>());
 }
 
 int check_conv(int dtype, const void* X, size_t ldx, const void* W, size_t taps, size_t N, size_t D, size_t nregion, const void* Z, size_t ldz)
@@ -355,11 +411,11 @@ int dbk_causalconv(dbk_stream_t stream, int dtype, const void* X, size_t ldx, co
     with_row_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
-        with_taps(taps, [&](auto k) {
-            k_conv_fprop<T, k.value><<<dim3((unsigned)nregion, p.tiles), 256, 0, st>>>(s, (const T*)X, (const A*)W, (const A*)bias, regions, (const T*)state, (T*)Z, (T*)last,
+        with_taps(taps, D % conv_width(dtype) == 0, [&](auto k, auto exact) {
+            k_conv_fprop<T, k.value, exact.value><<<dim3((unsigned)nregion, p.tiles), 256, 0, st>>>(s, (const T*)X, (const A*)W, (const A*)bias, regions, (const T*)state, (T*)Z, (T*)last,
                                                                                   p.slots ? (uint32_t*)work : nullptr);
             if (p.slots)
-                k_conv_fprop_long<T, k.value><<<dim3(p.slots, p.tiles), 256, 0, st>>>(s, (const T*)X, (const A*)W, (const A*)bias, regions, (const uint32_t*)work, (T*)Z);
+                k_conv_fprop_long<T, k.value, exact.value><<<dim3(p.slots, p.tiles), 256, 0, st>>>(s, (const T*)X, (const A*)W, (const A*)bias, regions, (const uint32_t*)work, (T*)Z);
         });
     });
     DBK_LAUNCH_OK();
@@ -389,10 +445,10 @@ int dbk_causalconv_bprop(dbk_stream_t stream, int dtype, const void* X, size_t l
     with_row_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
-        with_taps(taps, [&](auto k) {
-            k_conv_bprop<T, k.value><<<dim3(p.units, p.tiles), 256, 0, st>>>(s, lddz, (const T*)X, (const A*)W, (const A*)bias, regions, (const T*)dZ, (T*)dX, (A*)part, marks);
+        with_taps(taps, D % conv_width(dtype) == 0, [&](auto k, auto exact) {
+            k_conv_bprop<T, k.value, exact.value><<<dim3(p.units, p.tiles), 256, 0, st>>>(s, lddz, (const T*)X, (const A*)W, (const A*)bias, regions, (const T*)dZ, (T*)dX, (A*)part, marks);
             if (p.slots)
-                k_conv_bprop_long<T, k.value><<<dim3(p.slot_units, p.tiles), 256, 0, st>>>(s, lddz, p.slots, p.units, (const T*)X, (const A*)W, (const A*)bias, regions, marks,
+                k_conv_bprop_long<T, k.value, exact.value><<<dim3(p.slot_units, p.tiles), 256, 0, st>>>(s, lddz, p.slots, p.units, (const T*)X, (const A*)W, (const A*)bias, regions, marks,
                                                                                          (const T*)dZ, (T*)dX, (A*)part);
         });
     });
@@ -407,12 +463,13 @@ int dbk_causalconv_step(dbk_stream_t stream, int dtype, const void* X, size_t ld
     DBK_CHECK(!n || !D || taps == 1 || (state && into), "ValueError: null state");
     if (!n || !D) { clear_error(); return 0; }
     const conv_shape s = {(unsigned)n, (unsigned)D, (unsigned)n, 0u, 0u, (unsigned)(silu != 0), ldx, ldz};
-    const size_t vecs = (D + 16 / row_size(dtype) - 1) / (16 / row_size(dtype));
+    const size_t vecs = (D + conv_width(dtype) - 1) / conv_width(dtype);
     hipStream_t st = as_stream(stream);
     with_row_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
-        with_taps(taps, [&](auto k) {
+        with_taps(taps, D % conv_width(dtype) == 0, [&](auto k, auto exact) {
+            (void)exact;
             k_conv_step<T, k.value><<<divup(n * vecs, 256), 256, 0, st>>>(s, (const T*)X, (const A*)W, (const A*)bias, (const T*)state, (T*)into, (T*)Z);
         });
     });

@@ -51,38 +51,6 @@ template <int LANES, typename A> __device__ __forceinline__ void lanes_sum2(A& u
     }
 }
 
-// 16 bytes as they lie in memory, zeros where the chunk ends. EXACT: chunks are whole vectors, so a vector is there or not.
-template <typename T, bool EXACT> struct raw_vec {
-    static constexpr int N = row_vec<T>::N;
-    typedef typename acc_of<T>::type A;
-    typename row_vec<T>::raw r;
-    __device__ __forceinline__ void load(const T* p, unsigned valid)
-    {
-        if (EXACT || valid >= (unsigned)N || valid == 0) {
-            if (valid) r = *reinterpret_cast<const typename row_vec<T>::raw*>(p);
-            else
-#pragma unroll
-                for (int i = 0; i < N; ++i) r[i] = (T)A(0);
-        } else {
-#pragma unroll
-            for (int i = 0; i < N; ++i) r[i] = i < (int)valid ? p[i] : (T)A(0);
-        }
-    }
-    __device__ __forceinline__ A operator[](int i) const { return (A)r[i]; }
-    // (what was converted is not kept for the next time)
-    __device__ __forceinline__ void forget()
-    {
-        if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(r));
-    }
-};
-template <typename T, bool EXACT> __device__ __forceinline__ void store_vec(const row_vec<T>& v, T* p, unsigned valid)
-{
-    if (EXACT) {
-        if (valid) v.store(p, row_vec<T>::N);
-    } else
-        v.store(p, valid);
-}
-
 // A row's values come while the row before it is worked on, and stay as they lie in memory: for bfloat16 half the registers of what is
 // computed from them, which is computed twice instead.
 template <typename T, int LANES, int NV, bool EXACT>
@@ -147,7 +115,7 @@ __global__ __launch_bounds__(256) void k_norm_fprop(norm_shape p, const T* __res
             x[i].forget();
 #pragma unroll
             for (int j = 0; j < V; ++j) o.v[j] = fma((x[i][j] - mean) * rstd, g[i][j], b[i][j]);
-            store_vec<T, EXACT>(o, z + i * LANES * V, valid[i]);
+            store_vec<EXACT>(o, z + i * LANES * V, valid[i]);
         }
         if (stats && own && lane == 0) {
             const size_t at = (size_t)now * p.nchunk + chunk;
@@ -235,7 +203,7 @@ __global__ __launch_bounds__(256) void k_norm_bprop(norm_shape p, size_t lddz, c
                 const A h = (x[i][j] - mean) * rstd;
                 o.v[j] = rstd * (fma(d[i][j], g[i][j], -s1) - h * s2);
             }
-            store_vec<T, EXACT>(o, dx + i * LANES * V, valid[i]);
+            store_vec<EXACT>(o, dx + i * LANES * V, valid[i]);
         }
     }
     if (!part) return;
@@ -380,6 +348,7 @@ __global__ __launch_bounds__(1024) void k_sum_partials(const A* __restrict__ par
     const size_t c = (size_t)blockIdx.x * 16u + x;
     A s = 0;
     if (c < ncol)
+#pragma unroll 8
         for (size_t u = y; u < units; u += 64u) s += part[u * ncol + c];
     lds[y][x] = s;
     __syncthreads();
@@ -437,7 +406,7 @@ norm_plan plan_norm(int dtype, size_t n, size_t m, size_t group)
     p.ct_log2 = best;
     const unsigned rt = p.lanes ? (256u / p.lanes) >> best : 1u;
     p.gy = p.lanes ? divup(nchunk, size_t(1) << best) : 1u;
-    const unsigned most = NORM_WGS / p.gy ? NORM_WGS / p.gy : 1u;
+    const unsigned wgs = p.nv > 1 ? NORM_WGS / 2 : NORM_WGS, most = wgs / p.gy ? wgs / p.gy : 1u;      // (several vectors: two waves per SIMD fit)
     p.gx = divup(n, rt);
     if (p.gx > most) p.gx = most;
     p.shape.n = (unsigned)n;

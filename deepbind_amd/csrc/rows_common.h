@@ -25,12 +25,12 @@ template <typename F> inline void with_row_type(int dtype, F f)
     else f(bf16_t());
 }
 
-// 16 bytes of T in the accumulation type. Global memory takes vector accesses at any element's address, so odd row
+// 16 bytes of T (W elements) in the accumulation type. Global memory takes vector accesses at any element's address, so odd row
 // strides and odd widths use the same code as aligned ones; only a row's last, incomplete vector goes element by element.
-template <typename T> struct row_vec {
-    static constexpr int N = 16 / sizeof(T);
+template <typename T, int W = 16 / sizeof(T)> struct row_vec {
+    static constexpr int N = W;
     typedef typename acc_of<T>::type A;
-    typedef T raw __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
+    typedef T raw __attribute__((ext_vector_type(W), aligned(sizeof(T))));
     A v[N];
     __device__ __forceinline__ void load(const T* p, unsigned valid)
     {
@@ -61,6 +61,38 @@ template <typename T> struct row_vec {
         for (int i = 0; i < N; ++i) v[i] = x;
     }
 };
+// A vector as it lies in memory, zeros behind its `valid` elements. EXACT: rows are whole vectors, so a vector is there or not.
+template <typename T, bool EXACT, int W = 16 / sizeof(T)> struct raw_vec {
+    static constexpr int N = W;
+    typedef typename acc_of<T>::type A;
+    typename row_vec<T, W>::raw r;
+    __device__ __forceinline__ void load(const T* p, unsigned valid)
+    {
+        if (EXACT || valid >= (unsigned)N || valid == 0) {
+            if (valid) r = *reinterpret_cast<const typename row_vec<T, W>::raw*>(p);
+            else
+#pragma unroll
+                for (int i = 0; i < N; ++i) r[i] = (T)A(0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) r[i] = i < (int)valid ? p[i] : (T)A(0);
+        }
+    }
+    __device__ __forceinline__ A operator[](int i) const { return (A)r[i]; }
+    // (what was converted is not kept for the next time)
+    __device__ __forceinline__ void forget()
+    {
+        if constexpr (sizeof(T) == 2) asm volatile("" : "+v"(r));
+    }
+};
+template <bool EXACT, typename T, int W> __device__ __forceinline__ void store_vec(const row_vec<T, W>& v, T* p, unsigned valid)
+{
+    if (EXACT) {
+        if (valid) v.store(p, W);
+    } else
+        v.store(p, valid);
+}
+
 // N accumulation-type values (weights) beside one vector of T
 template <typename A, int N> __device__ __forceinline__ void load_weights(A (&w)[N], const A* p, unsigned valid, A other)
 {
