@@ -221,6 +221,44 @@ __device__ __forceinline__ bool cut_segment(const scan_shape& p, const uint32_t*
     return slot_segment(regions, p.nregion, p.N, marks, slot, seg, r, g, k) && is_cut(g, seg);
 }
 size_t bprop_work_bytes(const dbk_statescan_args& a);            // statescan_bprop.hip
+// One state's way through n segments: s = local + exp2(a2 * sum) s after each, written to out; the three pointers start at the first and move
+// on by `step` (sums by `sum_step`). U segments' values are on their way while U others are worked on.
+template <typename A> __device__ __forceinline__ void carry_chain(A a2, A s, unsigned n, const A* local, const A* sums, A* out, size_t step, size_t sum_step)
+{
+    constexpr unsigned U = 8;
+    A add[U], sum[U];
+    auto fetch = [&](unsigned left) {
+#pragma unroll
+        for (unsigned i = 0; i < U; ++i) {
+            add[i] = *local;
+            sum[i] = *sums;
+            local += i + 1u < left ? step : 0;
+            sums += i + 1u < left ? sum_step : 0;
+        }
+    };
+    if (!n) return;
+    fetch(n);
+    for (unsigned k = 0; k < n; k += U) {
+        A av[U], sv[U];
+#pragma unroll
+        for (unsigned i = 0; i < U; ++i) { av[i] = add[i]; sv[i] = exp2_fast(a2 * sum[i]); }
+        if (k + U < n) fetch(n - k - U);
+#pragma unroll
+        for (unsigned i = 0; i < U; ++i) {
+            if (k + i >= n) break;
+            s = fma_a(sv[i], s, av[i]);
+            *out = s;
+            out += step;
+        }
+    }
+}
+// workgroups per region for the carries: few regions share the chip, many take little of it each
+inline unsigned carry_blocks(const dbk_statescan_args& a)
+{
+    const size_t need = (a.S * a.D + 255) / 256, room = 2048 / a.nregion + 1;
+    return (unsigned)(need < room ? need : room);
+}
+
 int mark_cut_regions(hipStream_t st, const uint32_t* regions, size_t nregion, size_t N, unsigned seg, uint32_t* marks);
 
 }  // namespace dbk

@@ -123,34 +123,18 @@ __global__ __launch_bounds__(256) void k_scan_fprop(scan_shape p, unsigned seg, 
 }
 
 // The state in front of every segment of a cut region from the one in front of the segment before: what that one makes of zeros, and
-// its own carried state times exp(A * sum of its steps). A thread per state and channel; loads run ahead of the chain.
+// its own carried state times exp(A * sum of its steps). A thread per state and channel.
 template <typename A>
 __global__ __launch_bounds__(256) void k_scan_carry(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const A* __restrict__ A_,
                                                     const A* __restrict__ local, const A* __restrict__ sums, A* __restrict__ carry)
 {
-    constexpr unsigned U = 8;
     const row_range g = region_rows(regions, blockIdx.x, p.N);
-    const size_t block = (size_t)p.S * p.D, at = (size_t)blockIdx.y * 256u + threadIdx.x;
-    if (!is_cut(g, seg) || at >= block) return;
-    const size_t ch = at % p.D, first = g.start / seg + 1u;
-    const unsigned n = (g.end - g.start - 1u) / seg;             // segments behind the first
-    const A a2 = A_[at] * A(1.4426950408889634);
-    A h = carry[first * block + at];
-    for (unsigned k = 0; k + 1 < n; k += U) {
-        A add[U], sum[U];
-#pragma unroll
-        for (unsigned i = 0; i < U; ++i) {
-            const size_t s = first + min(k + i, n - 2u);
-            add[i] = local[s * block + at];
-            sum[i] = sums[s * p.D + ch];
-        }
-#pragma unroll
-        for (unsigned i = 0; i < U; ++i) {
-            if (k + i + 1 >= n) break;
-            h = fma_a(exp2_fast(a2 * sum[i]), h, add[i]);
-            carry[(first + k + i + 1u) * block + at] = h;
-        }
-    }
+    if (!is_cut(g, seg)) return;
+    const size_t block = (size_t)p.S * p.D, first = g.start / seg + 1u;
+    const unsigned n = (g.end - g.start - 1u) / seg;             // segments behind the first; the state in front of the first of them is there
+    for (size_t at = (size_t)blockIdx.y * 256u + threadIdx.x; at < block; at += (size_t)gridDim.y * 256u)
+        carry_chain<A>(A_[at] * A(1.4426950408889634), carry[first * block + at], n - 1u, local + first * block + at, sums + first * p.D + at % p.D,
+                       carry + (first + 1u) * block + at, block, p.D);
 }
 
 // The rows of every segment behind the first, from the state carried to it.
@@ -288,7 +272,7 @@ int dbk_statescan(dbk_stream_t stream, const dbk_statescan_args* a, void* work, 
                     s, p.seg, a->regions, g.marks, (const T*)a->X, (const T*)a->dt, (const A*)a->A, (const A*)a->B, (const A*)a->C, (const A*)a->skip, (const T*)a->gate,
                     (const A*)a->dt_bias, (const A*)a->state, (T*)a->Y, (A*)a->last, (A*)a->keep, (A*)g.local, (A*)g.steps, (A*)g.carry);
                 if (!p.slots) return;
-                k_scan_carry<A><<<dim3((unsigned)a->nregion, divup(a->S * a->D, 256)), 256, 0, st>>>(s, p.seg, a->regions, (const A*)a->A, (const A*)g.local, (const A*)g.steps,
+                k_scan_carry<A><<<dim3((unsigned)a->nregion, carry_blocks(*a)), 256, 0, st>>>(s, p.seg, a->regions, (const A*)a->A, (const A*)g.local, (const A*)g.steps,
                                                                                               (A*)g.carry);
                 k_scan_fprop_cut<T, lanes.value, ns.value><<<dim3(p.slots, divup(p.tiles, waves)), dim3(64, waves), 0, st>>>(
                     s, p.seg, a->regions, g.marks, (const T*)a->X, (const T*)a->dt, (const A*)a->A, (const A*)a->B, (const A*)a->C, (const A*)a->skip, (const T*)a->gate,

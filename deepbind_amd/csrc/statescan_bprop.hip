@@ -67,39 +67,81 @@ template <typename T> struct scan_rows_in {      // what the backward pass reads
 };
 template <typename T> struct scan_rows_out { T *dX, *ddt, *dgate; };
 
-// B and C of a chunk's rows in LDS, [row][B, C][group of the wave][S rounded up to fours], zeros behind the last row and state: in LDS rather than
-// in scalar registers, for which a row's work is too short to hide the loads of the next row's.
-template <typename T, int LG>
-__device__ __forceinline__ void stage_weights(const scan_shape& p, unsigned lane, unsigned nrow, size_t row0, const scan_rows_in<T>& in, typename acc_of<T>::type* bc)
-{
+// What a chunk of nrow <= 8 rows needs from memory, fetched into registers while the chunk behind it is worked on: the rows of its channels, and
+// its share of B and C, which then lie in LDS as [row][B, C][group of the wave][state], zeros behind the last row and state (in LDS rather
+// than in scalar registers, for which a row's work is too short to hide the loads of the next row's). With more than 16 states
+// the weights come when they are needed.
+template <typename T, int LG> struct scan_raw {
     typedef typename acc_of<T>::type A;
-    constexpr unsigned GW = 64 / LG;
-    const unsigned pad = (p.S + 3u) / 4u * 4u, width = 2u * GW * pad;
-    const unsigned first = LG == 64 ? blockIdx.y / p.tpg : blockIdx.y * GW;
-    unsigned across = 64;                        // lanes for one row: several rows at a time where they are few
-    while (across / 2u >= width) across /= 2u;
-    for (unsigned i = lane % across; i < width; i += across) {
-        const unsigned g = i / pad % GW, s = i % pad;
-        const bool c = i >= GW * pad, here = s < p.S && first + g < p.G;
-        const A* from = (c ? in.C + row0 * p.ldc : in.B + row0 * p.ldb) + (size_t)(first + g) * p.S + s;
-        const size_t ld = c ? p.ldc : p.ldb;
-#pragma unroll 8
-        for (unsigned r = lane / across; r < SCAN_CHUNK; r += 64u / across) bc[r * width + i] = here && r < nrow ? from[r * ld] : A(0);
+    static constexpr int R = SCAN_CHUNK, GW = 64 / LG, WIDTH = 2 * GW * 16, NW = R * WIDTH / 64;
+    T x[R], d[R], e[R], g[R];
+    A w[NW];
+    // (rows behind the chunk's last one repeat it)
+    __device__ __forceinline__ void fetch(const scan_shape& p, const scan_bshape& bp, const scan_lane& l, unsigned lane, unsigned nrow, size_t row0, const scan_rows_in<T>& in)
+    {
+        const unsigned place = opaque(l.ch * (unsigned)sizeof(T));
+        const T *xp = in.X + row0 * p.ldx, *dp = in.dt + row0 * p.lddt, *ep = in.dY + row0 * bp.lddy;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            x[i] = lane_load(xp, place);
+            d[i] = lane_load(dp, place);
+            e[i] = lane_load(ep, place);
+            const bool more = i + 1 < (int)nrow;
+            xp += more ? p.ldx : 0;
+            dp += more ? p.lddt : 0;
+            ep += more ? bp.lddy : 0;
+        }
+        if (in.gate) {
+            const T* gp = in.gate + row0 * p.ldg;
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                g[i] = lane_load(gp, place);
+                gp += i + 1 < (int)nrow ? p.ldg : 0;
+            }
+        }
+        if (p.S > 16u) return;
+        const unsigned first = first_group<LG>(p, blockIdx.y);
+#pragma unroll
+        for (int n = 0; n < NW; ++n) {
+            const unsigned at = lane % 64u + 64u * n, in_row = at % WIDTH, r = at / WIDTH, gr = in_row % (GW * 16) / 16, s = in_row % 16u;
+            const bool c = in_row >= GW * 16;
+            const A* from = (c ? in.C + row0 * p.ldc : in.B + row0 * p.ldb) + ((size_t)r * (c ? p.ldc : p.ldb) + (size_t)(first + gr) * p.S + s);
+            w[n] = s < p.S && first + gr < p.G && r < nrow ? *from : A(0);
+        }
     }
-    __builtin_amdgcn_wave_barrier();             // (one wave: LDS keeps its order)
-}
+    __device__ __forceinline__ void put(const scan_shape& p, unsigned lane, unsigned nrow, size_t row0, const scan_rows_in<T>& in, A* bc) const
+    {
+        if (p.S <= 16u) {
+#pragma unroll
+            for (int n = 0; n < NW; ++n) bc[lane + 64 * n] = w[n];
+        } else {
+            const unsigned pad = (p.S + 3u) / 4u * 4u, width = 2u * GW * pad, first = first_group<LG>(p, blockIdx.y);
+            for (unsigned i = lane; i < width; i += 64u) {
+                const unsigned gr = i / pad % GW, s = i % pad;
+                const bool c = i >= GW * pad, here = s < p.S && first + gr < p.G;
+                const A* from = (c ? in.C + row0 * p.ldc : in.B + row0 * p.ldb) + (size_t)(first + gr) * p.S + s;
+                const size_t ld = c ? p.ldc : p.ldb;
+#pragma unroll
+                for (unsigned r = 0; r < (unsigned)R; ++r) bc[r * width + i] = here && r < nrow ? from[r * ld] : A(0);
+            }
+        }
+        __builtin_amdgcn_wave_barrier();         // (one wave: LDS keeps its order)
+    }
+};
+template <typename T> __device__ __forceinline__ unsigned weights_pad(unsigned S) { return S <= 16u ? 16u : (S + 3u) / 4u * 4u; }
 
 // Backward over one chunk of nrow <= 8 rows: the states are formed again from the one kept before it, then the rows are taken from the last
 // to the first; four states at a time, whose values at all rows are in registers, while those of the other states wait in LDS.
 // ag: the gradient that the rows behind send to the chunk's last state, da: dA so far, both [state / 4][lane]; st: two values per
-// row and lane that are needed again at the end (the slope of the step; dY times the gate's derivative); bc: as stage_weights.
+// row and lane that are needed again at the end (the slope of the step; dY times the gate's derivative); bc: the weights (scan_raw). raw: this
+// chunk's values, and on return those of the one in front of it, which starts `ahead` rows earlier (0: there is none).
 template <typename T, int LG>
 __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan_bshape& bp, const scan_lane& l, unsigned lane, unsigned nrow, size_t row0,
                                                  const scan_rows_in<T>& in, const typename acc_of<T>::type* A_, typename acc_of<T>::type skip,
                                                  typename acc_of<T>::type bias, const typename acc_of<T>::type* before,
                                                  quad<typename acc_of<T>::type>* ag, quad<typename acc_of<T>::type>* da, typename acc_of<T>::type* st,
-                                                 typename acc_of<T>::type* bc, const scan_rows_out<T>& to, scan_out<typename acc_of<T>::type> out,
-                                                 typename acc_of<T>::type& dskip, typename acc_of<T>::type& dbias)
+                                                 typename acc_of<T>::type* bc, scan_raw<T, LG>& raw, unsigned ahead, const scan_rows_out<T>& to,
+                                                 scan_out<typename acc_of<T>::type> out, typename acc_of<T>::type& dskip, typename acc_of<T>::type& dbias)
 {
     typedef typename acc_of<T>::type A;
     constexpr int R = SCAN_CHUNK;
@@ -118,39 +160,18 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
     fetch(0);
     A x[R], d[R], e[R], sB[R], sA[R], y[R];
     {
-        T xr[R], dr[R], er[R], gr[R];
-        // (rows behind the chunk's last one repeat it; all loads are on their way before the first value is used)
-        const T *xp = in.X + row0 * p.ldx, *dp = in.dt + row0 * p.lddt, *ep = in.dY + row0 * bp.lddy;
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            xr[i] = lane_load(xp, place);
-            dr[i] = lane_load(dp, place);
-            er[i] = lane_load(ep, place);
-            const bool more = i + 1 < (int)nrow;
-            xp += more ? p.ldx : 0;
-            dp += more ? p.lddt : 0;
-            ep += more ? bp.lddy : 0;
-        }
-        if (gated) {
-            const T* gp = in.gate + row0 * p.ldg;
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                gr[i] = lane_load(gp, place);
-                gp += i + 1 < (int)nrow ? p.ldg : 0;
-            }
-        }
-        stage_weights<T, LG>(p, lane, nrow, row0, in, bc);
+        raw.put(p, lane, nrow, row0, in, bc);
         if (p.softplus) {
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 A slope;
-                d[i] = softplus_of((A)dr[i] + bias, slope);
+                d[i] = softplus_of((A)raw.d[i] + bias, slope);
                 st[i * 64u + lane] = slope;
             }
         } else {
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                d[i] = (A)dr[i] + bias;
+                d[i] = (A)raw.d[i] + bias;
                 st[i * 64u + lane] = A(1);
             }
         }
@@ -158,22 +179,23 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
 #pragma unroll
         for (int i = 0; i < R; ++i) {
             const bool here = i < (int)nrow;
-            x[i] = here ? (A)xr[i] : A(0);
+            x[i] = here ? (A)raw.x[i] : A(0);
             d[i] = here ? d[i] : A(0);
-            e[i] = here && l.active ? (A)er[i] : A(0);
+            e[i] = here && l.active ? (A)raw.e[i] : A(0);
             sB[i] = sA[i] = A(0);
             y[i] = skip * x[i];
         }
         if (gated) {
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                const A g = (A)gr[i], s = sigmoid_of(g);
+                const A g = (A)raw.g[i], s = sigmoid_of(g);
                 st[(R + i) * 64u + lane] = e[i] * s * fma_a(g, A(1) - s, A(1));
                 e[i] *= g * s;
             }
         }
     }
-    const unsigned pad = (p.S + 3u) / 4u * 4u, width = 2u * (64 / LG) * pad;
+    if (ahead) raw.fetch(p, bp, l, lane, SCAN_CHUNK, row0 - ahead, in);
+    const unsigned pad = weights_pad<T>(p.S), width = 2u * (64 / LG) * pad;
     const A* weights = bc + (lane / LG) * pad;
     for (unsigned q = 0; 4u * q < p.S; ++q) {
         const unsigned left = p.S - 4u * q;
@@ -206,19 +228,12 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
 #pragma unroll
         for (int i = 0; i < R; ++i) x[i] = opaque(x[i]);
         quad<A> g = ag[q * 64u + lane], sum = da[q * 64u + lane];
-        const unsigned top = (nrow + 3u) / 4u * 4u - 1u;
-        bn = *(const quad<A>*)(b + top * width);
-        quad<A> cn = *(const quad<A>*)(c + top * width);
         A rows[R];
 #pragma unroll
         for (int i = R - 1; i >= 0; --i) {
             rows[i] = A(0);
             if ((i & ~3) >= (int)nrow) continue;
-            const quad<A> bi = bn, ci = cn;
-            if (i) {
-                bn = *(const quad<A>*)(b + (i - 1) * width);
-                cn = *(const quad<A>*)(c + (i - 1) * width);
-            }
+            const quad<A> bi = *(const quad<A>*)(b + i * width), ci = *(const quad<A>*)(c + i * width);
             const A dx = d[i] * x[i];
             A v[8];
 #pragma unroll
@@ -239,32 +254,28 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
             v[0] = join<TOP - 1>(v[0], v[2], lane);
             v[1] = join<TOP - 1>(v[1], v[3], lane);
             rows[i] = join<TOP - 2>(v[0], v[1], lane);
+            // and the rows over the bits that are left, the first of them as soon as both are there
+            if (i < R / 2) rows[i] = join<TOP - 3>(rows[i], rows[i + R / 2], lane);
             __builtin_amdgcn_sched_barrier(0);
         }
         ag[q * 64u + lane] = g;
         da[q * 64u + lane] = sum;
-        // and the rows over the bits that are left: lane -> (matrix, state, rows)
+        // lane -> (matrix, state, rows)
         unsigned kind, state;
         if constexpr (LG == 64) {
             kind = lane >> 5;
             state = ((lane >> 4) & 1u) * 2u + ((lane >> 3) & 1u);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) rows[i] = join<2>(rows[i], rows[i + 4], lane);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) rows[i] = join<1>(rows[i], rows[i + 2], lane);
+            rows[0] = join<1>(rows[0], rows[2], lane);
+            rows[1] = join<1>(rows[1], rows[3], lane);
             rows[0] = join<0>(rows[0], rows[1], lane);
         } else if constexpr (LG == 32) {
             kind = (lane >> 4) & 1u;
             state = ((lane >> 3) & 1u) * 2u + ((lane >> 2) & 1u);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) rows[i] = join<1>(rows[i], rows[i + 4], lane);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) rows[i] = join<0>(rows[i], rows[i + 2], lane);
+            rows[0] = join<0>(rows[0], rows[2], lane);
+            rows[1] = join<0>(rows[1], rows[3], lane);
         } else {
             kind = (lane >> 3) & 1u;
             state = ((lane >> 2) & 1u) * 2u + ((lane >> 1) & 1u);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) rows[i] = join<0>(rows[i], rows[i + 4], lane);
         }
         constexpr int LEFT = LG == 64 ? 1 : LG == 32 ? 2 : 4;                  // rows that a lane now holds
         const unsigned base = LG == 64 ? (lane & 1u) + ((lane >> 1) & 1u) * 2u + ((lane >> 2) & 1u) * 4u
@@ -323,10 +334,15 @@ template <typename T, int LG> struct scan_wave {
     __device__ __forceinline__ void rows(const scan_shape& p, const scan_bshape& bp, unsigned start, unsigned from, unsigned n, const scan_rows_in<T>& in,
                                          const scan_rows_out<T>& to, const scan_out<A>& out)
     {
-        for (unsigned c = (n + SCAN_CHUNK - 1u) / SCAN_CHUNK; c-- > 0;) {
+        if (!n) return;
+        scan_raw<T, LG> raw;
+        unsigned c = (n - 1u) / SCAN_CHUNK;
+        raw.fetch(p, bp, l, lane, n - c * SCAN_CHUNK, from + c * SCAN_CHUNK, in);
+        for (;;) {
             const unsigned at = from + c * SCAN_CHUNK, chunk = (at - start) / SCAN_CHUNK;
             scan_chunk_bprop<T, LG>(p, bp, l, lane, min(SCAN_CHUNK, n - c * SCAN_CHUNK), at, in, A_, sk, bi, chunk ? kept_at(p, in.keep, start, chunk) : (const A*)nullptr,
-                                    ag, da, st, bc, to, out, dskip, dbias);
+                                    ag, da, st, bc, raw, c ? SCAN_CHUNK : 0u, to, out, dskip, dbias);
+            if (c-- == 0) break;
         }
     }
     __device__ __forceinline__ void leave(const scan_shape& p, A* part)
@@ -349,29 +365,45 @@ template <int LG, typename A> __device__ __forceinline__ scan_out<A> tile_share(
 }
 
 // A wave per tile of channels takes its share of the regions one after another, with dA in LDS, and leaves one block of sums:
-// part[unit][S + 2][D]. Of a region that is cut it takes the last segment, behind which nothing sends anything.
+// part[unit][S + 2][D]. Of a region that is cut it takes the last segment, behind which nothing sends anything. Units from unit0 on
+// take the other segments: the slot of segment k stands for segment k - 1, to which segment k sends what lies in the slot's carry.
 template <typename T, int LG>
-__global__ __launch_bounds__(64, 2) void k_scan_bprop(scan_shape p, scan_bshape bp, unsigned seg, scan_rows_in<T> in, const typename acc_of<T>::type* __restrict__ A_,
-                                                   const typename acc_of<T>::type* __restrict__ skip, const typename acc_of<T>::type* __restrict__ bias,
-                                                   scan_rows_out<T> to, scan_out<typename acc_of<T>::type> out, size_t tile_stride,
-                                                   typename acc_of<T>::type* __restrict__ part, typename acc_of<T>::type* __restrict__ carry)
+__global__ __launch_bounds__(64, 2) void k_scan_bprop(scan_shape p, scan_bshape bp, unsigned seg, unsigned unit0, unsigned nslot, scan_rows_in<T> in,
+                                                      const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ skip,
+                                                      const typename acc_of<T>::type* __restrict__ bias, scan_rows_out<T> to,
+                                                      scan_out<typename acc_of<T>::type> out, size_t tile_stride, typename acc_of<T>::type* __restrict__ part,
+                                                      const typename acc_of<T>::type* __restrict__ carry)
 {
     typedef typename acc_of<T>::type A;
     extern __shared__ char lds_raw[];
     scan_wave<T, LG> w(p, lds_raw, A_, skip, bias);
     out = tile_share<LG>(p, out, tile_stride);
-    for (unsigned r = blockIdx.x; r < p.nregion; r += gridDim.x) {
-        const row_range g = region_rows(in.regions, r, p.N);
-        if (g.start == g.end) continue;
-        states_from(p, w.l, w.lane, w.ag, (const A*)nullptr);
-        const unsigned k = in.marks && is_cut(g, seg) ? (g.end - g.start - 1u) / seg : 0u;
-        w.rows(p, bp, g.start, g.start + k * seg, g.end - g.start - k * seg, in, to, out);
-        if (k) states_to(p, w.l, w.lane, w.ag, carry + (size_t)(g.start / seg + k) * p.S * p.D);
+    const bool slots = blockIdx.x >= unit0;
+    const unsigned step = slots ? gridDim.x - unit0 : unit0, stop = slots ? nslot : p.nregion;
+    for (unsigned i = slots ? blockIdx.x - unit0 : blockIdx.x; i < stop; i += step) {
+        row_range g;
+        unsigned from, n;
+        const A* sent = nullptr;
+        if (slots) {
+            unsigned r, k;
+            if (!cut_segment(p, in.regions, in.marks, i, seg, r, g, k)) continue;
+            from = g.start + (k - 1u) * seg;
+            n = seg;
+            sent = carry + (size_t)i * p.S * p.D;
+        } else {
+            g = region_rows(in.regions, i, p.N);
+            if (g.start == g.end) continue;
+            from = g.start + (in.marks && is_cut(g, seg) ? (g.end - g.start - 1u) / seg * seg : 0u);
+            n = g.end - from;
+        }
+        // (a lane without a channel adds nothing to its group's sums: its e is zero, and so is what is sent to it)
+        states_from(p, w.l, w.lane, w.ag, w.l.active ? sent : (const A*)nullptr);
+        w.rows(p, bp, g.start, from, n, in, to, out);
     }
     w.leave(p, part + (size_t)blockIdx.x * (p.S + 2u) * p.D);
 }
 
-// What a middle segment sends back when nothing is sent to it, and the sum of its steps: the states' gradients alone.
+// What a segment behind the first sends back when nothing is sent to it, and the sum of its steps: the states' gradients alone.
 template <typename T, int LG, int NS>
 __global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t lddy, unsigned seg, scan_rows_in<T> in, const typename acc_of<T>::type* __restrict__ A_,
                                                          const typename acc_of<T>::type* __restrict__ bias, typename acc_of<T>::type* __restrict__ local,
@@ -383,7 +415,7 @@ __global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t ld
     __shared__ A lds[weights::SIZE];
     unsigned r, k;
     row_range g;
-    if (!cut_segment(p, in.regions, in.marks, blockIdx.x, seg, r, g, k) || g.start + (uint64_t)(k + 1u) * seg >= g.end) return;
+    if (!cut_segment(p, in.regions, in.marks, blockIdx.x, seg, r, g, k)) return;
     const scan_lane l = lane_channel<LG>(p, blockIdx.y, threadIdx.x);
     const A bi = bias ? bias[l.ch] : A(0);
     A a2[NS], ag[NS], steps = 0;
@@ -391,26 +423,28 @@ __global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t ld
     regs_from(p, l, ag, (const A*)nullptr, A(1));
     const size_t row = (size_t)g.start + (size_t)k * seg;
     const unsigned place = opaque(l.ch * (unsigned)sizeof(T));
-    weights w(p, threadIdx.x, first_group<LG>(p, blockIdx.y), (const A*)nullptr, in.C + row * p.ldc, lds, seg - U, true);
+    const unsigned n = min(seg, g.end - (unsigned)row), up = (n + U - 1u) / U * U;
+    weights w(p, threadIdx.x, first_group<LG>(p, blockIdx.y), (const A*)nullptr, in.C + row * p.ldc, lds, up - U, true);
     T dn[U], en[U], gn[U];
-    auto fetch = [&](unsigned t) {               // rows t .. t + U - 1 of the segment (a multiple of 8 rows)
+    auto fetch = [&](unsigned t) {               // rows t .. t + U - 1 of the segment (behind its last row: that one again)
 #pragma unroll
         for (unsigned i = 0; i < U; ++i) {
-            const size_t at = row + t + i;
+            const size_t at = row + min(t + i, n - 1u);
             dn[i] = lane_load(in.dt + at * p.lddt, place);
             en[i] = lane_load(in.dY + at * lddy, place);
             if (in.gate) gn[i] = lane_load(in.gate + at * p.ldg, place);
         }
-        w.fetch(U);
+        w.fetch(n - t);
     };
-    fetch(seg - U);
-    for (unsigned left = seg; left > 0; left -= U) {
+    fetch(up - U);
+    for (unsigned left = up; left > 0; left -= U) {
         A d[U], e[U];
 #pragma unroll
         for (unsigned i = 0; i < U; ++i) {
             A slope;
             d[i] = step_of(p, (A)dn[i] + bi, slope);
             e[i] = (A)en[i];
+            if (left - U + i >= n) d[i] = e[i] = A(0);
             if (in.gate) { const A gg = (A)gn[i]; e[i] *= gg * sigmoid_of(gg); }
         }
         w.put();
@@ -431,58 +465,19 @@ __global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t ld
     if (l.active) sums[(size_t)blockIdx.x * p.D + l.ch] = steps;
 }
 
-// carry[slot of segment k]: what segment k >= 1 of a cut region sends to the one before it; the last segment's is there.
+// carry[slot of segment k]: what segment k >= 1 of a cut region sends to the one before it, from the last segment to the first: what it sends
+// by itself, and exp(A * sum of its steps) times what it is sent. Loads run ahead of the chain.
 template <typename A>
 __global__ __launch_bounds__(256) void k_scan_carry_back(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const A* __restrict__ A_,
                                                          const A* __restrict__ local, const A* __restrict__ sums, A* __restrict__ carry)
 {
-    constexpr unsigned U = 8;
     const row_range g = region_rows(regions, blockIdx.x, p.N);
-    const size_t block = (size_t)p.S * p.D, at = (size_t)blockIdx.y * 256u + threadIdx.x;
-    if (!is_cut(g, seg) || at >= block) return;
-    const size_t ch = at % p.D, zero = g.start / seg;
+    if (!is_cut(g, seg)) return;
+    const size_t block = (size_t)p.S * p.D, zero = g.start / seg;
     const unsigned n = (g.end - g.start - 1u) / seg;             // the last segment
-    const A a2 = A_[at] * A(1.4426950408889634);
-    A s = carry[(zero + n) * block + at];
-    for (unsigned k = n - 1u; k > 0;) {
-        A add[U], sum[U];
-#pragma unroll
-        for (unsigned i = 0; i < U; ++i) {
-            const size_t slot = zero + (k > i ? k - i : 1u);
-            add[i] = local[slot * block + at];
-            sum[i] = sums[slot * p.D + ch];
-        }
-#pragma unroll
-        for (unsigned i = 0; i < U; ++i) {
-            if (!k) break;
-            s = fma_a(exp2_fast(a2 * sum[i]), s, add[i]);
-            carry[(zero + k) * block + at] = s;
-            --k;
-        }
-    }
-}
-
-// The segments before the last one: the slot of segment k stands for segment k - 1, which takes in what segment k sends.
-template <typename T, int LG>
-__global__ __launch_bounds__(64, 2) void k_scan_bprop_cut(scan_shape p, scan_bshape bp, unsigned seg, unsigned nslot, unsigned unit0, scan_rows_in<T> in,
-                                                       const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ skip,
-                                                       const typename acc_of<T>::type* __restrict__ bias, scan_rows_out<T> to,
-                                                       scan_out<typename acc_of<T>::type> out, size_t tile_stride, typename acc_of<T>::type* __restrict__ part,
-                                                       const typename acc_of<T>::type* __restrict__ carry)
-{
-    typedef typename acc_of<T>::type A;
-    extern __shared__ char lds_raw[];
-    scan_wave<T, LG> w(p, lds_raw, A_, skip, bias);
-    out = tile_share<LG>(p, out, tile_stride);
-    for (unsigned slot = blockIdx.x; slot < nslot; slot += gridDim.x) {
-        unsigned r, k;
-        row_range g;
-        if (!cut_segment(p, in.regions, in.marks, slot, seg, r, g, k)) continue;
-        // (a lane without a channel adds nothing to its group's sums: its e is zero, and so is what is sent to it)
-        states_from(p, w.l, w.lane, w.ag, w.l.active ? carry + (size_t)slot * p.S * p.D : (const A*)nullptr);
-        w.rows(p, bp, g.start, g.start + (k - 1u) * seg, seg, in, to, out);
-    }
-    w.leave(p, part + (size_t)(unit0 + blockIdx.x) * (p.S + 2u) * p.D);
+    for (size_t at = (size_t)blockIdx.y * 256u + threadIdx.x; at < block; at += (size_t)gridDim.y * 256u)
+        carry_chain<A>(A_[at] * A(1.4426950408889634), A(0), n, local + (zero + n) * block + at, sums + (zero + n) * p.D + at % p.D, carry + (zero + n) * block + at,
+                       0 - block, 0 - (size_t)p.D);
 }
 
 // dB and dC from the tiles' shares, in the tiles' order: a region's rows (its first segment's where it is cut), or another segment's.
@@ -503,9 +498,10 @@ __global__ __launch_bounds__(256) void k_scan_weights(scan_shape p, unsigned seg
         g.end = min(g.end, from + seg);
     }
     const size_t n = (size_t)(g.end - from) * 2u * ncol;
-    for (size_t i = threadIdx.x; i < n; i += 256u) {
+    for (size_t i = (size_t)blockIdx.y * 256u + threadIdx.x; i < n; i += (size_t)gridDim.y * 256u) {
         const size_t row = from + i / (2u * ncol), c = i % (2u * ncol);
         A s = 0;
+#pragma unroll 4
         for (unsigned t = 0; t < tiles; ++t) s += share[t * tile_stride + row * 2u * ncol + c];
         if (c < ncol) dB[row * lddb + c] = s;
         else dC[row * lddc + c - ncol] = s;
@@ -580,22 +576,22 @@ int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* a, void* 
         const scan_out<A> out = shared ? scan_out<A>{share, share + ncol, 2 * ncol, 2 * ncol} : scan_out<A>{(A*)a->dB, (A*)a->dC, a->lddb, a->lddc};
         const scan_rows_in<T> in = {(const T*)a->X, (const T*)a->dt, (const T*)a->gate, (const T*)a->dY, (const A*)a->B, (const A*)a->C, (const A*)a->keep, a->regions, y.seg.marks};
         const scan_rows_out<T> to = {(T*)a->dX, (T*)a->ddt, (T*)a->dgate};
-        const size_t quads = (a->S + 3) / 4, lds = quads * 64 * 2 * sizeof(quad<A>) + (2 * 64 + 2 * (64 / p.lanes) * quads * 4) * SCAN_CHUNK * sizeof(A);
+        const size_t quads = (a->S + 3) / 4, pad = a->S <= 16 ? 16 : quads * 4;
+        const size_t lds = quads * 64 * 2 * sizeof(quad<A>) + (2 * 64 + 2 * (64 / p.lanes) * pad) * SCAN_CHUNK * sizeof(A);
         with_lanes(p.lanes, [&](auto lanes) {
-            k_scan_bprop<T, lanes.value><<<dim3(y.units, p.tiles), 64, lds, st>>>(s, b, p.seg, in, (const A*)a->A, (const A*)a->skip, (const A*)a->dt_bias, to, out, tile_stride,
-                                                                                 (A*)part, (A*)y.seg.carry);
-            if (!p.slots) return;
-            with_states(a->S, [&](auto ns) {
-                k_scan_bprop_local<T, lanes.value, ns.value><<<dim3(p.slots, p.tiles), 64, 0, st>>>(s, b.lddy, p.seg, in, (const A*)a->A, (const A*)a->dt_bias,
-                                                                                                                (A*)y.seg.local, (A*)y.seg.steps);
-            });
-            k_scan_carry_back<A><<<dim3((unsigned)a->nregion, divup(a->S * a->D, 256)), 256, 0, st>>>(s, p.seg, a->regions, (const A*)a->A, (const A*)y.seg.local,
-                                                                                                (const A*)y.seg.steps, (A*)y.seg.carry);
-            k_scan_bprop_cut<T, lanes.value><<<dim3(y.slot_units, p.tiles), 64, lds, st>>>(s, b, p.seg, p.slots, y.units, in, (const A*)a->A, (const A*)a->skip, (const A*)a->dt_bias,
-                                                                                          to, out, tile_stride, (A*)part, (const A*)y.seg.carry);
+            if (p.slots) {
+                with_states(a->S, [&](auto ns) {
+                    k_scan_bprop_local<T, lanes.value, ns.value><<<dim3(p.slots, p.tiles), 64, 0, st>>>(s, b.lddy, p.seg, in, (const A*)a->A, (const A*)a->dt_bias,
+                                                                                                        (A*)y.seg.local, (A*)y.seg.steps);
+                });
+                k_scan_carry_back<A><<<dim3((unsigned)a->nregion, carry_blocks(*a)), 256, 0, st>>>(s, p.seg, a->regions, (const A*)a->A, (const A*)y.seg.local,
+                                                                                                  (const A*)y.seg.steps, (A*)y.seg.carry);
+            }
+            k_scan_bprop<T, lanes.value><<<dim3(y.units + y.slot_units, p.tiles), 64, lds, st>>>(s, b, p.seg, y.units, p.slots, in, (const A*)a->A, (const A*)a->skip,
+                                                                                                (const A*)a->dt_bias, to, out, tile_stride, (A*)part, (const A*)y.seg.carry);
         });
         if (shared)
-            k_scan_weights<A><<<(unsigned)a->nregion + p.slots, 256, 0, st>>>(s, p.seg, a->regions, y.seg.marks, p.tpg, ncol, share, tile_stride, (A*)a->dB, a->lddb, (A*)a->dC,
+            k_scan_weights<A><<<dim3((unsigned)a->nregion + p.slots, divup((size_t)p.seg * 2 * ncol, 1024)), 256, 0, st>>>(s, p.seg, a->regions, y.seg.marks, p.tpg, ncol, share, tile_stride, (A*)a->dB, a->lddb, (A*)a->dC,
                                                                               a->lddc);
     });
     sum_partials(st, a->dtype, part, y.units + y.slot_units, a->S * a->D, a->dA, a->D, a->dskip, a->D, a->ddt_bias);
