@@ -63,6 +63,17 @@ template <typename A> __device__ __forceinline__ A step_of(const scan_shape& p, 
 
 template <typename A> struct quad { A v[4]; } __attribute__((aligned(16)));
 
+// v[j] += b_j x for four states j of every lane's channel x, where lane l of every four holds b_(l % 4) of its group: the 16 outer products of four by
+// four that v_mfma_f32_4x4x1 forms, lanes being channels and registers states. One instruction beside the vector unit's work in
+// place of four of it.
+__device__ __forceinline__ void outer_add(float (&v)[4], float b, float x)
+{
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    const f4 s = __builtin_amdgcn_mfma_f32_4x4x1f32(b, x, (f4){v[0], v[1], v[2], v[3]}, 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = s[j];
+}
+
 // The first of the groups that a wave's tile covers.
 template <int LG> __device__ __forceinline__ unsigned first_group(const scan_shape& p, unsigned tile) { return LG == 64 ? tile / p.tpg : tile * (64u / LG); }
 
@@ -71,10 +82,12 @@ template <int LG> __device__ __forceinline__ unsigned first_group(const scan_sha
 // channels are of one group, but a scalar load can not run far enough ahead of the rows: there are not the registers.
 constexpr int SCAN_AHEAD = 2;
 template <typename A, int LG, int NS, bool WITH_B, bool WITH_C> struct scan_weights {
+    static constexpr bool MATRIX = WITH_B && sizeof(A) == 4;     // B for the matrix cores
     static constexpr int GW = 64 / LG, PART = GW * NS, ROW = PART * (WITH_B + WITH_C), SIZE = SCAN_AHEAD * ROW, PER = (SIZE + 63) / 64;
     const A *from[PER];
     size_t step[PER];
     bool here[PER];
+    unsigned to[PER];
     A next[PER];
     A *lds, *mine;
     unsigned lane;
@@ -88,6 +101,7 @@ template <typename A, int LG, int NS, bool WITH_B, bool WITH_C> struct scan_weig
             const bool c = WITH_C && in >= (WITH_B ? PART : 0);
             const size_t ld = c ? p.ldc : p.ldb;
             here[i] = at < SIZE && s < p.S && first + g < p.G;
+            to[i] = MATRIX && !c ? at - s + s % 4u * (NS / 4) + s / 4u : at;
             from[i] = (c ? C : B) + (here[i] ? (first_row + at / ROW) * ld + (size_t)(first + g) * p.S + s : 0);
             step[i] = back ? 0 - SCAN_AHEAD * ld : SCAN_AHEAD * ld;
         }
@@ -104,10 +118,16 @@ template <typename A, int LG, int NS, bool WITH_B, bool WITH_C> struct scan_weig
     __device__ __forceinline__ void put()
     {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) if (SIZE % 64 == 0 || lane + 64u * i < SIZE) lds[lane + 64 * i] = next[i];
+        for (int i = 0; i < PER; ++i) if (SIZE % 64 == 0 || lane + 64u * i < SIZE) lds[to[i]] = next[i];
         __builtin_amdgcn_wave_barrier();         // (one wave: LDS keeps its order)
     }
     __device__ __forceinline__ quad<A> b(int r, int q) const { return *(const quad<A>*)(mine + r * ROW + q); }
+    // a lane's share of B where the matrix cores multiply it: state 4 q + lane % 4, one of its own four after another
+    __device__ __forceinline__ void b_of_lane(int r, A (&v)[NS / 4]) const
+    {
+#pragma unroll
+        for (int q = 0; q < NS / 4; ++q) v[q] = mine[r * ROW + (lane % 4u) * (NS / 4) + q];
+    }
     __device__ __forceinline__ quad<A> c(int r, int q) const { return *(const quad<A>*)(mine + r * ROW + (WITH_B ? PART : 0) + q); }
 };
 

@@ -53,11 +53,22 @@ __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& 
             if (t + i >= n) break;
             const A in = d[i] * x[i];
             A y[4] = {skip * x[i], A(0), A(0), A(0)};
+            A bl[NS / 4];
+            if constexpr (weights::MATRIX) w.b_of_lane(i, bl);
 #pragma unroll
             for (int q = 0; q < NS; q += 4) {
-                const quad<A> b = w.b(i, q);
+                if constexpr (weights::MATRIX) {
+                    A v[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) h[q + j] = fma_a(exp2_fast(d[i] * k[q + j]), h[q + j], in * b.v[j]);
+                    for (int j = 0; j < 4; ++j) v[j] = exp2_fast(d[i] * k[q + j]) * h[q + j];
+                    outer_add(v, bl[q / 4], in);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) h[q + j] = v[j];
+                } else {
+                    const quad<A> b = w.b(i, q);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) h[q + j] = fma_a(exp2_fast(d[i] * k[q + j]), h[q + j], in * b.v[j]);
+                }
                 if (OUT) {
                     const quad<A> c = w.c(i, q);
 #pragma unroll
@@ -79,7 +90,7 @@ __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& 
 // Blocks below nregion: a region, all of it or its first segment (the state behind which is carried to the second one); the
 // others: what a segment makes of a zero state, where another one follows.
 template <typename T, int LG, int NS>
-__global__ __launch_bounds__(256) void k_scan_fprop(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
+__global__ __launch_bounds__(256, 4) void k_scan_fprop(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
                                                    const T* __restrict__ X, const T* __restrict__ dt,
                                                    const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ B,
                                                    const typename acc_of<T>::type* __restrict__ C, const typename acc_of<T>::type* __restrict__ skip,
@@ -139,7 +150,7 @@ __global__ __launch_bounds__(256) void k_scan_carry(scan_shape p, unsigned seg, 
 
 // The rows of every segment behind the first, from the state carried to it.
 template <typename T, int LG, int NS>
-__global__ __launch_bounds__(256) void k_scan_fprop_cut(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
+__global__ __launch_bounds__(256, 4) void k_scan_fprop_cut(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
                                                        const T* __restrict__ X, const T* __restrict__ dt,
                                                        const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ B,
                                                        const typename acc_of<T>::type* __restrict__ C, const typename acc_of<T>::type* __restrict__ skip,
