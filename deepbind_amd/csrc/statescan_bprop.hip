@@ -203,8 +203,9 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
         A h[R + 1][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            k.v[j] = j < (int)left ? k.v[j] * A(1.4426950408889634) : A(0);
-            h[0][j] = j < (int)left ? hn.v[j] : A(0);
+            // (states that do not exist follow the last one: their weights and what is sent to them are zero, and so is all they add)
+            k.v[j] *= A(1.4426950408889634);
+            h[0][j] = hn.v[j];
         }
         if (left > 4u) fetch(q + 1u);
         const A *b = weights + 4u * q, *c = b + (64 / LG) * pad;
