@@ -231,7 +231,7 @@ __device__ __forceinline__ void conv_strip_bprop(conv_shape p, size_t lddz, cons
     }
 }
 
-// One row of partial sums per workgroup: part[unit][(K + 1) D]; the strips' sums are added in LDS in their order.
+// One row of partial sums per workgroup: part[unit][(K + 1) D]; the strips' sums are added in LDS, in a fixed order.
 template <typename T, int K>
 __device__ __forceinline__ void conv_leave_sums(conv_shape p, const conv_sums<T, K>& sums, unsigned c, unsigned valid, unsigned unit, typename acc_of<T>::type* part)
 {
@@ -244,15 +244,11 @@ __device__ __forceinline__ void conv_leave_sums(conv_shape p, const conv_sums<T,
         __syncthreads();
 #pragma unroll
         for (int v = 0; v < V; ++v) lds[threadIdx.x][v] = j < K ? sums.dw[j < K ? j : 0][v] : sums.db[v];
-        __syncthreads();
+        sum_strips(lds, across, V);
         if (threadIdx.x >= across) continue;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            if (v >= (int)valid) continue;
-            A a = 0;
-            for (unsigned t = threadIdx.x; t < 256u; t += across) a += lds[t][v];
-            part[((size_t)unit * (K + 1) + j) * p.D + c + v] = a;
-        }
+        for (int v = 0; v < V; ++v)
+            if (v < (int)valid) part[((size_t)unit * (K + 1) + j) * p.D + c + v] = lds[threadIdx.x][v];
     }
 }
 

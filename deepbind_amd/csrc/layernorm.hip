@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256) void k_norm_fprop(norm_shape p, const T* __res
 }
 
 // The backward pass walks the rows the same way and adds dz h and dz up in registers; the workgroup's row lanes are added in
-// LDS at the end, in their order, and leave one row of partial sums per workgroup: part[blockIdx.x][2][nchunk * width].
+// LDS at the end, in a fixed order, and leave one row of partial sums per workgroup: part[blockIdx.x][2][nchunk * width].
 // (Lanes without a column hold dz = 0, which leaves nothing in any sum.)
 template <typename T, int LANES, int NV, bool EXACT>
 __global__ __launch_bounds__(256) void k_norm_bprop(norm_shape p, size_t lddz, const T* __restrict__ X, const typename acc_of<T>::type* __restrict__ gamma,
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256) void k_norm_bprop(norm_shape p, size_t lddz, c
     typedef typename acc_of<T>::type A;
     constexpr int V = row_vec<T>::N;
     __shared__ A lds[8];
-    __shared__ A rows_lds[2][256][V];
+    __shared__ A rows_lds[2][256][V + 1];
     const unsigned unit = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const unsigned chunk = (blockIdx.y << p.ct_log2) + (unit & ((1u << p.ct_log2) - 1u));
     const unsigned first = blockIdx.x * (256u / LANES) >> p.ct_log2;
@@ -214,17 +214,16 @@ __global__ __launch_bounds__(256) void k_norm_bprop(norm_shape p, size_t lddz, c
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < V; ++j) { rows_lds[0][threadIdx.x][j] = dg[i][j]; rows_lds[1][threadIdx.x][j] = db[i][j]; }
-        __syncthreads();
+        sum_strips(rows_lds[0], across, V);
+        sum_strips(rows_lds[1], across, V);
         if (threadIdx.x >= across || !valid[i]) continue;
         const unsigned c = (lane + i * LANES) * V;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             if (j >= (int)valid[i]) continue;
-            A a = 0, b = 0;
-            for (unsigned t = threadIdx.x; t < 256u; t += across) { a += rows_lds[0][t][j]; b += rows_lds[1][t][j]; }
             A* o = part + (size_t)blockIdx.x * 2u * m + (size_t)chunk * p.width + c + j;
-            o[0] = a;
-            o[m] = b;
+            o[0] = rows_lds[0][threadIdx.x][j];
+            o[m] = rows_lds[1][threadIdx.x][j];
         }
     }
 }
@@ -395,12 +394,14 @@ norm_plan plan_norm(int dtype, size_t n, size_t m, size_t group)
     else if (vecs <= 256) p.nv = (int)((vecs + 63) / 64);
     else if (vecs <= 256 * NORM_NV_BLOCK) { p.lanes = 256; p.nv = vecs <= 512 ? 2 : NORM_NV_BLOCK; }
     else p.lanes = 0;
-    // chunks side by side: the power of two that leaves the fewest lanes of its last tile without a chunk, the larger of equals
+    // Chunks side by side: the power of two that costs least, counting the lanes whose chunk does not exist and, against short pieces of
+    // rows, 128 bytes more for every piece.
     unsigned best = 0;
-    size_t waste = ~size_t(0);
+    double least = 1e300;
     for (unsigned c = 0; p.lanes && (unsigned)p.lanes << c <= 256u; ++c) {
-        const size_t tiles = (nchunk + (size_t(1) << c) - 1) >> c, w = (tiles << c) - nchunk;
-        if (w <= waste) { waste = w; best = c; }
+        const size_t tiles = (nchunk + (size_t(1) << c) - 1) >> c;
+        const double cost = (double)(tiles << c) * (1.0 + 128.0 / (double)((size_t)p.lanes * 16 << c));
+        if (cost <= least) { least = cost; best = c; }
         if (tiles == 1) break;
     }
     p.ct_log2 = best;
@@ -438,7 +439,7 @@ int check_norm(int dtype, const void* X, size_t ldx, size_t n, size_t m, size_t 
     DBK_ROW_DTYPE_OK(dtype);
     DBK_CHECK(group >= 1 && m % group == 0, "ValueError: the number of columns must be divisible by the chunk's");
     DBK_CHECK(n < (size_t(1) << 31) && m < (size_t(1) << 31), "ValueError: matrix too large (%zu x %zu)", n, m);
-    DBK_CHECK(m / group <= 65535u || (m / group + 255) / 256 <= 65535u, "ValueError: too many chunks");
+    DBK_CHECK(plan_norm(dtype, 1, m, group).gy <= 65535u && (plan_norm(dtype, 1, m, group).lanes || m / group <= 65535u), "ValueError: too many chunks");
     DBK_CHECK(n == 0 || (X && Z), "ValueError: null matrix");
     DBK_CHECK(n <= 1 || (ldx >= m && ldz >= m), "ValueError: row strides must be at least the number of columns");
     return 0;

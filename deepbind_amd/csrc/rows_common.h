@@ -134,6 +134,17 @@ __device__ __forceinline__ double softplus_of(double x, double& slope)
     return fmax(x, 0.0) + log1p(e);
 }
 
+// Sums over a workgroup's strips of rows, in LDS: v[t] += v[t + 128], v[t + 64], ... down to the first `across` (a power of two) of 256 threads.
+template <typename A, int N> __device__ __forceinline__ void sum_strips(A (*v)[N], unsigned across, int n)
+{
+    for (unsigned o = 128; o >= across; o >>= 1) {
+        __syncthreads();
+        if (threadIdx.x < o)
+            for (int j = 0; j < n; ++j) v[threadIdx.x][j] += v[threadIdx.x + o][j];
+    }
+    __syncthreads();
+}
+
 // Region r's rows, bounded by the map: [start, end), empty where the table says so or lies outside. r is the same in all lanes of a wave, and
 // the compiler is told that what it reads is too: addresses and branches that depend on it are then scalar.
 struct row_range { unsigned start, end; };

@@ -170,7 +170,8 @@ inline scan_plan plan_scan(size_t N, size_t D, size_t G, size_t waves, size_t le
     const size_t share = (N * p.tiles / waves + SCAN_CHUNK - 1) / SCAN_CHUNK * SCAN_CHUNK;
     const size_t seg = share > least ? share : least, most = size_t(1) << 30;
     p.seg = (unsigned)(seg < most ? seg : most);
-    p.slots = N > 2 * (size_t)p.seg ? (unsigned)segment_slots(N, p.seg) : 0u;
+    // (up to 128 rows a second pass and three more launches cost more than one wave's way down them)
+    p.slots = N > 128 && N > 2 * (size_t)p.seg ? (unsigned)segment_slots(N, p.seg) : 0u;
     return p;
 }
 

@@ -369,7 +369,7 @@ template <int LG, typename A> __device__ __forceinline__ scan_out<A> tile_share(
 // part[unit][S + 2][D]. Of a region that is cut it takes the last segment, behind which nothing sends anything. Units from unit0 on
 // take the other segments: the slot of segment k stands for segment k - 1, to which segment k sends what lies in the slot's carry.
 template <typename T, int LG>
-__global__ __launch_bounds__(64, 2) void k_scan_bprop(scan_shape p, scan_bshape bp, unsigned seg, unsigned unit0, unsigned nslot, scan_rows_in<T> in,
+__global__ __launch_bounds__(64, sizeof(T) == 8 ? 1 : 2) void k_scan_bprop(scan_shape p, scan_bshape bp, unsigned seg, unsigned unit0, unsigned nslot, scan_rows_in<T> in,
                                                       const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ skip,
                                                       const typename acc_of<T>::type* __restrict__ bias, scan_rows_out<T> to,
                                                       scan_out<typename acc_of<T>::type> out, size_t tile_stride, typename acc_of<T>::type* __restrict__ part,
