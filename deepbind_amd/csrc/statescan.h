@@ -21,6 +21,7 @@ constexpr unsigned SCAN_CHUNK = 8;               // rows between two kept states
 struct scan_shape {
     unsigned N, D, S, G, gs, nregion;            // rows, channels, states, groups, channels per group, regions
     unsigned tpg, tiles, softplus;               // waves' tiles per group (64 lanes per group), or 0: several groups per wave; all tiles
+    unsigned seg, cut;                           // rows per segment of a region that is cut; regions of more rows than `cut` are
     size_t ldx, lddt, ldb, ldc, ldg, ldy;
 };
 
@@ -153,14 +154,14 @@ template <typename A> __device__ __forceinline__ A* kept_at(const scan_shape& p,
 
 constexpr unsigned SCAN_STATES = 64;             // the most states per channel
 
-// Lanes per group and tiles of channels; rows per segment of a long region and segment slots (0: no region can be long).
-struct scan_plan { int lanes; unsigned tpg, tiles, seg, slots; };
+// Lanes per group and tiles of channels; rows per segment, rows from which on a region is cut, and segment slots (0: none can be).
+struct scan_plan { int lanes; unsigned tpg, tiles, seg, cut, slots; };
 
-// A region of up to two segments is one wave's work, a longer one is cut: its segments' states are first found from zeros (which costs
-// a second pass over its rows), carried over from segment to segment, and the rows then written with the right states in
-// front. The segment is an even share of all rows for `waves` waves: where regions and tiles alone are that many, none is cut.
-
-inline scan_plan plan_scan(size_t N, size_t D, size_t G, size_t waves, size_t least)
+// A region is one wave's work, until it is so long that the others wait for it: then it is cut into segments. The segments' states are first
+// found from zeros (a second pass over the rows, with three more launches), carried over from segment to segment, and the rows
+// then written with the right states in front. The segment is an even share of all rows for `waves` waves, and a region is cut
+// from `shares` of them on, but never one of up to 128 rows, which a wave walks down in the time of the launches.
+inline scan_plan plan_scan(size_t N, size_t D, size_t G, size_t waves, size_t shares, size_t least)
 {
     scan_plan p;
     const size_t gs = D / G;
@@ -168,18 +169,18 @@ inline scan_plan plan_scan(size_t N, size_t D, size_t G, size_t waves, size_t le
     p.tpg = p.lanes == 64 ? divup(gs, 64) : 0u;
     p.tiles = p.lanes == 64 ? (unsigned)(G * p.tpg) : divup(G, 64 / p.lanes);
     const size_t share = (N * p.tiles / waves + SCAN_CHUNK - 1) / SCAN_CHUNK * SCAN_CHUNK;
-    const size_t seg = share > least ? share : least, most = size_t(1) << 30;
+    const size_t seg = share > least ? share : least, most = size_t(1) << 28;
     p.seg = (unsigned)(seg < most ? seg : most);
-    // (up to 128 rows a second pass and three more launches cost more than one wave's way down them)
-    p.slots = N > 128 && N > 2 * (size_t)p.seg ? (unsigned)segment_slots(N, p.seg) : 0u;
+    p.cut = (unsigned)(p.seg * shares > 128 ? p.seg * shares : 128);
+    p.slots = N > p.cut ? (unsigned)segment_slots(N, p.seg) : 0u;
     return p;
 }
 
-inline scan_shape shape_of(const dbk_statescan_args& a)
+inline scan_shape shape_of(const dbk_statescan_args& a, const scan_plan& p)
 {
     scan_shape s;
     s.N = (unsigned)a.N; s.D = (unsigned)a.D; s.S = (unsigned)a.S; s.G = (unsigned)a.G; s.gs = (unsigned)(a.D / a.G); s.nregion = (unsigned)a.nregion;
-    s.tpg = s.tiles = 0; s.softplus = a.softplus != 0;
+    s.tpg = p.tpg; s.tiles = p.tiles; s.seg = p.seg; s.cut = p.cut; s.softplus = a.softplus != 0;
     s.ldx = a.ldx; s.lddt = a.lddt; s.ldb = a.ldb; s.ldc = a.ldc; s.ldg = a.ldgate; s.ldy = a.ldy;
     return s;
 }
@@ -213,7 +214,7 @@ inline int check_scan(const dbk_statescan_args* a)
     DBK_CHECK(!a->N || !a->D || (a->X && a->dt && a->B && a->C), "ValueError: null matrix");
     DBK_CHECK(a->N <= 1 || (a->ldx >= a->D && a->lddt >= a->D && a->ldb >= a->G * a->S && a->ldc >= a->G * a->S && (!a->gate || a->ldgate >= a->D)),
               "ValueError: row strides must be at least the number of columns");
-    DBK_CHECK(plan_scan(0, a->D, a->G, 1, 1).tiles <= 65535u, "ValueError: too many groups (%zu of %zu channels)", a->G, a->G ? a->D / a->G : 0);
+    DBK_CHECK(plan_scan(0, a->D, a->G, 1, 2, 1).tiles <= 65535u, "ValueError: too many groups (%zu of %zu channels)", a->G, a->G ? a->D / a->G : 0);
     return 0;
 }
 
@@ -234,12 +235,10 @@ inline scan_segments segments_in(void* work, const dbk_statescan_args& a, const 
     return s;
 }
 
-// Marks the segments behind the first of every region that is cut: a wave per region.
-__device__ __forceinline__ bool is_cut(row_range g, unsigned seg) { return g.end - g.start > 2u * seg; }
-__device__ __forceinline__ bool cut_segment(const scan_shape& p, const uint32_t* regions, const uint32_t* marks, unsigned slot, unsigned seg,
-                                            unsigned& r, row_range& g, unsigned& k)
+__device__ __forceinline__ bool is_cut(const scan_shape& p, row_range g) { return g.end - g.start > p.cut; }
+__device__ __forceinline__ bool cut_segment(const scan_shape& p, const uint32_t* regions, const uint32_t* marks, unsigned slot, unsigned& r, row_range& g, unsigned& k)
 {
-    return slot_segment(regions, p.nregion, p.N, marks, slot, seg, r, g, k) && is_cut(g, seg);
+    return slot_segment(regions, p.nregion, p.N, marks, slot, p.seg, r, g, k) && is_cut(p, g);
 }
 size_t bprop_work_bytes(const dbk_statescan_args& a);            // statescan_bprop.hip
 // One state's way through n segments: s = local + exp2(a2 * sum) s after each, written to out; the three pointers start at the first and move
@@ -280,6 +279,7 @@ inline unsigned carry_blocks(const dbk_statescan_args& a)
     return (unsigned)(need < room ? need : room);
 }
 
-int mark_cut_regions(hipStream_t st, const uint32_t* regions, size_t nregion, size_t N, unsigned seg, uint32_t* marks);
+// marks the segments behind the first of every region that is cut: a wave per region
+int mark_cut_regions(hipStream_t st, const scan_shape& p, const uint32_t* regions, uint32_t* marks);
 
 }  // namespace dbk

@@ -90,7 +90,7 @@ __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& 
 // Blocks below nregion: a region, all of it or its first segment (the state behind which is carried to the second one); the
 // others: what a segment makes of a zero state, where another one follows.
 template <typename T, int LG, int NS>
-__global__ __launch_bounds__(256, 4) void k_scan_fprop(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
+__global__ __launch_bounds__(256, 4) void k_scan_fprop(scan_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
                                                    const T* __restrict__ X, const T* __restrict__ dt,
                                                    const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ B,
                                                    const typename acc_of<T>::type* __restrict__ C, const typename acc_of<T>::type* __restrict__ skip,
@@ -113,22 +113,22 @@ __global__ __launch_bounds__(256, 4) void k_scan_fprop(scan_shape p, unsigned se
     if (blockIdx.x < p.nregion) {
         const unsigned r = blockIdx.x;
         const row_range g = region_rows(regions, r, p.N);
-        const bool cut = marks && is_cut(g, seg);
+        const bool cut = marks && is_cut(p, g);
         regs_from(p, l, a2, A_, A(1.4426950408889634));
         regs_from(p, l, h, state ? state + (size_t)r * block : (const A*)nullptr, A(1));
-        scan_rows<T, LG, NS, true>(p, l, threadIdx.x, first, g.start, cut ? seg : g.end - g.start, X, dt, gate, B, C, sk, bi, h, a2, Y,
+        scan_rows<T, LG, NS, true>(p, l, threadIdx.x, first, g.start, cut ? p.seg : g.end - g.start, X, dt, gate, B, C, sk, bi, h, a2, Y,
                                          keep ? kept_at(p, keep, g.start, 0u) : (A*)nullptr, steps, lds);
-        if (cut) regs_to(p, l, h, carry + (size_t)(g.start / seg + 1u) * block);
+        if (cut) regs_to(p, l, h, carry + (size_t)(g.start / p.seg + 1u) * block);
         else if (last) regs_to(p, l, h, last + (size_t)r * block);
         return;
     }
     unsigned r, k;
     row_range g;
     const unsigned slot = blockIdx.x - p.nregion;
-    if (!cut_segment(p, regions, marks, slot, seg, r, g, k) || g.start + (uint64_t)(k + 1u) * seg >= g.end) return;
+    if (!cut_segment(p, regions, marks, slot, r, g, k) || g.start + (uint64_t)(k + 1u) * p.seg >= g.end) return;
     regs_from(p, l, a2, A_, A(1.4426950408889634));
     regs_from(p, l, h, (const A*)nullptr, A(1));
-    scan_rows<T, LG, NS, false>(p, l, threadIdx.x, first, (size_t)g.start + (size_t)k * seg, seg, X, dt, gate, B, C, sk, bi, h, a2, Y, (A*)nullptr, steps, lds);
+    scan_rows<T, LG, NS, false>(p, l, threadIdx.x, first, (size_t)g.start + (size_t)k * p.seg, p.seg, X, dt, gate, B, C, sk, bi, h, a2, Y, (A*)nullptr, steps, lds);
     regs_to(p, l, h, local + (size_t)slot * block);
     if (l.active) sums[(size_t)slot * p.D + l.ch] = steps;
 }
@@ -136,13 +136,13 @@ __global__ __launch_bounds__(256, 4) void k_scan_fprop(scan_shape p, unsigned se
 // The state in front of every segment of a cut region from the one in front of the segment before: what that one makes of zeros, and
 // its own carried state times exp(A * sum of its steps). A thread per state and channel.
 template <typename A>
-__global__ __launch_bounds__(256) void k_scan_carry(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const A* __restrict__ A_,
+__global__ __launch_bounds__(256) void k_scan_carry(scan_shape p, const uint32_t* __restrict__ regions, const A* __restrict__ A_,
                                                     const A* __restrict__ local, const A* __restrict__ sums, A* __restrict__ carry)
 {
     const row_range g = region_rows(regions, blockIdx.x, p.N);
-    if (!is_cut(g, seg)) return;
-    const size_t block = (size_t)p.S * p.D, first = g.start / seg + 1u;
-    const unsigned n = (g.end - g.start - 1u) / seg;             // segments behind the first; the state in front of the first of them is there
+    if (!is_cut(p, g)) return;
+    const size_t block = (size_t)p.S * p.D, first = g.start / p.seg + 1u;
+    const unsigned n = (g.end - g.start - 1u) / p.seg;             // segments behind the first; the state in front of the first of them is there
     for (size_t at = (size_t)blockIdx.y * 256u + threadIdx.x; at < block; at += (size_t)gridDim.y * 256u)
         carry_chain<A>(A_[at] * A(1.4426950408889634), carry[first * block + at], n - 1u, local + first * block + at, sums + first * p.D + at % p.D,
                        carry + (first + 1u) * block + at, block, p.D);
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256) void k_scan_carry(scan_shape p, unsigned seg, 
 
 // The rows of every segment behind the first, from the state carried to it.
 template <typename T, int LG, int NS>
-__global__ __launch_bounds__(256, 4) void k_scan_fprop_cut(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
+__global__ __launch_bounds__(256, 4) void k_scan_fprop_cut(scan_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
                                                        const T* __restrict__ X, const T* __restrict__ dt,
                                                        const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ B,
                                                        const typename acc_of<T>::type* __restrict__ C, const typename acc_of<T>::type* __restrict__ skip,
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256, 4) void k_scan_fprop_cut(scan_shape p, unsigne
     typedef typename acc_of<T>::type A;
     unsigned r, k;
     row_range g;
-    if (!cut_segment(p, regions, marks, blockIdx.x, seg, r, g, k)) return;
+    if (!cut_segment(p, regions, marks, blockIdx.x, r, g, k)) return;
     const unsigned tile = blockIdx.y * blockDim.y + uniform(threadIdx.y);
     if (tile >= p.tiles) return;
     __shared__ A lds_all[4][scan_weights<A, LG, NS, true, true>::SIZE];
@@ -170,25 +170,25 @@ __global__ __launch_bounds__(256, 4) void k_scan_fprop_cut(scan_shape p, unsigne
     const unsigned first = first_group<LG>(p, tile);
     const size_t block = (size_t)p.S * p.D;
     const A sk = skip ? skip[l.ch] : A(0), bi = bias ? bias[l.ch] : A(0);
-    A h[NS], a2[NS], steps = 0, *kept = keep ? kept_at(p, keep, g.start, k * (seg / SCAN_CHUNK)) : (A*)nullptr;
+    A h[NS], a2[NS], steps = 0, *kept = keep ? kept_at(p, keep, g.start, k * (p.seg / SCAN_CHUNK)) : (A*)nullptr;
     regs_from(p, l, a2, A_, A(1.4426950408889634));
     regs_from(p, l, h, carry + (size_t)blockIdx.x * block, A(1));
     if (kept) regs_to(p, l, h, kept);
-    const unsigned row = g.start + k * seg;
-    scan_rows<T, LG, NS, true>(p, l, threadIdx.x, first, row, min(seg, g.end - row), X, dt, gate, B, C, sk, bi, h, a2, Y, kept, steps, lds);
-    if (last && g.end - row <= seg) regs_to(p, l, h, last + (size_t)r * block);
+    const unsigned row = g.start + k * p.seg;
+    scan_rows<T, LG, NS, true>(p, l, threadIdx.x, first, row, min(p.seg, g.end - row), X, dt, gate, B, C, sk, bi, h, a2, Y, kept, steps, lds);
+    if (last && g.end - row <= p.seg) regs_to(p, l, h, last + (size_t)r * block);
 }
 
-__global__ __launch_bounds__(256) void k_mark_cut(const uint32_t* __restrict__ regions, unsigned nregion, unsigned N, unsigned seg, uint32_t* __restrict__ marks)
+__global__ __launch_bounds__(256) void k_mark_cut(scan_shape p, const uint32_t* __restrict__ regions, uint32_t* __restrict__ marks)
 {
     const unsigned r = blockIdx.x * 4u + (threadIdx.x >> 6);
-    if (r >= nregion) return;
-    const row_range g = region_rows(regions, r, N);
-    if (is_cut(g, seg)) mark_segments(marks, r, g, seg, threadIdx.x & 63u, 64u);
+    if (r >= p.nregion) return;
+    const row_range g = region_rows(regions, r, p.N);
+    if (is_cut(p, g)) mark_segments(marks, r, g, p.seg, threadIdx.x & 63u, 64u);
 }
-int mark_cut_regions(hipStream_t st, const uint32_t* regions, size_t nregion, size_t N, unsigned seg, uint32_t* marks)
+int mark_cut_regions(hipStream_t st, const scan_shape& p, const uint32_t* regions, uint32_t* marks)
 {
-    k_mark_cut<<<divup(nregion, 4), 256, 0, st>>>(regions, (unsigned)nregion, (unsigned)N, seg, marks);
+    k_mark_cut<<<divup(p.nregion, 4), 256, 0, st>>>(p, regions, marks);
     return 0;
 }
 
@@ -235,7 +235,7 @@ namespace {
 constexpr size_t SCAN_WAVES = 4096;              // waves that keep the vector units busy: four per SIMD (88 registers a lane allow five)
 constexpr size_t SCAN_LEAST = 32;                // rows of the shortest segment: its state's way through the carry costs as much as some ten rows
 
-scan_plan plan_fprop(const dbk_statescan_args& a) { return plan_scan(a.N, a.D, a.G, SCAN_WAVES, SCAN_LEAST); }
+scan_plan plan_fprop(const dbk_statescan_args& a) { return plan_scan(a.N, a.D, a.G, SCAN_WAVES, 4, SCAN_LEAST); }
 
 }  // namespace
 }  // namespace dbk
@@ -268,25 +268,23 @@ int dbk_statescan(dbk_stream_t stream, const dbk_statescan_args* a, void* work, 
     const scan_segments g = segments_in(work, *a, p);
     DBK_CHECK(!g.bytes || (work && work_bytes >= g.bytes), "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, g.bytes);
     DBK_CHECK(a->nregion + p.slots < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
-    scan_shape s = shape_of(*a);
-    s.tpg = p.tpg;
-    s.tiles = p.tiles;
+    const scan_shape s = shape_of(*a, p);
     hipStream_t st = as_stream(stream);
     const unsigned waves = p.tpg < 4 ? (p.tpg ? p.tpg : 1u) : 4u;
-    if (p.slots) mark_cut_regions(st, a->regions, a->nregion, a->N, p.seg, g.marks);
+    if (p.slots) mark_cut_regions(st, s, a->regions, g.marks);
     with_row_type(a->dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
         with_lanes(p.lanes, [&](auto lanes) {
             with_states(a->S, [&](auto ns) {
                 k_scan_fprop<T, lanes.value, ns.value><<<dim3((unsigned)a->nregion + p.slots, divup(p.tiles, waves)), dim3(64, waves), 0, st>>>(
-                    s, p.seg, a->regions, g.marks, (const T*)a->X, (const T*)a->dt, (const A*)a->A, (const A*)a->B, (const A*)a->C, (const A*)a->skip, (const T*)a->gate,
+                    s, a->regions, g.marks, (const T*)a->X, (const T*)a->dt, (const A*)a->A, (const A*)a->B, (const A*)a->C, (const A*)a->skip, (const T*)a->gate,
                     (const A*)a->dt_bias, (const A*)a->state, (T*)a->Y, (A*)a->last, (A*)a->keep, (A*)g.local, (A*)g.steps, (A*)g.carry);
                 if (!p.slots) return;
-                k_scan_carry<A><<<dim3((unsigned)a->nregion, carry_blocks(*a)), 256, 0, st>>>(s, p.seg, a->regions, (const A*)a->A, (const A*)g.local, (const A*)g.steps,
+                k_scan_carry<A><<<dim3((unsigned)a->nregion, carry_blocks(*a)), 256, 0, st>>>(s, a->regions, (const A*)a->A, (const A*)g.local, (const A*)g.steps,
                                                                                               (A*)g.carry);
                 k_scan_fprop_cut<T, lanes.value, ns.value><<<dim3(p.slots, divup(p.tiles, waves)), dim3(64, waves), 0, st>>>(
-                    s, p.seg, a->regions, g.marks, (const T*)a->X, (const T*)a->dt, (const A*)a->A, (const A*)a->B, (const A*)a->C, (const A*)a->skip, (const T*)a->gate,
+                    s, a->regions, g.marks, (const T*)a->X, (const T*)a->dt, (const A*)a->A, (const A*)a->B, (const A*)a->C, (const A*)a->skip, (const T*)a->gate,
                     (const A*)a->dt_bias, (T*)a->Y, (A*)a->last, (A*)a->keep, (const A*)g.carry);
             });
         });
@@ -301,7 +299,7 @@ int dbk_statescan_step(dbk_stream_t stream, const dbk_statescan_args* a)
     DBK_CHECK(a->N <= 1 || a->ldy >= a->D, "ValueError: row strides must be at least the number of columns");
     DBK_CHECK(a->N < (size_t(1) << 31), "ValueError: too many sequences (%zu)", a->N);
     if (!a->N || !a->D) { clear_error(); return 0; }
-    const scan_shape s = shape_of(*a);
+    const scan_shape s = shape_of(*a, plan_scan(0, a->D, a->G, 1, 2, 1));
     hipStream_t st = as_stream(stream);
     with_row_type(a->dtype, [&](auto t) {
         typedef decltype(t) T;

@@ -369,7 +369,7 @@ template <int LG, typename A> __device__ __forceinline__ scan_out<A> tile_share(
 // part[unit][S + 2][D]. Of a region that is cut it takes the last segment, behind which nothing sends anything. Units from unit0 on
 // take the other segments: the slot of segment k stands for segment k - 1, to which segment k sends what lies in the slot's carry.
 template <typename T, int LG>
-__global__ __launch_bounds__(64, sizeof(T) == 8 ? 1 : 2) void k_scan_bprop(scan_shape p, scan_bshape bp, unsigned seg, unsigned unit0, unsigned nslot, scan_rows_in<T> in,
+__global__ __launch_bounds__(64, sizeof(T) == 8 ? 1 : 2) void k_scan_bprop(scan_shape p, scan_bshape bp, unsigned unit0, unsigned nslot, scan_rows_in<T> in,
                                                       const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ skip,
                                                       const typename acc_of<T>::type* __restrict__ bias, scan_rows_out<T> to,
                                                       scan_out<typename acc_of<T>::type> out, size_t tile_stride, typename acc_of<T>::type* __restrict__ part,
@@ -387,14 +387,14 @@ __global__ __launch_bounds__(64, sizeof(T) == 8 ? 1 : 2) void k_scan_bprop(scan_
         const A* sent = nullptr;
         if (slots) {
             unsigned r, k;
-            if (!cut_segment(p, in.regions, in.marks, i, seg, r, g, k)) continue;
-            from = g.start + (k - 1u) * seg;
-            n = seg;
+            if (!cut_segment(p, in.regions, in.marks, i, r, g, k)) continue;
+            from = g.start + (k - 1u) * p.seg;
+            n = p.seg;
             sent = carry + (size_t)i * p.S * p.D;
         } else {
             g = region_rows(in.regions, i, p.N);
             if (g.start == g.end) continue;
-            from = g.start + (in.marks && is_cut(g, seg) ? (g.end - g.start - 1u) / seg * seg : 0u);
+            from = g.start + (in.marks && is_cut(p, g) ? (g.end - g.start - 1u) / p.seg * p.seg : 0u);
             n = g.end - from;
         }
         // (a lane without a channel adds nothing to its group's sums: its e is zero, and so is what is sent to it)
@@ -406,7 +406,7 @@ __global__ __launch_bounds__(64, sizeof(T) == 8 ? 1 : 2) void k_scan_bprop(scan_
 
 // What a segment behind the first sends back when nothing is sent to it, and the sum of its steps: the states' gradients alone.
 template <typename T, int LG, int NS>
-__global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t lddy, unsigned seg, scan_rows_in<T> in, const typename acc_of<T>::type* __restrict__ A_,
+__global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t lddy, scan_rows_in<T> in, const typename acc_of<T>::type* __restrict__ A_,
                                                          const typename acc_of<T>::type* __restrict__ bias, typename acc_of<T>::type* __restrict__ local,
                                                          typename acc_of<T>::type* __restrict__ sums)
 {
@@ -416,15 +416,15 @@ __global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t ld
     __shared__ A lds[weights::SIZE];
     unsigned r, k;
     row_range g;
-    if (!cut_segment(p, in.regions, in.marks, blockIdx.x, seg, r, g, k)) return;
+    if (!cut_segment(p, in.regions, in.marks, blockIdx.x, r, g, k)) return;
     const scan_lane l = lane_channel<LG>(p, blockIdx.y, threadIdx.x);
     const A bi = bias ? bias[l.ch] : A(0);
     A a2[NS], ag[NS], steps = 0;
     regs_from(p, l, a2, A_, A(1.4426950408889634));
     regs_from(p, l, ag, (const A*)nullptr, A(1));
-    const size_t row = (size_t)g.start + (size_t)k * seg;
+    const size_t row = (size_t)g.start + (size_t)k * p.seg;
     const unsigned place = opaque(l.ch * (unsigned)sizeof(T));
-    const unsigned n = min(seg, g.end - (unsigned)row), up = (n + U - 1u) / U * U;
+    const unsigned n = min(p.seg, g.end - (unsigned)row), up = (n + U - 1u) / U * U;
     weights w(p, threadIdx.x, first_group<LG>(p, blockIdx.y), (const A*)nullptr, in.C + row * p.ldc, lds, up - U, true);
     T dn[U], en[U], gn[U];
     auto fetch = [&](unsigned t) {               // rows t .. t + U - 1 of the segment (behind its last row: that one again)
@@ -469,13 +469,13 @@ __global__ __launch_bounds__(64) void k_scan_bprop_local(scan_shape p, size_t ld
 // carry[slot of segment k]: what segment k >= 1 of a cut region sends to the one before it, from the last segment to the first: what it sends
 // by itself, and exp(A * sum of its steps) times what it is sent. Loads run ahead of the chain.
 template <typename A>
-__global__ __launch_bounds__(256) void k_scan_carry_back(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const A* __restrict__ A_,
+__global__ __launch_bounds__(256) void k_scan_carry_back(scan_shape p, const uint32_t* __restrict__ regions, const A* __restrict__ A_,
                                                          const A* __restrict__ local, const A* __restrict__ sums, A* __restrict__ carry)
 {
     const row_range g = region_rows(regions, blockIdx.x, p.N);
-    if (!is_cut(g, seg)) return;
-    const size_t block = (size_t)p.S * p.D, zero = g.start / seg;
-    const unsigned n = (g.end - g.start - 1u) / seg;             // the last segment
+    if (!is_cut(p, g)) return;
+    const size_t block = (size_t)p.S * p.D, zero = g.start / p.seg;
+    const unsigned n = (g.end - g.start - 1u) / p.seg;             // the last segment
     for (size_t at = (size_t)blockIdx.y * 256u + threadIdx.x; at < block; at += (size_t)gridDim.y * 256u)
         carry_chain<A>(A_[at] * A(1.4426950408889634), A(0), n, local + (zero + n) * block + at, sums + (zero + n) * p.D + at % p.D, carry + (zero + n) * block + at,
                        0 - block, 0 - (size_t)p.D);
@@ -483,7 +483,7 @@ __global__ __launch_bounds__(256) void k_scan_carry_back(scan_shape p, unsigned 
 
 // dB and dC from the tiles' shares, in the tiles' order: a region's rows (its first segment's where it is cut), or another segment's.
 template <typename A>
-__global__ __launch_bounds__(256) void k_scan_weights(scan_shape p, unsigned seg, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, unsigned tiles,
+__global__ __launch_bounds__(256) void k_scan_weights(scan_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, unsigned tiles,
                                                       size_t ncol, const A* __restrict__ share, size_t tile_stride, A* __restrict__ dB, size_t lddb, A* __restrict__ dC, size_t lddc)
 {
     row_range g;
@@ -491,12 +491,12 @@ __global__ __launch_bounds__(256) void k_scan_weights(scan_shape p, unsigned seg
     if (blockIdx.x < p.nregion) {
         g = region_rows(regions, blockIdx.x, p.N);
         from = g.start;
-        if (marks && is_cut(g, seg)) g.end = g.start + seg;
+        if (marks && is_cut(p, g)) g.end = g.start + p.seg;
     } else {
         unsigned r, k;
-        if (!cut_segment(p, regions, marks, blockIdx.x - p.nregion, seg, r, g, k)) return;
-        from = g.start + k * seg;
-        g.end = min(g.end, from + seg);
+        if (!cut_segment(p, regions, marks, blockIdx.x - p.nregion, r, g, k)) return;
+        from = g.start + k * p.seg;
+        g.end = min(g.end, from + p.seg);
     }
     const size_t n = (size_t)(g.end - from) * 2u * ncol;
     for (size_t i = (size_t)blockIdx.y * 256u + threadIdx.x; i < n; i += (size_t)gridDim.y * 256u) {
@@ -515,7 +515,7 @@ constexpr size_t SCAN_UNITS = 4096;              // waves that add up dA, over a
 constexpr size_t SCAN_WAVES = 2048;              // waves that keep the vector units busy: two per SIMD, which 256 registers a lane allow
 constexpr size_t SCAN_LEAST = 32;                // rows of the shortest segment
 
-scan_plan plan_bprop(const dbk_statescan_args& a) { return plan_scan(a.N, a.D, a.G, SCAN_WAVES, SCAN_LEAST); }
+scan_plan plan_bprop(const dbk_statescan_args& a) { return plan_scan(a.N, a.D, a.G, SCAN_WAVES, 2, SCAN_LEAST); }
 
 // Workspace: segments, tiles' shares of dB and dC (a group of several tiles), units' sums of dA, dD and dbias.
 struct bprop_layout { scan_segments seg; size_t share, part, bytes; unsigned units, slot_units; };
@@ -561,14 +561,12 @@ int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* a, void* 
     const bprop_layout y = layout_of(work, *a, p);
     DBK_CHECK(work && work_bytes >= y.bytes, "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, y.bytes);
     DBK_CHECK(a->nregion + p.slots < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
-    scan_shape s = shape_of(*a);
-    s.tpg = p.tpg;
-    s.tiles = p.tiles;
+    const scan_shape s = shape_of(*a, p);
     const scan_bshape b = {a->lddy, a->lddx, a->ldddt, a->lddgate, a->lddb, a->lddc};
     const size_t ncol = a->G * a->S;
     const bool shared = p.tpg > 1;
     void* part = (char*)work + y.part;
-    if (p.slots) mark_cut_regions(st, a->regions, a->nregion, a->N, p.seg, y.seg.marks);
+    if (p.slots) mark_cut_regions(st, s, a->regions, y.seg.marks);
     with_row_type(a->dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
@@ -582,17 +580,17 @@ int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* a, void* 
         with_lanes(p.lanes, [&](auto lanes) {
             if (p.slots) {
                 with_states(a->S, [&](auto ns) {
-                    k_scan_bprop_local<T, lanes.value, ns.value><<<dim3(p.slots, p.tiles), 64, 0, st>>>(s, b.lddy, p.seg, in, (const A*)a->A, (const A*)a->dt_bias,
+                    k_scan_bprop_local<T, lanes.value, ns.value><<<dim3(p.slots, p.tiles), 64, 0, st>>>(s, b.lddy, in, (const A*)a->A, (const A*)a->dt_bias,
                                                                                                         (A*)y.seg.local, (A*)y.seg.steps);
                 });
-                k_scan_carry_back<A><<<dim3((unsigned)a->nregion, carry_blocks(*a)), 256, 0, st>>>(s, p.seg, a->regions, (const A*)a->A, (const A*)y.seg.local,
+                k_scan_carry_back<A><<<dim3((unsigned)a->nregion, carry_blocks(*a)), 256, 0, st>>>(s, a->regions, (const A*)a->A, (const A*)y.seg.local,
                                                                                                   (const A*)y.seg.steps, (A*)y.seg.carry);
             }
-            k_scan_bprop<T, lanes.value><<<dim3(y.units + y.slot_units, p.tiles), 64, lds, st>>>(s, b, p.seg, y.units, p.slots, in, (const A*)a->A, (const A*)a->skip,
+            k_scan_bprop<T, lanes.value><<<dim3(y.units + y.slot_units, p.tiles), 64, lds, st>>>(s, b, y.units, p.slots, in, (const A*)a->A, (const A*)a->skip,
                                                                                                 (const A*)a->dt_bias, to, out, tile_stride, (A*)part, (const A*)y.seg.carry);
         });
         if (shared)
-            k_scan_weights<A><<<dim3((unsigned)a->nregion + p.slots, divup((size_t)p.seg * 2 * ncol, 1024)), 256, 0, st>>>(s, p.seg, a->regions, y.seg.marks, p.tpg, ncol, share, tile_stride, (A*)a->dB, a->lddb, (A*)a->dC,
+            k_scan_weights<A><<<dim3((unsigned)a->nregion + p.slots, divup((size_t)p.seg * 2 * ncol, 1024)), 256, 0, st>>>(s, a->regions, y.seg.marks, p.tpg, ncol, share, tile_stride, (A*)a->dB, a->lddb, (A*)a->dC,
                                                                               a->lddc);
     });
     sum_partials(st, a->dtype, part, y.units + y.slot_units, a->S * a->D, a->dA, a->D, a->dskip, a->D, a->ddt_bias);
