@@ -99,46 +99,47 @@ __device__ __forceinline__ void conv_strip(conv_shape p, const conv_weights<T, K
     }
 }
 
-// A workgroup takes the first segment of a region (all of it, mostly), its lanes being 2^ct_log2 vectors of channels by strips of rows.
+// A workgroup's lanes are 2^ct_log2 vectors of channels by strips of rows. Item i < nregion is the first segment of region i (all of it, mostly),
+// the items behind are the slots of the other segments.
+struct conv_item { unsigned r, from, len; row_range g; };
+__device__ __forceinline__ bool conv_item_at(const conv_shape& p, const uint32_t* regions, const uint32_t* marks, unsigned i, conv_item& s)
+{
+    unsigned k = 0;
+    if (i < p.nregion) {
+        s.r = i;
+        s.g = region_rows(regions, i, p.N);
+    } else if (!slot_segment(regions, p.nregion, p.N, marks, i - p.nregion, p.seg, s.r, s.g, k))
+        return false;
+    s.from = s.g.start + k * p.seg;
+    s.len = min(s.g.end - s.from, p.seg);
+    return true;
+}
+
+__global__ __launch_bounds__(256) void k_conv_mark(conv_shape p, const uint32_t* __restrict__ regions, uint32_t* __restrict__ marks)
+{
+    const unsigned r = blockIdx.x * 4u + (threadIdx.x >> 6);
+    if (r < p.nregion) mark_segments(marks, r, region_rows(regions, r, p.N), p.seg, threadIdx.x & 63u, 64u);
+}
+
 template <typename T, int K, bool EXACT>
 __global__ __launch_bounds__(256) void k_conv_fprop(conv_shape p, const T* __restrict__ X, const typename acc_of<T>::type* __restrict__ W,
                                                     const typename acc_of<T>::type* __restrict__ bias, const uint32_t* __restrict__ regions,
-                                                    const T* __restrict__ state, T* __restrict__ Z, T* __restrict__ last, uint32_t* __restrict__ marks)
+                                                    const uint32_t* __restrict__ marks, const T* __restrict__ state, T* __restrict__ Z, T* __restrict__ last)
 {
     constexpr int V = conv_vec<T>::N;
+    conv_item s;
+    if (!conv_item_at(p, regions, marks, blockIdx.x, s)) return;
     const unsigned x = threadIdx.x & ((1u << p.ct_log2) - 1u), y = threadIdx.x >> p.ct_log2, strips = 256u >> p.ct_log2;
     const unsigned c = ((blockIdx.y << p.ct_log2) + x) * V, valid = c < p.D ? p.D - c : 0u;
-    const unsigned r = blockIdx.x;
-    const row_range g = region_rows(regions, r, p.N);
     conv_weights<T, K> w;
     w.load(W, bias, p.D, c, valid);
-    const unsigned len = min(g.end - g.start, p.seg), strip = (len + strips - 1) / strips;
-    const unsigned from = g.start + min(y * strip, len), to = g.start + min((y + 1) * strip, len);
-    conv_strip<T, K, EXACT>(p, w, X, state, Z, c, valid, r, g, from, to);
-    if (last && y < K - 1 && valid) {            // the K - 1 rows that the next piece of this sequence needs
+    const unsigned strip = (s.len + strips - 1) / strips;
+    conv_strip<T, K, EXACT>(p, w, X, state, Z, c, valid, s.r, s.g, s.from + min(y * strip, s.len), s.from + min((y + 1) * strip, s.len));
+    if (last && blockIdx.x < p.nregion && y < K - 1 && valid) {          // the K - 1 rows that the next piece of this sequence needs
         conv_vec<T> v;
-        conv_row<T, K>(v, X, p.ldx, state, p.D, c, valid, r, g, (int64_t)g.end - (K - 1) + y);
-        v.store(last + ((size_t)r * (K - 1) + y) * p.D + c, valid);
+        conv_row<T, K>(v, X, p.ldx, state, p.D, c, valid, s.r, s.g, (int64_t)s.g.end - (K - 1) + y);
+        v.store(last + ((size_t)s.r * (K - 1) + y) * p.D + c, valid);
     }
-    if (marks && blockIdx.y == 0) mark_segments(marks, r, g, p.seg, threadIdx.x, 256u);
-}
-
-// The other segments of long regions.
-template <typename T, int K, bool EXACT>
-__global__ __launch_bounds__(256) void k_conv_fprop_long(conv_shape p, const T* __restrict__ X, const typename acc_of<T>::type* __restrict__ W,
-                                                         const typename acc_of<T>::type* __restrict__ bias, const uint32_t* __restrict__ regions,
-                                                         const uint32_t* __restrict__ marks, T* __restrict__ Z)
-{
-    constexpr int V = conv_vec<T>::N;
-    unsigned r, k;
-    row_range g;
-    if (!slot_segment(regions, p.nregion, p.N, marks, blockIdx.x, p.seg, r, g, k)) return;
-    const unsigned x = threadIdx.x & ((1u << p.ct_log2) - 1u), y = threadIdx.x >> p.ct_log2, strips = 256u >> p.ct_log2;
-    const unsigned c = ((blockIdx.y << p.ct_log2) + x) * V, valid = c < p.D ? p.D - c : 0u;
-    conv_weights<T, K> w;
-    w.load(W, bias, p.D, c, valid);
-    const unsigned a = g.start + k * p.seg, len = min(g.end - a, p.seg), strip = (len + strips - 1) / strips;
-    conv_strip<T, K, EXACT>(p, w, X, (const T*)nullptr, Z, c, valid, r, g, a + min(y * strip, len), a + min((y + 1) * strip, len));
 }
 
 // Backward of rows [from, to) of region g, adding to the lane's dW, db. Each row's dp is formed once, but for the K - 1 rows below
@@ -253,10 +254,10 @@ __device__ __forceinline__ void conv_leave_sums(conv_shape p, const conv_sums<T,
 }
 
 template <typename T, int K, bool EXACT>
-__global__ __launch_bounds__(256) void k_conv_bprop(conv_shape p, size_t lddz, const T* __restrict__ X, const typename acc_of<T>::type* __restrict__ W,
+__global__ __launch_bounds__(256) void k_conv_bprop(conv_shape p, size_t lddz, unsigned items, const T* __restrict__ X, const typename acc_of<T>::type* __restrict__ W,
                                                     const typename acc_of<T>::type* __restrict__ bias, const uint32_t* __restrict__ regions,
-                                                    const T* __restrict__ dZ, T* __restrict__ dX, typename acc_of<T>::type* __restrict__ part,
-                                                    uint32_t* __restrict__ marks)
+                                                    const uint32_t* __restrict__ marks, const T* __restrict__ dZ, T* __restrict__ dX,
+                                                    typename acc_of<T>::type* __restrict__ part)
 {
     constexpr int V = conv_vec<T>::N;
     const unsigned x = threadIdx.x & ((1u << p.ct_log2) - 1u), y = threadIdx.x >> p.ct_log2, strips = 256u >> p.ct_log2;
@@ -265,36 +266,13 @@ __global__ __launch_bounds__(256) void k_conv_bprop(conv_shape p, size_t lddz, c
     conv_sums<T, K> sums;
     w.load(W, bias, p.D, c, valid);
     sums.clear();
-    for (unsigned r = blockIdx.x; r < p.nregion; r += gridDim.x) {
-        const row_range g = region_rows(regions, r, p.N);
-        const unsigned len = min(g.end - g.start, p.seg), strip = (len + strips - 1) / strips;
-        conv_strip_bprop<T, K, EXACT>(p, lddz, w, sums, X, dZ, dX, c, valid, g, g.start + min(y * strip, len), g.start + min((y + 1) * strip, len));
-        if (marks && blockIdx.y == 0) mark_segments(marks, r, g, p.seg, threadIdx.x, 256u);
+    for (unsigned i = blockIdx.x; i < items; i += gridDim.x) {
+        conv_item s;
+        if (!conv_item_at(p, regions, marks, i, s)) continue;
+        const unsigned strip = (s.len + strips - 1) / strips;
+        conv_strip_bprop<T, K, EXACT>(p, lddz, w, sums, X, dZ, dX, c, valid, s.g, s.from + min(y * strip, s.len), s.from + min((y + 1) * strip, s.len));
     }
     conv_leave_sums<T, K>(p, sums, c, valid, blockIdx.x, part);
-}
-
-template <typename T, int K, bool EXACT>
-__global__ __launch_bounds__(256) void k_conv_bprop_long(conv_shape p, size_t lddz, unsigned nslot, unsigned unit0, const T* __restrict__ X,
-                                                         const typename acc_of<T>::type* __restrict__ W, const typename acc_of<T>::type* __restrict__ bias,
-                                                         const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks,
-                                                         const T* __restrict__ dZ, T* __restrict__ dX, typename acc_of<T>::type* __restrict__ part)
-{
-    constexpr int V = conv_vec<T>::N;
-    const unsigned x = threadIdx.x & ((1u << p.ct_log2) - 1u), y = threadIdx.x >> p.ct_log2, strips = 256u >> p.ct_log2;
-    const unsigned c = ((blockIdx.y << p.ct_log2) + x) * V, valid = c < p.D ? p.D - c : 0u;
-    conv_weights<T, K> w;
-    conv_sums<T, K> sums;
-    w.load(W, bias, p.D, c, valid);
-    sums.clear();
-    for (unsigned slot = blockIdx.x; slot < nslot; slot += gridDim.x) {
-        unsigned r, k;
-        row_range g;
-        if (!slot_segment(regions, p.nregion, p.N, marks, slot, p.seg, r, g, k)) continue;
-        const unsigned a = g.start + k * p.seg, len = min(g.end - a, p.seg), strip = (len + strips - 1) / strips;
-        conv_strip_bprop<T, K, EXACT>(p, lddz, w, sums, X, dZ, dX, c, valid, g, a + min(y * strip, len), a + min((y + 1) * strip, len));
-    }
-    conv_leave_sums<T, K>(p, sums, c, valid, unit0 + blockIdx.x, part);
 }
 
 // One new row per sequence: the state's K - 1 rows move up by one.
@@ -333,7 +311,7 @@ constexpr size_t CONV_UNITS = 2048;              // workgroups that add up weigh
 
 size_t conv_width(int dtype) { return dtype == DBK_F64 ? 2 : 4; }
 
-struct conv_plan { unsigned ct_log2, tiles, seg, units, slots, slot_units; };
+struct conv_plan { unsigned ct_log2, tiles, seg, slots, units; };
 
 conv_plan plan_conv(int dtype, size_t N, size_t D, size_t P)
 {
@@ -344,9 +322,8 @@ conv_plan plan_conv(int dtype, size_t N, size_t D, size_t P)
     p.tiles = divup(vecs, size_t(1) << p.ct_log2);
     p.seg = (256u >> p.ct_log2) * CONV_STRIP;
     const size_t cap = CONV_UNITS / p.tiles ? CONV_UNITS / p.tiles : 1;
-    p.units = (unsigned)(P < cap ? P : cap);
     p.slots = N > p.seg ? (unsigned)segment_slots(N, p.seg) : 0u;
-    p.slot_units = (unsigned)(p.slots < cap ? p.slots : cap);
+    p.units = (unsigned)(P + p.slots < cap ? P + p.slots : cap);
     return p;
 }
 
@@ -369,6 +346,7 @@ int check_conv(int dtype, const void* X, size_t ldx, const void* W, size_t taps,
     DBK_CHECK(taps >= 1 && taps <= 4, "NotImplementedError: filters of 1 to 4 taps, got %zu", taps);
     DBK_CHECK(N < (size_t(1) << 32) - 1 && D < (size_t(1) << 31) && nregion < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu channels, %zu regions)", N, D, nregion);
     DBK_CHECK(D <= size_t(65535) * 64 * 2, "ValueError: too many channels (%zu)", D);
+    DBK_CHECK(nregion + N < (size_t(1) << 32) - 1, "ValueError: map too large (%zu rows, %zu regions)", N, nregion);
     DBK_CHECK(!N || !D || (X && W && Z), "ValueError: null matrix");
     DBK_CHECK(N <= 1 || (ldx >= D && ldz >= D), "ValueError: row strides must be at least the number of channels");
     return 0;
@@ -388,7 +366,7 @@ int dbk_causalconv_workspace(int dtype, size_t taps, size_t N, size_t D, size_t 
     *work_bytes = 0;
     if (N && D && nregion) {
         const conv_plan p = plan_conv(dtype, N, D, nregion);
-        *work_bytes = ((size_t)p.slots * 4 + 15) / 16 * 16 + (backward ? (size_t)(p.units + p.slot_units) * (taps + 1) * D * acc_size(dtype) : 0);
+        *work_bytes = ((size_t)p.slots * 4 + 15) / 16 * 16 + (backward ? (size_t)p.units * (taps + 1) * D * acc_size(dtype) : 0);
     }
     clear_error();
     return 0;
@@ -401,17 +379,17 @@ int dbk_causalconv(dbk_stream_t stream, int dtype, const void* X, size_t ldx, co
     DBK_CHECK(!nregion || regions, "ValueError: null regions");
     if (!D || !nregion) { clear_error(); return 0; }
     const conv_plan p = plan_conv(dtype, N, D, nregion);
+    DBK_CHECK(nregion + p.slots < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu regions)", N, nregion);
     DBK_CHECK(!p.slots || (work && work_bytes >= (size_t)p.slots * 4), "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, (size_t)p.slots * 4);
     const conv_shape s = {(unsigned)N, (unsigned)D, (unsigned)nregion, p.seg, p.ct_log2, (unsigned)(silu != 0), ldx, ldz};
     hipStream_t st = as_stream(stream);
+    if (p.slots) k_conv_mark<<<divup(nregion, 4), 256, 0, st>>>(s, regions, (uint32_t*)work);
     with_row_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
         with_taps(taps, D % conv_width(dtype) == 0, [&](auto k, auto exact) {
-            k_conv_fprop<T, k.value, exact.value><<<dim3((unsigned)nregion, p.tiles), 256, 0, st>>>(s, (const T*)X, (const A*)W, (const A*)bias, regions, (const T*)state, (T*)Z, (T*)last,
-                                                                                  p.slots ? (uint32_t*)work : nullptr);
-            if (p.slots)
-                k_conv_fprop_long<T, k.value, exact.value><<<dim3(p.slots, p.tiles), 256, 0, st>>>(s, (const T*)X, (const A*)W, (const A*)bias, regions, (const uint32_t*)work, (T*)Z);
+            k_conv_fprop<T, k.value, exact.value><<<dim3((unsigned)nregion + p.slots, p.tiles), 256, 0, st>>>(s, (const T*)X, (const A*)W, (const A*)bias, regions, (const uint32_t*)work,
+                                                                                                        (const T*)state, (T*)Z, (T*)last);
         });
     });
     DBK_LAUNCH_OK();
@@ -436,19 +414,17 @@ int dbk_causalconv_bprop(dbk_stream_t stream, int dtype, const void* X, size_t l
     DBK_CHECK(work && work_bytes >= need, "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, need);
     const conv_plan p = plan_conv(dtype, N, D, nregion);
     const conv_shape s = {(unsigned)N, (unsigned)D, (unsigned)nregion, p.seg, p.ct_log2, (unsigned)(silu != 0), ldx, lddx};
-    uint32_t* marks = p.slots ? (uint32_t*)work : nullptr;
+    if (p.slots) k_conv_mark<<<divup(nregion, 4), 256, 0, st>>>(s, regions, (uint32_t*)work);
     void* part = (char*)work + ((size_t)p.slots * 4 + 15) / 16 * 16;
     with_row_type(dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
         with_taps(taps, D % conv_width(dtype) == 0, [&](auto k, auto exact) {
-            k_conv_bprop<T, k.value, exact.value><<<dim3(p.units, p.tiles), 256, 0, st>>>(s, lddz, (const T*)X, (const A*)W, (const A*)bias, regions, (const T*)dZ, (T*)dX, (A*)part, marks);
-            if (p.slots)
-                k_conv_bprop_long<T, k.value, exact.value><<<dim3(p.slot_units, p.tiles), 256, 0, st>>>(s, lddz, p.slots, p.units, (const T*)X, (const A*)W, (const A*)bias, regions, marks,
-                                                                                         (const T*)dZ, (T*)dX, (A*)part);
+            k_conv_bprop<T, k.value, exact.value><<<dim3(p.units, p.tiles), 256, 0, st>>>(s, lddz, (unsigned)nregion + p.slots, (const T*)X, (const A*)W, (const A*)bias, regions,
+                                                                                    (const uint32_t*)work, (const T*)dZ, (T*)dX, (A*)part);
         });
     });
-    sum_partials(st, dtype, part, p.units + p.slot_units, taps * D, dW, D, dbias, 0, nullptr);
+    sum_partials(st, dtype, part, p.units, taps * D, dW, D, dbias, 0, nullptr);
     DBK_LAUNCH_OK();
 }
 

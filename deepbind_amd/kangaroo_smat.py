@@ -335,6 +335,7 @@ def causalconv_step(X, W, b, state, silu=True, into=None, out=None):
     its successor goes to `into`, which leaves it as it is."""
     code, wide, n, D, K = _conv_args(X, W, b)
     require(state is not None, "ValueError: state is needed")
+    into = None if into is state else into
     _lib.check_dense("state", state, (n, K - 1, D), X.dtype)
     _lib.check_dense("into", into, (n, K - 1, D), X.dtype)
     if out is not None:
@@ -445,6 +446,7 @@ def statescan_step(X, dt, A, B, C, state, D=None, gate=None, dt_bias=None, softp
     otherwise as in statescan. The state moves on in place, or its successor goes to `into`, which leaves it as it is."""
     a, wide, n, D_, S, G = _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus)
     require(state is not None, "ValueError: state is needed")
+    into = None if into is state else into
     _lib.check_dense("state", state, (n, S, D_), wide)
     _lib.check_dense("into", into, (n, S, D_), wide)
     if out is not None:
