@@ -448,3 +448,111 @@ def test_refusals_on_the_device():
               lambda: ks.causalconv(X, W, b, T.cpu())):
         with pytest.raises(DeepbindError):
             f()
+
+
+# ------------------------------------------------------------------------------------------------ sizes beyond the tables above
+def _many(rng, count, most):
+    """Regions of 0 to `most` rows in random order, with gaps between some of them."""
+    lens = rng.integers(0, most + 1, size=count)
+    starts = np.cumsum(np.concatenate([[2], lens[:-1] + rng.integers(0, 2, size=count - 1)]))
+    return np.stack([starts, starts + lens], 1)[rng.permutation(count)], int(starts[-1] + lens[-1]) + 3
+
+
+def test_more_regions_than_workgroups_that_add_up_gradients():
+    """5000 regions of up to three rows: each workgroup takes several; B and C with row strides of their own."""
+    from deepbind_amd import kangaroo_smat as ks
+    rng = np.random.default_rng(31)
+    R, N = _many(rng, 5000, 3)
+    D, S, K = 6, 3, 4
+    f = lambda *s: rng.standard_normal(s)  # noqa: E731
+    rows = inside(R, N)
+    T = regions(R)
+    X, x = put(f(N, D), torch.float32)
+    dt, dtv = sliced(f(N, D), torch.float32, 2)
+    B, b = sliced(f(N, S), torch.float32, 1)
+    C, c = put(f(N, S), torch.float32)
+    gate, gv = sliced(f(N, D), torch.float32, 5)
+    dY, dy = put(f(N, D), torch.float32)
+    A, a = put(-np.exp(f(S, D)), torch.float32)
+    skip, sv = put(f(1, D), torch.float32)
+    kw = dict(D=skip, gate=gate)
+    keep = ks.kept_states(X, A)
+    Y, last = ks.statescan(X, dt, A, B, C, T, keep=keep, want_state=True, **kw)
+    got = ks.statescan_bprop(X, dt, A, B, C, T, keep, dY, **kw)
+    want, size = ref.statescan(x, dtv, a, b, c, R, sv, gv, np.zeros((1, D)), dY=dy)
+    k = 16 * (3 + 8) + S
+    check(Y[rows], want[0][rows], size[0][rows], k, "float32", "Y")
+    check(last, want[1], size[1], k, "float32", "last", stored=False)
+    for name, g, w, z in zip(("dX", "ddt", "dA", "dB", "dC", "dD", "dgate"), got, want[2:], size[2:]):
+        per_row = name in ("dX", "ddt", "dB", "dC", "dgate")
+        if per_row:
+            g, w, z = g[rows], w[rows], z[rows]
+        check(g, w, z, 2 * k + D + (0 if per_row else len(rows)), "float32", name)
+    W, wv = put(f(K, D), torch.float32)
+    bias, bv = put(f(1, D), torch.float32)
+    Z, _ = ks.causalconv(X, W, bias, T)
+    (zr, _), (zs, _) = ref.causalconv(x, wv, bv, R)
+    check(Z[rows], zr[rows], zs[rows], K + 12, "float32", "Z")
+    grads = ks.causalconv_bprop(X, W, bias, T, dY)
+    (dxr, dwr, dbr), (dxs, dws, dbs) = ref.causalconv_bprop(x, wv, bv, R, dy)
+    check(grads[0][rows], dxr[rows], dxs[rows], 2 * (K + 12), "float32", "conv dX")
+    check(grads[1], dwr, dws, K + 12 + len(rows), "float32", "conv dW")
+    check(grads[2], dbr, dbs, K + 12 + len(rows), "float32", "conv db")
+
+
+def test_maps_of_more_than_2_to_the_31_values():
+    """The last rows of a map whose elements do not fit 31 bits give what the same rows give in a small map."""
+    from deepbind_amd import kangaroo_smat as ks, smat as sm
+    D, S, L = 1024, 2, 300
+    N = (1 << 21) + 1000                          # N * D = 2.148e9 elements, 4.3 GB of bfloat16
+    g = torch.Generator(device="cuda")
+    g.manual_seed(3)
+    small = lambda *s, dtype=torch.bfloat16: torch.randn(s, generator=g, device="cuda").to(dtype)  # noqa: E731
+    ends = [(0, L), (N - L, N)]
+    rows = {n: (small(L, D), small(L, D)) for n in ("X", "dt", "dY")}
+    wb = {n: (small(L, S, dtype=torch.float32), small(L, S, dtype=torch.float32)) for n in ("B", "C")}
+    big = {}
+    for n, parts in list(rows.items()) + list(wb.items()):
+        big[n] = torch.empty(N, parts[0].shape[1], dtype=parts[0].dtype, device="cuda")
+        for (s, e), part in zip(ends, parts):
+            big[n][s:e] = part
+    A, W, b = -torch.rand((S, D), generator=g, device="cuda"), small(4, D, dtype=torch.float32), small(1, D, dtype=torch.float32)
+    T, T1 = regions(ends), regions([[0, L]])
+    out = torch.empty(N, D, dtype=torch.bfloat16, device="cuda")
+    keep = ks.kept_states(big["X"], A)
+    grads = (torch.empty_like(out), torch.empty_like(out), None, torch.empty(N, S, device="cuda"), torch.empty(N, S, device="cuda"), None, None, None)
+    ks.statescan(big["X"], big["dt"], A, big["B"], big["C"], T, keep=keep, out=out)
+    got = ks.statescan_bprop(big["X"], big["dt"], A, big["B"], big["C"], T, keep, big["dY"], out=grads)
+    sums = 0
+    for i, (s, e) in enumerate(ends):
+        p = [rows["X"][i], rows["dt"][i], A, wb["B"][i], wb["C"][i], T1]
+        k1 = ks.kept_states(p[0], A)
+        y, _ = ks.statescan(*p, keep=k1)
+        want = ks.statescan_bprop(*p, k1, rows["dY"][i])
+        # the rows are cut differently in the two maps: two float32 ways to the same sums of some hundred terms, then bfloat16
+        near = lambda u, v: float((u.double() - v.double()).abs().max()) <= 2 * 2.0 ** -8 * float(v.double().abs().max())  # noqa: E731
+        assert near(out[s:e], y) and near(got[0][s:e], want[0]) and near(got[1][s:e], want[1]) and near(got[3][s:e], want[3]) and near(got[4][s:e], want[4])
+        sums = sums + want[2].double()
+    assert float((got[2].double() - sums).abs().max()) <= 1e-4 * float(sums.abs().max())
+    del keep, grads, got
+    ks.causalconv(big["X"], W, b, T, out=out)
+    dX, dW, _ = ks.causalconv_bprop(big["X"], W, b, T, big["dY"], out=(torch.empty_like(out), None, None))
+    for i, (s, e) in enumerate(ends):            # the same operations on the same numbers, row by row
+        assert torch.equal(out[s:e], ks.causalconv(rows["X"][i], W, b, T1)[0])
+        assert torch.equal(dX[s:e], ks.causalconv_bprop(rows["X"][i], W, b, T1, rows["dY"][i])[0])
+    Z, stats = sm.layernorm(big["X"], nchunk=4, want_stats=True, out=out)
+    for i, (s, e) in enumerate(ends):
+        z, _ = sm.layernorm(rows["X"][i], nchunk=4)
+        assert torch.equal(Z[s:e], z)
+
+
+def test_state_may_be_named_as_its_own_successor():
+    from deepbind_amd import kangaroo_smat as ks
+    X, W, b = torch.randn(3, 8, device="cuda"), torch.randn(3, 8, device="cuda"), torch.randn(1, 8, device="cuda")
+    s0 = torch.randn(3, 2, 8, device="cuda")
+    s1, s2 = s0.clone(), s0.clone()
+    assert torch.equal(ks.causalconv_step(X, W, b, s1), ks.causalconv_step(X, W, b, s2, into=s2)) and torch.equal(s1, s2)
+    A, B = -torch.rand(4, 8, device="cuda"), torch.randn(3, 4, device="cuda")
+    h0 = torch.randn(3, 4, 8, device="cuda")
+    h1, h2 = h0.clone(), h0.clone()
+    assert torch.equal(ks.statescan_step(X, X, A, B, B, h1), ks.statescan_step(X, X, A, B, B, h2, into=h2)) and torch.equal(h1, h2) and not torch.equal(h0, h1)
