@@ -235,69 +235,70 @@ def _shape_or_type(name, t, shape, dtype, what):
     raise DeepbindError("TypeError: %s must be %s, got %s" % (name, dtype, t.dtype))
 
 
-def check_rows(name, t, shape, dtype):
-    """A matrix of rows: its own row stride, elements of a row next to each other."""
-    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype:
-        _shape_or_type(name, t, shape, dtype, "a %s matrix")
-    if t.is_contiguous():
-        return
-    rows, cols = shape
-    if cols > 1 and t.stride(1) != 1:
-        raise DeepbindError("ValueError: the elements of a row of %s must lie next to each other" % name)
-    if rows > 1 and t.stride(0) < cols:
-        raise DeepbindError("ValueError: the rows of %s must not overlap" % name)
+_ITEM = {torch.float32: 4, torch.float64: 8, torch.bfloat16: 2, torch.uint32: 4, torch.int32: 4}
 
 
-def check_dense(name, t, shape, dtype):
-    """A contiguous array of weights or states; None passes."""
-    if t is None:
-        return
-    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype:
-        _shape_or_type(name, t, shape, dtype, "%s")
-    if not t.is_contiguous():
-        raise DeepbindError("ValueError: %s must be contiguous" % name)
+class Arguments(object):
+    """The tensors of one call of a row operator: each is checked as it is added, for shape, type and layout, and all of them in check()."""
+    __slots__ = ("ins", "outs")
 
+    def __init__(self):
+        self.ins, self.outs = [], []
 
-def row_stride(t):
-    if t is None:
-        return 0
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    def rows(self, name, t, shape, dtype, out=False):
+        """A matrix of rows, its own row stride, elements of a row next to each other: (pointer, row stride)."""
+        if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype:
+            _shape_or_type(name, t, shape, dtype, "a %s matrix")
+        p = t.data_ptr()
+        n, ld = shape
+        if t.is_contiguous():
+            hi = p + n * ld * _ITEM[dtype]
+        else:
+            step, one = t.stride()
+            if ld > 1 and one != 1:
+                raise DeepbindError("ValueError: the elements of a row of %s must lie next to each other" % name)
+            if n > 1:
+                if step < ld:
+                    raise DeepbindError("ValueError: the rows of %s must not overlap" % name)
+                hi = p + ((n - 1) * step + ld) * _ITEM[dtype]
+                ld = step
+            else:
+                hi = p + ld * _ITEM[dtype]
+        (self.outs if out else self.ins).append((p, hi, t.get_device(), t))
+        return p, ld
 
-
-def same_device(*tensors):
-    """Refuses tensors that are not on the current device, whose stream the call would run on."""
-    current = None
-    for t in tensors:
+    def dense(self, name, t, shape, dtype, out=False):
+        """The pointer of a contiguous array of weights or states; None passes."""
         if t is None:
-            continue
-        at = t.get_device()
-        if at != current:
-            if at < 0:
-                raise DeepbindError("TypeError: expected a device tensor, got a host tensor")
-            current = torch.cuda.current_device()
+            return None
+        if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not dtype:
+            _shape_or_type(name, t, shape, dtype, "%s")
+        if not t.is_contiguous():
+            raise DeepbindError("ValueError: %s must be contiguous" % name)
+        p = t.data_ptr()
+        (self.outs if out else self.ins).append((p, p + t.numel() * _ITEM[dtype], t.get_device(), t))
+        return p
+
+    def check(self):
+        """Everything on the current device, whose stream the call runs on, and no output on an input's memory or another output's."""
+        current = None
+        for _, _, at, _ in self.ins + self.outs:
             if at != current:
-                raise DeepbindError("ValueError: a tensor lies on device %d, the current device is %d" % (at, current))
-
-
-def _span(t):
-    lo = t.data_ptr()
-    if t.is_contiguous():
-        return lo, lo + t.numel() * t.element_size()
-    return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-
-
-def not_shared(outs, ins):
-    """Refuses outputs that overlap an input's memory or each other's."""
-    known = [_span(t) + (t,) for t in ins if t is not None and t.numel()]
-    for t in outs:
-        if t is None or not t.numel():
-            continue
-        lo, hi = _span(t)
-        for lo2, hi2, t2 in known:
-            # (blocks of columns of one wider matrix: their spans overlap, their elements need not)
-            if lo < hi2 and lo2 < hi and not _column_blocks(*((t, t2) if lo <= lo2 else (t2, t))):
-                raise DeepbindError("ValueError: an output shares memory with another argument")
-        known.append((lo, hi, t))
+                if at < 0:
+                    raise DeepbindError("TypeError: expected a device tensor, got a host tensor")
+                current = torch.cuda.current_device()
+                if at != current:
+                    raise DeepbindError("ValueError: a tensor lies on device %d, the current device is %d" % (at, current))
+        known = self.ins
+        for out in self.outs:
+            lo, hi, _, t = out
+            if lo == hi:
+                continue
+            for lo2, hi2, _, t2 in known:
+                # (blocks of columns of one wider matrix: their spans overlap, their elements need not)
+                if lo < hi2 and lo2 < hi and lo2 != hi2 and not _column_blocks(*((t, t2) if lo <= lo2 else (t2, t))):
+                    raise DeepbindError("ValueError: an output shares memory with another argument")
+            known = known + [out]
 
 
 def _column_blocks(a, b):
@@ -309,14 +310,16 @@ def _column_blocks(a, b):
     return off % ld >= a.shape[1] and off % ld + b.shape[1] <= ld
 
 
-def raw(t):
-    """Device pointer of a tensor that has been checked (None -> NULL)."""
-    return None if t is None else t.data_ptr()
+def row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def workspace(nbytes, like):
-    """Scratch of one call, from torch's allocator: its own under capture, returned to the stream's pool afterwards."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device) if nbytes else None
+    """Scratch of one call, from torch's allocator: its own under capture, returned to the stream's pool afterwards. (tensor, pointer)"""
+    if not nbytes:
+        return None, None
+    t = torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    return t, t.data_ptr()
 
 
 def require(cond, msg):

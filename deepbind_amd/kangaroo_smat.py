@@ -248,36 +248,36 @@ def scanpool_bprop(W, b, X, regions, ptype, pooled, argmax, dpooled, dW, db, ove
 # ------------------------------------------------------------------------------------------------
 # layers along the rows of every region, between the motif scan and the pooling
 # ------------------------------------------------------------------------------------------------
-def _row_regions(R):
+def _row_regions(a, R):
     _regions(R)
     if R.shape[1] != 2 or not R.is_contiguous():
         raise DeepbindError("ValueError: regions must be a contiguous (P x 2) array")
-    return R
+    return R.shape[0], a.dense("regions", R, R.shape, R.dtype)
 
 
 def _map(X):
     if not isinstance(X, torch.Tensor) or X.dim() != 2:
         raise DeepbindError("ValueError: X must be a matrix")
-    _lib.check_rows("X", X, X.shape, X.dtype)
     return _lib.row_dtype_code(X), _lib.wide_dtype(X), X.shape[0], X.shape[1]
 
 
-def _out(name, t, shape, dtype, device, dense=False):
-    """An output that the caller gave, or a new one: zeros, as rows in no region are not written."""
-    if t is None:
-        return (torch.empty if dense else torch.zeros)(shape, dtype=dtype, device=device)
-    (_lib.check_dense if dense else _lib.check_rows)(name, t, shape, dtype)
-    return t
+def _rows_out(t, shape, dtype, device):
+    """A matrix of rows that the caller gave, or a new one: zeros, as rows in no region are not written."""
+    return torch.zeros(shape, dtype=dtype, device=device) if t is None else t
+
+
+def _dense_out(t, shape, dtype, device):
+    return torch.empty(shape, dtype=dtype, device=device) if t is None else t
 
 
 def _conv_args(X, W, b):
     code, wide, N, D = _map(X)
     require(isinstance(W, torch.Tensor) and W.dim() == 2 and W.shape[1] == D, "ValueError: W must be (taps x channels)")
-    if not 1 <= W.shape[0] <= 4:
-        raise DeepbindError("NotImplementedError: filters of 1 to 4 taps, got %d" % W.shape[0])
-    _lib.check_dense("W", W, W.shape, wide)
-    _lib.check_dense("b", b, (1, D), wide)
-    return code, wide, N, D, W.shape[0]
+    K = W.shape[0]
+    if not 1 <= K <= 4:
+        raise DeepbindError("NotImplementedError: filters of 1 to 4 taps, got %d" % K)
+    a = _lib.Arguments()
+    return (a, code, wide, N, D, K) + a.rows("X", X, (N, D), X.dtype) + (a.dense("W", W, (K, D), wide), a.dense("b", b, (1, D), wide))
 
 
 def causalconv(X, W, b, regions, silu=True, state=None, want_state=False, out=None):
@@ -287,65 +287,59 @@ def causalconv(X, W, b, regions, silu=True, state=None, want_state=False, out=No
     order and must not overlap; rows in no region are zeros in a new output, and stay as they are in `out`.
     Rows before a region's first are those of state (P x taps-1 x D, X's type) or zeros.
     Returns (Z, last|None): with want_state, last is what the next piece of each sequence takes as its state."""
-    code, wide, N, D, K = _conv_args(X, W, b)
-    P = _row_regions(regions).shape[0]
-    _lib.check_dense("state", state, (P, K - 1, D), X.dtype)
+    a, code, wide, N, D, K, x, ldx, w, bp = _conv_args(X, W, b)
+    P, rp = _row_regions(a, regions)
+    sp = a.dense("state", state, (P, K - 1, D), X.dtype)
     if out is not None:
-        _lib.check_rows("out", out, (N, D), X.dtype)
-    _lib.same_device(X, W, b, regions, state, out)
-    if out is not None:
-        _lib.not_shared((out,), (X, W, b, regions, state))
-    Z = _out("out", out, (N, D), X.dtype, X.device)
+        a.rows("out", out, (N, D), X.dtype, out=True)
+    a.check()
+    Z = _rows_out(out, (N, D), X.dtype, X.device)
     last = torch.empty((P, K - 1, D), dtype=X.dtype, device=X.device) if want_state else None
     need = ctypes.c_size_t(0)
     call("dbk_causalconv_workspace", code, K, N, D, P, 0, ctypes.addressof(need))
-    work = _lib.workspace(need.value, X)
-    raw, ld = _lib.raw, _lib.row_stride
-    call("dbk_causalconv", stream(), code, raw(X), ld(X), raw(W), raw(b), K, N, D, raw(regions), P, int(bool(silu)), raw(state), raw(Z), ld(Z), raw(last),
-         raw(work), need.value)
+    work, wp = _lib.workspace(need.value, X)
+    call("dbk_causalconv", stream(), code, x, ldx, w, bp, K, N, D, rp, P, int(bool(silu)), sp, Z.data_ptr(), _lib.row_stride(Z),
+         None if last is None else last.data_ptr(), wp, need.value)
     return Z, last
 
 
 def causalconv_bprop(X, W, b, regions, dZ, silu=True, out=None):
     """Gradients (dX, dW, db|None) of causalconv at X, for sequences that start from zeros. out (optional): a tuple like the returned
     one of tensors to write into, None where one is to be made; rows of dX in no region are zeros, or stay as they are in out's."""
-    code, wide, N, D, K = _conv_args(X, W, b)
-    P = _row_regions(regions).shape[0]
-    _lib.check_rows("dZ", dZ, (N, D), X.dtype)
+    a, code, wide, N, D, K, x, ldx, w, bp = _conv_args(X, W, b)
+    P, rp = _row_regions(a, regions)
+    dz, lddz = a.rows("dZ", dZ, (N, D), X.dtype)
     dX, dW, db = (None, None, None) if out is None else out
     require(b is not None or db is None, "ValueError: no bias, no gradient of it")
-    _lib.same_device(X, W, b, regions, dZ, dX, dW, db)
-    if out is not None:
-        _lib.not_shared((dX, dW, db), (X, W, b, regions, dZ))
-    dX = _out("dX", dX, (N, D), X.dtype, X.device)
-    dW = _out("dW", dW, (K, D), wide, X.device, dense=True)
-    if b is not None:
-        db = _out("db", db, (1, D), wide, X.device, dense=True)
+    if dX is not None:
+        a.rows("dX", dX, (N, D), X.dtype, out=True)
+    a.dense("dW", dW, (K, D), wide, out=True)
+    a.dense("db", db, (1, D), wide, out=True)
+    a.check()
+    dX = _rows_out(dX, (N, D), X.dtype, X.device)
+    dW = _dense_out(dW, (K, D), wide, X.device)
+    db = None if b is None else _dense_out(db, (1, D), wide, X.device)
     need = ctypes.c_size_t(0)
     call("dbk_causalconv_workspace", code, K, N, D, P, 1, ctypes.addressof(need))
-    work = _lib.workspace(need.value, X)
-    raw, ld = _lib.raw, _lib.row_stride
-    call("dbk_causalconv_bprop", stream(), code, raw(X), ld(X), raw(W), raw(b), K, N, D, raw(regions), P, int(bool(silu)), raw(dZ), ld(dZ), raw(dX), ld(dX),
-         raw(dW), raw(db), raw(work), need.value)
+    work, wp = _lib.workspace(need.value, X)
+    call("dbk_causalconv_bprop", stream(), code, x, ldx, w, bp, K, N, D, rp, P, int(bool(silu)), dz, lddz, dX.data_ptr(), _lib.row_stride(dX),
+         dW.data_ptr(), None if db is None else db.data_ptr(), wp, need.value)
     return dX, dW, db
 
 
 def causalconv_step(X, W, b, state, silu=True, into=None, out=None):
     """One new row for each of n sequences: X (n x D) and state (n x taps-1 x D) give Z (n x D). The state moves on in place, or
     its successor goes to `into`, which leaves it as it is."""
-    code, wide, n, D, K = _conv_args(X, W, b)
+    a, code, wide, n, D, K, x, ldx, w, bp = _conv_args(X, W, b)
     require(state is not None, "ValueError: state is needed")
     into = None if into is state else into
-    _lib.check_dense("state", state, (n, K - 1, D), X.dtype)
-    _lib.check_dense("into", into, (n, K - 1, D), X.dtype)
+    sp = a.dense("state", state, (n, K - 1, D), X.dtype, out=into is None)
+    ip = sp if into is None else a.dense("into", into, (n, K - 1, D), X.dtype, out=True)
     if out is not None:
-        _lib.check_rows("out", out, (n, D), X.dtype)
-    _lib.same_device(X, W, b, state, into, out)
-    _lib.not_shared((out, into) if into is not None else (out, state), (X, W, b, state if into is not None else None))
-    Z = _out("out", out, (n, D), X.dtype, X.device, dense=out is None)
-    raw, ld = _lib.raw, _lib.row_stride
-    call("dbk_causalconv_step", stream(), code, raw(X), ld(X), raw(W), raw(b), K, n, D, int(bool(silu)), raw(state), raw(state if into is None else into),
-         raw(Z), ld(Z))
+        a.rows("out", out, (n, D), X.dtype, out=True)
+    a.check()
+    Z = _dense_out(out, (n, D), X.dtype, X.device)
+    call("dbk_causalconv_step", stream(), code, x, ldx, w, bp, K, n, D, int(bool(silu)), sp, ip, Z.data_ptr(), _lib.row_stride(Z))
     return Z
 
 
@@ -363,18 +357,16 @@ def _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus):
     require(isinstance(B, torch.Tensor) and B.dim() == 2 and B.shape[1] % S == 0 and B.shape[1] >= S, "ValueError: B must be (rows x groups * states)")
     G = B.shape[1] // S
     require(D_ % G == 0, "ValueError: the number of channels must be divisible by the number of groups")
-    _lib.check_rows("dt", dt, (N, D_), X.dtype)
-    _lib.check_dense("A", A, (S, D_), wide)
-    _lib.check_rows("B", B, (N, G * S), wide)
-    _lib.check_rows("C", C, (N, G * S), wide)
-    _lib.check_dense("D", D, (1, D_), wide)
-    _lib.check_dense("dt_bias", dt_bias, (1, D_), wide)
-    if gate is not None:
-        _lib.check_rows("gate", gate, (N, D_), X.dtype)
-    raw, ld = _lib.raw, _lib.row_stride
-    a = _lib.StateScanArgs(code, int(bool(softplus)), N, D_, S, G, None, 0, raw(X), ld(X), raw(dt), ld(dt), raw(A), raw(B), ld(B), raw(C), ld(C),
-                           raw(D), raw(dt_bias), raw(gate), ld(gate))
-    return a, wide, N, D_, S, G
+    g = _lib.Arguments()
+    kept, shape, weights = X.dtype, (N, D_), (N, G * S)
+    x, ldx = g.rows("X", X, shape, kept)
+    t, ldt = g.rows("dt", dt, shape, kept)
+    ap = g.dense("A", A, (S, D_), wide)
+    b, ldb = g.rows("B", B, weights, wide)
+    c, ldc = g.rows("C", C, weights, wide)
+    sk, bi = g.dense("D", D, (1, D_), wide), g.dense("dt_bias", dt_bias, (1, D_), wide)
+    gp, ldg = (None, 0) if gate is None else g.rows("gate", gate, shape, kept)
+    return g, _lib.StateScanArgs(code, int(bool(softplus)), N, D_, S, G, None, 0, x, ldx, t, ldt, ap, b, ldb, c, ldc, sk, bi, gp, ldg), wide, N, D_, S, G
 
 
 def statescan(X, dt, A, B, C, regions, D=None, gate=None, dt_bias=None, softplus=True, state=None, want_state=False, keep=None, out=None):
@@ -387,24 +379,25 @@ def statescan(X, dt, A, B, C, regions, D=None, gate=None, dt_bias=None, softplus
     they are in `out`. States start from state (P x S x D), or zeros.
     keep (optional, from kept_states): receives the states that statescan_bprop starts from (without `state` only).
     Returns (Y, last|None): with want_state, last (P x S x D) holds the states behind the regions' last rows."""
-    a, wide, N, D_, S, G = _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus)
-    P = _row_regions(regions).shape[0]
-    _lib.check_dense("state", state, (P, S, D_), wide)
-    _lib.check_dense("keep", keep, ((N + 7) // 8, S, D_), wide)
+    g, a, wide, N, D_, S, G = _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus)
+    P, a.regions = _row_regions(g, regions)
+    a.nregion = P
+    a.state = g.dense("state", state, (P, S, D_), wide)
+    a.keep = g.dense("keep", keep, ((N + 7) // 8, S, D_), wide, out=True)
     require(keep is None or state is None, "ValueError: states are kept for the backward pass of whole sequences, which starts from zeros: no initial state")
     if out is not None:
-        _lib.check_rows("out", out, (N, D_), X.dtype)
-    _lib.same_device(X, dt, A, B, C, regions, D, gate, dt_bias, state, keep, out)
-    if out is not None or keep is not None:
-        _lib.not_shared((out, keep), (X, dt, A, B, C, regions, D, gate, dt_bias, state))
-    Y = _out("out", out, (N, D_), X.dtype, X.device)
-    last = torch.empty((P, S, D_), dtype=wide, device=X.device) if want_state else None
-    raw = _lib.raw
-    a.regions, a.nregion, a.state, a.Y, a.ldy, a.last, a.keep = raw(regions), P, raw(state), raw(Y), _lib.row_stride(Y), raw(last), raw(keep)
-    need = ctypes.c_size_t(0)
-    call("dbk_statescan_workspace", ctypes.addressof(a), 0, ctypes.addressof(need))
-    work = _lib.workspace(need.value, X)
-    call("dbk_statescan", stream(), ctypes.addressof(a), raw(work), need.value)
+        g.rows("out", out, (N, D_), X.dtype, out=True)
+    g.check()
+    Y = _rows_out(out, (N, D_), X.dtype, X.device)
+    a.Y, a.ldy = Y.data_ptr(), _lib.row_stride(Y)
+    last = None
+    if want_state:
+        last = torch.empty((P, S, D_), dtype=wide, device=X.device)
+        a.last = last.data_ptr()
+    at, need = ctypes.addressof(a), ctypes.c_size_t(0)
+    call("dbk_statescan_workspace", at, 0, ctypes.addressof(need))
+    work, wp = _lib.workspace(need.value, X)
+    call("dbk_statescan", stream(), at, wp, need.value)
     return Y, last
 
 
@@ -412,49 +405,57 @@ def statescan_bprop(X, dt, A, B, C, regions, keep, dY, D=None, gate=None, dt_bia
     """Gradients (dX, ddt, dA, dB, dC, dD|None, dgate|None, ddt_bias|None) of statescan for sequences that start from zero states,
     from the states that the forward call kept. out (optional): a tuple like the returned one of tensors to write into, None where
     one is to be made; rows in no region are zeros, or stay as they are in out's."""
-    a, wide, N, D_, S, G = _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus)
-    P = _row_regions(regions).shape[0]
+    g, a, wide, N, D_, S, G = _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus)
+    P, a.regions = _row_regions(g, regions)
+    a.nregion = P
     require(keep is not None, "ValueError: the states that the forward call kept are needed")
-    _lib.check_dense("keep", keep, ((N + 7) // 8, S, D_), wide)
-    _lib.check_rows("dY", dY, (N, D_), X.dtype)
+    a.keep = g.dense("keep", keep, ((N + 7) // 8, S, D_), wide)
+    kept, dev, shape, weights = X.dtype, X.device, (N, D_), (N, G * S)
+    a.dY, a.lddy = g.rows("dY", dY, shape, kept)
     dX, ddt, dA, dB, dC, dD, dgate, dbias = (None,) * 8 if out is None else out
     for given, grad, name in ((D, dD, "D"), (gate, dgate, "gate"), (dt_bias, dbias, "dt_bias")):
-        require(given is not None or grad is None, "ValueError: no %s, no gradient of it" % name)
-    _lib.same_device(X, dt, A, B, C, regions, keep, dY, D, gate, dt_bias, dX, ddt, dA, dB, dC, dD, dgate, dbias)
-    if out is not None:
-        _lib.not_shared((dX, ddt, dA, dB, dC, dD, dgate, dbias), (X, dt, A, B, C, regions, keep, dY, D, gate, dt_bias))
-    dev = X.device
-    dX, ddt = _out("dX", dX, (N, D_), X.dtype, dev), _out("ddt", ddt, (N, D_), X.dtype, dev)
-    dA = _out("dA", dA, (S, D_), wide, dev, dense=True)
-    dB, dC = _out("dB", dB, (N, G * S), wide, dev), _out("dC", dC, (N, G * S), wide, dev)
-    dD = None if D is None else _out("dD", dD, (1, D_), wide, dev, dense=True)
-    dgate = None if gate is None else _out("dgate", dgate, (N, D_), X.dtype, dev)
-    dbias = None if dt_bias is None else _out("ddt_bias", dbias, (1, D_), wide, dev, dense=True)
-    raw, ld = _lib.raw, _lib.row_stride
-    a.regions, a.nregion, a.keep, a.dY, a.lddy = raw(regions), P, raw(keep), raw(dY), ld(dY)
-    a.dX, a.lddx, a.ddt, a.ldddt, a.dgate, a.lddgate = raw(dX), ld(dX), raw(ddt), ld(ddt), raw(dgate), ld(dgate)
-    a.dB, a.lddb, a.dC, a.lddc, a.dA, a.dskip, a.ddt_bias = raw(dB), ld(dB), raw(dC), ld(dC), raw(dA), raw(dD), raw(dbias)
-    need = ctypes.c_size_t(0)
-    call("dbk_statescan_workspace", ctypes.addressof(a), 1, ctypes.addressof(need))
-    work = _lib.workspace(need.value, X)
-    call("dbk_statescan_bprop", stream(), ctypes.addressof(a), raw(work), need.value)
+        if given is None and grad is not None:
+            raise DeepbindError("ValueError: no %s, no gradient of it" % name)
+    for name, t, s, dtype in (("dX", dX, shape, kept), ("ddt", ddt, shape, kept), ("dgate", dgate, shape, kept), ("dB", dB, weights, wide), ("dC", dC, weights, wide)):
+        if t is not None:
+            g.rows(name, t, s, dtype, out=True)
+    for name, t, s in (("dA", dA, (S, D_)), ("dD", dD, (1, D_)), ("ddt_bias", dbias, (1, D_))):
+        g.dense(name, t, s, wide, out=True)
+    g.check()
+    dX, ddt = _rows_out(dX, shape, kept, dev), _rows_out(ddt, shape, kept, dev)
+    dA = _dense_out(dA, (S, D_), wide, dev)
+    dB, dC = _rows_out(dB, weights, wide, dev), _rows_out(dC, weights, wide, dev)
+    dD = None if D is None else _dense_out(dD, (1, D_), wide, dev)
+    dgate = None if gate is None else _rows_out(dgate, shape, kept, dev)
+    dbias = None if dt_bias is None else _dense_out(dbias, (1, D_), wide, dev)
+    ld = _lib.row_stride
+    a.dX, a.lddx, a.ddt, a.ldddt, a.dB, a.lddb, a.dC, a.lddc = dX.data_ptr(), ld(dX), ddt.data_ptr(), ld(ddt), dB.data_ptr(), ld(dB), dC.data_ptr(), ld(dC)
+    a.dA = dA.data_ptr()
+    if dgate is not None:
+        a.dgate, a.lddgate = dgate.data_ptr(), ld(dgate)
+    if dD is not None:
+        a.dskip = dD.data_ptr()
+    if dbias is not None:
+        a.ddt_bias = dbias.data_ptr()
+    at, need = ctypes.addressof(a), ctypes.c_size_t(0)
+    call("dbk_statescan_workspace", at, 1, ctypes.addressof(need))
+    work, wp = _lib.workspace(need.value, X)
+    call("dbk_statescan_bprop", stream(), at, wp, need.value)
     return dX, ddt, dA, dB, dC, dD, dgate, dbias
 
 
 def statescan_step(X, dt, A, B, C, state, D=None, gate=None, dt_bias=None, softplus=True, into=None, out=None):
     """One new row for each of n sequences: Y (n x D) from X, dt, gate (n x D), B, C (n x G*S) and state (n x S x D), arguments
     otherwise as in statescan. The state moves on in place, or its successor goes to `into`, which leaves it as it is."""
-    a, wide, n, D_, S, G = _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus)
+    g, a, wide, n, D_, S, G = _scan_args(X, dt, A, B, C, D, gate, dt_bias, softplus)
     require(state is not None, "ValueError: state is needed")
     into = None if into is state else into
-    _lib.check_dense("state", state, (n, S, D_), wide)
-    _lib.check_dense("into", into, (n, S, D_), wide)
+    a.state = g.dense("state", state, (n, S, D_), wide, out=into is None)
+    a.last = a.state if into is None else g.dense("into", into, (n, S, D_), wide, out=True)
     if out is not None:
-        _lib.check_rows("out", out, (n, D_), X.dtype)
-    _lib.same_device(X, dt, A, B, C, D, gate, dt_bias, state, into, out)
-    _lib.not_shared((out, into) if into is not None else (out, state), (X, dt, A, B, C, D, gate, dt_bias, state if into is not None else None))
-    Y = _out("out", out, (n, D_), X.dtype, X.device, dense=out is None)
-    raw = _lib.raw
-    a.state, a.last, a.Y, a.ldy = raw(state), raw(state if into is None else into), raw(Y), _lib.row_stride(Y)
+        g.rows("out", out, (n, D_), X.dtype, out=True)
+    g.check()
+    Y = _dense_out(out, (n, D_), X.dtype, X.device)
+    a.Y, a.ldy = Y.data_ptr(), _lib.row_stride(Y)
     call("dbk_statescan_step", stream(), ctypes.addressof(a))
     return Y

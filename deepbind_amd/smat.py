@@ -112,13 +112,12 @@ def softmax(X, nchunk=1):
 
 
 def _norm_args(X, gamma, beta, nchunk):
-    require(isinstance(X, torch.Tensor) and X.dim() == 2, "ValueError: X must be a matrix")
+    if not isinstance(X, torch.Tensor) or X.dim() != 2:
+        raise _lib.DeepbindError("ValueError: X must be a matrix")
     code, wide, (n, m) = _lib.row_dtype_code(X), _lib.wide_dtype(X), X.shape
     require(nchunk >= 1 and m % nchunk == 0 and m >= nchunk, "ValueError: the number of columns must be divisible by nchunk")
-    _lib.check_rows("X", X, (n, m), X.dtype)
-    _lib.check_dense("gamma", gamma, (1, m), wide)
-    _lib.check_dense("beta", beta, (1, m), wide)
-    return code, wide, n, m
+    a = _lib.Arguments()
+    return (a, code, wide, n, m) + a.rows("X", X, (n, m), X.dtype) + (a.dense("gamma", gamma, (1, m), wide), a.dense("beta", beta, (1, m), wide))
 
 
 def layernorm(X, gamma=None, beta=None, nchunk=1, eps=1e-5, want_stats=False, out=None):
@@ -127,45 +126,42 @@ def layernorm(X, gamma=None, beta=None, nchunk=1, eps=1e-5, want_stats=False, ou
     X: float32, float64 or bfloat16 with a row stride of its own; weights and statistics float32 (float64 beside float64).
     Returns (Z, stats|None); stats (2 x n*nchunk): the chunks' means and reciprocal deviations, which layernorm_bprop takes.
     out (optional): the matrix to write into."""
-    code, wide, n, m = _norm_args(X, gamma, beta, nchunk)
-    Z = torch.empty((n, m), dtype=X.dtype, device=X.device) if out is None else out
-    _lib.check_rows("out", Z, (n, m), X.dtype)
-    _lib.same_device(X, gamma, beta, out)
+    a, code, wide, n, m, x, ldx, g, b = _norm_args(X, gamma, beta, nchunk)
     if out is not None:
-        _lib.not_shared((out,), (X, gamma, beta))
+        a.rows("out", out, (n, m), X.dtype, out=True)
+    a.check()
+    Z = torch.empty((n, m), dtype=X.dtype, device=X.device) if out is None else out
     stats = torch.empty((2, n * nchunk), dtype=wide, device=X.device) if want_stats else None
-    call("dbk_layernorm", stream(), code, _lib.raw(X), _lib.row_stride(X), _lib.raw(gamma), _lib.raw(beta), n, m, m // nchunk, float(eps),
-         _lib.raw(Z), _lib.row_stride(Z), _lib.raw(stats))
+    call("dbk_layernorm", stream(), code, x, ldx, g, b, n, m, m // nchunk, float(eps), Z.data_ptr(), _lib.row_stride(Z),
+         None if stats is None else stats.data_ptr())
     return Z, stats
 
 
 def layernorm_bprop(X, gamma, stats, dZ, nchunk=1, out=None):
     """Gradients (dX, dgamma, dbeta) of layernorm at X with the stats of its forward call; without gamma (None) the last two are None
     (pass ones to get them). out (optional): a tuple like the returned one of tensors to write into, None where one is to be made."""
-    code, wide, n, m = _norm_args(X, gamma, None, nchunk)
-    _lib.check_dense("stats", stats, (2, n * nchunk), wide)
+    a, code, wide, n, m, x, ldx, g, _ = _norm_args(X, gamma, None, nchunk)
     require(stats is not None, "ValueError: the statistics of the forward call are needed")
-    _lib.check_rows("dZ", dZ, (n, m), X.dtype)
+    st = a.dense("stats", stats, (2, n * nchunk), wide)
+    dz, lddz = a.rows("dZ", dZ, (n, m), X.dtype)
     dX, dgamma, dbeta = (None, None, None) if out is None else out
-    _lib.same_device(X, gamma, stats, dZ, dX, dgamma, dbeta)
-    if out is not None:
-        _lib.not_shared((dX, dgamma, dbeta), (X, gamma, stats, dZ))
+    require(gamma is not None or (dgamma is None and dbeta is None), "ValueError: no weights, no gradient of them")
+    if dX is not None:
+        a.rows("dX", dX, (n, m), X.dtype, out=True)
+    a.dense("dgamma", dgamma, (1, m), wide, out=True)
+    a.dense("dbeta", dbeta, (1, m), wide, out=True)
+    a.check()
     if dX is None:
         dX = torch.empty((n, m), dtype=X.dtype, device=X.device)
-    _lib.check_rows("dX", dX, (n, m), X.dtype)
-    if gamma is None:
-        require(dgamma is None and dbeta is None, "ValueError: no weights, no gradient of them")
-    else:
+    need = ctypes.c_size_t(0)
+    dg = db = None
+    if gamma is not None:
         dgamma = torch.empty_like(gamma) if dgamma is None else dgamma
         dbeta = torch.empty_like(gamma) if dbeta is None else dbeta
-        _lib.check_dense("dgamma", dgamma, (1, m), wide)
-        _lib.check_dense("dbeta", dbeta, (1, m), wide)
-    need = ctypes.c_size_t(0)
-    if gamma is not None:
+        dg, db = dgamma.data_ptr(), dbeta.data_ptr()
         call("dbk_layernorm_bprop_workspace", code, n, m, m // nchunk, ctypes.addressof(need))
-    work = _lib.workspace(need.value, X)
-    call("dbk_layernorm_bprop", stream(), code, _lib.raw(X), _lib.row_stride(X), _lib.raw(gamma), _lib.raw(stats), _lib.raw(dZ), _lib.row_stride(dZ),
-         n, m, m // nchunk, _lib.raw(dX), _lib.row_stride(dX), _lib.raw(dgamma), _lib.raw(dbeta), _lib.raw(work), need.value)
+    work, wp = _lib.workspace(need.value, X)
+    call("dbk_layernorm_bprop", stream(), code, x, ldx, g, st, dz, lddz, n, m, m // nchunk, dX.data_ptr(), _lib.row_stride(dX), dg, db, wp, need.value)
     return dX, dgamma, dbeta
 
 

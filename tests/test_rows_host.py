@@ -210,13 +210,33 @@ def test_library_refusals_reach_no_device():
 
 
 def test_outputs_that_share_memory_are_told_apart():
-    from deepbind_amd._lib import DeepbindError, not_shared
+    from deepbind_amd._lib import Arguments, DeepbindError
+
+    def shared(outs, ins):
+        a = Arguments()
+        for out, tensors in ((False, ins), (True, outs)):
+            for t in tensors:
+                a.rows("t", t, t.shape, t.dtype, out=out)
+        for group in (a.ins, a.outs):            # (as if they lay on the current device: there is none here)
+            group[:] = [(lo, hi, 0, t) for lo, hi, _, t in group]
+        try:
+            a.check()
+        except DeepbindError as e:
+            assert "shares memory" in str(e)
+            return True
+        return False
+
     base = torch.zeros(8, 12)
-    not_shared((base[:, :6],), (base[:, 6:],))
-    not_shared((base[:, 6:],), (base[:, :6], base[:, 2:4]))
-    not_shared((base[4:],), (base[:4],))
-    not_shared((), (base, base))
-    for outs, ins in (((base,), (base,)), ((base[:, :7],), (base[:, 6:],)), ((base[1:],), (base[:4],)), ((base[:, :3], base[:, 2:5]), ()),
-                      ((base[2:4, :3],), (base[:, 1:2],))):
-        with pytest.raises(DeepbindError):
-            not_shared(outs, ins)
+    before = torch.cuda.current_device
+    torch.cuda.current_device = lambda: 0
+    try:
+        assert not shared((base[:, :6],), (base[:, 6:],))
+        assert not shared((base[:, 6:],), (base[:, :6], base[:, 2:4]))
+        assert not shared((base[4:],), (base[:4],))
+        assert not shared((), (base, base))
+        assert not shared((base,), (base[:0],))
+        for outs, ins in (((base,), (base,)), ((base[:, :7],), (base[:, 6:],)), ((base[1:],), (base[:4],)), ((base[:, :3], base[:, 2:5]), ()),
+                          ((base[2:4, :3],), (base[:, 1:2],))):
+            assert shared(outs, ins)
+    finally:
+        torch.cuda.current_device = before
