@@ -75,7 +75,7 @@ template <typename T> struct scan_rows_out { T *dX, *ddt, *dgate; };
 // its share of B and C, which then lie in LDS as [row][B, C][group of the wave][state], zeros behind the last row and state (in LDS rather
 // than in scalar registers, for which a row's work is too short to hide the loads of the next row's). With more than 16 states
 // the weights come when they are needed.
-template <typename T, int LG> struct scan_raw {
+template <typename T, int LG, bool GATED> struct scan_raw {
     typedef typename acc_of<T>::type A;
     static constexpr int R = SCAN_CHUNK, GW = 64 / LG, WIDTH = 2 * GW * 16, NW = R * WIDTH / 64;
     T x[R], d[R], e[R], g[R];
@@ -95,7 +95,7 @@ template <typename T, int LG> struct scan_raw {
             dp += more ? p.lddt : 0;
             ep += more ? bp.lddy : 0;
         }
-        if (in.gate) {
+        if constexpr (GATED) {
             const T* gp = in.gate + row0 * p.ldg;
 #pragma unroll
             for (int i = 0; i < R; ++i) {
@@ -139,17 +139,16 @@ template <typename T> __device__ __forceinline__ unsigned weights_pad(unsigned S
 // ag: the gradient that the rows behind send to the chunk's last state, da: dA so far, both [state / 4][lane]; st: two values per
 // row and lane that are needed again at the end (the slope of the step; dY times the gate's derivative); bc: the weights (scan_raw). raw: this
 // chunk's values, and on return those of the one in front of it, which starts `ahead` rows earlier (0: there is none).
-template <typename T, int LG>
+template <typename T, int LG, bool GATED>
 __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan_bshape& bp, const scan_lane& l, unsigned lane, unsigned nrow, size_t row0,
                                                  const scan_rows_in<T>& in, const typename acc_of<T>::type* A_, typename acc_of<T>::type skip,
                                                  typename acc_of<T>::type bias, const typename acc_of<T>::type* before,
                                                  quad<typename acc_of<T>::type>* ag, quad<typename acc_of<T>::type>* da, typename acc_of<T>::type* st,
-                                                 typename acc_of<T>::type* bc, scan_raw<T, LG>& raw, unsigned ahead, const scan_rows_out<T>& to,
+                                                 typename acc_of<T>::type* bc, scan_raw<T, LG, GATED>& raw, unsigned ahead, const scan_rows_out<T>& to,
                                                  scan_out<typename acc_of<T>::type> out, typename acc_of<T>::type& dskip, typename acc_of<T>::type& dbias)
 {
     typedef typename acc_of<T>::type A;
     constexpr int R = SCAN_CHUNK;
-    const bool gated = in.gate != nullptr;
     const unsigned place = opaque(l.ch * (unsigned)sizeof(T)), place_a = opaque(l.ch * (unsigned)sizeof(A));
     // what the next four states start from is fetched while these are worked on
     quad<A> kn, hn;
@@ -187,9 +186,9 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
             d[i] = here ? d[i] : A(0);
             e[i] = here && l.active ? (A)raw.e[i] : A(0);
             sB[i] = sA[i] = A(0);
-            y[i] = skip * x[i];
+            if (GATED) y[i] = skip * x[i];
         }
-        if (gated) {
+        if constexpr (GATED) {
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const A g = (A)raw.g[i], s = sigmoid_of(g);
@@ -244,7 +243,7 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const A a = exp2_fast(d[i] * k.v[j]), now = fma_a(ci.v[j], e[i], g.v[j]), w = now * (a * h[i][j]);
-                y[i] = fma_a(ci.v[j], h[i + 1][j], y[i]);
+                if (GATED) y[i] = fma_a(ci.v[j], h[i + 1][j], y[i]);
                 v[j] = now * dx;
                 v[4 + j] = e[i] * h[i + 1][j];
                 sB[i] = fma_a(bi.v[j], now, sB[i]);
@@ -304,7 +303,7 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
         if (l.active) {
             lane_store(xp, place, (T)fma_a(d[i], sB[i], skip * e[i]));
             lane_store(dp, place, (T)dd);
-            if (gated) lane_store(gp, place, (T)(y[i] * st[(R + i) * 64u + lane]));
+            if constexpr (GATED) lane_store(gp, place, (T)(y[i] * st[(R + i) * 64u + lane]));
         }
         xp += bp.lddx;
         dp += bp.ldddt;
@@ -313,7 +312,7 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
 }
 
 // A wave's place in LDS and what it adds up over all its rows.
-template <typename T, int LG> struct scan_wave {
+template <typename T, int LG, bool GATED> struct scan_wave {
     typedef typename acc_of<T>::type A;
     unsigned lane;
     scan_lane l;
@@ -340,12 +339,12 @@ template <typename T, int LG> struct scan_wave {
                                          const scan_rows_out<T>& to, const scan_out<A>& out)
     {
         if (!n) return;
-        scan_raw<T, LG> raw;
+        scan_raw<T, LG, GATED> raw;
         unsigned c = (n - 1u) / SCAN_CHUNK;
         raw.fetch(p, bp, l, lane, n - c * SCAN_CHUNK, from + c * SCAN_CHUNK, in);
         for (;;) {
             const unsigned at = from + c * SCAN_CHUNK, chunk = (at - start) / SCAN_CHUNK;
-            scan_chunk_bprop<T, LG>(p, bp, l, lane, min(SCAN_CHUNK, n - c * SCAN_CHUNK), at, in, A_, sk, bi, chunk ? kept_at(p, in.keep, start, chunk) : (const A*)nullptr,
+            scan_chunk_bprop<T, LG, GATED>(p, bp, l, lane, min(SCAN_CHUNK, n - c * SCAN_CHUNK), at, in, A_, sk, bi, chunk ? kept_at(p, in.keep, start, chunk) : (const A*)nullptr,
                                     ag, da, st, bc, raw, c ? SCAN_CHUNK : 0u, to, out, dskip, dbias);
             if (c-- == 0) break;
         }
@@ -372,7 +371,7 @@ template <int LG, typename A> __device__ __forceinline__ scan_out<A> tile_share(
 // A wave per tile of channels takes its share of the regions one after another, with dA in LDS, and leaves one block of sums:
 // part[unit][S + 2][D]. Of a region that is cut it takes the last segment, behind which nothing sends anything. Units from unit0 on
 // take the other segments: the slot of segment k stands for segment k - 1, to which segment k sends what lies in the slot's carry.
-template <typename T, int LG>
+template <typename T, int LG, bool GATED>
 __global__ __launch_bounds__(64, sizeof(T) == 8 ? 1 : 2) void k_scan_bprop(scan_shape p, scan_bshape bp, unsigned unit0, unsigned nslot, scan_rows_in<T> in,
                                                       const typename acc_of<T>::type* __restrict__ A_, const typename acc_of<T>::type* __restrict__ skip,
                                                       const typename acc_of<T>::type* __restrict__ bias, scan_rows_out<T> to,
@@ -381,7 +380,7 @@ __global__ __launch_bounds__(64, sizeof(T) == 8 ? 1 : 2) void k_scan_bprop(scan_
 {
     typedef typename acc_of<T>::type A;
     extern __shared__ char lds_raw[];
-    scan_wave<T, LG> w(p, lds_raw, A_, skip, bias);
+    scan_wave<T, LG, GATED> w(p, lds_raw, A_, skip, bias);
     out = tile_share<LG>(p, out, tile_stride);
     const bool slots = blockIdx.x >= unit0;
     const unsigned step = slots ? gridDim.x - unit0 : unit0, stop = slots ? nslot : p.nregion;
@@ -590,8 +589,12 @@ int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* a, void* 
                 k_scan_carry_back<A><<<dim3((unsigned)a->nregion, carry_blocks(*a)), 256, 0, st>>>(s, a->regions, (const A*)a->A, (const A*)y.seg.local,
                                                                                                   (const A*)y.seg.steps, (A*)y.seg.carry);
             }
-            k_scan_bprop<T, lanes.value><<<dim3(y.units + y.slot_units, p.tiles), 64, lds, st>>>(s, b, y.units, p.slots, in, (const A*)a->A, (const A*)a->skip,
-                                                                                                (const A*)a->dt_bias, to, out, tile_stride, (A*)part, (const A*)y.seg.carry);
+            auto main = [&](auto gated) {
+                k_scan_bprop<T, lanes.value, gated.value><<<dim3(y.units + y.slot_units, p.tiles), 64, lds, st>>>(
+                    s, b, y.units, p.slots, in, (const A*)a->A, (const A*)a->skip, (const A*)a->dt_bias, to, out, tile_stride, (A*)part, (const A*)y.seg.carry);
+            };
+            if (a->gate) main(std::true_type());
+            else main(std::false_type());
         });
         if (shared)
             k_scan_weights<A><<<dim3((unsigned)a->nregion + p.slots, divup((size_t)p.seg * 2 * ncol, 1024)), 256, 0, st>>>(s, a->regions, y.seg.marks, p.tpg, ncol, share, tile_stride, (A*)a->dB, a->lddb, (A*)a->dC,
