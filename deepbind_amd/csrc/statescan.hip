@@ -2,7 +2,7 @@
 //
 // Bound by the vector unit: per row, channel and state one 2^x (8.3 clocks of a SIMD), two products and a sum over states (2.5 to 4 each), and a share of a
 // matrix instruction; per row and channel some forty more for softplus, gate and addresses. Measured: 191 thousand rows of 256 float channels
-// with 16 states 245 us (783 MB; memory alone would take 165), 37 thousand rows of 1024 in three long regions 306 us.
+// with 16 states 246 us (783 MB; memory alone would take 165), 37 thousand rows of 1024 in three long regions 302 us.
 #include "statescan.h"
 
 namespace dbk {

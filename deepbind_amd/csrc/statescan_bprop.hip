@@ -1,8 +1,9 @@
 // The scan's backward pass. Formulas and layout: statescan.h.
 //
-// Bound by the vector unit: 445 to 480 instructions per row and wave with 16 states, 332 of them the states' own (per state two 2^x, four products and sums to
+// Bound by the vector unit: 445 instructions per row and wave with 16 states, 332 of them the states' own (per state two 2^x, four products and sums to
 // form it again, ten on the way back, four for the sums over lanes). Eight rows are taken together because 16 would not fit the registers.
-// Measured: 15 thousand rows of 1024 bfloat16 channels in two long regions 417 us, 48 thousand rows of 24 models of 16 floats 486 us.
+// Measured: 15 thousand rows of 1024 bfloat16 channels in two long regions 278 us (and 113 for
+// what enters their segments), 48 thousand rows of 24 models of 16 floats, without a gate, 445 us (486 with the gated form).
 #include "statescan.h"
 
 namespace dbk {
