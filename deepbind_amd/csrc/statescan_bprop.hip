@@ -2,8 +2,8 @@
 //
 // Bound by the vector unit: 445 instructions per row and wave with 16 states, 332 of them the states' own (per state two 2^x, four products and sums to
 // form it again, ten on the way back, four for the sums over lanes). Eight rows are taken together because 16 would not fit the registers.
-// Measured: 15 thousand rows of 1024 bfloat16 channels in two long regions 278 us (and 113 for
-// what enters their segments), 48 thousand rows of 24 models of 16 floats, without a gate, 445 us (486 with the gated form).
+// Measured: 15 thousand rows of 1024 bfloat16 channels in two long regions 284 us (and 113 for
+// what enters their segments), 48 thousand rows of 24 models of 16 floats, without a gate, 452 us (40 more with the gated form).
 #include "statescan.h"
 
 namespace dbk {
@@ -237,7 +237,7 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
 #pragma unroll
         for (int i = R - 1; i >= 0; --i) {
             rows[i] = A(0);
-            if ((i & ~3) >= (int)nrow) continue;
+            if (i >= (int)nrow) continue;
             const quad<A> bi = *(const quad<A>*)(b + i * width), ci = *(const quad<A>*)(c + i * width);
             const A dx = d[i] * x[i];
             A v[8];

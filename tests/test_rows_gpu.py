@@ -556,3 +556,28 @@ def test_state_may_be_named_as_its_own_successor():
     h0 = torch.randn(3, 4, 8, device="cuda")
     h1, h2 = h0.clone(), h0.clone()
     assert torch.equal(ks.statescan_step(X, X, A, B, B, h1), ks.statescan_step(X, X, A, B, B, h2, into=h2)) and torch.equal(h1, h2) and not torch.equal(h0, h1)
+
+
+@pytest.mark.parametrize("kind", ["float32", "float64"])
+@pytest.mark.parametrize("gated", [False, True])
+def test_statescan_gradient_of_a_state_that_overflows_at_the_last_row(kind, gated):
+    """The last state enters the last row's value alone: the gradient of A holds no product with it and stays what it is, also
+    where rows are taken several at a time and the region ends among them."""
+    from deepbind_amd import kangaroo_smat as ks
+    t, v, R, N, rows = scan_inputs(kind, "ragged", 70, 1, 16, 0)
+    T = regions(R)
+    for s, e in ref.rows_of(R, N):
+        if e > s:
+            t["X"][e - 1, 3] = v["X"][e - 1, 3] = float("inf")
+    kw = dict(gate=t["gate"] if gated else None)
+    base = [t[n] for n in ("X", "dt", "A", "B", "C")]
+    keep = ks.kept_states(t["X"], t["A"])
+    ks.statescan(*base, T, keep=keep, **kw)
+    dA = ks.statescan_bprop(*base, T, keep, t["dY"], **kw)[2]
+    with np.errstate(invalid="ignore"):
+        (_, _, *grads), (_, _, *sizes) = ref.statescan(*[v[n] for n in ("X", "dt", "A", "B", "C")], R, np.zeros((1, 70)), v["gate"] if gated else None,
+                                                       np.zeros((1, 70)), True, dY=v["dY"])
+    assert np.isfinite(grads[2]).all()
+    longest = max(e - s for s, e in ref.rows_of(R, N))
+    # (the same roundings as in the other tests of the gradients)
+    check(dA, grads[2], sizes[2], 2 * (16 * (longest + 8) + 16) + 70 + len(rows), kind, "dA", stored=False)
