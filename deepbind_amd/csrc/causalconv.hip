@@ -345,7 +345,7 @@ int check_conv(int dtype, const void* X, size_t ldx, const void* W, size_t taps,
 {
     DBK_ROW_DTYPE_OK(dtype);
     DBK_CHECK(taps >= 1 && taps <= 4, "NotImplementedError: filters of 1 to 4 taps, got %zu", taps);
-    DBK_CHECK(N < (size_t(1) << 32) - 1 && D < (size_t(1) << 31) && nregion < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu channels, %zu regions)", N, D, nregion);
+    DBK_CHECK(N < (size_t(1) << 32) - 64 && D < (size_t(1) << 31) && nregion < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu channels, %zu regions)", N, D, nregion);
     DBK_CHECK(D <= size_t(65535) * 64 * 2, "ValueError: too many channels (%zu)", D);
     DBK_CHECK(nregion + N < (size_t(1) << 32) - 1, "ValueError: map too large (%zu rows, %zu regions)", N, nregion);
     DBK_CHECK(!N || !D || (X && W && Z), "ValueError: null matrix");
@@ -380,7 +380,7 @@ int dbk_causalconv(dbk_stream_t stream, int dtype, const void* X, size_t ldx, co
     DBK_CHECK(!nregion || regions, "ValueError: null regions");
     if (!D || !nregion) { clear_error(); return 0; }
     const conv_plan p = plan_conv(dtype, N, D, nregion);
-    DBK_CHECK(nregion + p.slots < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu regions)", N, nregion);
+    DBK_CHECK(grid_fits(nregion + p.slots, 256, p.tiles), "ValueError: map too large (%zu rows, %zu regions)", N, nregion);
     DBK_CHECK(!p.slots || (work && work_bytes >= (size_t)p.slots * 4), "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, (size_t)p.slots * 4);
     const conv_shape s = {(unsigned)N, (unsigned)D, (unsigned)nregion, p.seg, p.ct_log2, (unsigned)(silu != 0), ldx, ldz};
     hipStream_t st = as_stream(stream);
@@ -414,6 +414,7 @@ int dbk_causalconv_bprop(dbk_stream_t stream, int dtype, const void* X, size_t l
     if (int rc = dbk_causalconv_workspace(dtype, taps, N, D, nregion, 1, &need)) return rc;
     DBK_CHECK(work && work_bytes >= need, "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, need);
     const conv_plan p = plan_conv(dtype, N, D, nregion);
+    DBK_CHECK(grid_fits(nregion + p.slots, 256, p.tiles), "ValueError: map too large (%zu rows, %zu regions)", N, nregion);
     const conv_shape s = {(unsigned)N, (unsigned)D, (unsigned)nregion, p.seg, p.ct_log2, (unsigned)(silu != 0), ldx, lddx};
     if (p.slots) k_conv_mark<<<divup(nregion, 4), 256, 0, st>>>(s, regions, (uint32_t*)work);
     void* part = (char*)work + ((size_t)p.slots * 4 + 15) / 16 * 16;
@@ -437,6 +438,7 @@ int dbk_causalconv_step(dbk_stream_t stream, int dtype, const void* X, size_t ld
     if (!n || !D) { clear_error(); return 0; }
     const conv_shape s = {(unsigned)n, (unsigned)D, (unsigned)n, 0u, 0u, (unsigned)(silu != 0), ldx, ldz};
     const size_t vecs = (D + conv_width(dtype) - 1) / conv_width(dtype);
+    DBK_CHECK(grid_fits((n * vecs + 255) / 256, 256), "ValueError: too many sequences (%zu of %zu channels)", n, D);
     hipStream_t st = as_stream(stream);
     with_row_type(dtype, [&](auto t) {
         typedef decltype(t) T;

@@ -341,11 +341,11 @@ __global__ __launch_bounds__(256) void k_norm_wgrad_wide(norm_shape p, size_t ld
 // out[c] = sum over units of part[unit][c] in a fixed order: 16 columns x 64 groups of units per workgroup, each thread its
 // group's units one after another, the groups' sums through LDS.
 template <typename A>
-__global__ __launch_bounds__(1024) void k_sum_partials(const A* __restrict__ part, size_t units, size_t ncol, size_t n0, A* out0, size_t n1, A* out1, A* out2)
+__global__ __launch_bounds__(1024) void k_sum_partials(const A* __restrict__ part, size_t units, size_t first, size_t ncol, size_t n0, A* out0, size_t n1, A* out1, A* out2)
 {
     __shared__ A lds[64][17];
     const unsigned x = threadIdx.x & 15u, y = threadIdx.x >> 4;
-    const size_t c = (size_t)blockIdx.x * 16u + x;
+    const size_t c = first + (size_t)blockIdx.x * 16u + x;
     A s = 0;
     if (c < ncol)
 #pragma unroll 8
@@ -365,11 +365,14 @@ __global__ __launch_bounds__(1024) void k_sum_partials(const A* __restrict__ par
 int sum_partials(hipStream_t st, int dtype, const void* part, size_t units, size_t n0, void* out0, size_t n1, void* out1, size_t n2, void* out2)
 {
     const size_t ncol = n0 + n1 + n2;
-    if (!ncol) return 0;
-    if (dtype == DBK_F64)
-        k_sum_partials<double><<<divup(ncol, 16), 1024, 0, st>>>((const double*)part, units, ncol, n0, (double*)out0, n1, (double*)out1, (double*)out2);
-    else
-        k_sum_partials<float><<<divup(ncol, 16), 1024, 0, st>>>((const float*)part, units, ncol, n0, (float*)out0, n1, (float*)out1, (float*)out2);
+    constexpr size_t MOST = size_t(1) << 25;     // columns of a launch (grid_fits)
+    for (size_t first = 0; first < ncol; first += MOST) {
+        const unsigned wgs = divup(ncol - first < MOST ? ncol - first : MOST, 16);
+        if (dtype == DBK_F64)
+            k_sum_partials<double><<<wgs, 1024, 0, st>>>((const double*)part, units, first, ncol, n0, (double*)out0, n1, (double*)out1, (double*)out2);
+        else
+            k_sum_partials<float><<<wgs, 1024, 0, st>>>((const float*)part, units, first, ncol, n0, (float*)out0, n1, (float*)out1, (float*)out2);
+    }
     return 0;
 }
 
@@ -499,6 +502,8 @@ int dbk_layernorm_bprop(dbk_stream_t stream, int dtype, const void* X, size_t ld
     DBK_CHECK(n == 0 || (stats && dZ), "ValueError: null matrix");
     DBK_CHECK(n <= 1 || lddz >= m, "ValueError: row strides must be at least the number of columns");
     const bool weights = dgamma || dbeta;
+    const size_t per_wg = 256 * (dtype == DBK_F64 ? 2 : dtype == DBK_BF16 ? 8 : 4);       // columns of a workgroup of the wide form
+    DBK_CHECK(!weights || !n || plan_norm(dtype, n, m, group).lanes || grid_fits(1, 256, (group + per_wg - 1) / per_wg), "ValueError: chunks too wide (%zu columns)", group);
     size_t need = 0;
     if (weights) if (int rc = dbk_layernorm_bprop_workspace(dtype, rows, m, group, &need)) return rc;
     DBK_CHECK(!need || (work && work_bytes >= need), "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, need);

@@ -5,6 +5,10 @@
 
 namespace dbk {
 
+// What one launch can hold: fewer than 2^32 threads along x (a launch of more runs without an error, and only what is over a multiple of
+// 2^32 of them: 2^24 + 64 workgroups of 256 gave 64), 65535 workgroups along y and z.
+inline bool grid_fits(size_t x, size_t threads, size_t y = 1, size_t z = 1) { return x < (size_t(1) << 32) / threads && y <= 65535u && z <= 65535u; }
+
 // Rows are kept as float, double or bfloat16; every sum, statistic and state is float (double for double rows).
 typedef __bf16 bf16_t;
 template <typename T> struct acc_of { typedef float type; };

@@ -271,7 +271,7 @@ int dbk_statescan(dbk_stream_t stream, const dbk_statescan_args* a, void* work, 
     const scan_plan p = plan_fprop(*a);
     const scan_segments g = segments_in(work, *a, p);
     DBK_CHECK(!g.bytes || (work && work_bytes >= g.bytes), "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, g.bytes);
-    DBK_CHECK(a->nregion + p.slots < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
+    DBK_CHECK(grid_fits(a->nregion + p.slots, 256), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
     const scan_shape s = shape_of(*a, p);
     hipStream_t st = as_stream(stream);
     const unsigned waves = p.tpg < 4 ? (p.tpg ? p.tpg : 1u) : 4u;
@@ -301,7 +301,7 @@ int dbk_statescan_step(dbk_stream_t stream, const dbk_statescan_args* a)
     if (int rc = check_scan(a)) return rc;
     DBK_CHECK(!a->N || !a->D || (a->Y && a->state && a->last), "ValueError: null matrix or state");
     DBK_CHECK(a->N <= 1 || a->ldy >= a->D, "ValueError: row strides must be at least the number of columns");
-    DBK_CHECK(a->N < (size_t(1) << 31), "ValueError: too many sequences (%zu)", a->N);
+    DBK_CHECK(grid_fits(a->N, 256), "ValueError: too many sequences (%zu)", a->N);
     if (!a->N || !a->D) { clear_error(); return 0; }
     const scan_shape s = shape_of(*a, plan_scan(0, a->D, a->G, 1, 2, 1));
     hipStream_t st = as_stream(stream);

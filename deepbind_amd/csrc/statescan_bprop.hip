@@ -564,7 +564,8 @@ int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* a, void* 
     const scan_plan p = plan_bprop(*a);
     const bprop_layout y = layout_of(work, *a, p);
     DBK_CHECK(work && work_bytes >= y.bytes, "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, y.bytes);
-    DBK_CHECK(a->nregion + p.slots < (size_t(1) << 31), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
+    DBK_CHECK(grid_fits(a->nregion + p.slots, 256, p.tpg > 1 ? ((size_t)p.seg * 2 * a->G * a->S + 1023) / 1024 : 1), "ValueError: map too large (%zu rows, %zu regions)",
+              a->N, a->nregion);
     const scan_shape s = shape_of(*a, p);
     const scan_bshape b = {a->lddy, a->lddx, a->ldddt, a->lddgate, a->lddb, a->lddc};
     const size_t ncol = a->G * a->S;

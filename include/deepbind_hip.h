@@ -479,7 +479,8 @@ int dbk_gather_maps(dbk_stream_t stream, int dtype, const uint32_t* regions, siz
  * are contiguous. regions: (nregion, 2) row ranges in any order, which must not overlap; bounds are cut at N, and a range that
  * ends before it starts is empty. Rows in no region are not read, and left as they are in outputs. Outputs must not share memory
  * with inputs. Results do not depend on the order in which workgroups run. `work`: caller-owned device memory of at least the bytes that the call's
- * _workspace function names, 16-byte aligned, in any state; calls that overlap must not share it. */
+ * _workspace function names, 16-byte aligned, in any state; calls that overlap must not share it. A call takes fewer than 2^24 regions
+ * (with the segments that long ones are cut into) or sequences: more would be over what one launch holds, and are refused. */
 
 /* Z = c * gamma / sqrt(mean(c^2) + eps) + beta with c = X - mean(X), means over every chunk of `group` consecutive columns of each of the n
  * rows (m columns; group divides m, as in dbk_softmax). gamma, beta: (m), may be NULL (ones, zeros). stats (may be NULL): (2, n * m / group),

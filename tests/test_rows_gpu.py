@@ -581,3 +581,33 @@ def test_statescan_gradient_of_a_state_that_overflows_at_the_last_row(kind, gate
     longest = max(e - s for s, e in ref.rows_of(R, N))
     # (the same roundings as in the other tests of the gradients)
     check(dA, grads[2], sizes[2], 2 * (16 * (longest + 8) + 16) + 70 + len(rows), kind, "dA", stored=False)
+
+
+def test_as_many_sequences_as_a_launch_takes():
+    """Single rows of nearly 2^24 sequences, each against its own formula (one channel, one state: a few roundings, k = 16 as elsewhere)."""
+    from deepbind_amd import kangaroo_smat as ks
+    n = (1 << 24) - 4096
+    g = torch.Generator(device="cuda").manual_seed(3)
+    f = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    X, dt, B, C, A, state, W = f(n, 1), f(n, 1).abs(), f(n, 1), f(n, 1), -f(1, 1).abs(), f(n, 1, 1), f(2, 1)
+    i = torch.arange(n, dtype=torch.int64)
+    R = torch.stack([i, i + 1], 1).to(torch.uint32).cuda()
+    x, d, b, c, a, w = (v.double() for v in (X, dt, B, C, A, W))
+
+    def near(got, want, size):
+        return bool(((got.double() - want).abs() <= 16 * 2.0 ** -24 * size + 1e-35).all())
+
+    h = torch.exp(d * a)
+    for s in (state, None):
+        before = 0 if s is None else s.double().view(n, 1)
+        now, size = h * before + d * x * b, h * (1 + (d * a).abs()) * abs(before) + (d * x * b).abs()
+        Y = ks.statescan(X, dt, A, B, C, R, softplus=False)[0] if s is None else ks.statescan_step(X, dt, A, B, C, s, softplus=False, into=torch.empty_like(s))
+        assert near(Y, c * now, c.abs() * size)
+    assert near(ks.causalconv(X, W, None, R, silu=False)[0], x * w[1], (x * w[1]).abs())
+    last = state.clone()
+    Z = ks.causalconv_step(X, W, None, last, silu=False)
+    assert near(Z, x * w[1] + state.double().view(n, 1) * w[0], (x * w[1]).abs() + (state.double().view(n, 1) * w[0]).abs()) and torch.equal(last.view(n, 1), X)
+    dX, dW, _ = ks.causalconv_bprop(X, W, None, R, dt, silu=False)
+    assert near(dX, d * w[1], (d * w[1]).abs()) and not bool(dW[0].any())
+    # (each of 2048 workgroups adds 8192 products one after another, at most: n roundings bound it)
+    assert abs(float(dW[1]) - float((d * x).sum())) <= 16384 * 2.0 ** -24 * float((d * x).abs().sum())

@@ -240,3 +240,26 @@ def test_outputs_that_share_memory_are_told_apart():
             assert shared(outs, ins)
     finally:
         torch.cuda.current_device = before
+
+
+def test_calls_beyond_one_launch_are_refused():
+    """A launch holds fewer than 2^32 threads: 2^24 workgroups of 256 are one too many, and would run none of them without a word."""
+    from deepbind_amd import _lib
+    lib = _lib.dll()
+    one = ctypes.c_void_p(16)
+    err = lambda: lib.dbk_last_error().decode()  # noqa: E731
+    n = 1 << 24
+    assert lib.dbk_causalconv(None, 0, one, 1, one, None, 2, n, 1, one, n, 1, None, one, 1, None, one, 1 << 40) and "map too large" in err()
+    assert lib.dbk_causalconv_bprop(None, 0, one, 1, one, None, 2, n, 1, one, n, 1, one, 1, one, 1, one, None, one, 1 << 40) and "map too large" in err()
+    assert lib.dbk_causalconv(None, 0, one, 1, one, None, 2, (1 << 32) - 3, 1, one, 1, 1, None, one, 1, None, one, 1 << 40) and "map too large" in err()
+    assert lib.dbk_causalconv_step(None, 0, one, 1 << 12, one, None, 2, 1 << 22, 1 << 12, 1, one, one, one, 1 << 12) and "too many sequences" in err()
+    a = _lib.StateScanArgs()
+    at = ctypes.addressof(a)
+    a.N, a.D, a.S, a.G, a.nregion = n, 1, 1, 1, n
+    a.A = a.X = a.dt = a.B = a.C = a.regions = a.Y = a.dA = a.dY = a.dX = a.ddt = a.dB = a.dC = a.keep = 16
+    a.ldx = a.lddt = a.ldb = a.ldc = a.ldy = a.lddy = a.lddx = a.ldddt = a.lddb = a.lddc = 1
+    assert lib.dbk_statescan(None, at, one, 1 << 40) and "map too large" in err()
+    assert lib.dbk_statescan_bprop(None, at, one, 1 << 40) and "map too large" in err()
+    a.keep, a.state, a.last = None, 16, 16
+    assert lib.dbk_statescan_step(None, at) and "too many sequences" in err()
+    assert lib.dbk_layernorm_bprop(None, 0, one, 1 << 27, one, one, one, 1 << 27, 1, 1 << 27, 1 << 27, one, 1 << 27, one, one, one, 1 << 40) and "too wide" in err()
