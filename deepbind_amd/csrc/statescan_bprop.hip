@@ -563,9 +563,8 @@ int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* a, void* 
     }
     const scan_plan p = plan_bprop(*a);
     const bprop_layout y = layout_of(work, *a, p);
+    DBK_CHECK(grid_fits(a->nregion + p.slots, 256), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
     DBK_CHECK(work && work_bytes >= y.bytes, "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, y.bytes);
-    DBK_CHECK(grid_fits(a->nregion + p.slots, 256, p.tpg > 1 ? ((size_t)p.seg * 2 * a->G * a->S + 1023) / 1024 : 1), "ValueError: map too large (%zu rows, %zu regions)",
-              a->N, a->nregion);
     const scan_shape s = shape_of(*a, p);
     const scan_bshape b = {a->lddy, a->lddx, a->ldddt, a->lddgate, a->lddb, a->lddc};
     const size_t ncol = a->G * a->S;
@@ -598,9 +597,11 @@ int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* a, void* 
             if (a->gate) main(std::true_type());
             else main(std::false_type());
         });
-        if (shared)
-            k_scan_weights<A><<<dim3((unsigned)a->nregion + p.slots, divup((size_t)p.seg * 2 * ncol, 1024)), 256, 0, st>>>(s, a->regions, y.seg.marks, p.tpg, ncol, share, tile_stride, (A*)a->dB, a->lddb, (A*)a->dC,
-                                                                              a->lddc);
+        if (shared) {
+            const size_t wgs = ((size_t)p.seg * 2 * ncol + 1023) / 1024;       // per region or segment: four values a thread, more where a launch takes no more
+            k_scan_weights<A><<<dim3((unsigned)a->nregion + p.slots, (unsigned)(wgs < 65535u ? wgs : 65535u)), 256, 0, st>>>(
+                s, a->regions, y.seg.marks, p.tpg, ncol, share, tile_stride, (A*)a->dB, a->lddb, (A*)a->dC, a->lddc);
+        }
     });
     sum_partials(st, a->dtype, part, y.units + y.slot_units, a->S * a->D, a->dA, a->D, a->dskip, a->D, a->ddt_bias);
     DBK_LAUNCH_OK();

@@ -263,3 +263,18 @@ def test_calls_beyond_one_launch_are_refused():
     a.keep, a.state, a.last = None, 16, 16
     assert lib.dbk_statescan_step(None, at) and "too many sequences" in err()
     assert lib.dbk_layernorm_bprop(None, 0, one, 1 << 27, one, one, one, 1 << 27, 1, 1 << 27, 1 << 27, one, 1 << 27, one, one, one, 1 << 40) and "too wide" in err()
+
+
+def test_backward_scans_of_many_wide_groups_are_taken():
+    """A call within the limits named for regions and channels is not refused for what its groups' gradients come to: it gets as far as its workspace."""
+    from deepbind_amd import _lib
+    lib = _lib.dll()
+    a = _lib.StateScanArgs()
+    at = ctypes.addressof(a)
+    a.A = a.X = a.dt = a.B = a.C = a.regions = a.Y = a.dA = a.dY = a.dX = a.ddt = a.dB = a.dC = a.keep = 16
+    for dtype, N, D, S, G in ((_lib.DBK_BF16, 10 ** 6, 8192, 16, 64), (_lib.DBK_BF16, 10 ** 6, 2080, 64, 32), (_lib.DBK_F32, 520, 66560, 64, 1024)):
+        a.dtype, a.N, a.D, a.S, a.G, a.nregion = dtype, N, D, S, G, 5
+        a.ldx = a.lddt = a.ldy = a.lddy = a.lddx = a.ldddt = D
+        a.ldb = a.ldc = a.lddb = a.lddc = G * S
+        assert lib.dbk_statescan_bprop(None, at, None, 0)
+        assert "workspace has 0 bytes" in lib.dbk_last_error().decode()

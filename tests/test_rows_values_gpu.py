@@ -96,3 +96,29 @@ def test_statescan_of_long_regions_is_as_near_as_the_decays_remember(kind, D, G,
     v = values(rng, 9010, len(R), D, G, S)
     v["A"] = -np.exp(1.5 * np.log(-v["A"]))      # some forget in a row, some remember a thousand
     scan(kind, v, R, 9010, "long", segment=32)
+
+
+def test_statescan_gradient_of_very_many_groups():
+    """1024 groups of 65 channels and 64 states: a region's dB and dC are more than the workgroups of one launch take 1024 of each."""
+    from deepbind_amd import kangaroo_smat as ks
+    G, gs, S, N = 1024, 65, 64, 520
+    D = G * gs
+    g = torch.Generator(device="cuda").manual_seed(5)
+    f = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    X, dt, dY, A, B, C = f(N, D), f(N, D), f(N, D), -f(S, D).abs(), f(N, G * S), f(N, G * S)
+    T = regions([[i * 104, i * 104 + 104] for i in range(5)])                   # (short enough not to be cut, in either call)
+    keep = ks.kept_states(X, A)
+    Y, _ = ks.statescan(X, dt, A, B, C, T, keep=keep)
+    got = ks.statescan_bprop(X, dt, A, B, C, T, keep, dY)
+    for i in (0, 517, G - 1):
+        c, w = slice(i * gs, (i + 1) * gs), slice(i * S, (i + 1) * S)
+        one = [X[:, c], dt[:, c], A[:, c].contiguous(), B[:, w], C[:, w]]
+        k1 = ks.kept_states(one[0], one[2])
+        y1, _ = ks.statescan(*one, T, keep=k1)
+        want = ks.statescan_bprop(*one, T, k1, dY[:, c])
+        assert torch.equal(Y[:, c], y1)
+        for name, a, b in zip(NAMES, got, want):
+            if b is not None:
+                near = a[:, w] if name in ("dB", "dC") else a[:, c]
+                # (dA is added over another number of workgroups; the rest are the same operations)
+                assert torch.equal(near, b) if name != "dA" else float((near - b).abs().max()) <= 1e-5 * float(b.abs().max()), (i, name)
