@@ -52,6 +52,16 @@ template <int LANES, typename A> __device__ __forceinline__ void lanes_sum2(A& u
     }
 }
 
+// A chunk's mean and reciprocal deviation from its sum's mean `near`, the mean of the squared distances to that and the mean of the distances. The sum's
+// roundings make `near` miss the mean by a few units in its last place, which is all there is where the values are equal, and more than their
+// spread where they lie far from zero: the distances, of the spread's size, say by how much.
+template <typename A> __device__ __forceinline__ void norm_stats(A near, A sq, A rest, A eps, A& mean, A& rstd)
+{
+    const A var = fma(-rest, rest, sq);
+    mean = near + rest;
+    rstd = A(1) / sqrt((var < A(0) ? A(0) : var) + eps);        // (a NaN stays)
+}
+
 // A row's values come while the row before it is worked on, and stay as they lie in memory: for bfloat16 half the registers of what is
 // computed from them, which is computed twice instead.
 template <typename T, int LANES, int NV, bool EXACT>
@@ -61,7 +71,7 @@ __global__ __launch_bounds__(256) void k_norm_fprop(norm_shape p, const T* __res
 {
     typedef typename acc_of<T>::type A;
     constexpr int V = row_vec<T>::N;
-    __shared__ A lds[4];
+    __shared__ A lds[8];
     const unsigned unit = threadIdx.x / LANES, lane = threadIdx.x % LANES;
     const unsigned chunk = (blockIdx.y << p.ct_log2) + (unit & ((1u << p.ct_log2) - 1u));
     const unsigned first = blockIdx.x * (256u / LANES) >> p.ct_log2;
@@ -98,16 +108,19 @@ __global__ __launch_bounds__(256) void k_norm_fprop(norm_shape p, const T* __res
         }
         row += p.rstep;
         fetch();
-        const A mean = lanes_sum<LANES>(sum, lds) * inv;
-        A sq = 0;
+        const A near = lanes_sum<LANES>(sum, lds) * inv;
+        A sq = 0, rest = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const A c = (EXACT ? valid[i] != 0 : j < (int)valid[i]) ? x[i][j] - mean : A(0);
+                const A c = (EXACT ? valid[i] != 0 : j < (int)valid[i]) ? x[i][j] - near : A(0);
                 sq = fma(c, c, sq);
+                rest += c;
             }
-        const A rstd = A(1) / sqrt(lanes_sum<LANES>(sq, lds) * inv + eps);
+        lanes_sum2<LANES>(sq, rest, lds);
+        A mean, rstd;
+        norm_stats(near, sq * inv, rest * inv, eps, mean, rstd);
         if (now >= p.n) continue;
         T* z = Z + (size_t)now * p.ldz + column;
 #pragma unroll
@@ -237,7 +250,7 @@ __global__ __launch_bounds__(256) void k_norm_fprop_wide(norm_shape p, const T* 
 {
     typedef typename acc_of<T>::type A;
     constexpr int V = row_vec<T>::N;
-    __shared__ A lds[4];
+    __shared__ A lds[8];
     const A inv = A(1) / (A)p.width;
     for (size_t u = blockIdx.x; u < (size_t)p.n * p.nchunk; u += gridDim.x) {
         const size_t row = u / p.nchunk, chunk = u % p.nchunk;
@@ -250,14 +263,16 @@ __global__ __launch_bounds__(256) void k_norm_fprop_wide(norm_shape p, const T* 
 #pragma unroll
             for (int j = 0; j < V; ++j) s += v.v[j];
         }
-        const A mean = lanes_sum<256>(s, lds) * inv;
-        s = 0;
+        const A near = lanes_sum<256>(s, lds) * inv;
+        A rest = s = 0;
         for (unsigned c = threadIdx.x * V; c < p.width; c += 256u * V) {
             v.load(x + c, p.width - c);
 #pragma unroll
-            for (int j = 0; j < V; ++j) { const A d = c + j < p.width ? v.v[j] - mean : A(0); s += d * d; }
+            for (int j = 0; j < V; ++j) { const A d = c + j < p.width ? v.v[j] - near : A(0); s += d * d; rest += d; }
         }
-        const A rstd = A(1) / sqrt(lanes_sum<256>(s, lds) * inv + eps);
+        lanes_sum2<256>(s, rest, lds);
+        A mean, rstd;
+        norm_stats(near, s * inv, rest * inv, eps, mean, rstd);
         for (unsigned c = threadIdx.x * V; c < p.width; c += 256u * V) {
             A g[V], b[V];
             v.load(x + c, p.width - c);

@@ -122,3 +122,61 @@ def test_statescan_gradient_of_very_many_groups():
                 near = a[:, w] if name in ("dB", "dC") else a[:, c]
                 # (dA is added over another number of workgroups; the rest are the same operations)
                 assert torch.equal(near, b) if name != "dA" else float((near - b).abs().max()) <= 1e-5 * float(b.abs().max()), (i, name)
+
+
+# ------------------------------------------------------------------------------------------------ layer norm
+def _depth(w, kind):
+    """The most roundings on a value's way through a chunk's sum: one thread's values (at most 16 in registers; from 256 threads' vectors on, where the
+    chunk is wider), then 256 threads in pairs."""
+    per = {"float32": 4, "float64": 2, "bfloat16": 8}[kind]
+    return max(4 * per, w // 256 + per) + 8
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("nchunk,w", [(1, 7), (5, 12), (3, 24), (1, 100), (2, 1440), (1, 20001), (9, 16)])
+def test_layernorm_of_rows_of_one_value(kind, nchunk, w):
+    """A chunk of identical values lies on its mean: its rows are beta, and the deviation is that of eps alone."""
+    from deepbind_amd import smat as sm
+    rng = np.random.default_rng([w, nchunk])
+    n, eps = 61, 1e-5
+    X, x = put(np.repeat(10 ** rng.uniform(-1, 5, (n, nchunk)) * rng.choice([-1, 1], (n, nchunk)), w, 1), TYPES[kind])
+    g, gv = put(1 + 0.3 * rng.standard_normal((1, nchunk * w)), wide(kind))
+    b, bv = put(0.3 * rng.standard_normal((1, nchunk * w)), wide(kind))
+    Z, stats = sm.layernorm(X, g, b, nchunk=nchunk, eps=eps, want_stats=True)
+    assert torch.equal(Z, b.to(TYPES[kind]).expand_as(Z))
+    assert torch.equal(stats[0].view(n, nchunk), X[:, ::w].to(wide(kind)))
+    # the first mean is off by e <= k u |x|; the mean of its squares less the square of their mean by (k + 4) u e^2 of eps
+    k = _depth(w, kind) + 2
+    e = k * U[kind] * np.abs(x[:, ::w])
+    r = host(stats[1].double()).reshape(n, nchunk)
+    assert (np.abs(r * np.sqrt(eps) - 1) <= 4 * U[kind] + (k + 4) * U[kind] * e * e / (2 * eps)).all()
+    dX, dg, db = sm.layernorm_bprop(X, g, stats, torch.ones_like(X), nchunk=nchunk)
+    assert not dg.any() and torch.equal(db, torch.full_like(db, n))
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("nchunk,w", [(1, 7), (5, 12), (4, 16), (3, 100), (1, 1440), (1, 20001)])
+@pytest.mark.parametrize("offset", [30.0, 1e4])
+def test_layernorm_of_rows_far_from_zero(kind, nchunk, w, offset):
+    from deepbind_amd import smat as sm
+    rng = np.random.default_rng([w, nchunk, int(offset)])
+    n, eps, u = 200 if w < 2000 else 20, 1e-5, U[kind]
+    X, x = put(rng.standard_normal((n, nchunk * w)) + offset * rng.choice([-1, 1], (n, 1)), TYPES[kind])
+    g, gv = put(1 + 0.3 * rng.standard_normal((1, nchunk * w)), wide(kind))
+    Z, stats = sm.layernorm(X, g, None, nchunk=nchunk, eps=eps, want_stats=True)
+    V = x.reshape(n, nchunk, w).astype(np.longdouble)        # (64 bits would round the mean as the kernel does)
+    mean = V.mean(2, keepdims=True)
+    c = V - mean
+    var = (c * c).mean(2, keepdims=True)
+    r = 1 / np.sqrt(var + eps)
+    # the first mean is off by e; the mean of what is left corrects it up to its own rounding, u |mean|, and that of a sum of numbers of the deviation's size
+    k = _depth(w, kind) + 4
+    e = k * u * np.abs(V).mean(2, keepdims=True)
+    spread = np.abs(c).mean(2, keepdims=True) + e
+    dmean = u * np.abs(mean) + k * u * spread
+    drel = 4 * u + (k + 4) * u * (var + 2 * e * e) / (2 * (var + eps))          # of the deviation's reciprocal
+    assert (np.abs(host(stats[0].double()).reshape(mean.shape) - mean) <= dmean).all()
+    assert (np.abs(host(stats[1].double()).reshape(mean.shape) / r - 1) <= drel).all()
+    bound = np.abs(gv) * (r * (dmean + u * np.abs(c)) + np.abs(c) * r * (drel + 2 * u)).reshape(n, -1)
+    want = (c * r).reshape(n, -1) * gv
+    assert (np.abs(host(Z.double()) - want) <= 1.01 * bound + STORED[kind] * (np.abs(want) + bound)).all()
