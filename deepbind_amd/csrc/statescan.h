@@ -55,6 +55,9 @@ template <typename T> __device__ __forceinline__ void lane_store(T* row, unsigne
 __device__ __forceinline__ float fma_a(float a, float b, float c) { return fmaf(a, b, c); }
 __device__ __forceinline__ double fma_a(double a, double b, double c) { return fma(a, b, c); }
 
+__device__ __forceinline__ float ldexp_a(float a, int e) { return ldexpf(a, e); }
+__device__ __forceinline__ double ldexp_a(double a, int e) { return ldexp(a, e); }
+
 template <typename A> __device__ __forceinline__ A step_of(const scan_shape& p, A raw, A& slope)
 {
     if (p.softplus) return softplus_of(raw, slope);
@@ -79,16 +82,21 @@ __device__ __forceinline__ void outer_add(float (&v)[4], float b, float x)
 template <int LG> __device__ __forceinline__ unsigned first_group(const scan_shape& p, unsigned tile) { return LG == 64 ? tile / p.tpg : tile * (64u / LG); }
 
 // Weights of two rows for a wave: fetched from memory into registers, a few per lane, put into LDS and read from there by the lanes of
-// each group: [row][B, C][group of the wave][state], zeros from state S on. They could come as scalar operands where a wave's
+// each group: [row][B, C][group of the wave][state]. They could come as scalar operands where a wave's
 // channels are of one group, but a scalar load can not run far enough ahead of the rows: there are not the registers.
+// From state S on, registers follow the last state that exists: the same decay, input and start. Where the states are summed (B and C both)
+// they share its output, by halves: with n of them, 1/2, 1/4, ... 2^-n and 2^-n once more, which scale its C exactly. (With weights of zero in
+// their place an infinite input would leave 0 * inf = NaN in them, and in every sum from then on.)
 constexpr int SCAN_AHEAD = 2;
 template <typename A, int LG, int NS, bool WITH_B, bool WITH_C> struct scan_weights {
     static constexpr bool MATRIX = WITH_B && sizeof(A) == 4;     // B for the matrix cores
+    static constexpr bool SHARES = WITH_B && WITH_C;
     static constexpr int GW = 64 / LG, PART = GW * NS, ROW = PART * (WITH_B + WITH_C), SIZE = SCAN_AHEAD * ROW, PER = (SIZE + 63) / 64;
     const A *from[PER];
     size_t step[PER];
     bool here[PER];
     unsigned to[PER];
+    int share[PER];                              // exponent of the share of C
     A next[PER];
     A *lds, *mine;
     unsigned lane;
@@ -101,9 +109,10 @@ template <typename A, int LG, int NS, bool WITH_B, bool WITH_C> struct scan_weig
             const unsigned at = lane + 64u * i, in = at % ROW, g = in % PART / NS, s = in % NS;
             const bool c = WITH_C && in >= (WITH_B ? PART : 0);
             const size_t ld = c ? p.ldc : p.ldb;
-            here[i] = at < SIZE && s < p.S && first + g < p.G;
+            here[i] = at < SIZE && first + g < p.G;
             to[i] = MATRIX && !c ? at - s + s % 4u * (NS / 4) + s / 4u : at;
-            from[i] = (c ? C : B) + (here[i] ? (first_row + at / ROW) * ld + (size_t)(first + g) * p.S + s : 0);
+            from[i] = (c ? C : B) + (here[i] ? (first_row + at / ROW) * ld + (size_t)(first + g) * p.S + min(s, p.S - 1u) : 0);
+            share[i] = c && s + 1u >= p.S ? -(int)min(s + 2u - p.S, (unsigned)NS - p.S) : 0;
             step[i] = back ? 0 - SCAN_AHEAD * ld : SCAN_AHEAD * ld;
         }
     }
@@ -119,7 +128,7 @@ template <typename A, int LG, int NS, bool WITH_B, bool WITH_C> struct scan_weig
     __device__ __forceinline__ void put()
     {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) if (SIZE % 64 == 0 || lane + 64u * i < SIZE) lds[to[i]] = next[i];
+        for (int i = 0; i < PER; ++i) if (SIZE % 64 == 0 || lane + 64u * i < SIZE) lds[to[i]] = SHARES ? ldexp_a(next[i], share[i]) : next[i];
         __builtin_amdgcn_wave_barrier();         // (one wave: LDS keeps its order)
     }
     __device__ __forceinline__ quad<A> b(int r, int q) const { return *(const quad<A>*)(mine + r * ROW + q); }
@@ -132,12 +141,12 @@ template <typename A, int LG, int NS, bool WITH_B, bool WITH_C> struct scan_weig
     __device__ __forceinline__ quad<A> c(int r, int q) const { return *(const quad<A>*)(mine + r * ROW + (WITH_B ? PART : 0) + q); }
 };
 
-// the states of a lane's channel between registers and (S, D) memory; null: zeros
+// the states of a lane's channel between registers and (S, D) memory; null: zeros; behind the last one, that one again
 template <typename A, int NS> __device__ __forceinline__ void regs_from(const scan_shape& p, const scan_lane& l, A (&h)[NS], const A* from, A scale)
 {
     const unsigned at = opaque(l.ch * (unsigned)sizeof(A));
 #pragma unroll
-    for (int j = 0; j < NS; ++j) h[j] = from && j < (int)p.S ? lane_load(from + (size_t)j * p.D, at) * scale : A(0);
+    for (int j = 0; j < NS; ++j) h[j] = from ? lane_load(from + (size_t)min((unsigned)j, p.S - 1u) * p.D, at) * scale : A(0);
 }
 template <typename A, int NS> __device__ __forceinline__ void regs_to(const scan_shape& p, const scan_lane& l, const A (&h)[NS], A* to)
 {

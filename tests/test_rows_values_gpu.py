@@ -180,3 +180,16 @@ def test_layernorm_of_rows_far_from_zero(kind, nchunk, w, offset):
     bound = np.abs(gv) * (r * (dmean + u * np.abs(c)) + np.abs(c) * r * (drel + 2 * u)).reshape(n, -1)
     want = (c * r).reshape(n, -1) * gv
     assert (np.abs(host(Z.double()) - want) <= 1.01 * bound + STORED[kind] * (np.abs(want) + bound)).all()
+@pytest.mark.parametrize("kind", ["float32", "float64"])
+@pytest.mark.parametrize("S", [1, 5, 16, 17, 33])
+@pytest.mark.parametrize("D,G", [(5, 1), (70, 1), (24, 2)])
+@pytest.mark.parametrize("one_sign", [False, True])
+def test_statescan_forward_of_an_infinite_input(kind, S, D, G, one_sign):
+    """A state takes an infinite input in and stays infinite; the row's other values, later rows' and other channels' are what the definition makes of it."""
+    rng = np.random.default_rng([S, D, G])
+    v = values(rng, 75, len(RAGGED), D, G, S)
+    v["A"] = np.maximum(v["A"], -3)              # (no decay underflows: 0 * inf would be another definition's)
+    if one_sign:                                 # (sums of infinities of both signs would be NaN in either way)
+        v["B"], v["C"], v["D"] = np.abs(v["B"]), np.abs(v["C"]), np.abs(v["D"])
+    v["X"][40, 3], v["X"][2, 0], v["X"][10, D - 1] = np.inf, -np.inf, np.inf
+    scan(kind, v, RAGGED, 75, "S=%d" % S, grads=False, state=True)
