@@ -100,9 +100,10 @@ template <typename A, int LG, int NS, bool WITH_B, bool WITH_C> struct scan_weig
     A next[PER];
     A *lds, *mine;
     unsigned lane;
+    bool shared;                                 // some registers follow the last state
     // B and C at row `first_row` of the rows; back: from there towards the rows in front
     __device__ __forceinline__ scan_weights(const scan_shape& p, unsigned lane_, unsigned first, const A* B, const A* C, A* lds_, unsigned first_row, bool back)
-        : lds(lds_), mine(lds_ + lane_ / LG * NS), lane(lane_ & 63u)
+        : lds(lds_), mine(lds_ + lane_ / LG * NS), lane(lane_ & 63u), shared(p.S < (unsigned)NS)
     {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -128,7 +129,10 @@ template <typename A, int LG, int NS, bool WITH_B, bool WITH_C> struct scan_weig
     __device__ __forceinline__ void put()
     {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) if (SIZE % 64 == 0 || lane + 64u * i < SIZE) lds[to[i]] = SHARES ? ldexp_a(next[i], share[i]) : next[i];
+        for (int i = 0; i < PER; ++i) {
+            if (SHARES && shared) next[i] = ldexp_a(next[i], share[i]);
+            if (SIZE % 64 == 0 || lane + 64u * i < SIZE) lds[to[i]] = next[i];
+        }
         __builtin_amdgcn_wave_barrier();         // (one wave: LDS keeps its order)
     }
     __device__ __forceinline__ quad<A> b(int r, int q) const { return *(const quad<A>*)(mine + r * ROW + q); }
