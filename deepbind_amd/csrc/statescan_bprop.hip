@@ -8,12 +8,20 @@
 
 namespace dbk {
 
+// States go through the kernel by fours. What is left over of the last four follows the last state: the same decay, input and start, and shares of its C and
+// of what is sent to it that add up to one exactly, so that all its gradients are shares too, and no 0 * inf arises where the state has none. Their sum
+// is the state's: for dX, ddt and the gate it is formed with the sum over states anyway.
+// The exponent of the share of state s, which exists or follows.
+__device__ __forceinline__ int share_exp(unsigned S, unsigned s) { return s + 1u < S ? 0 : -(int)min(s + 2u - S, (0u - S) & 3u); }
+
 template <typename A> __device__ __forceinline__ void states_to(const scan_shape& p, const scan_lane& l, unsigned lane, const quad<A>* h, A* to)
 {
     if (!l.active) return;
     const unsigned at = opaque(l.ch * (unsigned)sizeof(A));
     for (unsigned q = 0; 4u * q < p.S; ++q) {
-        const quad<A> s = h[q * 64u + lane];
+        quad<A> s = h[q * 64u + lane];
+#pragma unroll
+        for (int j = 3; j > 0; --j) if (4u * q + j >= p.S) s.v[j - 1] += s.v[j];
 #pragma unroll
         for (int j = 0; j < 4; ++j) if (4u * q + j < p.S) lane_store(to + (size_t)(4u * q + j) * p.D, at, s.v[j]);
     }
@@ -25,7 +33,7 @@ template <typename A> __device__ __forceinline__ void states_from(const scan_sha
     for (unsigned q = 0; 4u * q < p.S; ++q) {
         quad<A> s;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s.v[j] = from && 4u * q + j < p.S ? lane_load(from + (size_t)(4u * q + j) * p.D, at) : A(0);
+        for (int j = 0; j < 4; ++j) s.v[j] = from ? ldexp_a(lane_load(from + (size_t)min(4u * q + j, p.S - 1u) * p.D, at), share_exp(p.S, 4u * q + j)) : A(0);
         h[q * 64u + lane] = s;
     }
 }
@@ -73,7 +81,7 @@ template <typename T> struct scan_rows_in {      // what the backward pass reads
 template <typename T> struct scan_rows_out { T *dX, *ddt, *dgate; };
 
 // What a chunk of nrow <= 8 rows needs from memory, fetched into registers while the chunk behind it is worked on: the rows of its channels, and
-// its share of B and C, which then lie in LDS as [row][B, C][group of the wave][state], zeros behind the last row and state (in LDS rather
+// its share of B and C, which then lie in LDS as [row][B, C][group of the wave][state], zeros behind the last row (in LDS rather
 // than in scalar registers, for which a row's work is too short to hide the loads of the next row's). With more than 16 states
 // the weights come when they are needed.
 template <typename T, int LG, bool GATED> struct scan_raw {
@@ -110,8 +118,8 @@ template <typename T, int LG, bool GATED> struct scan_raw {
         for (int n = 0; n < NW; ++n) {
             const unsigned at = lane % 64u + 64u * n, in_row = at % WIDTH, r = at / WIDTH, gr = in_row % (GW * 16) / 16, s = in_row % 16u;
             const bool c = in_row >= GW * 16;
-            const A* from = (c ? in.C + row0 * p.ldc : in.B + row0 * p.ldb) + ((size_t)r * (c ? p.ldc : p.ldb) + (size_t)(first + gr) * p.S + s);
-            w[n] = s < p.S && first + gr < p.G && r < nrow ? *from : A(0);
+            const A* from = (c ? in.C + row0 * p.ldc : in.B + row0 * p.ldb) + ((size_t)r * (c ? p.ldc : p.ldb) + (size_t)(first + gr) * p.S + min(s, p.S - 1u));
+            w[n] = first + gr < p.G && r < nrow ? *from : A(0);
         }
     }
     __device__ __forceinline__ void put(const scan_shape& p, unsigned lane, unsigned nrow, size_t row0, const scan_rows_in<T>& in, A* bc) const
@@ -119,15 +127,23 @@ template <typename T, int LG, bool GATED> struct scan_raw {
         if (p.S <= 16u) {
 #pragma unroll
             for (int n = 0; n < NW; ++n) bc[lane + 64 * n] = w[n];
+            if (p.S % 4u) {
+#pragma unroll
+                for (int n = 0; n < NW; ++n) {
+                    const unsigned at = lane + 64u * n;
+                    if (at % WIDTH >= GW * 16) bc[at] = ldexp_a(w[n], share_exp(p.S, at % 16u));
+                }
+            }
         } else {
             const unsigned pad = (p.S + 3u) / 4u * 4u, width = 2u * GW * pad, first = first_group<LG>(p, blockIdx.y);
             for (unsigned i = lane; i < width; i += 64u) {
                 const unsigned gr = i / pad % GW, s = i % pad;
-                const bool c = i >= GW * pad, here = s < p.S && first + gr < p.G;
-                const A* from = (c ? in.C + row0 * p.ldc : in.B + row0 * p.ldb) + (size_t)(first + gr) * p.S + s;
+                const bool c = i >= GW * pad, here = first + gr < p.G;
+                const A* from = (c ? in.C + row0 * p.ldc : in.B + row0 * p.ldb) + (size_t)(first + gr) * p.S + min(s, p.S - 1u);
                 const size_t ld = c ? p.ldc : p.ldb;
+                const int share = c ? share_exp(p.S, s) : 0;
 #pragma unroll
-                for (unsigned r = 0; r < (unsigned)R; ++r) bc[r * width + i] = here && r < nrow ? from[r * ld] : A(0);
+                for (unsigned r = 0; r < (unsigned)R; ++r) bc[r * width + i] = here && r < nrow ? ldexp_a(from[r * ld], share) : A(0);
             }
         }
         __builtin_amdgcn_wave_barrier();         // (one wave: LDS keeps its order)
@@ -207,7 +223,6 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
         A h[R + 1][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            // (states that do not exist follow the last one: their weights and what is sent to them are zero, and so is all they add)
             k.v[j] *= A(1.4426950408889634);
             h[0][j] = hn.v[j];
         }
@@ -285,6 +300,16 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
         constexpr int LEFT = LG == 64 ? 1 : LG == 32 ? 2 : 4;                  // rows that a lane now holds
         const unsigned base = LG == 64 ? (lane & 1u) + ((lane >> 1) & 1u) * 2u + ((lane >> 2) & 1u) * 4u
                             : LG == 32 ? (lane & 1u) * 2u + ((lane >> 1) & 1u) * 4u : (lane & 1u) * 4u;
+        if (left < 4u) {                         // (the last state's dB is in shares)
+            constexpr int BIT1 = LG == 64 ? 16 : LG == 32 ? 8 : 4;
+#pragma unroll
+            for (int i = 0; i < LEFT; ++i) {
+                A all = state + 1u >= left ? rows[i] : A(0);
+                all += __shfl_xor(all, BIT1);
+                all += __shfl_xor(all, BIT1 / 2);
+                rows[i] = kind == 0u && state + 1u == left ? all : rows[i];
+            }
+        }
         // (lanes of a group that does not exist carry zeros into it and their first lane says so)
         if (state < left && (LG == 64 || l.active || (lane % LG >= p.gs && (lane / LG) + blockIdx.y * (64u / LG) < p.G))) {
             A* o = kind ? out.dC : out.dB;

@@ -193,3 +193,19 @@ def test_statescan_forward_of_an_infinite_input(kind, S, D, G, one_sign):
         v["B"], v["C"], v["D"] = np.abs(v["B"]), np.abs(v["C"]), np.abs(v["D"])
     v["X"][40, 3], v["X"][2, 0], v["X"][10, D - 1] = np.inf, -np.inf, np.inf
     scan(kind, v, RAGGED, 75, "S=%d" % S, grads=False, state=True)
+
+
+@pytest.mark.parametrize("kind", ["float32", "float64"])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("S", [1, 5, 16, 17])
+@pytest.mark.parametrize("one_sign", [False, True])
+def test_statescan_gradients_of_an_infinite_input(kind, gated, S, one_sign):
+    """Where the number of states is no multiple of four: those that do not exist add nothing, whatever the others hold."""
+    for name, worst in (("X", np.inf), ("dY", -np.inf)):
+        rng = np.random.default_rng([S, gated])
+        v = values(rng, 75, len(RAGGED), 64, 1, S, gated)
+        v["A"] = np.maximum(v["A"], -3)
+        if one_sign:
+            v["B"], v["C"], v["D"], v["dY"] = np.abs(v["B"]), np.abs(v["C"]), np.abs(v["D"]), np.abs(v["dY"])
+        v[name][40, 3], v[name][10, 7] = np.inf, worst
+        scan(kind, v, RAGGED, 75, "%s, S=%d" % (name, S))
