@@ -195,23 +195,21 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
                 st[i * 64u + lane] = A(1);
             }
         }
-        // rows behind the last one: no step, so nothing is taken in or sent
+        // rows behind the last one, and lanes without a channel, whose sums go into their group's: no step, so nothing is taken in or sent
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const bool here = i < (int)nrow;
+            const bool here = i < (int)nrow && l.active;
+            A ee = (A)raw.e[i];
+            if constexpr (GATED) {
+                const A g = (A)raw.g[i], s = sigmoid_of(g);
+                st[(R + i) * 64u + lane] = ee * s * fma_a(g, A(1) - s, A(1));
+                ee *= g * s;
+            }
             x[i] = here ? (A)raw.x[i] : A(0);
             d[i] = here ? d[i] : A(0);
-            e[i] = here && l.active ? (A)raw.e[i] : A(0);
+            e[i] = here ? ee : A(0);
             sB[i] = sA[i] = A(0);
             if (GATED) y[i] = skip * x[i];
-        }
-        if constexpr (GATED) {
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const A g = (A)raw.g[i], s = sigmoid_of(g);
-                st[(R + i) * 64u + lane] = e[i] * s * fma_a(g, A(1) - s, A(1));
-                e[i] *= g * s;
-            }
         }
     }
     if (ahead) raw.fetch(p, bp, l, lane, SCAN_CHUNK, row0 - ahead, in);
@@ -223,8 +221,8 @@ __device__ __forceinline__ void scan_chunk_bprop(const scan_shape& p, const scan
         A h[R + 1][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            k.v[j] *= A(1.4426950408889634);
-            h[0][j] = hn.v[j];
+            k.v[j] = l.active ? k.v[j] * A(1.4426950408889634) : A(0);
+            h[0][j] = l.active ? hn.v[j] : A(0);
         }
         if (left > 4u) fetch(q + 1u);
         const A *b = weights + 4u * q, *c = b + (64 / LG) * pad;
@@ -426,7 +424,7 @@ __global__ __launch_bounds__(64, sizeof(T) == 8 ? 1 : 2) void k_scan_bprop(scan_
             from = g.start + (in.marks && is_cut(p, g) ? (g.end - g.start - 1u) / p.seg * p.seg : 0u);
             n = g.end - from;
         }
-        // (a lane without a channel adds nothing to its group's sums: its e is zero, and so is what is sent to it)
+        // (a lane without a channel adds nothing to its group's sums: it has no steps, rows or states, and nothing is sent to it)
         states_from(p, w.l, w.lane, w.ag, w.l.active ? sent : (const A*)nullptr);
         w.rows(p, bp, g.start, from, n, in, to, out);
     }

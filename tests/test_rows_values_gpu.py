@@ -209,3 +209,15 @@ def test_statescan_gradients_of_an_infinite_input(kind, gated, S, one_sign):
             v["B"], v["C"], v["D"], v["dY"] = np.abs(v["B"]), np.abs(v["C"]), np.abs(v["D"]), np.abs(v["dY"])
         v[name][40, 3], v[name][10, 7] = np.inf, worst
         scan(kind, v, RAGGED, 75, "%s, S=%d" % (name, S))
+
+
+@pytest.mark.parametrize("kind", ["float32", "float64"])
+@pytest.mark.parametrize("name", ["X", "dt", "dY", "gate"])
+@pytest.mark.parametrize("D,G", [(5, 1), (70, 1), (24, 2), (40, 2)])
+def test_statescan_gradients_of_an_infinite_last_channel(kind, name, D, G):
+    """A group that does not fill its lanes: the lanes without a channel add nothing to the group's sums, whatever its last channel holds."""
+    rng = np.random.default_rng([D, G, ord(name[0])])
+    v = values(rng, 75, len(RAGGED), D, G, 16)
+    v["A"] = np.maximum(v["A"], -3)
+    v[name][12, D // G - 1], v[name][36, D - 1] = np.inf, np.inf
+    scan(kind, v, RAGGED, 75, name)
