@@ -256,6 +256,14 @@ __device__ __forceinline__ bool cut_segment(const scan_shape& p, const uint32_t*
 size_t bprop_work_bytes(const dbk_statescan_args& a);            // statescan_bprop.hip
 // One state's way through n segments: s = local + exp2(a2 * sum) s after each, written to out; the three pointers start at the first and move
 // on by `step` (sums by `sum_step`). U segments' values are on their way while U others are worked on.
+// The factor comes in two halves: it may overflow or underflow where the product, which rows would form step by step, does not. A half is kept to what
+// a normal number holds, so that nothing times the most growth is nothing, and an infinite state times the most decay still infinite. That changes growth
+// by more than 2^254 (float), which overflows from any normal number, and decay by more than 2^252, which leaves less than 2^-124 of any.
+template <typename A> __device__ __forceinline__ A half_power(A x)
+{
+    constexpr A up = sizeof(A) == 8 ? A(1023) : A(127), down = A(1) - up;
+    return exp2_fast(x > up ? up : x < down ? down : x);        // (a NaN stays)
+}
 template <typename A> __device__ __forceinline__ void carry_chain(A a2, A s, unsigned n, const A* local, const A* sums, A* out, size_t step, size_t sum_step)
 {
     constexpr unsigned U = 8;
@@ -274,12 +282,12 @@ template <typename A> __device__ __forceinline__ void carry_chain(A a2, A s, uns
     for (unsigned k = 0; k < n; k += U) {
         A av[U], sv[U];
 #pragma unroll
-        for (unsigned i = 0; i < U; ++i) { av[i] = add[i]; sv[i] = exp2_fast(a2 * sum[i]); }
+        for (unsigned i = 0; i < U; ++i) { av[i] = add[i]; sv[i] = half_power(A(0.5) * a2 * sum[i]); }
         if (k + U < n) fetch(n - k - U);
 #pragma unroll
         for (unsigned i = 0; i < U; ++i) {
             if (k + i >= n) break;
-            s = fma_a(sv[i], s, av[i]);
+            s = fma_a(sv[i], sv[i] * s, av[i]);
             *out = s;
             out += step;
         }

@@ -221,3 +221,50 @@ def test_statescan_gradients_of_an_infinite_last_channel(kind, name, D, G):
     v["A"] = np.maximum(v["A"], -3)
     v[name][12, D // G - 1], v[name][36, D - 1] = np.inf, np.inf
     scan(kind, v, RAGGED, 75, name)
+
+
+@pytest.mark.parametrize("kind", ["float32", "float64"])
+def test_statescan_whose_states_grow(kind):
+    """A > 0 and steps as they are, in a region that is cut: nothing carried on over a segment whose growth overflows stays nothing, something small
+    becomes what it becomes row by row."""
+    P, N, D, S = [[3, 400]], 405, 3, 5
+    rng = np.random.default_rng(8)
+
+    def case():
+        v = values(rng, N, 1, D, 1, S, gate=False)
+        v["A"], v["bias"] = 2 + rng.random((S, D)), None
+        return v
+
+    big = 8 if kind == "float64" else 1          # (2^1024 is eight times 2^128)
+    v = case()
+    v["dt"][:] = big
+    v["A"] *= 2                                  # e^(4 * 32) and more in a segment of 32 rows
+    v["X"][:393], v["dY"][8:] = 0, 0             # inputs in the last rows, gradients from the first
+    scan(kind, v, P, N, "zeros", soft=False, segment=32)
+    v = case()
+    v["dt"][:], v["A"][:] = 0, 4 * big
+    v["dt"][8], v["dt"][3 + 32:3 + 64] = 1, 1    # into the first segment, through the second
+    v["X"][:], v["X"][8] = 0, 1e-25 ** big * rng.standard_normal(D)
+    v["D"] *= 0
+    scan(kind, v, P, N, "small", soft=False, grads=False, segment=32)
+    v = case()
+    v["dt"][:], v["A"][:] = 0, 4 * big
+    v["dt"][8], v["dt"][3 + 32:3 + 64] = 1, 1
+    v["X"][:], v["dY"][:] = 0, 0
+    v["dY"][80] = 1e-25 ** big
+    scan(kind, v, P, N, "small gradient", soft=False, segment=32)
+
+
+@pytest.mark.parametrize("kind", ["float32", "float64"])
+@pytest.mark.parametrize("name", ["X", "dY"])
+def test_statescan_of_an_infinite_state_that_is_carried(kind, name):
+    """An infinite state stays infinite, also over segments whose decay underflows."""
+    rng = np.random.default_rng(12)
+    v = values(rng, 405, 1, 6, 1, 4)
+    v["A"] = -1 - 6 * rng.random((4, 6))
+    if kind == "float64":
+        v["A"] *= 4
+    v["dt"][:] = 2
+    v["bias"] = np.zeros((1, 6))
+    v[name][20 if name == "X" else 380, 2] = np.inf
+    scan(kind, v, [[3, 400]], 405, name, segment=32, only=("dX", "dB", "dC"))
