@@ -305,8 +305,10 @@ def _column_blocks(a, b):
     """Whether b, which starts no earlier than a, is another block of columns of the same matrix."""
     if a.dim() != 2 or b.dim() != 2 or a.stride(0) != b.stride(0) or a.element_size() != b.element_size():
         return False
-    off = (b.data_ptr() - a.data_ptr()) // a.element_size()
     ld = a.stride(0)
+    if ld < a.shape[1]:                          # (one row, whose stride says nothing)
+        return False
+    off = (b.data_ptr() - a.data_ptr()) // a.element_size()
     return off % ld >= a.shape[1] and off % ld + b.shape[1] <= ld
 
 

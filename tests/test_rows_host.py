@@ -278,3 +278,26 @@ def test_backward_scans_of_many_wide_groups_are_taken():
         a.ldb = a.ldc = a.lddb = a.lddc = G * S
         assert lib.dbk_statescan_bprop(None, at, None, 0)
         assert "workspace has 0 bytes" in lib.dbk_last_error().decode()
+
+
+def test_one_row_without_a_row_stride_shares_memory_with_itself():
+    """A matrix of one row is taken with any row stride, none among them."""
+    from deepbind_amd._lib import Arguments, DeepbindError
+    base = torch.zeros(12)
+    for a, b, same in ((base.as_strided((1, 6), (0, 1)), base.as_strided((1, 6), (0, 1)), True), (base.as_strided((1, 6), (0, 1)), base.as_strided((1, 6), (0, 1), 4), True),
+                       (base.as_strided((1, 6), (2, 1)), base.as_strided((1, 6), (2, 1), 2), True), (base.as_strided((1, 6), (0, 1)), base.as_strided((1, 6), (0, 1), 6), False)):
+        args = Arguments()
+        args.rows("a", a, a.shape, a.dtype)
+        args.rows("b", b, b.shape, b.dtype, out=True)
+        for group in (args.ins, args.outs):      # (as if they lay on the current device: there is none here)
+            group[:] = [(lo, hi, 0, t) for lo, hi, _, t in group]
+        before = torch.cuda.current_device
+        torch.cuda.current_device = lambda: 0
+        try:
+            if same:
+                with pytest.raises(DeepbindError, match="shares memory"):
+                    args.check()
+            else:
+                args.check()
+        finally:
+            torch.cuda.current_device = before
