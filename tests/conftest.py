@@ -18,6 +18,15 @@ def oracle():
     return deepbind_oracle
 
 
+@pytest.fixture(autouse=True)
+def no_error_text_left_behind():
+    """The library keeps the text of its last refusal; a call with nothing to do clears it, so that no test finds another's."""
+    yield
+    _lib = sys.modules.get("deepbind_amd._lib")
+    if _lib is not None and _lib._dll is not None:
+        _lib._dll.dbk_corr1ord(None, 0, None, 5, 16, None, 0, 4, None)
+
+
 def pytest_terminal_summary(terminalreporter):
     """Worst elementwise relative error per benchmark configuration, as recorded by the GPU parity tests."""
     try:

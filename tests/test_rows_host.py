@@ -301,3 +301,15 @@ def test_one_row_without_a_row_stride_shares_memory_with_itself():
                 args.check()
         finally:
             torch.cuda.current_device = before
+
+
+def test_refusals_of_other_tests_leave_no_error_text():
+    from deepbind_amd import _lib
+    assert _lib.dll().dbk_last_error() == b""
+    with pytest.raises(_lib.DeepbindError):
+        _lib.call("dbk_layernorm", None, 3, None, 0, None, None, 0, 8, 8, 1e-5, None, 8, None)
+
+
+def test_nor_does_the_one_before():
+    from deepbind_amd import _lib
+    assert _lib.dll().dbk_last_error() == b""
