@@ -5,8 +5,8 @@
 //
 // Bound by memory: x in and z out forward, x and dz in and dx out backward (p is formed again from x: reading it would cost a
 // third map, keeping it another). A lane owns four channels (two of double) and walks down a strip of rows with the last K - 1 of
-// them in registers, so that a row is read once but for the K - 1 rows above each strip, which the caches hold. Measured: 117 thousand
-// rows of 1024 bfloat16 83 us forward and 155 us backward (480 and 720 MB), 191 thousand rows of 256 floats 81 us (391 MB).
+// them in registers, so that a row is read once but for the K - 1 rows above each strip, which the caches hold. Measured: 106 502
+// rows of 1024 bfloat16 83 us forward and 152 us backward (436 and 654 MB), 193 495 rows of 256 floats 81 us (396 MB).
 #include <type_traits>
 #include "rows_common.h"
 

@@ -6,7 +6,8 @@
 //
 // Bound by memory: the forward pass reads x and writes z, the backward pass reads x and dz and writes dx; a chunk's values stay
 // in registers between the passes over them (mean, squares, result), so that each is read once. Measured: 130003 x 1440 bfloat16 forward
-// 150 us (749 MB), backward 238 us (1.12 GB); 50021 rows of 64 chunks of 16 floats 80 and 143 us (410 and 615 MB).
+// 151 us (749 MB), backward 239 us (1.12 GB); 50021 rows of 64 chunks of 16 floats 79 and 140 us (410 and 615 MB). Chunks too wide for the registers are
+// read three times either way, from the caches where they hold them: 5003 x 20001 floats 337 us forward, 900 both ways (0.8 and 1.6 GB).
 #include <type_traits>
 #include "rows_common.h"
 

@@ -116,7 +116,7 @@ template <typename A> __device__ __forceinline__ A sigmoid_of(A x) { return rcp_
 
 // softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|) in (0, 1]. log(1 + e) = 2 artanh(z), z = e / (2 + e) <= 1/3, by the series
 // z + z^3/3 + z^5/5 + ...: keeps the relative precision of small steps, which log(1 + e) itself loses (1 + e rounds), in a dozen
-// operations; the first term left out, z^17/17, is below 2^-30 of z. slope: the derivative, 1 / (1 + exp(-x)), from the same e.
+// operations; the first term left out, z^17/17, is at most 2^-29.4 of z. slope: the derivative, 1 / (1 + exp(-x)), from the same e.
 __device__ __forceinline__ float softplus_of(float x, float& slope)
 {
     const float e = exp_fast(-fabsf(x)), z = e * rcp_fast(2.0f + e), q = z * z, r = rcp_fast(1.0f + e);

@@ -173,7 +173,8 @@ struct scan_plan { int lanes; unsigned tpg, tiles, seg, cut, slots; };
 // A region is one wave's work, until it is so long that the others wait for it: then it is cut into segments. The segments' states are first
 // found from zeros (a second pass over the rows, with three more launches), carried over from segment to segment, and the rows
 // then written with the right states in front. The segment is an even share of all rows for `waves` waves, and a region is cut
-// from `shares` of them on, but never one of up to 128 rows, which a wave walks down in the time of the launches.
+// from `shares` of them on, but never one of up to 128 rows: 17 sequences of up to 77 double rows took 435 us both ways cut into segments of 32, 299 whole.
+// (One line for all types: a wave walks 77 rows of five double states in some 100 us, of floats in a fraction of that; the four launches take 20.)
 inline scan_plan plan_scan(size_t N, size_t D, size_t G, size_t waves, size_t shares, size_t least)
 {
     scan_plan p;

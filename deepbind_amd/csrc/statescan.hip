@@ -1,8 +1,10 @@
 // The scan's forward pass, for whole regions and for single rows. Formulas and layout: statescan.h.
 //
-// Bound by the vector unit: per row, channel and state one 2^x (8.3 clocks of a SIMD), two products and a sum over states (2.5 to 4 each), and a share of a
-// matrix instruction; per row and channel some forty more for softplus, gate and addresses. Measured: 191 thousand rows of 256 float channels
-// with 16 states 246 us (783 MB; memory alone would take 165), 37 thousand rows of 1024 in three long regions 302 us.
+// Work per row, channel and state: one 2^x (8.3 clocks of a SIMD), two products and a sum over states (2.5 to 4 each), and a share of a
+// matrix instruction; per row and channel some forty instructions more for softplus, gate and addresses. Measured: 193 495 rows of 256 float channels
+// with 16 states 248 us (817 MB; memory alone would take 172), 33 282 rows of 1024 bfloat16 in three long regions 124 + 165 us. That is 720 clocks of a SIMD
+// per row and wave, where the instructions alone come to some 430 at the rates above: a third of the waves' time is issue, a third waits for its
+// turn to issue, a third for memory and LDS.
 #include "statescan.h"
 
 namespace dbk {
@@ -91,6 +93,8 @@ __device__ __forceinline__ void scan_rows(const scan_shape& p, const scan_lane& 
     }
 }
 
+// Four waves per SIMD, which float and bfloat16 rows with up to 16 states need no more than 89 of 128 registers for. More states, and doubles from 8 registers of states
+// on, do not fit and spill: 2048 reads x 256 channels take 232 us with 16 float states, 556 with 32 and 3410 with 64, 2234 with 16 double ones.
 // Blocks below nregion: a region, all of it or its first segment (the state behind which is carried to the second one); the
 // others: what a segment makes of a zero state, where another one follows.
 template <typename T, int LG, int NS>
@@ -236,7 +240,7 @@ __global__ __launch_bounds__(256) void k_scan_step(scan_shape p, const T* __rest
 
 namespace {
 
-constexpr size_t SCAN_WAVES = 4096;              // waves that keep the vector units busy: four per SIMD (88 registers a lane allow five)
+constexpr size_t SCAN_WAVES = 4096;              // waves that keep the vector units busy: four per SIMD (81 to 89 registers a lane, 16 float states, allow five)
 constexpr size_t SCAN_LEAST = 32;                // rows of the shortest segment: its state's way through the carry costs as much as some ten rows
 
 scan_plan plan_fprop(const dbk_statescan_args& a) { return plan_scan(a.N, a.D, a.G, SCAN_WAVES, 4, SCAN_LEAST); }

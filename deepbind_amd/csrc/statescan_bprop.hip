@@ -1,9 +1,11 @@
 // The scan's backward pass. Formulas and layout: statescan.h.
 //
-// Bound by the vector unit: 445 instructions per row and wave with 16 states, 332 of them the states' own (per state two 2^x, four products and sums to
+// 459 vector instructions per row and wave with 16 states, 332 of them the states' own (per state two 2^x, four products and sums to
 // form it again, ten on the way back, four for the sums over lanes). Eight rows are taken together because 16 would not fit the registers.
-// Measured: 15 thousand rows of 1024 bfloat16 channels in two long regions 284 us (and 113 for
-// what enters their segments), 48 thousand rows of 24 models of 16 floats, without a gate, 452 us (40 more with the gated form).
+// Measured: 14 576 rows of 1024 bfloat16 channels in two long regions 290 us (and 104 for
+// what enters their segments), 47 678 rows of 24 models of 16 floats, without a gate, 463 us (40 more with the gated form). The first are 2840 clocks of a SIMD
+// per row and wave, where the instructions alone come to some 1490 at the rates measured one by one: two waves per SIMD issue 58 % of their time, wait for
+// memory and LDS 27 %, for their turn 15 %, and the chains of dependent sums over lanes and of 2^x are not filled by other rows' work.
 #include "statescan.h"
 
 namespace dbk {
