@@ -561,6 +561,16 @@ bprop_layout layout_of(void* work, const dbk_statescan_args& a, const scan_plan&
     return y;
 }
 
+// Workgroups per region or segment that add the tiles' shares, four values a thread: as many as a whole segment has work for where there are few of them, what the
+// average has where there are many, whose sum would otherwise be workgroups without work (20 thousand reads x 256 channels: 97 of 100, 11.9 ms a pass instead of 11.3).
+unsigned weights_blocks(const dbk_statescan_args& a, const scan_plan& p)
+{
+    const size_t per_row = 2 * a.G * a.S, items = a.nregion + p.slots, most = ((size_t)p.seg * per_row + 1023) / 1024;
+    const size_t average = a.N * per_row / items / 1024 + 1, room = 65536 / items + 1, want = average > room ? average : room;
+    const size_t wgs = want < most ? want : most;
+    return (unsigned)(wgs < 65535 ? wgs : 65535);
+}
+
 }  // namespace
 
 size_t bprop_work_bytes(const dbk_statescan_args& a) { return layout_of(nullptr, a, plan_bprop(a)).bytes; }
@@ -622,11 +632,9 @@ int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* a, void* 
             if (a->gate) main(std::true_type());
             else main(std::false_type());
         });
-        if (shared) {
-            const size_t wgs = ((size_t)p.seg * 2 * ncol + 1023) / 1024;       // per region or segment: four values a thread, more where a launch takes no more
-            k_scan_weights<A><<<dim3((unsigned)a->nregion + p.slots, (unsigned)(wgs < 65535u ? wgs : 65535u)), 256, 0, st>>>(
-                s, a->regions, y.seg.marks, p.tpg, ncol, share, tile_stride, (A*)a->dB, a->lddb, (A*)a->dC, a->lddc);
-        }
+        if (shared)
+            k_scan_weights<A><<<dim3((unsigned)a->nregion + p.slots, weights_blocks(*a, p)), 256, 0, st>>>(s, a->regions, y.seg.marks, p.tpg, ncol, share, tile_stride,
+                                                                                                      (A*)a->dB, a->lddb, (A*)a->dC, a->lddc);
     });
     sum_partials(st, a->dtype, part, y.units + y.slot_units, a->S * a->D, a->dA, a->D, a->dskip, a->D, a->ddt_bias);
     DBK_LAUNCH_OK();

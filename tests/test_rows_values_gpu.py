@@ -268,3 +268,13 @@ def test_statescan_of_an_infinite_state_that_is_carried(kind, name):
     v["bias"] = np.zeros((1, 6))
     v[name][20 if name == "X" else 380, 2] = np.inf
     scan(kind, v, [[3, 400]], 405, name, segment=32, only=("dX", "dB", "dC"))
+
+
+def test_statescan_gradient_of_many_regions_of_a_wide_group():
+    """Groups of 130 channels, whose tiles' shares of dB and dC are added: thousands of short regions, and one just under the length that is cut."""
+    rng = np.random.default_rng(19)
+    lens = np.concatenate([rng.integers(0, 4, 3000), [120], rng.integers(0, 4, 500)])
+    starts = np.cumsum(np.concatenate([[0], lens[:-1]]))
+    R = np.stack([starts, starts + lens], 1)[rng.permutation(len(lens))].tolist()
+    N = int(lens.sum()) + 5
+    scan("float32", values(rng, N, len(R), 260, 2, 6), R, N, "many", segment=32)
