@@ -110,6 +110,11 @@ _SIGNATURES = {
     "dbk_statescan": [_P, _P, _P, _Z],
     "dbk_statescan_bprop": [_P, _P, _P, _Z],
     "dbk_statescan_step": [_P, _P],
+    "dbk_deltarule_args_size": [],
+    "dbk_deltarule_workspace": [_P, _I, _P],
+    "dbk_deltarule": [_P, _P, _P, _Z],
+    "dbk_deltarule_bprop": [_P, _P, _P, _Z],
+    "dbk_deltarule_step": [_P, _P],
     "dbk_train_step": [_P, _P],
     "dbk_train_steps": [_P, _Z, _P],
     "dbk_train_step_single_workspace": [_P, _P],
@@ -147,6 +152,17 @@ class StateScanArgs(ctypes.Structure):
         ("skip", _P), ("dt_bias", _P), ("gate", _P), ("ldgate", _Z), ("state", _P), ("Y", _P), ("ldy", _Z), ("last", _P), ("keep", _P),
         ("dY", _P), ("lddy", _Z), ("dX", _P), ("lddx", _Z), ("ddt", _P), ("ldddt", _Z), ("dgate", _P), ("lddgate", _Z),
         ("dB", _P), ("lddb", _Z), ("dC", _P), ("lddc", _Z), ("dA", _P), ("dskip", _P), ("ddt_bias", _P),
+    ]
+
+
+class DeltaRuleArgs(ctypes.Structure):
+    """dbk_deltarule_args of the public header, field for field."""
+    _fields_ = [
+        ("dtype", _I), ("N", _Z), ("H", _Z), ("G", _Z), ("K", _Z), ("V", _Z), ("regions", _P), ("nregion", _Z),
+        ("Q", _P), ("ldq", _Z), ("Kk", _P), ("ldk", _Z), ("Vv", _P), ("ldv", _Z), ("beta", _P), ("ldbeta", _Z), ("decay", _P), ("lddecay", _Z),
+        ("scale", _D), ("state", _P), ("O", _P), ("ldo", _Z), ("last", _P), ("keep", _P),
+        ("dO", _P), ("lddo", _Z), ("dQ", _P), ("lddq", _Z), ("dK", _P), ("lddk", _Z), ("dV", _P), ("lddv", _Z),
+        ("dbeta", _P), ("lddbeta", _Z), ("ddecay", _P), ("ldddecay", _Z),
     ]
 
 

@@ -1,0 +1,262 @@
+// The gated delta rule along the rows of every region: what its forward and backward kernels share.
+//
+// A head's state S (K x V) decays, is corrected by what a row's key finds in it, and is read by the row's query:
+//
+//   S' = a[t] S[t-1],  u[t] = b[t] (v[t] - S'^T k[t]),  S[t] = S' + k[t] u[t]^T,  o[t] = scale S[t]^T q[t],  a = exp(decay)
+//
+// Sixteen rows (a chunk) at once, from the state S0 before them: with the decays between rows D[i][j] = a[j+1] ... a[i], from the state to a row
+// first[i] = a[0] ... a[i] and from a row to the chunk's end last[j] = a[j+1] ... a[15],
+//
+//   N[i][j] = D[i][j] k[i].k[j] (j < i),  P[i][j] = D[i][j] q[i].k[j] (j <= i),  T = (I + diag(b) N)^-1
+//   X = V - first (K S0),  U = T (b X),  O = scale (first (Q S0) + P U),  S1 = first[15] S0 + K^T (last U)
+//
+// so that a chunk is a handful of 16-row products for the matrix cores. They run in the accumulation type (v_mfma_f32_16x16x4_f32, v_mfma_f64_16x16x4_f64): every
+// product and sum is as exact as the states, also where rows are bfloat16. Decays are products of the rows' own factors, never quotients
+// or exponentials of differences of sums, so that a factor of zero, or a long run of small ones, does what it does row by row.
+//
+// A matrix instruction's result and its right operand lie alike, but for the order in which the contraction runs: the lane that receives D[row(g, r)][c]
+// (g = lane / 16, c = lane % 16, r = 0..3) is the one that supplies B[g][c] of instruction r, if contraction index g of it stands for row(g, r). So a product's
+// result is the next one's right operand where it is, and, as the transposed result of the swapped product, its left one: states, U and their
+// gradients never leave the registers. A wave holds 16 columns of a head's state and shares nothing with those that hold the others.
+#pragma once
+#include <type_traits>
+#include "rows_common.h"
+
+namespace dbk {
+
+constexpr unsigned DELTA_CHUNK = 16;             // rows of a chunk: the matrix instructions' tile
+constexpr unsigned DELTA_BLOCK = 64;             // rows of a block, for which states are kept and chunks are prepared by one wave
+constexpr unsigned DELTA_CHUNKS = DELTA_BLOCK / DELTA_CHUNK;
+constexpr size_t DELTA_KEY = 128;                // the most columns of a key
+
+struct delta_shape {
+    unsigned N, nregion, H, G, K, V, ns;         // rows, regions, heads, key heads, columns of a key and of a value, tiles of 16 value columns per head
+    unsigned slots;                              // blocks that are not a region's first (segment_slots)
+    size_t ldq, ldk, ldv, ldb, ldg, ldo;
+};
+
+template <typename A> struct mm16;
+template <> struct mm16<float> {
+    typedef float vec __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ vec mac(float a, float b, vec c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ unsigned row(unsigned g, unsigned r) { return 4u * g + r; }
+};
+template <> struct mm16<double> {
+    typedef double vec __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ vec mac(double a, double b, vec c) { return __builtin_amdgcn_mfma_f64_16x16x4f64(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ unsigned row(unsigned g, unsigned r) { return g + 4u * r; }
+};
+
+// One 16 x 16 x 16 product: c + a b
+template <typename A> __device__ __forceinline__ typename mm16<A>::vec product(typename mm16<A>::vec a, typename mm16<A>::vec b, typename mm16<A>::vec c)
+{
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c = mm16<A>::mac(a[r], b[r], c);
+    return c;
+}
+template <typename A> __device__ __forceinline__ typename mm16<A>::vec zero16() { return typename mm16<A>::vec{A(0), A(0), A(0), A(0)}; }
+
+template <typename V> __device__ __forceinline__ bool all_finite(V v)
+{
+    typedef decltype(v[0] * v[0]) A;
+    const A z = (v[0] * A(0) + v[1] * A(0)) + (v[2] * A(0) + v[3] * A(0));
+    return z == A(0);
+}
+
+// c + a b where a is a triangle, zero above the diagonal (LOWER) or below it: a row of the result takes rows of b up to itself, or from itself on. A
+// product with the zeros would carry an infinity or NaN of the other rows to it as well, so where any shows the rows are done again one by one,
+// with the others left out.
+template <typename A, bool LOWER> __device__ __forceinline__ typename mm16<A>::vec triangle(typename mm16<A>::vec a, typename mm16<A>::vec b, typename mm16<A>::vec c, unsigned g)
+{
+    typename mm16<A>::vec o = product<A>(a, b, c);
+    if (__any(!all_finite(o))) {
+#pragma unroll 1
+        for (unsigned i = 0; i < 16u; ++i) {
+            typename mm16<A>::vec m;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const unsigned row = mm16<A>::row(g, r);
+                m[r] = (LOWER ? row <= i : row >= i) ? b[r] : A(0);
+            }
+            m = product<A>(a, m, c);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = mm16<A>::row(g, r) == i ? m[r] : o[r];
+        }
+    }
+    return o;
+}
+
+// What one wave prepares for a chunk of a head, as later kernels read it: matrices row by row, and per row what it decays and corrects by. Rows behind a
+// region's last: T is the identity there, N, P and b are zero, and nothing decays.
+template <typename A> struct delta_chunk {
+    A T[256], P[256];
+    A first[16], last[16], b[16], spare[16];
+};
+// and what the backward pass needs beside it
+template <typename A> struct delta_pairs {
+    A N[256], D[256];
+};
+
+// Blocks are numbered like segments (rows_common.h): a region's first by the region, the others by their slot behind those.
+struct delta_block {
+    unsigned r, k, at, slot;                     // region, block within it, first row, number
+    row_range g;
+    unsigned rows;                               // of this block
+};
+__device__ __forceinline__ bool find_block(const delta_shape& p, const uint32_t* regions, const uint32_t* marks, unsigned index, delta_block& b)
+{
+    b.slot = index;
+    if (index < p.nregion) {
+        b.r = index;
+        b.k = 0;
+        b.g = region_rows(regions, b.r, p.N);
+    } else if (!slot_segment(regions, p.nregion, p.N, marks, index - p.nregion, DELTA_BLOCK, b.r, b.g, b.k))
+        return false;
+    b.at = b.g.start + b.k * DELTA_BLOCK;
+    if (b.at >= b.g.end) return false;
+    b.rows = min(b.g.end - b.at, DELTA_BLOCK);
+    return true;
+}
+// the number of block k of region r
+__device__ __forceinline__ size_t block_number(const delta_shape& p, unsigned r, row_range g, unsigned k)
+{
+    return k ? (size_t)p.nregion + g.start / DELTA_BLOCK + k : r;
+}
+// its place in `keep`, which holds no region's first block
+__device__ __forceinline__ size_t kept_number(row_range g, unsigned k) { return g.start / DELTA_BLOCK + k; }
+
+// A wave's columns of a head and how a lane sees the 16-row tiles.
+template <typename A> struct delta_lane {
+    unsigned g, c, head, group, v;               // v: columns of V and O in front of the wave's
+    unsigned nv;                                 // its columns, 16 or fewer
+    __device__ __forceinline__ void place(const delta_shape& p, unsigned head_, unsigned tile)
+    {
+        g = (threadIdx.x & 63u) >> 4;
+        c = threadIdx.x & 15u;
+        head = head_;
+        group = head_ / (p.H / p.G);
+        v = head_ * p.V + tile * 16u;
+        nv = min(16u, p.V - tile * 16u);
+    }
+    __device__ __forceinline__ unsigned row(int r) const { return mm16<A>::row(g, r); }
+};
+
+// Tile operands of keys and queries. By rows: element [c][16 t + row(g, r)], the left operand of a product with the state; by columns: [row(g, r)][16 t + c], the left operand
+// (or the right one) where the contraction runs over the chunk's rows. Rows and columns that do not exist are zeros.
+template <typename T, int KT> __device__ __forceinline__ void load_by_rows(typename mm16<typename acc_of<T>::type>::vec (&f)[KT], const T* p, size_t ld, unsigned rows, unsigned cols,
+                                                                           unsigned g, unsigned c)
+{
+    typedef typename acc_of<T>::type A;
+    const bool here = c < rows;
+    const T* x = p + (size_t)(here ? c : 0u) * ld;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        if constexpr (sizeof(A) == 4) {
+            const unsigned at = 16u * t + 4u * g;
+            row_vec<T, 4> v;
+            v.load(x + at, here && at < cols ? cols - at : 0u);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) f[t][r] = v.v[r];
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const unsigned at = 16u * t + mm16<A>::row(g, r);
+                f[t][r] = here && at < cols ? (A)x[at] : A(0);
+            }
+        }
+    }
+}
+template <typename T, int KT> __device__ __forceinline__ void load_by_columns(typename mm16<typename acc_of<T>::type>::vec (&f)[KT], const T* p, size_t ld, unsigned rows, unsigned cols,
+                                                                              unsigned g, unsigned c)
+{
+    typedef typename acc_of<T>::type A;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const unsigned row = mm16<A>::row(g, r);
+        const bool here = row < rows;
+        const T* x = p + (size_t)(here ? row : 0u) * ld + c;
+#pragma unroll
+        for (int t = 0; t < KT; ++t) f[t][r] = here && 16u * t + c < cols ? (A)x[16 * t] : A(0);
+    }
+}
+// one tile of V, O or dO: [row(g, r)][c]
+template <typename T> __device__ __forceinline__ typename mm16<typename acc_of<T>::type>::vec load_tile(const T* p, size_t ld, unsigned rows, unsigned cols, unsigned g, unsigned c)
+{
+    typedef typename acc_of<T>::type A;
+    typename mm16<A>::vec f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const unsigned row = mm16<A>::row(g, r);
+        const bool here = row < rows && c < cols;
+        f[r] = here ? (A)p[(size_t)row * ld + c] : A(0);
+    }
+    return f;
+}
+// and of a chunk's own matrices: [c][row(g, r)] (by rows), [row(g, r)][c] (by columns); vectors [row(g, r)]
+template <typename A> __device__ __forceinline__ typename mm16<A>::vec matrix_by_rows(const A* m, unsigned g, unsigned c)
+{
+    typename mm16<A>::vec f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] = m[16u * c + mm16<A>::row(g, r)];
+    return f;
+}
+template <typename A> __device__ __forceinline__ typename mm16<A>::vec matrix_by_columns(const A* m, unsigned g, unsigned c)
+{
+    typename mm16<A>::vec f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] = m[16u * mm16<A>::row(g, r) + c];
+    return f;
+}
+template <typename A> __device__ __forceinline__ typename mm16<A>::vec by_row(const A* m, unsigned g)
+{
+    typename mm16<A>::vec f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] = m[mm16<A>::row(g, r)];
+    return f;
+}
+
+// A wave's columns of states (blocks of K x (H V)): tile t holds rows 16 t + row(g, r).
+template <typename A, int KT> __device__ __forceinline__ void load_state(typename mm16<A>::vec (&S)[KT], const A* p, const delta_shape& s, const delta_lane<A>& l)
+{
+    const size_t D = (size_t)s.H * s.V;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const unsigned k = 16u * t + l.row(r);
+            S[t][r] = p && k < s.K && l.c < l.nv ? p[k * D + l.v + l.c] : A(0);
+        }
+}
+template <typename A, int KT> __device__ __forceinline__ void store_state(const typename mm16<A>::vec (&S)[KT], A* p, const delta_shape& s, const delta_lane<A>& l)
+{
+    const size_t D = (size_t)s.H * s.V;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const unsigned k = 16u * t + l.row(r);
+            if (k < s.K && l.c < l.nv) p[k * D + l.v + l.c] = S[t][r];
+        }
+}
+
+template <typename F> inline void with_key_tiles(size_t K, F f)
+{
+    if (K <= 16) f(std::integral_constant<int, 1>());
+    else if (K <= 32) f(std::integral_constant<int, 2>());
+    else if (K <= 64) f(std::integral_constant<int, 4>());
+    else f(std::integral_constant<int, 8>());
+}
+
+// Defined in deltarule.hip.
+delta_shape delta_shape_of(const dbk_deltarule_args& a);
+int check_delta(const dbk_deltarule_args* a);
+int delta_mark(hipStream_t st, const delta_shape& s, const uint32_t* regions, uint32_t* marks);
+// chunks, and pairs where it is not null, of every block and head
+void delta_prepare(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const uint32_t* marks, void* chunks, void* pairs);
+inline size_t delta_blocks(const delta_shape& s) { return (size_t)s.nregion + s.slots; }
+inline size_t align16(size_t n) { return (n + 15) / 16 * 16; }
+
+// Defined in deltarule_bprop.hip.
+size_t delta_bprop_bytes(const dbk_deltarule_args& a);
+
+}  // namespace dbk

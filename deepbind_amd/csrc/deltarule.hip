@@ -1,0 +1,370 @@
+// The gated delta rule's forward pass, for whole regions and for single rows. Formulas and layout: deltarule.h.
+#include "deltarule.h"
+
+namespace dbk {
+
+__global__ __launch_bounds__(256) void k_delta_mark(delta_shape p, const uint32_t* __restrict__ regions, uint32_t* __restrict__ marks)
+{
+    // a wave per region
+    const unsigned r = blockIdx.x * 4u + (threadIdx.x >> 6);
+    if (r >= p.nregion) return;
+    mark_segments(marks, r, region_rows(regions, r, p.N), DELTA_BLOCK, threadIdx.x & 63u, 64u);
+}
+
+// A chunk's matrices. A wave takes a block of a head, four chunks: the products of its keys and queries on the matrix cores, then a lane per chunk and column for the
+// decays between rows and the triangle's inverse, column by column by substitution (powers of the triangle, which the matrix cores
+// could multiply instead, grow far beyond the inverse where keys come again, and lose it).
+template <typename T, int KT>
+__global__ __launch_bounds__(256) void k_delta_prepare(delta_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, const T* __restrict__ Q,
+                                                       const T* __restrict__ K, const typename acc_of<T>::type* __restrict__ beta,
+                                                       const typename acc_of<T>::type* __restrict__ decay, delta_chunk<typename acc_of<T>::type>* __restrict__ chunks,
+                                                       delta_pairs<typename acc_of<T>::type>* __restrict__ pairs)
+{
+    typedef typename acc_of<T>::type A;
+    typedef typename mm16<A>::vec vec;
+    __shared__ A kk_all[4][4][16][17], qk_all[4][4][16][17], a_all[4][64], b_all[4][64];
+    const unsigned wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u;
+    A (*kk)[16][17] = kk_all[wave], (*qk)[16][17] = qk_all[wave];
+    A *a = a_all[wave], *b = b_all[wave];
+    delta_block bl;
+    if (!find_block(p, regions, marks, blockIdx.x, bl)) return;
+    const unsigned head = min(blockIdx.y * 4u + wave, p.H - 1u), group = head / (p.H / p.G);      // (a wave too many does the last head again)
+    const unsigned nchunk = (bl.rows + 15u) / 16u;
+    for (unsigned i = 0; i < nchunk; ++i) {
+        const size_t row = bl.at + 16u * i;
+        const unsigned rows = min(bl.rows - 16u * i, 16u);
+        vec k[KT], q[KT], m = zero16<A>(), s = zero16<A>();
+        load_by_rows<T, KT>(k, K + row * p.ldk + (size_t)group * p.K, p.ldk, rows, p.K, g, c);
+        load_by_rows<T, KT>(q, Q + row * p.ldq + (size_t)group * p.K, p.ldq, rows, p.K, g, c);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            m = product<A>(k[t], k[t], m);
+            s = product<A>(q[t], k[t], s);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            kk[i][mm16<A>::row(g, r)][c] = m[r];
+            qk[i][mm16<A>::row(g, r)][c] = s[r];
+        }
+    }
+    {
+        const bool here = lane < bl.rows;
+        const size_t row = bl.at + (here ? lane : 0u);
+        a[lane] = here && decay ? exp(decay[row * p.ldg + head]) : A(1);
+        b[lane] = here ? beta[row * p.ldb + head] : A(0);
+    }
+    __syncthreads();
+    // lane (g, c): column c of chunk g
+    const bool there = g < nchunk;
+    const size_t at = ((size_t)bl.slot * p.H + head) * DELTA_CHUNKS + g;
+    A D = A(0), first = A(1);
+    if (there) {
+        A mine = A(1);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const A ai = a[16u * g + i];
+            D = i == (int)c ? A(1) : D * ai;     // (zero above the diagonal: nothing there yet)
+            first *= ai;
+            mine = i == (int)c ? first : mine;
+            const A n = i > (int)c ? D * kk[g][i][c] : A(0), s = i >= (int)c ? D * qk[g][i][c] : A(0);
+            kk[g][i][c] = n;
+            chunks[at].P[16 * i + c] = s;
+            if (pairs) {
+                pairs[at].N[16 * i + c] = n;
+                pairs[at].D[16 * i + c] = i >= (int)c ? D : A(0);
+            }
+        }
+        chunks[at].first[c] = mine;
+        chunks[at].last[c] = D;
+        chunks[at].b[c] = b[16u * g + c];
+    }
+    __syncthreads();
+    if (!there) return;
+    A x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        A s = A(0);
+#pragma unroll
+        for (int m = 0; m < i; ++m) s = fma(kk[g][i][m], x[m], s);
+        x[i] = i < (int)c ? A(0) : fma(-b[16u * g + i], s, i == (int)c ? A(1) : A(0));
+        chunks[at].T[16 * i + c] = x[i];
+    }
+}
+
+// Walks a wave's 16 columns of a head's state down `rows` rows from `row` on. number(k): the number of the block k blocks on from the first.
+template <typename T, int KT, typename NUMBER>
+__device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lane<typename acc_of<T>::type>& l, const T* Q, const T* K, const T* V,
+                                           const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, size_t row, unsigned rows, NUMBER number,
+                                           typename mm16<typename acc_of<T>::type>::vec (&S)[KT], T* O, typename acc_of<T>::type* keep, size_t kept)
+{
+    typedef typename acc_of<T>::type A;
+    typedef typename mm16<A>::vec vec;
+    const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K, *v = V + row * p.ldv + l.v;
+    T* o = O + row * p.ldo + l.v;
+    for (unsigned t = 0; t < rows; t += DELTA_CHUNK) {
+        const unsigned n = min(rows - t, DELTA_CHUNK);
+        if (keep && t && t % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + (kept + t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
+        const delta_chunk<A>& ch = chunks[(number(t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS];
+        vec f[KT];
+        load_by_rows<T, KT>(f, k, p.ldk, n, p.K, l.g, l.c);
+        vec w = zero16<A>(), z = zero16<A>();
+#pragma unroll
+        for (int i = 0; i < KT; ++i) w = product<A>(f[i], S[i], w);
+        load_by_rows<T, KT>(f, q, p.ldq, n, p.K, l.g, l.c);
+#pragma unroll
+        for (int i = 0; i < KT; ++i) z = product<A>(f[i], S[i], z);
+        const vec first = by_row(ch.first, l.g), b = by_row(ch.b, l.g), last = by_row(ch.last, l.g);
+        vec x = load_tile(v, p.ldv, n, l.nv, l.g, l.c);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = l.row(r) < n ? b[r] * (x[r] - first[r] * w[r]) : A(0);
+        const vec u = triangle<A, true>(matrix_by_rows(ch.T, l.g, l.c), x, zero16<A>(), l.g);
+        vec y = triangle<A, true>(matrix_by_rows(ch.P, l.g, l.c), u, first * z, l.g);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (l.row(r) < n && l.c < l.nv) o[(size_t)l.row(r) * p.ldo + l.c] = (T)(scale * y[r]);
+        load_by_columns<T, KT>(f, k, p.ldk, n, p.K, l.g, l.c);
+        const A through = ch.first[15];
+        const vec sent = last * u;
+#pragma unroll
+        for (int i = 0; i < KT; ++i) S[i] = product<A>(f[i], sent, through * S[i]);
+        q += DELTA_CHUNK * p.ldq;
+        k += DELTA_CHUNK * p.ldk;
+        v += DELTA_CHUNK * p.ldv;
+        o += DELTA_CHUNK * p.ldo;
+    }
+}
+
+template <typename T, int KT>
+__global__ __launch_bounds__(256) void k_delta_fprop(delta_shape p, const uint32_t* __restrict__ regions, const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
+                                                     const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, typename acc_of<T>::type scale,
+                                                     const typename acc_of<T>::type* __restrict__ state, T* __restrict__ O, typename acc_of<T>::type* __restrict__ last,
+                                                     typename acc_of<T>::type* __restrict__ keep)
+{
+    typedef typename acc_of<T>::type A;
+    typedef typename mm16<A>::vec vec;
+    const unsigned f = blockIdx.y * 4u + uniform(threadIdx.x >> 6);
+    if (f >= p.H * p.ns) return;
+    delta_lane<A> l;
+    l.place(p, f / p.ns, f % p.ns);
+    const unsigned r = blockIdx.x;
+    const row_range g = region_rows(regions, r, p.N);
+    const size_t block = (size_t)p.K * p.H * p.V;
+    vec S[KT];
+    load_state<A, KT>(S, state ? state + r * block : (const A*)nullptr, p, l);
+    delta_walk<T, KT>(p, l, Q, K, V, chunks, scale, g.start, g.end - g.start, [&](unsigned k) { return block_number(p, r, g, k); }, S, O, keep, kept_number(g, 0u));
+    if (last) store_state<A, KT>(S, last + r * block, p, l);
+}
+
+// One row of each sequence. A workgroup takes 64 columns of a head's state, a thread VEC neighbouring ones of RPT rows of it; what key and query find is added over the
+// row groups in LDS. o = scale S1^T q = scale (a S0^T q + (k.q) u), so that the state is read once and written once.
+template <typename T, int RPT>
+__global__ __launch_bounds__(256) void k_delta_step(delta_shape p, const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
+                                                    const typename acc_of<T>::type* __restrict__ beta, const typename acc_of<T>::type* __restrict__ decay, typename acc_of<T>::type scale,
+                                                    const typename acc_of<T>::type* state, typename acc_of<T>::type* into, T* __restrict__ O)
+{
+    typedef typename acc_of<T>::type A;
+    constexpr unsigned VEC = 4, CG = 16, RG = 16;
+    __shared__ A kq[2][128], sums[3][RG][64];
+    const unsigned n = blockIdx.x, parts = (p.V + 63u) / 64u, head = blockIdx.y / parts, part = blockIdx.y % parts, group = head / (p.H / p.G);
+    const unsigned cg = threadIdx.x % CG, rg = threadIdx.x / CG;
+    const unsigned col = part * 64u + cg * VEC, valid = col < p.V ? p.V - col : 0u;
+    const size_t D = (size_t)p.H * p.V, base = (size_t)n * p.K * D + (size_t)head * p.V + col;
+    const unsigned key = threadIdx.x & 127u;
+    kq[threadIdx.x >> 7][key] = key < p.K ? (A)(threadIdx.x < 128u ? K[n * p.ldk + (size_t)group * p.K + key] : Q[n * p.ldq + (size_t)group * p.K + key]) : A(0);
+    row_vec<A, VEC> S[RPT];
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const unsigned k = rg + RG * i;
+        S[i].load(state + base + k * D, k < p.K ? valid : 0u);
+    }
+    const A a = decay ? exp(decay[n * p.ldg + head]) : A(1), b = beta[n * p.ldb + head];
+    __syncthreads();
+    A w[VEC], z[VEC], both = A(0);
+#pragma unroll
+    for (int j = 0; j < (int)VEC; ++j) w[j] = z[j] = A(0);
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const A k = kq[0][rg + RG * i], q = kq[1][rg + RG * i];
+        both = fma(k, q, both);
+#pragma unroll
+        for (int j = 0; j < (int)VEC; ++j) {
+            S[i].v[j] *= a;
+            w[j] = fma(k, S[i].v[j], w[j]);
+            z[j] = fma(q, S[i].v[j], z[j]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < (int)VEC; ++j) {
+        sums[0][rg][cg * VEC + j] = w[j];
+        sums[1][rg][cg * VEC + j] = z[j];
+        sums[2][rg][cg * VEC + j] = both;
+    }
+    __syncthreads();
+    A u[VEC];
+#pragma unroll
+    for (int j = 0; j < (int)VEC; ++j) {
+        A ws = A(0);
+#pragma unroll
+        for (unsigned i = 0; i < RG; ++i) ws += sums[0][i][cg * VEC + j];
+        u[j] = j < (int)valid ? b * ((A)V[n * p.ldv + (size_t)head * p.V + col + j] - ws) : A(0);
+    }
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+        const unsigned k = rg + RG * i;
+        const A kv = kq[0][k];
+#pragma unroll
+        for (int j = 0; j < (int)VEC; ++j) S[i].v[j] = fma(kv, u[j], S[i].v[j]);
+        if (k < p.K) S[i].store(into + base + k * D, valid);
+    }
+    if (rg == 0u) {
+#pragma unroll
+        for (int j = 0; j < (int)VEC; ++j) {
+            A zs = A(0), bs = A(0);
+#pragma unroll
+            for (unsigned i = 0; i < RG; ++i) { zs += sums[1][i][cg * VEC + j]; bs += sums[2][i][cg * VEC + j]; }
+            if (j < (int)valid) O[n * p.ldo + (size_t)head * p.V + col + j] = (T)(scale * fma(bs, u[j], zs));
+        }
+    }
+}
+
+delta_shape delta_shape_of(const dbk_deltarule_args& a)
+{
+    delta_shape s = {};
+    s.N = (unsigned)a.N;
+    s.nregion = (unsigned)a.nregion;
+    s.H = (unsigned)a.H;
+    s.G = (unsigned)a.G;
+    s.K = (unsigned)a.K;
+    s.V = (unsigned)a.V;
+    s.ns = divup(a.V, 16);
+    s.slots = (unsigned)segment_slots(a.N, DELTA_BLOCK);
+    s.ldq = a.ldq;
+    s.ldk = a.ldk;
+    s.ldv = a.ldv;
+    s.ldb = a.ldbeta;
+    s.ldg = a.lddecay;
+    s.ldo = a.ldo;
+    return s;
+}
+
+int check_delta(const dbk_deltarule_args* a)
+{
+    DBK_CHECK(a, "ValueError: null arguments");
+    DBK_ROW_DTYPE_OK(a->dtype);
+    DBK_CHECK(a->H >= 1 && a->G >= 1 && a->H % a->G == 0, "ValueError: the number of heads must be divisible by the number of key heads");
+    DBK_CHECK(a->K >= 1 && a->K <= DELTA_KEY, "NotImplementedError: keys of 1 to %zu columns, got %zu", DELTA_KEY, a->K);
+    DBK_CHECK(a->N < (size_t(1) << 31) && a->V < (size_t(1) << 20) && a->H < (size_t(1) << 20) && a->H * ((a->V + 15) / 16) <= 65535, "ValueError: map too large (%zu rows, %zu heads of %zu columns)", a->N, a->H, a->V);
+    DBK_CHECK(a->nregion < (size_t(1) << 24), "ValueError: too many regions (%zu)", a->nregion);
+    DBK_CHECK(!a->N || !a->V || (a->Q && a->Kk && a->Vv && a->beta), "ValueError: null matrix");
+    DBK_CHECK(a->N <= 1 || (a->ldq >= a->G * a->K && a->ldk >= a->G * a->K && a->ldv >= a->H * a->V && a->ldbeta >= a->H && (!a->decay || a->lddecay >= a->H)),
+              "ValueError: row strides must be at least the number of columns");
+    return 0;
+}
+
+int delta_mark(hipStream_t st, const delta_shape& s, const uint32_t* regions, uint32_t* marks)
+{
+    k_delta_mark<<<divup(s.nregion, 4), 256, 0, st>>>(s, regions, marks);
+    return 0;
+}
+
+void delta_prepare(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const uint32_t* marks, void* chunks, void* pairs)
+{
+    with_row_type(a.dtype, [&](auto t) {
+        typedef decltype(t) T;
+        typedef typename acc_of<T>::type A;
+        with_key_tiles(a.K, [&](auto kt) {
+            k_delta_prepare<T, kt.value><<<dim3((unsigned)delta_blocks(s), divup(s.H, 4)), 256, 0, st>>>(s, a.regions, marks, (const T*)a.Q, (const T*)a.Kk, (const A*)a.beta, (const A*)a.decay,
+                                                                                                        (delta_chunk<A>*)chunks, (delta_pairs<A>*)pairs);
+        });
+    });
+}
+
+namespace {
+
+// Parts of the forward pass's workspace.
+struct delta_work {
+    uint32_t* marks;
+    char* chunks;
+    size_t bytes;
+};
+delta_work work_in(void* work, const dbk_deltarule_args& a, const delta_shape& s)
+{
+    delta_work w;
+    char* p = (char*)work;
+    size_t at = 0;
+    w.marks = (uint32_t*)p;
+    at += align16(s.slots * sizeof(uint32_t));
+    w.chunks = p + at;
+    at += delta_blocks(s) * a.H * DELTA_CHUNKS * (a.dtype == DBK_F64 ? sizeof(delta_chunk<double>) : sizeof(delta_chunk<float>));
+    w.bytes = at;
+    return w;
+}
+
+}  // namespace
+}  // namespace dbk
+
+using namespace dbk;
+
+extern "C" {
+
+int dbk_deltarule_args_size(void) { return (int)sizeof(dbk_deltarule_args); }
+
+int dbk_deltarule_workspace(const dbk_deltarule_args* a, int backward, size_t* work_bytes)
+{
+    if (int rc = check_delta(a)) return rc;
+    DBK_CHECK(work_bytes, "ValueError: null result");
+    *work_bytes = 0;
+    if (a->N && a->V && a->nregion) *work_bytes = backward ? delta_bprop_bytes(*a) : work_in(nullptr, *a, delta_shape_of(*a)).bytes;
+    clear_error();
+    return 0;
+}
+
+int dbk_deltarule(dbk_stream_t stream, const dbk_deltarule_args* a, void* work, size_t work_bytes)
+{
+    if (int rc = check_delta(a)) return rc;
+    DBK_CHECK(!a->nregion || a->regions, "ValueError: null regions");
+    DBK_CHECK(!a->N || !a->V || a->O, "ValueError: null matrix");
+    DBK_CHECK(a->N <= 1 || a->ldo >= a->H * a->V, "ValueError: row strides must be at least the number of columns");
+    DBK_CHECK(!a->keep || !a->state, "ValueError: states are kept for the backward pass of whole sequences, which starts from zeros: no initial state");
+    if (!a->V || !a->nregion) { clear_error(); return 0; }
+    const delta_shape s = delta_shape_of(*a);
+    const delta_work w = work_in(work, *a, s);
+    DBK_CHECK(!w.bytes || (work && work_bytes >= w.bytes), "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, w.bytes);
+    DBK_CHECK(grid_fits(delta_blocks(s), 256), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
+    hipStream_t st = as_stream(stream);
+    if (a->N) {
+        delta_mark(st, s, a->regions, w.marks);
+        delta_prepare(st, *a, s, w.marks, w.chunks, nullptr);
+    }
+    with_row_type(a->dtype, [&](auto t) {
+        typedef decltype(t) T;
+        typedef typename acc_of<T>::type A;
+        with_key_tiles(a->K, [&](auto kt) {
+            k_delta_fprop<T, kt.value><<<dim3(s.nregion, divup((size_t)s.H * s.ns, 4)), 256, 0, st>>>(
+                s, a->regions, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const delta_chunk<A>*)w.chunks, (A)a->scale, (const A*)a->state, (T*)a->O, (A*)a->last, (A*)a->keep);
+        });
+    });
+    DBK_LAUNCH_OK();
+}
+
+int dbk_deltarule_step(dbk_stream_t stream, const dbk_deltarule_args* a)
+{
+    if (int rc = check_delta(a)) return rc;
+    DBK_CHECK(!a->N || !a->V || (a->O && a->state && a->last), "ValueError: null matrix or state");
+    DBK_CHECK(a->N <= 1 || a->ldo >= a->H * a->V, "ValueError: row strides must be at least the number of columns");
+    DBK_CHECK(grid_fits(a->N, 256, a->H * ((a->V + 63) / 64)), "ValueError: too many sequences (%zu)", a->N);
+    if (!a->N || !a->V) { clear_error(); return 0; }
+    const delta_shape s = delta_shape_of(*a);
+    hipStream_t st = as_stream(stream);
+    with_row_type(a->dtype, [&](auto t) {
+        typedef decltype(t) T;
+        typedef typename acc_of<T>::type A;
+        with_key_tiles(a->K, [&](auto kt) {
+            k_delta_step<T, kt.value><<<dim3(s.N, s.H * divup(a->V, 64)), 256, 0, st>>>(s, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const A*)a->beta, (const A*)a->decay, (A)a->scale,
+                                                                                       (const A*)a->state, (A*)a->last, (T*)a->O);
+        });
+    });
+    DBK_LAUNCH_OK();
+}
+
+}  // extern "C"

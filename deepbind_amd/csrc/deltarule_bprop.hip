@@ -1,0 +1,447 @@
+// The gated delta rule's backward pass. Notation: deltarule.h; dX stands for the gradient of X, dO carries the output's scale.
+//
+// From the chunk's end to its start, with S0 and dS1 (the gradient of the state behind the chunk):
+//
+//   dU = P^T dO + last (K dS1),  dY = T^T dU (Y = b X),  dX = b dY = dV,  dW = -first dX (W = K S0)
+//   dS0 = first[15] dS1 + K^T dW + Q^T (first dO)
+//   dP = dO U^T,  dL = -dY U^T (L = diag(b) N, as U = Y - L U)
+//   dQ = (first dO) S0^T + (dP D) K,  dK = dW S0^T + (last U) dS1^T + (dP D)^T Q + (M + M^T) K with M = b dL D below the diagonal
+//   db = sum_v dY X + sum_j dL N
+//
+// A decay acts on every pair of rows around it, on what comes from S0, on what goes to S1 and on what passes: with E = dP P + b dL N, whose
+// entries are the pairs' products of value and gradient,
+//
+//   ddecay[m] = sum_(i >= m > j) E[i][j] + sum_(i >= m) (q . (first dO S0^T) + k . (dW S0^T))[i] + sum_(j < m) (k . (last U dS1^T))[j] + first[15] <S0, dS1>
+//
+// Two kernels: a wave walks 16 columns of a head's dS up its region and leaves it behind every block of 64 rows; then all blocks are independent,
+// each from the state that the forward pass kept before it and the gradient behind it. What is summed over a value's columns (dQ, dK, dP, dL) passes through LDS
+// between the waves of a head, and through memory between the parts of 64 columns of wide values and between heads that share a key: added in a fixed order.
+#include "deltarule.h"
+
+namespace dbk {
+
+// dS of a chunk's start from that of its end
+template <typename T, int KT>
+__global__ __launch_bounds__(256) void k_delta_chain(delta_shape p, size_t lddo, const uint32_t* __restrict__ regions, const T* __restrict__ Q, const T* __restrict__ K,
+                                                     const T* __restrict__ dO, const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, typename acc_of<T>::type scale,
+                                                     typename acc_of<T>::type* __restrict__ dstates)
+{
+    typedef typename acc_of<T>::type A;
+    typedef typename mm16<A>::vec vec;
+    const unsigned f = blockIdx.y * 4u + uniform(threadIdx.x >> 6);
+    if (f >= p.H * p.ns) return;
+    delta_lane<A> l;
+    l.place(p, f / p.ns, f % p.ns);
+    const unsigned r = blockIdx.x;
+    const row_range g = region_rows(regions, r, p.N);
+    const unsigned rows = g.end - g.start;
+    if (rows <= DELTA_BLOCK) return;
+    vec S[KT];
+#pragma unroll
+    for (int i = 0; i < KT; ++i) S[i] = zero16<A>();
+    for (unsigned t = (rows - 1) / DELTA_CHUNK * DELTA_CHUNK; t >= DELTA_BLOCK; t -= DELTA_CHUNK) {
+        const unsigned n = min(rows - t, DELTA_CHUNK);
+        const size_t row = (size_t)g.start + t;
+        const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K;
+        const delta_chunk<A>& ch = chunks[(block_number(p, r, g, t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS];
+        vec f_[KT], y = zero16<A>();
+        load_by_rows<T, KT>(f_, k, p.ldk, n, p.K, l.g, l.c);
+#pragma unroll
+        for (int i = 0; i < KT; ++i) y = product<A>(f_[i], S[i], y);
+        const vec first = by_row(ch.first, l.g), b = by_row(ch.b, l.g), last = by_row(ch.last, l.g);
+        const vec d = scale * load_tile(dO + row * lddo + l.v, lddo, n, l.nv, l.g, l.c);
+        const vec du = triangle<A, false>(matrix_by_columns(ch.P, l.g, l.c), d, last * y, l.g);
+        const vec dy = triangle<A, false>(matrix_by_columns(ch.T, l.g, l.c), du, zero16<A>(), l.g);
+        const vec dw = -(first * (b * dy)), fd = first * d;
+        const A through = ch.first[15];
+        load_by_columns<T, KT>(f_, k, p.ldk, n, p.K, l.g, l.c);
+#pragma unroll
+        for (int i = 0; i < KT; ++i) S[i] = product<A>(f_[i], dw, through * S[i]);
+        load_by_columns<T, KT>(f_, q, p.ldq, n, p.K, l.g, l.c);
+#pragma unroll
+        for (int i = 0; i < KT; ++i) S[i] = product<A>(f_[i], fd, S[i]);
+        if (t % DELTA_BLOCK == 0) store_state<A, KT>(S, dstates + kept_number(g, t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
+    }
+}
+
+// transposed states: tile t holds [row(g, r)][16 t + c] of the wave's 16 columns by K
+template <typename A, int KT> __device__ __forceinline__ void load_state_t(typename mm16<A>::vec (&S)[KT], const A* p, const delta_shape& s, const delta_lane<A>& l)
+{
+    const size_t D = (size_t)s.H * s.V;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+        const unsigned k = 16u * t + l.c;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[t][r] = p && k < s.K && l.row(r) < l.nv ? p[k * D + l.v + l.row(r)] : A(0);
+    }
+}
+
+// The transposed tile of x. Products with zeros are as in triangle(): where the tile is not all finite, lanes exchange it value by value.
+template <typename A> __device__ __forceinline__ typename mm16<A>::vec exchange(typename mm16<A>::vec x, unsigned g, unsigned c)
+{
+    typename mm16<A>::vec o;
+    const unsigned gc = sizeof(A) == 4 ? c >> 2 : c & 3u, rc = sizeof(A) == 4 ? c & 3u : c >> 2;     // row(gc, rc) == c
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int from = (int)(16u * gc + mm16<A>::row(g, r));
+        const A v[4] = {__shfl(x[0], from), __shfl(x[1], from), __shfl(x[2], from), __shfl(x[3], from)};
+        o[r] = rc == 0u ? v[0] : rc == 1u ? v[1] : rc == 2u ? v[2] : v[3];
+    }
+    return o;
+}
+
+// sums over the 16 lanes of a row
+template <typename A> __device__ __forceinline__ A lanes16_sum(A v)
+{
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+template <typename T> struct delta_grads {
+    typedef typename acc_of<T>::type A;
+    T *dQ, *dK, *dV;
+    A *dbeta, *ddecay;
+    size_t lddq, lddk, lddv, lddb, lddg;
+    // where more than one unit (head and part of its value) has a share: (units of a key, N, G K) and (parts, N, H)
+    A *dq, *dk, *db, *dg;
+    unsigned parts, waves;                       // parts of a value, waves per unit (1, 2 or 4)
+};
+
+template <typename A, int KT> struct delta_share {
+    A pl[2][16][17];                             // dP, dL
+    A q[KT][16][17], k[KT][16][17];
+    A into[16], out[16], b[16], through;
+};
+
+template <typename T, int KT>
+__global__ __launch_bounds__(256) void k_delta_bprop(delta_shape p, size_t lddo, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, const T* __restrict__ Q,
+                                                     const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ dO,
+                                                     const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, const delta_pairs<typename acc_of<T>::type>* __restrict__ pairs,
+                                                     typename acc_of<T>::type scale, const typename acc_of<T>::type* __restrict__ keep,
+                                                     const typename acc_of<T>::type* __restrict__ dstates, delta_grads<T> out)
+{
+    typedef typename acc_of<T>::type A;
+    typedef typename mm16<A>::vec vec;
+    extern __shared__ __align__(16) char lds_bytes[];
+    delta_share<A, KT>* all = (delta_share<A, KT>*)lds_bytes;
+    const unsigned wave = uniform(threadIdx.x >> 6), slice = wave & (out.waves - 1u);
+    delta_block bl;
+    if (!find_block(p, regions, marks, blockIdx.x, bl)) return;
+    const unsigned unit = min((blockIdx.y * 4u + wave) / out.waves, p.H * out.parts - 1u), part = unit % out.parts;      // (a unit too many does the last one again)
+    const unsigned tile = part * 4u + slice;
+    delta_lane<A> l;
+    l.place(p, unit / out.parts, min(tile, p.ns - 1u));
+    if (tile >= p.ns) l.nv = 0u;
+    const unsigned g = l.g, c = l.c, nchunk = (bl.rows + 15u) / 16u;
+    const size_t state = (size_t)p.K * p.H * p.V;
+    const T *q0 = Q + (size_t)bl.at * p.ldq + (size_t)l.group * p.K, *k0 = K + (size_t)bl.at * p.ldk + (size_t)l.group * p.K;
+    const T *v0 = V + (size_t)bl.at * p.ldv + l.v, *d0 = dO + (size_t)bl.at * lddo + l.v;
+    const size_t first_chunk = ((size_t)bl.slot * p.H + l.head) * DELTA_CHUNKS;
+
+    // forward again, from the block's start: what the way back needs stays in registers
+    vec xs[DELTA_CHUNKS], uts[DELTA_CHUNKS], sts[DELTA_CHUNKS][KT];
+    {
+        vec S[KT], ST[KT];
+        const A* from = bl.k ? keep + kept_number(bl.g, bl.k) * state : (const A*)nullptr;
+        load_state<A, KT>(S, from, p, l);
+        load_state_t<A, KT>(ST, from, p, l);
+#pragma unroll
+        for (int i = 0; i < (int)DELTA_CHUNKS; ++i) {
+            if (i >= (int)nchunk) break;
+            const unsigned n = min(bl.rows - 16u * i, 16u);
+            const delta_chunk<A>& ch = chunks[first_chunk + i];
+            vec f[KT], w = zero16<A>();
+            load_by_rows<T, KT>(f, k0 + 16 * i * p.ldk, p.ldk, n, p.K, g, c);
+#pragma unroll
+            for (int t = 0; t < KT; ++t) w = product<A>(f[t], S[t], w);
+            const vec first = by_row(ch.first, g), b = by_row(ch.b, g), last = by_row(ch.last, g);
+            vec x = load_tile(v0 + 16 * i * p.ldv, p.ldv, n, l.nv, g, c), y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                x[r] = l.row(r) < n ? x[r] - first[r] * w[r] : A(0);
+                y[r] = b[r] * x[r];
+            }
+            const vec tr = matrix_by_rows(ch.T, g, c), u = triangle<A, true>(tr, y, zero16<A>(), g);
+            xs[i] = x;
+            uts[i] = product<A>(y, tr, zero16<A>());
+            if (__any(!all_finite(uts[i]))) uts[i] = exchange<A>(u, g, c);
+#pragma unroll
+            for (int t = 0; t < KT; ++t) sts[i][t] = ST[t];
+            if (i + 1 >= (int)nchunk) break;
+            const A through = ch.first[15];
+            const vec sent = last * u;
+            load_by_columns<T, KT>(f, k0 + 16 * i * p.ldk, p.ldk, n, p.K, g, c);
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                S[t] = product<A>(f[t], sent, through * S[t]);
+                ST[t] = product<A>(sent, f[t], through * ST[t]);
+            }
+        }
+    }
+
+    vec dS[KT], dST[KT];
+    {
+        const A* from = bl.at + bl.rows < bl.g.end ? dstates + kept_number(bl.g, bl.k + 1u) * state : (const A*)nullptr;
+        load_state<A, KT>(dS, from, p, l);
+        load_state_t<A, KT>(dST, from, p, l);
+    }
+#pragma unroll
+    for (int i = (int)DELTA_CHUNKS - 1; i >= 0; --i) {
+        if (i >= (int)nchunk) continue;
+        const unsigned n = min(bl.rows - 16u * i, 16u);
+        const size_t row = (size_t)bl.at + 16u * i;
+        const delta_chunk<A>& ch = chunks[first_chunk + i];
+        const delta_pairs<A>& pr = pairs[first_chunk + i];
+        vec f[KT], y = zero16<A>();
+        load_by_rows<T, KT>(f, k0 + 16 * i * p.ldk, p.ldk, n, p.K, g, c);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) y = product<A>(f[t], dS[t], y);
+        const vec first = by_row(ch.first, g), b = by_row(ch.b, g), last = by_row(ch.last, g);
+        const A first_c = ch.first[c], b_c = ch.b[c], last_c = ch.last[c], through = ch.first[15];
+        const vec d = scale * load_tile(d0 + 16 * i * lddo, lddo, n, l.nv, g, c);
+        vec dt[1];
+        load_by_rows<T, 1>(dt, d0 + 16 * i * lddo, lddo, n, l.nv, g, c);
+        dt[0] = scale * dt[0];
+        const vec du = triangle<A, false>(matrix_by_columns(ch.P, g, c), d, last * y, g);
+        const vec tc = matrix_by_columns(ch.T, g, c);
+        const vec dy = triangle<A, false>(tc, du, zero16<A>(), g);
+        vec dyt = product<A>(du, tc, zero16<A>());
+        if (__any(!all_finite(dyt))) dyt = exchange<A>(dy, g, c);
+        const vec dx = b * dy, dw = -(first * dx), dwt = -(first_c * b_c) * dyt, fd = first * d, fdt = first_c * dt[0], lut = last_c * uts[i];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (l.row(r) < n && c < l.nv) out.dV[(row + l.row(r)) * out.lddv + l.v + c] = (T)dx[r];
+
+        delta_share<A, KT>& mine = all[wave];
+        const vec dp = product<A>(dt[0], uts[i], zero16<A>()), dl = -product<A>(dyt, uts[i], zero16<A>());
+        vec kc[KT], qc[KT], into = zero16<A>(), sent = zero16<A>();
+        load_by_columns<T, KT>(kc, k0 + 16 * i * p.ldk, p.ldk, n, p.K, g, c);
+        load_by_columns<T, KT>(qc, q0 + 16 * i * p.ldq, p.ldq, n, p.K, g, c);
+        A passed = A(0);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            const vec a = product<A>(fdt, sts[i][t], zero16<A>()), e = product<A>(dwt, sts[i][t], zero16<A>()), s = product<A>(lut, dST[t], zero16<A>());
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                mine.q[t][l.row(r)][c] = a[r];
+                mine.k[t][l.row(r)][c] = e[r] + s[r];
+                into[r] = fma(qc[t][r], a[r], fma(kc[t][r], e[r], into[r]));
+                sent[r] = fma(kc[t][r], s[r], sent[r]);
+                passed = fma(sts[i][t][r], dST[t][r], passed);
+            }
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) passed += __shfl_xor(passed, o);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            mine.pl[0][l.row(r)][c] = dp[r];
+            mine.pl[1][l.row(r)][c] = dl[r];
+            const A in = lanes16_sum(into[r]), on = lanes16_sum(sent[r]), db = lanes16_sum(dy[r] * xs[i][r]);
+            if (c == 0u) {
+                mine.into[l.row(r)] = in;
+                mine.out[l.row(r)] = on;
+                mine.b[l.row(r)] = db;
+            }
+        }
+        if ((threadIdx.x & 63u) == 0u) mine.through = through * passed;
+        if (i > 0) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                dS[t] = product<A>(qc[t], fd, product<A>(kc[t], dw, through * dS[t]));
+                dST[t] = product<A>(fd, qc[t], product<A>(dw, kc[t], through * dST[t]));
+            }
+        }
+        __syncthreads();
+
+        // the unit's sums, and what the pairs of rows add to them
+        const delta_share<A, KT>* ours = all + (wave - slice);
+        vec pr_ = zero16<A>(), lr = zero16<A>(), pc = zero16<A>(), lc = zero16<A>();    // dP and dL: [c][row], [row][c]
+        for (unsigned s = 0; s < out.waves; ++s)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                pr_[r] += ours[s].pl[0][c][l.row(r)];
+                lr[r] += ours[s].pl[1][c][l.row(r)];
+                pc[r] += ours[s].pl[0][l.row(r)][c];
+                lc[r] += ours[s].pl[1][l.row(r)][c];
+            }
+        const vec Dr = matrix_by_rows(pr.D, g, c), Dc = matrix_by_columns(pr.D, g, c);
+        vec ar, ac, ms;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const unsigned j = l.row(r);
+            ar[r] = j <= c ? pr_[r] * Dr[r] : A(0);
+            ac[r] = c <= j ? pc[r] * Dc[r] : A(0);
+            ms[r] = j < c ? b_c * lr[r] * Dr[r] : c < j ? b[r] * lc[r] * Dc[r] : A(0);
+        }
+        const unsigned share = (l.head % (p.H / p.G)) * out.parts + part;
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+            if (((unsigned)t & (out.waves - 1u)) != slice || 16u * t >= p.K) continue;
+            vec dq = zero16<A>(), dk = zero16<A>();
+            for (unsigned s = 0; s < out.waves; ++s)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    dq[r] += ours[s].q[t][l.row(r)][c];
+                    dk[r] += ours[s].k[t][l.row(r)][c];
+                }
+            dq = triangle<A, true>(ar, kc[t], dq, g);
+            dk = product<A>(ms, kc[t], triangle<A, false>(ac, qc[t], dk, g));
+            const size_t col = (size_t)l.group * p.K + 16u * t + c;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (l.row(r) >= n || 16u * t + c >= p.K) continue;
+                const size_t at = row + l.row(r);
+                if (out.dq) {
+                    const size_t in = ((size_t)share * p.N + at) * p.G * p.K + col;
+                    out.dq[in] = dq[r];
+                    out.dk[in] = dk[r];
+                } else {
+                    out.dQ[at * out.lddq + col] = (T)dq[r];
+                    out.dK[at * out.lddk + col] = (T)dk[r];
+                }
+            }
+        }
+        if (slice == 0u) {
+            const vec Pr = matrix_by_rows(ch.P, g, c), Nr = matrix_by_rows(pr.N, g, c);
+            vec e, before;
+            A db = A(0), dg = A(0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const unsigned j = l.row(r);
+                const A ln = j < c ? lr[r] * Nr[r] : A(0);
+                e[r] = j < c ? fma(b_c, ln, pr_[r] * Pr[r]) : A(0);      // (the diagonal has no decay between its rows)
+                before[r] = j < c ? A(1) : A(0);
+                db += ln;
+            }
+            const vec upto = product<A>(e, before, zero16<A>());         // [i][m]: sum over j < m
+#pragma unroll
+            for (int r = 0; r < 4; ++r) dg += l.row(r) >= c ? upto[r] : A(0);
+            db += __shfl_xor(db, 16);
+            db += __shfl_xor(db, 32);
+            dg += __shfl_xor(dg, 16);
+            dg += __shfl_xor(dg, 32);
+            for (unsigned s = 0; s < out.waves; ++s) {
+                db += ours[s].b[c];
+                dg += ours[s].through;
+                for (unsigned m = 0; m < 16u; ++m) dg += m >= c ? ours[s].into[m] : ours[s].out[m];
+            }
+            if (g == 0u && c < n) {
+                const size_t at = row + c;
+                if (out.db) out.db[((size_t)part * p.N + at) * p.H + l.head] = db;
+                else out.dbeta[at * out.lddb + l.head] = db;
+                if (out.dg) out.dg[((size_t)part * p.N + at) * p.H + l.head] = dg;
+                else if (out.ddecay) out.ddecay[at * out.lddg + l.head] = dg;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// out[row][col] = sum over shares of part[share][row][col], for the rows of one block
+template <typename A, typename T>
+__device__ __forceinline__ void add_shares(const delta_block& bl, size_t N, unsigned cols, unsigned shares, const A* part, T* out, size_t ld)
+{
+    for (unsigned i = threadIdx.x; i < bl.rows * cols; i += 256u) {
+        const size_t row = bl.at + i / cols, col = i % cols;
+        A s = A(0);
+        for (unsigned u = 0; u < shares; ++u) s += part[((size_t)u * N + row) * cols + col];
+        out[row * ld + col] = (T)s;
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_delta_add(delta_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, delta_grads<T> out)
+{
+    delta_block bl;
+    if (!find_block(p, regions, marks, blockIdx.x, bl)) return;
+    if (blockIdx.y == 0u && out.dq) add_shares(bl, p.N, p.G * p.K, p.H / p.G * out.parts, out.dq, out.dQ, out.lddq);
+    if (blockIdx.y == 1u && out.dq) add_shares(bl, p.N, p.G * p.K, p.H / p.G * out.parts, out.dk, out.dK, out.lddk);
+    if (blockIdx.y == 2u && out.db) add_shares(bl, p.N, p.H, out.parts, out.db, out.dbeta, out.lddb);
+    if (blockIdx.y == 2u && out.dg) add_shares(bl, p.N, p.H, out.parts, out.dg, out.ddecay, out.lddg);
+}
+
+namespace {
+
+struct delta_bprop_work {
+    uint32_t* marks;
+    char *chunks, *pairs, *dstates, *dq, *dk, *db, *dg;
+    unsigned parts, waves;
+    size_t bytes;
+};
+
+delta_bprop_work bprop_work_in(void* work, const dbk_deltarule_args& a, const delta_shape& s)
+{
+    delta_bprop_work w = {};
+    char* base = (char*)work;
+    size_t at = 0;
+    auto take = [&](size_t n) { char* p = base + at; at += align16(n); return p; };
+    const size_t A = acc_size(a.dtype), units = delta_blocks(s) * a.H * DELTA_CHUNKS;
+    w.parts = (s.ns + 3) / 4;
+    w.waves = s.ns > 2 ? 4 : s.ns;
+    w.marks = (uint32_t*)take(s.slots * sizeof(uint32_t));
+    w.chunks = take(units * (A == 8 ? sizeof(delta_chunk<double>) : sizeof(delta_chunk<float>)));
+    w.pairs = take(units * (A == 8 ? sizeof(delta_pairs<double>) : sizeof(delta_pairs<float>)));
+    w.dstates = take((size_t)s.slots * a.K * a.H * a.V * A);
+    const size_t shares = a.H / a.G * w.parts;
+    if (shares > 1) {
+        w.dq = take(shares * a.N * a.G * a.K * A);
+        w.dk = take(shares * a.N * a.G * a.K * A);
+    }
+    if (w.parts > 1) {
+        w.db = take((size_t)w.parts * a.N * a.H * A);
+        w.dg = take((size_t)w.parts * a.N * a.H * A);
+    }
+    w.bytes = at;
+    return w;
+}
+
+}  // namespace
+
+size_t delta_bprop_bytes(const dbk_deltarule_args& a) { return bprop_work_in(nullptr, a, delta_shape_of(a)).bytes; }
+
+}  // namespace dbk
+
+using namespace dbk;
+
+extern "C" {
+
+int dbk_deltarule_bprop(dbk_stream_t stream, const dbk_deltarule_args* a, void* work, size_t work_bytes)
+{
+    if (int rc = check_delta(a)) return rc;
+    DBK_CHECK(!a->nregion || a->regions, "ValueError: null regions");
+    DBK_CHECK(!a->N || !a->V || (a->dO && a->dQ && a->dK && a->dV && a->dbeta), "ValueError: null matrix");
+    DBK_CHECK(a->decay || !a->ddecay, "ValueError: no decay, no gradient of it");
+    DBK_CHECK(!a->N || !a->V || a->keep, "ValueError: the states that the forward call kept are needed");
+    DBK_CHECK(a->N <= 1 || (a->lddo >= a->H * a->V && a->lddv >= a->H * a->V && a->lddq >= a->G * a->K && a->lddk >= a->G * a->K && a->lddbeta >= a->H && (!a->ddecay || a->ldddecay >= a->H)),
+              "ValueError: row strides must be at least the number of columns");
+    if (!a->N || !a->V || !a->nregion) { clear_error(); return 0; }
+    const delta_shape s = delta_shape_of(*a);
+    const delta_bprop_work w = bprop_work_in(work, *a, s);
+    DBK_CHECK(work && work_bytes >= w.bytes, "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, w.bytes);
+    DBK_CHECK(grid_fits(delta_blocks(s), 256), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
+    hipStream_t st = as_stream(stream);
+    delta_mark(st, s, a->regions, w.marks);
+    delta_prepare(st, *a, s, w.marks, w.chunks, w.pairs);
+    int rc = 0;
+    with_row_type(a->dtype, [&](auto t) {
+        typedef decltype(t) T;
+        typedef typename acc_of<T>::type A;
+        delta_grads<T> out = {(T*)a->dQ, (T*)a->dK, (T*)a->dV, (A*)a->dbeta, (A*)a->ddecay, a->lddq, a->lddk, a->lddv, a->lddbeta, a->ldddecay,
+                              (A*)w.dq, (A*)w.dk, (A*)w.db, a->ddecay ? (A*)w.dg : nullptr, w.parts, w.waves};
+        with_key_tiles(a->K, [&](auto kt) {
+            k_delta_chain<T, kt.value><<<dim3(s.nregion, divup((size_t)s.H * s.ns, 4)), 256, 0, st>>>(s, a->lddo, a->regions, (const T*)a->Q, (const T*)a->Kk, (const T*)a->dO,
+                                                                                                     (const delta_chunk<A>*)w.chunks, (A)a->scale, (A*)w.dstates);
+            constexpr size_t lds = 4 * sizeof(delta_share<A, kt.value>);
+            if (lds > 65536 && hipFuncSetAttribute((const void*)k_delta_bprop<T, kt.value>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) { rc = 1; return; }
+            k_delta_bprop<T, kt.value><<<dim3((unsigned)delta_blocks(s), divup((size_t)s.H * w.parts * w.waves, 4)), 256, lds, st>>>(
+                s, a->lddo, a->regions, w.marks, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const T*)a->dO, (const delta_chunk<A>*)w.chunks, (const delta_pairs<A>*)w.pairs,
+                (A)a->scale, (const A*)a->keep, (const A*)w.dstates, out);
+        });
+        if (!rc && (w.dq || w.db)) k_delta_add<T><<<dim3((unsigned)delta_blocks(s), 3), 256, 0, st>>>(s, a->regions, w.marks, out);
+    });
+    DBK_CHECK(!rc, "RuntimeError: the device has too little shared memory for a workgroup");
+    DBK_LAUNCH_OK();
+}
+
+}  // extern "C"

@@ -459,3 +459,119 @@ def statescan_step(X, dt, A, B, C, state, D=None, gate=None, dt_bias=None, softp
     a.Y, a.ldy = Y.data_ptr(), _lib.row_stride(Y)
     call("dbk_statescan_step", stream(), ctypes.addressof(a))
     return Y
+
+
+def _delta_shape(K, V, beta, groups):
+    """(heads, key heads, columns of a key, columns of a value) of the delta rule's maps."""
+    for name, t in (("K", K), ("V", V), ("beta", beta)):
+        if not isinstance(t, torch.Tensor) or t.dim() != 2:
+            raise DeepbindError("ValueError: %s must be a matrix" % name)
+    H = beta.shape[1]
+    G = H if groups is None else int(groups)
+    require(H >= 1 and G >= 1 and H % G == 0, "ValueError: the number of heads must be divisible by the number of key heads")
+    require(K.shape[1] >= G and K.shape[1] % G == 0, "ValueError: K must be (rows x key heads * columns of a key)")
+    require(V.shape[1] >= H and V.shape[1] % H == 0, "ValueError: V must be (rows x heads * columns of a value)")
+    if K.shape[1] // G > 128:
+        raise DeepbindError("NotImplementedError: keys of 1 to 128 columns, got %d" % (K.shape[1] // G))
+    return H, G, K.shape[1] // G, V.shape[1] // H
+
+
+def kept_delta(K, V, beta, groups=None):
+    """Empty buffer for the states that deltarule keeps for deltarule_bprop: one block (key x heads*value) per 64 rows."""
+    _, _, key, _ = _delta_shape(K, V, beta, groups)
+    return torch.empty(((V.shape[0] + 63) // 64, key, V.shape[1]), dtype=_lib.wide_dtype(V), device=V.device)
+
+
+def _delta_args(Q, K, V, beta, decay, groups, scale):
+    H, G, key, value = _delta_shape(K, V, beta, groups)
+    code, wide, N, D = _map(V)
+    g = _lib.Arguments()
+    kept, keys, rates = V.dtype, (N, G * key), (N, H)
+    q, ldq = g.rows("Q", Q, keys, kept)
+    k, ldk = g.rows("K", K, keys, kept)
+    v, ldv = g.rows("V", V, (N, D), kept)
+    b, ldb = g.rows("beta", beta, rates, wide)
+    d, ldd = (None, 0) if decay is None else g.rows("decay", decay, rates, wide)
+    scale = key ** -0.5 if scale is None else float(scale)
+    return g, _lib.DeltaRuleArgs(code, N, H, G, key, value, None, 0, q, ldq, k, ldk, v, ldv, b, ldb, d, ldd, scale), wide, N, key, D
+
+
+def deltarule(Q, K, V, beta, regions, decay=None, groups=None, scale=None, state=None, want_state=False, keep=None, out=None):
+    """Gated delta rule along the rows of every region. Every head has a state S (key x value), which a row first multiplies by
+    exp(decay), then corrects by what its key finds in it, u = beta * (v - S^T k) and S = S + k u^T, and its query reads: O = scale * S^T q.
+    V (N x heads*value); beta, decay (N x heads; decay None: nothing decays); Q, K (N x groups*key, up to 128 columns a key): the heads
+    form `groups` equal groups (None: as many as heads), each with its own query and key. scale: key ** -0.5 if None.
+    Keys of length 1 (blocknorm with rms and gamma = key ** -0.5) keep the state bounded for beta up to 2.
+    Rows: float32, float64 or bfloat16; beta, decay and states float32 (float64 beside float64); matrices of rows have row strides of
+    their own. Regions (P x 2) may come in any order and must not overlap; rows in no region are zeros in a new output, and stay as
+    they are in `out`. States start from state (P x key x heads*value), or zeros.
+    keep (optional, from kept_delta): receives the states that deltarule_bprop starts from (without `state` only).
+    Returns (O, last|None): with want_state, last (P x key x heads*value) holds the states behind the regions' last rows."""
+    g, a, wide, N, key, D = _delta_args(Q, K, V, beta, decay, groups, scale)
+    P, a.regions = _row_regions(g, regions)
+    a.nregion = P
+    a.state = g.dense("state", state, (P, key, D), wide)
+    a.keep = g.dense("keep", keep, ((N + 63) // 64, key, D), wide, out=True)
+    require(keep is None or state is None, "ValueError: states are kept for the backward pass of whole sequences, which starts from zeros: no initial state")
+    if out is not None:
+        g.rows("out", out, (N, D), V.dtype, out=True)
+    g.check()
+    O = _rows_out(out, (N, D), V.dtype, V.device)
+    a.O, a.ldo = O.data_ptr(), _lib.row_stride(O)
+    last = None
+    if want_state:
+        last = torch.empty((P, key, D), dtype=wide, device=V.device)
+        a.last = last.data_ptr()
+    at, need = ctypes.addressof(a), ctypes.c_size_t(0)
+    call("dbk_deltarule_workspace", at, 0, ctypes.addressof(need))
+    work, wp = _lib.workspace(need.value, V)
+    call("dbk_deltarule", stream(), at, wp, need.value)
+    return O, last
+
+
+def deltarule_bprop(Q, K, V, beta, regions, keep, dO, decay=None, groups=None, scale=None, out=None):
+    """Gradients (dQ, dK, dV, dbeta, ddecay|None) of deltarule for sequences that start from zero states, from the states that the
+    forward call kept. out (optional): a tuple like the returned one of tensors to write into, None where one is to be made; rows in
+    no region are zeros, or stay as they are in out's."""
+    g, a, wide, N, key, D = _delta_args(Q, K, V, beta, decay, groups, scale)
+    P, a.regions = _row_regions(g, regions)
+    a.nregion = P
+    require(keep is not None, "ValueError: the states that the forward call kept are needed")
+    a.keep = g.dense("keep", keep, ((N + 63) // 64, key, D), wide)
+    a.dO, a.lddo = g.rows("dO", dO, (N, D), V.dtype)
+    given = (None,) * 5 if out is None else tuple(out)
+    require(len(given) == 5, "ValueError: out must be (dQ, dK, dV, dbeta, ddecay)")
+    require(decay is not None or given[4] is None, "ValueError: no decay, no gradient of it")
+    likes = (("dQ", Q), ("dK", K), ("dV", V), ("dbeta", beta), ("ddecay", decay))
+    for (name, like), t in zip(likes, given):
+        if t is not None:
+            g.rows(name, t, tuple(like.shape), like.dtype, out=True)
+    g.check()
+    grads = tuple(None if like is None else _rows_out(t, like.shape, like.dtype, V.device) for (_, like), t in zip(likes, given))
+    ld = _lib.row_stride
+    a.dQ, a.lddq, a.dK, a.lddk, a.dV, a.lddv = grads[0].data_ptr(), ld(grads[0]), grads[1].data_ptr(), ld(grads[1]), grads[2].data_ptr(), ld(grads[2])
+    a.dbeta, a.lddbeta = grads[3].data_ptr(), ld(grads[3])
+    if grads[4] is not None:
+        a.ddecay, a.ldddecay = grads[4].data_ptr(), ld(grads[4])
+    at, need = ctypes.addressof(a), ctypes.c_size_t(0)
+    call("dbk_deltarule_workspace", at, 1, ctypes.addressof(need))
+    work, wp = _lib.workspace(need.value, V)
+    call("dbk_deltarule_bprop", stream(), at, wp, need.value)
+    return grads
+
+
+def deltarule_step(Q, K, V, beta, state, decay=None, groups=None, scale=None, into=None, out=None):
+    """One new row for each of n sequences: O (n x heads*value) from Q, K, V, beta, decay (n rows) and state (n x key x heads*value),
+    arguments otherwise as in deltarule. The state moves on in place, or its successor goes to `into`, which leaves it as it is."""
+    g, a, wide, n, key, D = _delta_args(Q, K, V, beta, decay, groups, scale)
+    require(state is not None, "ValueError: state is needed")
+    into = None if into is state else into
+    a.state = g.dense("state", state, (n, key, D), wide, out=into is None)
+    a.last = a.state if into is None else g.dense("into", into, (n, key, D), wide, out=True)
+    if out is not None:
+        g.rows("out", out, (n, D), V.dtype, out=True)
+    g.check()
+    O = _dense_out(out, (n, D), V.dtype, V.device)
+    a.O, a.ldo = O.data_ptr(), _lib.row_stride(O)
+    call("dbk_deltarule_step", stream(), ctypes.addressof(a))
+    return O

@@ -537,6 +537,34 @@ int dbk_statescan_bprop(dbk_stream_t stream, const dbk_statescan_args* args, voi
 /* One new row for each of N sequences (regions are not looked at): state (N, S, D), its successor goes to `last` (may be `state` itself). */
 int dbk_statescan_step(dbk_stream_t stream, const dbk_statescan_args* args);
 
+/* Gated delta rule along every region's rows. A head's state S (K, V) follows S' = exp(decay) S, u = beta (v - S'^T k), S = S' + k u^T, and its output is
+ * scale S^T q. The H heads form G equal groups, each with its own query and key. K <= 128. */
+typedef struct dbk_deltarule_args {
+    int dtype;
+    size_t N, H, G, K, V;                       /* rows, heads, key heads, columns of a key and of a value */
+    const uint32_t* regions; size_t nregion;
+    const void* Q; size_t ldq;                  /* (N, G * K) rows */
+    const void* Kk; size_t ldk;
+    const void* Vv; size_t ldv;                 /* (N, H * V) rows */
+    const void* beta; size_t ldbeta;            /* (N, H), kept as weights are */
+    const void* decay; size_t lddecay;          /* (N, H), logarithms, kept as weights are; may be NULL (zeros) */
+    double scale;
+    const void* state;                          /* (nregion, K, H * V): the states before the regions' first rows, may be NULL (zeros) */
+    void* O; size_t ldo;                        /* (N, H * V) rows */
+    void* last;                                 /* (nregion, K, H * V): the states behind the last rows, may be NULL */
+    void* keep;                                 /* forward: may be NULL; ceil(N / 64) blocks of (K, H * V): states that the backward pass starts from */
+    const void* dO; size_t lddo;                /* from here on: backward only */
+    void* dQ; size_t lddq; void* dK; size_t lddk; void* dV; size_t lddv;
+    void* dbeta; size_t lddbeta; void* ddecay; size_t ldddecay;      /* ddecay may be NULL */
+} dbk_deltarule_args;
+int dbk_deltarule_args_size(void);              /* sizeof(dbk_deltarule_args) as the library was built */
+int dbk_deltarule_workspace(const dbk_deltarule_args* args, int backward, size_t* work_bytes);
+int dbk_deltarule(dbk_stream_t stream, const dbk_deltarule_args* args, void* work, size_t work_bytes);
+/* Backward for sequences that start from zero states; keep: as the forward call with the same inputs filled it. */
+int dbk_deltarule_bprop(dbk_stream_t stream, const dbk_deltarule_args* args, void* work, size_t work_bytes);
+/* One new row for each of N sequences (regions are not looked at): state (N, K, H * V), its successor goes to `last` (may be `state` itself). */
+int dbk_deltarule_step(dbk_stream_t stream, const dbk_deltarule_args* args);
+
 /* ------------------------------------------------------------------ one whole optimiser step */
 
 /* Everything one step of a group of `nmodel` same-architecture models touches. The parameters, their
