@@ -101,6 +101,10 @@ _SIGNATURES = {
     "dbk_layernorm": [_P, _I, _P, _Z, _P, _P, _Z, _Z, _Z, _D, _P, _Z, _P],
     "dbk_layernorm_bprop_workspace": [_I, _Z, _Z, _Z, _P],
     "dbk_layernorm_bprop": [_P, _I, _P, _Z, _P, _P, _P, _Z, _Z, _Z, _Z, _P, _Z, _P, _P, _P, _Z],
+    "dbk_blocknorm_args_size": [],
+    "dbk_blocknorm": [_P, _P],
+    "dbk_blocknorm_bprop_workspace": [_P, _P],
+    "dbk_blocknorm_bprop": [_P, _P, _P, _Z],
     "dbk_causalconv_workspace": [_I, _Z, _Z, _Z, _Z, _I, _P],
     "dbk_causalconv": [_P, _I, _P, _Z, _P, _P, _Z, _Z, _Z, _P, _Z, _I, _P, _P, _Z, _P, _P, _Z],
     "dbk_causalconv_bprop": [_P, _I, _P, _Z, _P, _P, _Z, _Z, _Z, _P, _Z, _I, _P, _Z, _P, _Z, _P, _P, _P, _Z],
@@ -115,6 +119,8 @@ _SIGNATURES = {
     "dbk_deltarule": [_P, _P, _P, _Z],
     "dbk_deltarule_bprop": [_P, _P, _P, _Z],
     "dbk_deltarule_step": [_P, _P],
+    "dbk_clip_gradients_workspace": [_Z, _P, _Z, _P],
+    "dbk_clip_gradients": [_P, _Z, _P, _Z, _D, _P, _P, _Z],
     "dbk_train_step": [_P, _P],
     "dbk_train_steps": [_P, _Z, _P],
     "dbk_train_step_single_workspace": [_P, _P],
@@ -141,6 +147,23 @@ class TrainStepArgs(ctypes.Structure):
         ("L", _P), ("L_ready", _I),
         ("nfeat", _Z), ("feats", _P),
         ("ycol", _P), ("ldY", _Z),
+    ]
+
+
+class ClipTensor(ctypes.Structure):
+    """dbk_clip_tensor of the public header, field for field."""
+    _fields_ = [("in_", _P), ("out", _P), ("rows", _Z), ("cols", _Z), ("ld_in", _Z), ("ld_out", _Z), ("dtype", _I), ("by_rows", _I)]
+
+
+class BlockNormArgs(ctypes.Structure):
+    """dbk_blocknorm_args of the public header, field for field."""
+    _fields_ = [
+        ("dtype", _I), ("rms", _I), ("norm", _I), ("next", _I), ("n", _Z), ("m", _Z), ("group", _Z), ("eps", _D),
+        ("Y", _P), ("ldy", _Z), ("R", _P), ("ldr", _Z), ("gate", _P), ("ldgate", _Z),
+        ("gamma", _P), ("beta", _P), ("scale", _P), ("next_gamma", _P), ("next_beta", _P),
+        ("O", _P), ("ldo", _Z), ("Z", _P), ("ldz", _Z), ("stats", _P), ("dR", _P), ("lddr", _Z), ("dZ", _P), ("lddz", _Z),
+        ("dY", _P), ("lddy", _Z), ("dR_in", _P), ("lddr_in", _Z), ("dgate", _P), ("lddgate", _Z),
+        ("dgamma", _P), ("dbeta", _P), ("dscale", _P), ("dnext_gamma", _P), ("dnext_beta", _P),
     ]
 
 
@@ -315,6 +338,18 @@ class Arguments(object):
                 if lo < hi2 and lo2 < hi and lo2 != hi2 and not _column_blocks(*((t, t2) if lo <= lo2 else (t2, t))):
                     raise DeepbindError("ValueError: an output shares memory with another argument")
             known = known + [out]
+
+
+def check_many(a):
+    """Arguments.check for long lists: pairs are compared one by one only where memory of some tensors overlaps at all."""
+    both = sorted([(lo, hi, at) for lo, hi, at, _ in a.ins + a.outs if lo != hi])
+    if both and (both[0][2] < 0 or any(at != both[0][2] for _, _, at in both) or both[0][2] != torch.cuda.current_device()):
+        return a.check()
+    end = 0
+    for lo, hi, _ in both:
+        if lo < end:
+            return a.check()
+        end = hi
 
 
 def _column_blocks(a, b):

@@ -1,0 +1,559 @@
+// The norms around a block of layers, with the block's gate and residual, forward and backward: y is what the block makes, r the residual that goes past it.
+//
+//   p = norm(y) gamma + beta,  r' = r + scale p g sigmoid(g),  z = norm(r') next_gamma + next_beta
+//
+// norm(x) = (x - mean) / sqrt(mean((x - mean)^2) + eps) over a chunk of a row, or x / sqrt(mean(x^2) + eps) (rms). Every part may be left out. The second
+// norm is of r' as it is kept, which is what the next block and the backward pass see. With h1 = norm(y), h2 = norm(r') and the gradients dr (of r' from elsewhere) and dz:
+//
+//   t = dr + back(dz next_gamma, h2),  back(q, h) = rstd (q - mean(q) - h mean(q h))  (rms: without mean(q))
+//   dr_in = t,  dp = t scale g sigmoid(g),  dy = back(dp gamma, h1),  dg = t scale p (sigmoid(g) (1 + g (1 - sigmoid(g))))
+//   dgamma = sum dp h1,  dbeta = sum dp,  dscale = sum t p g sigmoid(g),  dnext_gamma = sum dz h2,  dnext_beta = sum dz
+//
+// Bound by memory: forward three maps in and two out, backward five in and three out. A thread holds one vector of 16 bytes of a chunk, a chunk belongs to a power of two
+// of neighbouring lanes (of a wave, or a workgroup of up to 1024), and a workgroup walks down the rows with its chunks' weights, and backward their gradients, in registers.
+#include <type_traits>
+#include "norm_common.h"
+
+namespace dbk {
+
+struct block_shape {
+    unsigned n, nchunk, width, ct_log2, rstep;
+    int rms, norm, next;                         // rms norms; whether y, and r', are normalised
+    size_t ldy, ldr, ldg, ldo, ldz;              // y, r, gate; r' and z
+    size_t lddr, lddz, lddy, lddo, lddg;         // backward: dr and dz in, dy, dr and dgate out (ldo: r')
+};
+
+template <int LANES, typename A> __device__ __forceinline__ void block_sum2(A& u, A& v, A (*lds)[16])
+{
+    constexpr int W = LANES < 64 ? LANES : 64;
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) {
+        u += __shfl_xor(u, o);
+        v += __shfl_xor(v, o);
+    }
+    if constexpr (LANES > 64) {
+        constexpr int WAVES = LANES / 64;
+        __syncthreads();                         // (the words may still be read from the sums before)
+        if ((threadIdx.x & 63) == 0) { lds[0][threadIdx.x >> 6] = u; lds[1][threadIdx.x >> 6] = v; }
+        __syncthreads();
+        u = v = A(0);
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) { u += lds[0][w]; v += lds[1][w]; }
+    }
+}
+
+// mean and reciprocal deviation of a chunk whose values lie in x
+template <int LANES, typename A, int V> __device__ __forceinline__ void chunk_stats(const A (&x)[V], unsigned valid, A inv, A eps, bool rms, A& mean, A& rstd, A (*lds)[16])
+{
+    A a = A(0), b = A(0);
+    if (rms) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) a = fma(x[j], x[j], a);      // (zeros behind the last)
+        block_sum2<LANES>(a, b, lds);
+        mean = A(0);
+        rstd = A(1) / sqrt(a * inv + eps);
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) a += x[j];
+    block_sum2<LANES>(a, b, lds);
+    const A near = a * inv;
+    a = b = A(0);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const A c = j < (int)valid ? x[j] - near : A(0);
+        a = fma(c, c, a);
+        b += c;
+    }
+    block_sum2<LANES>(a, b, lds);
+    norm_stats(near, a * inv, b * inv, eps, mean, rstd);
+}
+
+template <int LANES> constexpr int block_threads() { return LANES > 256 ? LANES : 256; }
+
+// Where a thread's vector lies: LANES lanes of a chunk; up to 256 lanes several chunks or rows share a workgroup.
+template <int LANES, int V> struct block_place {
+    unsigned chunk, lane, valid, first, row;     // first: of the workgroup's rows
+    size_t column;
+    __device__ __forceinline__ block_place(const block_shape& p)
+    {
+        const unsigned unit = threadIdx.x / LANES;
+        lane = threadIdx.x % LANES;
+        chunk = (blockIdx.y << p.ct_log2) + (unit & ((1u << p.ct_log2) - 1u));
+        valid = chunk < p.nchunk && lane * V < p.width ? p.width - lane * V : 0u;
+        first = blockIdx.x * (block_threads<LANES>() / LANES) >> p.ct_log2;
+        row = first + (unit >> p.ct_log2);
+        column = (size_t)chunk * p.width + lane * V;
+    }
+    __device__ __forceinline__ bool leads(const block_shape& p) const { return lane == 0u && chunk < p.nchunk; }
+};
+
+// LANES of more than 64 share a workgroup of their own size with no other chunk: plan_block gives it one row at a time.
+template <typename T, int LANES, bool EXACT>
+__global__ __launch_bounds__(block_threads<LANES>()) void k_block_fprop(block_shape p, const T* __restrict__ Y, const T* __restrict__ R, const T* __restrict__ gate,
+                                                                       const typename acc_of<T>::type* __restrict__ gamma, const typename acc_of<T>::type* __restrict__ beta,
+                                                                       const typename acc_of<T>::type* __restrict__ scale, const typename acc_of<T>::type* __restrict__ ngamma,
+                                                                       const typename acc_of<T>::type* __restrict__ nbeta, typename acc_of<T>::type eps, T* __restrict__ O,
+                                                                       T* __restrict__ Z, typename acc_of<T>::type* __restrict__ stats)
+{
+    typedef typename acc_of<T>::type A;
+    constexpr int V = row_vec<T>::N;
+    __shared__ A lds[2][16];
+    const block_place<LANES, V> at(p);
+    A g1[V], b1[V], sc[V], g2[V], b2[V];
+    load_weights(g1, gamma ? gamma + at.column : nullptr, at.valid, A(1));
+    load_weights(b1, beta ? beta + at.column : nullptr, at.valid, A(0));
+    load_weights(sc, scale ? scale + at.column : nullptr, at.valid, A(1));
+    load_weights(g2, ngamma ? ngamma + at.column : nullptr, at.valid, A(1));
+    load_weights(b2, nbeta ? nbeta + at.column : nullptr, at.valid, A(0));
+    const A inv = A(1) / (A)p.width;
+    const size_t units = (size_t)p.n * p.nchunk;
+    unsigned row = at.row;
+    raw_vec<T, EXACT> ny, nr, ng;
+    auto fetch = [&]() {
+        const unsigned valid = row < p.n ? at.valid : 0u;
+        ny.load(Y + row * p.ldy + at.column, valid);
+        if (R) nr.load(R + row * p.ldr + at.column, valid);
+        if (gate) ng.load(gate + row * p.ldg + at.column, valid);
+    };
+    fetch();
+    // (every lane of a workgroup makes the same number of steps: sums over its waves meet at barriers)
+    for (unsigned left = at.first; left < p.n; left += p.rstep) {
+        const raw_vec<T, EXACT> y = ny, r = nr, g = ng;
+        const unsigned now = row;
+        row += p.rstep;
+        fetch();
+        A x[V], mean = A(0), rstd = A(1);
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[j] = y[j];
+        if (p.norm) chunk_stats<LANES>(x, at.valid, inv, eps, p.rms, mean, rstd, lds);
+        if (stats && now < p.n && at.leads(p)) {
+            stats[(size_t)now * p.nchunk + at.chunk] = mean;
+            stats[units + (size_t)now * p.nchunk + at.chunk] = rstd;
+        }
+        row_vec<T> o;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            A v = fma((x[j] - mean) * rstd, g1[j], b1[j]) * sc[j];
+            if (gate) v *= g[j] * sigmoid_of(g[j]);
+            if (R) v += r[j];
+            x[j] = j < (int)at.valid ? (A)(T)v : A(0);           // (as it is kept)
+            o.v[j] = v;
+        }
+        const bool here = now < p.n;
+        store_vec<EXACT>(o, O + now * p.ldo + at.column, here ? at.valid : 0u);
+        if (!p.next) continue;
+        chunk_stats<LANES>(x, at.valid, inv, eps, p.rms, mean, rstd, lds);
+        if (stats && here && at.leads(p)) {
+            stats[2 * units + (size_t)now * p.nchunk + at.chunk] = mean;
+            stats[3 * units + (size_t)now * p.nchunk + at.chunk] = rstd;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) o.v[j] = fma((x[j] - mean) * rstd, g2[j], b2[j]);
+        store_vec<EXACT>(o, Z + now * p.ldz + at.column, here ? at.valid : 0u);
+    }
+}
+
+// The weights' gradients of a workgroup's rows are added in registers, its row lanes in LDS at the end, in a fixed order: part[blockIdx.x][5][m].
+template <typename T, int LANES, bool EXACT>
+__global__ __launch_bounds__(block_threads<LANES>()) void k_block_bprop(block_shape p, const T* __restrict__ Y, const T* __restrict__ O, const T* __restrict__ gate,
+                                                                       const typename acc_of<T>::type* __restrict__ gamma, const typename acc_of<T>::type* __restrict__ beta,
+                                                                       const typename acc_of<T>::type* __restrict__ scale, const typename acc_of<T>::type* __restrict__ ngamma,
+                                                                       const typename acc_of<T>::type* __restrict__ stats, const T* __restrict__ dR, const T* __restrict__ dZ,
+                                                                       T* __restrict__ dY, T* __restrict__ dO, T* __restrict__ dgate, typename acc_of<T>::type* __restrict__ part)
+{
+    typedef typename acc_of<T>::type A;
+    constexpr int V = row_vec<T>::N;
+    __shared__ A lds[2][16];
+    __shared__ A strips[LANES < 256 ? 256 : 1][V + 1];
+    const block_place<LANES, V> at(p);
+    A g1[V], b1[V], sc[V], g2[V], sums[5][V];
+    load_weights(g1, gamma ? gamma + at.column : nullptr, at.valid, A(1));
+    load_weights(b1, beta ? beta + at.column : nullptr, at.valid, A(0));
+    load_weights(sc, scale ? scale + at.column : nullptr, at.valid, A(1));
+    load_weights(g2, ngamma ? ngamma + at.column : nullptr, at.valid, A(1));
+#pragma unroll
+    for (int i = 0; i < 5; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) sums[i][j] = A(0);
+    const A inv = A(1) / (A)p.width;
+    const size_t units = (size_t)p.n * p.nchunk;
+    unsigned row = at.row;
+    raw_vec<T, EXACT> ny, no, ng, nd, nz;
+    A n1 = 0, n2 = 0, n3 = 0, n4 = 0;
+    auto fetch = [&]() {
+        const bool here = row < p.n && at.chunk < p.nchunk;
+        const unsigned valid = here ? at.valid : 0u;
+        const size_t u = (size_t)row * p.nchunk + at.chunk;
+        ny.load(Y + row * p.ldy + at.column, valid);
+        if (gate) ng.load(gate + row * p.ldg + at.column, valid);
+        nd.load(dR + row * p.lddr + at.column, dR ? valid : 0u);
+        if (p.norm) { n1 = here ? stats[u] : A(0); n2 = here ? stats[units + u] : A(0); }
+        if (p.next) {
+            no.load(O + row * p.ldo + at.column, valid);
+            nz.load(dZ + row * p.lddz + at.column, valid);
+            n3 = here ? stats[2 * units + u] : A(0);
+            n4 = here ? stats[3 * units + u] : A(0);
+        }
+    };
+    fetch();
+    for (unsigned left = at.first; left < p.n; left += p.rstep) {
+        const raw_vec<T, EXACT> y = ny, o = no, g = ng, d = nd, z = nz;
+        const A mean1 = n1, rstd1 = p.norm ? n2 : A(1), mean2 = n3, rstd2 = n4;
+        const unsigned now = row;
+        row += p.rstep;
+        fetch();
+        A t[V], a = A(0), b = A(0);
+        if (p.next) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const A h = (o[j] - mean2) * rstd2, q = z[j] * g2[j];
+                sums[3][j] = fma(z[j], h, sums[3][j]);
+                sums[4][j] += z[j];
+                a += q;
+                b = fma(q, h, b);
+            }
+            block_sum2<LANES>(a, b, lds);
+            a = p.rms ? A(0) : a * inv;
+            b *= inv;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            t[j] = d[j];
+            if (p.next) t[j] += rstd2 * (fma(z[j], g2[j], -a) - (o[j] - mean2) * rstd2 * b);
+        }
+        const bool here = now < p.n;
+        row_vec<T> out;
+        if (dO) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) out.v[j] = t[j];
+            store_vec<EXACT>(out, dO + now * p.lddo + at.column, here ? at.valid : 0u);
+        }
+        A q[V];
+        a = b = A(0);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const bool real = EXACT ? at.valid != 0u : j < (int)at.valid;
+            const A h = (y[j] - mean1) * rstd1, pv = fma(h, g1[j], b1[j]);
+            A act = A(1);
+            if (gate) {
+                const A e = sigmoid_of(g[j]);
+                act = g[j] * e;
+                out.v[j] = t[j] * sc[j] * pv * (e * fma(g[j], A(1) - e, A(1)));
+            }
+            if (!real || !here) { q[j] = A(0); continue; }
+            const A dp = t[j] * sc[j] * act;
+            sums[0][j] = fma(dp, h, sums[0][j]);
+            sums[1][j] += dp;
+            sums[2][j] = fma(t[j] * pv, act, sums[2][j]);
+            q[j] = dp * g1[j];
+            a += q[j];
+            b = fma(q[j], h, b);
+        }
+        if (gate) store_vec<EXACT>(out, dgate + now * p.lddg + at.column, here ? at.valid : 0u);
+        if (p.norm) {
+            block_sum2<LANES>(a, b, lds);
+            a = p.rms ? A(0) : a * inv;
+            b *= inv;
+#pragma unroll
+            for (int j = 0; j < V; ++j) out.v[j] = rstd1 * (q[j] - a - (y[j] - mean1) * rstd1 * b);
+        } else
+#pragma unroll
+            for (int j = 0; j < V; ++j) out.v[j] = q[j];
+        store_vec<EXACT>(out, dY + now * p.lddy + at.column, here ? at.valid : 0u);
+    }
+    if (!part) return;
+    const size_t m = (size_t)p.nchunk * p.width;
+    const unsigned across = LANES << p.ct_log2;                 // threads of one row lane
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+        if constexpr (LANES < 256) {
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < V; ++j) strips[threadIdx.x][j] = sums[i][j];
+            sum_strips(strips, across, V);
+        }
+        if (threadIdx.x >= across || !at.valid) continue;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < (int)at.valid) part[((size_t)blockIdx.x * 5u + i) * m + at.column + j] = LANES < 256 ? strips[LANES < 256 ? threadIdx.x : 0][j] : sums[i][j];
+    }
+}
+
+// Chunks too wide for a workgroup's threads: a workgroup per chunk goes over it once per sum (from the caches after the first time).
+constexpr int WIDE = 1024;
+
+template <typename T, typename F> __device__ __forceinline__ void wide_stats(unsigned width, typename acc_of<T>::type eps, bool rms, typename acc_of<T>::type& mean,
+                                                                            typename acc_of<T>::type& rstd, typename acc_of<T>::type (*lds)[16], F value)
+{
+    typedef typename acc_of<T>::type A;
+    const A inv = A(1) / (A)width;
+    A a = A(0), b = A(0);
+    for (unsigned c = threadIdx.x; c < width; c += WIDE) { const A x = value(c); a += rms ? x * x : x; }
+    block_sum2<WIDE>(a, b, lds);
+    if (rms) { mean = A(0); rstd = A(1) / sqrt(a * inv + eps); return; }
+    const A near = a * inv;
+    a = b = A(0);
+    for (unsigned c = threadIdx.x; c < width; c += WIDE) { const A x = value(c) - near; a = fma(x, x, a); b += x; }
+    block_sum2<WIDE>(a, b, lds);
+    norm_stats(near, a * inv, b * inv, eps, mean, rstd);
+}
+
+template <typename T>
+__global__ __launch_bounds__(WIDE) void k_block_fprop_wide(block_shape p, const T* __restrict__ Y, const T* __restrict__ R, const T* __restrict__ gate,
+                                                           const typename acc_of<T>::type* __restrict__ gamma, const typename acc_of<T>::type* __restrict__ beta,
+                                                           const typename acc_of<T>::type* __restrict__ scale, const typename acc_of<T>::type* __restrict__ ngamma,
+                                                           const typename acc_of<T>::type* __restrict__ nbeta, typename acc_of<T>::type eps, T* O, T* __restrict__ Z,
+                                                           typename acc_of<T>::type* __restrict__ stats)
+{
+    typedef typename acc_of<T>::type A;
+    __shared__ A lds[2][16];
+    const size_t units = (size_t)p.n * p.nchunk;
+    for (size_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const size_t row = u / p.nchunk, col = u % p.nchunk * p.width;
+        const T *y = Y + row * p.ldy + col, *r = R ? R + row * p.ldr + col : nullptr, *g = gate ? gate + row * p.ldg + col : nullptr;
+        T *o = O + row * p.ldo + col, *z = Z ? Z + row * p.ldz + col : nullptr;
+        A mean = A(0), rstd = A(1);
+        if (p.norm) wide_stats<T>(p.width, eps, p.rms, mean, rstd, lds, [&](unsigned c) { return (A)y[c]; });
+        for (unsigned c = threadIdx.x; c < p.width; c += WIDE) {
+            A v = fma(((A)y[c] - mean) * rstd, gamma ? gamma[col + c] : A(1), beta ? beta[col + c] : A(0)) * (scale ? scale[col + c] : A(1));
+            if (g) v *= (A)g[c] * sigmoid_of((A)g[c]);
+            if (r) v += (A)r[c];
+            o[c] = (T)v;
+        }
+        if (stats && threadIdx.x == 0) { stats[u] = mean; stats[units + u] = rstd; }
+        if (!p.next) continue;
+        // (a thread reads the values of r' that it wrote itself)
+        wide_stats<T>(p.width, eps, p.rms, mean, rstd, lds, [&](unsigned c) { return (A)o[c]; });
+        for (unsigned c = threadIdx.x; c < p.width; c += WIDE)
+            z[c] = (T)fma(((A)o[c] - mean) * rstd, ngamma ? ngamma[col + c] : A(1), nbeta ? nbeta[col + c] : A(0));
+        if (stats && threadIdx.x == 0) { stats[2 * units + u] = mean; stats[3 * units + u] = rstd; }
+    }
+}
+
+// What one value of r' and y sends back, given its chunk's sums: t and what the weights' gradients take
+template <typename A> struct block_value {
+    A t, h1, h2, p, act, open;                   // open: the gate's derivative
+    __device__ __forceinline__ void of(const block_shape& s, A y, A o, A g, bool gated, A d, A z, A g1, A b1, A g2, A mean1, A rstd1, A mean2, A rstd2, A a, A b)
+    {
+        h1 = (y - mean1) * rstd1;
+        h2 = s.next ? (o - mean2) * rstd2 : A(0);
+        t = d;
+        if (s.next) t += rstd2 * (fma(z, g2, -a) - h2 * b);
+        p = fma(h1, g1, b1);
+        act = open = A(1);
+        if (gated) { const A e = sigmoid_of(g); act = g * e; open = e * fma(g, A(1) - e, A(1)); }
+    }
+};
+
+template <typename T>
+__global__ __launch_bounds__(WIDE) void k_block_bprop_wide(block_shape p, const T* __restrict__ Y, const T* __restrict__ O, const T* __restrict__ gate,
+                                                           const typename acc_of<T>::type* __restrict__ gamma, const typename acc_of<T>::type* __restrict__ beta,
+                                                           const typename acc_of<T>::type* __restrict__ scale, const typename acc_of<T>::type* __restrict__ ngamma,
+                                                           const typename acc_of<T>::type* __restrict__ stats, const T* __restrict__ dR, const T* __restrict__ dZ, T* __restrict__ dY,
+                                                           T* __restrict__ dO, T* __restrict__ dgate, typename acc_of<T>::type* __restrict__ part)
+{
+    typedef typename acc_of<T>::type A;
+    __shared__ A lds[2][16];
+    const size_t units = (size_t)p.n * p.nchunk, m = (size_t)p.nchunk * p.width;
+    const A inv = A(1) / (A)p.width;
+    // chunk by chunk, each workgroup rows of its own: a thread's columns are always the same, and it adds its rows to its own partial sums
+    for (unsigned chunk = 0; chunk < p.nchunk; ++chunk) {
+        const size_t col = (size_t)chunk * p.width;
+        bool before = false;
+        for (size_t row = blockIdx.x; row < p.n; row += gridDim.x) {
+            const size_t u = row * p.nchunk + chunk;
+            const T *y = Y + row * p.ldy + col, *o = p.next ? O + row * p.ldo + col : nullptr, *g = gate ? gate + row * p.ldg + col : nullptr;
+            const T *d = dR ? dR + row * p.lddr + col : nullptr, *z = p.next ? dZ + row * p.lddz + col : nullptr;
+            const A mean1 = p.norm ? stats[u] : A(0), rstd1 = p.norm ? stats[units + u] : A(1), mean2 = p.next ? stats[2 * units + u] : A(0), rstd2 = p.next ? stats[3 * units + u] : A(0);
+            A a = A(0), b = A(0), a1 = A(0), b1 = A(0);
+            if (p.next) {
+                for (unsigned c = threadIdx.x; c < p.width; c += WIDE) {
+                    const A q = (A)z[c] * (ngamma ? ngamma[col + c] : A(1));
+                    a += q;
+                    b = fma(q, ((A)o[c] - mean2) * rstd2, b);
+                }
+                block_sum2<WIDE>(a, b, lds);
+                a = p.rms ? A(0) : a * inv;
+                b *= inv;
+            }
+            auto value = [&](unsigned c) {
+                block_value<A> v;
+                v.of(p, (A)y[c], p.next ? (A)o[c] : A(0), g ? (A)g[c] : A(0), g != nullptr, d ? (A)d[c] : A(0), p.next ? (A)z[c] : A(0), gamma ? gamma[col + c] : A(1),
+                     beta ? beta[col + c] : A(0), ngamma ? ngamma[col + c] : A(1), mean1, rstd1, mean2, rstd2, a, b);
+                return v;
+            };
+            if (p.norm) {
+                for (unsigned c = threadIdx.x; c < p.width; c += WIDE) {
+                    const block_value<A> v = value(c);
+                    const A q = v.t * (scale ? scale[col + c] : A(1)) * v.act * (gamma ? gamma[col + c] : A(1));
+                    a1 += q;
+                    b1 = fma(q, v.h1, b1);
+                }
+                block_sum2<WIDE>(a1, b1, lds);
+                a1 = p.rms ? A(0) : a1 * inv;
+                b1 *= inv;
+            }
+            for (unsigned c = threadIdx.x; c < p.width; c += WIDE) {
+                const block_value<A> v = value(c);
+                const A ts = v.t * (scale ? scale[col + c] : A(1)), dp = ts * v.act, q = dp * (gamma ? gamma[col + c] : A(1));
+                dY[row * p.lddy + col + c] = (T)(p.norm ? rstd1 * (q - a1 - v.h1 * b1) : q);
+                if (dO) dO[row * p.lddo + col + c] = (T)v.t;
+                if (g) dgate[row * p.lddg + col + c] = (T)(ts * v.p * v.open);
+                if (!part) continue;
+                A* s = part + (size_t)blockIdx.x * 5u * m + col + c;
+                const A zc = p.next ? (A)z[c] : A(0), more[5] = {dp * v.h1, dp, v.t * v.p * v.act, zc * v.h2, zc};
+#pragma unroll
+                for (int i = 0; i < 5; ++i) s[i * m] = before ? s[i * m] + more[i] : more[i];
+            }
+            before = true;
+        }
+    }
+}
+
+namespace {
+
+struct block_plan {
+    int lanes;                                   // 0: the wide kernels
+    unsigned gx, gy;
+    block_shape shape;
+};
+
+constexpr unsigned BLOCK_WAVES = 8192;           // forward: waves that walk the rows, eight per SIMD
+constexpr unsigned BLOCK_WAVES_BACK = 3072;      // backward: three per SIMD, whose partial sums are added up afterwards
+constexpr size_t WIDE_WGS = 512;
+
+block_plan plan_block(const dbk_blocknorm_args& a, bool backward)
+{
+    block_plan p = {};
+    const size_t V = 16 / row_size(a.dtype), vecs = (a.group + V - 1) / V, nchunk = a.m / a.group;
+    if (vecs <= 1024) { p.lanes = 1; while ((size_t)p.lanes < vecs) p.lanes *= 2; if (p.lanes == 128) p.lanes = 256; }
+    const unsigned threads = p.lanes > 256 ? p.lanes : 256u;
+    const unsigned ct = p.lanes && p.lanes <= 256 ? chunks_side_by_side((unsigned)p.lanes, nchunk) : 0u;
+    const unsigned rt = p.lanes ? (threads / p.lanes) >> ct : 1u;
+    p.gy = p.lanes ? divup(nchunk, size_t(1) << ct) : 1u;
+    const unsigned wgs = (backward ? BLOCK_WAVES_BACK : BLOCK_WAVES) / (threads / 64u), most = wgs / p.gy ? wgs / p.gy : 1u;
+    p.gx = divup(a.n, rt);
+    if (p.gx > most) p.gx = most;
+    if (!p.lanes) p.gx = (unsigned)(a.n < WIDE_WGS ? a.n : WIDE_WGS);
+    block_shape& s = p.shape;
+    s.n = (unsigned)a.n;
+    s.nchunk = (unsigned)nchunk;
+    s.width = (unsigned)a.group;
+    s.ct_log2 = ct;
+    s.rstep = p.gx * rt;
+    s.rms = a.rms;
+    s.norm = a.norm;
+    s.next = a.next;
+    s.ldy = a.ldy; s.ldr = a.ldr; s.ldg = a.ldgate; s.ldo = a.ldo; s.ldz = a.ldz;
+    s.lddr = a.lddr; s.lddz = a.lddz; s.lddy = a.lddy; s.lddo = a.lddr_in; s.lddg = a.lddgate;
+    return p;
+}
+
+template <typename F> bool block_layout(int lanes, bool exact, F f)
+{
+#define DBK_BLOCK_CASE(L)                                                        \
+    if (lanes == L) {                                                            \
+        if (exact) f(std::integral_constant<int, L>(), std::true_type());        \
+        else f(std::integral_constant<int, L>(), std::false_type());             \
+        return true;                                                             \
+    }
+    DBK_BLOCK_CASE(1) DBK_BLOCK_CASE(2) DBK_BLOCK_CASE(4) DBK_BLOCK_CASE(8) DBK_BLOCK_CASE(16) DBK_BLOCK_CASE(32) DBK_BLOCK_CASE(64)
+    DBK_BLOCK_CASE(256) DBK_BLOCK_CASE(512) DBK_BLOCK_CASE(1024)
+#undef DBK_BLOCK_CASE
+    return false;
+}
+
+int check_block(const dbk_blocknorm_args* a)
+{
+    DBK_CHECK(a, "ValueError: null argument block");
+    DBK_ROW_DTYPE_OK(a->dtype);
+    DBK_CHECK(a->group >= 1 && a->m % a->group == 0, "ValueError: the number of columns must be divisible by the chunk's");
+    DBK_CHECK(a->n < (size_t(1) << 31) && a->m < (size_t(1) << 31), "ValueError: matrix too large (%zu x %zu)", a->n, a->m);
+    DBK_CHECK(a->norm || (!a->gamma && !a->beta), "ValueError: weights of a norm that is left out");
+    DBK_CHECK(a->next || (!a->next_gamma && !a->next_beta), "ValueError: weights of a norm that is left out");
+    DBK_CHECK(!a->n || !a->m || a->Y, "ValueError: null matrix");
+    DBK_CHECK(!a->m || plan_block(*a, false).gy <= 65535u, "ValueError: too many chunks");
+    return 0;
+}
+
+bool stride_ok(const dbk_blocknorm_args& a, const void* p, size_t ld) { return !p || a.n <= 1 || ld >= a.m; }
+
+size_t block_work(const dbk_blocknorm_args& a) { return a.n && a.m ? (size_t)plan_block(a, true).gx * 5 * a.m * acc_size(a.dtype) : 0; }
+
+}  // namespace
+}  // namespace dbk
+
+using namespace dbk;
+
+extern "C" {
+
+int dbk_blocknorm_args_size(void) { return (int)sizeof(dbk_blocknorm_args); }
+
+int dbk_blocknorm(dbk_stream_t stream, const dbk_blocknorm_args* a)
+{
+    if (int rc = check_block(a)) return rc;
+    const bool some = a->n && a->m;
+    DBK_CHECK(!some || (a->O && (!a->next || a->Z)), "ValueError: null matrix");
+    DBK_CHECK(stride_ok(*a, a->Y, a->ldy) && stride_ok(*a, a->R, a->ldr) && stride_ok(*a, a->gate, a->ldgate) && stride_ok(*a, a->O, a->ldo) && stride_ok(*a, a->Z, a->ldz),
+              "ValueError: row strides must be at least the number of columns");
+    if (!some) { clear_error(); return 0; }
+    const block_plan p = plan_block(*a, false);
+    hipStream_t st = as_stream(stream);
+    with_row_type(a->dtype, [&](auto t) {
+        typedef decltype(t) T;
+        typedef typename acc_of<T>::type A;
+        if (!block_layout(p.lanes, a->group % row_vec<T>::N == 0, [&](auto lanes, auto exact) {
+                k_block_fprop<T, lanes.value, exact.value><<<dim3(p.gx, p.gy), block_threads<lanes.value>(), 0, st>>>(
+                    p.shape, (const T*)a->Y, (const T*)a->R, (const T*)a->gate, (const A*)a->gamma, (const A*)a->beta, (const A*)a->scale, (const A*)a->next_gamma,
+                    (const A*)a->next_beta, (A)a->eps, (T*)a->O, (T*)a->Z, (A*)a->stats);
+            })) {
+            const size_t units = a->n * (a->m / a->group);
+            k_block_fprop_wide<T><<<(unsigned)(units < WIDE_WGS ? units : WIDE_WGS), WIDE, 0, st>>>(
+                p.shape, (const T*)a->Y, (const T*)a->R, (const T*)a->gate, (const A*)a->gamma, (const A*)a->beta, (const A*)a->scale, (const A*)a->next_gamma,
+                (const A*)a->next_beta, (A)a->eps, (T*)a->O, a->next ? (T*)a->Z : nullptr, (A*)a->stats);
+        }
+    });
+    DBK_LAUNCH_OK();
+}
+
+int dbk_blocknorm_bprop_workspace(const dbk_blocknorm_args* a, size_t* work_bytes)
+{
+    if (int rc = check_block(a)) return rc;
+    DBK_CHECK(work_bytes, "ValueError: null result");
+    *work_bytes = block_work(*a);
+    clear_error();
+    return 0;
+}
+
+int dbk_blocknorm_bprop(dbk_stream_t stream, const dbk_blocknorm_args* a, void* work, size_t work_bytes)
+{
+    if (int rc = check_block(a)) return rc;
+    const bool some = a->n && a->m, weights = a->dgamma || a->dbeta || a->dscale || a->dnext_gamma || a->dnext_beta;
+    DBK_CHECK(!some || (a->dY && (a->dR || a->next) && (!a->next || (a->O && a->dZ)) && (!(a->norm || a->next) || a->stats) && (!a->gate || a->dgate)), "ValueError: null matrix");
+    DBK_CHECK(stride_ok(*a, a->Y, a->ldy) && stride_ok(*a, a->gate, a->ldgate) && stride_ok(*a, a->O, a->ldo) && stride_ok(*a, a->dR, a->lddr) && stride_ok(*a, a->dZ, a->lddz) &&
+                  stride_ok(*a, a->dY, a->lddy) && stride_ok(*a, a->dR_in, a->lddr_in) && stride_ok(*a, a->dgate, a->lddgate),
+              "ValueError: row strides must be at least the number of columns");
+    const size_t need = weights ? block_work(*a) : 0;
+    DBK_CHECK(!need || (work && work_bytes >= need), "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, need);
+    hipStream_t st = as_stream(stream);
+    const block_plan p = some ? plan_block(*a, true) : block_plan();
+    if (some)
+        with_row_type(a->dtype, [&](auto t) {
+            typedef decltype(t) T;
+            typedef typename acc_of<T>::type A;
+            A* part = weights ? (A*)work : nullptr;
+            if (!block_layout(p.lanes, a->group % row_vec<T>::N == 0, [&](auto lanes, auto exact) {
+                    k_block_bprop<T, lanes.value, exact.value><<<dim3(p.gx, p.gy), block_threads<lanes.value>(), 0, st>>>(
+                        p.shape, (const T*)a->Y, (const T*)a->O, (const T*)a->gate, (const A*)a->gamma, (const A*)a->beta, (const A*)a->scale, (const A*)a->next_gamma,
+                        (const A*)a->stats, (const T*)a->dR, (const T*)a->dZ, (T*)a->dY, (T*)a->dR_in, (T*)a->dgate, part);
+                }))
+                k_block_bprop_wide<T><<<p.gx, WIDE, 0, st>>>(p.shape, (const T*)a->Y, (const T*)a->O, (const T*)a->gate, (const A*)a->gamma, (const A*)a->beta, (const A*)a->scale,
+                                                             (const A*)a->next_gamma, (const A*)a->stats, (const T*)a->dR, (const T*)a->dZ, (T*)a->dY, (T*)a->dR_in, (T*)a->dgate, part);
+        });
+    // (sums of no rows: zeros)
+    if (weights) sum_partials(st, a->dtype, work, some ? p.gx : 0, {a->m, a->m, a->m, a->m, a->m}, {a->dgamma, a->dbeta, a->dscale, a->dnext_gamma, a->dnext_beta});
+    DBK_LAUNCH_OK();
+}
+
+}  // extern "C"

@@ -9,7 +9,7 @@
 // 151 us (749 MB), backward 239 us (1.12 GB); 50021 rows of 64 chunks of 16 floats 79 and 140 us (410 and 615 MB). Chunks too wide for the registers are
 // read three times either way, from the caches where they hold them: 5003 x 20001 floats 337 us forward, 900 both ways (0.8 and 1.6 GB).
 #include <type_traits>
-#include "rows_common.h"
+#include "norm_common.h"
 
 namespace dbk {
 
@@ -51,16 +51,6 @@ template <int LANES, typename A> __device__ __forceinline__ void lanes_sum2(A& u
         u = (lds[0] + lds[1]) + (lds[2] + lds[3]);
         v = (lds[4] + lds[5]) + (lds[6] + lds[7]);
     }
-}
-
-// A chunk's mean and reciprocal deviation from its sum's mean `near`, the mean of the squared distances to that and the mean of the distances. The sum's
-// roundings make `near` miss the mean by a few units in its last place, which is all there is where the values are equal, and more than their
-// spread where they lie far from zero: the distances, of the spread's size, say by how much.
-template <typename A> __device__ __forceinline__ void norm_stats(A near, A sq, A rest, A eps, A& mean, A& rstd)
-{
-    const A var = fma(-rest, rest, sq);
-    mean = near + rest;
-    rstd = A(1) / sqrt((var < A(0) ? A(0) : var) + eps);        // (a NaN stays)
 }
 
 // A row's values come while the row before it is worked on, and stay as they lie in memory: for bfloat16 half the registers of what is
@@ -356,8 +346,9 @@ __global__ __launch_bounds__(256) void k_norm_wgrad_wide(norm_shape p, size_t ld
 
 // out[c] = sum over units of part[unit][c] in a fixed order: 16 columns x 64 groups of units per workgroup, each thread its
 // group's units one after another, the groups' sums through LDS.
+template <typename A> struct sum_outputs { A* out[SUM_OUTPUTS]; size_t n[SUM_OUTPUTS]; };
 template <typename A>
-__global__ __launch_bounds__(1024) void k_sum_partials(const A* __restrict__ part, size_t units, size_t first, size_t ncol, size_t n0, A* out0, size_t n1, A* out1, A* out2)
+__global__ __launch_bounds__(1024) void k_sum_partials(const A* __restrict__ part, size_t units, size_t first, size_t ncol, sum_outputs<A> to)
 {
     __shared__ A lds[64][17];
     const unsigned x = threadIdx.x & 15u, y = threadIdx.x >> 4;
@@ -373,23 +364,40 @@ __global__ __launch_bounds__(1024) void k_sum_partials(const A* __restrict__ par
         __syncthreads();
     }
     if (y == 0 && c < ncol) {
-        A* out = c < n0 ? out0 : c < n0 + n1 ? out1 : out2;
-        if (out) out[c < n0 ? c : c < n0 + n1 ? c - n0 : c - n0 - n1] = lds[0][x];
+        size_t at = c;
+#pragma unroll
+        for (int i = 0; i < SUM_OUTPUTS; ++i) {
+            if (at < to.n[i]) {
+                if (to.out[i]) to.out[i][at] = lds[0][x];
+                break;
+            }
+            at -= to.n[i];
+        }
     }
+}
+
+int sum_partials(hipStream_t st, int dtype, const void* part, size_t units, const size_t (&n)[SUM_OUTPUTS], void* const (&out)[SUM_OUTPUTS])
+{
+    size_t ncol = 0;
+    for (size_t c : n) ncol += c;
+    constexpr size_t MOST = size_t(1) << 25;     // columns of a launch (grid_fits)
+    for (size_t first = 0; first < ncol; first += MOST) {
+        const unsigned wgs = divup(ncol - first < MOST ? ncol - first : MOST, 16);
+        auto launch = [&](auto a) {
+            typedef decltype(a) A;
+            sum_outputs<A> to;
+            for (int i = 0; i < SUM_OUTPUTS; ++i) { to.out[i] = (A*)out[i]; to.n[i] = n[i]; }
+            k_sum_partials<A><<<wgs, 1024, 0, st>>>((const A*)part, units, first, ncol, to);
+        };
+        if (dtype == DBK_F64) launch(double());
+        else launch(float());
+    }
+    return 0;
 }
 
 int sum_partials(hipStream_t st, int dtype, const void* part, size_t units, size_t n0, void* out0, size_t n1, void* out1, size_t n2, void* out2)
 {
-    const size_t ncol = n0 + n1 + n2;
-    constexpr size_t MOST = size_t(1) << 25;     // columns of a launch (grid_fits)
-    for (size_t first = 0; first < ncol; first += MOST) {
-        const unsigned wgs = divup(ncol - first < MOST ? ncol - first : MOST, 16);
-        if (dtype == DBK_F64)
-            k_sum_partials<double><<<wgs, 1024, 0, st>>>((const double*)part, units, first, ncol, n0, (double*)out0, n1, (double*)out1, (double*)out2);
-        else
-            k_sum_partials<float><<<wgs, 1024, 0, st>>>((const float*)part, units, first, ncol, n0, (float*)out0, n1, (float*)out1, (float*)out2);
-    }
-    return 0;
+    return sum_partials(st, dtype, part, units, {n0, n1, n2, 0, 0}, {out0, out1, out2, nullptr, nullptr});
 }
 
 namespace {
@@ -414,16 +422,7 @@ norm_plan plan_norm(int dtype, size_t n, size_t m, size_t group)
     else if (vecs <= 256) p.nv = (int)((vecs + 63) / 64);
     else if (vecs <= 256 * NORM_NV_BLOCK) { p.lanes = 256; p.nv = vecs <= 512 ? 2 : NORM_NV_BLOCK; }
     else p.lanes = 0;
-    // Chunks side by side: the power of two that costs least, counting the lanes whose chunk does not exist and, against short pieces of
-    // rows, 128 bytes more for every piece.
-    unsigned best = 0;
-    double least = 1e300;
-    for (unsigned c = 0; p.lanes && (unsigned)p.lanes << c <= 256u; ++c) {
-        const size_t tiles = (nchunk + (size_t(1) << c) - 1) >> c;
-        const double cost = (double)(tiles << c) * (1.0 + 128.0 / (double)((size_t)p.lanes * 16 << c));
-        if (cost <= least) { least = cost; best = c; }
-        if (tiles == 1) break;
-    }
+    const unsigned best = chunks_side_by_side((unsigned)p.lanes, nchunk);
     p.ct_log2 = best;
     const unsigned rt = p.lanes ? (256u / p.lanes) >> best : 1u;
     p.gy = p.lanes ? divup(nchunk, size_t(1) << best) : 1u;

@@ -182,8 +182,9 @@ __device__ __forceinline__ bool slot_segment(const uint32_t* regions, unsigned n
 }
 inline size_t segment_slots(size_t N, size_t L) { return (N + L - 1) / L; }
 
-// Ordered sum over units of part[unit][ncol]: columns [0, n0) go to out0, the next n1 to out1, the next n2 to out2 (null:
-// dropped). Defined in layernorm.hip.
+// Ordered sum over units of part[unit][ncol]: columns [0, n[0]) go to out[0], the next n[1] to out[1] and so on (null: dropped). Defined in layernorm.hip.
+constexpr int SUM_OUTPUTS = 5;
+int sum_partials(hipStream_t st, int dtype, const void* part, size_t units, const size_t (&n)[SUM_OUTPUTS], void* const (&out)[SUM_OUTPUTS]);
 int sum_partials(hipStream_t st, int dtype, const void* part, size_t units, size_t n0, void* out0, size_t n1, void* out1, size_t n2, void* out2);
 
 }  // namespace dbk

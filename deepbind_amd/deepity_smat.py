@@ -2,11 +2,13 @@
 conventions as the reference's shim (reference: code/libs/deepity/deepity/_ext/deepity_smat.py:77-254),
 plus the fused scoring head. All arithmetic happens in libdeepbind_hip.so on the current HIP stream.
 """
+import ctypes
 import numbers
 
 import numpy as np
 import torch
 
+from . import _lib
 from ._lib import LOSS_KIND, call, dtype_code, ptr, require, stream
 
 _rng_seed = 0
@@ -269,6 +271,54 @@ def l1_decay(P, decay, dP):
     """dP += sign(P) * decay, elementwise over a whole flat parameter vector (decay: one coefficient per element)."""
     require(P.shape == dP.shape == decay.shape and P.dtype == dP.dtype == decay.dtype, "ValueError: P, decay and dP must match")
     call("dbk_l1_decay", stream(), dtype_code(P), ptr(P), ptr(decay), ptr(dP), P.numel())
+
+
+def clip_gradients(grads, max_norm, nblock=1, by_rows=None, out=None):
+    """The 2-norm of all tensors of the list `grads` together, and the gradients times max_norm / norm where that is over max_norm, in
+    place or into the tensors of the list `out`. With nblock > 1 every tensor holds the gradients of that many models side by side, as equal
+    blocks of its columns, or of its rows where by_rows[i] is true (as the dense layers' weights have them), and every model's
+    gradients have their own norm.
+    Tensors: float32, float64 or bfloat16, mixed as they come; matrices may have row strides of their own, others (nblock 1 only) are
+    contiguous. Squares are added in double precision, in a fixed order. A norm that is NaN leaves its gradients as they are; an infinite one
+    leaves zeros, and NaN in place of infinities. Returns the norms (1 x nblock, float64)."""
+    grads = list(grads)
+    outs = grads if out is None else list(out)
+    nblock = int(nblock)
+    require(nblock >= 1, "ValueError: nblock must be at least 1")
+    require(float(max_norm) > 0, "ValueError: the largest norm must be positive")
+    require(len(outs) == len(grads), "ValueError: out must have as many tensors as grads")
+    require(by_rows is None or len(by_rows) == len(grads), "ValueError: by_rows must have an entry for every tensor")
+    require(len(grads) > 0, "ValueError: no tensors")
+    table = (_lib.ClipTensor * len(grads))()
+    a = _lib.Arguments()
+    for i, (g, o) in enumerate(zip(grads, outs)):
+        if not isinstance(g, torch.Tensor) or not isinstance(o, torch.Tensor):
+            raise _lib.DeepbindError("TypeError: grads and out must be lists of tensors")
+        code = _lib.row_dtype_code(g)
+        rows = by_rows is not None and bool(by_rows[i])
+        if g.dim() == 2:
+            n, m = g.shape
+            p, ld = a.rows("grads[%d]" % i, g, g.shape, g.dtype, out=o is g)
+            q, ldo = (p, ld) if o is g else a.rows("out[%d]" % i, o, g.shape, g.dtype, out=True)
+            require((n if rows else m) % nblock == 0, "ValueError: a tensor's models must be equal blocks of its columns, or rows")
+            if nblock == 1 and ld == m and ldo == m:
+                n, m = 1, n * m
+                ld = ldo = m
+        else:
+            require(nblock == 1, "ValueError: models side by side are blocks of matrices")
+            p = a.dense("grads[%d]" % i, g, g.shape, g.dtype, out=o is g)
+            q = p if o is g else a.dense("out[%d]" % i, o, g.shape, g.dtype, out=True)
+            n, m = 1, g.numel()
+            ld = ldo = m
+        table[i] = (p, q, n, m, ld, ldo, code, int(rows))
+    _lib.check_many(a)
+    norms = torch.empty((1, nblock), dtype=torch.float64, device=grads[0].device)
+    need = ctypes.c_size_t(0)
+    where = ctypes.addressof(table)
+    call("dbk_clip_gradients_workspace", len(grads), where, nblock, ctypes.addressof(need))
+    work, wp = _lib.workspace(need.value, norms)
+    call("dbk_clip_gradients", stream(), len(grads), where, nblock, float(max_norm), norms.data_ptr(), wp, need.value)
+    return norms
 
 
 def counter_add(counter, delta):

@@ -165,6 +165,97 @@ def layernorm_bprop(X, gamma, stats, dZ, nchunk=1, out=None):
     return dX, dgamma, dbeta
 
 
+def _block_args(Y, gate, gamma, beta, scale, next_gamma, next_beta, nchunk, rms, norm, next_norm, eps):
+    if not isinstance(Y, torch.Tensor) or Y.dim() != 2:
+        raise _lib.DeepbindError("ValueError: Y must be a matrix")
+    code, wide, (n, m) = _lib.row_dtype_code(Y), _lib.wide_dtype(Y), Y.shape
+    require(nchunk >= 1 and m % nchunk == 0 and m >= nchunk, "ValueError: the number of columns must be divisible by nchunk")
+    require(norm or (gamma is None and beta is None), "ValueError: without norm there is no gamma and no beta")
+    require(next_norm or (next_gamma is None and next_beta is None), "ValueError: without next_norm there is no next_gamma and no next_beta")
+    g = _lib.Arguments()
+    y, ldy = g.rows("Y", Y, (n, m), Y.dtype)
+    ga, ldg = (None, 0) if gate is None else g.rows("gate", gate, (n, m), Y.dtype)
+    weights = [g.dense(k, t, (1, m), wide) for k, t in (("gamma", gamma), ("beta", beta), ("scale", scale), ("next_gamma", next_gamma), ("next_beta", next_beta))]
+    return g, _lib.BlockNormArgs(code, int(bool(rms)), int(bool(norm)), int(bool(next_norm)), n, m, m // nchunk, float(eps), y, ldy, None, 0, ga, ldg, *weights), wide, n, m
+
+
+def blocknorm(Y, R=None, gate=None, gamma=None, beta=None, scale=None, next_gamma=None, next_beta=None, nchunk=1, rms=False, norm=True, next_norm=True,
+              eps=1e-5, want_stats=False, out=None):
+    """The norms around a block of layers with its gate and residual, in one pass over the rows: with P = norm(Y) * gamma + beta (P = Y
+    without norm), O = R + scale * P * gate * sigmoid(gate) and Z = norm(O) * next_gamma + next_beta (no Z without next_norm). norm as in
+    layernorm over every one of a row's nchunk equal chunks, or X / sqrt(mean(X^2) + eps) with rms. R and gate (n x m, Y's type) and the
+    weights (1 x m) may each be None: R and the betas are then zeros, the others ones.
+    Y: float32, float64 or bfloat16 with a row stride of its own; weights and statistics float32 (float64 beside float64). The second
+    norm is of O as it is stored.
+    Returns (O, Z|None, stats|None); stats (4 x n*nchunk), which blocknorm_bprop takes: means and reciprocal deviations of Y's chunks and of
+    O's. out (optional): (O, Z) matrices to write into, None where one is to be made."""
+    g, a, wide, n, m = _block_args(Y, gate, gamma, beta, scale, next_gamma, next_beta, nchunk, rms, norm, next_norm, eps)
+    if R is not None:
+        a.R, a.ldr = g.rows("R", R, (n, m), Y.dtype)
+    O, Z = (None, None) if out is None else out
+    require(next_norm or Z is None, "ValueError: without next_norm there is no Z")
+    for name, t in (("O", O), ("Z", Z)):
+        if t is not None:
+            g.rows(name, t, (n, m), Y.dtype, out=True)
+    g.check()
+    O = torch.empty((n, m), dtype=Y.dtype, device=Y.device) if O is None else O
+    a.O, a.ldo = O.data_ptr(), _lib.row_stride(O)
+    if next_norm:
+        Z = torch.empty((n, m), dtype=Y.dtype, device=Y.device) if Z is None else Z
+        a.Z, a.ldz = Z.data_ptr(), _lib.row_stride(Z)
+    stats = None
+    if want_stats:
+        stats = torch.empty((4, n * nchunk), dtype=wide, device=Y.device)
+        a.stats = stats.data_ptr()
+    call("dbk_blocknorm", stream(), ctypes.addressof(a))
+    return O, Z, stats
+
+
+def blocknorm_bprop(Y, O, stats, dR, dZ, gate=None, gamma=None, beta=None, scale=None, next_gamma=None, next_beta=None, nchunk=1, rms=False, norm=True,
+                    next_norm=True, out=None):
+    """Gradients (dY, dR, dgate, dgamma, dbeta, dscale, dnext_gamma, dnext_beta) of blocknorm at Y, with O and the stats of its forward call,
+    from dZ (None without next_norm) and dR, the gradient of O from elsewhere (None: zeros). What the forward call did not have has no
+    gradient (None). The returned dR is the gradient of R, which is O's whole one. out (optional): a tuple like the returned one of tensors to
+    write into, None where one is to be made."""
+    g, a, wide, n, m = _block_args(Y, gate, gamma, beta, scale, next_gamma, next_beta, nchunk, rms, norm, next_norm, 0.0)
+    require((dZ is not None) == bool(next_norm), "ValueError: dZ is given exactly with next_norm")
+    require(dR is not None or next_norm, "ValueError: neither dR nor dZ")
+    require(stats is not None or not (norm or next_norm), "ValueError: the statistics of the forward call are needed")
+    require(O is not None or not next_norm, "ValueError: O of the forward call is needed")
+    if next_norm:
+        a.O, a.ldo = g.rows("O", O, (n, m), Y.dtype)
+        a.dZ, a.lddz = g.rows("dZ", dZ, (n, m), Y.dtype)
+    if dR is not None:
+        a.dR, a.lddr = g.rows("dR", dR, (n, m), Y.dtype)
+    a.stats = g.dense("stats", stats, (4, n * nchunk), wide)
+    given = (None,) * 8 if out is None else tuple(out)
+    require(len(given) == 8, "ValueError: out must be (dY, dR, dgate, dgamma, dbeta, dscale, dnext_gamma, dnext_beta)")
+    likes = (("dY", Y), ("dR", Y), ("dgate", gate), ("dgamma", gamma), ("dbeta", beta), ("dscale", scale), ("dnext_gamma", next_gamma), ("dnext_beta", next_beta))
+    grads = []
+    for i, ((name, like), t) in enumerate(zip(likes, given)):
+        if like is None and t is not None:
+            raise _lib.DeepbindError("ValueError: no %s, no gradient of it" % name[1:])
+        if t is not None:
+            if i < 3:
+                g.rows(name, t, (n, m), Y.dtype, out=True)
+            else:
+                g.dense(name, t, (1, m), wide, out=True)
+    g.check()
+    for (name, like), t in zip(likes, given):
+        grads.append(torch.empty(like.shape, dtype=like.dtype, device=Y.device) if t is None and like is not None else t)
+    ld, at = _lib.row_stride, lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    a.dY, a.lddy, a.dR_in, a.lddr_in = at(grads[0]), ld(grads[0]), at(grads[1]), ld(grads[1])
+    if gate is not None:
+        a.dgate, a.lddgate = at(grads[2]), ld(grads[2])
+    a.dgamma, a.dbeta, a.dscale, a.dnext_gamma, a.dnext_beta = (at(t) for t in grads[3:])
+    where, need = ctypes.addressof(a), ctypes.c_size_t(0)
+    if any(t is not None for t in grads[3:]):
+        call("dbk_blocknorm_bprop_workspace", where, ctypes.addressof(need))
+    work, wp = _lib.workspace(need.value, Y)
+    call("dbk_blocknorm_bprop", stream(), where, wp, need.value)
+    return tuple(grads)
+
+
 def loss_terms(Z, Y, kind):
     """Elementwise loss terms before masking / averaging; kind is "nll", "mse", "nll_multiclass"
     (several columns per output: log(max(1e-15, Z)) * Y, reference: deepity/std/loss.py:147-151) or "hinge"

@@ -492,6 +492,32 @@ int dbk_layernorm_bprop_workspace(int dtype, size_t n, size_t m, size_t group, s
 int dbk_layernorm_bprop(dbk_stream_t stream, int dtype, const void* X, size_t ldx, const void* gamma, const void* stats, const void* dZ, size_t lddz,
                         size_t n, size_t m, size_t group, void* dX, size_t lddx, void* dgamma, void* dbeta, void* work, size_t work_bytes);
 
+/* The norms around a block of layers with its gate and residual, over every chunk of `group` columns of the n rows (m columns): P = norm(Y) * gamma + beta,
+ * O = R + scale * P * gate * sigmoid(gate), Z = norm(O) * next_gamma + next_beta; norm as in dbk_layernorm, or x / sqrt(mean(x^2) + eps) with rms.
+ * Without `norm`, P = Y; without `next` there is no Z. The second norm is of O as it is stored. */
+typedef struct dbk_blocknorm_args {
+    int dtype, rms, norm, next;
+    size_t n, m, group;
+    double eps;
+    const void* Y; size_t ldy;                  /* (n, m) rows */
+    const void* R; size_t ldr;                  /* may be NULL (zeros) */
+    const void* gate; size_t ldgate;            /* may be NULL (a factor of one) */
+    const void *gamma, *beta, *scale, *next_gamma, *next_beta;      /* (m) weights, each may be NULL (ones; beta: zeros) */
+    void* O; size_t ldo;                        /* forward: written; backward: as the forward call left it (read with `next` only) */
+    void* Z; size_t ldz;
+    void* stats;                                /* forward: may be NULL; (4, n * m / group): means and reciprocal deviations of Y's chunks, then of O's */
+    const void* dR; size_t lddr;                /* from here on: backward only. Gradient of O from elsewhere, may be NULL with `next` (zeros) */
+    const void* dZ; size_t lddz;
+    void* dY; size_t lddy;
+    void* dR_in; size_t lddr_in;                /* gradient of R, which is all of O's; may be NULL */
+    void* dgate; size_t lddgate;
+    void *dgamma, *dbeta, *dscale, *dnext_gamma, *dnext_beta;       /* (m), each may be NULL; written, not accumulated */
+} dbk_blocknorm_args;
+int dbk_blocknorm_args_size(void);              /* sizeof(dbk_blocknorm_args) as the library was built */
+int dbk_blocknorm(dbk_stream_t stream, const dbk_blocknorm_args* args);
+int dbk_blocknorm_bprop_workspace(const dbk_blocknorm_args* args, size_t* work_bytes);
+int dbk_blocknorm_bprop(dbk_stream_t stream, const dbk_blocknorm_args* args, void* work, size_t work_bytes);
+
 /* Causal convolution along every region's rows, a filter of 1 to 4 taps per channel: Z[t] = act(bias + sum_j W[j] * X[t - taps + 1 + j]), W (taps, D),
  * bias (D, may be NULL), act(p) = p * sigmoid(p) with silu, p without. Rows before a region's first come from state (nregion, taps - 1, D; kept
  * as the rows are, oldest first) or are zeros (NULL). last (nregion, taps - 1, D, may be NULL): the rows that the next piece of each sequence needs as its state. */
@@ -564,6 +590,21 @@ int dbk_deltarule(dbk_stream_t stream, const dbk_deltarule_args* args, void* wor
 int dbk_deltarule_bprop(dbk_stream_t stream, const dbk_deltarule_args* args, void* work, size_t work_bytes);
 /* One new row for each of N sequences (regions are not looked at): state (N, K, H * V), its successor goes to `last` (may be `state` itself). */
 int dbk_deltarule_step(dbk_stream_t stream, const dbk_deltarule_args* args);
+
+/* ------------------------------------------------------------------ gradients of many tensors */
+
+/* One tensor of a set: a matrix of rows with row strides of their own (a dense tensor of any shape: one row). Its nblock models are equal blocks of columns,
+ * or of rows (by_rows). out may be in. */
+typedef struct dbk_clip_tensor {
+    const void* in; void* out;
+    size_t rows, cols, ld_in, ld_out;
+    int dtype, by_rows;
+} dbk_clip_tensor;
+/* norms[b] (nblock doubles, device) = the 2-norm of all tensors' blocks b together, and out = in * max_norm / norms[b] where that is over max_norm, out = in
+ * elsewhere (also where the norm is NaN; an infinite one leaves zeros, and NaN for the infinite values). Squares are added in double precision, in a fixed order. work: as for the
+ * operators on rows. */
+int dbk_clip_gradients_workspace(size_t ntensor, const dbk_clip_tensor* tensors, size_t nblock, size_t* work_bytes);
+int dbk_clip_gradients(dbk_stream_t stream, size_t ntensor, const dbk_clip_tensor* tensors, size_t nblock, double max_norm, double* norms, void* work, size_t work_bytes);
 
 /* ------------------------------------------------------------------ one whole optimiser step */
 
