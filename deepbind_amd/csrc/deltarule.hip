@@ -22,10 +22,12 @@ __global__ __launch_bounds__(256) void k_delta_prepare(delta_shape p, const uint
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
-    __shared__ A kk_all[4][4][16][17], qk_all[4][4][16][17], a_all[4][64], b_all[4][64];
+    __shared__ A kk_all[4][4][16][17], qk_all[4][4][16][17], b_all[4][64];
+    __shared__ double a_all[4][64];
     const unsigned wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u;
     A (*kk)[16][17] = kk_all[wave], (*qk)[16][17] = qk_all[wave];
-    A *a = a_all[wave], *b = b_all[wave];
+    A* b = b_all[wave];
+    double* a = a_all[wave];
     delta_block bl;
     if (!find_block(p, regions, marks, blockIdx.x, bl)) return;
     const unsigned head = min(blockIdx.y * 4u + wave, p.H - 1u), group = head / (p.H / p.G);      // (a wave too many does the last head again)
@@ -50,22 +52,24 @@ __global__ __launch_bounds__(256) void k_delta_prepare(delta_shape p, const uint
     {
         const bool here = lane < bl.rows;
         const size_t row = bl.at + (here ? lane : 0u);
-        a[lane] = here && decay ? exp(decay[row * p.ldg + head]) : A(1);
+        a[lane] = here && decay ? exp((double)decay[row * p.ldg + head]) : 1.0;
         b[lane] = here ? beta[row * p.ldb + head] : A(0);
     }
     __syncthreads();
     // lane (g, c): column c of chunk g
     const bool there = g < nchunk;
     const size_t at = ((size_t)bl.slot * p.H + head) * DELTA_CHUNKS + g;
-    A D = A(0), first = A(1);
     if (there) {
-        A mine = A(1);
+        // (in double precision: a state that decays by a thousandth a row remembers a thousand of them, and would their factors' roundings)
+        double product = 0.0, first = 1.0;
+        A mine = A(1), D = A(0);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const A ai = a[16u * g + i];
-            D = i == (int)c ? A(1) : D * ai;     // (zero above the diagonal: nothing there yet)
+            const double ai = a[16u * g + i];
+            product = i == (int)c ? 1.0 : product * ai;          // (zero above the diagonal: nothing there yet)
+            D = (A)product;
             first *= ai;
-            mine = i == (int)c ? first : mine;
+            mine = i == (int)c ? (A)first : mine;
             const A n = i > (int)c ? D * kk[g][i][c] : A(0), s = i >= (int)c ? D * qk[g][i][c] : A(0);
             kk[g][i][c] = n;
             chunks[at].P[16 * i + c] = s;
@@ -329,7 +333,7 @@ int dbk_deltarule(dbk_stream_t stream, const dbk_deltarule_args* a, void* work, 
     if (!a->V || !a->nregion) { clear_error(); return 0; }
     const delta_shape s = delta_shape_of(*a);
     const delta_work w = work_in(work, *a, s);
-    DBK_CHECK(!w.bytes || (work && work_bytes >= w.bytes), "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, w.bytes);
+    DBK_CHECK(!a->N || (work && work_bytes >= w.bytes), "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, w.bytes);
     DBK_CHECK(grid_fits(delta_blocks(s), 256), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
     hipStream_t st = as_stream(stream);
     if (a->N) {
