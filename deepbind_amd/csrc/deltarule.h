@@ -125,20 +125,99 @@ __device__ __forceinline__ size_t block_number(const delta_shape& p, unsigned r,
 // its place in `keep`, which holds no region's first block
 __device__ __forceinline__ size_t kept_number(row_range g, unsigned k) { return g.start / DELTA_BLOCK + k; }
 
-// A wave's columns of a head and how a lane sees the 16-row tiles.
-template <typename A> struct delta_lane {
+// The waves that hold tiles of 16 columns of the same head are a team: 1, 2 or 4 of a workgroup's four (a head of more than 4 tiles has several), which share the head's keys and
+// queries. TEAM waves; of a workgroup, 4 / TEAM teams.
+template <typename A, int TEAM> struct delta_lane {
     unsigned g, c, head, group, v;               // v: columns of V and O in front of the wave's
-    unsigned nv;                                 // its columns, 16 or fewer
-    __device__ __forceinline__ void place(const delta_shape& p, unsigned head_, unsigned tile)
+    unsigned nv;                                 // its columns: 16, fewer, or none
+    unsigned team, thread;                       // of the workgroup's teams; of the team's threads
+    unsigned tile, unit;                         // tile of the head; head and part of it
+    // tiles: of a head. A team too many does the last one's work again.
+    __device__ __forceinline__ void place(const delta_shape& p, unsigned tiles)
     {
+        const unsigned wave = uniform(threadIdx.x >> 6), parts = (tiles + 3u) / 4u;
         g = (threadIdx.x & 63u) >> 4;
         c = threadIdx.x & 15u;
-        head = head_;
-        group = head_ / (p.H / p.G);
-        v = head_ * p.V + tile * 16u;
-        nv = min(16u, p.V - tile * 16u);
+        team = wave / TEAM;
+        thread = threadIdx.x & (64u * TEAM - 1u);
+        unit = min(blockIdx.y * (4u / TEAM) + team, p.H * parts - 1u);
+        head = unit / parts;
+        group = head / (p.H / p.G);
+        tile = unit % parts * 4u + wave % TEAM;
+        v = head * p.V + tile * 16u;
+        nv = tile * 16u < p.V ? min(16u, p.V - tile * 16u) : 0u;
+        if (!nv) v = head * p.V;
     }
     __device__ __forceinline__ unsigned row(int r) const { return mm16<A>::row(g, r); }
+};
+template <typename F> inline void with_key_tiles(size_t K, F f)
+{
+    if (K <= 16) f(std::integral_constant<int, 1>());
+    else if (K <= 32) f(std::integral_constant<int, 2>());
+    else if (K <= 64) f(std::integral_constant<int, 4>());
+    else f(std::integral_constant<int, 8>());
+}
+
+// Keys of more than 32 columns fill the LDS: there a team is always the whole workgroup, also where some of its waves have no tile and only help to fetch.
+inline int team_of(size_t K, size_t tiles) { return K > 32 || tiles > 2 ? 4 : (int)tiles; }
+inline unsigned team_blocks(const delta_shape& p, size_t tiles) { return divup((size_t)p.H * ((tiles + 3) / 4), 4u / team_of(p.K, tiles)); }
+template <typename F> inline void with_team(size_t K, size_t tiles, F f)
+{
+    auto pass = [&](auto kt) {
+        if constexpr (kt.value <= 2) {
+            if (tiles == 1) return f(kt, std::integral_constant<int, 1>());
+            if (tiles == 2) return f(kt, std::integral_constant<int, 2>());
+        }
+        f(kt, std::integral_constant<int, 4>());
+    };
+    with_key_tiles(K, pass);
+}
+
+// A team's keys and queries of one chunk in LDS, rows padded by 16 bytes: lanes read four neighbouring columns of 16 rows, or 16 neighbouring columns of
+// four rows, without meeting in the banks.
+template <typename A, int KT> struct delta_rows {
+    A k[16][16 * KT + 4], q[16][16 * KT + 4];
+};
+template <typename A, int W> __device__ __forceinline__ typename mm16<A>::vec tile_by_rows(const A (&m)[16][W], int t, unsigned g, unsigned c)
+{
+    typename mm16<A>::vec f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] = m[c][16u * t + mm16<A>::row(g, r)];
+    return f;
+}
+template <typename A, int W> __device__ __forceinline__ typename mm16<A>::vec tile_by_columns(const A (&m)[16][W], int t, unsigned g, unsigned c)
+{
+    typename mm16<A>::vec f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] = m[mm16<A>::row(g, r)][16u * t + c];
+    return f;
+}
+
+// Their way there: a thread's vectors come while the chunk before is worked on (fetch), and are put into LDS when it is done (put).
+template <typename T, int KT, int TEAM> struct delta_feed {
+    typedef typename acc_of<T>::type A;
+    static constexpr int EACH = KT >= TEAM ? KT / TEAM : 1, VECS = 64 * KT;      // vectors of 4 values: a thread's, a chunk's
+    raw_vec<T, false, 4> k[EACH], q[EACH];
+    __device__ __forceinline__ void fetch(const delta_shape& p, const T* Q, const T* K, unsigned thread, unsigned rows)
+    {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const unsigned v = thread + i * 64u * TEAM, row = v / (4u * KT), col = v % (4u * KT) * 4u;
+            const unsigned valid = row < rows && col < p.K ? p.K - col : 0u;
+            k[i].load(K + row * p.ldk + col, valid);
+            q[i].load(Q + row * p.ldq + col, valid);
+        }
+    }
+    __device__ __forceinline__ void put(delta_rows<A, KT>& to, unsigned thread) const
+    {
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const unsigned v = thread + i * 64u * TEAM, row = v / (4u * KT), col = v % (4u * KT) * 4u;
+            if (VECS < 64 * TEAM && v >= (unsigned)VECS) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { to.k[row][col + j] = k[i][j]; to.q[row][col + j] = q[i][j]; }
+        }
+    }
 };
 
 // Tile operands of keys and queries. By rows: element [c][16 t + row(g, r)], the left operand of a product with the state; by columns: [row(g, r)][16 t + c], the left operand
@@ -216,7 +295,7 @@ template <typename A> __device__ __forceinline__ typename mm16<A>::vec by_row(co
 }
 
 // A wave's columns of states (blocks of K x (H V)): tile t holds rows 16 t + row(g, r).
-template <typename A, int KT> __device__ __forceinline__ void load_state(typename mm16<A>::vec (&S)[KT], const A* p, const delta_shape& s, const delta_lane<A>& l)
+template <typename A, int KT, int TEAM> __device__ __forceinline__ void load_state(typename mm16<A>::vec (&S)[KT], const A* p, const delta_shape& s, const delta_lane<A, TEAM>& l)
 {
     const size_t D = (size_t)s.H * s.V;
 #pragma unroll
@@ -227,7 +306,7 @@ template <typename A, int KT> __device__ __forceinline__ void load_state(typenam
             S[t][r] = p && k < s.K && l.c < l.nv ? p[k * D + l.v + l.c] : A(0);
         }
 }
-template <typename A, int KT> __device__ __forceinline__ void store_state(const typename mm16<A>::vec (&S)[KT], A* p, const delta_shape& s, const delta_lane<A>& l)
+template <typename A, int KT, int TEAM> __device__ __forceinline__ void store_state(const typename mm16<A>::vec (&S)[KT], A* p, const delta_shape& s, const delta_lane<A, TEAM>& l)
 {
     const size_t D = (size_t)s.H * s.V;
 #pragma unroll
@@ -237,14 +316,6 @@ template <typename A, int KT> __device__ __forceinline__ void store_state(const 
             const unsigned k = 16u * t + l.row(r);
             if (k < s.K && l.c < l.nv) p[k * D + l.v + l.c] = S[t][r];
         }
-}
-
-template <typename F> inline void with_key_tiles(size_t K, F f)
-{
-    if (K <= 16) f(std::integral_constant<int, 1>());
-    else if (K <= 32) f(std::integral_constant<int, 2>());
-    else if (K <= 64) f(std::integral_constant<int, 4>());
-    else f(std::integral_constant<int, 8>());
 }
 
 // Defined in deltarule.hip.

@@ -95,50 +95,76 @@ __global__ __launch_bounds__(256) void k_delta_prepare(delta_shape p, const uint
     }
 }
 
+// What a wave reads of a chunk's matrices and of V, fetched a chunk ahead.
+template <typename T> struct delta_ahead {
+    typedef typename acc_of<T>::type A;
+    typename mm16<A>::vec T_, P, first, b, last;
+    T v[4];
+    A through;
+};
+
 // Walks a wave's 16 columns of a head's state down `rows` rows from `row` on. number(k): the number of the block k blocks on from the first.
-template <typename T, int KT, typename NUMBER>
-__device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lane<typename acc_of<T>::type>& l, const T* Q, const T* K, const T* V,
-                                           const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, size_t row, unsigned rows, NUMBER number,
+// Keys, queries, matrices and values of a chunk come while the one before it is worked on.
+template <typename T, int KT, int TEAM, typename NUMBER>
+__device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, delta_rows<typename acc_of<T>::type, KT>* lds, const T* Q, const T* K,
+                                           const T* V, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, size_t row, unsigned rows, NUMBER number,
                                            typename mm16<typename acc_of<T>::type>::vec (&S)[KT], T* O, typename acc_of<T>::type* keep, size_t kept)
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
+    if (!rows) return;
     const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K, *v = V + row * p.ldv + l.v;
     T* o = O + row * p.ldo + l.v;
+    delta_feed<T, KT, TEAM> feed;
+    delta_ahead<T> next;
+    auto fetch = [&](unsigned t) {
+        const delta_chunk<A>& ch = chunks[(number(t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS];
+        next.T_ = matrix_by_rows(ch.T, l.g, l.c);
+        next.P = matrix_by_rows(ch.P, l.g, l.c);
+        next.first = by_row(ch.first, l.g);
+        next.b = by_row(ch.b, l.g);
+        next.last = by_row(ch.last, l.g);
+        next.through = ch.first[15];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) next.v[r] = l.row(r) < rows - t && l.c < l.nv ? v[(t + l.row(r)) * p.ldv + l.c] : (T)A(0);
+    };
+    feed.fetch(p, q, k, l.thread, rows);
+    feed.put(lds[0], l.thread);
+    if (rows > DELTA_CHUNK) feed.fetch(p, q + DELTA_CHUNK * p.ldq, k + DELTA_CHUNK * p.ldk, l.thread, rows - DELTA_CHUNK);
+    fetch(0u);
+    __syncthreads();
     for (unsigned t = 0; t < rows; t += DELTA_CHUNK) {
         const unsigned n = min(rows - t, DELTA_CHUNK);
+        const delta_rows<A, KT>& here = lds[t / DELTA_CHUNK & 1u];
+        const delta_ahead<T> now = next;
+        if (t + DELTA_CHUNK < rows) {
+            feed.put(lds[~(t / DELTA_CHUNK) & 1u], l.thread);
+            fetch(t + DELTA_CHUNK);
+        }
+        if (t + 2u * DELTA_CHUNK < rows) feed.fetch(p, q + (t + 2u * DELTA_CHUNK) * p.ldq, k + (t + 2u * DELTA_CHUNK) * p.ldk, l.thread, rows - t - 2u * DELTA_CHUNK);
+        if (l.nv) {
         if (keep && t && t % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + (kept + t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
-        const delta_chunk<A>& ch = chunks[(number(t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS];
-        vec f[KT];
-        load_by_rows<T, KT>(f, k, p.ldk, n, p.K, l.g, l.c);
-        vec w = zero16<A>(), z = zero16<A>();
+        vec w = zero16<A>(), z = zero16<A>(), x;
 #pragma unroll
-        for (int i = 0; i < KT; ++i) w = product<A>(f[i], S[i], w);
-        load_by_rows<T, KT>(f, q, p.ldq, n, p.K, l.g, l.c);
+        for (int i = 0; i < KT; ++i) w = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], w);
 #pragma unroll
-        for (int i = 0; i < KT; ++i) z = product<A>(f[i], S[i], z);
-        const vec first = by_row(ch.first, l.g), b = by_row(ch.b, l.g), last = by_row(ch.last, l.g);
-        vec x = load_tile(v, p.ldv, n, l.nv, l.g, l.c);
+        for (int i = 0; i < KT; ++i) z = product<A>(tile_by_rows(here.q, i, l.g, l.c), S[i], z);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = l.row(r) < n ? b[r] * (x[r] - first[r] * w[r]) : A(0);
-        const vec u = triangle<A, true>(matrix_by_rows(ch.T, l.g, l.c), x, zero16<A>(), l.g);
-        vec y = triangle<A, true>(matrix_by_rows(ch.P, l.g, l.c), u, first * z, l.g);
+        for (int r = 0; r < 4; ++r) x[r] = l.row(r) < n ? now.b[r] * ((A)now.v[r] - now.first[r] * w[r]) : A(0);
+        const vec u = triangle<A, true>(now.T_, x, zero16<A>(), l.g);
+        const vec sent = now.last * u;
+#pragma unroll
+        for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.k, i, l.g, l.c), sent, now.through * S[i]);
+        const vec y = triangle<A, true>(now.P, u, now.first * z, l.g);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-            if (l.row(r) < n && l.c < l.nv) o[(size_t)l.row(r) * p.ldo + l.c] = (T)(scale * y[r]);
-        load_by_columns<T, KT>(f, k, p.ldk, n, p.K, l.g, l.c);
-        const A through = ch.first[15];
-        const vec sent = last * u;
-#pragma unroll
-        for (int i = 0; i < KT; ++i) S[i] = product<A>(f[i], sent, through * S[i]);
-        q += DELTA_CHUNK * p.ldq;
-        k += DELTA_CHUNK * p.ldk;
-        v += DELTA_CHUNK * p.ldv;
-        o += DELTA_CHUNK * p.ldo;
+            if (l.row(r) < n && l.c < l.nv) o[(size_t)(t + l.row(r)) * p.ldo + l.c] = (T)(scale * y[r]);
+        }
+        __syncthreads();
     }
 }
 
-template <typename T, int KT>
+template <typename T, int KT, int TEAM>
 __global__ __launch_bounds__(256) void k_delta_fprop(delta_shape p, const uint32_t* __restrict__ regions, const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                                                      const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, typename acc_of<T>::type scale,
                                                      const typename acc_of<T>::type* __restrict__ state, T* __restrict__ O, typename acc_of<T>::type* __restrict__ last,
@@ -146,16 +172,15 @@ __global__ __launch_bounds__(256) void k_delta_fprop(delta_shape p, const uint32
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
-    const unsigned f = blockIdx.y * 4u + uniform(threadIdx.x >> 6);
-    if (f >= p.H * p.ns) return;
-    delta_lane<A> l;
-    l.place(p, f / p.ns, f % p.ns);
+    __shared__ delta_rows<A, KT> lds[4 / TEAM][2];
+    delta_lane<A, TEAM> l;
+    l.place(p, p.ns);
     const unsigned r = blockIdx.x;
     const row_range g = region_rows(regions, r, p.N);
     const size_t block = (size_t)p.K * p.H * p.V;
     vec S[KT];
     load_state<A, KT>(S, state ? state + r * block : (const A*)nullptr, p, l);
-    delta_walk<T, KT>(p, l, Q, K, V, chunks, scale, g.start, g.end - g.start, [&](unsigned k) { return block_number(p, r, g, k); }, S, O, keep, kept_number(g, 0u));
+    delta_walk<T, KT, TEAM>(p, l, lds[l.team], Q, K, V, chunks, scale, g.start, g.end - g.start, [&](unsigned k) { return block_number(p, r, g, k); }, S, O, keep, kept_number(g, 0u));
     if (last) store_state<A, KT>(S, last + r * block, p, l);
 }
 
@@ -343,8 +368,8 @@ int dbk_deltarule(dbk_stream_t stream, const dbk_deltarule_args* a, void* work, 
     with_row_type(a->dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
-        with_key_tiles(a->K, [&](auto kt) {
-            k_delta_fprop<T, kt.value><<<dim3(s.nregion, divup((size_t)s.H * s.ns, 4)), 256, 0, st>>>(
+        with_team(a->K, s.ns, [&](auto kt, auto team) {
+            k_delta_fprop<T, kt.value, team.value><<<dim3(s.nregion, team_blocks(s, s.ns)), 256, 0, st>>>(
                 s, a->regions, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const delta_chunk<A>*)w.chunks, (A)a->scale, (const A*)a->state, (T*)a->O, (A*)a->last, (A*)a->keep);
         });
     });

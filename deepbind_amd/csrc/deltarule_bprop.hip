@@ -20,52 +20,74 @@
 
 namespace dbk {
 
-// dS of a chunk's start from that of its end
-template <typename T, int KT>
+// dS of a chunk's start from that of its end, chunk after chunk up the region. What a chunk needs comes while the one behind it is worked on.
+template <typename T, int KT, int TEAM>
 __global__ __launch_bounds__(256) void k_delta_chain(delta_shape p, size_t lddo, const uint32_t* __restrict__ regions, const T* __restrict__ Q, const T* __restrict__ K,
                                                      const T* __restrict__ dO, const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, typename acc_of<T>::type scale,
                                                      typename acc_of<T>::type* __restrict__ dstates)
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
-    const unsigned f = blockIdx.y * 4u + uniform(threadIdx.x >> 6);
-    if (f >= p.H * p.ns) return;
-    delta_lane<A> l;
-    l.place(p, f / p.ns, f % p.ns);
+    __shared__ delta_rows<A, KT> lds_all[4 / TEAM][2];
+    delta_lane<A, TEAM> l;
+    l.place(p, p.ns);
+    delta_rows<A, KT>* lds = lds_all[l.team];
     const unsigned r = blockIdx.x;
     const row_range g = region_rows(regions, r, p.N);
     const unsigned rows = g.end - g.start;
     if (rows <= DELTA_BLOCK) return;
+    const T *q = Q + (size_t)g.start * p.ldq + (size_t)l.group * p.K, *k = K + (size_t)g.start * p.ldk + (size_t)l.group * p.K, *d0 = dO + (size_t)g.start * lddo + l.v;
+    delta_feed<T, KT, TEAM> feed;
+    struct { vec T_, P, first, b, last; T d[4]; A through; } next;
+    auto fetch = [&](unsigned t) {
+        const delta_chunk<A>& ch = chunks[(block_number(p, r, g, t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS];
+        next.T_ = matrix_by_columns(ch.T, l.g, l.c);
+        next.P = matrix_by_columns(ch.P, l.g, l.c);
+        next.first = by_row(ch.first, l.g);
+        next.b = by_row(ch.b, l.g);
+        next.last = by_row(ch.last, l.g);
+        next.through = ch.first[15];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) next.d[i] = l.row(i) < rows - t && l.c < l.nv ? d0[(t + l.row(i)) * lddo + l.c] : (T)A(0);
+    };
+    auto keys = [&](unsigned t) { feed.fetch(p, q + t * p.ldq, k + t * p.ldk, l.thread, rows - t); };
     vec S[KT];
 #pragma unroll
     for (int i = 0; i < KT; ++i) S[i] = zero16<A>();
-    for (unsigned t = (rows - 1) / DELTA_CHUNK * DELTA_CHUNK; t >= DELTA_BLOCK; t -= DELTA_CHUNK) {
-        const unsigned n = min(rows - t, DELTA_CHUNK);
-        const size_t row = (size_t)g.start + t;
-        const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K;
-        const delta_chunk<A>& ch = chunks[(block_number(p, r, g, t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS];
-        vec f_[KT], y = zero16<A>();
-        load_by_rows<T, KT>(f_, k, p.ldk, n, p.K, l.g, l.c);
+    const unsigned end = (rows - 1) / DELTA_CHUNK * DELTA_CHUNK;
+    keys(end);
+    feed.put(lds[end / DELTA_CHUNK & 1u], l.thread);
+    keys(end - DELTA_CHUNK);                     // (there are more than four chunks)
+    fetch(end);
+    __syncthreads();
+    for (unsigned t = end; t >= DELTA_BLOCK; t -= DELTA_CHUNK) {
+        const delta_rows<A, KT>& here = lds[t / DELTA_CHUNK & 1u];
+        const auto now = next;
+        feed.put(lds[~(t / DELTA_CHUNK) & 1u], l.thread);
+        fetch(t - DELTA_CHUNK);
+        keys(t - 2u * DELTA_CHUNK);
+        if (l.nv) {
+            vec y = zero16<A>(), d;
 #pragma unroll
-        for (int i = 0; i < KT; ++i) y = product<A>(f_[i], S[i], y);
-        const vec first = by_row(ch.first, l.g), b = by_row(ch.b, l.g), last = by_row(ch.last, l.g);
-        const vec d = scale * load_tile(dO + row * lddo + l.v, lddo, n, l.nv, l.g, l.c);
-        const vec du = triangle<A, false>(matrix_by_columns(ch.P, l.g, l.c), d, last * y, l.g);
-        const vec dy = triangle<A, false>(matrix_by_columns(ch.T, l.g, l.c), du, zero16<A>(), l.g);
-        const vec dw = -(first * (b * dy)), fd = first * d;
-        const A through = ch.first[15];
-        load_by_columns<T, KT>(f_, k, p.ldk, n, p.K, l.g, l.c);
+            for (int i = 0; i < 4; ++i) d[i] = scale * (A)now.d[i];
 #pragma unroll
-        for (int i = 0; i < KT; ++i) S[i] = product<A>(f_[i], dw, through * S[i]);
-        load_by_columns<T, KT>(f_, q, p.ldq, n, p.K, l.g, l.c);
+            for (int i = 0; i < KT; ++i) y = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], y);
+            const vec du = triangle<A, false>(now.P, d, now.last * y, l.g);
+            const vec fd = now.first * d;
 #pragma unroll
-        for (int i = 0; i < KT; ++i) S[i] = product<A>(f_[i], fd, S[i]);
-        if (t % DELTA_BLOCK == 0) store_state<A, KT>(S, dstates + kept_number(g, t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
+            for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.q, i, l.g, l.c), fd, now.through * S[i]);
+            const vec dy = triangle<A, false>(now.T_, du, zero16<A>(), l.g);
+            const vec dw = -(now.first * (now.b * dy));
+#pragma unroll
+            for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.k, i, l.g, l.c), dw, S[i]);
+            if (t % DELTA_BLOCK == 0) store_state<A, KT>(S, dstates + kept_number(g, t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
+        }
+        __syncthreads();
     }
 }
 
 // transposed states: tile t holds [row(g, r)][16 t + c] of the wave's 16 columns by K
-template <typename A, int KT> __device__ __forceinline__ void load_state_t(typename mm16<A>::vec (&S)[KT], const A* p, const delta_shape& s, const delta_lane<A>& l)
+template <typename A, int KT, int TEAM> __device__ __forceinline__ void load_state_t(typename mm16<A>::vec (&S)[KT], const A* p, const delta_shape& s, const delta_lane<A, TEAM>& l)
 {
     const size_t D = (size_t)s.H * s.V;
 #pragma unroll
@@ -130,9 +152,12 @@ __global__ __launch_bounds__(256) void k_delta_bprop(delta_shape p, size_t lddo,
     if (!find_block(p, regions, marks, blockIdx.x, bl)) return;
     const unsigned unit = min((blockIdx.y * 4u + wave) / out.waves, p.H * out.parts - 1u), part = unit % out.parts;      // (a unit too many does the last one again)
     const unsigned tile = part * 4u + slice;
-    delta_lane<A> l;
-    l.place(p, unit / out.parts, min(tile, p.ns - 1u));
-    if (tile >= p.ns) l.nv = 0u;
+    delta_lane<A, 4> l;
+    l.place(p, p.ns);
+    l.head = unit / out.parts;
+    l.group = l.head / (p.H / p.G);
+    l.nv = tile < p.ns ? min(16u, p.V - tile * 16u) : 0u;
+    l.v = l.head * p.V + (l.nv ? tile * 16u : 0u);
     const unsigned g = l.g, c = l.c, nchunk = (bl.rows + 15u) / 16u;
     const size_t state = (size_t)p.K * p.H * p.V;
     const T *q0 = Q + (size_t)bl.at * p.ldq + (size_t)l.group * p.K, *k0 = K + (size_t)bl.at * p.ldk + (size_t)l.group * p.K;
@@ -429,9 +454,11 @@ int dbk_deltarule_bprop(dbk_stream_t stream, const dbk_deltarule_args* a, void* 
         typedef typename acc_of<T>::type A;
         delta_grads<T> out = {(T*)a->dQ, (T*)a->dK, (T*)a->dV, (A*)a->dbeta, (A*)a->ddecay, a->lddq, a->lddk, a->lddv, a->lddbeta, a->ldddecay,
                               (A*)w.dq, (A*)w.dk, (A*)w.db, a->ddecay ? (A*)w.dg : nullptr, w.parts, w.waves};
+        with_team(a->K, s.ns, [&](auto kt, auto team) {
+            k_delta_chain<T, kt.value, team.value><<<dim3(s.nregion, team_blocks(s, s.ns)), 256, 0, st>>>(s, a->lddo, a->regions, (const T*)a->Q, (const T*)a->Kk, (const T*)a->dO,
+                                                                                                         (const delta_chunk<A>*)w.chunks, (A)a->scale, (A*)w.dstates);
+        });
         with_key_tiles(a->K, [&](auto kt) {
-            k_delta_chain<T, kt.value><<<dim3(s.nregion, divup((size_t)s.H * s.ns, 4)), 256, 0, st>>>(s, a->lddo, a->regions, (const T*)a->Q, (const T*)a->Kk, (const T*)a->dO,
-                                                                                                     (const delta_chunk<A>*)w.chunks, (A)a->scale, (A*)w.dstates);
             constexpr size_t lds = 4 * sizeof(delta_share<A, kt.value>);
             if (lds > 65536 && hipFuncSetAttribute((const void*)k_delta_bprop<T, kt.value>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) { rc = 1; return; }
             k_delta_bprop<T, kt.value><<<dim3((unsigned)delta_blocks(s), divup((size_t)s.H * w.parts * w.waves, 4)), 256, lds, st>>>(
