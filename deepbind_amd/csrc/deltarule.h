@@ -173,10 +173,11 @@ template <typename F> inline void with_team(size_t K, size_t tiles, F f)
     with_key_tiles(K, pass);
 }
 
-// A team's keys and queries of one chunk in LDS, rows padded by 16 bytes: lanes read four neighbouring columns of 16 rows, or 16 neighbouring columns of
+// A team's keys, queries and matrices of one chunk in LDS, rows padded by 16 bytes: lanes read four neighbouring columns of 16 rows, or 16 neighbouring columns of
 // four rows, without meeting in the banks.
 template <typename A, int KT> struct delta_rows {
     A k[16][16 * KT + 4], q[16][16 * KT + 4];
+    delta_chunk<A> c;
 };
 template <typename A, int W> __device__ __forceinline__ typename mm16<A>::vec tile_by_rows(const A (&m)[16][W], int t, unsigned g, unsigned c)
 {
@@ -193,13 +194,23 @@ template <typename A, int W> __device__ __forceinline__ typename mm16<A>::vec ti
     return f;
 }
 
+// Waves per SIMD that the walks are compiled for: their registers hold 4 values per lane of a state's every 16 rows.
+template <typename A, int KT> constexpr int delta_waves() { return sizeof(A) == 4 ? (KT <= 4 ? 4 : 2) : KT <= 4 ? 2 : 1; }
+
 // Their way there: a thread's vectors come while the chunk before is worked on (fetch), and are put into LDS when it is done (put).
 template <typename T, int KT, int TEAM> struct delta_feed {
     typedef typename acc_of<T>::type A;
     static constexpr int EACH = KT >= TEAM ? KT / TEAM : 1, VECS = 64 * KT;      // vectors of 4 values: a thread's, a chunk's
+    static constexpr int PARTS = sizeof(delta_chunk<A>) / sizeof(A) / 4, SHARE = (PARTS + 64 * TEAM - 1) / (64 * TEAM);
     raw_vec<T, false, 4> k[EACH], q[EACH];
-    __device__ __forceinline__ void fetch(const delta_shape& p, const T* Q, const T* K, unsigned thread, unsigned rows)
+    row_vec<A, 4> part[SHARE];
+    __device__ __forceinline__ void fetch(const delta_shape& p, const T* Q, const T* K, const delta_chunk<A>& c, unsigned thread, unsigned rows)
     {
+#pragma unroll
+        for (int i = 0; i < SHARE; ++i) {
+            const unsigned v = thread + i * 64u * TEAM;
+            part[i].load(reinterpret_cast<const A*>(&c) + 4 * v, v < (unsigned)PARTS ? 4u : 0u);
+        }
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const unsigned v = thread + i * 64u * TEAM, row = v / (4u * KT), col = v % (4u * KT) * 4u;
@@ -210,6 +221,13 @@ template <typename T, int KT, int TEAM> struct delta_feed {
     }
     __device__ __forceinline__ void put(delta_rows<A, KT>& to, unsigned thread) const
     {
+#pragma unroll
+        for (int i = 0; i < SHARE; ++i) {
+            const unsigned v = thread + i * 64u * TEAM;
+            if (v >= (unsigned)PARTS) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) reinterpret_cast<A*>(&to.c)[4 * v + j] = part[i].v[j];
+        }
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const unsigned v = thread + i * 64u * TEAM, row = v / (4u * KT), col = v % (4u * KT) * 4u;

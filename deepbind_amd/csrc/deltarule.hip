@@ -95,14 +95,6 @@ __global__ __launch_bounds__(256) void k_delta_prepare(delta_shape p, const uint
     }
 }
 
-// What a wave reads of a chunk's matrices and of V, fetched a chunk ahead.
-template <typename T> struct delta_ahead {
-    typedef typename acc_of<T>::type A;
-    typename mm16<A>::vec T_, P, first, b, last;
-    T v[4];
-    A through;
-};
-
 // Walks a wave's 16 columns of a head's state down `rows` rows from `row` on. number(k): the number of the block k blocks on from the first.
 // Keys, queries, matrices and values of a chunk come while the one before it is worked on.
 template <typename T, int KT, int TEAM, typename NUMBER>
@@ -113,59 +105,59 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
     if (!rows) return;
-    const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K, *v = V + row * p.ldv + l.v;
-    T* o = O + row * p.ldo + l.v;
+    const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K, *v = V + row * p.ldv + l.v + l.c;
+    T* o = O + row * p.ldo + l.v + l.c;
     delta_feed<T, KT, TEAM> feed;
-    delta_ahead<T> next;
     auto fetch = [&](unsigned t) {
-        const delta_chunk<A>& ch = chunks[(number(t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS];
-        next.T_ = matrix_by_rows(ch.T, l.g, l.c);
-        next.P = matrix_by_rows(ch.P, l.g, l.c);
-        next.first = by_row(ch.first, l.g);
-        next.b = by_row(ch.b, l.g);
-        next.last = by_row(ch.last, l.g);
-        next.through = ch.first[15];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) next.v[r] = l.row(r) < rows - t && l.c < l.nv ? v[(t + l.row(r)) * p.ldv + l.c] : (T)A(0);
+        feed.fetch(p, q + t * p.ldq, k + t * p.ldk, chunks[(number(t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS], l.thread, rows - t);
     };
-    feed.fetch(p, q, k, l.thread, rows);
-    feed.put(lds[0], l.thread);
-    if (rows > DELTA_CHUNK) feed.fetch(p, q + DELTA_CHUNK * p.ldq, k + DELTA_CHUNK * p.ldk, l.thread, rows - DELTA_CHUNK);
+    T next[4];
+    auto values = [&](unsigned t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) next[r] = l.row(r) < rows - t && l.c < l.nv ? v[(t + l.row(r)) * p.ldv] : (T)A(0);
+    };
     fetch(0u);
+    values(0u);
+    feed.put(lds[0], l.thread);
+    if (rows > DELTA_CHUNK) fetch(DELTA_CHUNK);
     __syncthreads();
     for (unsigned t = 0; t < rows; t += DELTA_CHUNK) {
         const unsigned n = min(rows - t, DELTA_CHUNK);
         const delta_rows<A, KT>& here = lds[t / DELTA_CHUNK & 1u];
-        const delta_ahead<T> now = next;
+        vec x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = (A)next[r];
         if (t + DELTA_CHUNK < rows) {
             feed.put(lds[~(t / DELTA_CHUNK) & 1u], l.thread);
-            fetch(t + DELTA_CHUNK);
+            values(t + DELTA_CHUNK);
         }
-        if (t + 2u * DELTA_CHUNK < rows) feed.fetch(p, q + (t + 2u * DELTA_CHUNK) * p.ldq, k + (t + 2u * DELTA_CHUNK) * p.ldk, l.thread, rows - t - 2u * DELTA_CHUNK);
+        if (t + 2u * DELTA_CHUNK < rows) fetch(t + 2u * DELTA_CHUNK);
         if (l.nv) {
-        if (keep && t && t % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + (kept + t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
-        vec w = zero16<A>(), z = zero16<A>(), x;
+            if (keep && t && t % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + (kept + t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
+            vec w = zero16<A>(), z = zero16<A>();
 #pragma unroll
-        for (int i = 0; i < KT; ++i) w = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], w);
+            for (int i = 0; i < KT; ++i) w = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], w);
 #pragma unroll
-        for (int i = 0; i < KT; ++i) z = product<A>(tile_by_rows(here.q, i, l.g, l.c), S[i], z);
+            for (int i = 0; i < KT; ++i) z = product<A>(tile_by_rows(here.q, i, l.g, l.c), S[i], z);
+            const vec first = by_row(here.c.first, l.g), b = by_row(here.c.b, l.g);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = l.row(r) < n ? now.b[r] * ((A)now.v[r] - now.first[r] * w[r]) : A(0);
-        const vec u = triangle<A, true>(now.T_, x, zero16<A>(), l.g);
-        const vec sent = now.last * u;
+            for (int r = 0; r < 4; ++r) x[r] = l.row(r) < n ? b[r] * (x[r] - first[r] * w[r]) : A(0);
+            const vec u = triangle<A, true>(matrix_by_rows(here.c.T, l.g, l.c), x, zero16<A>(), l.g);
+            const vec sent = by_row(here.c.last, l.g) * u;
+            const A through = here.c.first[15];
 #pragma unroll
-        for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.k, i, l.g, l.c), sent, now.through * S[i]);
-        const vec y = triangle<A, true>(now.P, u, now.first * z, l.g);
+            for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.k, i, l.g, l.c), sent, through * S[i]);
+            const vec y = triangle<A, true>(matrix_by_rows(here.c.P, l.g, l.c), u, first * z, l.g);
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (l.row(r) < n && l.c < l.nv) o[(size_t)(t + l.row(r)) * p.ldo + l.c] = (T)(scale * y[r]);
+            for (int r = 0; r < 4; ++r)
+                if (l.row(r) < n && l.c < l.nv) o[(size_t)(t + l.row(r)) * p.ldo] = (T)(scale * y[r]);
         }
         __syncthreads();
     }
 }
 
 template <typename T, int KT, int TEAM>
-__global__ __launch_bounds__(256) void k_delta_fprop(delta_shape p, const uint32_t* __restrict__ regions, const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
+__global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT>())) void k_delta_fprop(delta_shape p, const uint32_t* __restrict__ regions, const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                                                      const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, typename acc_of<T>::type scale,
                                                      const typename acc_of<T>::type* __restrict__ state, T* __restrict__ O, typename acc_of<T>::type* __restrict__ last,
                                                      typename acc_of<T>::type* __restrict__ keep)

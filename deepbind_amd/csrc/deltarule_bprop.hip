@@ -22,7 +22,7 @@ namespace dbk {
 
 // dS of a chunk's start from that of its end, chunk after chunk up the region. What a chunk needs comes while the one behind it is worked on.
 template <typename T, int KT, int TEAM>
-__global__ __launch_bounds__(256) void k_delta_chain(delta_shape p, size_t lddo, const uint32_t* __restrict__ regions, const T* __restrict__ Q, const T* __restrict__ K,
+__global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT>())) void k_delta_chain(delta_shape p, size_t lddo, const uint32_t* __restrict__ regions, const T* __restrict__ Q, const T* __restrict__ K,
                                                      const T* __restrict__ dO, const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, typename acc_of<T>::type scale,
                                                      typename acc_of<T>::type* __restrict__ dstates)
 {
@@ -36,48 +36,45 @@ __global__ __launch_bounds__(256) void k_delta_chain(delta_shape p, size_t lddo,
     const row_range g = region_rows(regions, r, p.N);
     const unsigned rows = g.end - g.start;
     if (rows <= DELTA_BLOCK) return;
-    const T *q = Q + (size_t)g.start * p.ldq + (size_t)l.group * p.K, *k = K + (size_t)g.start * p.ldk + (size_t)l.group * p.K, *d0 = dO + (size_t)g.start * lddo + l.v;
+    const T *q = Q + (size_t)g.start * p.ldq + (size_t)l.group * p.K, *k = K + (size_t)g.start * p.ldk + (size_t)l.group * p.K, *d0 = dO + (size_t)g.start * lddo + l.v + l.c;
     delta_feed<T, KT, TEAM> feed;
-    struct { vec T_, P, first, b, last; T d[4]; A through; } next;
     auto fetch = [&](unsigned t) {
-        const delta_chunk<A>& ch = chunks[(block_number(p, r, g, t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS];
-        next.T_ = matrix_by_columns(ch.T, l.g, l.c);
-        next.P = matrix_by_columns(ch.P, l.g, l.c);
-        next.first = by_row(ch.first, l.g);
-        next.b = by_row(ch.b, l.g);
-        next.last = by_row(ch.last, l.g);
-        next.through = ch.first[15];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) next.d[i] = l.row(i) < rows - t && l.c < l.nv ? d0[(t + l.row(i)) * lddo + l.c] : (T)A(0);
+        feed.fetch(p, q + t * p.ldq, k + t * p.ldk, chunks[(block_number(p, r, g, t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS], l.thread, rows - t);
     };
-    auto keys = [&](unsigned t) { feed.fetch(p, q + t * p.ldq, k + t * p.ldk, l.thread, rows - t); };
+    T next[4];
+    auto values = [&](unsigned t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) next[i] = l.row(i) < rows - t && l.c < l.nv ? d0[(t + l.row(i)) * lddo] : (T)A(0);
+    };
     vec S[KT];
 #pragma unroll
     for (int i = 0; i < KT; ++i) S[i] = zero16<A>();
     const unsigned end = (rows - 1) / DELTA_CHUNK * DELTA_CHUNK;
-    keys(end);
-    feed.put(lds[end / DELTA_CHUNK & 1u], l.thread);
-    keys(end - DELTA_CHUNK);                     // (there are more than four chunks)
     fetch(end);
+    values(end);
+    feed.put(lds[end / DELTA_CHUNK & 1u], l.thread);
+    fetch(end - DELTA_CHUNK);                    // (there are more than four chunks)
     __syncthreads();
     for (unsigned t = end; t >= DELTA_BLOCK; t -= DELTA_CHUNK) {
         const delta_rows<A, KT>& here = lds[t / DELTA_CHUNK & 1u];
-        const auto now = next;
-        feed.put(lds[~(t / DELTA_CHUNK) & 1u], l.thread);
-        fetch(t - DELTA_CHUNK);
-        keys(t - 2u * DELTA_CHUNK);
-        if (l.nv) {
-            vec y = zero16<A>(), d;
+        vec d;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d[i] = scale * (A)now.d[i];
+        for (int i = 0; i < 4; ++i) d[i] = scale * (A)next[i];
+        feed.put(lds[~(t / DELTA_CHUNK) & 1u], l.thread);
+        values(t - DELTA_CHUNK);
+        fetch(t - 2u * DELTA_CHUNK);
+        if (l.nv) {
+            vec y = zero16<A>();
 #pragma unroll
             for (int i = 0; i < KT; ++i) y = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], y);
-            const vec du = triangle<A, false>(now.P, d, now.last * y, l.g);
-            const vec fd = now.first * d;
+            const vec first = by_row(here.c.first, l.g);
+            const A through = here.c.first[15];
+            const vec du = triangle<A, false>(matrix_by_columns(here.c.P, l.g, l.c), d, by_row(here.c.last, l.g) * y, l.g);
+            const vec fd = first * d;
 #pragma unroll
-            for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.q, i, l.g, l.c), fd, now.through * S[i]);
-            const vec dy = triangle<A, false>(now.T_, du, zero16<A>(), l.g);
-            const vec dw = -(now.first * (now.b * dy));
+            for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.q, i, l.g, l.c), fd, through * S[i]);
+            const vec dy = triangle<A, false>(matrix_by_columns(here.c.T, l.g, l.c), du, zero16<A>(), l.g);
+            const vec dw = -(first * (by_row(here.c.b, l.g) * dy));
 #pragma unroll
             for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.k, i, l.g, l.c), dw, S[i]);
             if (t % DELTA_BLOCK == 0) store_state<A, KT>(S, dstates + kept_number(g, t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
