@@ -115,6 +115,7 @@ _SIGNATURES = {
     "dbk_statescan_bprop": [_P, _P, _P, _Z],
     "dbk_statescan_step": [_P, _P],
     "dbk_deltarule_args_size": [],
+    "dbk_deltarule_kept": [_P, _P],
     "dbk_deltarule_workspace": [_P, _I, _P],
     "dbk_deltarule": [_P, _P, _P, _Z],
     "dbk_deltarule_bprop": [_P, _P, _P, _Z],

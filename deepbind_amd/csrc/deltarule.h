@@ -32,6 +32,7 @@ constexpr size_t DELTA_KEY = 128;                // the most columns of a key
 struct delta_shape {
     unsigned N, nregion, H, G, K, V, ns;         // rows, regions, heads, key heads, columns of a key and of a value, tiles of 16 value columns per head
     unsigned slots;                              // blocks that are not a region's first (segment_slots)
+    unsigned L, cuts;                            // rows of a segment (0: no region is cut), segments that are not a region's first
     size_t ldq, ldk, ldv, ldb, ldg, ldo;
 };
 
@@ -132,21 +133,22 @@ template <typename A, int TEAM> struct delta_lane {
     unsigned nv;                                 // its columns: 16, fewer, or none
     unsigned team, thread;                       // of the workgroup's teams; of the team's threads
     unsigned tile, unit;                         // tile of the head; head and part of it
-    // tiles: of a head. A team too many does the last one's work again.
-    __device__ __forceinline__ void place(const delta_shape& p, unsigned tiles)
+    size_t D;                                    // columns of all heads
+    // cols: of a head, in tiles of 16. A team too many does the last one's work again.
+    __device__ __forceinline__ void place(const delta_shape& p, unsigned index, unsigned cols)
     {
-        const unsigned wave = uniform(threadIdx.x >> 6), parts = (tiles + 3u) / 4u;
+        const unsigned wave = uniform(threadIdx.x >> 6), tiles = (cols + 15u) / 16u, parts = (tiles + TEAM - 1u) / TEAM;
         g = (threadIdx.x & 63u) >> 4;
         c = threadIdx.x & 15u;
         team = wave / TEAM;
         thread = threadIdx.x & (64u * TEAM - 1u);
-        unit = min(blockIdx.y * (4u / TEAM) + team, p.H * parts - 1u);
+        unit = min(index * (4u / TEAM) + team, p.H * parts - 1u);
         head = unit / parts;
         group = head / (p.H / p.G);
-        tile = unit % parts * 4u + wave % TEAM;
-        v = head * p.V + tile * 16u;
-        nv = tile * 16u < p.V ? min(16u, p.V - tile * 16u) : 0u;
-        if (!nv) v = head * p.V;
+        tile = unit % parts * TEAM + wave % TEAM;
+        nv = tile * 16u < cols ? min(16u, cols - tile * 16u) : 0u;
+        v = head * cols + (nv ? tile * 16u : 0u);
+        D = (size_t)p.H * cols;
     }
     __device__ __forceinline__ unsigned row(int r) const { return mm16<A>::row(g, r); }
 };
@@ -160,7 +162,7 @@ template <typename F> inline void with_key_tiles(size_t K, F f)
 
 // Keys of more than 32 columns fill the LDS: there a team is always the whole workgroup, also where some of its waves have no tile and only help to fetch.
 inline int team_of(size_t K, size_t tiles) { return K > 32 || tiles > 2 ? 4 : (int)tiles; }
-inline unsigned team_blocks(const delta_shape& p, size_t tiles) { return divup((size_t)p.H * ((tiles + 3) / 4), 4u / team_of(p.K, tiles)); }
+inline unsigned team_blocks(const delta_shape& p, size_t team, size_t cols) { return divup((size_t)p.H * (((cols + 15) / 16 + team - 1) / team), 4u / team); }
 template <typename F> inline void with_team(size_t K, size_t tiles, F f)
 {
     auto pass = [&](auto kt) {
@@ -194,8 +196,8 @@ template <typename A, int W> __device__ __forceinline__ typename mm16<A>::vec ti
     return f;
 }
 
-// Waves per SIMD that the walks are compiled for: their registers hold 4 values per lane of a state's every 16 rows.
-template <typename A, int KT> constexpr int delta_waves() { return sizeof(A) == 4 ? (KT <= 4 ? 4 : 2) : KT <= 4 ? 2 : 1; }
+// Waves per SIMD that the walks are compiled for: their registers hold 4 values per lane of a state's every 16 rows. (Four teams of 32-column keys fill half the LDS.)
+template <typename A, int KT, int TEAM> constexpr int delta_waves() { return sizeof(A) == 4 ? (KT > 4 || (KT == 2 && TEAM == 1) ? 2 : 4) : KT > 4 || (KT == 2 && TEAM == 1) ? 1 : 2; }
 
 // Their way there: a thread's vectors come while the chunk before is worked on (fetch), and are put into LDS when it is done (put).
 template <typename T, int KT, int TEAM> struct delta_feed {
@@ -315,33 +317,42 @@ template <typename A> __device__ __forceinline__ typename mm16<A>::vec by_row(co
 // A wave's columns of states (blocks of K x (H V)): tile t holds rows 16 t + row(g, r).
 template <typename A, int KT, int TEAM> __device__ __forceinline__ void load_state(typename mm16<A>::vec (&S)[KT], const A* p, const delta_shape& s, const delta_lane<A, TEAM>& l)
 {
-    const size_t D = (size_t)s.H * s.V;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const unsigned k = 16u * t + l.row(r);
-            S[t][r] = p && k < s.K && l.c < l.nv ? p[k * D + l.v + l.c] : A(0);
+            S[t][r] = p && k < s.K && l.c < l.nv ? p[k * l.D + l.v + l.c] : A(0);
         }
 }
 template <typename A, int KT, int TEAM> __device__ __forceinline__ void store_state(const typename mm16<A>::vec (&S)[KT], A* p, const delta_shape& s, const delta_lane<A, TEAM>& l)
 {
-    const size_t D = (size_t)s.H * s.V;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const unsigned k = 16u * t + l.row(r);
-            if (k < s.K && l.c < l.nv) p[k * D + l.v + l.c] = S[t][r];
+            if (k < s.K && l.c < l.nv) p[k * l.D + l.v + l.c] = S[t][r];
         }
 }
 
 // Defined in deltarule.hip.
 delta_shape delta_shape_of(const dbk_deltarule_args& a);
 int check_delta(const dbk_deltarule_args* a);
-int delta_mark(hipStream_t st, const delta_shape& s, const uint32_t* regions, uint32_t* marks);
+int delta_mark(hipStream_t st, const delta_shape& s, const uint32_t* regions, uint32_t* marks, uint32_t* cuts);
 // chunks, and pairs where it is not null, of every block and head
 void delta_prepare(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const uint32_t* marks, void* chunks, void* pairs);
+// What regions cut into segments need, in the workspace: whose segment a slot holds, and in front of every segment but a region's first the state (or its gradient) there.
+// Transitions (H, K, K), by which a segment takes what is in front of it to its end, lie behind the kept states, or in the workspace where none are kept.
+struct delta_cuts {
+    uint32_t* marks;
+    char* carry;
+    char* through;
+};
+void delta_carry(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const delta_cuts& w, bool backward);
+// values (not bytes) of the kept states, behind which the transitions lie
+inline size_t delta_kept(const delta_shape& s) { return (size_t)s.slots * s.K * s.H * s.V; }
+inline size_t delta_through(const delta_shape& s) { return (size_t)s.cuts * s.H * s.K * s.K; }
 inline size_t delta_blocks(const delta_shape& s) { return (size_t)s.nregion + s.slots; }
 inline size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 

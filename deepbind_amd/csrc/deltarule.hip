@@ -3,12 +3,14 @@
 
 namespace dbk {
 
-__global__ __launch_bounds__(256) void k_delta_mark(delta_shape p, const uint32_t* __restrict__ regions, uint32_t* __restrict__ marks)
+__global__ __launch_bounds__(256) void k_delta_mark(delta_shape p, const uint32_t* __restrict__ regions, uint32_t* __restrict__ marks, uint32_t* __restrict__ cuts)
 {
     // a wave per region
     const unsigned r = blockIdx.x * 4u + (threadIdx.x >> 6);
     if (r >= p.nregion) return;
-    mark_segments(marks, r, region_rows(regions, r, p.N), DELTA_BLOCK, threadIdx.x & 63u, 64u);
+    const row_range g = region_rows(regions, r, p.N);
+    mark_segments(marks, r, g, DELTA_BLOCK, threadIdx.x & 63u, 64u);
+    if (p.L) mark_segments(cuts, r, g, p.L, threadIdx.x & 63u, 64u);
 }
 
 // A chunk's matrices. A wave takes a block of a head, four chunks: the products of its keys and queries on the matrix cores, then a lane per chunk and column for the
@@ -95,11 +97,12 @@ __global__ __launch_bounds__(256) void k_delta_prepare(delta_shape p, const uint
     }
 }
 
-// Walks a wave's 16 columns of a head's state down `rows` rows from `row` on. number(k): the number of the block k blocks on from the first.
-// Keys, queries, matrices and values of a chunk come while the one before it is worked on.
-template <typename T, int KT, int TEAM, typename NUMBER>
+// Walks a wave's 16 columns of a head's state down `rows` rows from `row` on, of a region that starts at `first`. number(k): the number of the block k blocks on from the first.
+// Keys, queries, matrices and values of a chunk come while the one before it is worked on. OUT: rows of O are written; otherwise only the state moves on. V null:
+// without values, for what becomes of the state alone.
+template <typename T, int KT, int TEAM, bool OUT, typename NUMBER>
 __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, delta_rows<typename acc_of<T>::type, KT>* lds, const T* Q, const T* K,
-                                           const T* V, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, size_t row, unsigned rows, NUMBER number,
+                                           const T* V, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, size_t first, size_t row, unsigned rows, NUMBER number,
                                            typename mm16<typename acc_of<T>::type>::vec (&S)[KT], T* O, typename acc_of<T>::type* keep, size_t kept)
 {
     typedef typename acc_of<T>::type A;
@@ -114,7 +117,7 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
     T next[4];
     auto values = [&](unsigned t) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) next[r] = l.row(r) < rows - t && l.c < l.nv ? v[(t + l.row(r)) * p.ldv] : (T)A(0);
+        for (int r = 0; r < 4; ++r) next[r] = V && l.row(r) < rows - t && l.c < l.nv ? v[(t + l.row(r)) * p.ldv] : (T)A(0);
     };
     fetch(0u);
     values(0u);
@@ -133,12 +136,13 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
         }
         if (t + 2u * DELTA_CHUNK < rows) fetch(t + 2u * DELTA_CHUNK);
         if (l.nv) {
-            if (keep && t && t % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + (kept + t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
+            if (keep && (t || row != first) && t % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + (kept + t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
             vec w = zero16<A>(), z = zero16<A>();
 #pragma unroll
             for (int i = 0; i < KT; ++i) w = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], w);
+            if (OUT)
 #pragma unroll
-            for (int i = 0; i < KT; ++i) z = product<A>(tile_by_rows(here.q, i, l.g, l.c), S[i], z);
+                for (int i = 0; i < KT; ++i) z = product<A>(tile_by_rows(here.q, i, l.g, l.c), S[i], z);
             const vec first = by_row(here.c.first, l.g), b = by_row(here.c.b, l.g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[r] = l.row(r) < n ? b[r] * (x[r] - first[r] * w[r]) : A(0);
@@ -147,33 +151,121 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
             const A through = here.c.first[15];
 #pragma unroll
             for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.k, i, l.g, l.c), sent, through * S[i]);
-            const vec y = triangle<A, true>(matrix_by_rows(here.c.P, l.g, l.c), u, first * z, l.g);
+            if (OUT) {
+                const vec y = triangle<A, true>(matrix_by_rows(here.c.P, l.g, l.c), u, first * z, l.g);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (l.row(r) < n && l.c < l.nv) o[(size_t)(t + l.row(r)) * p.ldo] = (T)(scale * y[r]);
+                for (int r = 0; r < 4; ++r)
+                    if (l.row(r) < n && l.c < l.nv) o[(size_t)(t + l.row(r)) * p.ldo] = (T)(scale * y[r]);
+            }
         }
         __syncthreads();
     }
 }
 
+// Workgroups below nregion: a region, or the first segment of a cut one; the others: the segment of their slot, from the state carried there.
 template <typename T, int KT, int TEAM>
-__global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT>())) void k_delta_fprop(delta_shape p, const uint32_t* __restrict__ regions, const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
+__global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEAM>())) void k_delta_fprop(delta_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ cuts,
+                                                     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
                                                      const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, typename acc_of<T>::type scale,
-                                                     const typename acc_of<T>::type* __restrict__ state, T* __restrict__ O, typename acc_of<T>::type* __restrict__ last,
-                                                     typename acc_of<T>::type* __restrict__ keep)
+                                                     const typename acc_of<T>::type* __restrict__ state, const typename acc_of<T>::type* __restrict__ carry, T* __restrict__ O,
+                                                     typename acc_of<T>::type* __restrict__ last, typename acc_of<T>::type* __restrict__ keep)
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
     __shared__ delta_rows<A, KT> lds[4 / TEAM][2];
+    const size_t block = (size_t)p.K * p.H * p.V;
+    unsigned r = blockIdx.x, k = 0;
+    row_range g;
+    const A* from = nullptr;
+    if (r < p.nregion) {
+        g = region_rows(regions, r, p.N);
+        if (state) from = state + r * block;
+    } else {
+        const unsigned slot = r - p.nregion;
+        if (!slot_segment(regions, p.nregion, p.N, cuts, slot, p.L, r, g, k)) return;
+        from = carry + slot * block;
+    }
     delta_lane<A, TEAM> l;
-    l.place(p, p.ns);
+    l.place(p, blockIdx.y, p.V);
+    const unsigned start = g.start + k * p.L, rows = p.L && g.end - start > p.L ? p.L : g.end - start;
+    vec S[KT];
+    load_state<A, KT>(S, from, p, l);
+    const unsigned before = k * (p.L / DELTA_BLOCK);
+    delta_walk<T, KT, TEAM, true>(p, l, lds[l.team], Q, K, V, chunks, scale, g.start, start, rows, [&](unsigned i) { return block_number(p, r, g, before + i); }, S, O, keep, kept_number(g, before));
+    if (last && start + rows == g.end) store_state<A, KT>(S, last + r * block, p, l);
+}
+
+// What the segment in front of a slot's hands on: its state, from the region's own initial one (the first) or from zeros, and (the others) how it takes the
+// state in front of it to its end: the states that the unit vectors become. Workgroups from `values` on along y take those.
+template <typename T, int KT, int TEAM>
+__global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEAM>())) void k_delta_local(delta_shape p, unsigned values, const uint32_t* __restrict__ regions,
+                                                     const uint32_t* __restrict__ cuts, const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
+                                                     const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, const typename acc_of<T>::type* __restrict__ state,
+                                                     typename acc_of<T>::type* __restrict__ carry, typename acc_of<T>::type* __restrict__ through)
+{
+    typedef typename acc_of<T>::type A;
+    typedef typename mm16<A>::vec vec;
+    __shared__ delta_rows<A, KT> lds[4 / TEAM][2];
+    const unsigned slot = blockIdx.x;
+    unsigned r, k;
+    row_range g;
+    if (!slot_segment(regions, p.nregion, p.N, cuts, slot, p.L, r, g, k)) return;
+    const bool unit = blockIdx.y >= values;
+    if (unit && k == 1u) return;
+    delta_lane<A, TEAM> l;
+    l.place(p, unit ? blockIdx.y - values : blockIdx.y, unit ? p.K : p.V);
+    vec S[KT];
+    if (unit) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S[t][i] = 16u * t + l.row(i) == 16u * l.tile + l.c && l.nv ? A(1) : A(0);
+    } else
+        load_state<A, KT>(S, state && k == 1u ? state + (size_t)r * p.K * p.H * p.V : (const A*)nullptr, p, l);
+    const unsigned before = (k - 1u) * (p.L / DELTA_BLOCK);
+    delta_walk<T, KT, TEAM, false>(p, l, lds[l.team], Q, K, unit ? (const T*)nullptr : V, chunks, A(1), g.start, g.start + (k - 1u) * p.L, p.L,
+                                   [&](unsigned i) { return block_number(p, r, g, before + i); }, S, (T*)nullptr, (A*)nullptr, 0);
+    store_state<A, KT>(S, unit ? through + slot * ((size_t)p.K * p.H * p.K) : carry + slot * ((size_t)p.K * p.H * p.V), p, l);
+}
+
+// From segment to segment: what is in front of slot k + 1 is what its own segment made of zeros and what the transition makes of what is in front of slot k; backward
+// from the last segment to the first with the transposed transitions. A wave takes 16 columns of a head.
+template <typename A, int KT>
+__global__ __launch_bounds__(256) void k_delta_carry(delta_shape p, bool backward, const uint32_t* __restrict__ regions, A* __restrict__ carry, const A* __restrict__ through)
+{
+    typedef typename mm16<A>::vec vec;
     const unsigned r = blockIdx.x;
     const row_range g = region_rows(regions, r, p.N);
-    const size_t block = (size_t)p.K * p.H * p.V;
+    if (g.end - g.start <= 2u * p.L) return;     // (two segments: nothing to carry over one)
+    delta_lane<A, 4> l;
+    l.place(p, blockIdx.y, p.V);
+    if (!l.nv) return;
+    const unsigned n = (g.end - g.start + p.L - 1u) / p.L;      // segments; slots first + 1 .. first + n - 1
+    const size_t first = g.start / p.L, block = (size_t)p.K * p.H * p.V, D = (size_t)p.H * p.K;
     vec S[KT];
-    load_state<A, KT>(S, state ? state + r * block : (const A*)nullptr, p, l);
-    delta_walk<T, KT, TEAM>(p, l, lds[l.team], Q, K, V, chunks, scale, g.start, g.end - g.start, [&](unsigned k) { return block_number(p, r, g, k); }, S, O, keep, kept_number(g, 0u));
-    if (last) store_state<A, KT>(S, last + r * block, p, l);
+    load_state<A, KT>(S, carry + (first + (backward ? n - 1u : 1u)) * block, p, l);
+    for (unsigned i = 2; i < n; ++i) {
+        // forward: slot i from slot i - 1 by the transition of segment i - 1, which lies in slot i. Backward: slot n - i from slot n - i + 1 by that of segment n - i, in slot n - i + 1
+        const size_t to = first + (backward ? n - i : i), by = first + (backward ? n - i + 1u : i);
+        const A* m = through + by * ((size_t)p.K * D) + (size_t)l.head * p.K;
+        vec N[KT];
+        load_state<A, KT>(N, carry + to * block, p, l);
+#pragma unroll
+        for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int s = 0; s < KT; ++s) {
+                vec a;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned row = 16u * t + l.c, col = 16u * s + l.row(j);
+                    a[j] = row < p.K && col < p.K ? backward ? m[col * D + row] : m[row * D + col] : A(0);
+                }
+                N[t] = product<A>(a, S[s], N[t]);
+            }
+#pragma unroll
+        for (int t = 0; t < KT; ++t) S[t] = N[t];
+        store_state<A, KT>(S, carry + to * block, p, l);
+    }
 }
 
 // One row of each sequence. A workgroup takes 64 columns of a head's state, a thread VEC neighbouring ones of RPT rows of it; what key and query find is added over the
@@ -248,6 +340,8 @@ __global__ __launch_bounds__(256) void k_delta_step(delta_shape p, const T* __re
     }
 }
 
+constexpr size_t DELTA_WAVES = 2048, DELTA_LEAST = 256;
+
 delta_shape delta_shape_of(const dbk_deltarule_args& a)
 {
     delta_shape s = {};
@@ -259,6 +353,11 @@ delta_shape delta_shape_of(const dbk_deltarule_args& a)
     s.V = (unsigned)a.V;
     s.ns = divup(a.V, 16);
     s.slots = (unsigned)segment_slots(a.N, DELTA_BLOCK);
+    // An even share of all rows for each of DELTA_WAVES waves: a region of more is cut. A segment's rows are walked twice, and its transition costs as much again as K columns
+    // of values, so that fewer, longer regions than fill the chip are what is cut.
+    const size_t share = (a.N * a.H * s.ns + DELTA_WAVES - 1) / DELTA_WAVES, L = ((share > DELTA_LEAST ? share : DELTA_LEAST) + DELTA_BLOCK - 1) / DELTA_BLOCK * DELTA_BLOCK;
+    s.L = L < a.N ? (unsigned)L : 0u;
+    s.cuts = s.L ? (unsigned)segment_slots(a.N, s.L) : 0u;
     s.ldq = a.ldq;
     s.ldk = a.ldk;
     s.ldv = a.ldv;
@@ -268,7 +367,7 @@ delta_shape delta_shape_of(const dbk_deltarule_args& a)
     return s;
 }
 
-int check_delta(const dbk_deltarule_args* a)
+static int check_delta_shape(const dbk_deltarule_args* a)
 {
     DBK_CHECK(a, "ValueError: null arguments");
     DBK_ROW_DTYPE_OK(a->dtype);
@@ -276,16 +375,34 @@ int check_delta(const dbk_deltarule_args* a)
     DBK_CHECK(a->K >= 1 && a->K <= DELTA_KEY, "NotImplementedError: keys of 1 to %zu columns, got %zu", DELTA_KEY, a->K);
     DBK_CHECK(a->N < (size_t(1) << 31) && a->V < (size_t(1) << 20) && a->H < (size_t(1) << 20) && a->H * ((a->V + 15) / 16) <= 65535, "ValueError: map too large (%zu rows, %zu heads of %zu columns)", a->N, a->H, a->V);
     DBK_CHECK(a->nregion < (size_t(1) << 24), "ValueError: too many regions (%zu)", a->nregion);
+    return 0;
+}
+
+int check_delta(const dbk_deltarule_args* a)
+{
+    if (int rc = check_delta_shape(a)) return rc;
     DBK_CHECK(!a->N || !a->V || (a->Q && a->Kk && a->Vv && a->beta), "ValueError: null matrix");
     DBK_CHECK(a->N <= 1 || (a->ldq >= a->G * a->K && a->ldk >= a->G * a->K && a->ldv >= a->H * a->V && a->ldbeta >= a->H && (!a->decay || a->lddecay >= a->H)),
               "ValueError: row strides must be at least the number of columns");
     return 0;
 }
 
-int delta_mark(hipStream_t st, const delta_shape& s, const uint32_t* regions, uint32_t* marks)
+int delta_mark(hipStream_t st, const delta_shape& s, const uint32_t* regions, uint32_t* marks, uint32_t* cuts)
 {
-    k_delta_mark<<<divup(s.nregion, 4), 256, 0, st>>>(s, regions, marks);
+    k_delta_mark<<<divup(s.nregion, 4), 256, 0, st>>>(s, regions, marks, cuts);
     return 0;
+}
+
+void delta_carry(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const delta_cuts& w, bool backward)
+{
+    auto launch = [&](auto t) {
+        typedef decltype(t) A;
+        with_key_tiles(a.K, [&](auto kt) {
+            k_delta_carry<A, kt.value><<<dim3(s.nregion, team_blocks(s, 4, s.V)), 256, 0, st>>>(s, backward, a.regions, (A*)w.carry, (const A*)w.through);
+        });
+    };
+    if (a.dtype == DBK_F64) launch(double());
+    else launch(float());
 }
 
 void delta_prepare(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const uint32_t* marks, void* chunks, void* pairs)
@@ -306,6 +423,7 @@ namespace {
 struct delta_work {
     uint32_t* marks;
     char* chunks;
+    delta_cuts cuts;
     size_t bytes;
 };
 delta_work work_in(void* work, const dbk_deltarule_args& a, const delta_shape& s)
@@ -317,6 +435,14 @@ delta_work work_in(void* work, const dbk_deltarule_args& a, const delta_shape& s
     at += align16(s.slots * sizeof(uint32_t));
     w.chunks = p + at;
     at += delta_blocks(s) * a.H * DELTA_CHUNKS * (a.dtype == DBK_F64 ? sizeof(delta_chunk<double>) : sizeof(delta_chunk<float>));
+    const size_t A = acc_size(a.dtype);
+    at = align16(at);
+    w.cuts.marks = (uint32_t*)(p + at);
+    at += align16(s.cuts * sizeof(uint32_t));
+    w.cuts.carry = p + at;
+    at += align16((size_t)s.cuts * s.K * s.H * s.V * A);
+    w.cuts.through = a.keep ? (char*)a.keep + delta_kept(s) * A : p + at;
+    at += delta_through(s) * A;
     w.bytes = at;
     return w;
 }
@@ -340,6 +466,16 @@ int dbk_deltarule_workspace(const dbk_deltarule_args* a, int backward, size_t* w
     return 0;
 }
 
+int dbk_deltarule_kept(const dbk_deltarule_args* a, size_t* values)
+{
+    if (int rc = check_delta_shape(a)) return rc;
+    DBK_CHECK(values, "ValueError: null result");
+    const delta_shape s = delta_shape_of(*a);
+    *values = delta_kept(s) + delta_through(s);
+    clear_error();
+    return 0;
+}
+
 int dbk_deltarule(dbk_stream_t stream, const dbk_deltarule_args* a, void* work, size_t work_bytes)
 {
     if (int rc = check_delta(a)) return rc;
@@ -354,15 +490,23 @@ int dbk_deltarule(dbk_stream_t stream, const dbk_deltarule_args* a, void* work, 
     DBK_CHECK(grid_fits(delta_blocks(s), 256), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
     hipStream_t st = as_stream(stream);
     if (a->N) {
-        delta_mark(st, s, a->regions, w.marks);
+        delta_mark(st, s, a->regions, w.marks, w.cuts.marks);
         delta_prepare(st, *a, s, w.marks, w.chunks, nullptr);
     }
     with_row_type(a->dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
         with_team(a->K, s.ns, [&](auto kt, auto team) {
-            k_delta_fprop<T, kt.value, team.value><<<dim3(s.nregion, team_blocks(s, s.ns)), 256, 0, st>>>(
-                s, a->regions, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const delta_chunk<A>*)w.chunks, (A)a->scale, (const A*)a->state, (T*)a->O, (A*)a->last, (A*)a->keep);
+            if (s.L) {
+                const unsigned values = team_blocks(s, team.value, s.V);
+                k_delta_local<T, kt.value, team.value><<<dim3(s.cuts, values + team_blocks(s, team.value, s.K)), 256, 0, st>>>(
+                    s, values, a->regions, w.cuts.marks, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const delta_chunk<A>*)w.chunks, (const A*)a->state, (A*)w.cuts.carry,
+                    (A*)w.cuts.through);
+                delta_carry(st, *a, s, w.cuts, false);
+            }
+            k_delta_fprop<T, kt.value, team.value><<<dim3(s.nregion + s.cuts, team_blocks(s, team.value, s.V)), 256, 0, st>>>(
+                s, a->regions, w.cuts.marks, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const delta_chunk<A>*)w.chunks, (A)a->scale, (const A*)a->state, (const A*)w.cuts.carry, (T*)a->O,
+                (A*)a->last, (A*)a->keep);
         });
     });
     DBK_LAUNCH_OK();

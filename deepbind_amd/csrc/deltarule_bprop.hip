@@ -20,49 +20,42 @@
 
 namespace dbk {
 
-// dS of a chunk's start from that of its end, chunk after chunk up the region. What a chunk needs comes while the one behind it is worked on.
-template <typename T, int KT, int TEAM>
-__global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT>())) void k_delta_chain(delta_shape p, size_t lddo, const uint32_t* __restrict__ regions, const T* __restrict__ Q, const T* __restrict__ K,
-                                                     const T* __restrict__ dO, const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, typename acc_of<T>::type scale,
-                                                     typename acc_of<T>::type* __restrict__ dstates)
+// dS of a chunk's start from that of its end, chunk after chunk up `rows` rows from the last one down to row `stop` of them. What a chunk needs comes while the one
+// behind it is worked on. dstates: where the gradients in front of the blocks' first rows go, from this piece's first block on; null: nowhere.
+template <typename T, int KT, int TEAM, typename NUMBER>
+__device__ __forceinline__ void delta_walk_back(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, delta_rows<typename acc_of<T>::type, KT>* lds, size_t lddo, const T* Q,
+                                                const T* K, const T* dO, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, size_t row, unsigned rows,
+                                                unsigned stop, NUMBER number, typename mm16<typename acc_of<T>::type>::vec (&S)[KT], typename acc_of<T>::type* dstates)
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
-    __shared__ delta_rows<A, KT> lds_all[4 / TEAM][2];
-    delta_lane<A, TEAM> l;
-    l.place(p, p.ns);
-    delta_rows<A, KT>* lds = lds_all[l.team];
-    const unsigned r = blockIdx.x;
-    const row_range g = region_rows(regions, r, p.N);
-    const unsigned rows = g.end - g.start;
-    if (rows <= DELTA_BLOCK) return;
-    const T *q = Q + (size_t)g.start * p.ldq + (size_t)l.group * p.K, *k = K + (size_t)g.start * p.ldk + (size_t)l.group * p.K, *d0 = dO + (size_t)g.start * lddo + l.v + l.c;
+    if (rows <= stop) return;
+    const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K, *d0 = dO + row * lddo + l.v + l.c;
     delta_feed<T, KT, TEAM> feed;
     auto fetch = [&](unsigned t) {
-        feed.fetch(p, q + t * p.ldq, k + t * p.ldk, chunks[(block_number(p, r, g, t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS], l.thread, rows - t);
+        feed.fetch(p, q + t * p.ldq, k + t * p.ldk, chunks[(number(t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS], l.thread, rows - t);
     };
     T next[4];
     auto values = [&](unsigned t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) next[i] = l.row(i) < rows - t && l.c < l.nv ? d0[(t + l.row(i)) * lddo] : (T)A(0);
     };
-    vec S[KT];
-#pragma unroll
-    for (int i = 0; i < KT; ++i) S[i] = zero16<A>();
     const unsigned end = (rows - 1) / DELTA_CHUNK * DELTA_CHUNK;
     fetch(end);
     values(end);
     feed.put(lds[end / DELTA_CHUNK & 1u], l.thread);
-    fetch(end - DELTA_CHUNK);                    // (there are more than four chunks)
+    if (end > stop) fetch(end - DELTA_CHUNK);
     __syncthreads();
-    for (unsigned t = end; t >= DELTA_BLOCK; t -= DELTA_CHUNK) {
+    for (unsigned left = (end - stop) / DELTA_CHUNK + 1u, t = end; left > 0; --left, t -= DELTA_CHUNK) {
         const delta_rows<A, KT>& here = lds[t / DELTA_CHUNK & 1u];
         vec d;
 #pragma unroll
         for (int i = 0; i < 4; ++i) d[i] = scale * (A)next[i];
-        feed.put(lds[~(t / DELTA_CHUNK) & 1u], l.thread);
-        values(t - DELTA_CHUNK);
-        fetch(t - 2u * DELTA_CHUNK);
+        if (left > 1u) {
+            feed.put(lds[~(t / DELTA_CHUNK) & 1u], l.thread);
+            values(t - DELTA_CHUNK);
+        }
+        if (left > 2u) fetch(t - 2u * DELTA_CHUNK);
         if (l.nv) {
             vec y = zero16<A>();
 #pragma unroll
@@ -77,21 +70,73 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT>()))
             const vec dw = -(first * (by_row(here.c.b, l.g) * dy));
 #pragma unroll
             for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.k, i, l.g, l.c), dw, S[i]);
-            if (t % DELTA_BLOCK == 0) store_state<A, KT>(S, dstates + kept_number(g, t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
+            if (dstates && t % DELTA_BLOCK == 0) store_state<A, KT>(S, dstates + (size_t)(t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
         }
         __syncthreads();
     }
 }
 
+// Workgroups below nregion: a region, or the first segment of a cut one, down to its second block; the others: the segment of their slot, from the gradient carried to
+// its end. In front of every block but a region's first the gradient is left behind.
+template <typename T, int KT, int TEAM>
+__global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEAM>())) void k_delta_chain(delta_shape p, size_t lddo, const uint32_t* __restrict__ regions,
+                                                     const uint32_t* __restrict__ cuts, const T* __restrict__ Q, const T* __restrict__ K,
+                                                     const T* __restrict__ dO, const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, typename acc_of<T>::type scale,
+                                                     const typename acc_of<T>::type* __restrict__ carry, typename acc_of<T>::type* __restrict__ dstates)
+{
+    typedef typename acc_of<T>::type A;
+    typedef typename mm16<A>::vec vec;
+    __shared__ delta_rows<A, KT> lds[4 / TEAM][2];
+    unsigned r = blockIdx.x, k = 0;
+    row_range g;
+    if (r < p.nregion) {
+        g = region_rows(regions, r, p.N);
+        if (g.end - g.start <= DELTA_BLOCK) return;
+    } else if (!slot_segment(regions, p.nregion, p.N, cuts, r - p.nregion, p.L, r, g, k))
+        return;
+    delta_lane<A, TEAM> l;
+    l.place(p, blockIdx.y, p.V);
+    const size_t block = (size_t)p.K * p.H * p.V;
+    const unsigned start = g.start + k * p.L;
+    const bool more = p.L && g.end - start > p.L;
+    vec S[KT];
+    load_state<A, KT>(S, more ? carry + ((size_t)g.start / p.L + k + 1u) * block : (const A*)nullptr, p, l);
+    const unsigned before = k * (p.L / DELTA_BLOCK);
+    delta_walk_back<T, KT, TEAM>(p, l, lds[l.team], lddo, Q, K, dO, chunks, scale, start, more ? p.L : g.end - start, k ? 0u : DELTA_BLOCK, [&](unsigned i) { return block_number(p, r, g, before + i); },
+                                 S, dstates + kept_number(g, before) * block);
+}
+
+// What a slot's segment makes of a gradient of zeros behind it
+template <typename T, int KT, int TEAM>
+__global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEAM>())) void k_delta_chain_local(delta_shape p, size_t lddo, const uint32_t* __restrict__ regions,
+                                                     const uint32_t* __restrict__ cuts, const T* __restrict__ Q, const T* __restrict__ K,
+                                                     const T* __restrict__ dO, const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, typename acc_of<T>::type scale,
+                                                     typename acc_of<T>::type* __restrict__ carry)
+{
+    typedef typename acc_of<T>::type A;
+    typedef typename mm16<A>::vec vec;
+    __shared__ delta_rows<A, KT> lds[4 / TEAM][2];
+    unsigned r, k;
+    row_range g;
+    if (!slot_segment(regions, p.nregion, p.N, cuts, blockIdx.x, p.L, r, g, k)) return;
+    delta_lane<A, TEAM> l;
+    l.place(p, blockIdx.y, p.V);
+    const unsigned start = g.start + k * p.L, before = k * (p.L / DELTA_BLOCK);
+    vec S[KT];
+#pragma unroll
+    for (int i = 0; i < KT; ++i) S[i] = zero16<A>();
+    delta_walk_back<T, KT, TEAM>(p, l, lds[l.team], lddo, Q, K, dO, chunks, scale, start, min(g.end - start, p.L), 0u, [&](unsigned i) { return block_number(p, r, g, before + i); }, S, (A*)nullptr);
+    store_state<A, KT>(S, carry + blockIdx.x * ((size_t)p.K * p.H * p.V), p, l);
+}
+
 // transposed states: tile t holds [row(g, r)][16 t + c] of the wave's 16 columns by K
 template <typename A, int KT, int TEAM> __device__ __forceinline__ void load_state_t(typename mm16<A>::vec (&S)[KT], const A* p, const delta_shape& s, const delta_lane<A, TEAM>& l)
 {
-    const size_t D = (size_t)s.H * s.V;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
         const unsigned k = 16u * t + l.c;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) S[t][r] = p && k < s.K && l.row(r) < l.nv ? p[k * D + l.v + l.row(r)] : A(0);
+        for (int r = 0; r < 4; ++r) S[t][r] = p && k < s.K && l.row(r) < l.nv ? p[k * l.D + l.v + l.row(r)] : A(0);
     }
 }
 
@@ -150,7 +195,7 @@ __global__ __launch_bounds__(256) void k_delta_bprop(delta_shape p, size_t lddo,
     const unsigned unit = min((blockIdx.y * 4u + wave) / out.waves, p.H * out.parts - 1u), part = unit % out.parts;      // (a unit too many does the last one again)
     const unsigned tile = part * 4u + slice;
     delta_lane<A, 4> l;
-    l.place(p, p.ns);
+    l.place(p, 0u, p.V);
     l.head = unit / out.parts;
     l.group = l.head / (p.H / p.G);
     l.nv = tile < p.ns ? min(16u, p.V - tile * 16u) : 0u;
@@ -389,6 +434,7 @@ struct delta_bprop_work {
     uint32_t* marks;
     char *chunks, *pairs, *dstates, *dq, *dk, *db, *dg;
     unsigned parts, waves;
+    delta_cuts cuts;
     size_t bytes;
 };
 
@@ -414,6 +460,9 @@ delta_bprop_work bprop_work_in(void* work, const dbk_deltarule_args& a, const de
         w.db = take((size_t)w.parts * a.N * a.H * A);
         w.dg = take((size_t)w.parts * a.N * a.H * A);
     }
+    w.cuts.marks = (uint32_t*)take(s.cuts * sizeof(uint32_t));
+    w.cuts.carry = take((size_t)s.cuts * s.K * s.H * s.V * A);
+    w.cuts.through = (char*)a.keep + delta_kept(s) * A;
     w.bytes = at;
     return w;
 }
@@ -443,7 +492,7 @@ int dbk_deltarule_bprop(dbk_stream_t stream, const dbk_deltarule_args* a, void* 
     DBK_CHECK(work && work_bytes >= w.bytes, "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, w.bytes);
     DBK_CHECK(grid_fits(delta_blocks(s), 256), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
     hipStream_t st = as_stream(stream);
-    delta_mark(st, s, a->regions, w.marks);
+    delta_mark(st, s, a->regions, w.marks, w.cuts.marks);
     delta_prepare(st, *a, s, w.marks, w.chunks, w.pairs);
     int rc = 0;
     with_row_type(a->dtype, [&](auto t) {
@@ -452,8 +501,14 @@ int dbk_deltarule_bprop(dbk_stream_t stream, const dbk_deltarule_args* a, void* 
         delta_grads<T> out = {(T*)a->dQ, (T*)a->dK, (T*)a->dV, (A*)a->dbeta, (A*)a->ddecay, a->lddq, a->lddk, a->lddv, a->lddbeta, a->ldddecay,
                               (A*)w.dq, (A*)w.dk, (A*)w.db, a->ddecay ? (A*)w.dg : nullptr, w.parts, w.waves};
         with_team(a->K, s.ns, [&](auto kt, auto team) {
-            k_delta_chain<T, kt.value, team.value><<<dim3(s.nregion, team_blocks(s, s.ns)), 256, 0, st>>>(s, a->lddo, a->regions, (const T*)a->Q, (const T*)a->Kk, (const T*)a->dO,
-                                                                                                         (const delta_chunk<A>*)w.chunks, (A)a->scale, (A*)w.dstates);
+            const unsigned columns = team_blocks(s, team.value, s.V);
+            if (s.L) {
+                k_delta_chain_local<T, kt.value, team.value><<<dim3(s.cuts, columns), 256, 0, st>>>(
+                    s, a->lddo, a->regions, w.cuts.marks, (const T*)a->Q, (const T*)a->Kk, (const T*)a->dO, (const delta_chunk<A>*)w.chunks, (A)a->scale, (A*)w.cuts.carry);
+                delta_carry(st, *a, s, w.cuts, true);
+            }
+            k_delta_chain<T, kt.value, team.value><<<dim3(s.nregion + s.cuts, columns), 256, 0, st>>>(
+                s, a->lddo, a->regions, w.cuts.marks, (const T*)a->Q, (const T*)a->Kk, (const T*)a->dO, (const delta_chunk<A>*)w.chunks, (A)a->scale, (const A*)w.cuts.carry, (A*)w.dstates);
         });
         with_key_tiles(a->K, [&](auto kt) {
             constexpr size_t lds = 4 * sizeof(delta_share<A, kt.value>);

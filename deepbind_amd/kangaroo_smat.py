@@ -476,10 +476,17 @@ def _delta_shape(K, V, beta, groups):
     return H, G, K.shape[1] // G, V.shape[1] // H
 
 
+def _kept_values(code, N, H, G, key, value):
+    a, need = _lib.DeltaRuleArgs(code, N, H, G, key, value), ctypes.c_size_t(0)
+    call("dbk_deltarule_kept", ctypes.addressof(a), ctypes.addressof(need))
+    return need.value
+
+
 def kept_delta(K, V, beta, groups=None):
-    """Empty buffer for the states that deltarule keeps for deltarule_bprop: one block (key x heads*value) per 64 rows."""
-    _, _, key, _ = _delta_shape(K, V, beta, groups)
-    return torch.empty(((V.shape[0] + 63) // 64, key, V.shape[1]), dtype=_lib.wide_dtype(V), device=V.device)
+    """Empty buffer (1 x values) for what deltarule keeps for deltarule_bprop, for maps of these shapes: the states at every 64th row of a
+    region, and what takes them over the segments that long regions are cut into."""
+    H, G, key, value = _delta_shape(K, V, beta, groups)
+    return torch.empty((1, _kept_values(_lib.row_dtype_code(V), V.shape[0], H, G, key, value)), dtype=_lib.wide_dtype(V), device=V.device)
 
 
 def _delta_args(Q, K, V, beta, decay, groups, scale):
@@ -494,6 +501,11 @@ def _delta_args(Q, K, V, beta, decay, groups, scale):
     d, ldd = (None, 0) if decay is None else g.rows("decay", decay, rates, wide)
     scale = key ** -0.5 if scale is None else float(scale)
     return g, _lib.DeltaRuleArgs(code, N, H, G, key, value, None, 0, q, ldq, k, ldk, v, ldv, b, ldb, d, ldd, scale), wide, N, key, D
+
+
+def _delta_keep(g, a, keep, wide, out):
+    """The pointer of a buffer from kept_delta for a call's shapes."""
+    return None if keep is None else g.dense("keep", keep, (1, _kept_values(a.dtype, a.N, a.H, a.G, a.K, a.V)), wide, out=out)
 
 
 def deltarule(Q, K, V, beta, regions, decay=None, groups=None, scale=None, state=None, want_state=False, keep=None, out=None):
@@ -511,7 +523,7 @@ def deltarule(Q, K, V, beta, regions, decay=None, groups=None, scale=None, state
     P, a.regions = _row_regions(g, regions)
     a.nregion = P
     a.state = g.dense("state", state, (P, key, D), wide)
-    a.keep = g.dense("keep", keep, ((N + 63) // 64, key, D), wide, out=True)
+    a.keep = _delta_keep(g, a, keep, wide, True)
     require(keep is None or state is None, "ValueError: states are kept for the backward pass of whole sequences, which starts from zeros: no initial state")
     if out is not None:
         g.rows("out", out, (N, D), V.dtype, out=True)
@@ -537,7 +549,7 @@ def deltarule_bprop(Q, K, V, beta, regions, keep, dO, decay=None, groups=None, s
     P, a.regions = _row_regions(g, regions)
     a.nregion = P
     require(keep is not None, "ValueError: the states that the forward call kept are needed")
-    a.keep = g.dense("keep", keep, ((N + 63) // 64, key, D), wide)
+    a.keep = _delta_keep(g, a, keep, wide, False)
     a.dO, a.lddo = g.rows("dO", dO, (N, D), V.dtype)
     given = (None,) * 5 if out is None else tuple(out)
     require(len(given) == 5, "ValueError: out must be (dQ, dK, dV, dbeta, ddecay)")

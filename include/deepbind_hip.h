@@ -578,12 +578,13 @@ typedef struct dbk_deltarule_args {
     const void* state;                          /* (nregion, K, H * V): the states before the regions' first rows, may be NULL (zeros) */
     void* O; size_t ldo;                        /* (N, H * V) rows */
     void* last;                                 /* (nregion, K, H * V): the states behind the last rows, may be NULL */
-    void* keep;                                 /* forward: may be NULL; ceil(N / 64) blocks of (K, H * V): states that the backward pass starts from */
+    void* keep;                                 /* forward: may be NULL; dbk_deltarule_kept values, kept as weights are: what the backward pass starts from */
     const void* dO; size_t lddo;                /* from here on: backward only */
     void* dQ; size_t lddq; void* dK; size_t lddk; void* dV; size_t lddv;
     void* dbeta; size_t lddbeta; void* ddecay; size_t ldddecay;      /* ddecay may be NULL */
 } dbk_deltarule_args;
 int dbk_deltarule_args_size(void);              /* sizeof(dbk_deltarule_args) as the library was built */
+int dbk_deltarule_kept(const dbk_deltarule_args* args, size_t* values);     /* looks at dtype and sizes only */
 int dbk_deltarule_workspace(const dbk_deltarule_args* args, int backward, size_t* work_bytes);
 int dbk_deltarule(dbk_stream_t stream, const dbk_deltarule_args* args, void* work, size_t work_bytes);
 /* Backward for sequences that start from zero states; keep: as the forward call with the same inputs filled it. */

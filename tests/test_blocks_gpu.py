@@ -215,7 +215,7 @@ def test_delta_rule_of_nothing():
     O, last = ks.deltarule(z(0, 8), z(0, 8), z(0, 6), z(0, 2), R, state=state, want_state=True)
     assert O.shape == (0, 6) and torch.equal(last, state)
     keep = ks.kept_delta(z(0, 8), z(0, 6), z(0, 2))
-    assert keep.shape == (0, 4, 6)
+    assert keep.shape == (1, 0)
     grads = ks.deltarule_bprop(z(0, 8), z(0, 8), z(0, 6), z(0, 2), R, keep, z(0, 6))
     assert grads[0].shape == (0, 8) and grads[4] is None
     none, _ = ks.deltarule(z(5, 8), z(5, 8), z(5, 6), z(5, 2), regions([]).view(0, 2))

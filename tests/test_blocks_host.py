@@ -171,7 +171,7 @@ def test_restated_clipping_agrees_with_torch():
 def test_delta_rule_refusals():
     from deepbind_amd import kangaroo_smat as ks
     Q, V, b, R = torch.zeros(9, 10), torch.zeros(9, 12), torch.zeros(9, 4), torch.zeros(2, 2, dtype=torch.int32)
-    keep = torch.zeros(1, 5, 12)
+    keep = torch.zeros(1, 60)
     call = lambda *a, **k: ks.deltarule(*a, **dict(dict(groups=2), **k))  # noqa: E731
     _refused("divisible by the number of key heads", call, Q, Q, V, b, R, groups=3)
     _refused("K must be (rows x key heads", call, Q, torch.zeros(9, 11), V, b, R)
@@ -185,7 +185,7 @@ def test_delta_rule_refusals():
     _refused("regions must be uint32", call, Q, Q, V, b, R.long())
     _refused("state must be (2, 5, 12)", call, Q, Q, V, b, R, state=torch.zeros(2, 4, 12))
     _refused("state must be torch.float32", call, Q, Q, V, b, R, state=torch.zeros(2, 5, 12).bfloat16())
-    _refused("keep must be (1, 5, 12)", call, Q, Q, V, b, R, keep=torch.zeros(2, 5, 12))
+    _refused("keep must be (1, 60)", call, Q, Q, V, b, R, keep=torch.zeros(1, 5, 12))
     _refused("no initial state", call, Q, Q, V, b, R, keep=keep, state=torch.zeros(2, 5, 12))
     _refused("out must be a (9, 12) matrix", call, Q, Q, V, b, R, out=torch.zeros(9, 11))
     _refused("expected a device tensor", call, Q, Q, V, b, R)
@@ -196,7 +196,7 @@ def test_delta_rule_refusals():
     _refused("dbeta must be a (9, 4) matrix", ks.deltarule_bprop, Q, Q, V, b, R, keep, V, groups=2, out=(None, None, None, V, None))
     _refused("state is needed", ks.deltarule_step, Q, Q, V, b, None, groups=2)
     _refused("state must be (9, 5, 12)", ks.deltarule_step, Q, Q, V, b, torch.zeros(2, 5, 12), groups=2)
-    assert ks.kept_delta(Q, V, b, groups=2).shape == (1, 5, 12)
+    assert ks.kept_delta(Q, V, b, groups=2).shape == (1, 60)
 
 
 def test_block_norm_refusals():
