@@ -128,7 +128,7 @@ __device__ __forceinline__ size_t kept_number(row_range g, unsigned k) { return 
 
 // The waves that hold tiles of 16 columns of the same head are a team: 1, 2 or 4 of a workgroup's four (a head of more than 4 tiles has several), which share the head's keys and
 // queries. TEAM waves; of a workgroup, 4 / TEAM teams.
-template <typename A, int TEAM> struct delta_lane {
+template <typename A, int TEAM, int WAVES = 4> struct delta_lane {
     unsigned g, c, head, group, v;               // v: columns of V and O in front of the wave's
     unsigned nv;                                 // its columns: 16, fewer, or none
     unsigned team, thread;                       // of the workgroup's teams; of the team's threads
@@ -142,7 +142,7 @@ template <typename A, int TEAM> struct delta_lane {
         c = threadIdx.x & 15u;
         team = wave / TEAM;
         thread = threadIdx.x & (64u * TEAM - 1u);
-        unit = min(index * (4u / TEAM) + team, p.H * parts - 1u);
+        unit = min(index * (unsigned)(WAVES / TEAM) + team, p.H * parts - 1u);
         head = unit / parts;
         group = head / (p.H / p.G);
         tile = unit % parts * TEAM + wave % TEAM;
@@ -162,7 +162,7 @@ template <typename F> inline void with_key_tiles(size_t K, F f)
 
 // Keys of more than 32 columns fill the LDS: there a team is always the whole workgroup, also where some of its waves have no tile and only help to fetch.
 inline int team_of(size_t K, size_t tiles) { return K > 32 || tiles > 2 ? 4 : (int)tiles; }
-inline unsigned team_blocks(const delta_shape& p, size_t team, size_t cols) { return divup((size_t)p.H * (((cols + 15) / 16 + team - 1) / team), 4u / team); }
+inline unsigned team_blocks(const delta_shape& p, size_t team, size_t cols, size_t waves = 4) { return divup((size_t)p.H * (((cols + 15) / 16 + team - 1) / team), waves / team); }
 template <typename F> inline void with_team(size_t K, size_t tiles, F f)
 {
     auto pass = [&](auto kt) {
@@ -315,7 +315,7 @@ template <typename A> __device__ __forceinline__ typename mm16<A>::vec by_row(co
 }
 
 // A wave's columns of states (blocks of K x (H V)): tile t holds rows 16 t + row(g, r).
-template <typename A, int KT, int TEAM> __device__ __forceinline__ void load_state(typename mm16<A>::vec (&S)[KT], const A* p, const delta_shape& s, const delta_lane<A, TEAM>& l)
+template <typename A, int KT, int TEAM, int WAVES> __device__ __forceinline__ void load_state(typename mm16<A>::vec (&S)[KT], const A* p, const delta_shape& s, const delta_lane<A, TEAM, WAVES>& l)
 {
 #pragma unroll
     for (int t = 0; t < KT; ++t)

@@ -229,42 +229,64 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
 }
 
 // From segment to segment: what is in front of slot k + 1 is what its own segment made of zeros and what the transition makes of what is in front of slot k; backward
-// from the last segment to the first with the transposed transitions. A wave takes 16 columns of a head.
+// from the last segment to the first with the transposed transitions. A workgroup takes 16 columns of a head, a wave 16 rows of what comes out; what goes in lies in LDS as
+// it lies in registers, and the next transition's rows come meanwhile.
 template <typename A, int KT>
-__global__ __launch_bounds__(256) void k_delta_carry(delta_shape p, bool backward, const uint32_t* __restrict__ regions, A* __restrict__ carry, const A* __restrict__ through)
+__global__ __launch_bounds__(64 * KT) void k_delta_carry(delta_shape p, bool backward, const uint32_t* __restrict__ regions, A* __restrict__ carry, const A* __restrict__ through)
 {
     typedef typename mm16<A>::vec vec;
-    const unsigned r = blockIdx.x;
-    const row_range g = region_rows(regions, r, p.N);
-    if (g.end - g.start <= 2u * p.L) return;     // (two segments: nothing to carry over one)
-    delta_lane<A, 4> l;
-    l.place(p, blockIdx.y, p.V);
-    if (!l.nv) return;
-    const unsigned n = (g.end - g.start + p.L - 1u) / p.L;      // segments; slots first + 1 .. first + n - 1
-    const size_t first = g.start / p.L, block = (size_t)p.K * p.H * p.V, D = (size_t)p.H * p.K;
-    vec S[KT];
-    load_state<A, KT>(S, carry + (first + (backward ? n - 1u : 1u)) * block, p, l);
-    for (unsigned i = 2; i < n; ++i) {
-        // forward: slot i from slot i - 1 by the transition of segment i - 1, which lies in slot i. Backward: slot n - i from slot n - i + 1 by that of segment n - i, in slot n - i + 1
-        const size_t to = first + (backward ? n - i : i), by = first + (backward ? n - i + 1u : i);
-        const A* m = through + by * ((size_t)p.K * D) + (size_t)l.head * p.K;
-        vec N[KT];
-        load_state<A, KT>(N, carry + to * block, p, l);
+    __shared__ A lds[2][KT][4][64];
+    const unsigned r = blockIdx.x, lane = threadIdx.x & 63u, t = uniform(threadIdx.x >> 6), g = lane >> 4, c = lane & 15u;
+    const row_range rows = region_rows(regions, r, p.N);
+    if (rows.end - rows.start <= 2u * p.L) return;               // (two segments: nothing to carry over one)
+    const unsigned head = blockIdx.y / p.ns, tile = blockIdx.y % p.ns, n = (rows.end - rows.start + p.L - 1u) / p.L;      // segments: slots first + 1 .. first + n - 1
+    const size_t first = rows.start / p.L, HV = (size_t)p.H * p.V, HK = (size_t)p.H * p.K, col = (size_t)head * p.V + 16u * tile + c;
+    const bool here = 16u * tile + c < p.V;
+    auto state = [&](size_t slot, int i) { return carry + (slot * p.K + 16u * t + mm16<A>::row(g, i)) * HV + col; };
+    auto load = [&](size_t slot) {
+        vec x;
 #pragma unroll
-        for (int t = 0; t < KT; ++t)
+        for (int i = 0; i < 4; ++i) x[i] = here && 16u * t + mm16<A>::row(g, i) < p.K ? *state(slot, i) : A(0);
+        return x;
+    };
+    // forward: slot i from slot i - 1 by the transition of segment i - 1, which lies in slot i; backward: slot n - i from slot n - i + 1 by that of segment n - i, in slot n - i + 1
+    auto to = [&](unsigned i) { return first + (backward ? n - i : i); };
+    vec a[KT];
+    auto transition = [&](unsigned i) {
+        const A* m = through + (first + (backward ? n - i + 1u : i)) * (p.K * HK) + (size_t)head * p.K;
 #pragma unroll
-            for (int s = 0; s < KT; ++s) {
-                vec a;
+        for (int s = 0; s < KT; ++s)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const unsigned row = 16u * t + l.c, col = 16u * s + l.row(j);
-                    a[j] = row < p.K && col < p.K ? backward ? m[col * D + row] : m[row * D + col] : A(0);
-                }
-                N[t] = product<A>(a, S[s], N[t]);
+            for (int j = 0; j < 4; ++j) {
+                const unsigned row = 16u * t + c, k = 16u * s + mm16<A>::row(g, j);
+                a[s][j] = row < p.K && k < p.K ? backward ? m[k * HK + row] : m[row * HK + k] : A(0);
             }
+    };
+    const vec start = load(first + (backward ? n - 1u : 1u));
 #pragma unroll
-        for (int t = 0; t < KT; ++t) S[t] = N[t];
-        store_state<A, KT>(S, carry + to * block, p, l);
+    for (int i = 0; i < 4; ++i) lds[0][t][i][lane] = start[i];
+    transition(2u);
+    vec own = load(to(2u));
+    __syncthreads();
+    for (unsigned i = 2; i < n; ++i) {
+        vec x = own;
+#pragma unroll
+        for (int s = 0; s < KT; ++s) {
+            vec b;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = lds[i & 1u][s][j][lane];
+            x = product<A>(a[s], b, x);
+        }
+        if (i + 1u < n) {
+            transition(i + 1u);
+            own = load(to(i + 1u));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            lds[~i & 1u][t][j][lane] = x[j];
+            if (here && 16u * t + mm16<A>::row(g, j) < p.K) *state(to(i), j) = x[j];
+        }
+        __syncthreads();
     }
 }
 
@@ -398,7 +420,7 @@ void delta_carry(hipStream_t st, const dbk_deltarule_args& a, const delta_shape&
     auto launch = [&](auto t) {
         typedef decltype(t) A;
         with_key_tiles(a.K, [&](auto kt) {
-            k_delta_carry<A, kt.value><<<dim3(s.nregion, team_blocks(s, 4, s.V)), 256, 0, st>>>(s, backward, a.regions, (A*)w.carry, (const A*)w.through);
+            k_delta_carry<A, kt.value><<<dim3(s.nregion, s.H * s.ns), 64 * kt.value, 0, st>>>(s, backward, a.regions, (A*)w.carry, (const A*)w.through);
         });
     };
     if (a.dtype == DBK_F64) launch(double());

@@ -129,31 +129,6 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
     store_state<A, KT>(S, carry + blockIdx.x * ((size_t)p.K * p.H * p.V), p, l);
 }
 
-// transposed states: tile t holds [row(g, r)][16 t + c] of the wave's 16 columns by K
-template <typename A, int KT, int TEAM> __device__ __forceinline__ void load_state_t(typename mm16<A>::vec (&S)[KT], const A* p, const delta_shape& s, const delta_lane<A, TEAM>& l)
-{
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-        const unsigned k = 16u * t + l.c;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[t][r] = p && k < s.K && l.row(r) < l.nv ? p[k * l.D + l.v + l.row(r)] : A(0);
-    }
-}
-
-// The transposed tile of x. Products with zeros are as in triangle(): where the tile is not all finite, lanes exchange it value by value.
-template <typename A> __device__ __forceinline__ typename mm16<A>::vec exchange(typename mm16<A>::vec x, unsigned g, unsigned c)
-{
-    typename mm16<A>::vec o;
-    const unsigned gc = sizeof(A) == 4 ? c >> 2 : c & 3u, rc = sizeof(A) == 4 ? c & 3u : c >> 2;     // row(gc, rc) == c
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int from = (int)(16u * gc + mm16<A>::row(g, r));
-        const A v[4] = {__shfl(x[0], from), __shfl(x[1], from), __shfl(x[2], from), __shfl(x[3], from)};
-        o[r] = rc == 0u ? v[0] : rc == 1u ? v[1] : rc == 2u ? v[2] : v[3];
-    }
-    return o;
-}
-
 // sums over the 16 lanes of a row
 template <typename A> __device__ __forceinline__ A lanes16_sum(A v)
 {
@@ -169,17 +144,35 @@ template <typename T> struct delta_grads {
     size_t lddq, lddk, lddv, lddb, lddg;
     // where more than one unit (head and part of its value) has a share: (units of a key, N, G K) and (parts, N, H)
     A *dq, *dk, *db, *dg;
-    unsigned parts, waves;                       // parts of a value, waves per unit (1, 2 or 4)
+    unsigned parts;                              // of a value: as many tiles as a team has waves
 };
 
-template <typename A, int KT> struct delta_share {
-    A pl[2][16][17];                             // dP, dL
-    A q[KT][16][17], k[KT][16][17];
-    A into[16], out[16], b[16], through;
+// What the waves of a team show each other of one chunk: S0 and dS1 by rows of the state (a wave's own columns of them lie in its registers), dO, dY and U by rows of the
+// chunk, the waves' shares of dP and dL and of what is one value a row.
+// (A wave by itself leaves out the padding, with which only two of these workgroups fit a CU and not three.)
+template <typename A, int KT, int TEAM> struct delta_back {
+    static constexpr int W = 16 * TEAM + (TEAM > 1 ? 4 : 0);
+    A s[16 * KT][W], d[16 * KT][W];
+    A o[16][W], y[16][W], u[16][W];
+    A pl[TEAM][2][16][17];
+    A into[TEAM][16], out[TEAM][16], b[TEAM][16], through[TEAM][4];
+    delta_rows<A, KT> rows;
 };
+template <typename A, int R, int W> __device__ __forceinline__ typename mm16<A>::vec rows_of_tile(const A (&m)[R][W], unsigned row, unsigned t, unsigned g)
+{
+    typename mm16<A>::vec f;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[r] = m[row][16u * t + mm16<A>::row(g, r)];
+    return f;
+}
 
-template <typename T, int KT>
-__global__ __launch_bounds__(256) void k_delta_bprop(delta_shape p, size_t lddo, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, const T* __restrict__ Q,
+// The gradients of one block of 64 rows, from the state in front of it and the gradient of the state behind it: forward again over its chunks, whose states stay in registers, and
+// back. Two kinds of work alternate: what runs over a head's keys (a wave's 16 columns of the value, the states in registers) and what runs over its value (16 columns of the
+// key for a wave, the states in LDS), so that neither dQ and dK nor the states are ever added up or turned over between waves.
+template <typename A, int KT, int TEAM> constexpr int back_waves() { return sizeof(A) == 8 ? (KT == 1 && TEAM > 1 ? 2 : 1) : KT == 1 ? 3 : KT == 2 && TEAM == 1 ? 1 : KT <= 4 ? 2 : 1; }
+
+template <typename T, int KT, int TEAM, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, KT, TEAM>())) void k_delta_bprop(delta_shape p, size_t lddo, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, const T* __restrict__ Q,
                                                      const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ dO,
                                                      const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, const delta_pairs<typename acc_of<T>::type>* __restrict__ pairs,
                                                      typename acc_of<T>::type scale, const typename acc_of<T>::type* __restrict__ keep,
@@ -187,152 +180,177 @@ __global__ __launch_bounds__(256) void k_delta_bprop(delta_shape p, size_t lddo,
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
+    constexpr int TW = KT > TEAM ? KT / TEAM : 1;
     extern __shared__ __align__(16) char lds_bytes[];
-    delta_share<A, KT>* all = (delta_share<A, KT>*)lds_bytes;
-    const unsigned wave = uniform(threadIdx.x >> 6), slice = wave & (out.waves - 1u);
     delta_block bl;
     if (!find_block(p, regions, marks, blockIdx.x, bl)) return;
-    const unsigned unit = min((blockIdx.y * 4u + wave) / out.waves, p.H * out.parts - 1u), part = unit % out.parts;      // (a unit too many does the last one again)
-    const unsigned tile = part * 4u + slice;
-    delta_lane<A, 4> l;
-    l.place(p, 0u, p.V);
-    l.head = unit / out.parts;
-    l.group = l.head / (p.H / p.G);
-    l.nv = tile < p.ns ? min(16u, p.V - tile * 16u) : 0u;
-    l.v = l.head * p.V + (l.nv ? tile * 16u : 0u);
-    const unsigned g = l.g, c = l.c, nchunk = (bl.rows + 15u) / 16u;
+    delta_lane<A, TEAM, WAVES> l;
+    l.place(p, blockIdx.y, p.V);
+    delta_back<A, KT, TEAM>& lds = reinterpret_cast<delta_back<A, KT, TEAM>*>(lds_bytes)[l.team];
+    const unsigned g = l.g, c = l.c, nchunk = (bl.rows + 15u) / 16u, slice = uniform(threadIdx.x >> 6) % TEAM, part = l.unit % out.parts;
     const size_t state = (size_t)p.K * p.H * p.V;
     const T *q0 = Q + (size_t)bl.at * p.ldq + (size_t)l.group * p.K, *k0 = K + (size_t)bl.at * p.ldk + (size_t)l.group * p.K;
-    const T *v0 = V + (size_t)bl.at * p.ldv + l.v, *d0 = dO + (size_t)bl.at * lddo + l.v;
+    const T *v0 = V + (size_t)bl.at * p.ldv + l.v + c, *d0 = dO + (size_t)bl.at * lddo + l.v + c;
     const size_t first_chunk = ((size_t)bl.slot * p.H + l.head) * DELTA_CHUNKS;
+    delta_feed<T, KT, TEAM> feed;
+    auto fetch = [&](unsigned i) { feed.fetch(p, q0 + 16u * i * p.ldq, k0 + 16u * i * p.ldk, chunks[first_chunk + i], l.thread, bl.rows - 16u * i); };
+    T next[4];
+    auto values = [&](const T* x, size_t ld, unsigned i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) next[r] = 16u * i + l.row(r) < bl.rows && c < l.nv ? x[(16u * i + l.row(r)) * ld] : (T)A(0);
+    };
 
-    // forward again, from the block's start: what the way back needs stays in registers
-    vec xs[DELTA_CHUNKS], uts[DELTA_CHUNKS], sts[DELTA_CHUNKS][KT];
+    vec xs[DELTA_CHUNKS], us[DELTA_CHUNKS], sts[DELTA_CHUNKS][KT], dS[KT];
+    fetch(0u);
+    values(v0, p.ldv, 0u);
     {
-        vec S[KT], ST[KT];
-        const A* from = bl.k ? keep + kept_number(bl.g, bl.k) * state : (const A*)nullptr;
-        load_state<A, KT>(S, from, p, l);
-        load_state_t<A, KT>(ST, from, p, l);
+        vec S[KT];
+        load_state<A, KT>(S, bl.k ? keep + kept_number(bl.g, bl.k) * state : (const A*)nullptr, p, l);
+        load_state<A, KT>(dS, bl.at + bl.rows < bl.g.end ? dstates + kept_number(bl.g, bl.k + 1u) * state : (const A*)nullptr, p, l);
 #pragma unroll
         for (int i = 0; i < (int)DELTA_CHUNKS; ++i) {
             if (i >= (int)nchunk) break;
             const unsigned n = min(bl.rows - 16u * i, 16u);
-            const delta_chunk<A>& ch = chunks[first_chunk + i];
-            vec f[KT], w = zero16<A>();
-            load_by_rows<T, KT>(f, k0 + 16 * i * p.ldk, p.ldk, n, p.K, g, c);
+            if (i) __syncthreads();
+            feed.put(lds.rows, l.thread);
+            vec x, w = zero16<A>(), y;
 #pragma unroll
-            for (int t = 0; t < KT; ++t) w = product<A>(f[t], S[t], w);
-            const vec first = by_row(ch.first, g), b = by_row(ch.b, g), last = by_row(ch.last, g);
-            vec x = load_tile(v0 + 16 * i * p.ldv, p.ldv, n, l.nv, g, c), y;
+            for (int r = 0; r < 4; ++r) x[r] = (A)next[r];
+            if (i + 1 < (int)nchunk) {
+                fetch(i + 1u);
+                values(v0, p.ldv, i + 1u);
+            } else {
+                if (i) fetch(i - 1u);
+                values(d0, lddo, i);
+            }
+            __syncthreads();
+            const delta_rows<A, KT>& here = lds.rows;
+#pragma unroll
+            for (int t = 0; t < KT; ++t) w = product<A>(tile_by_rows(here.k, t, g, c), S[t], w);
+            const vec first = by_row(here.c.first, g), b = by_row(here.c.b, g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 x[r] = l.row(r) < n ? x[r] - first[r] * w[r] : A(0);
                 y[r] = b[r] * x[r];
             }
-            const vec tr = matrix_by_rows(ch.T, g, c), u = triangle<A, true>(tr, y, zero16<A>(), g);
             xs[i] = x;
-            uts[i] = product<A>(y, tr, zero16<A>());
-            if (__any(!all_finite(uts[i]))) uts[i] = exchange<A>(u, g, c);
+            us[i] = triangle<A, true>(matrix_by_rows(here.c.T, g, c), y, zero16<A>(), g);
 #pragma unroll
-            for (int t = 0; t < KT; ++t) sts[i][t] = ST[t];
+            for (int t = 0; t < KT; ++t) sts[i][t] = S[t];
             if (i + 1 >= (int)nchunk) break;
-            const A through = ch.first[15];
-            const vec sent = last * u;
-            load_by_columns<T, KT>(f, k0 + 16 * i * p.ldk, p.ldk, n, p.K, g, c);
+            const A through = here.c.first[15];
+            const vec sent = by_row(here.c.last, g) * us[i];
 #pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                S[t] = product<A>(f[t], sent, through * S[t]);
-                ST[t] = product<A>(sent, f[t], through * ST[t]);
-            }
+            for (int t = 0; t < KT; ++t) S[t] = product<A>(tile_by_columns(here.k, t, g, c), sent, through * S[t]);
         }
     }
 
-    vec dS[KT], dST[KT];
-    {
-        const A* from = bl.at + bl.rows < bl.g.end ? dstates + kept_number(bl.g, bl.k + 1u) * state : (const A*)nullptr;
-        load_state<A, KT>(dS, from, p, l);
-        load_state_t<A, KT>(dST, from, p, l);
-    }
 #pragma unroll
     for (int i = (int)DELTA_CHUNKS - 1; i >= 0; --i) {
         if (i >= (int)nchunk) continue;
         const unsigned n = min(bl.rows - 16u * i, 16u);
         const size_t row = (size_t)bl.at + 16u * i;
-        const delta_chunk<A>& ch = chunks[first_chunk + i];
         const delta_pairs<A>& pr = pairs[first_chunk + i];
-        vec f[KT], y = zero16<A>();
-        load_by_rows<T, KT>(f, k0 + 16 * i * p.ldk, p.ldk, n, p.K, g, c);
+        if (i + 1 < (int)nchunk) {               // (the last chunk's rows are there)
+            __syncthreads();
+            feed.put(lds.rows, l.thread);
+            if (i) fetch(i - 1u);
+            __syncthreads();
+        }
+        const delta_rows<A, KT>& here = lds.rows;
+        vec d, y = zero16<A>();
 #pragma unroll
-        for (int t = 0; t < KT; ++t) y = product<A>(f[t], dS[t], y);
-        const vec first = by_row(ch.first, g), b = by_row(ch.b, g), last = by_row(ch.last, g);
-        const A first_c = ch.first[c], b_c = ch.b[c], last_c = ch.last[c], through = ch.first[15];
-        const vec d = scale * load_tile(d0 + 16 * i * lddo, lddo, n, l.nv, g, c);
-        vec dt[1];
-        load_by_rows<T, 1>(dt, d0 + 16 * i * lddo, lddo, n, l.nv, g, c);
-        dt[0] = scale * dt[0];
-        const vec du = triangle<A, false>(matrix_by_columns(ch.P, g, c), d, last * y, g);
-        const vec tc = matrix_by_columns(ch.T, g, c);
-        const vec dy = triangle<A, false>(tc, du, zero16<A>(), g);
-        vec dyt = product<A>(du, tc, zero16<A>());
-        if (__any(!all_finite(dyt))) dyt = exchange<A>(dy, g, c);
-        const vec dx = b * dy, dw = -(first * dx), dwt = -(first_c * b_c) * dyt, fd = first * d, fdt = first_c * dt[0], lut = last_c * uts[i];
+        for (int r = 0; r < 4; ++r) d[r] = scale * (A)next[r];
+        if (i) values(d0, lddo, i - 1u);
+        // (fetched here, used behind the next barriers)
+        const vec Dr = matrix_by_rows(pr.D, g, c), Dc = matrix_by_columns(pr.D, g, c), Nr = matrix_by_rows(pr.N, g, c);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) y = product<A>(tile_by_rows(here.k, t, g, c), dS[t], y);
+        const vec first = by_row(here.c.first, g), b = by_row(here.c.b, g);
+        const A first_c = here.c.first[c], b_c = here.c.b[c], last_c = here.c.last[c], through = here.c.first[15];
+        const vec du = triangle<A, false>(matrix_by_columns(here.c.P, g, c), d, by_row(here.c.last, g) * y, g);
+        const vec dy = triangle<A, false>(matrix_by_columns(here.c.T, g, c), du, zero16<A>(), g);
+        const vec dx = b * dy, dw = -(first * dx), fd = first * d;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
             if (l.row(r) < n && c < l.nv) out.dV[(row + l.row(r)) * out.lddv + l.v + c] = (T)dx[r];
-
-        delta_share<A, KT>& mine = all[wave];
-        const vec dp = product<A>(dt[0], uts[i], zero16<A>()), dl = -product<A>(dyt, uts[i], zero16<A>());
-        vec kc[KT], qc[KT], into = zero16<A>(), sent = zero16<A>();
-        load_by_columns<T, KT>(kc, k0 + 16 * i * p.ldk, p.ldk, n, p.K, g, c);
-        load_by_columns<T, KT>(qc, q0 + 16 * i * p.ldq, p.ldq, n, p.K, g, c);
+        const unsigned mine = 16u * slice + c;
         A passed = A(0);
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-            const vec a = product<A>(fdt, sts[i][t], zero16<A>()), e = product<A>(dwt, sts[i][t], zero16<A>()), s = product<A>(lut, dST[t], zero16<A>());
+        for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                mine.q[t][l.row(r)][c] = a[r];
-                mine.k[t][l.row(r)][c] = e[r] + s[r];
-                into[r] = fma(qc[t][r], a[r], fma(kc[t][r], e[r], into[r]));
-                sent[r] = fma(kc[t][r], s[r], sent[r]);
-                passed = fma(sts[i][t][r], dST[t][r], passed);
+                lds.s[16u * t + l.row(r)][mine] = sts[i][t][r];
+                lds.d[16u * t + l.row(r)][mine] = dS[t][r];
+                passed = fma(sts[i][t][r], dS[t][r], passed);
             }
-        }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) passed += __shfl_xor(passed, o);
+        if ((threadIdx.x & 63u) == 0u) lds.through[slice][0] = through * passed;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            mine.pl[0][l.row(r)][c] = dp[r];
-            mine.pl[1][l.row(r)][c] = dl[r];
-            const A in = lanes16_sum(into[r]), on = lanes16_sum(sent[r]), db = lanes16_sum(dy[r] * xs[i][r]);
-            if (c == 0u) {
-                mine.into[l.row(r)] = in;
-                mine.out[l.row(r)] = on;
-                mine.b[l.row(r)] = db;
+            lds.o[l.row(r)][mine] = d[r];
+            lds.y[l.row(r)][mine] = dy[r];
+            lds.u[l.row(r)][mine] = us[i][r];
+            const A db = lanes16_sum(dy[r] * xs[i][r]);
+            if (c == 0u) lds.b[slice][l.row(r)] = db;
+        }
+        if (i)
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+                dS[t] = product<A>(tile_by_columns(here.q, t, g, c), fd, product<A>(tile_by_columns(here.k, t, g, c), dw, through * dS[t]));
+        __syncthreads();
+
+        // over the value: this wave's columns of the key
+        vec qs[TW], ks[TW], into = zero16<A>(), sent = zero16<A>();
+#pragma unroll
+        for (int j = 0; j < TW; ++j) {
+            const unsigned t = slice + (unsigned)TEAM * j;
+            qs[j] = ks[j] = zero16<A>();
+            if (t >= (unsigned)KT || 16u * t >= p.K) continue;
+            vec e = zero16<A>(), s = zero16<A>();
+#pragma unroll
+            for (int x = 0; x < TEAM; ++x) {
+                const vec s0 = rows_of_tile(lds.s, 16u * t + c, x, g);
+                qs[j] = product<A>(first_c * tile_by_rows(lds.o, x, g, c), s0, qs[j]);
+                e = product<A>(-(first_c * b_c) * tile_by_rows(lds.y, x, g, c), s0, e);
+                s = product<A>(last_c * tile_by_rows(lds.u, x, g, c), rows_of_tile(lds.d, 16u * t + c, x, g), s);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const A k = here.k[l.row(r)][16u * t + c], q = here.q[l.row(r)][16u * t + c];
+                into[r] = fma(q, qs[j][r], fma(k, e[r], into[r]));
+                sent[r] = fma(k, s[r], sent[r]);
+                ks[j][r] = e[r] + s[r];
             }
         }
-        if ((threadIdx.x & 63u) == 0u) mine.through = through * passed;
-        if (i > 0) {
+        {
+            const vec u = tile_by_rows(lds.u, (int)slice, g, c);
+            const vec dp = product<A>(tile_by_rows(lds.o, (int)slice, g, c), u, zero16<A>()), dl = -product<A>(tile_by_rows(lds.y, (int)slice, g, c), u, zero16<A>());
 #pragma unroll
-            for (int t = 0; t < KT; ++t) {
-                dS[t] = product<A>(qc[t], fd, product<A>(kc[t], dw, through * dS[t]));
-                dST[t] = product<A>(fd, qc[t], product<A>(dw, kc[t], through * dST[t]));
+            for (int r = 0; r < 4; ++r) {
+                lds.pl[slice][0][l.row(r)][c] = dp[r];
+                lds.pl[slice][1][l.row(r)][c] = dl[r];
+                const A in = lanes16_sum(into[r]), on = lanes16_sum(sent[r]);
+                if (c == 0u) {
+                    lds.into[slice][l.row(r)] = in;
+                    lds.out[slice][l.row(r)] = on;
+                }
             }
         }
         __syncthreads();
 
-        // the unit's sums, and what the pairs of rows add to them
-        const delta_share<A, KT>* ours = all + (wave - slice);
+        // the team's sums, and what the pairs of rows add
         vec pr_ = zero16<A>(), lr = zero16<A>(), pc = zero16<A>(), lc = zero16<A>();    // dP and dL: [c][row], [row][c]
-        for (unsigned s = 0; s < out.waves; ++s)
+#pragma unroll
+        for (int s = 0; s < TEAM; ++s)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                pr_[r] += ours[s].pl[0][c][l.row(r)];
-                lr[r] += ours[s].pl[1][c][l.row(r)];
-                pc[r] += ours[s].pl[0][l.row(r)][c];
-                lc[r] += ours[s].pl[1][l.row(r)][c];
+                pr_[r] += lds.pl[s][0][c][l.row(r)];
+                lr[r] += lds.pl[s][1][c][l.row(r)];
+                pc[r] += lds.pl[s][0][l.row(r)][c];
+                lc[r] += lds.pl[s][1][l.row(r)][c];
             }
-        const vec Dr = matrix_by_rows(pr.D, g, c), Dc = matrix_by_columns(pr.D, g, c);
         vec ar, ac, ms;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -343,17 +361,11 @@ __global__ __launch_bounds__(256) void k_delta_bprop(delta_shape p, size_t lddo,
         }
         const unsigned share = (l.head % (p.H / p.G)) * out.parts + part;
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-            if (((unsigned)t & (out.waves - 1u)) != slice || 16u * t >= p.K) continue;
-            vec dq = zero16<A>(), dk = zero16<A>();
-            for (unsigned s = 0; s < out.waves; ++s)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    dq[r] += ours[s].q[t][l.row(r)][c];
-                    dk[r] += ours[s].k[t][l.row(r)][c];
-                }
-            dq = triangle<A, true>(ar, kc[t], dq, g);
-            dk = product<A>(ms, kc[t], triangle<A, false>(ac, qc[t], dk, g));
+        for (int j = 0; j < TW; ++j) {
+            const unsigned t = slice + (unsigned)TEAM * j;
+            if (t >= (unsigned)KT || 16u * t >= p.K) continue;
+            const vec kc = tile_by_columns(here.k, (int)t, g, c), qc = tile_by_columns(here.q, (int)t, g, c);
+            const vec dq = triangle<A, true>(ar, kc, qs[j], g), dk = product<A>(ms, kc, triangle<A, false>(ac, qc, ks[j], g));
             const size_t col = (size_t)l.group * p.K + 16u * t + c;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -370,7 +382,7 @@ __global__ __launch_bounds__(256) void k_delta_bprop(delta_shape p, size_t lddo,
             }
         }
         if (slice == 0u) {
-            const vec Pr = matrix_by_rows(ch.P, g, c), Nr = matrix_by_rows(pr.N, g, c);
+            const vec Pr = matrix_by_rows(here.c.P, g, c);
             vec e, before;
             A db = A(0), dg = A(0);
 #pragma unroll
@@ -388,10 +400,15 @@ __global__ __launch_bounds__(256) void k_delta_bprop(delta_shape p, size_t lddo,
             db += __shfl_xor(db, 32);
             dg += __shfl_xor(dg, 16);
             dg += __shfl_xor(dg, 32);
-            for (unsigned s = 0; s < out.waves; ++s) {
-                db += ours[s].b[c];
-                dg += ours[s].through;
-                for (unsigned m = 0; m < 16u; ++m) dg += m >= c ? ours[s].into[m] : ours[s].out[m];
+#pragma unroll
+            for (int s = 0; s < TEAM; ++s) {
+                db += lds.b[s][c];
+                dg += lds.through[s][0];
+            }
+            for (unsigned m = 0; m < 16u; ++m) {
+                const A (*from)[16] = m >= c ? lds.into : lds.out;
+#pragma unroll
+                for (int s = 0; s < TEAM; ++s) dg += from[s][m];
             }
             if (g == 0u && c < n) {
                 const size_t at = row + c;
@@ -401,7 +418,6 @@ __global__ __launch_bounds__(256) void k_delta_bprop(delta_shape p, size_t lddo,
                 else if (out.ddecay) out.ddecay[at * out.lddg + l.head] = dg;
             }
         }
-        __syncthreads();
     }
 }
 
@@ -433,10 +449,13 @@ namespace {
 struct delta_bprop_work {
     uint32_t* marks;
     char *chunks, *pairs, *dstates, *dq, *dk, *db, *dg;
-    unsigned parts, waves;
+    unsigned parts;
     delta_cuts cuts;
     size_t bytes;
 };
+
+// Tiles of a value that a team takes at once: its states' share of the LDS, in double precision and with keys of more than 64 columns, is that of two.
+unsigned back_team(const dbk_deltarule_args& a) { return a.dtype == DBK_F64 && a.K > 64 ? 2u : (unsigned)team_of(a.K, (a.V + 15) / 16); }
 
 delta_bprop_work bprop_work_in(void* work, const dbk_deltarule_args& a, const delta_shape& s)
 {
@@ -445,8 +464,7 @@ delta_bprop_work bprop_work_in(void* work, const dbk_deltarule_args& a, const de
     size_t at = 0;
     auto take = [&](size_t n) { char* p = base + at; at += align16(n); return p; };
     const size_t A = acc_size(a.dtype), units = delta_blocks(s) * a.H * DELTA_CHUNKS;
-    w.parts = (s.ns + 3) / 4;
-    w.waves = s.ns > 2 ? 4 : s.ns;
+    w.parts = (s.ns + back_team(a) - 1) / back_team(a);
     w.marks = (uint32_t*)take(s.slots * sizeof(uint32_t));
     w.chunks = take(units * (A == 8 ? sizeof(delta_chunk<double>) : sizeof(delta_chunk<float>)));
     w.pairs = take(units * (A == 8 ? sizeof(delta_pairs<double>) : sizeof(delta_pairs<float>)));
@@ -499,7 +517,7 @@ int dbk_deltarule_bprop(dbk_stream_t stream, const dbk_deltarule_args* a, void* 
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
         delta_grads<T> out = {(T*)a->dQ, (T*)a->dK, (T*)a->dV, (A*)a->dbeta, (A*)a->ddecay, a->lddq, a->lddk, a->lddv, a->lddbeta, a->ldddecay,
-                              (A*)w.dq, (A*)w.dk, (A*)w.db, a->ddecay ? (A*)w.dg : nullptr, w.parts, w.waves};
+                              (A*)w.dq, (A*)w.dk, (A*)w.db, a->ddecay ? (A*)w.dg : nullptr, w.parts};
         with_team(a->K, s.ns, [&](auto kt, auto team) {
             const unsigned columns = team_blocks(s, team.value, s.V);
             if (s.L) {
@@ -509,11 +527,13 @@ int dbk_deltarule_bprop(dbk_stream_t stream, const dbk_deltarule_args* a, void* 
             }
             k_delta_chain<T, kt.value, team.value><<<dim3(s.nregion + s.cuts, columns), 256, 0, st>>>(
                 s, a->lddo, a->regions, w.cuts.marks, (const T*)a->Q, (const T*)a->Kk, (const T*)a->dO, (const delta_chunk<A>*)w.chunks, (A)a->scale, (const A*)w.cuts.carry, (A*)w.dstates);
-        });
-        with_key_tiles(a->K, [&](auto kt) {
-            constexpr size_t lds = 4 * sizeof(delta_share<A, kt.value>);
-            if (lds > 65536 && hipFuncSetAttribute((const void*)k_delta_bprop<T, kt.value>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) { rc = 1; return; }
-            k_delta_bprop<T, kt.value><<<dim3((unsigned)delta_blocks(s), divup((size_t)s.H * w.parts * w.waves, 4)), 256, lds, st>>>(
+            constexpr bool half = sizeof(A) == 8 && kt.value == 8;
+            constexpr int TEAM = half ? 2 : team.value, WAVES = half ? 2 : 4;
+            constexpr size_t lds = WAVES / TEAM * sizeof(delta_back<A, kt.value, TEAM>);
+            static_assert(lds <= 163840, "a workgroup's shared memory");
+            auto kernel = k_delta_bprop<T, kt.value, TEAM, WAVES>;
+            if (lds > 65536 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) { rc = 1; return; }
+            kernel<<<dim3((unsigned)delta_blocks(s), team_blocks(s, TEAM, s.V, WAVES)), 64 * WAVES, lds, st>>>(
                 s, a->lddo, a->regions, w.marks, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const T*)a->dO, (const delta_chunk<A>*)w.chunks, (const delta_pairs<A>*)w.pairs,
                 (A)a->scale, (const A*)a->keep, (const A*)w.dstates, out);
         });
