@@ -55,6 +55,16 @@ template <typename A> __device__ __forceinline__ typename mm16<A>::vec product(t
     for (int r = 0; r < 4; ++r) c = mm16<A>::mac(a[r], b[r], c);
     return c;
 }
+// Two of them with the same right operand side by side, and one right operand with the left ones of many tiles: a matrix instruction waits for the one whose result it adds
+// to, not for others.
+template <typename A> __device__ __forceinline__ void products(typename mm16<A>::vec a, typename mm16<A>::vec b, typename mm16<A>::vec right, typename mm16<A>::vec& x, typename mm16<A>::vec& y)
+{
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        x = mm16<A>::mac(a[r], right[r], x);
+        y = mm16<A>::mac(b[r], right[r], y);
+    }
+}
 template <typename A> __device__ __forceinline__ typename mm16<A>::vec zero16() { return typename mm16<A>::vec{A(0), A(0), A(0), A(0)}; }
 
 template <typename V> __device__ __forceinline__ bool all_finite(V v)
@@ -199,29 +209,74 @@ template <typename A, int W> __device__ __forceinline__ typename mm16<A>::vec ti
 // Waves per SIMD that the walks are compiled for: their registers hold 4 values per lane of a state's every 16 rows. (Four teams of 32-column keys fill half the LDS.)
 template <typename A, int KT, int TEAM> constexpr int delta_waves() { return sizeof(A) == 4 ? (KT > 4 || (KT == 2 && TEAM == 1) ? 2 : 4) : KT > 4 || (KT == 2 && TEAM == 1) ? 1 : 2; }
 
+// S[t] += m's tile t by columns, transposed, times x
+template <typename A, int KT, int W> __device__ __forceinline__ void add_products(typename mm16<A>::vec (&S)[KT], const A (&m)[16][W], typename mm16<A>::vec x, unsigned g, unsigned c)
+{
+    constexpr int S2 = KT < 4 ? KT : 4;
+#pragma unroll
+    for (int t = 0; t < KT; t += S2) {
+        typename mm16<A>::vec f[S2];
+#pragma unroll
+        for (int i = 0; i < S2; ++i) f[i] = tile_by_columns(m, t + i, g, c);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int i = 0; i < S2; ++i) S[t + i] = mm16<A>::mac(f[i][r], x[r], S[t + i]);
+    }
+}
+
+// One value as it lies in memory. Whatever is fetched ahead is read from an address that is there (of the same chunk's first row or column where its own is not) and made zero where it
+// is used: a load behind a branch, or one whose value is converted at once, would be waited for there.
+template <typename T> struct raw_one {
+    typedef typename acc_of<T>::type A;
+    typename std::conditional<sizeof(T) == 8, double, unsigned>::type r;
+    __device__ __forceinline__ void load(const T* p)
+    {
+        if constexpr (sizeof(T) == 2) r = *reinterpret_cast<const unsigned short*>(p);
+        else if constexpr (sizeof(T) == 4) r = *reinterpret_cast<const unsigned*>(p);
+        else r = *p;
+    }
+    __device__ __forceinline__ A get(bool there)
+    {
+        asm volatile("" : "+v"(r));
+        if constexpr (sizeof(T) == 2) return there ? __uint_as_float(r << 16) : A(0);
+        else if constexpr (sizeof(T) == 4) return there ? __uint_as_float(r) : A(0);
+        else return there ? r : A(0);
+    }
+};
+
 // Their way there: a thread's vectors come while the chunk before is worked on (fetch), and are put into LDS when it is done (put).
 template <typename T, int KT, int TEAM> struct delta_feed {
     typedef typename acc_of<T>::type A;
     static constexpr int EACH = KT >= TEAM ? KT / TEAM : 1, VECS = 64 * KT;      // vectors of 4 values: a thread's, a chunk's
     static constexpr int PARTS = sizeof(delta_chunk<A>) / sizeof(A) / 4, SHARE = (PARTS + 64 * TEAM - 1) / (64 * TEAM);
-    raw_vec<T, false, 4> k[EACH], q[EACH];
+    typedef typename row_vec<T, 4>::raw raw;
+    raw k[EACH], q[EACH];
     row_vec<A, 4> part[SHARE];
-    __device__ __forceinline__ void fetch(const delta_shape& p, const T* Q, const T* K, const delta_chunk<A>& c, unsigned thread, unsigned rows)
+    unsigned rows;
+    __device__ __forceinline__ void fetch(const delta_shape& p, const T* Q, const T* K, const delta_chunk<A>& c, unsigned thread, unsigned rows_)
     {
+        rows = rows_;
 #pragma unroll
-        for (int i = 0; i < SHARE; ++i) {
-            const unsigned v = thread + i * 64u * TEAM;
-            part[i].load(reinterpret_cast<const A*>(&c) + 4 * v, v < (unsigned)PARTS ? 4u : 0u);
-        }
+        for (int i = 0; i < SHARE; ++i) part[i].load(reinterpret_cast<const A*>(&c) + 4u * min(thread + i * 64u * TEAM, (unsigned)PARTS - 1u), 4u);
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const unsigned v = thread + i * 64u * TEAM, row = v / (4u * KT), col = v % (4u * KT) * 4u;
-            const unsigned valid = row < rows && col < p.K ? p.K - col : 0u;
-            k[i].load(K + row * p.ldk + col, valid);
-            q[i].load(Q + row * p.ldq + col, valid);
+            const T *ki = K + (row < rows ? row : 0u) * p.ldk, *qi = Q + (row < rows ? row : 0u) * p.ldq;
+            if (p.K % 4u == 0u) {
+                const unsigned at = col < p.K ? col : 0u;
+                k[i] = *reinterpret_cast<const raw*>(ki + at);
+                q[i] = *reinterpret_cast<const raw*>(qi + at);
+            } else
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned at = col + j < p.K ? col + j : 0u;
+                    k[i][j] = ki[at];
+                    q[i][j] = qi[at];
+                }
         }
     }
-    __device__ __forceinline__ void put(delta_rows<A, KT>& to, unsigned thread) const
+    __device__ __forceinline__ void put(const delta_shape& p, delta_rows<A, KT>& to, unsigned thread)
     {
 #pragma unroll
         for (int i = 0; i < SHARE; ++i) {
@@ -234,63 +289,67 @@ template <typename T, int KT, int TEAM> struct delta_feed {
         for (int i = 0; i < EACH; ++i) {
             const unsigned v = thread + i * 64u * TEAM, row = v / (4u * KT), col = v % (4u * KT) * 4u;
             if (VECS < 64 * TEAM && v >= (unsigned)VECS) break;
+            if constexpr (sizeof(T) < 8) asm volatile("" : "+v"(k[i]), "+v"(q[i]));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { to.k[row][col + j] = k[i][j]; to.q[row][col + j] = q[i][j]; }
+            for (int j = 0; j < 4; ++j) {
+                const bool there = row < rows && col + j < p.K;
+                to.k[row][col + j] = there ? (A)k[i][j] : A(0);
+                to.q[row][col + j] = there ? (A)q[i][j] : A(0);
+            }
         }
     }
 };
 
-// Tile operands of keys and queries. By rows: element [c][16 t + row(g, r)], the left operand of a product with the state; by columns: [row(g, r)][16 t + c], the left operand
-// (or the right one) where the contraction runs over the chunk's rows. Rows and columns that do not exist are zeros.
-template <typename T, int KT> __device__ __forceinline__ void load_by_rows(typename mm16<typename acc_of<T>::type>::vec (&f)[KT], const T* p, size_t ld, unsigned rows, unsigned cols,
-                                                                           unsigned g, unsigned c)
-{
+// A wave's values of a chunk (of V or dO), a chunk ahead: [row(g, r)][c]
+template <typename T> struct delta_values {
     typedef typename acc_of<T>::type A;
-    const bool here = c < rows;
-    const T* x = p + (size_t)(here ? c : 0u) * ld;
+    raw_one<T> v[4];
+    unsigned rows;
+    // p: the chunk's first row, at the wave's first column
+    template <typename L> __device__ __forceinline__ void fetch(const L& l, const T* p, size_t ld, unsigned rows_)
+    {
+        rows = rows_;
+        const T* x = p + (l.c < l.nv ? l.c : 0u);
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-        if constexpr (sizeof(A) == 4) {
+        for (int r = 0; r < 4; ++r) v[r].load(x + (l.row(r) < rows ? l.row(r) : 0u) * ld);
+    }
+    template <typename L> __device__ __forceinline__ typename mm16<A>::vec get(const L& l)
+    {
+        typename mm16<A>::vec x;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = v[r].get(l.row(r) < rows && l.c < l.nv);
+        return x;
+    }
+};
+
+// Tiles of keys and queries from memory, by rows: element [c][16 t + row(g, r)], as they lie there (fetch), and with zeros for rows and columns that do not exist (get).
+template <typename T, int KT> struct delta_tiles {
+    typedef typename acc_of<T>::type A;
+    typename row_vec<T, 4>::raw f[KT];
+    __device__ __forceinline__ void fetch(const T* p, size_t ld, unsigned rows, unsigned cols, unsigned g, unsigned c)
+    {
+        const T* x = p + (size_t)(c < rows ? c : 0u) * ld;
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
             const unsigned at = 16u * t + 4u * g;
-            row_vec<T, 4> v;
-            v.load(x + at, here && at < cols ? cols - at : 0u);
+            if (sizeof(A) == 4 && cols % 4u == 0u) f[t] = *reinterpret_cast<const typename row_vec<T, 4>::raw*>(x + (at < cols ? at : 0u));
+            else
 #pragma unroll
-            for (int r = 0; r < 4; ++r) f[t][r] = v.v[r];
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const unsigned at = 16u * t + mm16<A>::row(g, r);
-                f[t][r] = here && at < cols ? (A)x[at] : A(0);
-            }
+                for (int r = 0; r < 4; ++r) {
+                    const unsigned i = 16u * t + mm16<A>::row(g, r);
+                    f[t][r] = x[i < cols ? i : 0u];
+                }
         }
     }
-}
-template <typename T, int KT> __device__ __forceinline__ void load_by_columns(typename mm16<typename acc_of<T>::type>::vec (&f)[KT], const T* p, size_t ld, unsigned rows, unsigned cols,
-                                                                              unsigned g, unsigned c)
-{
-    typedef typename acc_of<T>::type A;
+    __device__ __forceinline__ typename mm16<A>::vec get(int t, unsigned rows, unsigned cols, unsigned g, unsigned c)
+    {
+        if constexpr (sizeof(T) < 8) asm volatile("" : "+v"(f[t]));
+        typename mm16<A>::vec v;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const unsigned row = mm16<A>::row(g, r);
-        const bool here = row < rows;
-        const T* x = p + (size_t)(here ? row : 0u) * ld + c;
-#pragma unroll
-        for (int t = 0; t < KT; ++t) f[t][r] = here && 16u * t + c < cols ? (A)x[16 * t] : A(0);
+        for (int r = 0; r < 4; ++r) v[r] = c < rows && 16u * t + mm16<A>::row(g, r) < cols ? (A)f[t][r] : A(0);
+        return v;
     }
-}
-// one tile of V, O or dO: [row(g, r)][c]
-template <typename T> __device__ __forceinline__ typename mm16<typename acc_of<T>::type>::vec load_tile(const T* p, size_t ld, unsigned rows, unsigned cols, unsigned g, unsigned c)
-{
-    typedef typename acc_of<T>::type A;
-    typename mm16<A>::vec f;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const unsigned row = mm16<A>::row(g, r);
-        const bool here = row < rows && c < cols;
-        f[r] = here ? (A)p[(size_t)row * ld + c] : A(0);
-    }
-    return f;
-}
+};
 // and of a chunk's own matrices: [c][row(g, r)] (by rows), [row(g, r)][c] (by columns); vectors [row(g, r)]
 template <typename A> __device__ __forceinline__ typename mm16<A>::vec matrix_by_rows(const A* m, unsigned g, unsigned c)
 {

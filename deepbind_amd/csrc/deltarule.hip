@@ -34,16 +34,29 @@ __global__ __launch_bounds__(256) void k_delta_prepare(delta_shape p, const uint
     if (!find_block(p, regions, marks, blockIdx.x, bl)) return;
     const unsigned head = min(blockIdx.y * 4u + wave, p.H - 1u), group = head / (p.H / p.G);      // (a wave too many does the last head again)
     const unsigned nchunk = (bl.rows + 15u) / 16u;
-    for (unsigned i = 0; i < nchunk; ++i) {
+    // two chunks' tiles are on their way at a time, in turn
+    delta_tiles<T, KT> k[2], q[2];
+    auto fetch = [&](unsigned i, int to) {
         const size_t row = bl.at + 16u * i;
-        const unsigned rows = min(bl.rows - 16u * i, 16u);
-        vec k[KT], q[KT], m = zero16<A>(), s = zero16<A>();
-        load_by_rows<T, KT>(k, K + row * p.ldk + (size_t)group * p.K, p.ldk, rows, p.K, g, c);
-        load_by_rows<T, KT>(q, Q + row * p.ldq + (size_t)group * p.K, p.ldq, rows, p.K, g, c);
+        const unsigned rows = bl.rows - 16u * i;
+        k[to].fetch(K + row * p.ldk + (size_t)group * p.K, p.ldk, rows, p.K, g, c);
+        q[to].fetch(Q + row * p.ldq + (size_t)group * p.K, p.ldq, rows, p.K, g, c);
+    };
+    fetch(0u, 0);
+#pragma unroll
+    for (int i = 0; i < (int)DELTA_CHUNKS; ++i) {
+        if (i >= (int)nchunk) break;
+        if (i + 1 < (int)nchunk) fetch(i + 1u, (i + 1) & 1);
+        const unsigned rows = bl.rows - 16u * i;
+        vec m = zero16<A>(), s = zero16<A>();
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
-            m = product<A>(k[t], k[t], m);
-            s = product<A>(q[t], k[t], s);
+            const vec kt = k[i & 1].get(t, rows, p.K, g, c), qt = q[i & 1].get(t, rows, p.K, g, c);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                m = mm16<A>::mac(kt[r], kt[r], m);
+                s = mm16<A>::mac(qt[r], kt[r], s);
+            }
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -108,41 +121,37 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
     if (!rows) return;
-    const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K, *v = V + row * p.ldv + l.v + l.c;
+    const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K, *v = V + row * p.ldv + l.v;
     T* o = O + row * p.ldo + l.v + l.c;
     delta_feed<T, KT, TEAM> feed;
     auto fetch = [&](unsigned t) {
         feed.fetch(p, q + t * p.ldq, k + t * p.ldk, chunks[(number(t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS], l.thread, rows - t);
     };
-    T next[4];
-    auto values = [&](unsigned t) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) next[r] = V && l.row(r) < rows - t && l.c < l.nv ? v[(t + l.row(r)) * p.ldv] : (T)A(0);
-    };
+    delta_values<T> values;
     fetch(0u);
-    values(0u);
-    feed.put(lds[0], l.thread);
+    if (V) values.fetch(l, v, p.ldv, rows);
+    feed.put(p, lds[0], l.thread);
     if (rows > DELTA_CHUNK) fetch(DELTA_CHUNK);
     __syncthreads();
     for (unsigned t = 0; t < rows; t += DELTA_CHUNK) {
         const unsigned n = min(rows - t, DELTA_CHUNK);
         const delta_rows<A, KT>& here = lds[t / DELTA_CHUNK & 1u];
-        vec x;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = (A)next[r];
+        vec x = V ? values.get(l) : zero16<A>();
         if (t + DELTA_CHUNK < rows) {
-            feed.put(lds[~(t / DELTA_CHUNK) & 1u], l.thread);
-            values(t + DELTA_CHUNK);
+            feed.put(p, lds[~(t / DELTA_CHUNK) & 1u], l.thread);
+            if (V) values.fetch(l, v + (t + DELTA_CHUNK) * p.ldv, p.ldv, rows - t - DELTA_CHUNK);
         }
         if (t + 2u * DELTA_CHUNK < rows) fetch(t + 2u * DELTA_CHUNK);
         if (l.nv) {
             if (keep && (t || row != first) && t % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + (kept + t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
             vec w = zero16<A>(), z = zero16<A>();
 #pragma unroll
-            for (int i = 0; i < KT; ++i) w = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], w);
-            if (OUT)
-#pragma unroll
-                for (int i = 0; i < KT; ++i) z = product<A>(tile_by_rows(here.q, i, l.g, l.c), S[i], z);
+            for (int i = 0; i < KT; ++i) {
+                if (OUT) products<A>(tile_by_rows(here.k, i, l.g, l.c), tile_by_rows(here.q, i, l.g, l.c), S[i], w, z);
+                else if (i & 1) z = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], z);
+                else w = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], w);
+            }
+            if (!OUT) w += z;
             const vec first = by_row(here.c.first, l.g), b = by_row(here.c.b, l.g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[r] = l.row(r) < n ? b[r] * (x[r] - first[r] * w[r]) : A(0);
@@ -150,7 +159,8 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
             const vec sent = by_row(here.c.last, l.g) * u;
             const A through = here.c.first[15];
 #pragma unroll
-            for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.k, i, l.g, l.c), sent, through * S[i]);
+            for (int i = 0; i < KT; ++i) S[i] *= through;
+            add_products<A, KT>(S, here.k, sent, l.g, l.c);
             if (OUT) {
                 const vec y = triangle<A, true>(matrix_by_rows(here.c.P, l.g, l.c), u, first * z, l.g);
 #pragma unroll

@@ -30,46 +30,41 @@ __device__ __forceinline__ void delta_walk_back(const delta_shape& p, const delt
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
     if (rows <= stop) return;
-    const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K, *d0 = dO + row * lddo + l.v + l.c;
+    const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K, *d0 = dO + row * lddo + l.v;
     delta_feed<T, KT, TEAM> feed;
     auto fetch = [&](unsigned t) {
         feed.fetch(p, q + t * p.ldq, k + t * p.ldk, chunks[(number(t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS], l.thread, rows - t);
     };
-    T next[4];
-    auto values = [&](unsigned t) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) next[i] = l.row(i) < rows - t && l.c < l.nv ? d0[(t + l.row(i)) * lddo] : (T)A(0);
-    };
+    delta_values<T> values;
     const unsigned end = (rows - 1) / DELTA_CHUNK * DELTA_CHUNK;
     fetch(end);
-    values(end);
-    feed.put(lds[end / DELTA_CHUNK & 1u], l.thread);
+    values.fetch(l, d0 + end * lddo, lddo, rows - end);
+    feed.put(p, lds[end / DELTA_CHUNK & 1u], l.thread);
     if (end > stop) fetch(end - DELTA_CHUNK);
     __syncthreads();
     for (unsigned left = (end - stop) / DELTA_CHUNK + 1u, t = end; left > 0; --left, t -= DELTA_CHUNK) {
         const delta_rows<A, KT>& here = lds[t / DELTA_CHUNK & 1u];
-        vec d;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = scale * (A)next[i];
+        const vec d = scale * values.get(l);
         if (left > 1u) {
-            feed.put(lds[~(t / DELTA_CHUNK) & 1u], l.thread);
-            values(t - DELTA_CHUNK);
+            feed.put(p, lds[~(t / DELTA_CHUNK) & 1u], l.thread);
+            values.fetch(l, d0 + (t - DELTA_CHUNK) * lddo, lddo, rows - t + DELTA_CHUNK);
         }
         if (left > 2u) fetch(t - 2u * DELTA_CHUNK);
         if (l.nv) {
-            vec y = zero16<A>();
+            vec y = zero16<A>(), z = zero16<A>();
 #pragma unroll
-            for (int i = 0; i < KT; ++i) y = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], y);
+            for (int i = 0; i < KT; ++i) (i & 1 ? z : y) = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], i & 1 ? z : y);
+            y += z;
             const vec first = by_row(here.c.first, l.g);
             const A through = here.c.first[15];
             const vec du = triangle<A, false>(matrix_by_columns(here.c.P, l.g, l.c), d, by_row(here.c.last, l.g) * y, l.g);
             const vec fd = first * d;
 #pragma unroll
-            for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.q, i, l.g, l.c), fd, through * S[i]);
+            for (int i = 0; i < KT; ++i) S[i] *= through;
+            add_products<A, KT>(S, here.q, fd, l.g, l.c);
             const vec dy = triangle<A, false>(matrix_by_columns(here.c.T, l.g, l.c), du, zero16<A>(), l.g);
             const vec dw = -(first * (by_row(here.c.b, l.g) * dy));
-#pragma unroll
-            for (int i = 0; i < KT; ++i) S[i] = product<A>(tile_by_columns(here.k, i, l.g, l.c), dw, S[i]);
+            add_products<A, KT>(S, here.k, dw, l.g, l.c);
             if (dstates && t % DELTA_BLOCK == 0) store_state<A, KT>(S, dstates + (size_t)(t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
         }
         __syncthreads();
@@ -190,15 +185,12 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
     const unsigned g = l.g, c = l.c, nchunk = (bl.rows + 15u) / 16u, slice = uniform(threadIdx.x >> 6) % TEAM, part = l.unit % out.parts;
     const size_t state = (size_t)p.K * p.H * p.V;
     const T *q0 = Q + (size_t)bl.at * p.ldq + (size_t)l.group * p.K, *k0 = K + (size_t)bl.at * p.ldk + (size_t)l.group * p.K;
-    const T *v0 = V + (size_t)bl.at * p.ldv + l.v + c, *d0 = dO + (size_t)bl.at * lddo + l.v + c;
+    const T *v0 = V + (size_t)bl.at * p.ldv + l.v, *d0 = dO + (size_t)bl.at * lddo + l.v;
     const size_t first_chunk = ((size_t)bl.slot * p.H + l.head) * DELTA_CHUNKS;
     delta_feed<T, KT, TEAM> feed;
     auto fetch = [&](unsigned i) { feed.fetch(p, q0 + 16u * i * p.ldq, k0 + 16u * i * p.ldk, chunks[first_chunk + i], l.thread, bl.rows - 16u * i); };
-    T next[4];
-    auto values = [&](const T* x, size_t ld, unsigned i) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) next[r] = 16u * i + l.row(r) < bl.rows && c < l.nv ? x[(16u * i + l.row(r)) * ld] : (T)A(0);
-    };
+    delta_values<T> next;
+    auto values = [&](const T* x, size_t ld, unsigned i) { next.fetch(l, x + 16u * i * ld, ld, bl.rows - 16u * i); };
 
     vec xs[DELTA_CHUNKS], us[DELTA_CHUNKS], sts[DELTA_CHUNKS][KT], dS[KT];
     fetch(0u);
@@ -212,10 +204,8 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
             if (i >= (int)nchunk) break;
             const unsigned n = min(bl.rows - 16u * i, 16u);
             if (i) __syncthreads();
-            feed.put(lds.rows, l.thread);
-            vec x, w = zero16<A>(), y;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = (A)next[r];
+            feed.put(p, lds.rows, l.thread);
+            vec x = next.get(l), w = zero16<A>(), y;
             if (i + 1 < (int)nchunk) {
                 fetch(i + 1u);
                 values(v0, p.ldv, i + 1u);
@@ -253,14 +243,13 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
         const delta_pairs<A>& pr = pairs[first_chunk + i];
         if (i + 1 < (int)nchunk) {               // (the last chunk's rows are there)
             __syncthreads();
-            feed.put(lds.rows, l.thread);
+            feed.put(p, lds.rows, l.thread);
             if (i) fetch(i - 1u);
             __syncthreads();
         }
         const delta_rows<A, KT>& here = lds.rows;
-        vec d, y = zero16<A>();
-#pragma unroll
-        for (int r = 0; r < 4; ++r) d[r] = scale * (A)next[r];
+        const vec d = scale * next.get(l);
+        vec y = zero16<A>();
         if (i) values(d0, lddo, i - 1u);
         // (fetched here, used behind the next barriers)
         const vec Dr = matrix_by_rows(pr.D, g, c), Dc = matrix_by_columns(pr.D, g, c), Nr = matrix_by_rows(pr.N, g, c);
