@@ -385,9 +385,12 @@ delta_shape delta_shape_of(const dbk_deltarule_args& a)
     s.V = (unsigned)a.V;
     s.ns = divup(a.V, 16);
     s.slots = (unsigned)segment_slots(a.N, DELTA_BLOCK);
-    // An even share of all rows for each of DELTA_WAVES waves: a region of more is cut. A segment's rows are walked twice, and its transition costs as much again as K columns
-    // of values, so that fewer, longer regions than fill the chip are what is cut.
-    const size_t share = (a.N * a.H * s.ns + DELTA_WAVES - 1) / DELTA_WAVES, L = ((share > DELTA_LEAST ? share : DELTA_LEAST) + DELTA_BLOCK - 1) / DELTA_BLOCK * DELTA_BLOCK;
+    // Regions are cut into as many segments as DELTA_WAVES waves take at once, a region's last one counted as a whole one: two waves per SIMD, and none left over for a second round
+    // (34 segments of 16 workgroups on 256 CUs that hold two took as long as 64). Where regions alone are half as many, only those of more than twice an even share are cut: a segment's
+    // rows are walked twice, and its transition costs as much again as K columns of values.
+    const size_t tracks = DELTA_WAVES / (a.H * ((s.ns + 3) / 4 * 4)), even = tracks ? tracks : 1;
+    size_t L = even > 2 * a.nregion ? (a.N + even - a.nregion - 1) / (even - a.nregion) : (2 * a.N + even - 1) / even;
+    L = ((L > DELTA_LEAST ? L : DELTA_LEAST) + DELTA_BLOCK - 1) / DELTA_BLOCK * DELTA_BLOCK;
     s.L = L < a.N ? (unsigned)L : 0u;
     s.cuts = s.L ? (unsigned)segment_slots(a.N, s.L) : 0u;
     s.ldq = a.ldq;

@@ -410,15 +410,27 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
     }
 }
 
-// out[row][col] = sum over shares of part[share][row][col], for the rows of one block
+// out[row][col] = sum over shares of part[share][row][col], in order, for 16 rows of a block; four values a thread where they fit
 template <typename A, typename T>
-__device__ __forceinline__ void add_shares(const delta_block& bl, size_t N, unsigned cols, unsigned shares, const A* part, T* out, size_t ld)
+__device__ __forceinline__ void add_shares(size_t at, unsigned rows, size_t N, unsigned cols, unsigned shares, const A* part, T* out, size_t ld)
 {
-    for (unsigned i = threadIdx.x; i < bl.rows * cols; i += 256u) {
-        const size_t row = bl.at + i / cols, col = i % cols;
-        A s = A(0);
-        for (unsigned u = 0; u < shares; ++u) s += part[((size_t)u * N + row) * cols + col];
-        out[row * ld + col] = (T)s;
+    const unsigned vecs = (cols + 3u) / 4u;
+    for (unsigned i = threadIdx.x; i < rows * vecs; i += 256u) {
+        const unsigned row = i / vecs, col = i % vecs * 4u, valid = cols - col;
+        const A* p = part + (at + row) * cols + col;
+        row_vec<A, 4> s;
+        row_vec<T, 4> o;
+        s.load(p, valid);
+#pragma unroll 4
+        for (unsigned u = 1; u < shares; ++u) {
+            row_vec<A, 4> x;
+            x.load(p + (size_t)u * N * cols, valid);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s.v[j] += x.v[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.v[j] = s.v[j];
+        o.store(out + (at + row) * ld + col, valid);
     }
 }
 
@@ -427,10 +439,13 @@ __global__ __launch_bounds__(256) void k_delta_add(delta_shape p, const uint32_t
 {
     delta_block bl;
     if (!find_block(p, regions, marks, blockIdx.x, bl)) return;
-    if (blockIdx.y == 0u && out.dq) add_shares(bl, p.N, p.G * p.K, p.H / p.G * out.parts, out.dq, out.dQ, out.lddq);
-    if (blockIdx.y == 1u && out.dq) add_shares(bl, p.N, p.G * p.K, p.H / p.G * out.parts, out.dk, out.dK, out.lddk);
-    if (blockIdx.y == 2u && out.db) add_shares(bl, p.N, p.H, out.parts, out.db, out.dbeta, out.lddb);
-    if (blockIdx.y == 2u && out.dg) add_shares(bl, p.N, p.H, out.parts, out.dg, out.ddecay, out.lddg);
+    const unsigned first = 16u * (blockIdx.y / 3u), what = blockIdx.y % 3u, rows = min(bl.rows - first, 16u);
+    if (first >= bl.rows) return;
+    const size_t at = (size_t)bl.at + first;
+    if (what == 0u && out.dq) add_shares(at, rows, p.N, p.G * p.K, p.H / p.G * out.parts, out.dq, out.dQ, out.lddq);
+    if (what == 1u && out.dq) add_shares(at, rows, p.N, p.G * p.K, p.H / p.G * out.parts, out.dk, out.dK, out.lddk);
+    if (what == 2u && out.db) add_shares(at, rows, p.N, p.H, out.parts, out.db, out.dbeta, out.lddb);
+    if (what == 2u && out.dg) add_shares(at, rows, p.N, p.H, out.parts, out.dg, out.ddecay, out.lddg);
 }
 
 namespace {
@@ -526,7 +541,7 @@ int dbk_deltarule_bprop(dbk_stream_t stream, const dbk_deltarule_args* a, void* 
                 s, a->lddo, a->regions, w.marks, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const T*)a->dO, (const delta_chunk<A>*)w.chunks, (const delta_pairs<A>*)w.pairs,
                 (A)a->scale, (const A*)a->keep, (const A*)w.dstates, out);
         });
-        if (!rc && (w.dq || w.db)) k_delta_add<T><<<dim3((unsigned)delta_blocks(s), 3), 256, 0, st>>>(s, a->regions, w.marks, out);
+        if (!rc && (w.dq || w.db)) k_delta_add<T><<<dim3((unsigned)delta_blocks(s), 3 * DELTA_CHUNKS), 256, 0, st>>>(s, a->regions, w.marks, out);
     });
     DBK_CHECK(!rc, "RuntimeError: the device has too little shared memory for a workgroup");
     DBK_LAUNCH_OK();
