@@ -23,22 +23,46 @@ struct block_shape {
     size_t lddr, lddz, lddy, lddo, lddg;         // backward: dr and dz in, dy, dr and dgate out (ldo: r')
 };
 
+// v of the lane n places further on in its row of 16, round it: no trip through LDS as for lanes further apart
+template <int N> __device__ __forceinline__ float rotated(float v)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, true));
+}
+template <int N> __device__ __forceinline__ double rotated(double v)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, 0x120 + N, 0xf, 0xf, true), hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), 0x120 + N, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// sums over LANES lanes of two values at once
 template <int LANES, typename A> __device__ __forceinline__ void block_sum2(A& u, A& v, A (*lds)[16])
 {
-    constexpr int W = LANES < 64 ? LANES : 64;
+    if constexpr (LANES >= 16) {
+        u += rotated<8>(u); v += rotated<8>(v);
+        u += rotated<4>(u); v += rotated<4>(v);
+        u += rotated<2>(u); v += rotated<2>(v);
+        u += rotated<1>(u); v += rotated<1>(v);
+        constexpr int W = LANES < 64 ? LANES : 64;
 #pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) {
-        u += __shfl_xor(u, o);
-        v += __shfl_xor(v, o);
-    }
+        for (int o = 16; o < W; o *= 2) {
+            u += __shfl_xor(u, o);
+            v += __shfl_xor(v, o);
+        }
+    } else
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+            u += __shfl_xor(u, o);
+            v += __shfl_xor(v, o);
+        }
     if constexpr (LANES > 64) {
-        constexpr int WAVES = LANES / 64;
+        constexpr int N = LANES / 64;
         __syncthreads();                         // (the words may still be read from the sums before)
         if ((threadIdx.x & 63) == 0) { lds[0][threadIdx.x >> 6] = u; lds[1][threadIdx.x >> 6] = v; }
         __syncthreads();
         u = v = A(0);
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) { u += lds[0][w]; v += lds[1][w]; }
+        for (int w = 0; w < N; ++w) { u += lds[0][w]; v += lds[1][w]; }
     }
 }
 
@@ -155,7 +179,7 @@ __global__ __launch_bounds__(block_threads<LANES>()) void k_block_fprop(block_sh
 }
 
 // The weights' gradients of a workgroup's rows are added in registers, its row lanes in LDS at the end, in a fixed order: part[blockIdx.x][5][m].
-template <typename T, int LANES, bool EXACT>
+template <typename T, int LANES, bool EXACT, bool RMS>
 __global__ __launch_bounds__(block_threads<LANES>()) void k_block_bprop(block_shape p, const T* __restrict__ Y, const T* __restrict__ O, const T* __restrict__ gate,
                                                                        const typename acc_of<T>::type* __restrict__ gamma, const typename acc_of<T>::type* __restrict__ beta,
                                                                        const typename acc_of<T>::type* __restrict__ scale, const typename acc_of<T>::type* __restrict__ ngamma,
@@ -203,26 +227,31 @@ __global__ __launch_bounds__(block_threads<LANES>()) void k_block_bprop(block_sh
         const unsigned now = row;
         row += p.rstep;
         fetch();
+        const bool here = now < p.n;
+        // (lanes and rows that do not exist send nothing back: t is zero there, and with it all that follows)
         A t[V], a = A(0), b = A(0);
         if (p.next) {
+            A h[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const A h = (o[j] - mean2) * rstd2, q = z[j] * g2[j];
-                sums[3][j] = fma(z[j], h, sums[3][j]);
+                h[j] = RMS ? o[j] * rstd2 : (o[j] - mean2) * rstd2;
+                t[j] = z[j] * g2[j];
+                sums[3][j] = fma(z[j], h[j], sums[3][j]);
                 sums[4][j] += z[j];
-                a += q;
-                b = fma(q, h, b);
+                if (!RMS) a += t[j];
+                b = fma(t[j], h[j], b);
             }
             block_sum2<LANES>(a, b, lds);
-            a = p.rms ? A(0) : a * inv;
-            b *= inv;
-        }
+            a = RMS ? A(0) : a * inv;
+            b *= -inv;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            t[j] = d[j];
-            if (p.next) t[j] += rstd2 * (fma(z[j], g2[j], -a) - (o[j] - mean2) * rstd2 * b);
-        }
-        const bool here = now < p.n;
+            for (int j = 0; j < V; ++j) {
+                const A q = fma(h[j], b, RMS ? t[j] : t[j] - a);
+                t[j] = (EXACT ? at.valid != 0u : j < (int)at.valid) && here ? fma(rstd2, q, d[j]) : A(0);
+            }
+        } else
+#pragma unroll
+            for (int j = 0; j < V; ++j) t[j] = d[j];
         row_vec<T> out;
         if (dO) {
 #pragma unroll
@@ -233,30 +262,31 @@ __global__ __launch_bounds__(block_threads<LANES>()) void k_block_bprop(block_sh
         a = b = A(0);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const bool real = EXACT ? at.valid != 0u : j < (int)at.valid;
-            const A h = (y[j] - mean1) * rstd1, pv = fma(h, g1[j], b1[j]);
-            A act = A(1);
+            const A h = RMS ? y[j] * rstd1 : (y[j] - mean1) * rstd1, pv = RMS && !beta ? h * g1[j] : fma(h, g1[j], b1[j]), ts = t[j] * sc[j], tp = t[j] * pv;
+            A dp = ts;
             if (gate) {
-                const A e = sigmoid_of(g[j]);
-                act = g[j] * e;
-                out.v[j] = t[j] * sc[j] * pv * (e * fma(g[j], A(1) - e, A(1)));
-            }
-            if (!real || !here) { q[j] = A(0); continue; }
-            const A dp = t[j] * sc[j] * act;
+                const A e = sigmoid_of(g[j]), act = g[j] * e;
+                dp = ts * act;
+                out.v[j] = ts * pv * fma(act, A(1) - e, e);
+                sums[2][j] = fma(tp, act, sums[2][j]);
+            } else
+                sums[2][j] += tp;
             sums[0][j] = fma(dp, h, sums[0][j]);
             sums[1][j] += dp;
-            sums[2][j] = fma(t[j] * pv, act, sums[2][j]);
             q[j] = dp * g1[j];
-            a += q[j];
+            if (!RMS) a += q[j];
             b = fma(q[j], h, b);
         }
         if (gate) store_vec<EXACT>(out, dgate + now * p.lddg + at.column, here ? at.valid : 0u);
         if (p.norm) {
             block_sum2<LANES>(a, b, lds);
-            a = p.rms ? A(0) : a * inv;
-            b *= inv;
+            a = RMS ? A(0) : a * inv;
+            b *= -inv;
 #pragma unroll
-            for (int j = 0; j < V; ++j) out.v[j] = rstd1 * (q[j] - a - (y[j] - mean1) * rstd1 * b);
+            for (int j = 0; j < V; ++j) {
+                const A h = RMS ? y[j] * rstd1 : (y[j] - mean1) * rstd1;
+                out.v[j] = rstd1 * fma(h, b, RMS ? q[j] : q[j] - a);
+            }
         } else
 #pragma unroll
             for (int j = 0; j < V; ++j) out.v[j] = q[j];
@@ -420,7 +450,8 @@ struct block_plan {
 };
 
 constexpr unsigned BLOCK_WAVES = 8192;           // forward: waves that walk the rows, eight per SIMD
-constexpr unsigned BLOCK_WAVES_BACK = 3072;      // backward: three per SIMD, whose partial sums are added up afterwards
+// Backward, whose workgroups' partial sums are added up afterwards: as many as the registers let run at once, two per SIMD with 8 values a lane (bfloat16), four with 4.
+inline unsigned back_waves_of(int dtype) { return dtype == DBK_F32 ? 4096u : 2048u; }
 constexpr size_t WIDE_WGS = 512;
 
 block_plan plan_block(const dbk_blocknorm_args& a, bool backward)
@@ -432,7 +463,7 @@ block_plan plan_block(const dbk_blocknorm_args& a, bool backward)
     const unsigned ct = p.lanes && p.lanes <= 256 ? chunks_side_by_side((unsigned)p.lanes, nchunk) : 0u;
     const unsigned rt = p.lanes ? (threads / p.lanes) >> ct : 1u;
     p.gy = p.lanes ? divup(nchunk, size_t(1) << ct) : 1u;
-    const unsigned wgs = (backward ? BLOCK_WAVES_BACK : BLOCK_WAVES) / (threads / 64u), most = wgs / p.gy ? wgs / p.gy : 1u;
+    const unsigned wgs = (backward ? back_waves_of(a.dtype) : BLOCK_WAVES) / (threads / 64u), most = wgs / p.gy ? wgs / p.gy : 1u;
     p.gx = divup(a.n, rt);
     if (p.gx > most) p.gx = most;
     if (!p.lanes) p.gx = (unsigned)(a.n < WIDE_WGS ? a.n : WIDE_WGS);
@@ -544,7 +575,8 @@ int dbk_blocknorm_bprop(dbk_stream_t stream, const dbk_blocknorm_args* a, void* 
             typedef typename acc_of<T>::type A;
             A* part = weights ? (A*)work : nullptr;
             if (!block_layout(p.lanes, a->group % row_vec<T>::N == 0, [&](auto lanes, auto exact) {
-                    k_block_bprop<T, lanes.value, exact.value><<<dim3(p.gx, p.gy), block_threads<lanes.value>(), 0, st>>>(
+                    auto kernel = a->rms ? k_block_bprop<T, lanes.value, exact.value, true> : k_block_bprop<T, lanes.value, exact.value, false>;
+                    kernel<<<dim3(p.gx, p.gy), block_threads<lanes.value>(), 0, st>>>(
                         p.shape, (const T*)a->Y, (const T*)a->O, (const T*)a->gate, (const A*)a->gamma, (const A*)a->beta, (const A*)a->scale, (const A*)a->next_gamma,
                         (const A*)a->stats, (const T*)a->dR, (const T*)a->dZ, (T*)a->dY, (T*)a->dR_in, (T*)a->dgate, part);
                 }))
