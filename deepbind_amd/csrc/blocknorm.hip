@@ -112,6 +112,20 @@ template <int LANES, int V> struct block_place {
     __device__ __forceinline__ bool leads(const block_shape& p) const { return lane == 0u && chunk < p.nchunk; }
 };
 
+// step(ahead, row) for every row of a lane, each fetched one or two (as many as `ahead` holds) of the lane's rows before. Every lane of a workgroup makes the same number of
+// steps, whether its row exists or not: sums over its waves meet at barriers.
+template <typename AHEAD, int N, typename FETCH, typename STEP>
+__device__ __forceinline__ void walk_rows(const block_shape& p, unsigned first, size_t row, AHEAD (&ahead)[N], FETCH fetch, STEP step)
+{
+    const size_t by = (size_t)N * p.rstep;
+#pragma unroll
+    for (int i = 0; i < N; ++i) fetch(ahead[i], row + (size_t)i * p.rstep);
+    for (size_t left = first; left < p.n; left += by, row += by) {
+        step(ahead[0], row);
+        if (N > 1 && left + p.rstep < p.n) step(ahead[N - 1], row + p.rstep);
+    }
+}
+
 // LANES of more than 64 share a workgroup of their own size with no other chunk: plan_block gives it one row at a time.
 template <typename T, int LANES, bool EXACT>
 __global__ __launch_bounds__(block_threads<LANES>()) void k_block_fprop(block_shape p, const T* __restrict__ Y, const T* __restrict__ R, const T* __restrict__ gate,
@@ -132,21 +146,18 @@ __global__ __launch_bounds__(block_threads<LANES>()) void k_block_fprop(block_sh
     load_weights(b2, nbeta ? nbeta + at.column : nullptr, at.valid, A(0));
     const A inv = A(1) / (A)p.width;
     const size_t units = (size_t)p.n * p.nchunk;
-    unsigned row = at.row;
-    raw_vec<T, EXACT> ny, nr, ng;
-    auto fetch = [&]() {
+    // (a second row ahead is worth 170 to 158 us on 50021 rows of 64 chunks of 16 floats; bfloat16 ones it costs a fourth wave per SIMD: 491 us for 435 on 130003 x 1440)
+    constexpr unsigned AHEAD = sizeof(T) == 2 ? 1 : 2;
+    struct { raw_vec<T, EXACT> y, r, g; } ahead[AHEAD];
+    auto fetch = [&](auto& to, size_t row) {
         const unsigned valid = row < p.n ? at.valid : 0u;
-        ny.load(Y + row * p.ldy + at.column, valid);
-        if (R) nr.load(R + row * p.ldr + at.column, valid);
-        if (gate) ng.load(gate + row * p.ldg + at.column, valid);
+        to.y.load(Y + row * p.ldy + at.column, valid);
+        if (R) to.r.load(R + row * p.ldr + at.column, valid);
+        if (gate) to.g.load(gate + row * p.ldg + at.column, valid);
     };
-    fetch();
-    // (every lane of a workgroup makes the same number of steps: sums over its waves meet at barriers)
-    for (unsigned left = at.first; left < p.n; left += p.rstep) {
-        const raw_vec<T, EXACT> y = ny, r = nr, g = ng;
-        const unsigned now = row;
-        row += p.rstep;
-        fetch();
+    auto step = [&](auto& from, size_t now) {
+        const raw_vec<T, EXACT> y = from.y, r = from.r, g = from.g;
+        fetch(from, now + AHEAD * (size_t)p.rstep);
         A x[V], mean = A(0), rstd = A(1);
 #pragma unroll
         for (int j = 0; j < V; ++j) x[j] = y[j];
@@ -166,7 +177,7 @@ __global__ __launch_bounds__(block_threads<LANES>()) void k_block_fprop(block_sh
         }
         const bool here = now < p.n;
         store_vec<EXACT>(o, O + now * p.ldo + at.column, here ? at.valid : 0u);
-        if (!p.next) continue;
+        if (!p.next) return;
         chunk_stats<LANES>(x, at.valid, inv, eps, p.rms, mean, rstd, lds);
         if (stats && here && at.leads(p)) {
             stats[2 * units + (size_t)now * p.nchunk + at.chunk] = mean;
@@ -175,7 +186,8 @@ __global__ __launch_bounds__(block_threads<LANES>()) void k_block_fprop(block_sh
 #pragma unroll
         for (int j = 0; j < V; ++j) o.v[j] = fma((x[j] - mean) * rstd, g2[j], b2[j]);
         store_vec<EXACT>(o, Z + now * p.ldz + at.column, here ? at.valid : 0u);
-    }
+    };
+    walk_rows(p, at.first, at.row, ahead, fetch, step);
 }
 
 // The weights' gradients of a workgroup's rows are added in registers, its row lanes in LDS at the end, in a fixed order: part[blockIdx.x][5][m].
@@ -202,31 +214,28 @@ __global__ __launch_bounds__(block_threads<LANES>()) void k_block_bprop(block_sh
         for (int j = 0; j < V; ++j) sums[i][j] = A(0);
     const A inv = A(1) / (A)p.width;
     const size_t units = (size_t)p.n * p.nchunk;
-    unsigned row = at.row;
-    raw_vec<T, EXACT> ny, no, ng, nd, nz;
-    A n1 = 0, n2 = 0, n3 = 0, n4 = 0;
-    auto fetch = [&]() {
+    // (a second row ahead costs float rows two of four waves per SIMD: 262 us where it is 247 on 50021 rows of 64 chunks; bfloat16 ones nothing: 744 for 857 on 130003 x 1440)
+    constexpr unsigned AHEAD = sizeof(T) == 2 ? 2 : 1;
+    struct { raw_vec<T, EXACT> y, o, g, d, z; A s[4]; } ahead[AHEAD];
+    auto fetch = [&](auto& to, size_t row) {
         const bool here = row < p.n && at.chunk < p.nchunk;
         const unsigned valid = here ? at.valid : 0u;
-        const size_t u = (size_t)row * p.nchunk + at.chunk;
-        ny.load(Y + row * p.ldy + at.column, valid);
-        if (gate) ng.load(gate + row * p.ldg + at.column, valid);
-        nd.load(dR + row * p.lddr + at.column, dR ? valid : 0u);
-        if (p.norm) { n1 = here ? stats[u] : A(0); n2 = here ? stats[units + u] : A(0); }
+        const size_t u = row * p.nchunk + at.chunk;
+        to.y.load(Y + row * p.ldy + at.column, valid);
+        if (gate) to.g.load(gate + row * p.ldg + at.column, valid);
+        to.d.load(dR + row * p.lddr + at.column, dR ? valid : 0u);
+        if (p.norm) { to.s[0] = here && !RMS ? stats[u] : A(0); to.s[1] = here ? stats[units + u] : A(0); }
         if (p.next) {
-            no.load(O + row * p.ldo + at.column, valid);
-            nz.load(dZ + row * p.lddz + at.column, valid);
-            n3 = here ? stats[2 * units + u] : A(0);
-            n4 = here ? stats[3 * units + u] : A(0);
+            to.o.load(O + row * p.ldo + at.column, valid);
+            to.z.load(dZ + row * p.lddz + at.column, valid);
+            to.s[2] = here && !RMS ? stats[2 * units + u] : A(0);
+            to.s[3] = here ? stats[3 * units + u] : A(0);
         }
     };
-    fetch();
-    for (unsigned left = at.first; left < p.n; left += p.rstep) {
-        const raw_vec<T, EXACT> y = ny, o = no, g = ng, d = nd, z = nz;
-        const A mean1 = n1, rstd1 = p.norm ? n2 : A(1), mean2 = n3, rstd2 = n4;
-        const unsigned now = row;
-        row += p.rstep;
-        fetch();
+    auto step = [&](auto& from, size_t now) {
+        const raw_vec<T, EXACT> y = from.y, o = from.o, g = from.g, d = from.d, z = from.z;
+        const A mean1 = p.norm ? from.s[0] : A(0), rstd1 = p.norm ? from.s[1] : A(1), mean2 = from.s[2], rstd2 = from.s[3];
+        fetch(from, now + AHEAD * (size_t)p.rstep);
         const bool here = now < p.n;
         // (lanes and rows that do not exist send nothing back: t is zero there, and with it all that follows)
         A t[V], a = A(0), b = A(0);
@@ -291,7 +300,8 @@ __global__ __launch_bounds__(block_threads<LANES>()) void k_block_bprop(block_sh
 #pragma unroll
             for (int j = 0; j < V; ++j) out.v[j] = q[j];
         store_vec<EXACT>(out, dY + now * p.lddy + at.column, here ? at.valid : 0u);
-    }
+    };
+    walk_rows(p, at.first, at.row, ahead, fetch, step);
     if (!part) return;
     const size_t m = (size_t)p.nchunk * p.width;
     const unsigned across = LANES << p.ct_log2;                 // threads of one row lane
@@ -449,9 +459,9 @@ struct block_plan {
     block_shape shape;
 };
 
-constexpr unsigned BLOCK_WAVES = 8192;           // forward: waves that walk the rows, eight per SIMD
-// Backward, whose workgroups' partial sums are added up afterwards: as many as the registers let run at once, two per SIMD with 8 values a lane (bfloat16), four with 4.
-inline unsigned back_waves_of(int dtype) { return dtype == DBK_F32 ? 4096u : 2048u; }
+// Waves that walk the rows. Forward several rounds of them even out (bfloat16 435 us with 8192, 483 with the 4096 that run at once); backward, where each workgroup's partial sums are
+// added up afterwards, no more than run at once: three per SIMD with four floats a lane, two with eight bfloat16 values, three with two doubles.
+inline unsigned block_waves_of(int dtype, bool backward) { return !backward ? 8192u : dtype == DBK_BF16 ? 2048u : 3072u; }
 constexpr size_t WIDE_WGS = 512;
 
 block_plan plan_block(const dbk_blocknorm_args& a, bool backward)
@@ -463,7 +473,7 @@ block_plan plan_block(const dbk_blocknorm_args& a, bool backward)
     const unsigned ct = p.lanes && p.lanes <= 256 ? chunks_side_by_side((unsigned)p.lanes, nchunk) : 0u;
     const unsigned rt = p.lanes ? (threads / p.lanes) >> ct : 1u;
     p.gy = p.lanes ? divup(nchunk, size_t(1) << ct) : 1u;
-    const unsigned wgs = (backward ? back_waves_of(a.dtype) : BLOCK_WAVES) / (threads / 64u), most = wgs / p.gy ? wgs / p.gy : 1u;
+    const unsigned wgs = block_waves_of(a.dtype, backward) / (threads / 64u), most = wgs / p.gy ? wgs / p.gy : 1u;
     p.gx = divup(a.n, rt);
     if (p.gx > most) p.gx = most;
     if (!p.lanes) p.gx = (unsigned)(a.n < WIDE_WGS ? a.n : WIDE_WGS);

@@ -97,7 +97,7 @@ template <typename A, bool LOWER> __device__ __forceinline__ typename mm16<A>::v
     return o;
 }
 
-// What one wave prepares for a chunk of a head, as later kernels read it: matrices row by row, and per row what it decays and corrects by. Rows behind a
+// What one wave prepares for a chunk of a head, as later kernels read it: matrices column by column, and per row what it decays and corrects by. Rows behind a
 // region's last: T is the identity there, N, P and b are zero, and nothing decays.
 template <typename A> struct delta_chunk {
     A T[256], P[256];
@@ -350,19 +350,19 @@ template <typename T, int KT> struct delta_tiles {
         return v;
     }
 };
-// and of a chunk's own matrices: [c][row(g, r)] (by rows), [row(g, r)][c] (by columns); vectors [row(g, r)]
+// and of a chunk's own matrices, which lie by columns: [c][row(g, r)] (by rows), [row(g, r)][c] (by columns); vectors [row(g, r)]
 template <typename A> __device__ __forceinline__ typename mm16<A>::vec matrix_by_rows(const A* m, unsigned g, unsigned c)
 {
     typename mm16<A>::vec f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) f[r] = m[16u * c + mm16<A>::row(g, r)];
+    for (int r = 0; r < 4; ++r) f[r] = m[16u * mm16<A>::row(g, r) + c];
     return f;
 }
 template <typename A> __device__ __forceinline__ typename mm16<A>::vec matrix_by_columns(const A* m, unsigned g, unsigned c)
 {
     typename mm16<A>::vec f;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) f[r] = m[16u * mm16<A>::row(g, r) + c];
+    for (int r = 0; r < 4; ++r) f[r] = m[16u * c + mm16<A>::row(g, r)];
     return f;
 }
 template <typename A> __device__ __forceinline__ typename mm16<A>::vec by_row(const A* m, unsigned g)

@@ -15,7 +15,8 @@ __global__ __launch_bounds__(256) void k_delta_mark(delta_shape p, const uint32_
 
 // A chunk's matrices. A wave takes a block of a head, four chunks: the products of its keys and queries on the matrix cores, then a lane per chunk and column for the
 // decays between rows and the triangle's inverse, column by column by substitution (powers of the triangle, which the matrix cores
-// could multiply instead, grow far beyond the inverse where keys come again, and lose it).
+// could multiply instead, grow far beyond the inverse where keys come again, and lose it). A wave waits for memory most of its time, first for its block, then for its
+// rows: what it needs is asked for at once, and its share of LDS, which keys' products and queries' use in turn, lets six of them run per SIMD.
 template <typename T, int KT>
 __global__ __launch_bounds__(256) void k_delta_prepare(delta_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, const T* __restrict__ Q,
                                                        const T* __restrict__ K, const typename acc_of<T>::type* __restrict__ beta,
@@ -24,10 +25,11 @@ __global__ __launch_bounds__(256) void k_delta_prepare(delta_shape p, const uint
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
-    __shared__ A kk_all[4][4][16][17], qk_all[4][4][16][17], b_all[4][64];
+    __shared__ __align__(16) A lds_all[4][4][16][20];
     __shared__ double a_all[4][64];
+    __shared__ A b_all[4][64];
     const unsigned wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63u, g = lane >> 4, c = lane & 15u;
-    A (*kk)[16][17] = kk_all[wave], (*qk)[16][17] = qk_all[wave];
+    A (*lds)[16][20] = lds_all[wave];
     A* b = b_all[wave];
     double* a = a_all[wave];
     delta_block bl;
@@ -43,71 +45,103 @@ __global__ __launch_bounds__(256) void k_delta_prepare(delta_shape p, const uint
         q[to].fetch(Q + row * p.ldq + (size_t)group * p.K, p.ldq, rows, p.K, g, c);
     };
     fetch(0u, 0);
+    raw_one<A> rate, step;
+    {
+        const size_t row = bl.at + min(lane, bl.rows - 1u);
+        step.load(beta + row * p.ldb + head);
+        rate.load(decay ? decay + row * p.ldg + head : beta + row * p.ldb + head);
+    }
+    vec ms[DELTA_CHUNKS], ss[DELTA_CHUNKS];
 #pragma unroll
     for (int i = 0; i < (int)DELTA_CHUNKS; ++i) {
-        if (i >= (int)nchunk) break;
+        ms[i] = ss[i] = zero16<A>();
+        if (i >= (int)nchunk) continue;
         if (i + 1 < (int)nchunk) fetch(i + 1u, (i + 1) & 1);
         const unsigned rows = bl.rows - 16u * i;
-        vec m = zero16<A>(), s = zero16<A>();
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             const vec kt = k[i & 1].get(t, rows, p.K, g, c), qt = q[i & 1].get(t, rows, p.K, g, c);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                m = mm16<A>::mac(kt[r], kt[r], m);
-                s = mm16<A>::mac(qt[r], kt[r], s);
+                ms[i] = mm16<A>::mac(kt[r], kt[r], ms[i]);
+                ss[i] = mm16<A>::mac(qt[r], kt[r], ss[i]);
             }
         }
+    }
+    // (a wave's LDS is its own: its instructions there run in order, and only the compiler is kept from changing it)
+    auto sync = []() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); };
+    auto put = [&](const vec (&x)[DELTA_CHUNKS]) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            kk[i][mm16<A>::row(g, r)][c] = m[r];
-            qk[i][mm16<A>::row(g, r)][c] = s[r];
+        for (int i = 0; i < (int)DELTA_CHUNKS; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) lds[i][mm16<A>::row(g, r)][c] = x[i][r];
+        sync();
+    };
+    // columns of all chunks' matrices through LDS to memory, a matrix of 16 x 16 values at a time, consecutive lanes to consecutive places
+    const size_t number = ((size_t)bl.slot * p.H + head) * DELTA_CHUNKS;
+    auto store = [&](auto matrix, const A (&x)[16]) {
+        sync();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) lds[g][c][i] = x[i];
+        sync();
+        for (unsigned i = 0; i < nchunk; ++i) {
+            row_vec<A, 4> v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v.v[j] = lds[i][lane >> 2][4u * (lane & 3u) + j];
+            v.store(matrix(number + i) + 4u * lane, 4u);
         }
-    }
-    {
-        const bool here = lane < bl.rows;
-        const size_t row = bl.at + (here ? lane : 0u);
-        a[lane] = here && decay ? exp((double)decay[row * p.ldg + head]) : 1.0;
-        b[lane] = here ? beta[row * p.ldb + head] : A(0);
-    }
-    __syncthreads();
+        sync();
+    };
+    put(ms);
+    a[lane] = decay && lane < bl.rows ? exp((double)rate.get(true)) : 1.0;
+    b[lane] = step.get(lane < bl.rows);
+    sync();
     // lane (g, c): column c of chunk g
-    const bool there = g < nchunk;
-    const size_t at = ((size_t)bl.slot * p.H + head) * DELTA_CHUNKS + g;
-    if (there) {
+    A D[16], n[16];
+    {
         // (in double precision: a state that decays by a thousandth a row remembers a thousand of them, and would their factors' roundings)
         double product = 0.0, first = 1.0;
-        A mine = A(1), D = A(0);
+        A mine = A(1);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const double ai = a[16u * g + i];
             product = i == (int)c ? 1.0 : product * ai;          // (zero above the diagonal: nothing there yet)
-            D = (A)product;
+            D[i] = i >= (int)c ? (A)product : A(0);
             first *= ai;
             mine = i == (int)c ? (A)first : mine;
-            const A n = i > (int)c ? D * kk[g][i][c] : A(0), s = i >= (int)c ? D * qk[g][i][c] : A(0);
-            kk[g][i][c] = n;
-            chunks[at].P[16 * i + c] = s;
-            if (pairs) {
-                pairs[at].N[16 * i + c] = n;
-                pairs[at].D[16 * i + c] = i >= (int)c ? D : A(0);
-            }
+            n[i] = i > (int)c ? D[i] * lds[g][i][c] : A(0);
         }
-        chunks[at].first[c] = mine;
-        chunks[at].last[c] = D;
-        chunks[at].b[c] = b[16u * g + c];
+        if (g < nchunk) {
+            delta_chunk<A>& to = chunks[number + g];
+            to.first[c] = mine;
+            to.last[c] = D[15];
+            to.b[c] = b[16u * g + c];
+        }
     }
-    __syncthreads();
-    if (!there) return;
-    A x[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        A s = A(0);
-#pragma unroll
-        for (int m = 0; m < i; ++m) s = fma(kk[g][i][m], x[m], s);
-        x[i] = i < (int)c ? A(0) : fma(-b[16u * g + i], s, i == (int)c ? A(1) : A(0));
-        chunks[at].T[16 * i + c] = x[i];
+    if (pairs) {
+        store([&](size_t i) { return pairs[i].N; }, n);
+        store([&](size_t i) { return pairs[i].D; }, D);
     }
+    sync();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) lds[g][i][c] = n[i];
+    sync();
+    {
+        A x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            A s[4] = {A(0), A(0), A(0), A(0)};
+#pragma unroll
+            for (int m = 0; m < i; ++m) s[m & 3] = fma(lds[g][i][m], x[m], s[m & 3]);
+            x[i] = i < (int)c ? A(0) : fma(-b[16u * g + i], (s[0] + s[1]) + (s[2] + s[3]), i == (int)c ? A(1) : A(0));
+        }
+        store([&](size_t i) { return chunks[i].T; }, x);
+    }
+    put(ss);
+    A s[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = i >= (int)c ? D[i] * lds[g][i][c] : A(0);
+    store([&](size_t i) { return chunks[i].P; }, s);
 }
 
 // Walks a wave's 16 columns of a head's state down `rows` rows from `row` on, of a region that starts at `first`. number(k): the number of the block k blocks on from the first.

@@ -283,41 +283,51 @@ def clip_gradients(grads, max_norm, nblock=1, by_rows=None, out=None):
     leaves zeros, and NaN in place of infinities. Returns the norms (1 x nblock, float64)."""
     grads = list(grads)
     outs = grads if out is None else list(out)
-    nblock = int(nblock)
+    nblock, max_norm, count = int(nblock), float(max_norm), len(grads)
     require(nblock >= 1, "ValueError: nblock must be at least 1")
-    require(float(max_norm) > 0, "ValueError: the largest norm must be positive")
-    require(len(outs) == len(grads), "ValueError: out must have as many tensors as grads")
-    require(by_rows is None or len(by_rows) == len(grads), "ValueError: by_rows must have an entry for every tensor")
-    require(len(grads) > 0, "ValueError: no tensors")
-    table = (_lib.ClipTensor * len(grads))()
+    require(max_norm > 0, "ValueError: the largest norm must be positive")
+    require(len(outs) == count, "ValueError: out must have as many tensors as grads")
+    require(by_rows is None or len(by_rows) == count, "ValueError: by_rows must have an entry for every tensor")
+    require(count > 0, "ValueError: no tensors")
     a = _lib.Arguments()
-    for i, (g, o) in enumerate(zip(grads, outs)):
+    table = []                                   # dbk_clip_tensor's words: in, out, rows, cols, strides, dtype and by_rows
+    for i, g in enumerate(grads):
+        o = outs[i]
         if not isinstance(g, torch.Tensor) or not isinstance(o, torch.Tensor):
             raise _lib.DeepbindError("TypeError: grads and out must be lists of tensors")
         code = _lib.row_dtype_code(g)
-        rows = by_rows is not None and bool(by_rows[i])
-        if g.dim() == 2:
-            n, m = g.shape
-            p, ld = a.rows("grads[%d]" % i, g, g.shape, g.dtype, out=o is g)
-            q, ldo = (p, ld) if o is g else a.rows("out[%d]" % i, o, g.shape, g.dtype, out=True)
-            require((n if rows else m) % nblock == 0, "ValueError: a tensor's models must be equal blocks of its columns, or rows")
-            if nblock == 1 and ld == m and ldo == m:
-                n, m = 1, n * m
-                ld = ldo = m
+        rows = 1 if by_rows is not None and by_rows[i] else 0
+        same, n = o is g, g.numel()
+        if nblock == 1 and g.is_contiguous() and (same or (o.is_contiguous() and o.dtype is g.dtype and o.shape == g.shape)):
+            # (the common case, without names for messages: a set of many tensors is bound by what a call costs the host)
+            p, m, at = g.data_ptr(), n, g.get_device()
+            q, size = p, n * g.element_size()
+            if not same:
+                a.ins.append((p, p + size, at, g))
+                q, at = o.data_ptr(), o.get_device()
+            a.outs.append((q, q + size, at, o))
+            n, ld, ldo = 1, m, m
+        elif g.dim() == 2:
+            n, m = shape = g.shape
+            p, ld = a.rows("grads[%d]" % i, g, shape, g.dtype, same)
+            q, ldo = (p, ld) if same else a.rows("out[%d]" % i, o, shape, g.dtype, True)
+            if nblock > 1 and (n if rows else m) % nblock:
+                raise _lib.DeepbindError("ValueError: a tensor's models must be equal blocks of its columns, or rows")
         else:
             require(nblock == 1, "ValueError: models side by side are blocks of matrices")
-            p = a.dense("grads[%d]" % i, g, g.shape, g.dtype, out=o is g)
-            q = p if o is g else a.dense("out[%d]" % i, o, g.shape, g.dtype, out=True)
+            p = a.dense("grads[%d]" % i, g, g.shape, g.dtype, out=same)
+            q = p if same else a.dense("out[%d]" % i, o, g.shape, g.dtype, out=True)
             n, m = 1, g.numel()
             ld = ldo = m
-        table[i] = (p, q, n, m, ld, ldo, code, int(rows))
+        table += (p, q, n, m, ld, ldo, code | rows << 32)
     _lib.check_many(a)
     norms = torch.empty((1, nblock), dtype=torch.float64, device=grads[0].device)
+    table = (ctypes.c_uint64 * len(table))(*table)
     need = ctypes.c_size_t(0)
     where = ctypes.addressof(table)
-    call("dbk_clip_gradients_workspace", len(grads), where, nblock, ctypes.addressof(need))
+    call("dbk_clip_gradients_workspace", count, where, nblock, ctypes.addressof(need))
     work, wp = _lib.workspace(need.value, norms)
-    call("dbk_clip_gradients", stream(), len(grads), where, nblock, float(max_norm), norms.data_ptr(), wp, need.value)
+    call("dbk_clip_gradients", stream(), count, where, nblock, max_norm, norms.data_ptr(), wp, need.value)
     return norms
 
 
