@@ -10,8 +10,8 @@
 //   N[i][j] = D[i][j] k[i].k[j] (j < i),  P[i][j] = D[i][j] q[i].k[j] (j <= i),  T = (I + diag(b) N)^-1
 //   X = V - first (K S0),  U = T (b X),  O = scale (first (Q S0) + P U),  S1 = first[15] S0 + K^T (last U)
 //
-// so that a chunk is a handful of 16-row products for the matrix cores. They run in the accumulation type (v_mfma_f32_16x16x4_f32, v_mfma_f64_16x16x4_f64): every
-// product and sum is as exact as the states, also where rows are bfloat16. Decays are products of the rows' own factors, never quotients
+// so that a chunk is a handful of 16-row products for the matrix cores. They run in the accumulation type (v_mfma_f32_16x16x4_f32, v_mfma_f64_16x16x4_f64), or on exact pieces of it
+// (delta_ops): every product and sum is as exact as the states, also where rows are bfloat16. Decays are products of the rows' own factors, never quotients
 // or exponentials of differences of sums, so that a factor of zero, or a long run of small ones, does what it does row by row.
 //
 // A matrix instruction's result and its right operand lie alike, but for the order in which the contraction runs: the lane that receives D[row(g, r)][c]
@@ -20,6 +20,7 @@
 // gradients never leave the registers. A wave holds 16 columns of a head's state and shares nothing with those that hold the others.
 #pragma once
 #include <type_traits>
+#include "mfma_common.h"
 #include "rows_common.h"
 
 namespace dbk {
@@ -209,21 +210,111 @@ template <typename A, int W> __device__ __forceinline__ typename mm16<A>::vec ti
 // Waves per SIMD that the walks are compiled for: their registers hold 4 values per lane of a state's every 16 rows. (Four teams of 32-column keys fill half the LDS.)
 template <typename A, int KT, int TEAM> constexpr int delta_waves() { return sizeof(A) == 4 ? (KT > 4 || (KT == 2 && TEAM == 1) ? 2 : 4) : KT > 4 || (KT == 2 && TEAM == 1) ? 1 : 2; }
 
-// S[t] += m's tile t by columns, transposed, times x
-template <typename A, int KT, int W> __device__ __forceinline__ void add_products(typename mm16<A>::vec (&S)[KT], const A (&m)[16][W], typename mm16<A>::vec x, unsigned g, unsigned c)
-{
-    constexpr int S2 = KT < 4 ? KT : 4;
+// What the walks along a region do with keys, queries and the state: w = k S (and z = q S), and S += m^T x for m of keys or queries.
+template <typename T, int KT> struct delta_ops {
+    typedef typename acc_of<T>::type A;
+    typedef typename mm16<A>::vec vec;
+    typedef delta_rows<A, KT> rows;
+    template <bool BOTH, int W> static __device__ __forceinline__ void find(const A (&k)[16][W], const A (&q)[16][W], const vec (&S)[KT], vec& w, vec& z, unsigned g, unsigned c)
+    {
 #pragma unroll
-    for (int t = 0; t < KT; t += S2) {
-        typename mm16<A>::vec f[S2];
-#pragma unroll
-        for (int i = 0; i < S2; ++i) f[i] = tile_by_columns(m, t + i, g, c);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int i = 0; i < S2; ++i) S[t + i] = mm16<A>::mac(f[i][r], x[r], S[t + i]);
+        for (int i = 0; i < KT; ++i) {
+            if (BOTH) products<A>(tile_by_rows(k, i, g, c), tile_by_rows(q, i, g, c), S[i], w, z);
+            else (i & 1 ? z : w) = product<A>(tile_by_rows(k, i, g, c), S[i], i & 1 ? z : w);
+        }
+        if (!BOTH) w += z;
     }
-}
+    template <int W> static __device__ __forceinline__ void add(vec (&S)[KT], const A (&m)[16][W], vec x, unsigned g, unsigned c)
+    {
+        constexpr int N = KT < 4 ? KT : 4;
+#pragma unroll
+        for (int t = 0; t < KT; t += N) {
+            vec f[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = tile_by_columns(m, t + i, g, c);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int i = 0; i < N; ++i) S[t + i] = mm16<A>::mac(f[i][r], x[r], S[t + i]);
+        }
+    }
+};
+
+// Rows kept in bfloat16 are matrix operands as they are; the float on the other side is the exact sum of three bfloat16 numbers (split3), so that three products on the 16 times
+// faster bfloat16 instructions take the place of one in float, as exact as it: two tiles of the state at once where its rows are what is summed over, and one where the
+// chunk's are. An infinite state or correction is a NaN here: its remainders are. Keys and queries stay bfloat16 in LDS, from where the transposing read takes them by columns:
+// lane (g, i) names four columns of row 4 g + i / 4 and receives column i of rows 4 g to 4 g + 3.
+template <int KT> struct delta_rows16 {
+    __align__(16) unsigned short k[16][16 * KT + 8], q[16][16 * KT + 8];
+    delta_chunk<float> c;
+};
+template <int KT> struct delta_ops<bf16_t, KT> {
+    typedef mm16<float>::vec vec;
+    typedef delta_rows16<KT> rows;
+    typedef short quad __attribute__((ext_vector_type(4)));
+    struct pieces { uint2 hi, mid, lo; };
+    static __device__ __forceinline__ pieces split(vec x)
+    {
+        unsigned h[4], m[4], l[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) dbk_mfma::split3(x[r], l[r], m[r], h[r]);
+        using dbk_mfma::pack_upper_halves;
+        return {make_uint2(pack_upper_halves(h[0], h[1]), pack_upper_halves(h[2], h[3])), make_uint2(pack_upper_halves(m[0], m[1]), pack_upper_halves(m[2], m[3])),
+                make_uint2(pack_upper_halves(l[0], l[1]), pack_upper_halves(l[2], l[3]))};
+    }
+    static __device__ __forceinline__ vec mac16(uint2 a, uint2 b, vec c) { return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(quad, a), __builtin_bit_cast(quad, b), c, 0, 0, 0); }
+    static __device__ __forceinline__ vec mac32(uint2 a, uint2 a2, uint2 b, uint2 b2, vec c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dbk_mfma::bf16x8_t, make_uint4(a.x, a.y, a2.x, a2.y)), __builtin_bit_cast(dbk_mfma::bf16x8_t, make_uint4(b.x, b.y, b2.x, b2.y)),
+                                                       c, 0, 0, 0);
+    }
+    template <int W> static __device__ __forceinline__ uint2 by_rows(const unsigned short (&m)[16][W], int t, unsigned g, unsigned c)
+    {
+        return *reinterpret_cast<const uint2*>(&m[c][16u * t + 4u * g]);
+    }
+    template <int W> static __device__ __forceinline__ uint2 by_columns(const unsigned short (&m)[16][W], int t, unsigned g, unsigned c)
+    {
+        typedef __attribute__((address_space(3))) quad* at;
+        return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((at)(const_cast<unsigned short*>(&m[4u * g + (c >> 2)][16u * t + 4u * (c & 3u)]))));
+    }
+    template <bool BOTH, int W> static __device__ __forceinline__ void find(const unsigned short (&k)[16][W], const unsigned short (&q)[16][W], const vec (&S)[KT], vec& w, vec& z, unsigned g, unsigned c)
+    {
+        if constexpr (KT == 1) {
+            const pieces s = split(S[0]);
+            const uint2 a = by_rows(k, 0, g, c), b = by_rows(q, 0, g, c);
+            w = mac16(a, s.hi, mac16(a, s.mid, mac16(a, s.lo, w)));
+            if (BOTH) z = mac16(b, s.hi, mac16(b, s.mid, mac16(b, s.lo, z)));
+        } else {
+#pragma unroll
+            for (int t = 0; t < KT; t += 2) {
+                const pieces s = split(S[t]), r = split(S[t + 1]);
+                const uint2 a = by_rows(k, t, g, c), a2 = by_rows(k, t + 1, g, c);
+                w = mac32(a, a2, s.lo, r.lo, w);
+                w = mac32(a, a2, s.mid, r.mid, w);
+                w = mac32(a, a2, s.hi, r.hi, w);
+                if (BOTH) {
+                    const uint2 b = by_rows(q, t, g, c), b2 = by_rows(q, t + 1, g, c);
+                    z = mac32(b, b2, s.lo, r.lo, z);
+                    z = mac32(b, b2, s.mid, r.mid, z);
+                    z = mac32(b, b2, s.hi, r.hi, z);
+                }
+            }
+        }
+    }
+    template <int W> static __device__ __forceinline__ void add(vec (&S)[KT], const unsigned short (&m)[16][W], vec x, unsigned g, unsigned c)
+    {
+        const pieces s = split(x);
+        uint2 f[KT];
+#pragma unroll
+        for (int t = 0; t < KT; ++t) f[t] = by_columns(m, t, g, c);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) S[t] = mac16(f[t], s.lo, S[t]);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) S[t] = mac16(f[t], s.mid, S[t]);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) S[t] = mac16(f[t], s.hi, S[t]);
+    }
+};
 
 // One value as it lies in memory. Whatever is fetched ahead is read from an address that is there (of the same chunk's first row or column where its own is not) and made zero where it
 // is used: a load behind a branch, or one whose value is converted at once, would be waited for there.
@@ -276,15 +367,39 @@ template <typename T, int KT, int TEAM> struct delta_feed {
                 }
         }
     }
-    __device__ __forceinline__ void put(const delta_shape& p, delta_rows<A, KT>& to, unsigned thread)
+    __device__ __forceinline__ void put_parts(delta_chunk<A>& to, unsigned thread) const
     {
 #pragma unroll
         for (int i = 0; i < SHARE; ++i) {
             const unsigned v = thread + i * 64u * TEAM;
             if (v >= (unsigned)PARTS) break;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) reinterpret_cast<A*>(&to.c)[4 * v + j] = part[i].v[j];
+            for (int j = 0; j < 4; ++j) reinterpret_cast<A*>(&to)[4 * v + j] = part[i].v[j];
         }
+    }
+    __device__ __forceinline__ void put(const delta_shape& p, delta_rows16<KT>& to, unsigned thread)
+    {
+        put_parts(to.c, thread);
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const unsigned v = thread + i * 64u * TEAM, row = v / (4u * KT), col = v % (4u * KT) * 4u;
+            if (VECS < 64 * TEAM && v >= (unsigned)VECS) break;
+            asm volatile("" : "+v"(k[i]), "+v"(q[i]));
+            typedef unsigned short quad __attribute__((ext_vector_type(4)));
+            quad a = __builtin_bit_cast(quad, k[i]), b = __builtin_bit_cast(quad, q[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool there = row < rows && col + j < p.K;
+                a[j] = there ? a[j] : (unsigned short)0;
+                b[j] = there ? b[j] : (unsigned short)0;
+            }
+            *reinterpret_cast<quad*>(&to.k[row][col]) = a;
+            *reinterpret_cast<quad*>(&to.q[row][col]) = b;
+        }
+    }
+    __device__ __forceinline__ void put(const delta_shape& p, delta_rows<A, KT>& to, unsigned thread)
+    {
+        put_parts(to.c, thread);
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const unsigned v = thread + i * 64u * TEAM, row = v / (4u * KT), col = v % (4u * KT) * 4u;

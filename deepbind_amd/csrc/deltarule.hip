@@ -18,7 +18,7 @@ __global__ __launch_bounds__(256) void k_delta_mark(delta_shape p, const uint32_
 // could multiply instead, grow far beyond the inverse where keys come again, and lose it). A wave waits for memory most of its time, first for its block, then for its
 // rows: what it needs is asked for at once, and its share of LDS, which keys' products and queries' use in turn, lets six of them run per SIMD.
 template <typename T, int KT>
-__global__ __launch_bounds__(256) void k_delta_prepare(delta_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, const T* __restrict__ Q,
+__global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)) void k_delta_prepare(delta_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, const T* __restrict__ Q,
                                                        const T* __restrict__ K, const typename acc_of<T>::type* __restrict__ beta,
                                                        const typename acc_of<T>::type* __restrict__ decay, delta_chunk<typename acc_of<T>::type>* __restrict__ chunks,
                                                        delta_pairs<typename acc_of<T>::type>* __restrict__ pairs)
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(256) void k_delta_prepare(delta_shape p, const uint
 // Keys, queries, matrices and values of a chunk come while the one before it is worked on. OUT: rows of O are written; otherwise only the state moves on. V null:
 // without values, for what becomes of the state alone.
 template <typename T, int KT, int TEAM, bool OUT, typename NUMBER>
-__device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, delta_rows<typename acc_of<T>::type, KT>* lds, const T* Q, const T* K,
+__device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, typename delta_ops<T, KT>::rows* lds, const T* Q, const T* K,
                                            const T* V, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, size_t first, size_t row, unsigned rows, NUMBER number,
                                            typename mm16<typename acc_of<T>::type>::vec (&S)[KT], T* O, typename acc_of<T>::type* keep, size_t kept)
 {
@@ -169,7 +169,7 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
     __syncthreads();
     for (unsigned t = 0; t < rows; t += DELTA_CHUNK) {
         const unsigned n = min(rows - t, DELTA_CHUNK);
-        const delta_rows<A, KT>& here = lds[t / DELTA_CHUNK & 1u];
+        const typename delta_ops<T, KT>::rows& here = lds[t / DELTA_CHUNK & 1u];
         vec x = V ? values.get(l) : zero16<A>();
         if (t + DELTA_CHUNK < rows) {
             feed.put(p, lds[~(t / DELTA_CHUNK) & 1u], l.thread);
@@ -179,13 +179,7 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
         if (l.nv) {
             if (keep && (t || row != first) && t % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + (kept + t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
             vec w = zero16<A>(), z = zero16<A>();
-#pragma unroll
-            for (int i = 0; i < KT; ++i) {
-                if (OUT) products<A>(tile_by_rows(here.k, i, l.g, l.c), tile_by_rows(here.q, i, l.g, l.c), S[i], w, z);
-                else if (i & 1) z = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], z);
-                else w = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], w);
-            }
-            if (!OUT) w += z;
+            delta_ops<T, KT>::template find<OUT>(here.k, here.q, S, w, z, l.g, l.c);
             const vec first = by_row(here.c.first, l.g), b = by_row(here.c.b, l.g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) x[r] = l.row(r) < n ? b[r] * (x[r] - first[r] * w[r]) : A(0);
@@ -194,7 +188,7 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
             const A through = here.c.first[15];
 #pragma unroll
             for (int i = 0; i < KT; ++i) S[i] *= through;
-            add_products<A, KT>(S, here.k, sent, l.g, l.c);
+            delta_ops<T, KT>::add(S, here.k, sent, l.g, l.c);
             if (OUT) {
                 const vec y = triangle<A, true>(matrix_by_rows(here.c.P, l.g, l.c), u, first * z, l.g);
 #pragma unroll
@@ -216,7 +210,7 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
-    __shared__ delta_rows<A, KT> lds[4 / TEAM][2];
+    __shared__ typename delta_ops<T, KT>::rows lds[4 / TEAM][2];
     const size_t block = (size_t)p.K * p.H * p.V;
     unsigned r = blockIdx.x, k = 0;
     row_range g;
@@ -249,7 +243,7 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
-    __shared__ delta_rows<A, KT> lds[4 / TEAM][2];
+    __shared__ typename delta_ops<T, KT>::rows lds[4 / TEAM][2];
     const unsigned slot = blockIdx.x;
     unsigned r, k;
     row_range g;

@@ -23,7 +23,7 @@ namespace dbk {
 // dS of a chunk's start from that of its end, chunk after chunk up `rows` rows from the last one down to row `stop` of them. What a chunk needs comes while the one
 // behind it is worked on. dstates: where the gradients in front of the blocks' first rows go, from this piece's first block on; null: nowhere.
 template <typename T, int KT, int TEAM, typename NUMBER>
-__device__ __forceinline__ void delta_walk_back(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, delta_rows<typename acc_of<T>::type, KT>* lds, size_t lddo, const T* Q,
+__device__ __forceinline__ void delta_walk_back(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, typename delta_ops<T, KT>::rows* lds, size_t lddo, const T* Q,
                                                 const T* K, const T* dO, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, size_t row, unsigned rows,
                                                 unsigned stop, NUMBER number, typename mm16<typename acc_of<T>::type>::vec (&S)[KT], typename acc_of<T>::type* dstates)
 {
@@ -43,7 +43,7 @@ __device__ __forceinline__ void delta_walk_back(const delta_shape& p, const delt
     if (end > stop) fetch(end - DELTA_CHUNK);
     __syncthreads();
     for (unsigned left = (end - stop) / DELTA_CHUNK + 1u, t = end; left > 0; --left, t -= DELTA_CHUNK) {
-        const delta_rows<A, KT>& here = lds[t / DELTA_CHUNK & 1u];
+        const typename delta_ops<T, KT>::rows& here = lds[t / DELTA_CHUNK & 1u];
         const vec d = scale * values.get(l);
         if (left > 1u) {
             feed.put(p, lds[~(t / DELTA_CHUNK) & 1u], l.thread);
@@ -52,19 +52,17 @@ __device__ __forceinline__ void delta_walk_back(const delta_shape& p, const delt
         if (left > 2u) fetch(t - 2u * DELTA_CHUNK);
         if (l.nv) {
             vec y = zero16<A>(), z = zero16<A>();
-#pragma unroll
-            for (int i = 0; i < KT; ++i) (i & 1 ? z : y) = product<A>(tile_by_rows(here.k, i, l.g, l.c), S[i], i & 1 ? z : y);
-            y += z;
+            delta_ops<T, KT>::template find<false>(here.k, here.k, S, y, z, l.g, l.c);
             const vec first = by_row(here.c.first, l.g);
             const A through = here.c.first[15];
             const vec du = triangle<A, false>(matrix_by_columns(here.c.P, l.g, l.c), d, by_row(here.c.last, l.g) * y, l.g);
             const vec fd = first * d;
 #pragma unroll
             for (int i = 0; i < KT; ++i) S[i] *= through;
-            add_products<A, KT>(S, here.q, fd, l.g, l.c);
+            delta_ops<T, KT>::add(S, here.q, fd, l.g, l.c);
             const vec dy = triangle<A, false>(matrix_by_columns(here.c.T, l.g, l.c), du, zero16<A>(), l.g);
             const vec dw = -(first * (by_row(here.c.b, l.g) * dy));
-            add_products<A, KT>(S, here.k, dw, l.g, l.c);
+            delta_ops<T, KT>::add(S, here.k, dw, l.g, l.c);
             if (dstates && t % DELTA_BLOCK == 0) store_state<A, KT>(S, dstates + (size_t)(t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
         }
         __syncthreads();
@@ -81,7 +79,7 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
-    __shared__ delta_rows<A, KT> lds[4 / TEAM][2];
+    __shared__ typename delta_ops<T, KT>::rows lds[4 / TEAM][2];
     unsigned r = blockIdx.x, k = 0;
     row_range g;
     if (r < p.nregion) {
@@ -110,7 +108,7 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
-    __shared__ delta_rows<A, KT> lds[4 / TEAM][2];
+    __shared__ typename delta_ops<T, KT>::rows lds[4 / TEAM][2];
     unsigned r, k;
     row_range g;
     if (!slot_segment(regions, p.nregion, p.N, cuts, blockIdx.x, p.L, r, g, k)) return;
