@@ -23,18 +23,6 @@ struct block_shape {
     size_t lddr, lddz, lddy, lddo, lddg;         // backward: dr and dz in, dy, dr and dgate out (ldo: r')
 };
 
-// v of the lane n places further on in its row of 16, round it: no trip through LDS as for lanes further apart
-template <int N> __device__ __forceinline__ float rotated(float v)
-{
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, true));
-}
-template <int N> __device__ __forceinline__ double rotated(double v)
-{
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, 0x120 + N, 0xf, 0xf, true), hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), 0x120 + N, 0xf, 0xf, true);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-
 // sums over LANES lanes of two values at once
 template <int LANES, typename A> __device__ __forceinline__ void block_sum2(A& u, A& v, A (*lds)[16])
 {

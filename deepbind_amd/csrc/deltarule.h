@@ -186,6 +186,16 @@ template <typename F> inline void with_team(size_t K, size_t tiles, F f)
     with_key_tiles(K, pass);
 }
 
+// A team's waves meet; a wave by itself, whose instructions on its share of LDS run in order, only keeps the compiler from changing it.
+template <int TEAM> __device__ __forceinline__ void team_sync()
+{
+    if constexpr (TEAM == 1) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else
+        __syncthreads();
+}
+
 // A team's keys, queries and matrices of one chunk in LDS, rows padded by 16 bytes: lanes read four neighbouring columns of 16 rows, or 16 neighbouring columns of
 // four rows, without meeting in the banks.
 template <typename A, int KT> struct delta_rows {

@@ -68,8 +68,7 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
             }
         }
     }
-    // (a wave's LDS is its own: its instructions there run in order, and only the compiler is kept from changing it)
-    auto sync = []() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); __builtin_amdgcn_wave_barrier(); };
+    auto sync = []() { team_sync<1>(); };        // (a wave's LDS is its own)
     auto put = [&](const vec (&x)[DELTA_CHUNKS]) {
 #pragma unroll
         for (int i = 0; i < (int)DELTA_CHUNKS; ++i)
@@ -166,7 +165,7 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
     if (V) values.fetch(l, v, p.ldv, rows);
     feed.put(p, lds[0], l.thread);
     if (rows > DELTA_CHUNK) fetch(DELTA_CHUNK);
-    __syncthreads();
+    team_sync<TEAM>();
     for (unsigned t = 0; t < rows; t += DELTA_CHUNK) {
         const unsigned n = min(rows - t, DELTA_CHUNK);
         const typename delta_ops<T, KT>::rows& here = lds[t / DELTA_CHUNK & 1u];
@@ -196,7 +195,7 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
                     if (l.row(r) < n && l.c < l.nv) o[(size_t)(t + l.row(r)) * p.ldo] = (T)(scale * y[r]);
             }
         }
-        __syncthreads();
+        team_sync<TEAM>();
     }
 }
 

@@ -41,7 +41,7 @@ __device__ __forceinline__ void delta_walk_back(const delta_shape& p, const delt
     values.fetch(l, d0 + end * lddo, lddo, rows - end);
     feed.put(p, lds[end / DELTA_CHUNK & 1u], l.thread);
     if (end > stop) fetch(end - DELTA_CHUNK);
-    __syncthreads();
+    team_sync<TEAM>();
     for (unsigned left = (end - stop) / DELTA_CHUNK + 1u, t = end; left > 0; --left, t -= DELTA_CHUNK) {
         const typename delta_ops<T, KT>::rows& here = lds[t / DELTA_CHUNK & 1u];
         const vec d = scale * values.get(l);
@@ -65,7 +65,7 @@ __device__ __forceinline__ void delta_walk_back(const delta_shape& p, const delt
             delta_ops<T, KT>::add(S, here.k, dw, l.g, l.c);
             if (dstates && t % DELTA_BLOCK == 0) store_state<A, KT>(S, dstates + (size_t)(t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
         }
-        __syncthreads();
+        team_sync<TEAM>();
     }
 }
 
@@ -125,9 +125,10 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
 // sums over the 16 lanes of a row
 template <typename A> __device__ __forceinline__ A lanes16_sum(A v)
 {
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    v += rotated<8>(v);
+    v += rotated<4>(v);
+    v += rotated<2>(v);
+    return v + rotated<1>(v);
 }
 
 template <typename T> struct delta_grads {
@@ -201,7 +202,7 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
         for (int i = 0; i < (int)DELTA_CHUNKS; ++i) {
             if (i >= (int)nchunk) break;
             const unsigned n = min(bl.rows - 16u * i, 16u);
-            if (i) __syncthreads();
+            if (i) team_sync<TEAM>();
             feed.put(p, lds.rows, l.thread);
             vec x = next.get(l), w = zero16<A>(), y;
             if (i + 1 < (int)nchunk) {
@@ -211,7 +212,7 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
                 if (i) fetch(i - 1u);
                 values(d0, lddo, i);
             }
-            __syncthreads();
+            team_sync<TEAM>();
             const delta_rows<A, KT>& here = lds.rows;
 #pragma unroll
             for (int t = 0; t < KT; ++t) w = product<A>(tile_by_rows(here.k, t, g, c), S[t], w);
@@ -240,10 +241,10 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
         const size_t row = (size_t)bl.at + 16u * i;
         const delta_pairs<A>& pr = pairs[first_chunk + i];
         if (i + 1 < (int)nchunk) {               // (the last chunk's rows are there)
-            __syncthreads();
+            team_sync<TEAM>();
             feed.put(p, lds.rows, l.thread);
             if (i) fetch(i - 1u);
-            __syncthreads();
+            team_sync<TEAM>();
         }
         const delta_rows<A, KT>& here = lds.rows;
         const vec d = scale * next.get(l);
@@ -271,9 +272,8 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
                 lds.d[16u * t + l.row(r)][mine] = dS[t][r];
                 passed = fma(sts[i][t][r], dS[t][r], passed);
             }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) passed += __shfl_xor(passed, o);
-        if ((threadIdx.x & 63u) == 0u) lds.through[slice][0] = through * passed;
+        passed = lanes16_sum(passed);
+        if (c == 0u) lds.through[slice][g] = through * passed;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             lds.o[l.row(r)][mine] = d[r];
@@ -286,7 +286,7 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
 #pragma unroll
             for (int t = 0; t < KT; ++t)
                 dS[t] = product<A>(tile_by_columns(here.q, t, g, c), fd, product<A>(tile_by_columns(here.k, t, g, c), dw, through * dS[t]));
-        __syncthreads();
+        team_sync<TEAM>();
 
         // over the value: this wave's columns of the key
         vec qs[TW], ks[TW], into = zero16<A>(), sent = zero16<A>();
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
                 }
             }
         }
-        __syncthreads();
+        team_sync<TEAM>();
 
         // the team's sums, and what the pairs of rows add
         vec pr_ = zero16<A>(), lr = zero16<A>(), pc = zero16<A>(), lc = zero16<A>();    // dP and dL: [c][row], [row][c]
@@ -387,16 +387,25 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
             db += __shfl_xor(db, 32);
             dg += __shfl_xor(dg, 16);
             dg += __shfl_xor(dg, 32);
+            A in = A(0), on = A(0);
 #pragma unroll
             for (int s = 0; s < TEAM; ++s) {
                 db += lds.b[s][c];
-                dg += lds.through[s][0];
+                dg += (lds.through[s][0] + lds.through[s][1]) + (lds.through[s][2] + lds.through[s][3]);
+                in += lds.into[s][c];
+                on += lds.out[s][c];
             }
-            for (unsigned m = 0; m < 16u; ++m) {
-                const A (*from)[16] = m >= c ? lds.into : lds.out;
-#pragma unroll
-                for (int s = 0; s < TEAM; ++s) dg += from[s][m];
-            }
+            // rows from here on, and rows before
+            in += from_after<1>(in);
+            in += from_after<2>(in);
+            in += from_after<4>(in);
+            in += from_after<8>(in);
+            on = from_before<1>(on);
+            on += from_before<1>(on);
+            on += from_before<2>(on);
+            on += from_before<4>(on);
+            on += from_before<8>(on);
+            dg += in + on;
             if (g == 0u && c < n) {
                 const size_t at = row + c;
                 if (out.db) out.db[((size_t)part * p.N + at) * p.H + l.head] = db;

@@ -114,6 +114,22 @@ __device__ __forceinline__ double rcp_fast(double x) { return 1.0 / x; }
 // 1 / (1 + e^-x)
 template <typename A> __device__ __forceinline__ A sigmoid_of(A x) { return rcp_fast(A(1) + exp_fast(-x)); }
 
+// v of another lane of a row of 16, without a trip through LDS: HOW names the move (zero where no lane is).
+template <int HOW> __device__ __forceinline__ float lane_moved(float v)
+{
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), HOW, 0xf, 0xf, true));
+}
+template <int HOW> __device__ __forceinline__ double lane_moved(double v)
+{
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)b, HOW, 0xf, 0xf, true), hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), HOW, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// round the row; from n lanes further on; from n lanes before
+template <int N, typename A> __device__ __forceinline__ A rotated(A v) { return lane_moved<0x120 + N>(v); }
+template <int N, typename A> __device__ __forceinline__ A from_after(A v) { return lane_moved<0x100 + N>(v); }
+template <int N, typename A> __device__ __forceinline__ A from_before(A v) { return lane_moved<0x110 + N>(v); }
+
 // softplus(x) = max(x, 0) + log(1 + e), e = exp(-|x|) in (0, 1]. log(1 + e) = 2 artanh(z), z = e / (2 + e) <= 1/3, by the series
 // z + z^3/3 + z^5/5 + ...: keeps the relative precision of small steps, which log(1 + e) itself loses (1 + e rounds), in a dozen
 // operations; the first term left out, z^17/17, is at most 2^-29.4 of z. slope: the derivative, 1 / (1 + exp(-x)), from the same e.
