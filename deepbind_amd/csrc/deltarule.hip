@@ -269,13 +269,20 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
 // from the last segment to the first with the transposed transitions. A workgroup takes 16 columns of a head, a wave 16 rows of what comes out; what goes in lies in LDS as
 // it lies in registers, and the next transition's rows come meanwhile.
 template <typename A, int KT>
-__global__ __launch_bounds__(64 * KT) void k_delta_carry(delta_shape p, bool backward, const uint32_t* __restrict__ regions, A* __restrict__ carry, const A* __restrict__ through)
+__global__ __launch_bounds__(64 * KT) void k_delta_carry(delta_shape p, bool backward, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ cuts, A* __restrict__ carry, const A* __restrict__ through)
 {
     typedef typename mm16<A>::vec vec;
     __shared__ A lds[2][KT][4][64];
-    const unsigned r = blockIdx.x, lane = threadIdx.x & 63u, t = uniform(threadIdx.x >> 6), g = lane >> 4, c = lane & 15u;
-    const row_range rows = region_rows(regions, r, p.N);
-    if (rows.end - rows.start <= 2u * p.L) return;               // (two segments: nothing to carry over one)
+    const unsigned lane = threadIdx.x & 63u, t = uniform(threadIdx.x >> 6), g = lane >> 4, c = lane & 15u;
+    // a workgroup per region; of many regions only those that the slots of third segments name (with two segments there is nothing to carry over one). The few workgroups that
+    // have work should stand side by side in the grid where they can: those of two regions 29 slots apart took 77 us for 36.
+    unsigned r = blockIdx.x, third;
+    row_range rows = {0u, 0u};
+    if (p.nregion > p.cuts) {
+        if (!slot_segment(regions, p.nregion, p.N, cuts, blockIdx.x, p.L, r, rows, third) || third != 2u) return;
+    } else
+        rows = region_rows(regions, r, p.N);
+    if (rows.end - rows.start <= 2u * p.L) return;
     const unsigned head = blockIdx.y / p.ns, tile = blockIdx.y % p.ns, n = (rows.end - rows.start + p.L - 1u) / p.L;      // segments: slots first + 1 .. first + n - 1
     const size_t first = rows.start / p.L, HV = (size_t)p.H * p.V, HK = (size_t)p.H * p.K, col = (size_t)head * p.V + 16u * tile + c;
     const bool here = 16u * tile + c < p.V;
@@ -460,7 +467,7 @@ void delta_carry(hipStream_t st, const dbk_deltarule_args& a, const delta_shape&
     auto launch = [&](auto t) {
         typedef decltype(t) A;
         with_key_tiles(a.K, [&](auto kt) {
-            k_delta_carry<A, kt.value><<<dim3(s.nregion, s.H * s.ns), 64 * kt.value, 0, st>>>(s, backward, a.regions, (A*)w.carry, (const A*)w.through);
+            k_delta_carry<A, kt.value><<<dim3(s.nregion > s.cuts ? s.cuts : s.nregion, s.H * s.ns), 64 * kt.value, 0, st>>>(s, backward, a.regions, w.marks, (A*)w.carry, (const A*)w.through);
         });
     };
     if (a.dtype == DBK_F64) launch(double());

@@ -46,9 +46,12 @@ def delta_case(kind, N, H, G, Kd, Vd, decays, pad, seed, level=2.0):
     return t, v
 
 
+# one long region among many short ones, and a few of a handful of segments; a region that ends with a segment, and one row behind
+MIXED = [[i * 9, i * 9 + 3 + i % 6] for i in range(200)] + [[1900, 5000], [5000, 5001], [5001, 6000]] + [[6000 + i * 5, 6004 + i * 5] for i in range(200)]
+TABLES = dict(TABLES, mixed=(MIXED, 7010), segments=([[300, 1068], [1068, 1837], [0, 256], [256, 300]], 1840))
 DELTA = [("one", 1, 1, 16, 16, True, 0), ("ragged", 3, 1, 19, 13, True, 1), ("ragged", 2, 2, 1, 1, False, 0), ("outside", 4, 2, 7, 33, True, 0), ("reads", 4, 4, 16, 16, True, 0),
          ("ragged", 2, 1, 64, 64, True, 3), ("outside", 1, 1, 128, 128, True, 0), ("reads", 2, 1, 33, 50, False, 1), ("long", 2, 2, 16, 16, True, 0), ("long", 1, 1, 40, 65, True, 2),
-         ("none", 2, 2, 8, 8, True, 0)]
+         ("none", 2, 2, 8, 8, True, 0), ("mixed", 1, 1, 16, 16, True, 0), ("mixed", 2, 1, 40, 33, True, 1), ("segments", 2, 2, 64, 64, True, 0), ("segments", 3, 1, 100, 20, True, 0)]
 
 
 @pytest.mark.parametrize("kind", list(TYPES))
