@@ -343,11 +343,12 @@ class Arguments(object):
 
 def check_many(a):
     """Arguments.check for long lists: pairs are compared one by one only where memory of some tensors overlaps at all."""
-    both = sorted([(lo, hi, at) for lo, hi, at, _ in a.ins + a.outs if lo != hi])
-    if both and (both[0][2] < 0 or any(at != both[0][2] for _, _, at in both) or both[0][2] != torch.cuda.current_device()):
+    every = a.ins + a.outs
+    current = every[0][2]
+    if current < 0 or any(t[2] != current for t in every) or current != torch.cuda.current_device():
         return a.check()
     end = 0
-    for lo, hi, _ in both:
+    for lo, hi in sorted([(t[0], t[1]) for t in every if t[0] != t[1]]):
         if lo < end:
             return a.check()
         end = hi

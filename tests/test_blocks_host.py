@@ -241,6 +241,8 @@ def test_clip_refusals():
     _refused("must be contiguous", ds.clip_gradients, [torch.zeros(3, 4, 5).transpose(0, 1)], 1.0)
     _refused("out[0] must be torch.float32", ds.clip_gradients, [X], 1.0, out=[X.double()])
     _refused("expected a device tensor", ds.clip_gradients, [X, X.double()], 1.0)
+    # nor where there is nothing in them: the norms would lie on the host
+    _refused("expected a device tensor", ds.clip_gradients, [torch.zeros(0)], 1.0)
 
 
 def test_library_refusals_of_blocks_reach_no_device():
