@@ -442,7 +442,8 @@ static int check_delta_shape(const dbk_deltarule_args* a)
     DBK_ROW_DTYPE_OK(a->dtype);
     DBK_CHECK(a->H >= 1 && a->G >= 1 && a->H % a->G == 0, "ValueError: the number of heads must be divisible by the number of key heads");
     DBK_CHECK(a->K >= 1 && a->K <= DELTA_KEY, "NotImplementedError: keys of 1 to %zu columns, got %zu", DELTA_KEY, a->K);
-    DBK_CHECK(a->N < (size_t(1) << 31) && a->V < (size_t(1) << 20) && a->H < (size_t(1) << 20) && a->H * ((a->V + 15) / 16) <= 65535, "ValueError: map too large (%zu rows, %zu heads of %zu columns)", a->N, a->H, a->V);
+    DBK_CHECK(a->N < (size_t(1) << 31) && a->V < (size_t(1) << 20) && a->H < (size_t(1) << 20), "ValueError: map too large (%zu rows, %zu heads of %zu columns)", a->N, a->H, a->V);
+    DBK_CHECK(a->H * ((a->V + 15) / 16 + (a->K + 15) / 16) <= 65535, "ValueError: too many heads (%zu of %zu and %zu columns)", a->H, a->K, a->V);
     DBK_CHECK(a->nregion < (size_t(1) << 24), "ValueError: too many regions (%zu)", a->nregion);
     return 0;
 }
@@ -539,7 +540,10 @@ int dbk_deltarule_kept(const dbk_deltarule_args* a, size_t* values)
 {
     if (int rc = check_delta_shape(a)) return rc;
     DBK_CHECK(values, "ValueError: null result");
-    const delta_shape s = delta_shape_of(*a);
+    // (as many segments as any number of regions may be cut into)
+    dbk_deltarule_args any = *a;
+    any.nregion = 0;
+    const delta_shape s = a->V ? delta_shape_of(any) : delta_shape();
     *values = delta_kept(s) + delta_through(s);
     clear_error();
     return 0;

@@ -290,6 +290,19 @@ def test_library_refusals_of_blocks_reach_no_device():
     assert lib.dbk_deltarule(None, at, one, 1 << 60) and "too many regions" in err()
     a.nregion = 1
     assert lib.dbk_deltarule_step(None, at) and "too many sequences" in err()
+    a.H, a.K, a.V = 60000, 128, 16
+    assert lib.dbk_deltarule(None, at, one, 1 << 60) and "too many heads" in err()
+    a.H, a.K, a.V = 4, 5, 6
+    # what is kept goes by the sizes alone, whatever the regions
+    need = ctypes.c_size_t(0)
+    kept = []
+    for a.N, a.nregion in ((100000, 0), (100000, 9), (100000, 5000)):
+        assert lib.dbk_deltarule_kept(at, ctypes.addressof(need)) == 0
+        kept.append(need.value)
+    assert kept[0] == kept[1] == kept[2] >= (100000 + 63) // 64 * 5 * 24
+    a.V = 0
+    assert lib.dbk_deltarule_kept(at, ctypes.addressof(need)) == 0 and need.value == 0
+    a.V, a.nregion = 6, 1
     a.N = 0
     assert lib.dbk_deltarule_step(None, at) == 0 and err() == ""
 
