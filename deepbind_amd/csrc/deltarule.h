@@ -129,12 +129,13 @@ __device__ __forceinline__ bool find_block(const delta_shape& p, const uint32_t*
     b.rows = min(b.g.end - b.at, DELTA_BLOCK);
     return true;
 }
-// the number of block k of region r
-__device__ __forceinline__ size_t block_number(const delta_shape& p, unsigned r, row_range g, unsigned k)
+// A chunk's matrices: a head's lie one after the other, chunks numbered like blocks, a region's first by the region, so that short regions take no more than they have.
+__host__ __device__ __forceinline__ size_t delta_chunks(const delta_shape& p) { return p.nregion + (p.N + DELTA_CHUNK - 1u) / DELTA_CHUNK; }
+__device__ __forceinline__ size_t chunk_number(const delta_shape& p, unsigned r, unsigned start, unsigned chunk, unsigned head)
 {
-    return k ? (size_t)p.nregion + g.start / DELTA_BLOCK + k : r;
+    return head * delta_chunks(p) + (chunk ? (size_t)p.nregion + start / DELTA_CHUNK + chunk : r);
 }
-// its place in `keep`, which holds no region's first block
+// a block's place in `keep`, which holds no region's first block
 __device__ __forceinline__ size_t kept_number(row_range g, unsigned k) { return g.start / DELTA_BLOCK + k; }
 
 // The waves that hold tiles of 16 columns of the same head are a team: 1, 2 or 4 of a workgroup's four (a head of more than 4 tiles has several), which share the head's keys and

@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
         sync();
     };
     // columns of all chunks' matrices through LDS to memory, a matrix of 16 x 16 values at a time, consecutive lanes to consecutive places
-    const size_t number = ((size_t)bl.slot * p.H + head) * DELTA_CHUNKS;
+    auto number = [&](unsigned i) { return chunk_number(p, bl.r, bl.g.start, bl.k * DELTA_CHUNKS + i, head); };
     auto store = [&](auto matrix, const A (&x)[16]) {
         sync();
 #pragma unroll
@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
             row_vec<A, 4> v;
 #pragma unroll
             for (int j = 0; j < 4; ++j) v.v[j] = lds[i][lane >> 2][4u * (lane & 3u) + j];
-            v.store(matrix(number + i) + 4u * lane, 4u);
+            v.store(matrix(number(i)) + 4u * lane, 4u);
         }
         sync();
     };
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
             n[i] = i > (int)c ? D[i] * lds[g][i][c] : A(0);
         }
         if (g < nchunk) {
-            delta_chunk<A>& to = chunks[number + g];
+            delta_chunk<A>& to = chunks[number(g)];
             to.first[c] = mine;
             to.last[c] = D[15];
             to.b[c] = b[16u * g + c];
@@ -143,12 +143,12 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
     store([&](size_t i) { return chunks[i].P; }, s);
 }
 
-// Walks a wave's 16 columns of a head's state down `rows` rows from `row` on, of a region that starts at `first`. number(k): the number of the block k blocks on from the first.
+// Walks a wave's 16 columns of a head's state down `rows` rows from `row` on, of region r, which starts at `first`.
 // Keys, queries, matrices and values of a chunk come while the one before it is worked on. OUT: rows of O are written; otherwise only the state moves on. V null:
 // without values, for what becomes of the state alone.
-template <typename T, int KT, int TEAM, bool OUT, typename NUMBER>
+template <typename T, int KT, int TEAM, bool OUT>
 __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, typename delta_ops<T, KT>::rows* lds, const T* Q, const T* K,
-                                           const T* V, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, size_t first, size_t row, unsigned rows, NUMBER number,
+                                           const T* V, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, unsigned r, unsigned first, size_t row, unsigned rows,
                                            typename mm16<typename acc_of<T>::type>::vec (&S)[KT], T* O, typename acc_of<T>::type* keep, size_t kept)
 {
     typedef typename acc_of<T>::type A;
@@ -157,8 +157,10 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
     const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K, *v = V + row * p.ldv + l.v;
     T* o = O + row * p.ldo + l.v + l.c;
     delta_feed<T, KT, TEAM> feed;
+    const delta_chunk<A>* at = chunks + chunk_number(p, r, first, (unsigned)(row - first) / DELTA_CHUNK, l.head);
     auto fetch = [&](unsigned t) {
-        feed.fetch(p, q + t * p.ldq, k + t * p.ldk, chunks[(number(t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS], l.thread, rows - t);
+        feed.fetch(p, q + t * p.ldq, k + t * p.ldk, *at, l.thread, rows - t);
+        at = t ? at + 1 : chunks + chunk_number(p, r, first, (unsigned)(row - first) / DELTA_CHUNK + 1u, l.head);
     };
     delta_values<T> values;
     fetch(0u);
@@ -179,9 +181,9 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
             if (keep && (t || row != first) && t % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + (kept + t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
             vec w = zero16<A>(), z = zero16<A>();
             delta_ops<T, KT>::template find<OUT>(here.k, here.q, S, w, z, l.g, l.c);
-            const vec first = by_row(here.c.first, l.g), b = by_row(here.c.b, l.g);
+            const vec decayed = by_row(here.c.first, l.g), b = by_row(here.c.b, l.g);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) x[r] = l.row(r) < n ? b[r] * (x[r] - first[r] * w[r]) : A(0);
+            for (int r = 0; r < 4; ++r) x[r] = l.row(r) < n ? b[r] * (x[r] - decayed[r] * w[r]) : A(0);
             const vec u = triangle<A, true>(matrix_by_rows(here.c.T, l.g, l.c), x, zero16<A>(), l.g);
             const vec sent = by_row(here.c.last, l.g) * u;
             const A through = here.c.first[15];
@@ -189,7 +191,7 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
             for (int i = 0; i < KT; ++i) S[i] *= through;
             delta_ops<T, KT>::add(S, here.k, sent, l.g, l.c);
             if (OUT) {
-                const vec y = triangle<A, true>(matrix_by_rows(here.c.P, l.g, l.c), u, first * z, l.g);
+                const vec y = triangle<A, true>(matrix_by_rows(here.c.P, l.g, l.c), u, decayed * z, l.g);
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (l.row(r) < n && l.c < l.nv) o[(size_t)(t + l.row(r)) * p.ldo] = (T)(scale * y[r]);
@@ -228,7 +230,7 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
     vec S[KT];
     load_state<A, KT>(S, from, p, l);
     const unsigned before = k * (p.L / DELTA_BLOCK);
-    delta_walk<T, KT, TEAM, true>(p, l, lds[l.team], Q, K, V, chunks, scale, g.start, start, rows, [&](unsigned i) { return block_number(p, r, g, before + i); }, S, O, keep, kept_number(g, before));
+    delta_walk<T, KT, TEAM, true>(p, l, lds[l.team], Q, K, V, chunks, scale, r, g.start, start, rows, S, O, keep, kept_number(g, before));
     if (last && start + rows == g.end) store_state<A, KT>(S, last + r * block, p, l);
 }
 
@@ -259,9 +261,7 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
             for (int i = 0; i < 4; ++i) S[t][i] = 16u * t + l.row(i) == 16u * l.tile + l.c && l.nv ? A(1) : A(0);
     } else
         load_state<A, KT>(S, state && k == 1u ? state + (size_t)r * p.K * p.H * p.V : (const A*)nullptr, p, l);
-    const unsigned before = (k - 1u) * (p.L / DELTA_BLOCK);
-    delta_walk<T, KT, TEAM, false>(p, l, lds[l.team], Q, K, unit ? (const T*)nullptr : V, chunks, A(1), g.start, g.start + (k - 1u) * p.L, p.L,
-                                   [&](unsigned i) { return block_number(p, r, g, before + i); }, S, (T*)nullptr, (A*)nullptr, 0);
+    delta_walk<T, KT, TEAM, false>(p, l, lds[l.team], Q, K, unit ? (const T*)nullptr : V, chunks, A(1), r, g.start, g.start + (k - 1u) * p.L, p.L, S, (T*)nullptr, (A*)nullptr, 0);
     store_state<A, KT>(S, unit ? through + slot * ((size_t)p.K * p.H * p.K) : carry + slot * ((size_t)p.K * p.H * p.V), p, l);
 }
 
@@ -504,7 +504,7 @@ delta_work work_in(void* work, const dbk_deltarule_args& a, const delta_shape& s
     w.marks = (uint32_t*)p;
     at += align16(s.slots * sizeof(uint32_t));
     w.chunks = p + at;
-    at += delta_blocks(s) * a.H * DELTA_CHUNKS * (a.dtype == DBK_F64 ? sizeof(delta_chunk<double>) : sizeof(delta_chunk<float>));
+    at += delta_chunks(s) * a.H * (a.dtype == DBK_F64 ? sizeof(delta_chunk<double>) : sizeof(delta_chunk<float>));
     const size_t A = acc_size(a.dtype);
     at = align16(at);
     w.cuts.marks = (uint32_t*)(p + at);

@@ -22,10 +22,10 @@ namespace dbk {
 
 // dS of a chunk's start from that of its end, chunk after chunk up `rows` rows from the last one down to row `stop` of them. What a chunk needs comes while the one
 // behind it is worked on. dstates: where the gradients in front of the blocks' first rows go, from this piece's first block on; null: nowhere.
-template <typename T, int KT, int TEAM, typename NUMBER>
+template <typename T, int KT, int TEAM>
 __device__ __forceinline__ void delta_walk_back(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, typename delta_ops<T, KT>::rows* lds, size_t lddo, const T* Q,
-                                                const T* K, const T* dO, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, size_t row, unsigned rows,
-                                                unsigned stop, NUMBER number, typename mm16<typename acc_of<T>::type>::vec (&S)[KT], typename acc_of<T>::type* dstates)
+                                                const T* K, const T* dO, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, unsigned r, unsigned first,
+                                                size_t row, unsigned rows, unsigned stop, typename mm16<typename acc_of<T>::type>::vec (&S)[KT], typename acc_of<T>::type* dstates)
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
@@ -33,7 +33,7 @@ __device__ __forceinline__ void delta_walk_back(const delta_shape& p, const delt
     const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K, *d0 = dO + row * lddo + l.v;
     delta_feed<T, KT, TEAM> feed;
     auto fetch = [&](unsigned t) {
-        feed.fetch(p, q + t * p.ldq, k + t * p.ldk, chunks[(number(t / DELTA_BLOCK) * p.H + l.head) * DELTA_CHUNKS + t / DELTA_CHUNK % DELTA_CHUNKS], l.thread, rows - t);
+        feed.fetch(p, q + t * p.ldq, k + t * p.ldk, chunks[chunk_number(p, r, first, (unsigned)(row - first + t) / DELTA_CHUNK, l.head)], l.thread, rows - t);
     };
     delta_values<T> values;
     const unsigned end = (rows - 1) / DELTA_CHUNK * DELTA_CHUNK;
@@ -53,15 +53,15 @@ __device__ __forceinline__ void delta_walk_back(const delta_shape& p, const delt
         if (l.nv) {
             vec y = zero16<A>(), z = zero16<A>();
             delta_ops<T, KT>::template find<false>(here.k, here.k, S, y, z, l.g, l.c);
-            const vec first = by_row(here.c.first, l.g);
+            const vec decayed = by_row(here.c.first, l.g);
             const A through = here.c.first[15];
             const vec du = triangle<A, false>(matrix_by_columns(here.c.P, l.g, l.c), d, by_row(here.c.last, l.g) * y, l.g);
-            const vec fd = first * d;
+            const vec fd = decayed * d;
 #pragma unroll
             for (int i = 0; i < KT; ++i) S[i] *= through;
             delta_ops<T, KT>::add(S, here.q, fd, l.g, l.c);
             const vec dy = triangle<A, false>(matrix_by_columns(here.c.T, l.g, l.c), du, zero16<A>(), l.g);
-            const vec dw = -(first * (by_row(here.c.b, l.g) * dy));
+            const vec dw = -(decayed * (by_row(here.c.b, l.g) * dy));
             delta_ops<T, KT>::add(S, here.k, dw, l.g, l.c);
             if (dstates && t % DELTA_BLOCK == 0) store_state<A, KT>(S, dstates + (size_t)(t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
         }
@@ -95,8 +95,7 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
     vec S[KT];
     load_state<A, KT>(S, more ? carry + ((size_t)g.start / p.L + k + 1u) * block : (const A*)nullptr, p, l);
     const unsigned before = k * (p.L / DELTA_BLOCK);
-    delta_walk_back<T, KT, TEAM>(p, l, lds[l.team], lddo, Q, K, dO, chunks, scale, start, more ? p.L : g.end - start, k ? 0u : DELTA_BLOCK, [&](unsigned i) { return block_number(p, r, g, before + i); },
-                                 S, dstates + kept_number(g, before) * block);
+    delta_walk_back<T, KT, TEAM>(p, l, lds[l.team], lddo, Q, K, dO, chunks, scale, r, g.start, start, more ? p.L : g.end - start, k ? 0u : DELTA_BLOCK, S, dstates + kept_number(g, before) * block);
 }
 
 // What a slot's segment makes of a gradient of zeros behind it
@@ -114,11 +113,11 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
     if (!slot_segment(regions, p.nregion, p.N, cuts, blockIdx.x, p.L, r, g, k)) return;
     delta_lane<A, TEAM> l;
     l.place(p, blockIdx.y, p.V);
-    const unsigned start = g.start + k * p.L, before = k * (p.L / DELTA_BLOCK);
+    const unsigned start = g.start + k * p.L;
     vec S[KT];
 #pragma unroll
     for (int i = 0; i < KT; ++i) S[i] = zero16<A>();
-    delta_walk_back<T, KT, TEAM>(p, l, lds[l.team], lddo, Q, K, dO, chunks, scale, start, min(g.end - start, p.L), 0u, [&](unsigned i) { return block_number(p, r, g, before + i); }, S, (A*)nullptr);
+    delta_walk_back<T, KT, TEAM>(p, l, lds[l.team], lddo, Q, K, dO, chunks, scale, r, g.start, start, min(g.end - start, p.L), 0u, S, (A*)nullptr);
     store_state<A, KT>(S, carry + blockIdx.x * ((size_t)p.K * p.H * p.V), p, l);
 }
 
@@ -185,9 +184,9 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
     const size_t state = (size_t)p.K * p.H * p.V;
     const T *q0 = Q + (size_t)bl.at * p.ldq + (size_t)l.group * p.K, *k0 = K + (size_t)bl.at * p.ldk + (size_t)l.group * p.K;
     const T *v0 = V + (size_t)bl.at * p.ldv + l.v, *d0 = dO + (size_t)bl.at * lddo + l.v;
-    const size_t first_chunk = ((size_t)bl.slot * p.H + l.head) * DELTA_CHUNKS;
+    auto number = [&](unsigned i) { return chunk_number(p, bl.r, bl.g.start, bl.k * DELTA_CHUNKS + i, l.head); };
     delta_feed<T, KT, TEAM> feed;
-    auto fetch = [&](unsigned i) { feed.fetch(p, q0 + 16u * i * p.ldq, k0 + 16u * i * p.ldk, chunks[first_chunk + i], l.thread, bl.rows - 16u * i); };
+    auto fetch = [&](unsigned i) { feed.fetch(p, q0 + 16u * i * p.ldq, k0 + 16u * i * p.ldk, chunks[number(i)], l.thread, bl.rows - 16u * i); };
     delta_values<T> next;
     auto values = [&](const T* x, size_t ld, unsigned i) { next.fetch(l, x + 16u * i * ld, ld, bl.rows - 16u * i); };
 
@@ -239,7 +238,7 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
         if (i >= (int)nchunk) continue;
         const unsigned n = min(bl.rows - 16u * i, 16u);
         const size_t row = (size_t)bl.at + 16u * i;
-        const delta_pairs<A>& pr = pairs[first_chunk + i];
+        const delta_pairs<A>& pr = pairs[number(i)];
         if (i + 1 < (int)nchunk) {               // (the last chunk's rows are there)
             team_sync<TEAM>();
             feed.put(p, lds.rows, l.thread);
@@ -474,7 +473,7 @@ delta_bprop_work bprop_work_in(void* work, const dbk_deltarule_args& a, const de
     char* base = (char*)work;
     size_t at = 0;
     auto take = [&](size_t n) { char* p = base + at; at += align16(n); return p; };
-    const size_t A = acc_size(a.dtype), units = delta_blocks(s) * a.H * DELTA_CHUNKS;
+    const size_t A = acc_size(a.dtype), units = delta_chunks(s) * a.H;
     w.parts = (s.ns + back_team(a) - 1) / back_team(a);
     w.marks = (uint32_t*)take(s.slots * sizeof(uint32_t));
     w.chunks = take(units * (A == 8 ? sizeof(delta_chunk<double>) : sizeof(delta_chunk<float>)));
