@@ -296,20 +296,27 @@ template <int KT> struct delta_ops<bf16_t, KT> {
             w = mac16(a, s.hi, mac16(a, s.mid, mac16(a, s.lo, w)));
             if (BOTH) z = mac16(b, s.hi, mac16(b, s.mid, mac16(b, s.lo, z)));
         } else {
+            // (without queries three sums, one for each piece: a single one's products would wait for each other)
+            vec low = zero16<float>(), mid = zero16<float>();
 #pragma unroll
             for (int t = 0; t < KT; t += 2) {
                 const pieces s = split(S[t]), r = split(S[t + 1]);
                 const uint2 a = by_rows(k, t, g, c), a2 = by_rows(k, t + 1, g, c);
-                w = mac32(a, a2, s.lo, r.lo, w);
-                w = mac32(a, a2, s.mid, r.mid, w);
-                w = mac32(a, a2, s.hi, r.hi, w);
                 if (BOTH) {
                     const uint2 b = by_rows(q, t, g, c), b2 = by_rows(q, t + 1, g, c);
+                    w = mac32(a, a2, s.lo, r.lo, w);
                     z = mac32(b, b2, s.lo, r.lo, z);
+                    w = mac32(a, a2, s.mid, r.mid, w);
                     z = mac32(b, b2, s.mid, r.mid, z);
+                    w = mac32(a, a2, s.hi, r.hi, w);
                     z = mac32(b, b2, s.hi, r.hi, z);
+                } else {
+                    low = mac32(a, a2, s.lo, r.lo, low);
+                    mid = mac32(a, a2, s.mid, r.mid, mid);
+                    w = mac32(a, a2, s.hi, r.hi, w);
                 }
             }
+            if (!BOTH) w += mid + low;
         }
     }
     template <int W> static __device__ __forceinline__ void add(vec (&S)[KT], const unsigned short (&m)[16][W], vec x, unsigned g, unsigned c)
@@ -347,8 +354,8 @@ template <typename T> struct raw_one {
     }
 };
 
-// Their way there: a thread's vectors come while the chunk before is worked on (fetch), and are put into LDS when it is done (put).
-template <typename T, int KT, int TEAM> struct delta_feed {
+// Their way there: a thread's vectors come while the chunk before is worked on (fetch), and are put into LDS when it is done (put). BOTH: queries too.
+template <typename T, int KT, int TEAM, bool BOTH = true> struct delta_feed {
     typedef typename acc_of<T>::type A;
     static constexpr int EACH = KT >= TEAM ? KT / TEAM : 1, VECS = 64 * KT;      // vectors of 4 values: a thread's, a chunk's
     static constexpr int PARTS = sizeof(delta_chunk<A>) / sizeof(A) / 4, SHARE = (PARTS + 64 * TEAM - 1) / (64 * TEAM);
@@ -364,17 +371,17 @@ template <typename T, int KT, int TEAM> struct delta_feed {
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const unsigned v = thread + i * 64u * TEAM, row = v / (4u * KT), col = v % (4u * KT) * 4u;
-            const T *ki = K + (row < rows ? row : 0u) * p.ldk, *qi = Q + (row < rows ? row : 0u) * p.ldq;
+            const T *ki = K + (row < rows ? row : 0u) * p.ldk, *qi = BOTH ? Q + (row < rows ? row : 0u) * p.ldq : nullptr;
             if (p.K % 4u == 0u) {
                 const unsigned at = col < p.K ? col : 0u;
                 k[i] = *reinterpret_cast<const raw*>(ki + at);
-                q[i] = *reinterpret_cast<const raw*>(qi + at);
+                if (BOTH) q[i] = *reinterpret_cast<const raw*>(qi + at);
             } else
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const unsigned at = col + j < p.K ? col + j : 0u;
                     k[i][j] = ki[at];
-                    q[i][j] = qi[at];
+                    if (BOTH) q[i][j] = qi[at];
                 }
         }
     }
@@ -395,9 +402,10 @@ template <typename T, int KT, int TEAM> struct delta_feed {
         for (int i = 0; i < EACH; ++i) {
             const unsigned v = thread + i * 64u * TEAM, row = v / (4u * KT), col = v % (4u * KT) * 4u;
             if (VECS < 64 * TEAM && v >= (unsigned)VECS) break;
-            asm volatile("" : "+v"(k[i]), "+v"(q[i]));
+            asm volatile("" : "+v"(k[i]));
+            if (BOTH) asm volatile("" : "+v"(q[i]));
             typedef unsigned short quad __attribute__((ext_vector_type(4)));
-            quad a = __builtin_bit_cast(quad, k[i]), b = __builtin_bit_cast(quad, q[i]);
+            quad a = __builtin_bit_cast(quad, k[i]), b = BOTH ? __builtin_bit_cast(quad, q[i]) : a;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const bool there = row < rows && col + j < p.K;
@@ -405,7 +413,7 @@ template <typename T, int KT, int TEAM> struct delta_feed {
                 b[j] = there ? b[j] : (unsigned short)0;
             }
             *reinterpret_cast<quad*>(&to.k[row][col]) = a;
-            *reinterpret_cast<quad*>(&to.q[row][col]) = b;
+            if (BOTH) *reinterpret_cast<quad*>(&to.q[row][col]) = b;
         }
     }
     __device__ __forceinline__ void put(const delta_shape& p, delta_rows<A, KT>& to, unsigned thread)
@@ -415,12 +423,15 @@ template <typename T, int KT, int TEAM> struct delta_feed {
         for (int i = 0; i < EACH; ++i) {
             const unsigned v = thread + i * 64u * TEAM, row = v / (4u * KT), col = v % (4u * KT) * 4u;
             if (VECS < 64 * TEAM && v >= (unsigned)VECS) break;
-            if constexpr (sizeof(T) < 8) asm volatile("" : "+v"(k[i]), "+v"(q[i]));
+            if constexpr (sizeof(T) < 8) {
+                asm volatile("" : "+v"(k[i]));
+                if (BOTH) asm volatile("" : "+v"(q[i]));
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const bool there = row < rows && col + j < p.K;
                 to.k[row][col + j] = there ? (A)k[i][j] : A(0);
-                to.q[row][col + j] = there ? (A)q[i][j] : A(0);
+                if (BOTH) to.q[row][col + j] = there ? (A)q[i][j] : A(0);
             }
         }
     }

@@ -156,7 +156,7 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
     if (!rows) return;
     const T *q = Q + row * p.ldq + (size_t)l.group * p.K, *k = K + row * p.ldk + (size_t)l.group * p.K, *v = V + row * p.ldv + l.v;
     T* o = O + row * p.ldo + l.v + l.c;
-    delta_feed<T, KT, TEAM> feed;
+    delta_feed<T, KT, TEAM, OUT> feed;
     const delta_chunk<A>* at = chunks + chunk_number(p, r, first, (unsigned)(row - first) / DELTA_CHUNK, l.head);
     auto fetch = [&](unsigned t) {
         feed.fetch(p, q + t * p.ldq, k + t * p.ldk, *at, l.thread, rows - t);
