@@ -11,6 +11,8 @@
 //
 // Bound by memory: forward three maps in and two out, backward five in and three out. A thread holds one vector of 16 bytes of a chunk, a chunk belongs to a power of two
 // of neighbouring lanes (of a wave, or a workgroup of up to 1024), and a workgroup walks down the rows with its chunks' weights, and backward their gradients, in registers.
+// 50 021 rows x 64 chunks of 16 floats, rms, no gate: 160 us forward (820 MB, 5.1 TB/s), 250 backward (1230 MB, 4.9) and 8 for the sums; 130 003 rows x 1440 bfloat16 with a gate: 435-480
+// (1870 MB, 3.9-4.3; vector instructions 64 % of the time: two norms, a sigmoid and conversions for ten bytes) and 747 (2996 MB, 4.0; 50 %, three barriers a row).
 #include <type_traits>
 #include "norm_common.h"
 
