@@ -98,15 +98,21 @@ template <typename A, bool LOWER> __device__ __forceinline__ typename mm16<A>::v
     return o;
 }
 
-// What one wave prepares for a chunk of a head, as later kernels read it: matrices column by column, and per row what it decays and corrects by. Rows behind a
-// region's last: T is the identity there, N, P and b are zero, and nothing decays.
+// What one wave prepares for a chunk of a head: T and P, and per row what it decays and corrects by. Rows behind a region's last: T is the identity there, N, P and b are
+// zero, and nothing decays. T is a lower triangle with ones on the diagonal and P one with its own, so that in memory they share a square, and N and D another:
+// [c][row] is P[row][c] from the diagonal on and T[c][row] before it; N[row][c] and D[c][row]. (Matrices of their own are most of what 24 heads of 16 columns read and write.)
 template <typename A> struct delta_chunk {
-    A T[256], P[256];
+    A TP[256];
     A first[16], last[16], b[16], spare[16];
 };
 // and what the backward pass needs beside it
 template <typename A> struct delta_pairs {
-    A N[256], D[256];
+    A ND[256];
+};
+// A chunk's as it lies in LDS, by columns: [c][row]
+template <typename A> struct delta_matrices {
+    A T[256], P[256];
+    A first[16], last[16], b[16], spare[16];
 };
 
 // Blocks are numbered like segments (rows_common.h): a region's first by the region, the others by their slot behind those.
@@ -201,7 +207,7 @@ template <int TEAM> __device__ __forceinline__ void team_sync()
 // four rows, without meeting in the banks.
 template <typename A, int KT> struct delta_rows {
     A k[16][16 * KT + 4], q[16][16 * KT + 4];
-    delta_chunk<A> c;
+    delta_matrices<A> c;
 };
 template <typename A, int W> __device__ __forceinline__ typename mm16<A>::vec tile_by_rows(const A (&m)[16][W], int t, unsigned g, unsigned c)
 {
@@ -257,7 +263,7 @@ template <typename T, int KT> struct delta_ops {
 // lane (g, i) names four columns of row 4 g + i / 4 and receives column i of rows 4 g to 4 g + 3.
 template <int KT> struct delta_rows16 {
     __align__(16) unsigned short k[16][16 * KT + 8], q[16][16 * KT + 8];
-    delta_chunk<float> c;
+    delta_matrices<float> c;
 };
 template <int KT> struct delta_ops<bf16_t, KT> {
     typedef mm16<float>::vec vec;
@@ -385,14 +391,31 @@ template <typename T, int KT, int TEAM, bool BOTH = true> struct delta_feed {
                 }
         }
     }
-    __device__ __forceinline__ void put_parts(delta_chunk<A>& to, unsigned thread) const
+    // what no chunk changes of its matrices in LDS
+    static __device__ __forceinline__ void clear(delta_matrices<A>& to, unsigned thread)
+    {
+        if (thread >= 64u) return;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned c = thread / 4u, row = thread % 4u * 4u + j;
+            if (row <= c) to.T[16u * c + row] = row == c ? A(1) : A(0);
+            if (row < c) to.P[16u * c + row] = A(0);
+        }
+    }
+    __device__ __forceinline__ void put_parts(delta_matrices<A>& to, unsigned thread) const
     {
 #pragma unroll
         for (int i = 0; i < SHARE; ++i) {
-            const unsigned v = thread + i * 64u * TEAM;
+            unsigned v = thread + i * 64u * TEAM;
             if (v >= (unsigned)PARTS) break;
+            if (TEAM > 1) asm volatile("" : "+v"(v));            // (places are found anew: kept, they would not fit beside the states)
+            if (v < 64u) {
+                const unsigned c = v / 4u, row = v % 4u * 4u;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) reinterpret_cast<A*>(&to)[4 * v + j] = part[i].v[j];
+                for (int j = 0; j < 4; ++j) (row + j < c ? to.T + 16u * (row + j) + c : to.P + 16u * c + row + j)[0] = part[i].v[j];
+            } else
+#pragma unroll
+                for (int j = 0; j < 4; ++j) to.first[4u * (v - 64u) + j] = part[i].v[j];
         }
     }
     __device__ __forceinline__ void put(const delta_shape& p, delta_rows16<KT>& to, unsigned thread)
@@ -487,7 +510,7 @@ template <typename T, int KT> struct delta_tiles {
         return v;
     }
 };
-// and of a chunk's own matrices, which lie by columns: [c][row(g, r)] (by rows), [row(g, r)][c] (by columns); vectors [row(g, r)]
+// and of a chunk's own matrices: [c][row(g, r)] (by rows), [row(g, r)][c] (by columns); vectors [row(g, r)]
 template <typename A> __device__ __forceinline__ typename mm16<A>::vec matrix_by_rows(const A* m, unsigned g, unsigned c)
 {
     typename mm16<A>::vec f;

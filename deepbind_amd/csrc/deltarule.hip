@@ -17,7 +17,8 @@ __global__ __launch_bounds__(256) void k_delta_mark(delta_shape p, const uint32_
 // decays between rows and the triangle's inverse, column by column by substitution (powers of the triangle, which the matrix cores
 // could multiply instead, grow far beyond the inverse where keys come again, and lose it). A wave waits for memory most of its time, first for its block, then for its
 // rows: what it needs is asked for at once, and its share of LDS, which keys' products and queries' use in turn, lets six of them run per SIMD. 191 284 rows in 2048 regions, 4 heads of
-// 64 floats: 112 us, of which the bytes (keys and queries in, matrices out, 510 MB) take 99 at a copy's rate; 48 532 rows of 24 heads of 16, where four waves share a row's line: 106 us for 546 MB.
+// 64 floats: 112 us for 460 MB (keys and queries in, matrices out; 90 at a copy's rate); 48 532 rows of 24 heads of 16, where four waves share a row's line: 86 us for 306 MB
+// forward and 390 backward (106 with a square for each triangle).
 template <typename T, int KT>
 __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)) void k_delta_prepare(delta_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, const T* __restrict__ Q,
                                                        const T* __restrict__ K, const typename acc_of<T>::type* __restrict__ beta,
@@ -77,12 +78,16 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
             for (int r = 0; r < 4; ++r) lds[i][mm16<A>::row(g, r)][c] = x[i][r];
         sync();
     };
-    // columns of all chunks' matrices through LDS to memory, a matrix of 16 x 16 values at a time, consecutive lanes to consecutive places
+    // two triangles of every chunk through LDS to memory, as a square of 16 x 16 values, consecutive lanes to consecutive places: what is below lies at [c][row], what is
+    // above at [row][c]
     auto number = [&](unsigned i) { return chunk_number(p, bl.r, bl.g.start, bl.k * DELTA_CHUNKS + i, head); };
-    auto store = [&](auto matrix, const A (&x)[16]) {
+    auto store = [&](auto matrix, const A (&below)[16], const A (&above)[16]) {
         sync();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) lds[g][c][i] = x[i];
+        for (int i = 0; i < 16; ++i) {
+            if (i >= (int)c) lds[g][c][i] = below[i];
+            if (i > (int)c) lds[g][i][c] = above[i];
+        }
         sync();
         for (unsigned i = 0; i < nchunk; ++i) {
             row_vec<A, 4> v;
@@ -118,36 +123,33 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
             to.b[c] = b[16u * g + c];
         }
     }
-    if (pairs) {
-        store([&](size_t i) { return pairs[i].N; }, n);
-        store([&](size_t i) { return pairs[i].D; }, D);
-    }
+    if (pairs) store([&](size_t i) { return pairs[i].ND; }, n, D);
     sync();
 #pragma unroll
     for (int i = 0; i < 16; ++i) lds[g][i][c] = n[i];
     sync();
+    A x[16];
     {
-        A x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             A s[4] = {A(0), A(0), A(0), A(0)};
 #pragma unroll
             for (int m = 0; m < i; ++m) s[m & 3] = fma(lds[g][i][m], x[m], s[m & 3]);
-            x[i] = i < (int)c ? A(0) : fma(-b[16u * g + i], (s[0] + s[1]) + (s[2] + s[3]), i == (int)c ? A(1) : A(0));
+            x[i] = i <= (int)c ? (i == (int)c ? A(1) : A(0)) : -b[16u * g + i] * ((s[0] + s[1]) + (s[2] + s[3]));
         }
-        store([&](size_t i) { return chunks[i].T; }, x);
     }
+    sync();
     put(ss);
     A s[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = i >= (int)c ? D[i] * lds[g][i][c] : A(0);
-    store([&](size_t i) { return chunks[i].P; }, s);
+    store([&](size_t i) { return chunks[i].TP; }, s, x);
 }
 
 // Walks a wave's 16 columns of a head's state down `rows` rows from `row` on, of region r, which starts at `first`.
 // Keys, queries, matrices and values of a chunk come while the one before it is worked on. OUT: rows of O are written; otherwise only the state moves on. V null:
 // without values, for what becomes of the state alone. Bound by issue and by one chunk's chain, which waves of other heads and regions fill: 191 284 rows, 4 heads of 64 x 64 floats 314 us
-// (906 MB at 2.9 TB/s, 23 GFLOP: matrix units busy for 46 % of the time, vector instructions 27 %); 41 816 bfloat16 rows, 8 heads of 128 x 128 in 32 segments 275 us (25 % and 49 %, most of
+// (850 MB at 2.7 TB/s, 23 GFLOP: matrix units busy for 46 % of the time, vector instructions 27 %); 41 816 bfloat16 rows, 8 heads of 128 x 128 in 32 segments 275 us (25 % and 49 %, most of
 // which takes the states apart into pieces). Four waves on the same head's keys share what is fetched: alone, each would read all of it.
 template <typename T, int KT, int TEAM, bool OUT>
 __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, typename delta_ops<T, KT>::rows* lds, const T* Q, const T* K,
@@ -168,6 +170,8 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
     delta_values<T> values;
     fetch(0u);
     if (V) values.fetch(l, v, p.ldv, rows);
+    feed.clear(lds[0].c, l.thread);
+    feed.clear(lds[1].c, l.thread);
     feed.put(p, lds[0], l.thread);
     if (rows > DELTA_CHUNK) fetch(DELTA_CHUNK);
     team_sync<TEAM>();

@@ -16,7 +16,7 @@
 // Two kernels: a wave walks 16 columns of a head's dS up its region and leaves it behind every block of 64 rows; then all blocks are independent,
 // each from the state that the forward pass kept before it and the gradient behind it. What is summed over a value's columns (dQ, dK, dP, dL) passes through LDS
 // between the waves of a head, and through memory between the parts of 64 columns of wide values and between heads that share a key: added in a fixed order.
-// 48 532 rows in 512 regions, 24 heads of 16 x 16 floats: 46 us up the regions, 306 for the blocks; 16 028 bfloat16 rows in two, 16 heads of 64 x 64 on 4 keys: 81 us (75 more for the
+// 48 532 rows in 512 regions, 24 heads of 16 x 16 floats: 33 us up the regions, 275 for the blocks; 16 028 bfloat16 rows in two, 16 heads of 64 x 64 on 4 keys: 81 us (75 more for the
 // segments from zeros and 36 for the carry), 372 for the blocks and 30 to add heads that share.
 #include "deltarule.h"
 
@@ -41,6 +41,8 @@ __device__ __forceinline__ void delta_walk_back(const delta_shape& p, const delt
     const unsigned end = (rows - 1) / DELTA_CHUNK * DELTA_CHUNK;
     fetch(end);
     values.fetch(l, d0 + end * lddo, lddo, rows - end);
+    feed.clear(lds[0].c, l.thread);
+    feed.clear(lds[1].c, l.thread);
     feed.put(p, lds[end / DELTA_CHUNK & 1u], l.thread);
     if (end > stop) fetch(end - DELTA_CHUNK);
     team_sync<TEAM>();
@@ -164,7 +166,7 @@ template <typename A, int R, int W> __device__ __forceinline__ typename mm16<A>:
 // The gradients of one block of 64 rows, from the state in front of it and the gradient of the state behind it: forward again over its chunks, whose states stay in registers, and
 // back. Two kinds of work alternate: what runs over a head's keys (a wave's 16 columns of the value, the states in registers) and what runs over its value (16 columns of the
 // key for a wave, the states in LDS), so that neither dQ and dK nor the states are ever added up or turned over between waves. Bound by what lies between: barriers, LDS and waits for
-// both; the matrix units are busy for 22 % (heads of 16) and 33 % (of 64) of the time, vector instructions for 32 % and 31 %.
+// both; the matrix units are busy for 24 % (heads of 16) and 33 % (of 64) of the time, vector instructions for 35 % and 31 %.
 template <typename A, int KT, int TEAM> constexpr int back_waves() { return sizeof(A) == 8 ? (KT == 1 && TEAM > 1 ? 2 : 1) : KT == 1 ? 3 : KT == 2 && TEAM == 1 ? 1 : KT <= 4 ? 2 : 1; }
 
 template <typename T, int KT, int TEAM, int WAVES>
@@ -196,6 +198,7 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
     vec xs[DELTA_CHUNKS], us[DELTA_CHUNKS], sts[DELTA_CHUNKS][KT], dS[KT];
     fetch(0u);
     values(v0, p.ldv, 0u);
+    feed.clear(lds.rows.c, l.thread);
     {
         vec S[KT];
         load_state<A, KT>(S, bl.k ? keep + kept_number(bl.g, bl.k) * state : (const A*)nullptr, p, l);
@@ -253,7 +256,7 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
         vec y = zero16<A>();
         if (i) values(d0, lddo, i - 1u);
         // (fetched here, used behind the next barriers)
-        const vec Dr = matrix_by_rows(pr.D, g, c), Dc = matrix_by_columns(pr.D, g, c), Nr = matrix_by_rows(pr.N, g, c);
+        const vec Dr = matrix_by_columns(pr.ND, g, c), NDc = matrix_by_rows(pr.ND, g, c);            // D[c][row] (row < c); N[c][row] (row < c) and D[row][c] (row > c)
 #pragma unroll
         for (int t = 0; t < KT; ++t) y = product<A>(tile_by_rows(here.k, t, g, c), dS[t], y);
         const vec first = by_row(here.c.first, g), b = by_row(here.c.b, g);
@@ -344,9 +347,9 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const unsigned j = l.row(r);
-            ar[r] = j <= c ? pr_[r] * Dr[r] : A(0);
-            ac[r] = c <= j ? pc[r] * Dc[r] : A(0);
-            ms[r] = j < c ? b_c * lr[r] * Dr[r] : c < j ? b[r] * lc[r] * Dc[r] : A(0);
+            ar[r] = j < c ? pr_[r] * Dr[r] : j == c ? pr_[r] : A(0);
+            ac[r] = c < j ? pc[r] * NDc[r] : j == c ? pc[r] : A(0);
+            ms[r] = j < c ? b_c * lr[r] * Dr[r] : c < j ? b[r] * lc[r] * NDc[r] : A(0);
         }
         const unsigned share = (l.head % (p.H / p.G)) * out.parts + part;
 #pragma unroll
@@ -377,7 +380,7 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const unsigned j = l.row(r);
-                const A ln = j < c ? lr[r] * Nr[r] : A(0);
+                const A ln = j < c ? lr[r] * NDc[r] : A(0);
                 e[r] = j < c ? fma(b_c, ln, pr_[r] * Pr[r]) : A(0);      // (the diagonal has no decay between its rows)
                 before[r] = j < c ? A(1) : A(0);
                 db += ln;
