@@ -10,9 +10,9 @@
 //   dgamma = sum dp h1,  dbeta = sum dp,  dscale = sum t p g sigmoid(g),  dnext_gamma = sum dz h2,  dnext_beta = sum dz
 //
 // Bound by memory: forward three maps in and two out, backward five in and three out. A thread holds one vector of 16 bytes of a chunk, a chunk belongs to a power of two
-// of neighbouring lanes (of a wave, or a workgroup of up to 1024), and a workgroup walks down the rows with its chunks' weights, and backward their gradients, in registers.
-// 50 021 rows x 64 chunks of 16 floats, rms, no gate: 160 us forward (820 MB, 5.1 TB/s), 250 backward (1230 MB, 4.9) and 8 for the sums; 130 003 rows x 1440 bfloat16 with a gate: 435-480
-// (1870 MB, 3.9-4.3; vector instructions 64 % of the time: two norms, a sigmoid and conversions for ten bytes) and 747 (2996 MB, 4.0; 50 %, three barriers a row).
+// of a wave's lanes, or to a workgroup of two to sixteen waves, and a workgroup walks down the rows with its chunks' weights, and backward their gradients, in registers.
+// 50 021 rows x 64 chunks of 16 floats, rms, no gate: 160 us forward (820 MB, 5.1 TB/s), 250 backward (1230 MB, 4.9) and 8 for the sums; 130 003 rows x 1440 bfloat16 with a gate: 424
+// (1870 MB, 4.4 TB/s; vector instructions over half of the time: two norms, a sigmoid and conversions for ten bytes) and 620 (2996 MB, 4.8; three barriers a row).
 #include <type_traits>
 #include "norm_common.h"
 
@@ -83,9 +83,9 @@ template <int LANES, typename A, int V> __device__ __forceinline__ void chunk_st
     norm_stats(near, a * inv, b * inv, eps, mean, rstd);
 }
 
-template <int LANES> constexpr int block_threads() { return LANES > 256 ? LANES : 256; }
+template <int LANES> constexpr int block_threads() { return LANES > 64 ? LANES : 256; }
 
-// Where a thread's vector lies: LANES lanes of a chunk; up to 256 lanes several chunks or rows share a workgroup.
+// Where a thread's vector lies: LANES lanes of a chunk; up to 64 lanes several chunks or rows share a workgroup.
 template <int LANES, int V> struct block_place {
     unsigned chunk, lane, valid, first, row;     // first: of the workgroup's rows
     size_t column;
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(block_threads<LANES>()) void k_block_bprop(block_sh
     typedef typename acc_of<T>::type A;
     constexpr int V = row_vec<T>::N;
     __shared__ A lds[2][16];
-    __shared__ A strips[LANES < 256 ? 256 : 1][V + 1];
+    __shared__ A strips[LANES <= 64 ? 256 : 1][V + 1];
     const block_place<LANES, V> at(p);
     A g1[V], b1[V], sc[V], g2[V], sums[5][V];
     load_weights(g1, gamma ? gamma + at.column : nullptr, at.valid, A(1));
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(block_threads<LANES>()) void k_block_bprop(block_sh
     const unsigned across = LANES << p.ct_log2;                 // threads of one row lane
 #pragma unroll
     for (int i = 0; i < 5; ++i) {
-        if constexpr (LANES < 256) {
+        if constexpr (LANES <= 64) {
             __syncthreads();
 #pragma unroll
             for (int j = 0; j < V; ++j) strips[threadIdx.x][j] = sums[i][j];
@@ -306,7 +306,7 @@ __global__ __launch_bounds__(block_threads<LANES>()) void k_block_bprop(block_sh
         if (threadIdx.x >= across || !at.valid) continue;
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            if (j < (int)at.valid) part[((size_t)blockIdx.x * 5u + i) * m + at.column + j] = LANES < 256 ? strips[LANES < 256 ? threadIdx.x : 0][j] : sums[i][j];
+            if (j < (int)at.valid) part[((size_t)blockIdx.x * 5u + i) * m + at.column + j] = LANES <= 64 ? strips[LANES <= 64 ? threadIdx.x : 0][j] : sums[i][j];
     }
 }
 
@@ -449,21 +449,30 @@ struct block_plan {
     block_shape shape;
 };
 
-// Waves that walk the rows. Forward several rounds of them even out (bfloat16 435 us with 8192, 483 with the 4096 that run at once); backward, where each workgroup's partial sums are
-// added up afterwards, no more than run at once: three per SIMD with four floats a lane, two with eight bfloat16 values, three with two doubles.
-inline unsigned block_waves_of(int dtype, bool backward) { return !backward ? 8192u : dtype == DBK_BF16 ? 2048u : 3072u; }
+// Workgroups that walk the rows. Forward several rounds of waves even out (bfloat16 435 us with 8192, 483 with the 4096 that run at once); backward, where each workgroup's partial sums are
+// added up afterwards, no more than run at once: three waves per SIMD with four floats a lane, two with eight bfloat16 values, three with two doubles.
+inline unsigned block_wgs(int dtype, bool backward, unsigned waves)
+{
+    if (!backward) return 8192u / waves;
+    const unsigned fit = (dtype == DBK_BF16 ? 8u : 12u) / waves;
+    return 256u * (fit ? fit : 1u);
+}
 constexpr size_t WIDE_WGS = 512;
 
 block_plan plan_block(const dbk_blocknorm_args& a, bool backward)
 {
     block_plan p = {};
     const size_t V = 16 / row_size(a.dtype), vecs = (a.group + V - 1) / V, nchunk = a.m / a.group;
-    if (vecs <= 1024) { p.lanes = 1; while ((size_t)p.lanes < vecs) p.lanes *= 2; if (p.lanes == 128) p.lanes = 256; }
-    const unsigned threads = p.lanes > 256 ? p.lanes : 256u;
-    const unsigned ct = p.lanes && p.lanes <= 256 ? chunks_side_by_side((unsigned)p.lanes, nchunk) : 0u;
+    // Six waves only backward (60 003 x 1400 floats 581 -> 555 us, x 700 doubles 828 -> 632; forward 351 -> 395, as fewer waves fit a CU), twelve both ways (40 003 x 2500 floats 434 -> 405 and
+    // 639 -> 598); three gain nothing (100 003 x 700 floats 311 -> 320 and 450 -> 475). More than eight waves of bfloat16 rows backward lack registers: 50 003 x 5600 takes 3640 us with
+    // twelve, 6870 with sixteen, 7220 without them at all.
+    for (int lanes : {1, 2, 4, 8, 16, 32, 64, 128, 256, 384, 512, 768, 1024})
+        if (!p.lanes && vecs <= (size_t)lanes && (backward || lanes != 384)) p.lanes = lanes;
+    const unsigned threads = p.lanes > 64 ? p.lanes : 256u;
+    const unsigned ct = p.lanes && p.lanes <= 64 ? chunks_side_by_side((unsigned)p.lanes, nchunk) : 0u;
     const unsigned rt = p.lanes ? (threads / p.lanes) >> ct : 1u;
     p.gy = p.lanes ? divup(nchunk, size_t(1) << ct) : 1u;
-    const unsigned wgs = block_waves_of(a.dtype, backward) / (threads / 64u), most = wgs / p.gy ? wgs / p.gy : 1u;
+    const unsigned wgs = block_wgs(a.dtype, backward, threads / 64u), most = wgs / p.gy ? wgs / p.gy : 1u;
     p.gx = divup(a.n, rt);
     if (p.gx > most) p.gx = most;
     if (!p.lanes) p.gx = (unsigned)(a.n < WIDE_WGS ? a.n : WIDE_WGS);
@@ -481,16 +490,17 @@ block_plan plan_block(const dbk_blocknorm_args& a, bool backward)
     return p;
 }
 
-template <typename F> bool block_layout(int lanes, bool exact, F f)
+template <bool BACK, typename F> bool block_layout(int lanes, bool exact, F f)
 {
 #define DBK_BLOCK_CASE(L)                                                        \
-    if (lanes == L) {                                                            \
-        if (exact) f(std::integral_constant<int, L>(), std::true_type());        \
-        else f(std::integral_constant<int, L>(), std::false_type());             \
-        return true;                                                             \
-    }
+    if constexpr (BACK || L != 384)                                                   \
+        if (lanes == L) {                                                        \
+            if (exact) f(std::integral_constant<int, L>(), std::true_type());    \
+            else f(std::integral_constant<int, L>(), std::false_type());         \
+            return true;                                                         \
+        }
     DBK_BLOCK_CASE(1) DBK_BLOCK_CASE(2) DBK_BLOCK_CASE(4) DBK_BLOCK_CASE(8) DBK_BLOCK_CASE(16) DBK_BLOCK_CASE(32) DBK_BLOCK_CASE(64)
-    DBK_BLOCK_CASE(256) DBK_BLOCK_CASE(512) DBK_BLOCK_CASE(1024)
+    DBK_BLOCK_CASE(128) DBK_BLOCK_CASE(256) DBK_BLOCK_CASE(384) DBK_BLOCK_CASE(512) DBK_BLOCK_CASE(768) DBK_BLOCK_CASE(1024)
 #undef DBK_BLOCK_CASE
     return false;
 }
@@ -534,7 +544,7 @@ int dbk_blocknorm(dbk_stream_t stream, const dbk_blocknorm_args* a)
     with_row_type(a->dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
-        if (!block_layout(p.lanes, a->group % row_vec<T>::N == 0, [&](auto lanes, auto exact) {
+        if (!block_layout<false>(p.lanes, a->group % row_vec<T>::N == 0, [&](auto lanes, auto exact) {
                 k_block_fprop<T, lanes.value, exact.value><<<dim3(p.gx, p.gy), block_threads<lanes.value>(), 0, st>>>(
                     p.shape, (const T*)a->Y, (const T*)a->R, (const T*)a->gate, (const A*)a->gamma, (const A*)a->beta, (const A*)a->scale, (const A*)a->next_gamma,
                     (const A*)a->next_beta, (A)a->eps, (T*)a->O, (T*)a->Z, (A*)a->stats);
@@ -574,7 +584,7 @@ int dbk_blocknorm_bprop(dbk_stream_t stream, const dbk_blocknorm_args* a, void* 
             typedef decltype(t) T;
             typedef typename acc_of<T>::type A;
             A* part = weights ? (A*)work : nullptr;
-            if (!block_layout(p.lanes, a->group % row_vec<T>::N == 0, [&](auto lanes, auto exact) {
+            if (!block_layout<true>(p.lanes, a->group % row_vec<T>::N == 0, [&](auto lanes, auto exact) {
                     auto kernel = a->rms ? k_block_bprop<T, lanes.value, exact.value, true> : k_block_bprop<T, lanes.value, exact.value, false>;
                     kernel<<<dim3(p.gx, p.gy), block_threads<lanes.value>(), 0, st>>>(
                         p.shape, (const T*)a->Y, (const T*)a->O, (const T*)a->gate, (const A*)a->gamma, (const A*)a->beta, (const A*)a->scale, (const A*)a->next_gamma,

@@ -296,6 +296,13 @@ def test_block_norms_and_their_gradients(kind, rms, n, nchunk, w, pad):
             assert all(a is None or torch.equal(a, b) for a, b in zip(without, zeros))
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("n,nchunk,w,pad", [(3300, 1, 300, 0), (1100, 1, 700, 1), (900, 1, 1300, 0), (530, 2, 1440, 0), (600, 1, 2500, 3), (300, 1, 4000, 0), (270, 1, 6001, 0)])
+def test_block_norms_of_chunks_of_two_to_sixteen_waves(kind, n, nchunk, w, pad):
+    # (more rows than workgroups, so that each walks several)
+    test_block_norms_and_their_gradients(kind, bool(n % 4), n, nchunk, w, pad)
+
+
 def test_block_norms_of_no_rows_and_of_bad_rows():
     from deepbind_amd import smat as sm
     X, g = torch.zeros(0, 12, device="cuda"), torch.ones(1, 12, device="cuda")
