@@ -364,16 +364,20 @@ template <typename T> struct raw_one {
 template <typename T, int KT, int TEAM, bool BOTH = true> struct delta_feed {
     typedef typename acc_of<T>::type A;
     static constexpr int EACH = KT >= TEAM ? KT / TEAM : 1, VECS = 64 * KT;      // vectors of 4 values: a thread's, a chunk's
-    static constexpr int PARTS = sizeof(delta_chunk<A>) / sizeof(A) / 4, SHARE = (PARTS + 64 * TEAM - 1) / (64 * TEAM);
+    static constexpr int W = 4 / TEAM;                                           // a thread's values of the matrices' square, and of the vectors as long as there are any
     typedef typename row_vec<T, 4>::raw raw;
     raw k[EACH], q[EACH];
-    row_vec<A, 4> part[SHARE];
+    A square[W], vectors[W];
     unsigned rows;
     __device__ __forceinline__ void fetch(const delta_shape& p, const T* Q, const T* K, const delta_chunk<A>& c, unsigned thread, unsigned rows_)
     {
         rows = rows_;
+        const A *s = c.TP + W * thread, *v = c.first + min(W * thread, 64u - W);
 #pragma unroll
-        for (int i = 0; i < SHARE; ++i) part[i].load(reinterpret_cast<const A*>(&c) + 4u * min(thread + i * 64u * TEAM, (unsigned)PARTS - 1u), 4u);
+        for (int j = 0; j < W; ++j) {
+            square[j] = s[j];
+            vectors[j] = v[j];
+        }
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             const unsigned v = thread + i * 64u * TEAM, row = v / (4u * KT), col = v % (4u * KT) * 4u;
@@ -405,18 +409,13 @@ template <typename T, int KT, int TEAM, bool BOTH = true> struct delta_feed {
     __device__ __forceinline__ void put_parts(delta_matrices<A>& to, unsigned thread) const
     {
 #pragma unroll
-        for (int i = 0; i < SHARE; ++i) {
-            unsigned v = thread + i * 64u * TEAM;
-            if (v >= (unsigned)PARTS) break;
-            if (TEAM > 1) asm volatile("" : "+v"(v));            // (places are found anew: kept, they would not fit beside the states)
-            if (v < 64u) {
-                const unsigned c = v / 4u, row = v % 4u * 4u;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) (row + j < c ? to.T + 16u * (row + j) + c : to.P + 16u * c + row + j)[0] = part[i].v[j];
-            } else
-#pragma unroll
-                for (int j = 0; j < 4; ++j) to.first[4u * (v - 64u) + j] = part[i].v[j];
+        for (int j = 0; j < W; ++j) {
+            const unsigned c = (W * thread + j) / 16u, row = (W * thread + j) % 16u;
+            (row < c ? to.T + 16u * row + c : to.P + 16u * c + row)[0] = square[j];
         }
+        if (W * thread >= 64u) return;
+#pragma unroll
+        for (int j = 0; j < W; ++j) to.first[W * thread + j] = vectors[j];
     }
     __device__ __forceinline__ void put(const delta_shape& p, delta_rows16<KT>& to, unsigned thread)
     {
