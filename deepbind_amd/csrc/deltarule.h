@@ -554,6 +554,32 @@ template <typename A, int KT, int TEAM> __device__ __forceinline__ void store_st
         }
 }
 
+// Columns of a state as c 2^e with c of size one, so that what becomes of them over many rows neither overflows nor vanishes: e takes what is taken out of S. Powers of two change no digit.
+// Columns of zeros and with an infinity stay as they are; a NaN is no size and stays.
+__device__ __forceinline__ float scaled(float x, int e) { return ldexpf(x, e); }
+__device__ __forceinline__ double scaled(double x, int e) { return ldexp(x, e); }
+template <typename A, int KT> __device__ __forceinline__ A largest(const typename mm16<A>::vec (&S)[KT])
+{
+    A m = A(0);
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m = fmax(m, fabs(S[t][r]));
+    return m;
+}
+template <typename A, int KT> __device__ __forceinline__ void level(typename mm16<A>::vec (&S)[KT], int& e)
+{
+    A m = largest<A, KT>(S);
+    m = fmax(m, __shfl_xor(m, 16));
+    m = fmax(m, __shfl_xor(m, 32));
+    const int x = m > A(0) && m * A(0) == A(0) ? ilogb(m) : 0;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[t][r] = scaled(S[t][r], -x);
+    e += x;
+}
+
 // Defined in deltarule.hip.
 delta_shape delta_shape_of(const dbk_deltarule_args& a);
 int check_delta(const dbk_deltarule_args* a);
@@ -561,7 +587,9 @@ int delta_mark(hipStream_t st, const delta_shape& s, const uint32_t* regions, ui
 // chunks, and pairs where it is not null, of every block and head
 void delta_prepare(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const uint32_t* marks, void* chunks, void* pairs);
 // What regions cut into segments need, in the workspace: whose segment a slot holds, and in front of every segment but a region's first the state (or its gradient) there.
-// Transitions (H, K, K), by which a segment takes what is in front of it to its end, lie behind the kept states, or in the workspace where none are kept.
+// Transitions, by which a segment takes what is in front of it to its end, lie behind the kept states, or in the workspace where none are kept: (H, K, K) values for a segment, and behind those
+// of all segments (H, K) exponents, kept as values are, of the powers of two by which the transitions' columns are larger (level): a segment may grow or shrink a state beyond the type's
+// range, where what is in front of it is small or nothing, or the segment behind does the opposite.
 struct delta_cuts {
     uint32_t* marks;
     char* carry;
@@ -570,7 +598,7 @@ struct delta_cuts {
 void delta_carry(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const delta_cuts& w, bool backward);
 // values (not bytes) of the kept states, behind which the transitions lie
 inline size_t delta_kept(const delta_shape& s) { return (size_t)s.slots * s.K * s.H * s.V; }
-inline size_t delta_through(const delta_shape& s) { return (size_t)s.cuts * s.H * s.K * s.K; }
+inline size_t delta_through(const delta_shape& s) { return (size_t)s.cuts * s.H * s.K * (s.K + 1); }
 inline size_t delta_blocks(const delta_shape& s) { return (size_t)s.nregion + s.slots; }
 inline size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 

@@ -148,13 +148,14 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
 
 // Walks a wave's 16 columns of a head's state down `rows` rows from `row` on, of region r, which starts at `first`.
 // Keys, queries, matrices and values of a chunk come while the one before it is worked on. OUT: rows of O are written; otherwise only the state moves on. V null:
-// without values, for what becomes of the state alone. Bound by issue and by one chunk's chain, which waves of other heads and regions fill: 191 284 rows, 4 heads of 64 x 64 floats 314 us
+// without values, for what becomes of the state alone, whose columns are then kept near one (level, exponents in e). Bound by issue and by one chunk's chain, which waves of other heads and regions fill: 191 284 rows, 4 heads of 64 x 64 floats 314 us
 // (850 MB at 2.7 TB/s, 23 GFLOP: matrix units busy for 46 % of the time, vector instructions 27 %); 41 816 bfloat16 rows, 8 heads of 128 x 128 in 32 segments 275 us (25 % and 49 %, most of
 // which takes the states apart into pieces). Four waves on the same head's keys share what is fetched: alone, each would read all of it.
+constexpr double LEVEL_MOST = 1099511627776.0;    // 2^40
 template <typename T, int KT, int TEAM, bool OUT>
 __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, typename delta_ops<T, KT>::rows* lds, const T* Q, const T* K,
                                            const T* V, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, unsigned r, unsigned first, size_t row, unsigned rows,
-                                           typename mm16<typename acc_of<T>::type>::vec (&S)[KT], T* O, typename acc_of<T>::type* keep, size_t kept)
+                                           typename mm16<typename acc_of<T>::type>::vec (&S)[KT], T* O, typename acc_of<T>::type* keep, size_t kept, int& e)
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
@@ -185,6 +186,8 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
         }
         if (t + 2u * DELTA_CHUNK < rows) fetch(t + 2u * DELTA_CHUNK);
         if (l.nv) {
+            if constexpr (!OUT)                  // (what has grown before every chunk, what has shrunk before every block)
+                if (!V && (t % DELTA_BLOCK == 0 || __any(largest<A, KT>(S) > LEVEL_MOST))) level<A, KT>(S, e);
             if (keep && (t || row != first) && t % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + (kept + t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
             vec w = zero16<A>(), z = zero16<A>();
             delta_ops<T, KT>::template find<OUT>(here.k, here.q, S, w, z, l.g, l.c);
@@ -237,12 +240,13 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
     vec S[KT];
     load_state<A, KT>(S, from, p, l);
     const unsigned before = k * (p.L / DELTA_BLOCK);
-    delta_walk<T, KT, TEAM, true>(p, l, lds[l.team], Q, K, V, chunks, scale, r, g.start, start, rows, S, O, keep, kept_number(g, before));
+    int e = 0;
+    delta_walk<T, KT, TEAM, true>(p, l, lds[l.team], Q, K, V, chunks, scale, r, g.start, start, rows, S, O, keep, kept_number(g, before), e);
     if (last && start + rows == g.end) store_state<A, KT>(S, last + r * block, p, l);
 }
 
 // What the segment in front of a slot's hands on: its state, from the region's own initial one (the first) or from zeros, and (the others) how it takes the
-// state in front of it to its end: the states that the unit vectors become. Workgroups from `values` on along y take those. Keys of 128 columns beside values of 128: twice the
+// state in front of it to its end: the states that the unit vectors become, times powers of two. Workgroups from `values` on along y take those. Keys of 128 columns beside values of 128: twice the
 // forward pass's columns without its outputs, 350 us where that takes 275 (vector instructions 54 % of the time; four waves per SIMD instead of two, for which registers spill, gain nothing).
 template <typename T, int KT, int TEAM>
 __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEAM>())) void k_delta_local(delta_shape p, unsigned values, const uint32_t* __restrict__ regions,
@@ -262,6 +266,7 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
     delta_lane<A, TEAM> l;
     l.place(p, unit ? blockIdx.y - values : blockIdx.y, unit ? p.K : p.V);
     vec S[KT];
+    int e = 0;
     if (unit) {
 #pragma unroll
         for (int t = 0; t < KT; ++t)
@@ -269,7 +274,11 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
             for (int i = 0; i < 4; ++i) S[t][i] = 16u * t + l.row(i) == 16u * l.tile + l.c && l.nv ? A(1) : A(0);
     } else
         load_state<A, KT>(S, state && k == 1u ? state + (size_t)r * p.K * p.H * p.V : (const A*)nullptr, p, l);
-    delta_walk<T, KT, TEAM, false>(p, l, lds[l.team], Q, K, unit ? (const T*)nullptr : V, chunks, A(1), r, g.start, g.start + (k - 1u) * p.L, p.L, S, (T*)nullptr, (A*)nullptr, 0);
+    delta_walk<T, KT, TEAM, false>(p, l, lds[l.team], Q, K, unit ? (const T*)nullptr : V, chunks, A(1), r, g.start, g.start + (k - 1u) * p.L, p.L, S, (T*)nullptr, (A*)nullptr, 0, e);
+    if (unit) {
+        level<A, KT>(S, e);
+        if (l.g == 0u && l.c < l.nv) through[((size_t)p.cuts * p.K + slot) * p.H * p.K + l.v + l.c] = (A)e;
+    }
     store_state<A, KT>(S, unit ? through + slot * ((size_t)p.K * p.H * p.K) : carry + slot * ((size_t)p.K * p.H * p.V), p, l);
 }
 
@@ -315,14 +324,25 @@ __global__ __launch_bounds__(64 * KT) void k_delta_carry(delta_shape p, bool bac
                 a[s][j] = row < p.K && k < p.K ? backward ? m[k * HK + row] : m[row * HK + k] : A(0);
             }
     };
-    const vec start = load(first + (backward ? n - 1u : 1u));
+    // the exponents of a transition's columns: forward they belong to the rows of what goes in, backward to those of what comes out
+    struct { int e[4]; } power, next = {};
+    auto exponents = [&](unsigned i) {
+        const A* m = through + ((size_t)p.cuts * p.K + first + (backward ? n - i + 1u : i)) * HK + (size_t)head * p.K;
+        decltype(power) x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) lds[0][t][i][lane] = start[i];
+        for (int j = 0; j < 4; ++j) x.e[j] = 16u * t + mm16<A>::row(g, j) < p.K ? (int)m[16u * t + mm16<A>::row(g, j)] : 0;
+        return x;
+    };
+    const vec start = load(first + (backward ? n - 1u : 1u));
+    power = exponents(2u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lds[0][t][i][lane] = backward ? start[i] : scaled(start[i], power.e[i]);
     transition(2u);
     vec own = load(to(2u));
     __syncthreads();
     for (unsigned i = 2; i < n; ++i) {
-        vec x = own;
+        if (i + 1u < n) next = exponents(i + 1u);
+        vec x = backward ? zero16<A>() : own;
 #pragma unroll
         for (int s = 0; s < KT; ++s) {
             vec b;
@@ -330,13 +350,17 @@ __global__ __launch_bounds__(64 * KT) void k_delta_carry(delta_shape p, bool bac
             for (int j = 0; j < 4; ++j) b[j] = lds[i & 1u][s][j][lane];
             x = product<A>(a[s], b, x);
         }
+        if (backward)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = own[j] + scaled(x[j], power.e[j]);
+        power = next;
         if (i + 1u < n) {
             transition(i + 1u);
             own = load(to(i + 1u));
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            lds[~i & 1u][t][j][lane] = x[j];
+            lds[~i & 1u][t][j][lane] = backward ? x[j] : scaled(x[j], power.e[j]);
             if (here && 16u * t + mm16<A>::row(g, j) < p.K) *state(to(i), j) = x[j];
         }
         __syncthreads();

@@ -1,0 +1,113 @@
+"""The gated delta rule, the norms around a block and clipping at values where they can go wrong: states that grow or vanish over the segments of long
+regions, resets, infinities and undefined values there, bad rows in wide chunks, factors beyond a float's range. Tolerances as in test_blocks_gpu."""
+import numpy as np
+import pytest
+import torch
+
+from tests import blocks_ref as ref
+from tests.gpu_util import host
+from tests.test_blocks_gpu import delta_case
+from tests.test_rows_gpu import STORED, TYPES, U, inside, put, regions, wide
+
+pytestmark = pytest.mark.gpu
+
+GRADS = ("dQ", "dK", "dV", "dbeta", "ddecay")
+LONG = [[1030, 1100], [0, 1030]]                 # one not cut, one of four whole segments of 256 rows and a short one
+SEGMENT = 256
+
+
+def near(got, want, bound, kind, what, rows, stored=True, least=1e-35):
+    """Within the bound, the stored type's rounding and `least`, which is what falls below the type's range."""
+    got = host(got.double())
+    got, want, bound = (got, want, bound) if rows is None else (got[rows], want[rows], bound[rows])
+    assert got.shape == want.shape and np.isfinite(want).all(), what
+    bound = 1.01 * U[kind] * bound + (STORED[kind] if stored else U[kind]) * np.abs(want) + least
+    bad = ~(np.abs(got - want) <= bound)
+    assert not bad.any(), "%s: %d of %d values off at rows %s, worst %.3g of the bound" % (what, bad.sum(), bad.size, np.unique(np.argwhere(bad)[:, 0])[:5].tolist(),
+                                                                                          (np.abs(got - want) / bound).max())
+
+
+def delta_as_by_rows(kind, t, v, R, G, Kd, what, least=1e-35, grads=True, state=None):
+    """Forward, and backward from zero states, against the definition."""
+    from deepbind_amd import kangaroo_smat as ks
+    N = v["beta"].shape[0]
+    T, rows = regions(R), inside(R, N)
+    args = (t["Q"], t["K"], t["V"], t["beta"], T)
+    kw = dict(decay=t["decay"], groups=G)
+    plain = (v["Q"], v["K"], v["V"], v["beta"], v["decay"], R, G, Kd ** -0.5)
+    with np.errstate(all="ignore"):
+        want = ref.delta(*plain, dO=v["dO"] if grads else None, state=None if state is None else state[1])
+        bound = ref.delta_bounds(*plain, dO=v["dO"] if grads else None, state=None if state is None else state[1], segment=SEGMENT)
+    keep = ks.kept_delta(t["K"], t["V"], t["beta"], groups=G) if grads else None
+    O, last = ks.deltarule(*args, keep=keep, want_state=True, state=None if state is None else state[0], **kw)
+    near(O, want[0], bound[0], kind, what + ": O", rows, least=least)
+    near(last, want[1], bound[1], kind, what + ": last", None, stored=False, least=least)
+    if grads:
+        for name, g, w, b in zip(GRADS, ks.deltarule_bprop(*args, keep, t["dO"], **kw), want[2:], bound[2:]):
+            if g is not None:
+                near(g, w, b, kind, "%s: %s" % (what, name), rows, stored=name in GRADS[:3], least=least)
+
+
+def changed(t, v, name, rows, value):
+    """Rows of a map set to a value, or multiplied by it (a factor in a tuple), on the device and in the plain form."""
+    t[name][rows] = t[name][rows] * value[0] if isinstance(value, tuple) else value
+    v[name] = t[name].double().cpu().numpy()
+
+
+SHAPES = [(2, 1, 16, 16), (2, 2, 40, 33), (1, 1, 128, 70), (3, 1, 20, 5)]
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("H,G,Kd,Vd", SHAPES)
+def test_delta_rule_of_segments_whose_states_grow_and_vanish(kind, H, G, Kd, Vd):
+    """A segment of a long region may grow or shrink a state by more than the type's range: what is nothing in front of it stays nothing, what is small
+    or large becomes what it becomes row by row."""
+    N = 1100
+    big = 8 if kind == "float64" else 1          # (2^1024 is eight times 2^128)
+    rate = 0.36 * big                            # e^92 in a segment of 256 rows; 16 rows stay far within the range
+    case = lambda: delta_case(kind, N, H, G, Kd, Vd, True, 0, [H, Kd, Vd])  # noqa: E731
+    t, v = case()
+    changed(t, v, "beta", slice(0, 520), 0.0)
+    changed(t, v, "decay", slice(0, 520), rate)
+    delta_as_by_rows(kind, t, v, LONG, G, Kd, "nothing in front", grads=False)
+    t, v = case()
+    changed(t, v, "decay", slice(520, 521), -1e4)
+    changed(t, v, "beta", slice(520, 1030), 0.0)
+    changed(t, v, "decay", slice(521, 1030), rate)
+    changed(t, v, "dO", slice(520, 1030), 0.0)
+    delta_as_by_rows(kind, t, v, LONG, G, Kd, "no gradient behind")
+    if kind == "float64":                        # (the bounds' norms square what is over 1e160 then)
+        return
+    for first, second, value, grad in ((rate, -rate, 1e-20, 1e-10), (-rate, rate, 1e15, 1e-15)):
+        t, v = case()
+        changed(t, v, "beta", slice(256, 768), (0.02,))
+        changed(t, v, "decay", slice(256, 512), first)
+        changed(t, v, "decay", slice(512, 768), second)
+        changed(t, v, "V", slice(0, N), (value,))
+        if first < 0:
+            changed(t, v, "V", slice(256, 768), (1e-38,))                      # (1e-23: the growth behind makes it 1e17)
+        changed(t, v, "dO", slice(0, N), (grad,))
+        delta_as_by_rows(kind, t, v, LONG, G, Kd, "up and down" if first > 0 else "down and up")
+
+
+def test_delta_rule_in_double_of_segments_whose_states_grow_and_vanish_is_that_of_shorter_pieces():
+    from deepbind_amd import kangaroo_smat as ks
+    N, H, Kd, Vd = 1030, 2, 40, 20
+    for first, value in ((2.88, 1e-160), (-2.88, 1e120)):
+        t, v = delta_case("float64", N, H, 1, Kd, Vd, True, 0, 31)
+        changed(t, v, "beta", slice(256, 768), (0.02,))
+        changed(t, v, "decay", slice(256, 512), first)
+        changed(t, v, "decay", slice(512, 768), -first)
+        changed(t, v, "V", slice(0, N), (value,))
+        if first < 0:
+            changed(t, v, "V", slice(256, 768), (1e-300,))
+        call = lambda a, b, **kw: ks.deltarule(t["Q"][a:b], t["K"][a:b], t["V"][a:b], t["beta"][a:b], regions([[0, b - a]]), decay=t["decay"][a:b], groups=1, want_state=True, **kw)  # noqa: E731
+        O, last = call(0, N)
+        parts, state = [], None
+        for a in range(0, N, 128):
+            o, state = call(a, min(a + 128, N), state=state)
+            parts.append(o)
+        # both are off by at most what the bounds of the float32 cases above come to in units of their values, some 12 000
+        for got, want in ((O, torch.cat(parts)), (last.view(Kd, -1), state.view(Kd, -1))):
+            assert got.isfinite().all()
+            assert float(((got - want).abs().amax(1) / want.abs().amax(1)).max()) < 2 * 12000 * 2.0 ** -53
