@@ -129,15 +129,22 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
     for (int i = 0; i < 16; ++i) lds[g][i][c] = n[i];
     sync();
     A x[16];
-    {
+    // A column of the inverse is zero above its own row, and takes nothing from columns before it: where a value in them is not finite (zero times it would be a NaN, and
+    // send one back to rows behind a bad key or decay, whose own gradients do not know of it) their places are left out one by one.
+    auto substitute = [&](auto careful) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             A s[4] = {A(0), A(0), A(0), A(0)};
 #pragma unroll
-            for (int m = 0; m < i; ++m) s[m & 3] = fma(lds[g][i][m], x[m], s[m & 3]);
+            for (int m = 0; m < i; ++m) s[m & 3] = careful.value && m < (int)c ? s[m & 3] : fma(lds[g][i][m], x[m], s[m & 3]);
             x[i] = i <= (int)c ? (i == (int)c ? A(1) : A(0)) : -b[16u * g + i] * ((s[0] + s[1]) + (s[2] + s[3]));
         }
-    }
+    };
+    substitute(std::false_type());
+    A finite = A(0);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) finite = fma(x[i], A(0), finite);
+    if (__any(finite != A(0))) substitute(std::true_type());
     sync();
     put(ss);
     A s[16];

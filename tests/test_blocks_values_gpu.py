@@ -111,3 +111,41 @@ def test_delta_rule_in_double_of_segments_whose_states_grow_and_vanish_is_that_o
         for got, want in ((O, torch.cat(parts)), (last.view(Kd, -1), state.view(Kd, -1))):
             assert got.isfinite().all()
             assert float(((got - want).abs().amax(1) / want.abs().amax(1)).max()) < 2 * 12000 * 2.0 ** -53
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("H,G,Kd,Vd,R,rows", [(2, 1, 20, 24, [[0, 100], [100, 150]], (37, 99)), (3, 3, 16, 16, [[0, 100], [100, 150]], (37, 140)),
+                                              (2, 2, 40, 20, LONG, (37, 300, 511, 512, 1029)), (2, 1, 128, 20, LONG, (300, 700))])
+def test_delta_rule_carries_what_is_not_finite_exactly_as_far_as_the_formulas(kind, H, G, Kd, Vd, R, rows):
+    """One value that is not finite, anywhere: what the row by row formulas, forward and backward, keep finite is the same bits as without it, and what they
+    do not keep finite is not."""
+    from deepbind_amd import kangaroo_smat as ks
+    N = max(e for _, e in R)
+    t, v = delta_case(kind, N, H, G, Kd, Vd, True, 0, 12)
+    args = (t["Q"], t["K"], t["V"], t["beta"], regions(R))
+    kw = dict(decay=t["decay"], groups=G)
+    keep = ks.kept_delta(t["K"], t["V"], t["beta"], groups=G)
+
+    def both():
+        O, last = ks.deltarule(*args, keep=keep, want_state=True, **kw)
+        return (O, last) + ks.deltarule_bprop(*args, keep, t["dO"], **kw)
+
+    good = both()
+    for row in rows:
+        for name in ("V", "Q", "K", "beta", "decay", "dO"):
+            for bad in (float("nan"), float("inf")):
+                x, col = t[name], min(5, t[name].shape[1] - 1)
+                old = x[row, col].clone()
+                x[row, col] = bad
+                got = both()
+                x[row, col] = old
+                w = {k: a.copy() if k == name else a for k, a in v.items()}
+                w[name][row, col] = bad
+                with np.errstate(all="ignore"):
+                    want = ref.delta(w["Q"], w["K"], w["V"], w["beta"], w["decay"], R, G, Kd ** -0.5, dO=w["dO"])
+                for what, g, clean, wanted in zip(("O", "last") + GRADS[:4], got, good, want):
+                    keeps = torch.from_numpy(np.isfinite(wanted)).cuda()
+                    same = g == clean
+                    assert bool(same[keeps].all()), "%s[%d] = %s: %s changes at rows %s" % (name, row, bad, what, np.unique(np.argwhere(host(keeps & ~same))[:, 0]).tolist()[:20])
+                    left = g.isfinite() & ~keeps
+                    assert not bool(left.any()), "%s[%d] = %s: %s is finite at rows %s" % (name, row, bad, what, np.unique(np.argwhere(host(left))[:, 0]).tolist()[:20])
