@@ -385,7 +385,20 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
                 before[r] = j < c ? A(1) : A(0);
                 db += ln;
             }
-            const vec upto = product<A>(e, before, zero16<A>());         // [i][m]: sum over j < m
+            vec upto = product<A>(e, before, zero16<A>());               // [i][m]: sum over j < m
+            if (__any(!all_finite(upto)))                                // (one m after the other, without the pairs from m on, whose zeros would take a NaN from what is not finite in them)
+#pragma unroll 1
+                for (unsigned m = 0; m < 16u; ++m) {
+                    vec some, one;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        some[r] = l.row(r) < m ? e[r] : A(0);
+                        one[r] = A(1);
+                    }
+                    some = product<A>(some, one, zero16<A>());
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) upto[r] = c == m ? some[r] : upto[r];
+                }
 #pragma unroll
             for (int r = 0; r < 4; ++r) dg += l.row(r) >= c ? upto[r] : A(0);
             db += __shfl_xor(db, 16);

@@ -143,7 +143,7 @@ def test_delta_rule_carries_what_is_not_finite_exactly_as_far_as_the_formulas(ki
                 w[name][row, col] = bad
                 with np.errstate(all="ignore"):
                     want = ref.delta(w["Q"], w["K"], w["V"], w["beta"], w["decay"], R, G, Kd ** -0.5, dO=w["dO"])
-                for what, g, clean, wanted in zip(("O", "last") + GRADS[:4], got, good, want):
+                for what, g, clean, wanted in zip(("O", "last") + GRADS, got, good, want):
                     keeps = torch.from_numpy(np.isfinite(wanted)).cuda()
                     same = g == clean
                     assert bool(same[keeps].all()), "%s[%d] = %s: %s changes at rows %s" % (name, row, bad, what, np.unique(np.argwhere(host(keeps & ~same))[:, 0]).tolist()[:20])
