@@ -30,6 +30,9 @@ constexpr unsigned DELTA_BLOCK = 64;             // rows of a block, for which s
 constexpr unsigned DELTA_CHUNKS = DELTA_BLOCK / DELTA_CHUNK;
 constexpr size_t DELTA_KEY = 128;                // the most columns of a key
 
+// marks of a head in a region: a chunk whose matrices leave the type's range; a row that may lengthen a state
+constexpr unsigned DELTA_ODD = 1, DELTA_GROWS = 2;
+
 struct delta_shape {
     unsigned N, nregion, H, G, K, V, ns;         // rows, regions, heads, key heads, columns of a key and of a value, tiles of 16 value columns per head
     unsigned slots;                              // blocks that are not a region's first (segment_slots)
@@ -114,6 +117,13 @@ template <typename A> struct delta_matrices {
     A T[256], P[256];
     A first[16], last[16], b[16], spare[16];
 };
+
+// What a chunk's matrices may hold. Decays above zero, or keys longer than one, take them beyond the type's range in 16 rows where the rows themselves may find nothing to multiply, and
+// infinity times nothing is a NaN; a product that has almost vanished and grows again has lost its digits. A head with such a chunk in a region, whose keys, queries, factors and corrections
+// are all finite, is marked (prepare); three of the largest entries multiplied, as they are in a chunk, stay within the range. What the kernels make of it is made again row by row, as the definition has it (k_delta_rows, k_delta_bprop_rows): slow, but as far as that goes.
+template <typename A> struct delta_range;
+template <> struct delta_range<float> { static constexpr double most = 0x1p36, least = 0x1p-100; };
+template <> struct delta_range<double> { static constexpr double most = 0x1p300, least = 0x1p-900; };
 
 // Blocks are numbered like segments (rows_common.h): a region's first by the region, the others by their slot behind those.
 struct delta_block {
@@ -543,7 +553,7 @@ template <typename A, int KT, int TEAM, int WAVES> __device__ __forceinline__ vo
             S[t][r] = p && k < s.K && l.c < l.nv ? p[k * l.D + l.v + l.c] : A(0);
         }
 }
-template <typename A, int KT, int TEAM> __device__ __forceinline__ void store_state(const typename mm16<A>::vec (&S)[KT], A* p, const delta_shape& s, const delta_lane<A, TEAM>& l)
+template <typename A, int KT, int TEAM, int WAVES> __device__ __forceinline__ void store_state(const typename mm16<A>::vec (&S)[KT], A* p, const delta_shape& s, const delta_lane<A, TEAM, WAVES>& l)
 {
 #pragma unroll
     for (int t = 0; t < KT; ++t)
@@ -558,18 +568,13 @@ template <typename A, int KT, int TEAM> __device__ __forceinline__ void store_st
 // Columns of zeros and with an infinity stay as they are; a NaN is no size and stays.
 __device__ __forceinline__ float scaled(float x, int e) { return ldexpf(x, e); }
 __device__ __forceinline__ double scaled(double x, int e) { return ldexp(x, e); }
-template <typename A, int KT> __device__ __forceinline__ A largest(const typename mm16<A>::vec (&S)[KT])
+template <typename A, int KT> __device__ __forceinline__ int level(typename mm16<A>::vec (&S)[KT], int& e)
 {
     A m = A(0);
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) m = fmax(m, fabs(S[t][r]));
-    return m;
-}
-template <typename A, int KT> __device__ __forceinline__ void level(typename mm16<A>::vec (&S)[KT], int& e)
-{
-    A m = largest<A, KT>(S);
     m = fmax(m, __shfl_xor(m, 16));
     m = fmax(m, __shfl_xor(m, 32));
     const int x = m > A(0) && m * A(0) == A(0) ? ilogb(m) : 0;
@@ -577,19 +582,45 @@ template <typename A, int KT> __device__ __forceinline__ void level(typename mm1
     for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[t][r] = scaled(S[t][r], -x);
-    e += x;
+    return e += x;
 }
+
+// Keys or queries of one row in the order of a state's registers, and what a state holds of them: the sum over a column's lanes.
+template <typename A, int KT, typename T> __device__ __forceinline__ void row_tiles(typename mm16<A>::vec (&x)[KT], const T* row, unsigned K, unsigned g)
+{
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const unsigned k = 16u * t + mm16<A>::row(g, r);
+            x[t][r] = k < K ? (A)row[k] : A(0);
+        }
+}
+template <typename A, int KT> __device__ __forceinline__ A found(const typename mm16<A>::vec (&x)[KT], const typename mm16<A>::vec (&S)[KT])
+{
+    A w = A(0);
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w = fma(x[t][r], S[t][r], w);
+    w += __shfl_xor(w, 16);
+    return w + __shfl_xor(w, 32);
+}
+constexpr unsigned DELTA_ROWS_WGS = 512;         // workgroups that look for marked heads
+// What a row multiplies the state by
+template <typename A> __device__ __forceinline__ A row_factor(const delta_shape& p, const A* decay, size_t row, unsigned head) { return decay ? (A)exp((double)decay[row * p.ldg + head]) : A(1); }
 
 // Defined in deltarule.hip.
 delta_shape delta_shape_of(const dbk_deltarule_args& a);
 int check_delta(const dbk_deltarule_args* a);
-int delta_mark(hipStream_t st, const delta_shape& s, const uint32_t* regions, uint32_t* marks, uint32_t* cuts);
+// odd: the marks of regions' heads (nregion, H), and behind them whether any is DELTA_ODD; cleared by the first and set by the second
+int delta_mark(hipStream_t st, const delta_shape& s, const uint32_t* regions, uint32_t* marks, uint32_t* cuts, uint32_t* odd);
 // chunks, and pairs where it is not null, of every block and head
-void delta_prepare(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const uint32_t* marks, void* chunks, void* pairs);
+void delta_prepare(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const uint32_t* marks, void* chunks, void* pairs, uint32_t* odd);
 // What regions cut into segments need, in the workspace: whose segment a slot holds, and in front of every segment but a region's first the state (or its gradient) there.
 // Transitions, by which a segment takes what is in front of it to its end, lie behind the kept states, or in the workspace where none are kept: (H, K, K) values for a segment, and behind those
-// of all segments (H, K) exponents, kept as values are, of the powers of two by which the transitions' columns are larger (level): a segment may grow or shrink a state beyond the type's
-// range, where what is in front of it is small or nothing, or the segment behind does the opposite.
+// of all segments (H, K) exponents, kept as values are, of the powers of two by which the transitions' columns are larger (level), and behind those a mark per 16 columns that have any: a
+// segment may grow or shrink a state beyond the type's range, where what is in front of it is small or nothing, or the segment behind does the opposite.
 struct delta_cuts {
     uint32_t* marks;
     char* carry;
@@ -598,7 +629,8 @@ struct delta_cuts {
 void delta_carry(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const delta_cuts& w, bool backward);
 // values (not bytes) of the kept states, behind which the transitions lie
 inline size_t delta_kept(const delta_shape& s) { return (size_t)s.slots * s.K * s.H * s.V; }
-inline size_t delta_through(const delta_shape& s) { return (size_t)s.cuts * s.H * s.K * (s.K + 1); }
+inline size_t delta_through(const delta_shape& s) { return (size_t)s.cuts * s.H * (s.K * (s.K + 1) + DELTA_KEY / 16); }
+inline size_t delta_odd_bytes(const delta_shape& s) { return ((size_t)s.nregion * s.H + 1) * sizeof(uint32_t); }
 inline size_t delta_blocks(const delta_shape& s) { return (size_t)s.nregion + s.slots; }
 inline size_t align16(size_t n) { return (n + 15) / 16 * 16; }
 

@@ -3,7 +3,7 @@
 
 namespace dbk {
 
-__global__ __launch_bounds__(256) void k_delta_mark(delta_shape p, const uint32_t* __restrict__ regions, uint32_t* __restrict__ marks, uint32_t* __restrict__ cuts)
+__global__ __launch_bounds__(256) void k_delta_mark(delta_shape p, const uint32_t* __restrict__ regions, uint32_t* __restrict__ marks, uint32_t* __restrict__ cuts, uint32_t* __restrict__ odd)
 {
     // a wave per region
     const unsigned r = blockIdx.x * 4u + (threadIdx.x >> 6);
@@ -11,6 +11,8 @@ __global__ __launch_bounds__(256) void k_delta_mark(delta_shape p, const uint32_
     const row_range g = region_rows(regions, r, p.N);
     mark_segments(marks, r, g, DELTA_BLOCK, threadIdx.x & 63u, 64u);
     if (p.L) mark_segments(cuts, r, g, p.L, threadIdx.x & 63u, 64u);
+    for (unsigned h = threadIdx.x & 63u; h < p.H; h += 64u) odd[(size_t)r * p.H + h] = 0u;
+    if (blockIdx.x == 0u && threadIdx.x == 0u) odd[(size_t)p.nregion * p.H] = 0u;
 }
 
 // A chunk's matrices. A wave takes a block of a head, four chunks: the products of its keys and queries on the matrix cores, then a lane per chunk and column for the
@@ -23,7 +25,7 @@ template <typename T, int KT>
 __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)) void k_delta_prepare(delta_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, const T* __restrict__ Q,
                                                        const T* __restrict__ K, const typename acc_of<T>::type* __restrict__ beta,
                                                        const typename acc_of<T>::type* __restrict__ decay, delta_chunk<typename acc_of<T>::type>* __restrict__ chunks,
-                                                       delta_pairs<typename acc_of<T>::type>* __restrict__ pairs)
+                                                       delta_pairs<typename acc_of<T>::type>* __restrict__ pairs, uint32_t* __restrict__ odd)
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
@@ -102,7 +104,7 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
     b[lane] = step.get(lane < bl.rows);
     sync();
     // lane (g, c): column c of chunk g
-    A D[16], n[16];
+    A D[16], n[16], finite = A(0), size = A(0);
     {
         // (in double precision: a state that decays by a thousandth a row remembers a thousand of them, and would their factors' roundings)
         double product = 0.0, first = 1.0;
@@ -115,6 +117,24 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
             first *= ai;
             mine = i == (int)c ? (A)first : mine;
             n[i] = i > (int)c ? D[i] * lds[g][i][c] : A(0);
+            finite = fma(lds[g][i][c], A(0), finite);
+            size = fmax(size, D[i]);
+        }
+        size = fmax(size, mine);
+        finite = fma((A)a[16u * g + c], A(0), fma(b[16u * g + c], A(0), finite));
+        // a row lengthens what lies along its key by the factor |1 - b k.k|, which lies within rounding's reach of one where keys of length one are learnt by b = 2
+        const A turned = b[16u * g + c] * lds[g][c][c];
+        if (__any(a[lane] > 1.0 || turned > A(2.05) || turned < A(-0.05)) && lane == 0u) atomicOr(odd + (size_t)bl.r * p.H + head, DELTA_GROWS);
+        if (__any(a[lane] > 1.0)) {              // (does a product that is almost nothing grow again)
+            product = 0.0;
+            first = 1.0;
+#pragma unroll 1
+            for (unsigned i = 0; i < 16u; ++i) {
+                const double ai = a[16u * g + i];
+                if (ai > 1.0 && ((product > 0.0 && product < delta_range<A>::least) || (first > 0.0 && first < delta_range<A>::least))) size = A(INFINITY);
+                product = i == c ? 1.0 : product * ai;
+                first *= ai;
+            }
         }
         if (g < nchunk) {
             delta_chunk<A>& to = chunks[number(g)];
@@ -141,28 +161,37 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
         }
     };
     substitute(std::false_type());
-    A finite = A(0);
+    A stray = A(0);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) finite = fma(x[i], A(0), finite);
-    if (__any(finite != A(0))) substitute(std::true_type());
+    for (int i = 0; i < 16; ++i) stray = fma(x[i], A(0), stray);
+    if (__any(stray != A(0))) substitute(std::true_type());
     sync();
     put(ss);
     A s[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = i >= (int)c ? D[i] * lds[g][i][c] : A(0);
+    for (int i = 0; i < 16; ++i) {
+        s[i] = i >= (int)c ? D[i] * lds[g][i][c] : A(0);
+        finite = fma(lds[g][i][c], A(0), finite);
+        size = fmax(size, fmax(fabs(x[i]), fabs(s[i]) * A(0x1p-64)));       // (a query's product with a key goes nowhere but into its own output)
+    }
+    const uint64_t beyond = __ballot(size > A(delta_range<A>::most)), bad = __ballot(finite != A(0));
+    // (rarely any; the order in which marks are added does not matter)
+    if (c == 0u && (beyond >> 16u * g & 0xffffu) && !(bad >> 16u * g & 0xffffu)) {
+        atomicOr(odd + (size_t)bl.r * p.H + head, DELTA_ODD);
+        odd[(size_t)p.nregion * p.H] = 1u;
+    }
     store([&](size_t i) { return chunks[i].TP; }, s, x);
 }
 
 // Walks a wave's 16 columns of a head's state down `rows` rows from `row` on, of region r, which starts at `first`.
 // Keys, queries, matrices and values of a chunk come while the one before it is worked on. OUT: rows of O are written; otherwise only the state moves on. V null:
-// without values, for what becomes of the state alone, whose columns are then kept near one (level, exponents in e). Bound by issue and by one chunk's chain, which waves of other heads and regions fill: 191 284 rows, 4 heads of 64 x 64 floats 314 us
+// without values, for what becomes of the state alone, whose columns are kept near one where they may grow (leveled; exponents in e). Bound by issue and by one chunk's chain, which waves of other heads and regions fill: 191 284 rows, 4 heads of 64 x 64 floats 314 us
 // (850 MB at 2.7 TB/s, 23 GFLOP: matrix units busy for 46 % of the time, vector instructions 27 %); 41 816 bfloat16 rows, 8 heads of 128 x 128 in 32 segments 275 us (25 % and 49 %, most of
 // which takes the states apart into pieces). Four waves on the same head's keys share what is fetched: alone, each would read all of it.
-constexpr double LEVEL_MOST = 1099511627776.0;    // 2^40
 template <typename T, int KT, int TEAM, bool OUT>
 __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, typename delta_ops<T, KT>::rows* lds, const T* Q, const T* K,
                                            const T* V, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, unsigned r, unsigned first, size_t row, unsigned rows,
-                                           typename mm16<typename acc_of<T>::type>::vec (&S)[KT], T* O, typename acc_of<T>::type* keep, size_t kept, int& e)
+                                           typename mm16<typename acc_of<T>::type>::vec (&S)[KT], T* O, typename acc_of<T>::type* keep, size_t kept, bool leveled, int& e)
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
@@ -193,8 +222,8 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
         }
         if (t + 2u * DELTA_CHUNK < rows) fetch(t + 2u * DELTA_CHUNK);
         if (l.nv) {
-            if constexpr (!OUT)                  // (what has grown before every chunk, what has shrunk before every block)
-                if (!V && (t % DELTA_BLOCK == 0 || __any(largest<A, KT>(S) > LEVEL_MOST))) level<A, KT>(S, e);
+            if constexpr (!OUT)
+                if (leveled) level<A, KT>(S, e);
             if (keep && (t || row != first) && t % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + (kept + t / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
             vec w = zero16<A>(), z = zero16<A>();
             delta_ops<T, KT>::template find<OUT>(here.k, here.q, S, w, z, l.g, l.c);
@@ -248,18 +277,59 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
     load_state<A, KT>(S, from, p, l);
     const unsigned before = k * (p.L / DELTA_BLOCK);
     int e = 0;
-    delta_walk<T, KT, TEAM, true>(p, l, lds[l.team], Q, K, V, chunks, scale, r, g.start, start, rows, S, O, keep, kept_number(g, before), e);
+    delta_walk<T, KT, TEAM, true>(p, l, lds[l.team], Q, K, V, chunks, scale, r, g.start, start, rows, S, O, keep, kept_number(g, before), false, e);
     if (last && start + rows == g.end) store_state<A, KT>(S, last + r * block, p, l);
 }
 
+// The regions of marked heads, row by row, in the place of what the kernel above made of them: a wave takes 16 columns of a head through one. 4096 rows of 16 heads of
+// 64 x 64 floats 5.8 ms (by chunks 0.25), and 33 backward (0.33): nothing is overlapped here.
+template <typename T, int KT>
+__global__ __launch_bounds__(64) void k_delta_rows(delta_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ odd, const T* __restrict__ Q, const T* __restrict__ K,
+                                                   const T* __restrict__ V, const typename acc_of<T>::type* __restrict__ beta, const typename acc_of<T>::type* __restrict__ decay,
+                                                   typename acc_of<T>::type scale, const typename acc_of<T>::type* __restrict__ state, T* __restrict__ O,
+                                                   typename acc_of<T>::type* __restrict__ last, typename acc_of<T>::type* __restrict__ keep)
+{
+    typedef typename acc_of<T>::type A;
+    typedef typename mm16<A>::vec vec;
+    if (!uniform(odd[(size_t)p.nregion * p.H])) return;
+    const size_t block = (size_t)p.K * p.H * p.V;
+    for (size_t i = blockIdx.x; i < (size_t)p.nregion * p.H * p.ns; i += gridDim.x) {
+        const unsigned r = (unsigned)(i / (p.H * p.ns));
+        delta_lane<A, 1, 1> l;
+        l.place(p, (unsigned)(i % (p.H * p.ns)), p.V);
+        if (!(uniform(odd[(size_t)r * p.H + l.head]) & DELTA_ODD)) continue;
+        const row_range g = region_rows(regions, r, p.N);
+        const bool here = l.c < l.nv;
+        vec S[KT], x[KT];
+        load_state<A, KT>(S, state ? state + r * block : (const A*)nullptr, p, l);
+#pragma unroll 1
+        for (size_t row = g.start; row < g.end; ++row) {
+            const unsigned at = (unsigned)row - g.start;
+            if (keep && at && at % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + kept_number(g, at / DELTA_BLOCK) * block, p, l);
+            const A a = row_factor(p, decay, row, l.head);
+            row_tiles<A, KT>(x, K + row * p.ldk + (size_t)l.group * p.K, p.K, l.g);
+#pragma unroll
+            for (int t = 0; t < KT; ++t) S[t] *= a;
+            const A u = beta[row * p.ldb + l.head] * ((here ? (A)V[row * p.ldv + l.v + l.c] : A(0)) - found<A, KT>(x, S));
+#pragma unroll
+            for (int t = 0; t < KT; ++t) S[t] += x[t] * u;
+            row_tiles<A, KT>(x, Q + row * p.ldq + (size_t)l.group * p.K, p.K, l.g);
+            const A o = scale * found<A, KT>(x, S);
+            if (here && l.g == 0u) O[row * p.ldo + l.v + l.c] = (T)o;
+        }
+        if (last) store_state<A, KT>(S, last + r * block, p, l);
+    }
+}
+
+constexpr int LEVEL_PLAIN = 60;                   // columns of up to this power of two, either way, are stored as they are
 // What the segment in front of a slot's hands on: its state, from the region's own initial one (the first) or from zeros, and (the others) how it takes the
 // state in front of it to its end: the states that the unit vectors become, times powers of two. Workgroups from `values` on along y take those. Keys of 128 columns beside values of 128: twice the
 // forward pass's columns without its outputs, 350 us where that takes 275 (vector instructions 54 % of the time; four waves per SIMD instead of two, for which registers spill, gain nothing).
 template <typename T, int KT, int TEAM>
 __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEAM>())) void k_delta_local(delta_shape p, unsigned values, const uint32_t* __restrict__ regions,
-                                                     const uint32_t* __restrict__ cuts, const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
-                                                     const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, const typename acc_of<T>::type* __restrict__ state,
-                                                     typename acc_of<T>::type* __restrict__ carry, typename acc_of<T>::type* __restrict__ through)
+                                                     const uint32_t* __restrict__ cuts, const uint32_t* __restrict__ odd, const T* __restrict__ Q, const T* __restrict__ K,
+                                                     const T* __restrict__ V, const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks,
+                                                     const typename acc_of<T>::type* __restrict__ state, typename acc_of<T>::type* __restrict__ carry, typename acc_of<T>::type* __restrict__ through)
 {
     typedef typename acc_of<T>::type A;
     typedef typename mm16<A>::vec vec;
@@ -273,6 +343,7 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
     delta_lane<A, TEAM> l;
     l.place(p, unit ? blockIdx.y - values : blockIdx.y, unit ? p.K : p.V);
     vec S[KT];
+    const bool grows = unit && (uniform(odd[(size_t)r * p.H + l.head]) & DELTA_GROWS);
     int e = 0;
     if (unit) {
 #pragma unroll
@@ -281,9 +352,21 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
             for (int i = 0; i < 4; ++i) S[t][i] = 16u * t + l.row(i) == 16u * l.tile + l.c && l.nv ? A(1) : A(0);
     } else
         load_state<A, KT>(S, state && k == 1u ? state + (size_t)r * p.K * p.H * p.V : (const A*)nullptr, p, l);
-    delta_walk<T, KT, TEAM, false>(p, l, lds[l.team], Q, K, unit ? (const T*)nullptr : V, chunks, A(1), r, g.start, g.start + (k - 1u) * p.L, p.L, S, (T*)nullptr, (A*)nullptr, 0, e);
+    delta_walk<T, KT, TEAM, false>(p, l, lds[l.team], Q, K, unit ? (const T*)nullptr : V, chunks, A(1), r, g.start, g.start + (k - 1u) * p.L, p.L, S, (T*)nullptr, (A*)nullptr, 0, grows, e);
     if (unit) {
-        level<A, KT>(S, e);
+        // (powers of two only where a column's size is far from one and something grows: the carry looks at them then alone, and what only ever shrinks is not missed)
+        if (grows) {
+            const int size = level<A, KT>(S, e);
+            if (size > -LEVEL_PLAIN && size < LEVEL_PLAIN) {
+#pragma unroll
+                for (int t = 0; t < KT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) S[t][i] = scaled(S[t][i], e);
+                e = 0;
+            }
+        }
+        const bool some = __any(e != 0);
+        if (l.g == 0u && l.c == 0u && l.nv) through[((size_t)p.cuts * (p.K + 1u) * p.K + (size_t)slot * KT + l.tile) * p.H + l.head] = some ? A(1) : A(0);
         if (l.g == 0u && l.c < l.nv) through[((size_t)p.cuts * p.K + slot) * p.H * p.K + l.v + l.c] = (A)e;
     }
     store_state<A, KT>(S, unit ? through + slot * ((size_t)p.K * p.H * p.K) : carry + slot * ((size_t)p.K * p.H * p.V), p, l);
@@ -320,6 +403,45 @@ __global__ __launch_bounds__(64 * KT) void k_delta_carry(delta_shape p, bool bac
     };
     // forward: slot i from slot i - 1 by the transition of segment i - 1, which lies in slot i; backward: slot n - i from slot n - i + 1 by that of segment n - i, in slot n - i + 1
     auto to = [&](unsigned i) { return first + (backward ? n - i : i); };
+    // Where a column of a transition has an exponent, the workgroup takes one step after the other as it stands: forward what goes in is multiplied, backward what comes out.
+    const A *exponents = through + (size_t)p.cuts * p.K * HK + (size_t)head * p.K, *marks = through + (size_t)p.cuts * (p.K + 1u) * HK + head;
+    bool some = false;
+    for (unsigned i = 2u + lane; i < n; i += 64u) some |= 16u * t < p.K && marks[((first + i) * KT + t) * p.H] != A(0);
+    if (__syncthreads_or(some)) {
+        vec x = load(first + (backward ? n - 1u : 1u));
+#pragma unroll 1
+        for (unsigned i = 2; i < n; ++i) {
+            const size_t at = first + (backward ? n - i + 1u : i);
+            auto grown = [&](vec v) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = scaled(v[j], 16u * t + mm16<A>::row(g, j) < p.K ? (int)exponents[at * HK + 16u * t + mm16<A>::row(g, j)] : 0);
+                return v;
+            };
+            if (!backward) x = grown(x);
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) lds[0][t][j][lane] = x[j];
+            __syncthreads();
+            const A* m = through + at * (p.K * HK) + (size_t)head * p.K;
+            x = zero16<A>();
+#pragma unroll 1
+            for (int s = 0; s < KT; ++s) {
+                vec left, right;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const unsigned row = 16u * t + c, k = 16u * s + mm16<A>::row(g, j);
+                    left[j] = row < p.K && k < p.K ? backward ? m[k * HK + row] : m[row * HK + k] : A(0);
+                    right[j] = lds[0][s][j][lane];
+                }
+                x = product<A>(left, right, x);
+            }
+            x = load(to(i)) + (backward ? grown(x) : x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (here && 16u * t + mm16<A>::row(g, j) < p.K) *state(to(i), j) = x[j];
+        }
+        return;
+    }
     vec a[KT];
     auto transition = [&](unsigned i) {
         const A* m = through + (first + (backward ? n - i + 1u : i)) * (p.K * HK) + (size_t)head * p.K;
@@ -331,25 +453,14 @@ __global__ __launch_bounds__(64 * KT) void k_delta_carry(delta_shape p, bool bac
                 a[s][j] = row < p.K && k < p.K ? backward ? m[k * HK + row] : m[row * HK + k] : A(0);
             }
     };
-    // the exponents of a transition's columns: forward they belong to the rows of what goes in, backward to those of what comes out
-    struct { int e[4]; } power, next = {};
-    auto exponents = [&](unsigned i) {
-        const A* m = through + ((size_t)p.cuts * p.K + first + (backward ? n - i + 1u : i)) * HK + (size_t)head * p.K;
-        decltype(power) x;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x.e[j] = 16u * t + mm16<A>::row(g, j) < p.K ? (int)m[16u * t + mm16<A>::row(g, j)] : 0;
-        return x;
-    };
     const vec start = load(first + (backward ? n - 1u : 1u));
-    power = exponents(2u);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) lds[0][t][i][lane] = backward ? start[i] : scaled(start[i], power.e[i]);
+    for (int i = 0; i < 4; ++i) lds[0][t][i][lane] = start[i];
     transition(2u);
     vec own = load(to(2u));
     __syncthreads();
     for (unsigned i = 2; i < n; ++i) {
-        if (i + 1u < n) next = exponents(i + 1u);
-        vec x = backward ? zero16<A>() : own;
+        vec x = own;
 #pragma unroll
         for (int s = 0; s < KT; ++s) {
             vec b;
@@ -357,17 +468,13 @@ __global__ __launch_bounds__(64 * KT) void k_delta_carry(delta_shape p, bool bac
             for (int j = 0; j < 4; ++j) b[j] = lds[i & 1u][s][j][lane];
             x = product<A>(a[s], b, x);
         }
-        if (backward)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = own[j] + scaled(x[j], power.e[j]);
-        power = next;
         if (i + 1u < n) {
             transition(i + 1u);
             own = load(to(i + 1u));
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            lds[~i & 1u][t][j][lane] = backward ? x[j] : scaled(x[j], power.e[j]);
+            lds[~i & 1u][t][j][lane] = x[j];
             if (here && 16u * t + mm16<A>::row(g, j) < p.K) *state(to(i), j) = x[j];
         }
         __syncthreads();
@@ -498,9 +605,9 @@ int check_delta(const dbk_deltarule_args* a)
     return 0;
 }
 
-int delta_mark(hipStream_t st, const delta_shape& s, const uint32_t* regions, uint32_t* marks, uint32_t* cuts)
+int delta_mark(hipStream_t st, const delta_shape& s, const uint32_t* regions, uint32_t* marks, uint32_t* cuts, uint32_t* odd)
 {
-    k_delta_mark<<<divup(s.nregion, 4), 256, 0, st>>>(s, regions, marks, cuts);
+    k_delta_mark<<<divup(s.nregion, 4), 256, 0, st>>>(s, regions, marks, cuts, odd);
     return 0;
 }
 
@@ -516,14 +623,14 @@ void delta_carry(hipStream_t st, const dbk_deltarule_args& a, const delta_shape&
     else launch(float());
 }
 
-void delta_prepare(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const uint32_t* marks, void* chunks, void* pairs)
+void delta_prepare(hipStream_t st, const dbk_deltarule_args& a, const delta_shape& s, const uint32_t* marks, void* chunks, void* pairs, uint32_t* odd)
 {
     with_row_type(a.dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
         with_key_tiles(a.K, [&](auto kt) {
             k_delta_prepare<T, kt.value><<<dim3((unsigned)delta_blocks(s), divup(s.H, 4)), 256, 0, st>>>(s, a.regions, marks, (const T*)a.Q, (const T*)a.Kk, (const A*)a.beta, (const A*)a.decay,
-                                                                                                        (delta_chunk<A>*)chunks, (delta_pairs<A>*)pairs);
+                                                                                                        (delta_chunk<A>*)chunks, (delta_pairs<A>*)pairs, odd);
         });
     });
 }
@@ -532,7 +639,7 @@ namespace {
 
 // Parts of the forward pass's workspace.
 struct delta_work {
-    uint32_t* marks;
+    uint32_t *marks, *odd;
     char* chunks;
     delta_cuts cuts;
     size_t bytes;
@@ -544,6 +651,8 @@ delta_work work_in(void* work, const dbk_deltarule_args& a, const delta_shape& s
     size_t at = 0;
     w.marks = (uint32_t*)p;
     at += align16(s.slots * sizeof(uint32_t));
+    w.odd = (uint32_t*)(p + at);
+    at += align16(delta_odd_bytes(s));
     w.chunks = p + at;
     at += delta_chunks(s) * a.H * (a.dtype == DBK_F64 ? sizeof(delta_chunk<double>) : sizeof(delta_chunk<float>));
     const size_t A = acc_size(a.dtype);
@@ -604,8 +713,8 @@ int dbk_deltarule(dbk_stream_t stream, const dbk_deltarule_args* a, void* work, 
     DBK_CHECK(grid_fits(delta_blocks(s), 256), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
     hipStream_t st = as_stream(stream);
     if (a->N) {
-        delta_mark(st, s, a->regions, w.marks, w.cuts.marks);
-        delta_prepare(st, *a, s, w.marks, w.chunks, nullptr);
+        delta_mark(st, s, a->regions, w.marks, w.cuts.marks, w.odd);
+        delta_prepare(st, *a, s, w.marks, w.chunks, nullptr, w.odd);
     }
     with_row_type(a->dtype, [&](auto t) {
         typedef decltype(t) T;
@@ -614,13 +723,17 @@ int dbk_deltarule(dbk_stream_t stream, const dbk_deltarule_args* a, void* work, 
             if (s.L) {
                 const unsigned values = team_blocks(s, team.value, s.V);
                 k_delta_local<T, kt.value, team.value><<<dim3(s.cuts, values + team_blocks(s, team.value, s.K)), 256, 0, st>>>(
-                    s, values, a->regions, w.cuts.marks, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const delta_chunk<A>*)w.chunks, (const A*)a->state, (A*)w.cuts.carry,
+                    s, values, a->regions, w.cuts.marks, w.odd, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const delta_chunk<A>*)w.chunks, (const A*)a->state, (A*)w.cuts.carry,
                     (A*)w.cuts.through);
                 delta_carry(st, *a, s, w.cuts, false);
             }
             k_delta_fprop<T, kt.value, team.value><<<dim3(s.nregion + s.cuts, team_blocks(s, team.value, s.V)), 256, 0, st>>>(
                 s, a->regions, w.cuts.marks, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const delta_chunk<A>*)w.chunks, (A)a->scale, (const A*)a->state, (const A*)w.cuts.carry, (T*)a->O,
                 (A*)a->last, (A*)a->keep);
+            // (no rows, no marks)
+            if (a->N)
+                k_delta_rows<T, kt.value><<<DELTA_ROWS_WGS, 64, 0, st>>>(s, a->regions, w.odd, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const A*)a->beta, (const A*)a->decay, (A)a->scale,
+                                                                         (const A*)a->state, (T*)a->O, (A*)a->last, (A*)a->keep);
         });
     });
     DBK_LAUNCH_OK();

@@ -435,6 +435,133 @@ __global__ __launch_bounds__(64 * WAVES, (back_waves<typename acc_of<T>::type, K
     }
 }
 
+// The gradients of marked heads, row by row, in the place of what the kernels above made of them: a team takes its columns of a head up a region, with the state's gradient in registers and
+// the state in front of each row made again from the one that the forward call kept in front of its block of 64 rows.
+template <typename A, int KT, int TEAM> struct delta_sums { A q[16 * KT][TEAM], k[16 * KT][TEAM], b[TEAM], g[TEAM][4]; };
+template <typename T, int KT, int TEAM>
+__global__ __launch_bounds__(64 * TEAM) void k_delta_bprop_rows(delta_shape p, unsigned units, size_t lddo, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ odd,
+                                                                const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, const T* __restrict__ dO,
+                                                                const typename acc_of<T>::type* __restrict__ beta, const typename acc_of<T>::type* __restrict__ decay,
+                                                                typename acc_of<T>::type scale, const typename acc_of<T>::type* __restrict__ keep, delta_grads<T> out)
+{
+    typedef typename acc_of<T>::type A;
+    typedef typename mm16<A>::vec vec;
+    __shared__ delta_sums<A, KT, TEAM> lds;
+    if (!uniform(odd[(size_t)p.nregion * p.H])) return;
+    const unsigned slice = uniform(threadIdx.x >> 6);
+    for (size_t i = blockIdx.x; i < (size_t)p.nregion * units; i += gridDim.x) {
+        const unsigned r = (unsigned)(i / units);
+        delta_lane<A, TEAM, TEAM> l;
+        l.place(p, (unsigned)(i % units), p.V);
+        if (!(uniform(odd[(size_t)r * p.H + l.head]) & DELTA_ODD)) continue;
+        const row_range g = region_rows(regions, r, p.N);
+        const bool here = l.c < l.nv;
+        const unsigned part = l.unit % out.parts, share = (l.head % (p.H / p.G)) * out.parts + part;
+        const T *q0 = Q + (size_t)l.group * p.K, *k0 = K + (size_t)l.group * p.K;
+        vec dS[KT];
+#pragma unroll
+        for (int t = 0; t < KT; ++t) dS[t] = zero16<A>();
+        A a, b, miss;
+        vec S[KT], x[KT];                        // S: what a row leaves of the state in front of it; x: its key
+        auto decayed = [&](size_t row) {
+            a = row_factor(p, decay, row, l.head);
+            b = beta[row * p.ldb + l.head];
+            row_tiles<A, KT>(x, k0 + row * p.ldk, p.K, l.g);
+#pragma unroll
+            for (int t = 0; t < KT; ++t) S[t] *= a;
+            miss = (here ? (A)V[row * p.ldv + l.v + l.c] : A(0)) - found<A, KT>(x, S);
+        };
+        auto corrected = [&]() {
+#pragma unroll
+            for (int t = 0; t < KT; ++t) S[t] += x[t] * (b * miss);
+        };
+        // eight rows at a time, whose first state is made once and those of its rows from there
+        vec first[KT];
+        size_t eighth = g.end;
+#pragma unroll 1
+        for (size_t row = g.end; row-- > g.start;) {
+            if (row < eighth) {
+                eighth = g.start + (row - g.start) / 8u * 8u;
+                const unsigned block = ((unsigned)eighth - g.start) / DELTA_BLOCK;
+                load_state<A, KT>(S, block ? keep + kept_number(g, block) * ((size_t)p.K * p.H * p.V) : (const A*)nullptr, p, l);
+#pragma unroll 1
+                for (size_t before = g.start + (size_t)block * DELTA_BLOCK; before < eighth; ++before) {
+                    decayed(before);
+                    corrected();
+                }
+#pragma unroll
+                for (int t = 0; t < KT; ++t) first[t] = S[t];
+            }
+#pragma unroll
+            for (int t = 0; t < KT; ++t) S[t] = first[t];
+#pragma unroll 1
+            for (size_t before = eighth;; ++before) {
+                decayed(before);
+                if (before == row) break;
+                corrected();
+            }
+            const A d = here ? scale * (A)dO[row * lddo + l.v + l.c] : A(0), u = b * miss;
+            {
+                vec q[KT];
+                row_tiles<A, KT>(q, q0 + row * p.ldq, p.K, l.g);
+#pragma unroll
+                for (int t = 0; t < KT; ++t) dS[t] += q[t] * d;
+            }
+            const A du = found<A, KT>(x, dS), dx = b * du, db = lanes16_sum(du * miss);
+            A dg = A(0);
+            __syncthreads();                     // (the sums of the row behind have been taken)
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const A dq = lanes16_sum(fma(x[t][j], u, S[t][j]) * d), dk = lanes16_sum(dS[t][j] * u - S[t][j] * dx), old = fma(-x[t][j], dx, dS[t][j]);
+                    if (l.c == 0u) {
+                        lds.q[16u * t + l.row(j)][slice] = dq;
+                        lds.k[16u * t + l.row(j)][slice] = dk;
+                    }
+                    dg = fma(old, S[t][j], dg);
+                    dS[t][j] = a * old;
+                }
+            dg = lanes16_sum(dg);
+            if (l.c == 0u) {
+                lds.b[slice] = db;
+                lds.g[slice][l.g] = dg;
+            }
+            if (here && l.g == 0u) out.dV[row * out.lddv + l.v + l.c] = (T)dx;
+            __syncthreads();
+            for (unsigned k = threadIdx.x; k < p.K; k += 64u * TEAM) {
+                A dq = A(0), dk = A(0);
+#pragma unroll
+                for (int s = 0; s < TEAM; ++s) {
+                    dq += lds.q[k][s];
+                    dk += lds.k[k][s];
+                }
+                const size_t col = (size_t)l.group * p.K + k;
+                if (out.dq) {
+                    const size_t in = ((size_t)share * p.N + row) * p.G * p.K + col;
+                    out.dq[in] = dq;
+                    out.dk[in] = dk;
+                } else {
+                    out.dQ[row * out.lddq + col] = (T)dq;
+                    out.dK[row * out.lddk + col] = (T)dk;
+                }
+            }
+            if (threadIdx.x == 0u) {
+                A bs = A(0), gs = A(0);
+#pragma unroll
+                for (int s = 0; s < TEAM; ++s) {
+                    bs += lds.b[s];
+                    gs += (lds.g[s][0] + lds.g[s][1]) + (lds.g[s][2] + lds.g[s][3]);
+                }
+                if (out.db) out.db[((size_t)part * p.N + row) * p.H + l.head] = bs;
+                else out.dbeta[row * out.lddb + l.head] = bs;
+                if (out.dg) out.dg[((size_t)part * p.N + row) * p.H + l.head] = gs;
+                else if (out.ddecay) out.ddecay[row * out.lddg + l.head] = gs;
+            }
+        }
+    }
+}
+
 // out[row][col] = sum over shares of part[share][row][col], in order, for 16 rows of a block; four values a thread where they fit
 template <typename A, typename T>
 __device__ __forceinline__ void add_shares(size_t at, unsigned rows, size_t N, unsigned cols, unsigned shares, const A* part, T* out, size_t ld)
@@ -476,7 +603,7 @@ __global__ __launch_bounds__(256) void k_delta_add(delta_shape p, const uint32_t
 namespace {
 
 struct delta_bprop_work {
-    uint32_t* marks;
+    uint32_t *marks, *odd;
     char *chunks, *pairs, *dstates, *dq, *dk, *db, *dg;
     unsigned parts;
     delta_cuts cuts;
@@ -495,6 +622,7 @@ delta_bprop_work bprop_work_in(void* work, const dbk_deltarule_args& a, const de
     const size_t A = acc_size(a.dtype), units = delta_chunks(s) * a.H;
     w.parts = (s.ns + back_team(a) - 1) / back_team(a);
     w.marks = (uint32_t*)take(s.slots * sizeof(uint32_t));
+    w.odd = (uint32_t*)take(delta_odd_bytes(s));
     w.chunks = take(units * (A == 8 ? sizeof(delta_chunk<double>) : sizeof(delta_chunk<float>)));
     w.pairs = take(units * (A == 8 ? sizeof(delta_pairs<double>) : sizeof(delta_pairs<float>)));
     w.dstates = take((size_t)s.slots * a.K * a.H * a.V * A);
@@ -539,8 +667,8 @@ int dbk_deltarule_bprop(dbk_stream_t stream, const dbk_deltarule_args* a, void* 
     DBK_CHECK(work && work_bytes >= w.bytes, "ValueError: the workspace has %zu bytes, %zu are needed", work_bytes, w.bytes);
     DBK_CHECK(grid_fits(delta_blocks(s), 256), "ValueError: map too large (%zu rows, %zu regions)", a->N, a->nregion);
     hipStream_t st = as_stream(stream);
-    delta_mark(st, s, a->regions, w.marks, w.cuts.marks);
-    delta_prepare(st, *a, s, w.marks, w.chunks, w.pairs);
+    delta_mark(st, s, a->regions, w.marks, w.cuts.marks, w.odd);
+    delta_prepare(st, *a, s, w.marks, w.chunks, w.pairs, w.odd);
     int rc = 0;
     with_row_type(a->dtype, [&](auto t) {
         typedef decltype(t) T;
@@ -565,6 +693,9 @@ int dbk_deltarule_bprop(dbk_stream_t stream, const dbk_deltarule_args* a, void* 
             kernel<<<dim3((unsigned)delta_blocks(s), team_blocks(s, TEAM, s.V, WAVES)), 64 * WAVES, lds, st>>>(
                 s, a->lddo, a->regions, w.marks, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const T*)a->dO, (const delta_chunk<A>*)w.chunks, (const delta_pairs<A>*)w.pairs,
                 (A)a->scale, (const A*)a->keep, (const A*)w.dstates, out);
+            const unsigned units = team_blocks(s, TEAM, s.V, TEAM);
+            k_delta_bprop_rows<T, kt.value, TEAM><<<DELTA_ROWS_WGS, 64 * TEAM, 0, st>>>(s, units, a->lddo, a->regions, w.odd, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const T*)a->dO,
+                                                                                        (const A*)a->beta, (const A*)a->decay, (A)a->scale, (const A*)a->keep, out);
         });
         if (!rc && (w.dq || w.db)) k_delta_add<T><<<dim3((unsigned)delta_blocks(s), 3 * DELTA_CHUNKS), 256, 0, st>>>(s, a->regions, w.marks, out);
     });

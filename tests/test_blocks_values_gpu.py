@@ -48,9 +48,9 @@ def delta_as_by_rows(kind, t, v, R, G, Kd, what, least=1e-35, grads=True, state=
                 near(g, w, b, kind, "%s: %s" % (what, name), rows, stored=name in GRADS[:3], least=least)
 
 
-def changed(t, v, name, rows, value):
+def changed(t, v, name, rows, value, cols=slice(None)):
     """Rows of a map set to a value, or multiplied by it (a factor in a tuple), on the device and in the plain form."""
-    t[name][rows] = t[name][rows] * value[0] if isinstance(value, tuple) else value
+    t[name][rows, cols] = t[name][rows, cols] * value[0] if isinstance(value, tuple) else value
     v[name] = t[name].double().cpu().numpy()
 
 
@@ -149,3 +149,55 @@ def test_delta_rule_carries_what_is_not_finite_exactly_as_far_as_the_formulas(ki
                     assert bool(same[keeps].all()), "%s[%d] = %s: %s changes at rows %s" % (name, row, bad, what, np.unique(np.argwhere(host(keeps & ~same))[:, 0]).tolist()[:20])
                     left = g.isfinite() & ~keeps
                     assert not bool(left.any()), "%s[%d] = %s: %s is finite at rows %s" % (name, row, bad, what, np.unique(np.argwhere(host(left))[:, 0]).tolist()[:20])
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("one", [True, False])
+@pytest.mark.parametrize("H,G,Kd,Vd,R,at", [(2, 1, 16, 16, [[0, 100], [100, 150]], 0), (4, 2, 16, 20, [[0, 100], [100, 150]], 0), (5, 5, 7, 40, [[50, 150], [0, 50]], 50),
+                                            (2, 2, 40, 33, LONG, 480), (2, 1, 128, 70, [[0, 130]], 0), (3, 1, 20, 20, LONG, 240)])
+def test_delta_rule_whose_factors_within_a_chunk_leave_the_range(kind, one, H, G, Kd, Vd, R, at):
+    """Sixteen rows may grow or shrink a state by more than the type's range, by their decays (of one head, or of all) or by keys longer than one, where the
+    rows by themselves find nothing to grow, or something small."""
+    N = max(e for _, e in R)
+    rate = 40.0 if kind == "float64" else 7.5    # e^640 and e^120 in a chunk: more than its matrices are let hold, and in single precision than they can
+    heads = slice(0, 1) if one else slice(0, H)
+    end = max(e for s, e in R if s <= at < e)
+    case = lambda: delta_case(kind, N, H, G, Kd, Vd, True, 0, [H, Kd, Vd])  # noqa: E731
+    rows = lambda a, b: slice(at + a, at + b)  # noqa: E731
+    t, v = case()
+    start = max(s for s, e in R if s <= at < e)
+    changed(t, v, "beta", slice(start, at + 40), 0.0, heads)
+    changed(t, v, "decay", slice(start, at + 40), rate, heads)
+    delta_as_by_rows(kind, t, v, R, G, Kd, "nothing in front", grads=False)
+    t, v = case()
+    changed(t, v, "decay", rows(50, 51), -1e4, heads)
+    changed(t, v, "beta", slice(at + 50, end), 0.0, heads)
+    changed(t, v, "decay", slice(at + 51, end), rate, heads)
+    changed(t, v, "dO", slice(at + 50, end), 0.0, slice(0, (heads.stop - heads.start) * Vd))
+    delta_as_by_rows(kind, t, v, R, G, Kd, "no gradient behind")
+    if kind == "float64":                        # (the bounds' norms square what is over 1e160 then, and keys would have to be 1e10 long)
+        return
+    for first, value, between, grad in ((rate, 1e-25, 1.0, 1e-15), (-rate, 1e18, 1e-38, 1e-18)):
+        t, v = case()
+        changed(t, v, "beta", rows(33, 61), (0.02,), heads)
+        changed(t, v, "decay", rows(33, 47), first, heads)
+        changed(t, v, "decay", rows(47, 61), -first, heads)
+        cols = slice(0, (heads.stop - heads.start) * Vd)
+        changed(t, v, "V", slice(0, N), (value,), cols)
+        changed(t, v, "V", rows(33, 61), (between,), cols)
+        changed(t, v, "dO", slice(0, N), (grad,), cols)
+        # (heads that share a key add their gradients of it: the others' are no smaller than these)
+        delta_as_by_rows(kind, t, v, R, G, Kd, "up and down" if first > 0 else "down and up")
+    # (long keys that find nothing, and send nothing back, change nothing: the plain form goes without them)
+    t, v = case()
+    changed(t, v, "V", slice(start, at + 31), 0.0)
+    changed(t, v, "beta", rows(10, 31), 1.0)
+    t["K"][rows(10, 31)] *= 100.0
+    delta_as_by_rows(kind, t, v, R, G, Kd, "long keys, nothing in front", grads=False)
+    t, v = case()
+    changed(t, v, "decay", rows(45, 46), -1e4)
+    changed(t, v, "V", slice(at + 45, end), 0.0)
+    changed(t, v, "beta", slice(at + 47, end), 1.0)
+    changed(t, v, "dO", slice(at + 45, end), 0.0)
+    t["K"][at + 47:end] *= 100.0
+    delta_as_by_rows(kind, t, v, R, G, Kd, "long keys, no gradient behind")
