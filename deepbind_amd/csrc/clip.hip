@@ -85,24 +85,32 @@ template <int THREADS> __device__ __forceinline__ double clip_squares(const clip
     return s;
 }
 
-template <int THREADS> __device__ __forceinline__ void clip_scale(const clip_part& p, size_t block, unsigned piece, double factor)
+__device__ __forceinline__ double clip_factor(double norm, double most) { return norm > most ? most / norm : 1.0; }
+
+// A factor below the type's smallest normal number has lost its digits, or is nothing, where what it makes of large gradients is neither: there floats are multiplied in double
+// precision, and doubles by the two parts of the factor one after the other.
+template <int THREADS> __device__ __forceinline__ void clip_scale(const clip_part& p, size_t block, unsigned piece, double norm, double most)
 {
+    const double factor = clip_factor(norm, most);
     if (factor == 1.0 && p.in == p.out) return;
     with_clip_type(p.dtype, [&](auto t) {
         typedef decltype(t) T;
         typedef typename acc_of<T>::type A;
-        const A by = (A)factor;
-        clip_walk<T, THREADS>(p, (const T*)p.in + block * p.nexti, (T*)p.out + block * p.nexto, piece, [&](const T* x, T* y, unsigned valid) {
-            row_vec<T> v;
-            v.load(x, valid);
+        auto walk = [&](auto scaled) {
+            clip_walk<T, THREADS>(p, (const T*)p.in + block * p.nexti, (T*)p.out + block * p.nexto, piece, [&](const T* x, T* y, unsigned valid) {
+                row_vec<T> v;
+                v.load(x, valid);
 #pragma unroll
-            for (int j = 0; j < row_vec<T>::N; ++j) v.v[j] *= by;
-            v.store(y, valid);
-        });
+                for (int j = 0; j < row_vec<T>::N; ++j) v.v[j] = scaled(v.v[j]);
+                v.store(y, valid);
+            });
+        };
+        const A by = (A)factor;
+        if (factor >= (sizeof(A) == 4 ? 0x1p-126 : 0x1p-1022)) walk([&](A v) { return v * by; });
+        else if constexpr (sizeof(A) == 4) walk([&](A v) { return (A)((double)v * factor); });
+        else walk([&](A v) { return v / norm * most; });
     });
 }
-
-__device__ __forceinline__ double clip_factor(double norm, double most) { return norm > most ? most / norm : 1.0; }
 
 // the tensor and piece of a workgroup, whose number counts the pieces of this launch's tensors
 __device__ __forceinline__ const clip_part& clip_find(const clip_table& t, unsigned index, unsigned& piece)
@@ -132,7 +140,7 @@ __global__ __launch_bounds__(256) void k_clip_scale(clip_table t, const double* 
     for (unsigned i = threadIdx.x; i < t.all; i += 256u) s += sums[block * t.all + i];
     const double norm = sqrt(clip_sum<256>(s, lds));
     if (p.first + piece == 0u && threadIdx.x == 0) norms[block] = norm;
-    clip_scale<256>(p, block, piece, clip_factor(norm, most));
+    clip_scale<256>(p, block, piece, norm, most);
 }
 
 // Everything of a model in one workgroup.
@@ -141,9 +149,9 @@ __global__ __launch_bounds__(1024) void k_clip_one(clip_table t, double most, do
     __shared__ double lds[16];
     double s = 0;
     for (unsigned i = 0; i < t.n; ++i) s += clip_squares<1024>(t.part[i], blockIdx.x, 0u);
-    const double norm = sqrt(clip_sum<1024>(s, lds)), factor = clip_factor(norm, most);
+    const double norm = sqrt(clip_sum<1024>(s, lds));
     if (threadIdx.x == 0) norms[blockIdx.x] = norm;
-    for (unsigned i = 0; i < t.n; ++i) clip_scale<1024>(t.part[i], blockIdx.x, 0u, factor);
+    for (unsigned i = 0; i < t.n; ++i) clip_scale<1024>(t.part[i], blockIdx.x, 0u, norm, most);
 }
 
 namespace {

@@ -201,3 +201,28 @@ def test_delta_rule_whose_factors_within_a_chunk_leave_the_range(kind, one, H, G
     changed(t, v, "dO", slice(at + 45, end), 0.0)
     t["K"][at + 47:end] *= 100.0
     delta_as_by_rows(kind, t, v, R, G, Kd, "long keys, no gradient behind")
+
+
+# ------------------------------------------------------------------------------------------------ clipping
+@pytest.mark.parametrize("nblock", [1, 3])
+@pytest.mark.parametrize("size", [120, 60000])
+@pytest.mark.parametrize("kind,value,most", [("float32", 1e36, 1e-4), ("float32", 1e30, 1e-12), ("float32", 1e38, 1e-6), ("float32", 3e38, 1.0), ("float32", 1e37, 1e-30), ("bfloat16", 1e38, 1e-6),
+                                             ("bfloat16", 1e30, 1e-12), ("float64", 1e140, 1e-150), ("float64", 1e150, 1e-170), ("float32", 1.0, 0.5)])
+def test_clipping_by_factors_below_the_types_range(kind, value, most, size, nblock):
+    """The factor may be far smaller than the smallest number of the gradients' type; what it makes of them is not."""
+    from deepbind_amd import deepity_smat as ds
+    rng = np.random.default_rng(4)
+    # of one magnitude, so that every result is an ordinary number
+    grads, plain = zip(*(put(value * rng.choice([-1, 1], s) * (1 + rng.random(s)) / 2, TYPES[kind]) for s in ((size // 12, 6), (1, size // 2))))
+    norms, _ = ref.clip(plain, most, nblock, [False] * 2)
+    want = [(p.astype(np.longdouble) * np.longdouble(most) / np.repeat(norms, p.shape[1] // nblock)).astype(float) for p in plain]
+    out = [torch.empty_like(g) for g in grads]
+    got = ds.clip_gradients(grads, most, nblock=nblock, out=out)
+    n = size * 2.0 ** -53
+    np.testing.assert_allclose(host(got)[0], norms, rtol=n)
+    for o, w in zip(out, want):
+        # the factor's own rounding, the product's, and the stored one's (a small factor is two: one more product); below the range half a step of it
+        least = {"float32": 2.0 ** -150, "bfloat16": 2.0 ** -134, "float64": 0.0}[kind]
+        assert (np.abs(host(o.double()) - w) <= (3 * U[kind] + STORED[kind] + n) * np.abs(w) + least).all()
+    again = ds.clip_gradients(grads, most, nblock=nblock)
+    assert torch.equal(again, got) and all(torch.equal(a, b) for a, b in zip(grads, out))
