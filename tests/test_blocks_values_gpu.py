@@ -203,6 +203,106 @@ def test_delta_rule_whose_factors_within_a_chunk_leave_the_range(kind, one, H, G
     delta_as_by_rows(kind, t, v, R, G, Kd, "long keys, no gradient behind")
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("H,G,Kd,Vd", SHAPES)
+def test_delta_rule_with_resets_and_large_steps_over_segments(kind, H, G, Kd, Vd):
+    """Hard resets at, before and behind the borders of segments, rows that learn nothing and rows that turn what they find around; minus infinity resets too."""
+    t, v = delta_case(kind, 1100, H, G, Kd, Vd, True, 0, [H, Kd])
+    for name, rows, value in (("decay", [20, 255, 256, 511, 700, 1029, 1030], -1e4), ("decay", [300, 769], -60.0), ("beta", [3, 257, 512], 0.0), ("beta", [60, 61, 510, 768, 1050], 2.0),
+                              ("decay", [33, 257], 0.0)):
+        changed(t, v, name, rows, value)
+    delta_as_by_rows(kind, t, v, LONG, G, Kd, "resets")
+    state = put(np.random.default_rng(3).standard_normal((2, Kd, H * Vd)), wide(kind))
+    delta_as_by_rows(kind, t, v, LONG, G, Kd, "from a state", grads=False, state=state)
+    changed(t, v, "decay", [255, 700], -float("inf"))
+    # (the bounds' running products go without it; what it leaves is what -1e4 leaves)
+    v["decay"][[255, 700]] = -1e4
+    delta_as_by_rows(kind, t, v, LONG, G, Kd, "minus infinity")
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("H,G,Kd,Vd,R", [(4, 2, 40, 130, [[30, 100], [0, 30], [100, 101]]), (4, 2, 128, 130, [[300, 1068], [0, 256], [256, 300]]), (6, 2, 16, 70, [[0, 600]]),
+                                        (2, 1, 100, 129, [[5, 700]])])
+def test_delta_rule_of_shared_heads_with_values_in_parts(kind, H, G, Kd, Vd, R):
+    """Gradients of a key that heads share, each of whose values takes several teams of waves."""
+    N = max(e for _, e in R) + 3
+    t, v = delta_case(kind, N, H, G, Kd, Vd, True, 1, [H, Kd, Vd])
+    delta_as_by_rows(kind, t, v, R, G, Kd, "shared")
+
+
+def test_delta_rule_on_two_streams_at_once():
+    """Calls with everything in their scratch (segments, transitions, carried states, heads' shares, marked heads) in flight on two streams, on their own data each."""
+    from deepbind_amd import kangaroo_smat as ks
+    R, sides = regions([[0, 3000], [3000, 3300]]), []
+    for seed in (41, 42):
+        t, _ = delta_case("bfloat16" if seed == 41 else "float32", 3300, 4, 2, 64, 80, True, 0, seed)
+        if seed == 42:
+            t["beta"][3000:3050, 0], t["decay"][3000:3050, 0] = 0.0, 8.0
+        sides.append(t)
+
+    def both(t):
+        kw = dict(decay=t["decay"], groups=2)
+        keep = ks.kept_delta(t["K"], t["V"], t["beta"], groups=2)
+        O, last = ks.deltarule(t["Q"], t["K"], t["V"], t["beta"], R, keep=keep, want_state=True, **kw)
+        return (O, last) + ks.deltarule_bprop(t["Q"], t["K"], t["V"], t["beta"], R, keep, t["dO"], **kw)
+
+    want = [both(t) for t in sides]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(4):
+        for t, s in zip(sides, streams):
+            with torch.cuda.stream(s):
+                got.append(both(t))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        # (the marked head's gradients grow by e^400 over its fifty rows, beyond the range, by the formulas too)
+        for a, b in zip(g, want[i % 2]):
+            assert bool(((a == b) | (a.isnan() & b.isnan())).all())
+        assert g[0].isfinite().all() and g[1].isfinite().all()
+
+
+# ------------------------------------------------------------------------------------------------ norms around a block
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rms", [True, False])
+@pytest.mark.parametrize("n,nchunk,w", [(50, 3, 16), (50, 2, 5), (2300, 1, 300), (700, 2, 700), (600, 1, 1440), (560, 1, 2500), (530, 1, 5000), (520, 2, 9001)])
+def test_block_norms_and_their_gradients_keep_a_bad_row_to_its_chunk(kind, rms, n, nchunk, w):
+    """What is not finite in a chunk of a row, of any map, reaches that chunk's outputs and row gradients, and the weights' gradients of its columns, and nothing else."""
+    from deepbind_amd import smat as sm
+    gen = torch.Generator(device="cuda").manual_seed(n + w)
+    m, wd = nchunk * w, wide(kind)
+    f = lambda *s: torch.randn(*s, generator=gen, device="cuda", dtype=wd)  # noqa: E731
+    t = {k: f(n, m).to(TYPES[kind]) for k in ("Y", "R", "gate", "dR", "dZ")}
+    W = {k: f(1, m) for k in ("gamma", "scale", "next_gamma") + (() if rms else ("beta", "next_beta"))}
+    kw = dict(nchunk=nchunk, rms=rms, **W)
+
+    def both():
+        O, Z, stats = sm.blocknorm(t["Y"], t["R"], gate=t["gate"], want_stats=True, **kw)
+        return (O, Z) + sm.blocknorm_bprop(t["Y"], O, stats, t["dR"], t["dZ"], gate=t["gate"], **kw)
+
+    want = both()
+    assert all(x is None or x.isfinite().all() for x in want)
+    last = n - 1                                 # (rows that workgroups reach first and last)
+    for name, row, col, bad in (("Y", 7, w - 1, float("nan")), ("R", last, 0, float("inf")), ("gate", 30, 2, float("inf")), ("dZ", last, m - 1, float("nan")), ("dR", 0, 1, float("-inf"))):
+        old = t[name][row, col].clone()
+        t[name][row, col] = bad
+        got = both()
+        t[name][row, col] = old
+        chunk = slice(col // w * w, col // w * w + w)
+        rows = torch.zeros(n, m, dtype=torch.bool, device="cuda")
+        rows[row, chunk] = True
+        for i, (a, b) in enumerate(zip(got, want)):
+            if a is None:
+                continue
+            away = ~rows if i < 5 else ~rows[row:row + 1]
+            assert torch.equal(a[away], b[away]), (name, i)
+            if i < 2 and name in ("dZ", "dR"):
+                assert torch.equal(a, b)
+        # and where it cannot but be seen
+        seen = {"Y": (0, 1, 2, 3), "R": (0, 1, 2, 3), "gate": (0, 1, 2, 3, 4), "dZ": (2, 3, 4), "dR": (2, 3, 4)}[name]
+        for i in seen:
+            assert not got[i][row, chunk].isfinite().all(), (name, i)
+
+
 # ------------------------------------------------------------------------------------------------ clipping
 @pytest.mark.parametrize("nblock", [1, 3])
 @pytest.mark.parametrize("size", [120, 60000])
