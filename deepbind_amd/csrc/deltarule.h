@@ -119,8 +119,8 @@ template <typename A> struct delta_matrices {
 };
 
 // What a chunk's matrices may hold. Decays above zero, or keys longer than one, take them beyond the type's range in 16 rows where the rows themselves may find nothing to multiply, and
-// infinity times nothing is a NaN; a product that has almost vanished and grows again has lost its digits. A head with such a chunk in a region, whose keys, queries, factors and corrections
-// are all finite, is marked (prepare); three of the largest entries multiplied, as they are in a chunk, stay within the range. What the kernels make of it is made again row by row, as the definition has it (k_delta_rows, k_delta_bprop_rows): slow, but as far as that goes.
+// infinity times nothing is a NaN; a product that has almost vanished and grows again has lost its digits. A head with such a chunk in a region, whose keys, factors and corrections
+// are all finite, is marked (prepare); three of the largest entries multiplied, as they are in a chunk, stay within the range. It goes row by row there, as the definition has it (delta_walk_rows, k_delta_bprop_rows): slow, but as far as that goes.
 template <typename A> struct delta_range;
 template <> struct delta_range<float> { static constexpr double most = 0x1p36, least = 0x1p-100; };
 template <> struct delta_range<double> { static constexpr double most = 0x1p300, least = 0x1p-900; };
@@ -179,6 +179,14 @@ template <typename A, int TEAM, int WAVES = 4> struct delta_lane {
         D = (size_t)p.H * cols;
     }
     __device__ __forceinline__ unsigned row(int r) const { return mm16<A>::row(g, r); }
+    // Whether this team's head goes row by row in a region; where two teams meet at the same barriers, either's.
+    __device__ __forceinline__ bool marked(const delta_shape& p, const uint32_t* odd, unsigned r, unsigned index, unsigned cols) const
+    {
+        const uint32_t* of = odd + (size_t)r * p.H;
+        if (TEAM != 2 || WAVES == TEAM) return (uniform(of[head]) & DELTA_ODD) != 0u;
+        const unsigned parts = ((cols + 15u) / 16u + TEAM - 1u) / TEAM, last = p.H * parts - 1u;
+        return ((uniform(of[min(index * 2u, last) / parts]) | uniform(of[min(index * 2u + 1u, last) / parts])) & DELTA_ODD) != 0u;
+    }
 };
 template <typename F> inline void with_key_tiles(size_t K, F f)
 {

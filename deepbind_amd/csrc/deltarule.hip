@@ -117,11 +117,11 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
             first *= ai;
             mine = i == (int)c ? (A)first : mine;
             n[i] = i > (int)c ? D[i] * lds[g][i][c] : A(0);
-            finite = fma(lds[g][i][c], A(0), finite);
             size = fmax(size, D[i]);
         }
         size = fmax(size, mine);
-        finite = fma((A)a[16u * g + c], A(0), fma(b[16u * g + c], A(0), finite));
+        // (a key's product with itself is finite where it is, and then those with all others are)
+        finite = fma((A)a[16u * g + c], A(0), fma(b[16u * g + c], A(0), lds[g][c][c] * A(0)));
         // a row lengthens what lies along its key by the factor |1 - b k.k|, which lies within rounding's reach of one where keys of length one are learnt by b = 2
         const A turned = b[16u * g + c] * lds[g][c][c];
         if (__any(a[lane] > 1.0 || turned > A(2.05) || turned < A(-0.05)) && lane == 0u) atomicOr(odd + (size_t)bl.r * p.H + head, DELTA_GROWS);
@@ -163,23 +163,22 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
     substitute(std::false_type());
     A stray = A(0);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) stray = fma(x[i], A(0), stray);
-    if (__any(stray != A(0))) substitute(std::true_type());
-    sync();
-    put(ss);
-    A s[16];
-#pragma unroll
     for (int i = 0; i < 16; ++i) {
-        s[i] = i >= (int)c ? D[i] * lds[g][i][c] : A(0);
-        finite = fma(lds[g][i][c], A(0), finite);
-        size = fmax(size, fmax(fabs(x[i]), fabs(s[i]) * A(0x1p-64)));       // (a query's product with a key goes nowhere but into its own output)
+        stray = fma(x[i], A(0), stray);
+        size = fmax(size, fabs(x[i]));
     }
+    if (__any(stray != A(0))) substitute(std::true_type());
     const uint64_t beyond = __ballot(size > A(delta_range<A>::most)), bad = __ballot(finite != A(0));
     // (rarely any; the order in which marks are added does not matter)
     if (c == 0u && (beyond >> 16u * g & 0xffffu) && !(bad >> 16u * g & 0xffffu)) {
         atomicOr(odd + (size_t)bl.r * p.H + head, DELTA_ODD);
         odd[(size_t)p.nregion * p.H] = 1u;
     }
+    sync();
+    put(ss);
+    A s[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = i >= (int)c ? D[i] * lds[g][i][c] : A(0);
     store([&](size_t i) { return chunks[i].TP; }, s, x);
 }
 
@@ -247,10 +246,38 @@ __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lan
     }
 }
 
-// Workgroups below nregion: a region, or the first segment of a cut one; the others: the segment of their slot, from the state carried there.
+// A region of a marked head, row by row: 4096 rows of 16 heads of 64 x 64 floats 5.8 ms (by chunks 0.25), and 33 backward (0.33), as nothing is overlapped here.
+template <typename T, int KT, int TEAM>
+__device__ __forceinline__ void delta_walk_rows(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, const T* Q, const T* K, const T* V, const typename acc_of<T>::type* beta,
+                                                const typename acc_of<T>::type* decay, typename acc_of<T>::type scale, row_range g, typename mm16<typename acc_of<T>::type>::vec (&S)[KT], T* O,
+                                                typename acc_of<T>::type* keep)
+{
+    typedef typename acc_of<T>::type A;
+    const bool here = l.c < l.nv;
+#pragma unroll 1
+    for (size_t row = g.start; row < g.end; ++row) {
+        const unsigned at = (unsigned)row - g.start;
+        if (keep && at && at % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + kept_number(g, at / DELTA_BLOCK) * ((size_t)p.K * p.H * p.V), p, l);
+        typename mm16<A>::vec x[KT];
+        const A a = row_factor(p, decay, row, l.head);
+        row_tiles<A, KT>(x, K + row * p.ldk + (size_t)l.group * p.K, p.K, l.g);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) S[t] *= a;
+        const A u = beta[row * p.ldb + l.head] * ((here ? (A)V[row * p.ldv + l.v + l.c] : A(0)) - found<A, KT>(x, S));
+#pragma unroll
+        for (int t = 0; t < KT; ++t) S[t] += x[t] * u;
+        row_tiles<A, KT>(x, Q + row * p.ldq + (size_t)l.group * p.K, p.K, l.g);
+        const A o = scale * found<A, KT>(x, S);
+        if (here && l.g == 0u) O[row * p.ldo + l.v + l.c] = (T)o;
+    }
+}
+
+// Workgroups below nregion: a region, or the first segment of a cut one; the others: the segment of their slot, from the state carried there. Of a marked head the first
+// does the whole region (a kernel of their own for marked heads, behind this one, is a launch more: 30 us for 27 on a region of 63 rows).
 template <typename T, int KT, int TEAM>
 __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEAM>())) void k_delta_fprop(delta_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ cuts,
-                                                     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
+                                                     const uint32_t* __restrict__ odd, const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V,
+                                                     const typename acc_of<T>::type* __restrict__ beta, const typename acc_of<T>::type* __restrict__ decay,
                                                      const delta_chunk<typename acc_of<T>::type>* __restrict__ chunks, typename acc_of<T>::type scale,
                                                      const typename acc_of<T>::type* __restrict__ state, const typename acc_of<T>::type* __restrict__ carry, T* __restrict__ O,
                                                      typename acc_of<T>::type* __restrict__ last, typename acc_of<T>::type* __restrict__ keep)
@@ -274,51 +301,18 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
     l.place(p, blockIdx.y, p.V);
     const unsigned start = g.start + k * p.L, rows = p.L && g.end - start > p.L ? p.L : g.end - start;
     vec S[KT];
+    if (g.start < g.end && l.marked(p, odd, r, blockIdx.y, p.V)) {               // (a call of no rows has no marks)
+        if (k || !l.nv) return;
+        load_state<A, KT>(S, from, p, l);
+        delta_walk_rows<T, KT, TEAM>(p, l, Q, K, V, beta, decay, scale, g, S, O, keep);
+        if (last) store_state<A, KT>(S, last + r * block, p, l);
+        return;
+    }
     load_state<A, KT>(S, from, p, l);
     const unsigned before = k * (p.L / DELTA_BLOCK);
     int e = 0;
     delta_walk<T, KT, TEAM, true>(p, l, lds[l.team], Q, K, V, chunks, scale, r, g.start, start, rows, S, O, keep, kept_number(g, before), false, e);
     if (last && start + rows == g.end) store_state<A, KT>(S, last + r * block, p, l);
-}
-
-// The regions of marked heads, row by row, in the place of what the kernel above made of them: a wave takes 16 columns of a head through one. 4096 rows of 16 heads of
-// 64 x 64 floats 5.8 ms (by chunks 0.25), and 33 backward (0.33): nothing is overlapped here.
-template <typename T, int KT>
-__global__ __launch_bounds__(64) void k_delta_rows(delta_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ odd, const T* __restrict__ Q, const T* __restrict__ K,
-                                                   const T* __restrict__ V, const typename acc_of<T>::type* __restrict__ beta, const typename acc_of<T>::type* __restrict__ decay,
-                                                   typename acc_of<T>::type scale, const typename acc_of<T>::type* __restrict__ state, T* __restrict__ O,
-                                                   typename acc_of<T>::type* __restrict__ last, typename acc_of<T>::type* __restrict__ keep)
-{
-    typedef typename acc_of<T>::type A;
-    typedef typename mm16<A>::vec vec;
-    if (!uniform(odd[(size_t)p.nregion * p.H])) return;
-    const size_t block = (size_t)p.K * p.H * p.V;
-    for (size_t i = blockIdx.x; i < (size_t)p.nregion * p.H * p.ns; i += gridDim.x) {
-        const unsigned r = (unsigned)(i / (p.H * p.ns));
-        delta_lane<A, 1, 1> l;
-        l.place(p, (unsigned)(i % (p.H * p.ns)), p.V);
-        if (!(uniform(odd[(size_t)r * p.H + l.head]) & DELTA_ODD)) continue;
-        const row_range g = region_rows(regions, r, p.N);
-        const bool here = l.c < l.nv;
-        vec S[KT], x[KT];
-        load_state<A, KT>(S, state ? state + r * block : (const A*)nullptr, p, l);
-#pragma unroll 1
-        for (size_t row = g.start; row < g.end; ++row) {
-            const unsigned at = (unsigned)row - g.start;
-            if (keep && at && at % DELTA_BLOCK == 0) store_state<A, KT>(S, keep + kept_number(g, at / DELTA_BLOCK) * block, p, l);
-            const A a = row_factor(p, decay, row, l.head);
-            row_tiles<A, KT>(x, K + row * p.ldk + (size_t)l.group * p.K, p.K, l.g);
-#pragma unroll
-            for (int t = 0; t < KT; ++t) S[t] *= a;
-            const A u = beta[row * p.ldb + l.head] * ((here ? (A)V[row * p.ldv + l.v + l.c] : A(0)) - found<A, KT>(x, S));
-#pragma unroll
-            for (int t = 0; t < KT; ++t) S[t] += x[t] * u;
-            row_tiles<A, KT>(x, Q + row * p.ldq + (size_t)l.group * p.K, p.K, l.g);
-            const A o = scale * found<A, KT>(x, S);
-            if (here && l.g == 0u) O[row * p.ldo + l.v + l.c] = (T)o;
-        }
-        if (last) store_state<A, KT>(S, last + r * block, p, l);
-    }
 }
 
 constexpr int LEVEL_PLAIN = 60;                   // columns of up to this power of two, either way, are stored as they are
@@ -728,12 +722,9 @@ int dbk_deltarule(dbk_stream_t stream, const dbk_deltarule_args* a, void* work, 
                 delta_carry(st, *a, s, w.cuts, false);
             }
             k_delta_fprop<T, kt.value, team.value><<<dim3(s.nregion + s.cuts, team_blocks(s, team.value, s.V)), 256, 0, st>>>(
-                s, a->regions, w.cuts.marks, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const delta_chunk<A>*)w.chunks, (A)a->scale, (const A*)a->state, (const A*)w.cuts.carry, (T*)a->O,
+                s, a->regions, w.cuts.marks, w.odd, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const A*)a->beta, (const A*)a->decay, (const delta_chunk<A>*)w.chunks, (A)a->scale,
+                (const A*)a->state, (const A*)w.cuts.carry, (T*)a->O,
                 (A*)a->last, (A*)a->keep);
-            // (no rows, no marks)
-            if (a->N)
-                k_delta_rows<T, kt.value><<<DELTA_ROWS_WGS, 64, 0, st>>>(s, a->regions, w.odd, (const T*)a->Q, (const T*)a->Kk, (const T*)a->Vv, (const A*)a->beta, (const A*)a->decay, (A)a->scale,
-                                                                         (const A*)a->state, (T*)a->O, (A*)a->last, (A*)a->keep);
         });
     });
     DBK_LAUNCH_OK();
