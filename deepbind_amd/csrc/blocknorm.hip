@@ -11,8 +11,9 @@
 //
 // Bound by memory: forward three maps in and two out, backward five in and three out. A thread holds one vector of 16 bytes of a chunk, a chunk belongs to a power of two
 // of a wave's lanes, or to a workgroup of two to sixteen waves, and a workgroup walks down the rows with its chunks' weights, and backward their gradients, in registers.
-// 50 021 rows x 64 chunks of 16 floats, rms, no gate: 160 us forward (820 MB, 5.1 TB/s), 250 backward (1230 MB, 4.9) and 8 for the sums; 130 003 rows x 1440 bfloat16 with a gate: 424
-// (1870 MB, 4.4 TB/s; vector instructions over half of the time: two norms, a sigmoid and conversions for ten bytes) and 620 (2996 MB, 4.8; three barriers a row).
+// 50 021 rows x 64 chunks of 16 floats, rms, no gate: 160 us forward (820 MB, 5.1 TB/s), 252 backward (1230 MB, 4.9) and 8 for the sums; 130 003 rows x 1440 bfloat16 with a gate: 417
+// (1870 MB, 4.5 TB/s; vector instructions 74 % of the time: two norms, a sigmoid and conversions for ten bytes) and 622 (2996 MB, 4.8; three barriers a row), once the clocks have settled: the
+// first dozen passes after a pause take 440 to 500 and 650 to 760.
 #include <type_traits>
 #include "norm_common.h"
 

@@ -18,8 +18,9 @@ __global__ __launch_bounds__(256) void k_delta_mark(delta_shape p, const uint32_
 // A chunk's matrices. A wave takes a block of a head, four chunks: the products of its keys and queries on the matrix cores, then a lane per chunk and column for the
 // decays between rows and the triangle's inverse, column by column by substitution (powers of the triangle, which the matrix cores
 // could multiply instead, grow far beyond the inverse where keys come again, and lose it). A wave waits for memory most of its time, first for its block, then for its
-// rows: what it needs is asked for at once, and its share of LDS, which keys' products and queries' use in turn, lets six of them run per SIMD. 191 284 rows in 2048 regions, 4 heads of
-// 64 floats: 112 us for 460 MB (keys and queries in, matrices out; 90 at a copy's rate); 48 532 rows of 24 heads of 16, where four waves share a row's line: 86 us for 306 MB
+// rows: what it needs is asked for at once, and keys' products and queries' use its share of LDS in turn. Five waves run per SIMD with keys of up to 32 columns (bfloat16: 64), three with 64 floats
+// or 128 bfloat16 values, two with 128 floats: as many as their registers allow. 191 284 rows in 2048 regions, 4 heads of
+// 64 floats: 108 us for 460 MB (keys and queries in, matrices out; 90 at a copy's rate); 48 532 rows of 24 heads of 16, where four waves share a row's line: 84 us for 306 MB
 // forward and 390 backward (106 with a square for each triangle).
 template <typename T, int KT>
 __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)) void k_delta_prepare(delta_shape p, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ marks, const T* __restrict__ Q,
@@ -184,9 +185,10 @@ __global__ __launch_bounds__(256, (sizeof(T) < 8 && sizeof(T) * KT <= 8 ? 5 : 1)
 
 // Walks a wave's 16 columns of a head's state down `rows` rows from `row` on, of region r, which starts at `first`.
 // Keys, queries, matrices and values of a chunk come while the one before it is worked on. OUT: rows of O are written; otherwise only the state moves on. V null:
-// without values, for what becomes of the state alone, whose columns are kept near one where they may grow (leveled; exponents in e). Bound by issue and by one chunk's chain, which waves of other heads and regions fill: 191 284 rows, 4 heads of 64 x 64 floats 314 us
-// (850 MB at 2.7 TB/s, 23 GFLOP: matrix units busy for 46 % of the time, vector instructions 27 %); 41 816 bfloat16 rows, 8 heads of 128 x 128 in 32 segments 275 us (25 % and 49 %, most of
-// which takes the states apart into pieces). Four waves on the same head's keys share what is fetched: alone, each would read all of it.
+// without values, for what becomes of the state alone, whose columns are kept near one where they may grow (leveled; exponents in e). Bound by issue and by one chunk's chain, which waves of
+// other heads and regions fill: 191 284 rows, 4 heads of 64 x 64 floats 293 us (850 MB at 2.9 TB/s, 23 GFLOP: matrix units busy for 51 % of the time, vector instructions 31 %); 41 816 bfloat16
+// rows, 8 heads of 128 x 128 in 32 segments 249 us (28 % and 57 %, most of which takes the states apart into pieces). Four waves on the same head's keys share what is fetched: alone,
+// each would read all of it.
 template <typename T, int KT, int TEAM, bool OUT>
 __device__ __forceinline__ void delta_walk(const delta_shape& p, const delta_lane<typename acc_of<T>::type, TEAM>& l, typename delta_ops<T, KT>::rows* lds, const T* Q, const T* K,
                                            const T* V, const delta_chunk<typename acc_of<T>::type>* chunks, typename acc_of<T>::type scale, unsigned r, unsigned first, size_t row, unsigned rows,
@@ -318,7 +320,7 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
 constexpr int LEVEL_PLAIN = 60;                   // columns of up to this power of two, either way, are stored as they are
 // What the segment in front of a slot's hands on: its state, from the region's own initial one (the first) or from zeros, and (the others) how it takes the
 // state in front of it to its end: the states that the unit vectors become, times powers of two. Workgroups from `values` on along y take those. Keys of 128 columns beside values of 128: twice the
-// forward pass's columns without its outputs, 350 us where that takes 275 (vector instructions 54 % of the time; four waves per SIMD instead of two, for which registers spill, gain nothing).
+// forward pass's columns without its outputs, 278 us where that takes 249 (vector instructions 69 % of the time).
 template <typename T, int KT, int TEAM>
 __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEAM>())) void k_delta_local(delta_shape p, unsigned values, const uint32_t* __restrict__ regions,
                                                      const uint32_t* __restrict__ cuts, const uint32_t* __restrict__ odd, const T* __restrict__ Q, const T* __restrict__ K,
@@ -368,7 +370,7 @@ __global__ __launch_bounds__(256, (delta_waves<typename acc_of<T>::type, KT, TEA
 
 // From segment to segment: what is in front of slot k + 1 is what its own segment made of zeros and what the transition makes of what is in front of slot k; backward
 // from the last segment to the first with the transposed transitions. A workgroup takes 16 columns of a head, a wave 16 rows of what comes out; what goes in lies in LDS as
-// it lies in registers, and the next transition's rows come meanwhile. One step after the other: 6 us each with keys of 128 columns (65 us for
+// it lies in registers, and the next transition's rows come meanwhile. One step after the other: 6 us each with keys of 128 columns (67 us for
 // regions of 11 segments), where a transition's 64 KB have to come, 2.4 with 64; asking for them two steps ahead gained nothing.
 template <typename A, int KT>
 __global__ __launch_bounds__(64 * KT) void k_delta_carry(delta_shape p, bool backward, const uint32_t* __restrict__ regions, const uint32_t* __restrict__ cuts, A* __restrict__ carry, const A* __restrict__ through)

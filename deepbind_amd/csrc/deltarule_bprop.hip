@@ -16,8 +16,8 @@
 // Two kernels: a wave walks 16 columns of a head's dS up its region and leaves it behind every block of 64 rows; then all blocks are independent,
 // each from the state that the forward pass kept before it and the gradient behind it. What is summed over a value's columns (dQ, dK, dP, dL) passes through LDS
 // between the waves of a head, and through memory between the parts of 64 columns of wide values and between heads that share a key: added in a fixed order.
-// 48 532 rows in 512 regions, 24 heads of 16 x 16 floats: 33 us up the regions, 275 for the blocks; 16 028 bfloat16 rows in two, 16 heads of 64 x 64 on 4 keys: 81 us (75 more for the
-// segments from zeros and 36 for the carry), 372 for the blocks and 30 to add heads that share.
+// 48 532 rows in 512 regions, 24 heads of 16 x 16 floats: 31 us up the regions, 264 for the blocks; 16 028 bfloat16 rows in two, 16 heads of 64 x 64 on 4 keys: 72 us (68 more for the
+// segments from zeros and 37 for the carry), 345 for the blocks and 30 to add heads that share.
 #include "deltarule.h"
 
 namespace dbk {
@@ -166,7 +166,10 @@ template <typename A, int R, int W> __device__ __forceinline__ typename mm16<A>:
 // The gradients of one block of 64 rows, from the state in front of it and the gradient of the state behind it: forward again over its chunks, whose states stay in registers, and
 // back. Two kinds of work alternate: what runs over a head's keys (a wave's 16 columns of the value, the states in registers) and what runs over its value (16 columns of the
 // key for a wave, the states in LDS), so that neither dQ and dK nor the states are ever added up or turned over between waves. Bound by what lies between: barriers, LDS and waits for
-// both; the matrix units are busy for 24 % (heads of 16) and 33 % (of 64) of the time, vector instructions for 35 % and 31 %.
+// both; the matrix units are busy for 25 % (heads of 16) and 36 % (of 64) of the time, vector instructions for 39 % and 34 %.
+// Waves per SIMD it is compiled for, and with it how many registers a wave has. One more and one fewer, a call's backward pass of 47 303 rows in 512 regions: floats of 16 x 16 (24 heads) 448 us with
+// three waves, 472 with two, 580 with four; 16 x 64 (8 heads) 536, 558, 839; 32 x 32 (16) 666 with two, 708 with one, 733 with three; 64 x 64 (8) 818, 1286, 1356. What the registers do not hold spills:
+// 5 to 31 of them with keys of up to 16 columns in single precision, 32 (values of 32 columns) and 171 (wider) in double, where keys of more than 64 columns keep 1.3 KB a lane in memory.
 template <typename A, int KT, int TEAM> constexpr int back_waves() { return sizeof(A) == 8 ? (KT == 1 && TEAM > 1 ? 2 : 1) : KT == 1 ? 3 : KT == 2 && TEAM == 1 ? 1 : KT <= 4 ? 2 : 1; }
 
 template <typename T, int KT, int TEAM, int WAVES>

@@ -261,6 +261,41 @@ def test_delta_rule_on_two_streams_at_once():
         assert g[0].isfinite().all() and g[1].isfinite().all()
 
 
+def test_captured_delta_rule_keeps_no_marks_from_one_replay_to_the_next():
+    """Ordinary rows, rows whose states grow over a segment, rows that leave the range within a chunk, in turn through the same captured call and the same kept buffer."""
+    from deepbind_amd import kangaroo_smat as ks
+    H, Kd, Vd, N = 3, 20, 20, 1100
+    t, v = delta_case("float32", N, H, 1, Kd, Vd, True, 0, 51)
+    plain = {k: x.clone() for k, x in t.items()}
+    R = regions(LONG)
+    keep = ks.kept_delta(t["K"], t["V"], t["beta"], groups=1)
+
+    def both(keep):
+        kw = dict(decay=t["decay"], groups=1)
+        O, last = ks.deltarule(t["Q"], t["K"], t["V"], t["beta"], R, keep=keep, want_state=True, **kw)
+        return (O, last) + ks.deltarule_bprop(t["Q"], t["K"], t["V"], t["beta"], R, keep, t["dO"], **kw)
+
+    both(keep)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = both(keep)
+    for turn in (0, 1, 0, 2, 1, 2, 0):
+        for k, x in plain.items():
+            t[k].copy_(x)
+        if turn == 1:
+            t["decay"][520, 1], t["decay"][521:1030, 1] = -1e4, 0.36
+        elif turn == 2:
+            t["decay"][520, 0], t["decay"][521:560, 0] = -1e4, 7.5
+        if turn:
+            t["beta"][520:1030], t["dO"][520:1030] = 0.0, 0.0
+        graph.replay()
+        torch.cuda.synchronize()
+        want = both(torch.full_like(keep, float("nan")))
+        for a, b in zip(held, want):
+            assert b.isfinite().all() and torch.equal(a, b), turn
+
+
 # ------------------------------------------------------------------------------------------------ norms around a block
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("rms", [True, False])
